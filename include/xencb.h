@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define XENCB_ABI_VERSION 6
+#define XENCB_ABI_VERSION 7
 
 #if defined(__GNUC__)
 #define XENCB_API __attribute__((visibility("default")))
@@ -49,6 +49,7 @@ extern "C" {
 #define XENCB_DEV_TIMEOUT 1u /* an mbarrier wait gave up after its time limit                  */
 #define XENCB_DEV_CLAMPED 2u /* an n_valid entry exceeded page_rows and was clamped            */
 #define XENCB_DEV_BADPAGE 4u /* a page_of entry was outside [0, n_pages); that chunk was skipped */
+#define XENCB_DEV_BADADAPTER 16u /* an adapter_of entry was past the last adapter; its rows ran without one */
 #define XENCB_DEV_BADROWS 8u /* a library_build row range was outside the row buffer; built empty */
 
 /* element type codes */
@@ -319,6 +320,67 @@ XENCB_API int xencb_project_out(const float* r, int64_t n_rows, int d_s, const f
                       const float* log_alpha_dev, const float* pos_mask,
                       const void* h, int h_dtype, void* delta_out, void* h_out, float* rel_out, void* workspace,
                       size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * The projections with low-rank adapters of many requests beside the shared weight:
+ *   x @ W^T  becomes  x @ W^T + s_a (x @ A_a^T) @ B_a^T,   a = adapter_of[row / rows_per_adapter]
+ * in xencb_project_in (x = rms_norm(h) or h; before the bias, the L2 norm) and xencb_project_out (x = r; before the
+ * bias, the gate and the scale); every other argument is theirs. The gate and the selector logits are not adapted.
+ *   adapt_a      [n_adapters, rank, d_in] of adapt_dtype, adapt_b [n_adapters, d_out, rank] of adapt_dtype
+ *   adapt_scale  [n_adapters] float32, or NULL (1)
+ *   adapter_of   [ceil(n_rows / rows_per_adapter)] int32; a negative entry: these rows have no adapter; an entry
+ *                past n_adapters - 1 is flagged (XENCB_DEV_BADADAPTER) and read as none
+ *   1 <= rank <= 256. Sums in float32. Workspace: the matching *_adapted_workspace bytes, 256-byte aligned.
+ * No counterpart in the reference: it serves one interface at a time. */
+XENCB_API size_t xencb_project_in_adapted_workspace(int64_t n_rows, int d_m, int d_s, int rank);
+XENCB_API int xencb_project_in_adapted(const void* h, int h_dtype, int64_t n_rows, int d_m, const float* w_in,
+                                       const void* w_prep, const float* b_in, int d_s, int flags,
+                                       const float* gate_w, float gate_b, const float* gate_b_dev,
+                                       const float* sel_w, const float* sel_b, int n_cand, float rms_eps,
+                                       float* q_out, float* gate_out, float* rstd_out, float* z_out,
+                                       const void* adapt_a, const void* adapt_b, int adapt_dtype,
+                                       const float* adapt_scale, int n_adapters, int rank,
+                                       const int32_t* adapter_of, int64_t rows_per_adapter, void* workspace,
+                                       size_t workspace_bytes, void* stream);
+XENCB_API size_t xencb_project_out_adapted_workspace(int64_t n_rows, int d_s, int d_m, int rank);
+XENCB_API int xencb_project_out_adapted(const float* r, int64_t n_rows, int d_s, const float* w_out,
+                                        const void* w_prep, const float* b_out, int d_m, float scale,
+                                        const float* log_scale_dev, const float* gate, const float* sel_w,
+                                        float log_alpha, const float* log_alpha_dev, const float* pos_mask,
+                                        const void* h, int h_dtype, void* delta_out, void* h_out, float* rel_out,
+                                        const void* adapt_a, const void* adapt_b, int adapt_dtype,
+                                        const float* adapt_scale, int n_adapters, int rank,
+                                        const int32_t* adapter_of, int64_t rows_per_adapter, void* workspace,
+                                        size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * Page operators of pools that several Libraries share (no counterpart in the reference, whose Library owns its
+ * tensors). A page is live when a table entry [lib, c], c < n_chunks_of[lib], names it; freeing a Library means
+ * dropping its table row. pools: host array of n_pools device pointers (one per depth, keys and values), pool i
+ * holding n_pages pages of page_rows rows of row_bytes[i] bytes (even), densely. The tables are the same for every
+ * pool; n_chunks_of may be NULL. Nothing is read back by the host. n_pages <= 2^20.
+ *
+ * xencb_pages_fork: child i names parent parents[i]'s pages for its chunks below own_from[i], and for every chunk
+ * from own_from[i] on a free page, taken in ascending order over (child, chunk), that receives a copy of the parent's
+ * rows (n_valid of them, then zeros). child_page_of [n_children, n_chunks]; entries past the parent's chunk count
+ * are 0. short_out[0] = fresh pages that were missing: those entries are -1 and nothing is copied for them. An unknown
+ * parent or a page outside the pool gives -1 and XENCB_DEV_BADPAGE. The parents' tables stay valid.
+ *
+ * xencb_pages_compact: with n live pages, every live page at or above n moves to a free page below it (both in
+ * ascending order; the rows that some Library reads, then zeros), so that pages [0, n) are the live ones.
+ * page_of_out [n_lib, n_chunks] names the pages' new places (0 past a Library's chunk count; an entry outside the
+ * pool stays as it is, flagged XENCB_DEV_BADPAGE); n_live_out[0] = n. */
+XENCB_API size_t xencb_pages_fork_workspace(int64_t n_children, int n_chunks);
+XENCB_API int xencb_pages_fork(void* const* pools, const int64_t* row_bytes, int n_pools, int64_t n_pages,
+                               int page_rows, const int32_t* page_of, const int32_t* n_valid, int n_chunks,
+                               const int32_t* n_chunks_of, int64_t n_lib, const int32_t* parents,
+                               const int32_t* own_from, int64_t n_children, int32_t* child_page_of,
+                               int32_t* short_out, void* workspace, size_t workspace_bytes, void* stream);
+XENCB_API size_t xencb_pages_compact_workspace(int64_t n_pages);
+XENCB_API int xencb_pages_compact(void* const* pools, const int64_t* row_bytes, int n_pools, int64_t n_pages,
+                                  int page_rows, const int32_t* page_of, const int32_t* n_valid, int n_chunks,
+                                  const int32_t* n_chunks_of, int64_t n_lib, int32_t* page_of_out,
+                                  int32_t* n_live_out, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------------------
  * LayerSelector weights from logits. Replaces LayerSelector._weights_from_logits (xenc/selector.py:59-67),

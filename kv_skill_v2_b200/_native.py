@@ -16,10 +16,10 @@ LIB_PATH = Path(__file__).resolve().with_name("libxencb.so")
 # element type codes, status codes and flags (include/xencb.h)
 F32, F16, BF16 = 0, 1, 2
 OK, EINVAL, ECUDA, ENOTSUP = 0, 1, 2, 3
-DEV_TIMEOUT, DEV_CLAMPED, DEV_BADPAGE = 1, 2, 4
+DEV_TIMEOUT, DEV_CLAMPED, DEV_BADPAGE, DEV_BADROWS, DEV_BADADAPTER = 1, 2, 4, 8, 16
 PIN_RMS, PIN_L2 = 1, 2
 NOALLOC_SCRATCH_BYTES = 16 << 20
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 _p, _i, _i64, _f, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
 
@@ -69,6 +69,16 @@ SIGNATURES: dict = {
     "xencb_project_out_workspace": (_sz, [_i64, _i, _i]),
     "xencb_project_out": (_i, [_p, _i64, _i, _p, _p, _p, _i, _f, _p, _p, _p, _f, _p, _p, _p, _i, _p, _p, _p, _p,
                                _sz, _p]),
+    "xencb_project_in_adapted_workspace": (_sz, [_i64, _i, _i, _i]),
+    "xencb_project_in_adapted": (_i, [_p, _i, _i64, _i, _p, _p, _p, _i, _i, _p, _f, _p, _p, _p, _i, _f, _p, _p, _p, _p,
+                                      _p, _p, _i, _p, _i, _i, _p, _i64, _p, _sz, _p]),
+    "xencb_project_out_adapted_workspace": (_sz, [_i64, _i, _i, _i]),
+    "xencb_project_out_adapted": (_i, [_p, _i64, _i, _p, _p, _p, _i, _f, _p, _p, _p, _f, _p, _p, _p, _i, _p, _p, _p,
+                                       _p, _p, _i, _p, _i, _i, _p, _i64, _p, _sz, _p]),
+    "xencb_pages_fork_workspace": (_sz, [_i64, _i]),
+    "xencb_pages_fork": (_i, [_p, _p, _i, _i64, _i, _p, _p, _i, _p, _i64, _p, _p, _i64, _p, _p, _p, _sz, _p]),
+    "xencb_pages_compact_workspace": (_sz, [_i64]),
+    "xencb_pages_compact": (_i, [_p, _p, _i, _i64, _i, _p, _p, _i, _p, _i64, _p, _p, _p, _sz, _p]),
     "xencb_selector_weights": (_i, [_p, _i64, _i, _i, _i, _p, _p]),
     "xencb_selector_logits": (_i, [_p, _i, _i64, _i, _p, _p, _i, _i, _f, _p, _p]),
     "xencb_selector_apply": (_i, [_p, _i, _p, _i, _i64, _i, _p, _i, _i, _f, _p, _p]),

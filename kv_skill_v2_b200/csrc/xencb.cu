@@ -27,6 +27,8 @@
 #include "topk_read.cuh"
 #include "attn.cuh"
 #include "exchange.cuh"
+#include "pages.cuh"
+#include "adapt.cuh"
 
 // Scratch of xencb_read_decode_noalloc: a fixed device array, so that entry point never allocates.
 static __device__ __align__(256) unsigned char g_noalloc_scratch[XENCB_NOALLOC_SCRATCH_BYTES];
@@ -311,6 +313,46 @@ int launch_gemm(const void* X, int64_t M, int K, const float* W, int N, int sms,
                                                            row_done);
   XENCB_CHECK_LAUNCH("gemm_simt launch");
   *used = p;
+  return XENCB_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ adapters
+// Extra workspace of a projection with adapters: one more split partial (behind the GEMM's) and t [n_rows, rank].
+size_t adapt_slice_bytes(int64_t M, int N) { return align_up((size_t)M * N * sizeof(float), 256); }
+size_t adapt_t_bytes(int64_t M, int rank) { return align_up((size_t)M * rank * sizeof(float), 256); }
+
+int check_adapters(const char* what, const AdaptArgs& ad, int dtype) {
+  if (!ad.a || !ad.b || !ad.of) return fail(XENCB_EINVAL, "%s: adapt_a, adapt_b and adapter_of are required", what);
+  if (!elem_size(dtype)) return fail(XENCB_EINVAL, "%s: adapt_dtype %d unknown", what, dtype);
+  if (ad.n <= 0 || ad.rows_per_adapter <= 0)
+    return fail(XENCB_EINVAL, "%s: n_adapters=%d and rows_per_adapter=%lld must be positive", what, ad.n,
+                (long long)ad.rows_per_adapter);
+  if (ad.r <= 0 || ad.r > AD_MAX_RANK)
+    return fail(XENCB_EINVAL, "%s: rank=%d outside 1..%d", what, ad.r, AD_MAX_RANK);
+  return XENCB_OK;
+}
+
+// t = x A^T, before the GEMM (the row split that follows reads only x).
+template <typename TX>
+int launch_adapt_shrink(const void* x, int64_t M, const AdaptArgs& ad, int dtype, cudaStream_t st) {
+  const TX* xp = static_cast<const TX*>(x);
+  switch (dtype) {
+    case XENCB_F32: adapt_shrink_kernel<TX, float><<<(unsigned)M, 256, 0, st>>>(xp, ad); break;
+    case XENCB_F16: adapt_shrink_kernel<TX, __half><<<(unsigned)M, 256, 0, st>>>(xp, ad); break;
+    default: adapt_shrink_kernel<TX, __nv_bfloat16><<<(unsigned)M, 256, 0, st>>>(xp, ad); break;
+  }
+  XENCB_CHECK_LAUNCH("adapt_shrink launch");
+  return XENCB_OK;
+}
+
+int launch_adapt_expand(float* out, int64_t M, const AdaptArgs& ad, int dtype, cudaStream_t st) {
+  const dim3 grid((unsigned)M, (unsigned)((ad.d_out + 255) / 256));
+  switch (dtype) {
+    case XENCB_F32: adapt_expand_kernel<float><<<grid, 256, 0, st>>>(ad, out); break;
+    case XENCB_F16: adapt_expand_kernel<__half><<<grid, 256, 0, st>>>(ad, out); break;
+    default: adapt_expand_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(ad, out); break;
+  }
+  XENCB_CHECK_LAUNCH("adapt_expand launch");
   return XENCB_OK;
 }
 
@@ -656,7 +698,8 @@ static int project_in_impl(const void* h, int h_dtype, int64_t n_rows, int d_m, 
                            const float* b_in, int d_s, int flags, const float* gate_w, float gate_b,
                            const float* gate_b_dev, const float* sel_w, const float* sel_b, int n_cand, float rms_eps,
                            float* q_out, float* gate_out, float* rstd_out, float* z_out, void* workspace,
-                           size_t workspace_bytes, void* stream, const RouteFuse* rf) {
+                           size_t workspace_bytes, void* stream, const RouteFuse* rf,
+                           const AdaptArgs* adapters = nullptr, int adapt_dtype = 0) {
   if (flags & ~(XENCB_PIN_RMS | XENCB_PIN_L2)) return fail(XENCB_EINVAL, "project_in: unknown flags 0x%x", flags);
   if (!h || (!w_in && !w_prep) || !q_out) return fail(XENCB_EINVAL, "project_in: h, w_in (or w_prep) and q_out are required");
   if (!w_in && (d_m % 8 != 0 || !aligned(w_prep, 256)))
@@ -677,9 +720,11 @@ static int project_in_impl(const void* h, int h_dtype, int64_t n_rows, int d_m, 
   int rc = device_info(&di);
   if (rc) return rc;
   const int nch = (d_s + PIN_CHUNK - 1) / PIN_CHUNK;
-  const size_t g_bytes = gemm_ws_bytes(n_rows, d_s, d_m, di.sms, true);
+  const size_t slice = adapters ? adapt_slice_bytes(n_rows, d_s) : 0;
+  const size_t g_bytes = gemm_ws_bytes(n_rows, d_s, d_m, di.sms, true) + slice;
   const size_t nq_bytes = align_up((size_t)n_rows * nch * sizeof(float), 256);
-  const size_t need = g_bytes + nq_bytes + align_up((size_t)n_rows * sizeof(int), 256);
+  const size_t rd_bytes = align_up((size_t)n_rows * sizeof(int), 256);
+  const size_t need = g_bytes + nq_bytes + rd_bytes + (adapters ? adapt_t_bytes(n_rows, adapters->r) : 0);
   if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
     return fail(XENCB_EINVAL, "project_in: workspace needs %zu bytes, 256-byte aligned (got %zu)", need,
                 workspace_bytes);
@@ -688,9 +733,22 @@ static int project_in_impl(const void* h, int h_dtype, int64_t n_rows, int d_m, 
   float* nq_part = reinterpret_cast<float*>(ws + g_bytes);
   int* row_done = reinterpret_cast<int*>(ws + g_bytes + nq_bytes);
   // X staging for the tensor-core paths sits after the tensor-core partials
-  float* xbuf = (d_m % 4 == 0) ? reinterpret_cast<float*>(ws + gemm_part_bytes(n_rows, d_s, d_m, di.sms)) : nullptr;
+  float* xbuf = (d_m % 4 == 0) ? reinterpret_cast<float*>(ws + gemm_part_bytes(n_rows, d_s, d_m, di.sms) + slice) : nullptr;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   GemmPlan gp;
+  AdaptArgs ad{};
+  if (adapters) {
+    ad = *adapters;
+    ad.d_in = d_m;
+    ad.d_out = d_s;
+    ad.t = reinterpret_cast<float*>(ws + g_bytes + nq_bytes + rd_bytes);
+    switch (h_dtype) {
+      case XENCB_F32: rc = launch_adapt_shrink<float>(h, n_rows, ad, adapt_dtype, st); break;
+      case XENCB_F16: rc = launch_adapt_shrink<__half>(h, n_rows, ad, adapt_dtype, st); break;
+      default: rc = launch_adapt_shrink<__nv_bfloat16>(h, n_rows, ad, adapt_dtype, st); break;
+    }
+    if (rc) return rc;
+  }
   switch (h_dtype) {
     case XENCB_F32:
       rc = launch_gemm<float>(h, n_rows, d_m, w_in, d_s, di.sms, part, w_prep ? xbuf : nullptr, row_done, st, &gp,
@@ -704,6 +762,11 @@ static int project_in_impl(const void* h, int h_dtype, int64_t n_rows, int d_m, 
       break;
   }
   if (rc) return rc;
+  if (adapters) {  // the low-rank term is one more split partial
+    rc = launch_adapt_expand(part + (size_t)gp.splits * n_rows * d_s, n_rows, ad, adapt_dtype, st);
+    if (rc) return rc;
+    ++gp.splits;
+  }
   if (d_s <= 12 * ROW_THREADS) {  // one CTA per row: the reduce, 1/rms, bias and L2 norm in registers
     const int vpt = (d_s + 4 * ROW_THREADS - 1) / (4 * ROW_THREADS);  // float4 columns per thread: 1..3
     const unsigned thr = (unsigned)std::min<int>(ROW_THREADS, (d_s / 4 + 31) / 32 * 32);
@@ -1337,12 +1400,12 @@ size_t xencb_project_out_workspace(int64_t n_rows, int d_s, int d_m) {
          align_up((size_t)n_rows * nch * 3 * sizeof(float), 256) + align_up((size_t)n_rows * sizeof(int), 256);
 }
 
-int xencb_project_out(const float* r, int64_t n_rows, int d_s, const float* w_out, const void* w_prep,
-                      const float* b_out, int d_m,
-                      float scale, const float* log_scale_dev, const float* gate, const float* sel_w, float log_alpha,
-                      const float* log_alpha_dev, const float* pos_mask,
-                      const void* h, int h_dtype, void* delta_out, void* h_out, float* rel_out, void* workspace,
-                      size_t workspace_bytes, void* stream) {
+static int project_out_impl(const float* r, int64_t n_rows, int d_s, const float* w_out, const void* w_prep,
+                            const float* b_out, int d_m, float scale, const float* log_scale_dev, const float* gate,
+                            const float* sel_w, float log_alpha, const float* log_alpha_dev, const float* pos_mask,
+                            const void* h, int h_dtype, void* delta_out, void* h_out, float* rel_out, void* workspace,
+                            size_t workspace_bytes, void* stream, const AdaptArgs* adapters = nullptr,
+                            int adapt_dtype = 0) {
   if (!r || (!w_out && !w_prep) || !h) return fail(XENCB_EINVAL, "project_out: r, w_out (or w_prep) and h are required");
   if (!w_out && (d_s % 8 != 0 || !aligned(w_prep, 256)))
     return fail(XENCB_EINVAL, "project_out: without w_out, w_prep must be 256-byte aligned and d_s %% 8 == 0");
@@ -1354,10 +1417,12 @@ int xencb_project_out(const float* r, int64_t n_rows, int d_s, const float* w_ou
   int rc = device_info(&di);
   if (rc) return rc;
   const int nch = (d_m + PIN_CHUNK - 1) / PIN_CHUNK;
-  const size_t g_bytes = gemm_ws_bytes(n_rows, d_m, d_s, di.sms, false);
+  const size_t slice = adapters ? adapt_slice_bytes(n_rows, d_m) : 0;
+  const size_t g_bytes = gemm_ws_bytes(n_rows, d_m, d_s, di.sms, false) + slice;
   const size_t d_bytes = align_up((size_t)n_rows * d_m * sizeof(float), 256);
   const size_t np_bytes = align_up((size_t)n_rows * nch * 3 * sizeof(float), 256);
-  const size_t need = g_bytes + d_bytes + np_bytes + align_up((size_t)n_rows * sizeof(int), 256);
+  const size_t rd_bytes = align_up((size_t)n_rows * sizeof(int), 256);
+  const size_t need = g_bytes + d_bytes + np_bytes + rd_bytes + (adapters ? adapt_t_bytes(n_rows, adapters->r) : 0);
   if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
     return fail(XENCB_EINVAL, "project_out: workspace needs %zu bytes, 256-byte aligned (got %zu)", need,
                 workspace_bytes);
@@ -1369,9 +1434,23 @@ int xencb_project_out(const float* r, int64_t n_rows, int d_s, const float* w_ou
   float* cn_part = norm_part + (size_t)n_rows * nch * 2;
   int* row_done = reinterpret_cast<int*>(ws + g_bytes + d_bytes + np_bytes);
   GemmPlan gp;
-  float* xbuf = (d_s % 4 == 0) ? reinterpret_cast<float*>(ws + gemm_part_bytes(n_rows, d_m, d_s, di.sms)) : nullptr;
+  float* xbuf = (d_s % 4 == 0) ? reinterpret_cast<float*>(ws + gemm_part_bytes(n_rows, d_m, d_s, di.sms) + slice) : nullptr;
+  AdaptArgs ad{};
+  if (adapters) {
+    ad = *adapters;
+    ad.d_in = d_s;
+    ad.d_out = d_m;
+    ad.t = reinterpret_cast<float*>(ws + g_bytes + d_bytes + np_bytes + rd_bytes);
+    rc = launch_adapt_shrink<float>(r, n_rows, ad, adapt_dtype, st);
+    if (rc) return rc;
+  }
   rc = launch_gemm<float>(r, n_rows, d_s, w_out, d_m, di.sms, part, w_prep ? xbuf : nullptr, nullptr, st, &gp, w_prep);
   if (rc) return rc;
+  if (adapters) {  // the low-rank term is one more split partial
+    rc = launch_adapt_expand(part + (size_t)gp.splits * n_rows * d_m, n_rows, ad, adapt_dtype, st);
+    if (rc) return rc;
+    ++gp.splits;
+  }
   const float alpha = expf(log_alpha);
   if (d_m <= 12 * ROW_THREADS) {  // one CTA per row: the reduce, the norms and the epilogue in registers
     const int vpt = (d_m + 4 * ROW_THREADS - 1) / (4 * ROW_THREADS);  // float4 columns per thread: 1..3
@@ -1413,6 +1492,177 @@ int xencb_project_out(const float* r, int64_t n_rows, int d_s, const float* w_ou
 #undef XENCB_POUT
   XENCB_CHECK_LAUNCH_N("project_out reduce + epilogue launch", 2);
   return XENCB_OK;
+}
+
+int xencb_project_out(const float* r, int64_t n_rows, int d_s, const float* w_out, const void* w_prep,
+                      const float* b_out, int d_m,
+                      float scale, const float* log_scale_dev, const float* gate, const float* sel_w, float log_alpha,
+                      const float* log_alpha_dev, const float* pos_mask,
+                      const void* h, int h_dtype, void* delta_out, void* h_out, float* rel_out, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  return project_out_impl(r, n_rows, d_s, w_out, w_prep, b_out, d_m, scale, log_scale_dev, gate, sel_w, log_alpha,
+                          log_alpha_dev, pos_mask, h, h_dtype, delta_out, h_out, rel_out, workspace, workspace_bytes,
+                          stream);
+}
+
+// ------------------------------------------------------------------------------------------------ with adapters
+size_t xencb_project_in_adapted_workspace(int64_t n_rows, int d_m, int d_s, int rank) {
+  const size_t base = xencb_project_in_workspace(n_rows, d_m, d_s);
+  return base && rank > 0 ? base + adapt_slice_bytes(n_rows, d_s) + adapt_t_bytes(n_rows, rank) : 0;
+}
+
+int xencb_project_in_adapted(const void* h, int h_dtype, int64_t n_rows, int d_m, const float* w_in, const void* w_prep,
+                             const float* b_in, int d_s, int flags, const float* gate_w, float gate_b,
+                             const float* gate_b_dev, const float* sel_w, const float* sel_b, int n_cand, float rms_eps,
+                             float* q_out, float* gate_out, float* rstd_out, float* z_out, const void* adapt_a,
+                             const void* adapt_b, int adapt_dtype, const float* adapt_scale, int n_adapters, int rank,
+                             const int32_t* adapter_of, int64_t rows_per_adapter, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+  const AdaptArgs ad{adapt_a, adapt_b, adapt_scale, adapter_of, rows_per_adapter, n_adapters, rank, 0, 0, nullptr};
+  const int rc = check_adapters("project_in_adapted", ad, adapt_dtype);
+  if (rc) return rc;
+  return project_in_impl(h, h_dtype, n_rows, d_m, w_in, w_prep, b_in, d_s, flags, gate_w, gate_b, gate_b_dev, sel_w,
+                         sel_b, n_cand, rms_eps, q_out, gate_out, rstd_out, z_out, workspace, workspace_bytes, stream,
+                         nullptr, &ad, adapt_dtype);
+}
+
+size_t xencb_project_out_adapted_workspace(int64_t n_rows, int d_s, int d_m, int rank) {
+  const size_t base = xencb_project_out_workspace(n_rows, d_s, d_m);
+  return base && rank > 0 ? base + adapt_slice_bytes(n_rows, d_m) + adapt_t_bytes(n_rows, rank) : 0;
+}
+
+int xencb_project_out_adapted(const float* r, int64_t n_rows, int d_s, const float* w_out, const void* w_prep,
+                              const float* b_out, int d_m, float scale, const float* log_scale_dev, const float* gate,
+                              const float* sel_w, float log_alpha, const float* log_alpha_dev, const float* pos_mask,
+                              const void* h, int h_dtype, void* delta_out, void* h_out, float* rel_out,
+                              const void* adapt_a, const void* adapt_b, int adapt_dtype, const float* adapt_scale,
+                              int n_adapters, int rank, const int32_t* adapter_of, int64_t rows_per_adapter,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+  const AdaptArgs ad{adapt_a, adapt_b, adapt_scale, adapter_of, rows_per_adapter, n_adapters, rank, 0, 0, nullptr};
+  const int rc = check_adapters("project_out_adapted", ad, adapt_dtype);
+  if (rc) return rc;
+  return project_out_impl(r, n_rows, d_s, w_out, w_prep, b_out, d_m, scale, log_scale_dev, gate, sel_w, log_alpha,
+                          log_alpha_dev, pos_mask, h, h_dtype, delta_out, h_out, rel_out, workspace, workspace_bytes,
+                          stream, &ad, adapt_dtype);
+}
+
+// ------------------------------------------------------------------------------------------------ pages
+static int check_pools(const char* what, void* const* pools, const int64_t* row_bytes, int n_pools, int64_t n_pages,
+                       int page_rows) {
+  if (!pools || !row_bytes || n_pools <= 0) return fail(XENCB_EINVAL, "%s: at least one pool is required", what);
+  if (n_pages <= 0 || page_rows <= 0) return fail(XENCB_EINVAL, "%s: n_pages and page_rows must be positive", what);
+  if (n_pages > PG_MAX_PAGES)
+    return fail(XENCB_ENOTSUP, "%s: %lld pages, at most %d are supported", what, (long long)n_pages, PG_MAX_PAGES);
+  for (int i = 0; i < n_pools; ++i)
+    if (!pools[i] || row_bytes[i] <= 0 || row_bytes[i] % 2 != 0 || !aligned(pools[i], 2))
+      return fail(XENCB_EINVAL, "%s: pool %d needs a base pointer and a positive, even row size", what, i);
+  return XENCB_OK;
+}
+
+static int launch_page_copies(void* const* pools, const int64_t* row_bytes, int n_pools, int page_rows,
+                              const PageMove* moves, const int* n_moves, int sms, cudaStream_t st) {
+  for (int i0 = 0; i0 < n_pools; i0 += PG_POOLS) {
+    PagePools pp{};
+    pp.n = std::min(PG_POOLS, n_pools - i0);
+    pp.page_rows = page_rows;
+    bool vec = true;
+    for (int i = 0; i < pp.n; ++i) {
+      pp.base[i] = static_cast<char*>(pools[i0 + i]);
+      pp.row_bytes[i] = row_bytes[i0 + i];
+      vec = vec && aligned(pools[i0 + i], 16) && pp.row_bytes[i] * page_rows % 16 == 0;
+    }
+    const unsigned grid = (unsigned)(8 * sms);
+    if (vec) pages_copy_kernel<uint4><<<grid, 256, 0, st>>>(pp, moves, n_moves);
+    else pages_copy_kernel<uint16_t><<<grid, 256, 0, st>>>(pp, moves, n_moves);
+    XENCB_CHECK_LAUNCH("pages_copy launch");
+  }
+  return XENCB_OK;
+}
+
+static size_t pages_list_bytes(int64_t n) { return align_up((size_t)n * sizeof(int), 256); }
+
+size_t xencb_pages_fork_workspace(int64_t n_children, int n_chunks) {
+  if (n_children <= 0 || n_chunks <= 0) return 0;
+  const int64_t n = n_children * n_chunks;
+  return 256 + align_up((size_t)n * sizeof(PageMove), 256) + pages_list_bytes(n);
+}
+
+int xencb_pages_fork(void* const* pools, const int64_t* row_bytes, int n_pools, int64_t n_pages, int page_rows,
+                     const int32_t* page_of, const int32_t* n_valid, int n_chunks, const int32_t* n_chunks_of,
+                     int64_t n_lib, const int32_t* parents, const int32_t* own_from, int64_t n_children,
+                     int32_t* child_page_of, int32_t* short_out, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+  int rc = check_pools("pages_fork", pools, row_bytes, n_pools, n_pages, page_rows);
+  if (rc) return rc;
+  if (!page_of || !n_valid || !parents || !own_from || !child_page_of || !short_out)
+    return fail(XENCB_EINVAL, "pages_fork: page_of, n_valid, parents, own_from and the outputs are required");
+  if (n_chunks <= 0 || n_lib <= 0 || n_children <= 0)
+    return fail(XENCB_EINVAL, "pages_fork: n_lib, n_chunks and n_children must be positive");
+  if (n_children * n_chunks > INT32_MAX || n_lib * n_chunks > INT32_MAX)
+    return fail(XENCB_ENOTSUP, "pages_fork: the tables are too large");
+  const size_t need = xencb_pages_fork_workspace(n_children, n_chunks);
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < need)
+    return fail(XENCB_EINVAL, "pages_fork: workspace needs %zu bytes, 256-byte aligned (got %zu)", need,
+                workspace_bytes);
+  DevInfo di;
+  rc = device_info(&di);
+  if (rc) return rc;
+  char* ws = static_cast<char*>(workspace);
+  PagePlanArgs a{};
+  a.page_of = page_of; a.n_valid = n_valid; a.n_chunks_of = n_chunks_of; a.n_lib = n_lib; a.C = n_chunks;
+  a.n_pages = (int)n_pages; a.page_rows = page_rows; a.parents = parents; a.own_from = own_from; a.m = n_children;
+  a.table = child_page_of; a.count = short_out;
+  a.n_moves = reinterpret_cast<int*>(ws);
+  a.moves = reinterpret_cast<PageMove*>(ws + 256);
+  a.list = reinterpret_cast<int*>(ws + 256 + align_up((size_t)n_children * n_chunks * sizeof(PageMove), 256));
+  const int smem = (int)((n_pages + 31) / 32 * 4);
+  rc = ensure_smem(pages_fork_plan_kernel, smem);
+  if (rc) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  pages_fork_plan_kernel<<<1, PG_THREADS, smem, st>>>(a);
+  XENCB_CHECK_LAUNCH("pages_fork_plan launch");
+  return launch_page_copies(pools, row_bytes, n_pools, page_rows, a.moves, a.n_moves, di.sms, st);
+}
+
+size_t xencb_pages_compact_workspace(int64_t n_pages) {
+  if (n_pages <= 0) return 0;
+  return 256 + align_up((size_t)n_pages * sizeof(PageMove), 256) + 3 * pages_list_bytes(n_pages);
+}
+
+int xencb_pages_compact(void* const* pools, const int64_t* row_bytes, int n_pools, int64_t n_pages, int page_rows,
+                        const int32_t* page_of, const int32_t* n_valid, int n_chunks, const int32_t* n_chunks_of,
+                        int64_t n_lib, int32_t* page_of_out, int32_t* n_live_out, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  int rc = check_pools("pages_compact", pools, row_bytes, n_pools, n_pages, page_rows);
+  if (rc) return rc;
+  if (!page_of || !n_valid || !page_of_out || !n_live_out)
+    return fail(XENCB_EINVAL, "pages_compact: page_of, n_valid and the outputs are required");
+  if (n_chunks <= 0 || n_lib <= 0) return fail(XENCB_EINVAL, "pages_compact: n_lib and n_chunks must be positive");
+  if (n_lib * n_chunks > INT32_MAX) return fail(XENCB_ENOTSUP, "pages_compact: the table is too large");
+  const size_t need = xencb_pages_compact_workspace(n_pages);
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < need)
+    return fail(XENCB_EINVAL, "pages_compact: workspace needs %zu bytes, 256-byte aligned (got %zu)", need,
+                workspace_bytes);
+  DevInfo di;
+  rc = device_info(&di);
+  if (rc) return rc;
+  char* ws = static_cast<char*>(workspace);
+  PagePlanArgs a{};
+  a.page_of = page_of; a.n_valid = n_valid; a.n_chunks_of = n_chunks_of; a.n_lib = n_lib; a.C = n_chunks;
+  a.n_pages = (int)n_pages; a.page_rows = page_rows; a.table = page_of_out; a.count = n_live_out;
+  a.n_moves = reinterpret_cast<int*>(ws);
+  a.moves = reinterpret_cast<PageMove*>(ws + 256);
+  char* lists = ws + 256 + align_up((size_t)n_pages * sizeof(PageMove), 256);
+  a.list = reinterpret_cast<int*>(lists);
+  a.to = reinterpret_cast<int*>(lists + pages_list_bytes(n_pages));
+  a.rows = reinterpret_cast<int*>(lists + 2 * pages_list_bytes(n_pages));
+  const int smem = (int)((n_pages + 31) / 32 * 4);
+  rc = ensure_smem(pages_compact_plan_kernel, smem);
+  if (rc) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  pages_compact_plan_kernel<<<1, PG_THREADS, smem, st>>>(a);
+  XENCB_CHECK_LAUNCH("pages_compact_plan launch");
+  return launch_page_copies(pools, row_bytes, n_pools, page_rows, a.moves, a.n_moves, di.sms, st);
 }
 
 // ------------------------------------------------------------------------------------------------ selector

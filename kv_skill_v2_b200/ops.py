@@ -114,15 +114,57 @@ def weights_prep(w: torch.Tensor) -> torch.Tensor:
     return prep
 
 
+@dataclass
+class Adapters:
+    """Low-rank adapters of one projection, one per request (or per group of requests).
+
+    a      [n, rank, d_in]  (float16 / bfloat16 / float32)
+    b      [n, d_out, rank] of a's dtype
+    scale  [n] float32 (None: 1); the projection adds scale[i] * (x @ a[i]^T) @ b[i]^T to the shared x @ W^T"""
+
+    a: torch.Tensor
+    b: torch.Tensor
+    scale: Optional[torch.Tensor] = None
+
+    @property
+    def rank(self) -> int:
+        return int(self.a.shape[1])
+
+
+def _adapter_args(what: str, dev, ad: Adapters, of: Optional[torch.Tensor], rows_per_adapter: int, R: int, d_in: int,
+                  d_out: int):
+    """(a, b, dtype, scale, n, rank, of, rows_per_adapter), checked; the tensors are contiguous and on `dev`."""
+    if of is None:
+        raise ValueError(f"{what}: adapters need adapter_of")
+    if _cuda(what, ad.a, ad.b, ad.scale, of) != dev:
+        raise RuntimeError(f"{what}: the adapters are on {ad.a.device}, the rows on {dev}")
+    if ad.a.dim() != 3 or ad.b.dim() != 3 or ad.a.dtype != ad.b.dtype:
+        raise ValueError(f"{what}: adapters are a [n, rank, d_in] and b [n, d_out, rank] of one dtype")
+    n, r, k = ad.a.shape
+    if k != d_in or tuple(ad.b.shape) != (n, d_out, r):
+        raise ValueError(f"{what}: adapters a {tuple(ad.a.shape)}, b {tuple(ad.b.shape)} do not fit {d_in} -> {d_out}")
+    rpa = int(rows_per_adapter)
+    if rpa <= 0 or of.dtype != torch.int32 or of.numel() != -(-R // rpa):
+        raise ValueError(f"{what}: adapter_of must be int32 with one entry per {rpa} rows of {R}")
+    scale = _f32(ad.scale, "adapters.scale")
+    if scale is not None and scale.numel() != n:
+        raise ValueError(f"{what}: {scale.numel()} scales for {n} adapters")
+    return ad.a.contiguous(), ad.b.contiguous(), _hdt(ad.a, "adapters"), scale, n, r, of.contiguous(), rpa
+
+
 def project_in(h2: torch.Tensor, w_in: torch.Tensor, b_in=None, *, rms: bool = True, l2: bool = True,
                gate_w=None, gate_b=0.0, sel_w=None, sel_b=None, eps: float = 1e-6,
-               w_prep: Optional[torch.Tensor] = None, prefer_prep: bool = False):
+               w_prep: Optional[torch.Tensor] = None, prefer_prep: bool = False,
+               adapters: Optional[Adapters] = None, adapter_of: Optional[torch.Tensor] = None,
+               rows_per_adapter: int = 1):
     """(q [R, d_s], gate [R] | None, rstd [R], z [R, n_cand] | None) for rows h2 [R, d_m].
 
     q = L2((rms_norm(h2) if rms else h2) @ w_in^T + b_in) (L2 only if l2); w_in is [d_s, d_m] (nn.Linear).
     gate_b: a number, or a one-element device tensor read by the kernel. w_prep: weights_prep(w_in), to run the
     GEMM as 3xF16 on the f16 tensor cores (same accuracy as 3xTF32, half its MMAs); prefer_prep=True passes only
-    the prepared form (w_in then only gives the shape)."""
+    the prepared form (w_in then only gives the shape).
+    adapters: low-rank adapters added to w_in, adapter_of [ceil(R / rows_per_adapter)] int32 the one of each group of
+    rows_per_adapter rows (negative: none)."""
     dev = _cuda("project_in", h2, w_in, b_in, gate_w, sel_w, sel_b)
     h2 = h2.contiguous()
     w_in = _f32(w_in, "w_in")
@@ -141,9 +183,18 @@ def project_in(h2: torch.Tensor, w_in: torch.Tensor, b_in=None, *, rms: bool = T
     sel_w, sel_b = _f32(sel_w, "sel_w"), _f32(sel_b, "sel_b")
     gb, gb_dev = _dev_scalar(gate_b, "gate_b")
     with _on_device(dev):
+        w_arg = None if (prefer_prep and w_prep is not None) else w_in
+        if adapters is not None:
+            a, b, dt, scale, n, r, of, rpa = _adapter_args("project_in", dev, adapters, adapter_of, rows_per_adapter,
+                                                           R, d_m, d_s)
+            ws = _workspace(N.lib().xencb_project_in_adapted_workspace(R, d_m, d_s, r), dev)
+            N.call("xencb_project_in_adapted", _ptr(h2), _hdt(h2, "h"), R, d_m, _ptr(w_arg), _ptr(w_prep), _ptr(b_in),
+                   d_s, flags, _ptr(gate_w), gb, _ptr(gb_dev), _ptr(sel_w), _ptr(sel_b), n_cand, eps, _ptr(q),
+                   _ptr(gate), _ptr(rstd), _ptr(z), _ptr(a), _ptr(b), dt, _ptr(scale), n, r, _ptr(of), rpa, _ptr(ws),
+                   ws.numel(), _stream(dev))
+            return q, gate, rstd, z
         ws_bytes = N.lib().xencb_project_in_workspace(R, d_m, d_s)
         ws = _workspace(ws_bytes, dev)
-        w_arg = None if (prefer_prep and w_prep is not None) else w_in
         N.call("xencb_project_in", _ptr(h2), _hdt(h2, "h"), R, d_m, _ptr(w_arg), _ptr(w_prep), _ptr(b_in), d_s, flags,
                _ptr(gate_w), gb, _ptr(gb_dev), _ptr(sel_w), _ptr(sel_b), n_cand, eps, _ptr(q), _ptr(gate),
                _ptr(rstd), _ptr(z), _ptr(ws), ws.numel(), _stream(dev))
@@ -253,14 +304,17 @@ def project_in_route_lse(h2: torch.Tensor, w_in: torch.Tensor, b_in=None, *, S: 
 def project_out(r: torch.Tensor, w_out: torch.Tensor, h2: torch.Tensor, *, b_out=None, scale: float = 1.0,
                 log_scale: Optional[torch.Tensor] = None, gate=None, sel_w=None, log_alpha=0.0, pos_mask=None,
                 want_delta: bool = True, h_out: Optional[torch.Tensor] = None, want_rel: bool = False,
-                w_prep: Optional[torch.Tensor] = None, prefer_prep: bool = False):
+                w_prep: Optional[torch.Tensor] = None, prefer_prep: bool = False,
+                adapters: Optional[Adapters] = None, adapter_of: Optional[torch.Tensor] = None,
+                rows_per_adapter: int = 1):
     """(delta | None, h_out | None, rel | None).
 
     d = scale * exp(log_scale) * gate * (r @ w_out^T + b_out), w_out [d_m, d_s] (nn.Linear); optional
     LayerSelector matched norm with per-row weight sel_w and log_alpha (a number or a one-element device tensor;
     log_scale is a one-element device tensor or None);
     d *= pos_mask; delta = d in h2's dtype; h_out = h2 + delta; rel = ||delta|| / (||h2|| + 1e-6).
-    w_prep: weights_prep(w_out) for the 3xF16 GEMM."""
+    w_prep: weights_prep(w_out) for the 3xF16 GEMM. adapters, adapter_of, rows_per_adapter: as in project_in, added
+    to w_out."""
     dev = _cuda("project_out", r, w_out, h2, b_out, gate, sel_w, pos_mask, h_out)
     r = _f32(r, "r")
     w_out = _f32(w_out, "w_out")
@@ -278,9 +332,18 @@ def project_out(r: torch.Tensor, w_out: torch.Tensor, h2: torch.Tensor, *, b_out
     la, la_dev = _dev_scalar(log_alpha, "log_alpha")
     ls_dev = None if log_scale is None else _dev_scalar(log_scale, "log_scale")[1]
     with _on_device(dev):
+        w_arg = None if (prefer_prep and w_prep is not None) else w_out
+        if adapters is not None:
+            a, b, dt, ad_scale, n, rk, of, rpa = _adapter_args("project_out", dev, adapters, adapter_of,
+                                                               rows_per_adapter, R, d_s, d_m)
+            ws = _workspace(N.lib().xencb_project_out_adapted_workspace(R, d_s, d_m, rk), dev)
+            N.call("xencb_project_out_adapted", _ptr(r), R, d_s, _ptr(w_arg), _ptr(w_prep), _ptr(b_out), d_m,
+                   float(scale), _ptr(ls_dev), _ptr(gate), _ptr(sel_w), la, _ptr(la_dev), _ptr(pos_mask), _ptr(h2),
+                   _hdt(h2, "h"), _ptr(delta), _ptr(h_out), _ptr(rel), _ptr(a), _ptr(b), dt, _ptr(ad_scale), n, rk,
+                   _ptr(of), rpa, _ptr(ws), ws.numel(), _stream(dev))
+            return delta, h_out, rel
         ws_bytes = N.lib().xencb_project_out_workspace(R, d_s, d_m)
         ws = _workspace(ws_bytes, dev)
-        w_arg = None if (prefer_prep and w_prep is not None) else w_out
         N.call("xencb_project_out", _ptr(r), R, d_s, _ptr(w_arg), _ptr(w_prep), _ptr(b_out), d_m, float(scale),
                _ptr(ls_dev),
                _ptr(gate), _ptr(sel_w), la, _ptr(la_dev), _ptr(pos_mask), _ptr(h2), _hdt(h2, "h"), _ptr(delta),
@@ -709,6 +772,77 @@ def library_build(rows: torch.Tensor, counts, *, page_rows: Optional[int] = None
                _ptr(slots), _hdt(slots, "slots"), slots.shape[0], page_rows * d_s, page_rows, _ptr(page_of),
                _ptr(n_valid), _ptr(S), _ptr(ws), ws.numel(), _stream(dev))
     return slots, n_valid, S
+
+
+# ------------------------------------------------------------------------------------------------ pages
+def _pool_args(what: str, pools, page_of: torch.Tensor, n_valid: torch.Tensor, n_chunks_of):
+    """(device, pointer array, row-byte array, n_pages, page_rows) of pools that one page table describes."""
+    pools = list(pools)
+    if not pools:
+        raise ValueError(f"{what}: at least one pool is required")
+    dev = _cuda(what, *pools, page_of, n_valid, n_chunks_of)
+    P, N_rows = pools[0].shape[:2]
+    for p in pools:
+        _hdt(p, f"{what}: pool")
+        if p.dim() != 3 or not p.is_contiguous() or tuple(p.shape[:2]) != (P, N_rows):
+            raise ValueError(f"{what}: pools must be contiguous [pages, page_rows, d] tensors with the same pages, got "
+                             f"{tuple(p.shape)} beside {tuple(pools[0].shape)}")
+    for name, t in (("page_of", page_of), ("n_valid", n_valid)):
+        if t.dtype != torch.int32 or t.dim() != 2 or t.shape != page_of.shape or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be a contiguous int32 [n_lib, C] tensor")
+    if n_chunks_of is not None and (n_chunks_of.dtype != torch.int32 or n_chunks_of.numel() != page_of.shape[0]
+                                    or not n_chunks_of.is_contiguous()):
+        raise ValueError(f"{what}: n_chunks_of must be a contiguous int32 [n_lib] tensor")
+    ptrs = (ctypes.c_void_p * len(pools))(*[p.data_ptr() for p in pools])
+    sizes = (ctypes.c_int64 * len(pools))(*[p.shape[2] * p.element_size() for p in pools])
+    return dev, ptrs, sizes, P, N_rows
+
+
+def pages_fork(pools, page_of: torch.Tensor, n_valid: torch.Tensor, parents: torch.Tensor, own_from: torch.Tensor, *,
+               n_chunks_of: Optional[torch.Tensor] = None):
+    """(child_page_of [m, C] int32, missing [1] int32): fork m Libraries inside the pools they live in.
+
+    pools: the [P, page_rows, d] tensors that share one page table (every depth, keys and values). Child i shares
+    Library parents[i]'s pages for the chunks below own_from[i]; each chunk from there on gets a free page (one that no
+    entry of page_of names, in ascending order) holding a copy of the parent's valid rows, zeros behind them. missing
+    counts fresh pages that the pool did not have (their entries are -1); it is not read back here. Parents, page_of
+    and n_valid stay valid; page_of must name every page in use."""
+    dev, ptrs, sizes, P, page_rows = _pool_args("pages_fork", pools, page_of, n_valid, n_chunks_of)
+    if _cuda("pages_fork", parents, own_from) != dev:
+        raise RuntimeError(f"pages_fork: parents on {parents.device}, pools on {dev}")
+    for name, t in (("parents", parents), ("own_from", own_from)):
+        if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != parents.numel() or not t.is_contiguous():
+            raise ValueError(f"pages_fork: {name} must be a contiguous int32 [m] tensor")
+    n_lib, C = page_of.shape
+    m = int(parents.numel())
+    child = torch.empty(m, C, dtype=torch.int32, device=dev)
+    missing = torch.zeros(1, dtype=torch.int32, device=dev)
+    if m == 0:
+        return child, missing
+    with _on_device(dev):
+        ws = _workspace(N.lib().xencb_pages_fork_workspace(m, C), dev)
+        N.call("xencb_pages_fork", ptrs, sizes, len(ptrs), P, page_rows, _ptr(page_of), _ptr(n_valid), C,
+               _ptr(n_chunks_of), n_lib, _ptr(parents), _ptr(own_from), m, _ptr(child), _ptr(missing), _ptr(ws),
+               ws.numel(), _stream(dev))
+    return child, missing
+
+
+def pages_compact(pools, page_of: torch.Tensor, n_valid: torch.Tensor, *,
+                  n_chunks_of: Optional[torch.Tensor] = None):
+    """(page_of [n_lib, C] int32, n_live [1] int32): move the pages that page_of names to the front of the pools.
+
+    With n live pages, every live page at or above n moves to a free page below it (the rows some Library reads, zeros
+    behind them) in every pool; the returned table names the new places and pages [n, P) are free. n_live is not read
+    back here. The table given stays as it was."""
+    dev, ptrs, sizes, P, page_rows = _pool_args("pages_compact", pools, page_of, n_valid, n_chunks_of)
+    n_lib, C = page_of.shape
+    out = torch.empty_like(page_of)
+    n_live = torch.empty(1, dtype=torch.int32, device=dev)
+    with _on_device(dev):
+        ws = _workspace(N.lib().xencb_pages_compact_workspace(P), dev)
+        N.call("xencb_pages_compact", ptrs, sizes, len(ptrs), P, page_rows, _ptr(page_of), _ptr(n_valid), C,
+               _ptr(n_chunks_of), n_lib, _ptr(out), _ptr(n_live), _ptr(ws), ws.numel(), _stream(dev))
+    return out, n_live
 
 
 # ------------------------------------------------------------------------------------------------ D8 top-k read
