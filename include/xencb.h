@@ -261,6 +261,31 @@ XENCB_API int xencb_read_prefill(const float* q, int64_t n_rows, int d_s, const 
                                  int read_softmax, float* r_out, void* workspace, size_t workspace_bytes,
                                  void* stream);
 
+/* Shared read: the result of xencb_read_decode with every page fetched once for all query rows that read it, whichever
+ * Libraries they belong to (Libraries whose tables name the same pages, many rows of one Library, prompts with top-k
+ * routing; xenc/injector.py:239-245, 263-265). The (row, routed chunk) pairs are grouped by page on the device and
+ * each page is read by up to 64 of them at once on the tensor cores (32 for float32 results).
+ *   q       [n_rows, d_s] of q_dtype
+ *   r_out   [n_rows, d_s] of out_dtype. XENCB_F32: q and the softmax weights enter the tensor cores as pairs of
+ *           16-bit values (22 bits with f16 slots, 16 with bf16). XENCB_F16 / XENCB_BF16: one rounding of each, and
+ *           one of the result.
+ *   idx, wk as xencb_route writes them; a chunk may appear more than once in a row; entries with idx < 0 or
+ *           wk == 0 are skipped, a row without any gives 0. idx >= n_chunks or a page outside the pool is skipped and
+ *           flagged (XENCB_DEV_BADPAGE).
+ * A page's Libraries may disagree on its n_valid; a slot that some row of the call reads must be finite for the
+ * rows that mask it (slots past every reader's n_valid may hold anything). Chunks with n_valid 0 contribute 0.
+ * f16 / bf16 slots, d_s a multiple of 8 up to 4096, a dense pool (page_stride == page_rows * d_s), any page_rows; else
+ * XENCB_ENOTSUP. The result does not depend on how the pairs are grouped. Workspace:
+ * xencb_read_shared_workspace bytes, 256-byte aligned. */
+XENCB_API size_t xencb_read_shared_workspace(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows,
+                                             int slots_dtype, int out_dtype);
+XENCB_API int xencb_read_shared(const void* q, int q_dtype, int64_t n_rows, int d_s, const void* slots,
+                                const void* vslots, int slots_dtype, int64_t n_pages, int64_t page_stride,
+                                int page_rows, const int32_t* page_of, const int32_t* n_valid, int n_chunks,
+                                int64_t rows_per_lib, int64_t n_lib, const int32_t* idx, const float* wk, int k,
+                                float read_temp, int read_softmax, void* r_out, int out_dtype, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
 /* Dense routing of one chunk shard of a Library (the routing softmax of xenc/injector.py:220-229 with top_k = 0,
  * regrouped by shard): w_out [n_rows, n_chunks] = e^(l_c - max_c l_c) with l = route_temp * q . S_c, and
  * header_out [n_rows, 4] = (max_c l_c, sum_c e^(l_c - max), 0, 0). Feeding w_out to xencb_read_multi gives the

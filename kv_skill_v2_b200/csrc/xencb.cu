@@ -29,6 +29,7 @@
 #include "exchange.cuh"
 #include "pages.cuh"
 #include "adapt.cuh"
+#include "read_shared.cuh"
 
 // Scratch of xencb_read_decode_noalloc: a fixed device array, so that entry point never allocates.
 static __device__ __align__(256) unsigned char g_noalloc_scratch[XENCB_NOALLOC_SCRATCH_BYTES];
@@ -654,6 +655,144 @@ int plan_build(int n_chunks, int d_s, int page_rows, BuildPlan* p) {
   p->n_split = (page_rows + p->split_rows - 1) / p->split_rows;
   p->part_bytes = align_up((size_t)n_chunks * p->n_split * d_s * sizeof(float), 256);
   p->threads = (int)align_up((size_t)((d_s + LB_VEC - 1) / LB_VEC), 32);
+  return XENCB_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ shared read plan
+struct SharedPlan {
+  int terms, cs, ns, slab, seg_rows, segs, mt;
+  int64_t n_pairs, max_tiles;
+  size_t cnt, pair, tiles, q, part, ml, total;  // bytes of each workspace part
+};
+
+int plan_shared(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows, int slots_dtype, int out_dtype,
+                SharedPlan* p) {
+  if (n_rows <= 0 || k <= 0 || d_s <= 0 || n_pages <= 0 || page_rows <= 0)
+    return fail(XENCB_EINVAL, "read_shared: sizes must be positive");
+  if (slots_dtype != XENCB_F16 && slots_dtype != XENCB_BF16)
+    return fail(XENCB_ENOTSUP, "read_shared: the tensor-core read takes f16 / bf16 slots");
+  if (!elem_size(out_dtype)) return fail(XENCB_EINVAL, "read_shared: out_dtype %d unknown", out_dtype);
+  if (d_s % 8 != 0 || d_s > RS_SLAB * RS_MAX_CS)
+    return fail(XENCB_ENOTSUP, "read_shared: d_s=%d must be a multiple of 8, at most %d", d_s, RS_SLAB * RS_MAX_CS);
+  if (n_rows > INT32_MAX / k || 2 * n_rows * k + RS_AROWS > INT32_MAX)
+    return fail(XENCB_ENOTSUP, "read_shared: %lld rows x %d routed chunks are too many", (long long)n_rows, k);
+  if (n_pages * (int64_t)page_rows + 1024 > INT32_MAX)
+    return fail(XENCB_ENOTSUP, "read_shared: the slot pool is too large for 32-bit TMA coordinates");
+  p->n_pairs = n_rows * k;
+  p->terms = out_dtype == XENCB_F32 ? 2 : 1;
+  p->mt = RS_AROWS / p->terms;
+  p->cs = d_s <= 4 * RS_SLAB ? 4 : 8;
+  p->slab = (int)align_up((size_t)(d_s + p->cs - 1) / p->cs, 64);
+  p->ns = 512 / p->cs;
+  p->seg_rows = 512;
+  p->segs = (page_rows + p->seg_rows - 1) / p->seg_rows;
+  if (p->n_pairs * p->segs > INT32_MAX)
+    return fail(XENCB_ENOTSUP, "read_shared: page_rows=%d is too long for this many rows", page_rows);
+  p->max_tiles = p->n_pairs / p->mt + std::min<int64_t>(n_pages, p->n_pairs) + 1;
+  p->cnt = align_up((size_t)n_pages * 8, 256);
+  p->pair = align_up((size_t)p->n_pairs * 4, 256);
+  p->tiles = align_up((size_t)p->max_tiles * sizeof(SharedTile), 256);
+  p->q = align_up((size_t)p->terms * p->n_pairs * d_s * 2, 256);
+  p->part = align_up((size_t)p->n_pairs * p->segs * d_s * 4, 256);
+  p->ml = align_up((size_t)p->n_pairs * p->segs * 8, 256);
+  p->total = p->cnt + 4 * p->pair + p->tiles + 256 + p->q + p->part + p->ml;
+  return XENCB_OK;
+}
+
+// Clusters of the read kernel that fit the device at once, per device, cluster size and kernel.
+template <typename K>
+int shared_clusters(K kern, int cs, int* out) {
+  static std::mutex mu;
+  static std::unordered_map<const void*, int> known[kMaxDev][RS_MAX_CS + 1];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lk(mu);
+  auto& m = known[dev][cs];
+  const auto itr = m.find(reinterpret_cast<const void*>(kern));
+  if (itr != m.end()) {
+    *out = itr->second;
+    return XENCB_OK;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)cs);
+  cfg.blockDim = dim3(RS_THREADS);
+  cfg.dynamicSmemBytes = RS_SMEM;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)cs;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  int n = 0;
+  const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
+  if (e != cudaSuccess) return cuda_fail(e, "read_shared: cudaOccupancyMaxActiveClusters");
+  if (n <= 0) return fail(XENCB_ENOTSUP, "read_shared: no cluster of %d CTAs fits this device", cs);
+  m[reinterpret_cast<const void*>(kern)] = n;
+  *out = n;
+  return XENCB_OK;
+}
+
+template <typename T, int TERMS>
+int run_shared(const void* q, int q_dtype, const SharedPlan& p, SharedArgs a, const void* slots, const void* vslots,
+               void* q16, int64_t n_rows, void* r_out, int out_dtype, int sms, cudaStream_t st) {
+  const CUtensorMapDataType dt =
+      std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const uint64_t d = (uint64_t)a.d_s, pool_rows = (uint64_t)a.n_pages * a.page_rows;
+  CUtensorMap mq, mk, mv;
+  int rc = tensor_map_2d(&mq, dt, 2, q16, d, (uint64_t)TERMS * p.n_pairs, d * 2, 64, (uint32_t)p.mt);
+  if (!rc) rc = tensor_map_2d(&mk, dt, 2, slots, d, pool_rows, d * 2, 64, (uint32_t)p.ns);
+  if (!rc) rc = tensor_map_2d(&mv, dt, 2, vslots ? vslots : slots, d, pool_rows, d * 2, 64, 64);
+  auto kern = shared_read_kernel<T, TERMS>;
+  if (!rc) rc = ensure_smem(kern, (int)RS_SMEM);
+  int n_clusters = 0;
+  if (!rc) rc = shared_clusters(kern, p.cs, &n_clusters);
+  if (rc) return rc;
+  n_clusters = (int)std::min<int64_t>(n_clusters, p.max_tiles * p.segs);
+  if (p.n_pairs <= 4096) {
+    shared_plan_kernel<<<1, 1024, 0, st>>>(a, p.mt);
+    XENCB_CHECK_LAUNCH("shared_plan launch");
+  } else {
+    const cudaError_t e = cudaMemsetAsync(a.cnt, 0, (size_t)a.n_pages * 8, st);
+    if (e != cudaSuccess) return cuda_fail(e, "read_shared: memset");
+    shared_count_kernel<<<(unsigned)std::min<int64_t>((p.n_pairs + 255) / 256, 4 * sms), 256, 0, st>>>(a);
+    XENCB_CHECK_LAUNCH("shared_count launch");
+    shared_scan_kernel<<<1, 1024, 0, st>>>(a, p.mt);
+    XENCB_CHECK_LAUNCH("shared_scan launch");
+  }
+  T* qo = static_cast<T*>(q16);
+  switch (q_dtype) {
+    case XENCB_F32:
+      shared_split_kernel<float, T, TERMS><<<(unsigned)p.n_pairs, 256, 0, st>>>(static_cast<const float*>(q), a, qo);
+      break;
+    case XENCB_F16:
+      shared_split_kernel<__half, T, TERMS><<<(unsigned)p.n_pairs, 256, 0, st>>>(static_cast<const __half*>(q), a, qo);
+      break;
+    default:
+      shared_split_kernel<__nv_bfloat16, T, TERMS>
+          <<<(unsigned)p.n_pairs, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(q), a, qo);
+      break;
+  }
+  XENCB_CHECK_LAUNCH("shared_split launch");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(n_clusters * p.cs));
+  cfg.blockDim = dim3(RS_THREADS);
+  cfg.dynamicSmemBytes = RS_SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)p.cs;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  (void)cudaLaunchKernelEx(&cfg, kern, mq, mk, mv, a);
+  XENCB_CHECK_LAUNCH("shared_read launch");
+  const dim3 grid((unsigned)n_rows, (unsigned)((a.d_s + 1023) / 1024));
+  switch (out_dtype) {
+    case XENCB_F32: shared_combine_kernel<float><<<grid, 256, 0, st>>>(a, static_cast<float*>(r_out)); break;
+    case XENCB_F16: shared_combine_kernel<__half><<<grid, 256, 0, st>>>(a, static_cast<__half*>(r_out)); break;
+    default: shared_combine_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a, static_cast<__nv_bfloat16*>(r_out)); break;
+  }
+  XENCB_CHECK_LAUNCH("shared_combine launch");
   return XENCB_OK;
 }
 }  // namespace
@@ -1388,6 +1527,72 @@ int xencb_read_prefill(const float* q, int64_t n_rows, int d_s, const void* slot
   }
   XENCB_CHECK_LAUNCH("prefill_read launch");
   return XENCB_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ read_shared
+size_t xencb_read_shared_workspace(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows, int slots_dtype,
+                                   int out_dtype) {
+  SharedPlan p;
+  return plan_shared(n_rows, k, d_s, n_pages, page_rows, slots_dtype, out_dtype, &p) ? 0 : p.total;
+}
+
+int xencb_read_shared(const void* q, int q_dtype, int64_t n_rows, int d_s, const void* slots, const void* vslots,
+                      int slots_dtype, int64_t n_pages, int64_t page_stride, int page_rows, const int32_t* page_of,
+                      const int32_t* n_valid, int n_chunks, int64_t rows_per_lib, int64_t n_lib, const int32_t* idx,
+                      const float* wk, int k, float read_temp, int read_softmax, void* r_out, int out_dtype,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+  if (!q || !slots || !page_of || !n_valid || !idx || !wk || !r_out)
+    return fail(XENCB_EINVAL, "read_shared: q, slots, page_of, n_valid, idx, wk and r_out are required");
+  if (!elem_size(q_dtype)) return fail(XENCB_EINVAL, "read_shared: q_dtype %d unknown", q_dtype);
+  if (n_chunks <= 0 || rows_per_lib <= 0 || n_lib <= 0)
+    return fail(XENCB_EINVAL, "read_shared: sizes must be positive");
+  SharedPlan p;
+  int rc = plan_shared(n_rows, k, d_s, n_pages, page_rows, slots_dtype, out_dtype, &p);
+  if (rc) return rc;
+  if ((n_rows + rows_per_lib - 1) / rows_per_lib > n_lib)
+    return fail(XENCB_EINVAL, "read_shared: %lld rows need more than %lld Libraries", (long long)n_rows,
+                (long long)n_lib);
+  if (page_stride != (int64_t)page_rows * d_s)
+    return fail(XENCB_ENOTSUP, "read_shared: the slot pool must be dense ([pages, page_rows, d_s])");
+  if (!aligned(slots, 16) || !aligned(q, 16) || !aligned(r_out, 16) || (vslots && !aligned(vslots, 16)))
+    return fail(XENCB_EINVAL, "read_shared: slots, vslots, q and r_out must be 16-byte aligned");
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < p.total)
+    return fail(XENCB_EINVAL, "read_shared: workspace needs %zu bytes, 256-byte aligned (got %zu)", p.total,
+                workspace_bytes);
+  DevInfo di;
+  rc = device_info(&di);
+  if (rc) return rc;
+  char* ws = static_cast<char*>(workspace);
+  auto take = [&](size_t bytes) {
+    char* at = ws;
+    ws += bytes;
+    return at;
+  };
+  SharedArgs a{};
+  a.page_of = page_of; a.n_valid = n_valid; a.idx = idx; a.wk = wk; a.n_rows = n_rows; a.rows_per_lib = rows_per_lib;
+  a.n_lib = n_lib; a.k = k; a.C = n_chunks; a.n_pages = (int)n_pages; a.page_rows = page_rows; a.d_s = d_s;
+  a.n_pairs = (int)p.n_pairs;
+  a.cnt = reinterpret_cast<int*>(take(p.cnt));
+  a.nvmax = a.cnt + n_pages;
+  a.page = reinterpret_cast<int*>(take(p.pair));
+  a.rank = reinterpret_cast<int*>(take(p.pair));
+  a.pnv = reinterpret_cast<int*>(take(p.pair));
+  a.qinv = reinterpret_cast<float*>(take(p.pair));
+  a.tiles = reinterpret_cast<SharedTile*>(take(p.tiles));
+  a.n_tiles = reinterpret_cast<int*>(take(256));
+  void* q16 = take(p.q);
+  a.part = reinterpret_cast<float*>(take(p.part));
+  a.ml = reinterpret_cast<float2*>(take(p.ml));
+  a.segs = p.segs; a.seg_rows = p.seg_rows; a.cs = p.cs; a.ns = p.ns; a.slab = p.slab;
+  a.softmax = read_softmax ? 1 : 0;
+  a.qscale = read_softmax ? read_temp * 1.4426950408889634f : 1.f;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (slots_dtype == XENCB_F16)
+    return p.terms == 2 ? run_shared<__half, 2>(q, q_dtype, p, a, slots, vslots, q16, n_rows, r_out, out_dtype, di.sms, st)
+                        : run_shared<__half, 1>(q, q_dtype, p, a, slots, vslots, q16, n_rows, r_out, out_dtype, di.sms, st);
+  return p.terms == 2
+             ? run_shared<__nv_bfloat16, 2>(q, q_dtype, p, a, slots, vslots, q16, n_rows, r_out, out_dtype, di.sms, st)
+             : run_shared<__nv_bfloat16, 1>(q, q_dtype, p, a, slots, vslots, q16, n_rows, r_out, out_dtype, di.sms, st);
 }
 
 // ------------------------------------------------------------------------------------------------ project_out

@@ -588,6 +588,47 @@ def read_prefill(q: torch.Tensor, pages: Pages, w: torch.Tensor, *, rows_per_lib
     return out
 
 
+def read_shared(q: torch.Tensor, pages: Pages, idx: torch.Tensor, wk: torch.Tensor, *, rows_per_lib: int,
+                read_temp: float = 12.0, read_softmax: bool = True,
+                out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """r [R, d_s]: the read of read_decode with every page fetched once for all rows that read it -- Libraries whose
+    tables name the same pages (forks of a document), many rows on one document, prompts with top-k routing.
+
+    q [R, d_s] float32 / float16 / bfloat16; idx, wk [R, k] as route gives them. out_dtype float32: 22 bits of q and of
+    the softmax weights (16 with bfloat16 slots); float16 / bfloat16: each rounded once, and the result. Raises
+    NotImplementedError for float32 slots and d_s above 4096 or not a multiple of 8 (use read_decode)."""
+    dev = _cuda("read_shared", q, pages.slots, pages.page_of, pages.n_valid, idx, wk)
+    q = q.contiguous()
+    wk = _f32(wk, "wk")
+    if q.dim() != 2:
+        raise ValueError("read_shared: q must be [R, d_s]")
+    R, d_s = q.shape
+    slots = pages.slots
+    if not slots.is_contiguous():
+        raise ValueError("read_shared: the slot pool must be contiguous")
+    if slots.shape[-1] != d_s:
+        raise ValueError(f"read_shared: q has d_s={d_s}, slots have {slots.shape[-1]}")
+    if idx.dtype != torch.int32 or idx.dim() != 2 or idx.shape != wk.shape or idx.shape[0] != R:
+        raise ValueError("read_shared: idx must be int32 [R, k] matching wk")
+    if out_dtype not in _DT:
+        raise ValueError(f"read_shared: out_dtype {out_dtype} not supported (float32 / float16 / bfloat16)")
+    k = int(idx.shape[1])
+    idx = idx.contiguous()
+    r = torch.empty(R, d_s, dtype=out_dtype, device=dev)
+    dt, odt = _hdt(slots, "slots"), _DT[out_dtype]
+    P, page_rows = slots.shape[0], pages.page_rows
+    with _on_device(dev):
+        ws_bytes = N.lib().xencb_read_shared_workspace(R, k, d_s, P, page_rows, dt, odt)
+        if ws_bytes == 0:
+            N.check(N.EINVAL if min(R, k) <= 0 else N.ENOTSUP, "read_shared_workspace")
+        ws = _workspace(ws_bytes, dev)
+        N.call("xencb_read_shared", _ptr(q), _hdt(q, "q"), R, d_s, _ptr(slots), _ptr(_vpool(pages)), dt, P,
+               page_rows * d_s, page_rows, _ptr(pages.page_of), _ptr(pages.n_valid), pages.n_chunks, int(rows_per_lib),
+               pages.n_lib, _ptr(idx), _ptr(wk), k, float(read_temp), int(bool(read_softmax)), _ptr(r), odt, _ptr(ws),
+               ws.numel(), _stream(dev))
+    return r
+
+
 def multi_supported(pages: Pages, n_rows: int, rows_per_lib: int) -> bool:
     """Whether read_multi takes this slot pool (f16 / bf16 slots, d_s % 16 == 0, the stages fit on chip)."""
     if pages.slots.dtype not in (torch.float16, torch.bfloat16) or pages.d_s % 16:
