@@ -35,16 +35,31 @@
 
 namespace xencb {
 
-constexpr int RS_AROWS = 64;      // rows of the A operands that carry data (TERMS * MT); the MMA's M is 128
-constexpr int RS_MAX_CS = 8;      // CTAs per cluster: 4 (d_s <= 2048) or 8
+constexpr int RS_MAX_CS = 8;      // CTAs per cluster: 4 or 8
 constexpr int RS_SLAB = 512;      // columns of d_s per CTA at most (TMEM)
-constexpr int RS_STAGES = 4;
-constexpr int RS_STAGE = 32768;   // scores: A 8 KB + B 16 KB; read: 4 boxes of 64 slots x 64 columns
-constexpr int RS_PBLK = RS_AROWS * 128;       // P of 64 slots: one 128-byte swizzle row per pair
-constexpr int RS_THREADS = 32 * 10;           // producer, MMA, 8 softmax / epilogue warps
+constexpr int RS_VROWS = 32;      // slots per stage of the read product
 constexpr int RS_ACC = 4;         // score accumulators in TMEM (ns columns each)
 constexpr int RS_CHUNK = 2;       // TERMS = 2: k-blocks per accumulator (8 accumulation steps)
 constexpr float RS_P_SCALE = 16384.f;         // P is scaled by 2^14
+
+// The kernel's shapes. AROWS: rows of the A operands that carry data (TERMS * MT pairs; the MMA's M is 128 whatever
+// they are, the other rows are not looked at).
+//   32: clusters of 8, two CTAs per SM (256 TMEM columns each): one unit's softmax and epilogue run under the other's
+//       loads. For pages that few rows read: the tile of Q is small beside the page's.
+//   64: one CTA per SM with a deeper ring: each page is fetched for twice the pairs.
+template <int AROWS>
+struct RsShape {
+  static constexpr int quarters = AROWS / 32;               // TMEM lane quarters that carry data
+  static constexpr int stage = AROWS == 32 ? 16384 : 24576;  // scores: A tile + B tile; read: 4 boxes of 32 x 64
+  static constexpr int stages = AROWS == 32 ? 4 : 6;
+  static constexpr int pblk = AROWS * 128;                  // P of 64 slots: one 128-byte swizzle row per A row
+  static constexpr int producer = quarters, mma = quarters + 1;  // warps; 0..quarters-1 and 4.. do the softmax
+  static constexpr int threads = 32 * (4 + quarters);
+  static constexpr int ctas = AROWS == 32 ? 2 : 1;          // per SM
+  static constexpr int stat_floats = 2 * 2 * RS_MAX_CS * AROWS;  // [2][2 * cs][MT]
+  static constexpr size_t smem =
+      1024 + 8 * pblk + (size_t)stages * stage + 2 * stat_floats * 4 + (2 * stages + 2 * RS_ACC + 5) * 8 + 16;
+};
 
 struct __align__(16) SharedTile {
   int page, start, count, nv;  // pairs [start, start + count) in grouped order; nv: the page's most valid slots
@@ -69,7 +84,7 @@ struct SharedArgs {
   int* pnv;        // [n_pairs] by position: valid slots
   float* qinv;     // [n_pairs] by position: 1 / (the row's power-of-two scale)
   // read
-  int segs, seg_rows, cs, ns, slab;
+  int segs, seg_rows, cs, ns, slab, tmem_cols;
   float qscale;    // read_temp * log2(e), or 1
   int softmax;
   float* part;     // [n_pairs][segs][d_s], normalised per segment
@@ -212,6 +227,18 @@ __global__ void __launch_bounds__(256) shared_split_kernel(const TQ* __restrict_
 }
 
 // ----------------------------------------------------------------------------------------------------- cluster PTX
+// True in one thread of a converged warp. The compiler issues TMA and MMA instructions of an elected thread from
+// uniform registers; under `lane == 0` each cost about 150 cycles to issue, which bound the kernel (one stage of three
+// copies 770 cycles, whatever its bytes).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred P;\n\t"
+      "elect.sync _|P, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, P;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
@@ -249,28 +276,52 @@ __device__ __forceinline__ void bulk_s2s(uint32_t dst_cluster, const void* src, 
       : "memory");
 }
 
+// Two floats rounded to 16 bits in one instruction (x in the low half), and the rounded values.
+__device__ __forceinline__ uint32_t rs_pack(__half, float x, float y, float2& r) {
+  const __half2 h = __floats2half2_rn(x, y);
+  r = __half22float2(h);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t rs_pack(__nv_bfloat16, float x, float y, float2& r) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  r = __bfloat1622float2(h);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 // ----------------------------------------------------------------------------------------------------- read
 struct RsSmem {
-  unsigned char* p;       // [8 blocks][RS_PBLK]
-  unsigned char* stages;  // [RS_STAGES][RS_STAGE]
+  unsigned char* p;       // [8 blocks][pblk]
+  unsigned char* stages;  // the ring
   float* smax;            // [2][2 * cs][MT]: by the parity of the unit (a CTA without scores may lag a unit behind)
-  float* ssum;            // [2][2 * cs][MT]
+  float* ssum;            // [2][16][MT]: per 32 slots
   uint64_t *full, *empty, *s_full, *s_empty, *p_full, *o_full, *o_empty, *stat, *sums;
   uint32_t* tmem;
   volatile int* abort_flag;
 };
-constexpr size_t RS_SMEM = 1024 + 8 * RS_PBLK + (size_t)RS_STAGES * RS_STAGE + 2 * 4 * RS_MAX_CS * RS_AROWS * 4 +
-                           (2 * RS_STAGES + 2 * RS_ACC + 5) * 8 + 16;
 
+// A place in the ring of stages: the stage and the parity of its next completion.
+struct RsRing {
+  uint32_t st, phase;
+  __device__ __forceinline__ void next(uint32_t n) {
+    if (++st == n) { st = 0; phase ^= 1; }
+  }
+  __device__ __forceinline__ void back(uint32_t n) {
+    if (st == 0) { st = n; phase ^= 1; }
+    --st;
+  }
+};
+
+template <int AROWS>
 __device__ __forceinline__ RsSmem rs_smem(unsigned char* base) {
+  using C = RsShape<AROWS>;
   RsSmem s;
   s.p = base;
-  s.stages = base + 8 * RS_PBLK;
-  s.smax = reinterpret_cast<float*>(s.stages + RS_STAGES * RS_STAGE);
-  s.ssum = s.smax + 4 * RS_MAX_CS * RS_AROWS;
-  s.full = reinterpret_cast<uint64_t*>(s.ssum + 4 * RS_MAX_CS * RS_AROWS);
-  s.empty = s.full + RS_STAGES;
-  s.s_full = s.empty + RS_STAGES;
+  s.stages = base + 8 * C::pblk;
+  s.smax = reinterpret_cast<float*>(s.stages + C::stages * C::stage);
+  s.ssum = s.smax + C::stat_floats;
+  s.full = reinterpret_cast<uint64_t*>(s.ssum + C::stat_floats);
+  s.empty = s.full + C::stages;
+  s.s_full = s.empty + C::stages;
   s.s_empty = s.s_full + RS_ACC;
   s.p_full = s.s_empty + RS_ACC;
   s.o_full = s.p_full + 1;
@@ -282,33 +333,36 @@ __device__ __forceinline__ RsSmem rs_smem(unsigned char* base) {
   return s;
 }
 
-template <typename T, int TERMS>
-__global__ void __launch_bounds__(RS_THREADS, 1)
-    shared_read_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                       const __grid_constant__ CUtensorMap map_v, const SharedArgs a) {
-  constexpr int MT = RS_AROWS / TERMS;              // pairs per tile
+template <typename T, int TERMS, int AROWS>
+__global__ void __launch_bounds__(RsShape<AROWS>::threads, RsShape<AROWS>::ctas)
+    shared_read_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_q8,
+                       const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                       const SharedArgs a) {
+  using C = RsShape<AROWS>;
+  constexpr int MT = AROWS / TERMS;                 // pairs per tile
   constexpr int FMT = std::is_same<T, __half>::value ? UMMA_F16 : UMMA_BF16;
-  constexpr int QUARTERS = RS_AROWS / 32;           // TMEM lane quarters that carry data
-  constexpr int CQ = QUARTERS / TERMS;              // quarters of the hi terms: the warps that do the softmax
-  constexpr int CW = 2 * CQ, AW = 2 * QUARTERS;     // their warps (two column halves each); warps that read TMEM
+  constexpr bool SAME = AROWS == 32 && TERMS == 2;  // a pair's hi and lo rows are lanes i and i + 16 of one warp
+  constexpr int CQ = SAME ? 1 : C::quarters / TERMS;  // quarters of the hi terms
+  constexpr int CW = 2 * CQ, AW = 2 * C::quarters;    // warps that do the softmax (two column halves); that read TMEM
   extern __shared__ unsigned char rs_smem_raw[];
-  const RsSmem s = rs_smem(reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(rs_smem_raw) + 1023) &
-                                                            ~uintptr_t(1023)));
+  const RsSmem s = rs_smem<AROWS>(reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(rs_smem_raw) + 1023) & ~uintptr_t(1023)));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cs = a.cs, ns = a.ns;
   const int rank = (int)cluster_rank();
   const int cluster = blockIdx.x / cs, n_clusters = gridDim.x / cs;
   const int nkb = (a.d_s + 63) / 64;
-  const int kpc = TERMS == 2 ? RS_CHUNK : nkb;                    // k-blocks per score accumulator
-  const int x0 = rank * a.slab;                                   // this CTA's columns of d_s
+  const int kpc = TERMS == 2 ? RS_CHUNK : nkb;                     // k-blocks per score accumulator
+  const int x0 = rank * a.slab;                                    // this CTA's columns of d_s
   const int my_boxes = max(0, min(a.slab, a.d_s - x0) + 63) / 64;  // in boxes of 64
-  const uint32_t blk_bytes = (uint32_t)(ns / 64) * RS_PBLK;       // this CTA's share of P
+  const uint32_t blk_bytes = (uint32_t)(ns / 64) * C::pblk;        // this CTA's share of P
 
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_q);
+    prefetch_tensormap(&map_q8);
     prefetch_tensormap(&map_k);
     prefetch_tensormap(&map_v);
-    for (int i = 0; i < RS_STAGES; ++i) {
+    for (int i = 0; i < C::stages; ++i) {
       mbar_init(&s.full[i], 1);
       mbar_init(&s.empty[i], 1);
     }
@@ -324,8 +378,8 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
     *s.abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 1) {
-    tc_alloc(s.tmem, 512);
+  if (warp == C::mma) {
+    tc_alloc(s.tmem, (uint32_t)a.tmem_cols);
     tc_relinquish();
   }
   tc_fence_before();
@@ -336,22 +390,12 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
   pdl_wait();
   const int n_units = *a.n_tiles * a.segs;
 
-  if (warp == 0) {
+  if (warp == C::producer) {
     // --------------------------------------------------------------------------------------------- producer
-    if (lane == 0) {
-      uint32_t it = 0;
+    if (elect_one()) {
+      RsRing ring{0, 0};
+      uint32_t used = 0;
       bool ok = true;
-      auto stage = [&](uint32_t bytes) -> unsigned char* {
-        const uint32_t st = it % RS_STAGES, use = it / RS_STAGES;
-        if (use > 0 && (!mbar_wait_bounded(&s.empty[st], (use - 1) & 1) || *s.abort_flag)) {
-          *s.abort_flag = 1;
-          ok = false;
-          return nullptr;
-        }
-        mbar_arrive_expect_tx(&s.full[st], bytes);
-        ++it;
-        return s.stages + st * RS_STAGE;
-      };
       for (int u = cluster; u < n_units && ok; u += n_clusters) {
         const SharedTile t = a.tiles[u / a.segs];
         const int seg0 = (u % a.segs) * a.seg_rows;
@@ -359,347 +403,397 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
         if (nv <= 0) continue;
         const int y0 = t.page * a.page_rows + seg0;
         if (rank * ns < nv) {
+          const bool few = t.count <= 8;  // eight rows of Q a term; what lies in the others is not looked at
+          const uint32_t tx = (uint32_t)((few ? 8 : MT) * TERMS + ns) * 128;
           for (int kb = 0; kb < nkb && ok; ++kb) {
-            unsigned char* st = stage((uint32_t)(RS_AROWS * 128 + ns * 128));
-            if (!st) break;
-            uint64_t* bar = &s.full[(it - 1) % RS_STAGES];
+            if (used >= C::stages) ok = mbar_wait_bounded(&s.empty[ring.st], ring.phase ^ 1);
+            if (!ok) break;
+            uint64_t* bar = &s.full[ring.st];
+            unsigned char* st = s.stages + ring.st * C::stage;
+            mbar_arrive_expect_tx(bar, tx);
+            tma_load_2d(st + AROWS * 128, &map_k, kb * 64, y0 + rank * ns, bar);
+            if (few) {
 #pragma unroll
-            for (int x = 0; x < TERMS; ++x)
-              tma_load_2d(st + x * MT * 128, &map_q, kb * 64, x * a.n_pairs + t.start, bar);
-            tma_load_2d(st + RS_AROWS * 128, &map_k, kb * 64, y0 + rank * ns, bar);
+              for (int x = 0; x < TERMS; ++x)
+                tma_load_2d(st + x * MT * 128, &map_q8, kb * 64, x * a.n_pairs + t.start, bar);
+            } else {
+#pragma unroll
+              for (int x = 0; x < TERMS; ++x)
+                tma_load_2d(st + x * MT * 128, &map_q, kb * 64, x * a.n_pairs + t.start, bar);
+            }
+            ring.next(C::stages);
+            ++used;
           }
         }
-        for (int b = 0; b < (nv + 63) / 64 && ok; ++b)
-          for (int h = 0; h < my_boxes && ok; h += 4) {
+        for (int b = 0; b < (nv + RS_VROWS - 1) / RS_VROWS && ok; ++b)
+          for (int h = 0; h < my_boxes; h += 4) {
             const int n = min(4, my_boxes - h);
-            unsigned char* st = stage((uint32_t)n * 64 * 128);
-            if (!st) break;
+            if (used >= C::stages) ok = mbar_wait_bounded(&s.empty[ring.st], ring.phase ^ 1);
+            if (!ok) break;
+            uint64_t* bar = &s.full[ring.st];
+            unsigned char* st = s.stages + ring.st * C::stage;
+            mbar_arrive_expect_tx(bar, (uint32_t)n * RS_VROWS * 128);
             for (int i = 0; i < n; ++i)
-              tma_load_2d(st + i * 64 * 128, &map_v, x0 + (h + i) * 64, y0 + b * 64, &s.full[(it - 1) % RS_STAGES]);
+              tma_load_2d(st + i * RS_VROWS * 128, &map_v, x0 + (h + i) * 64, y0 + b * RS_VROWS, bar);
+            ring.next(C::stages);
+            ++used;
           }
       }
+      if (!ok) *s.abort_flag = 1;
       // the copies in flight end before the CTA's shared memory goes away
-      const uint32_t n_last = it < RS_STAGES ? it : RS_STAGES;
-      for (uint32_t i = 0; i < n_last; ++i) {
-        const uint32_t last = it - 1 - i;
-        mbar_wait_bounded(&s.full[last % RS_STAGES], (last / RS_STAGES) & 1);
+      for (uint32_t i = min(used, (uint32_t)C::stages); i > 0; --i) {
+        ring.back(C::stages);
+        mbar_wait_bounded(&s.full[ring.st], ring.phase);
       }
     }
     __syncwarp();
-  } else if (warp == 1) {
+  } else if (warp == C::mma) {
     // --------------------------------------------------------------------------------------------- MMA issuer
-    uint32_t it = 0, unit = 0, acc = 0;
-    bool ok = true;
-    auto wait_full = [&]() -> int {  // the next stage, or -1
-      const uint32_t st = it % RS_STAGES;
-      if (!mbar_wait_bounded(&s.full[st], (it / RS_STAGES) & 1) || *s.abort_flag) {
-        *s.abort_flag = 1;
-        ok = false;
-        return -1;
-      }
-      ++it;
-      tc_fence_after();
-      return (int)st;
-    };
-    const uint32_t id_s = umma_idesc(FMT, FMT, 128, ns);
-    for (int u = cluster; u < n_units && ok; u += n_clusters) {
-      const SharedTile t = a.tiles[u / a.segs];
-      const int nv = min(t.nv - (u % a.segs) * a.seg_rows, a.seg_rows);
-      if (nv <= 0) continue;
-      if (unit > 0 && (!mbar_wait_bounded(s.o_empty, (unit - 1) & 1) || *s.abort_flag)) {
-        *s.abort_flag = 1;
-        break;
-      }
-      tc_fence_after();
-      if (rank * ns < nv) {
-        for (int kb = 0; kb < nkb; ++kb) {
-          const int in = kb % kpc;
-          const uint32_t buf = acc % RS_ACC, use = acc / RS_ACC;
-          if (in == 0 && use > 0) {
-            if (!mbar_wait_bounded(&s.s_empty[buf], (use - 1) & 1) || *s.abort_flag) {
-              *s.abort_flag = 1;
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-          }
-          const int st = wait_full();
-          if (st < 0) break;
-          const bool last = in == kpc - 1 || kb == nkb - 1;
-          if (lane == 0) {
-            const uint32_t sa = smem_u32(s.stages + st * RS_STAGE), sb = sa + RS_AROWS * 128;
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-              tc_mma<0>(taddr + buf * (uint32_t)ns, umma_desc_k_sw128(sa + ks * 32), umma_desc_k_sw128(sb + ks * 32),
-                        id_s, in > 0 || ks > 0);
-            tc_commit(&s.empty[st]);
-            if (last) tc_commit(&s.s_full[buf]);
-          }
-          acc += last;
-          __syncwarp();
-        }
-        if (!ok) break;
-      }
-      // every CTA's block of P is here (and this CTA's softmax warps have read the scores)
-      if (!mbar_wait_cluster(s.p_full, unit & 1) || *s.abort_flag) {
-        *s.abort_flag = 1;
-        break;
-      }
-      tc_fence_after();
-      for (int b = 0; b < (nv + 63) / 64 && ok; ++b) {
-        const int left = nv - b * 64, steps = min(4, (left + 15) / 16);
-        for (int h = 0; h < my_boxes; h += 4) {
-          const int n = min(4, my_boxes - h);
-          const int st = wait_full();
-          if (st < 0) break;
-          unsigned char* base = s.stages + st * RS_STAGE;
-          if (left < steps * 16) {  // rows of V behind the last valid slot: zeros
-            for (int i = lane; i < (steps * 16 - left) * n * 8; i += 32) {
-              const int r = left + i / (n * 8), c = i % (n * 8);
-              *reinterpret_cast<uint4*>(base + (c >> 3) * 64 * 128 + r * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-          }
-          if (lane == 0) {
-            const uint32_t sp = smem_u32(s.p + b * RS_PBLK), sv = smem_u32(base);
-            const uint32_t id = umma_idesc(FMT, FMT, 128, n * 64, 1);
-            for (int ks = 0; ks < steps; ++ks)
-              tc_mma<0>(taddr + (uint32_t)h * 64, umma_desc_k_sw128(sp + ks * 32),
-                        umma_desc_mn_sw128(sv + ks * 2048, 64 * 128), id, b > 0 || ks > 0);
-            tc_commit(&s.empty[st]);
-          }
-          __syncwarp();
-        }
-      }
-      if (!ok) break;
-      if (lane == 0) tc_commit(s.o_full);
-      __syncwarp();
-      ++unit;
-    }
-  } else {
-    // --------------------------------------------------------------------------------------------- softmax, epilogue
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
-    if (quarter < QUARTERS) {
-      const int term = quarter / CQ;                  // 0: hi rows, which do the softmax
-      const int row = (quarter % CQ) * 32 + lane;     // pair of the tile
-      const uint32_t tl = taddr + ((uint32_t)(quarter * 32) << 16);
-      const int hw = ns / 2;                          // score columns of this warp
-      // scratch of the lo -> hi hand-over: the block of P that belongs to another CTA (no copy reads it, and none
-      // arrives before this CTA's maxima of the unit are out): [columns][rows of a pair of warps]
-      float* xch = reinterpret_cast<float*>(s.p + (size_t)((rank + 1 + half) % cs) * blk_bytes) +
-                   (quarter % CQ) * 32 * ns;
+    if (elect_one()) {
+      RsRing ring{0, 0};
       uint32_t unit = 0, acc = 0;
-      // A wait that runs out sets the abort flag; from then on nothing is waited for, and the warps run through their
-      // units on whatever is there, so that the named barriers they share stay matched.
-      auto done = [&](bool arrived) {
-        if (!arrived) *s.abort_flag = 1;
-      };
+      bool ok = true;
+      const uint32_t id_s = umma_idesc(FMT, FMT, 128, ns);
+      // operand descriptors: the constant part, and addresses in 16-byte units (14 bits: the address of a CTA's shared
+      // memory carries its cluster rank above them)
+      const uint64_t dk = umma_desc_k_sw128(0), dv = umma_desc_mn_sw128(0, RS_VROWS * 128);
+      const uint32_t st0 = (smem_u32(s.stages) >> 4) & 0x3FFFu, p0 = (smem_u32(s.p) >> 4) & 0x3FFFu;
       for (int u = cluster; u < n_units; u += n_clusters) {
         const SharedTile t = a.tiles[u / a.segs];
-        const int seg = u % a.segs, seg0 = seg * a.seg_rows;
-        const int nv = min(t.nv - seg0, a.seg_rows);
+        const int nv = min(t.nv - (u % a.segs) * a.seg_rows, a.seg_rows);
         if (nv <= 0) continue;
-        const bool mine = rank * ns < nv;
-        float* smax = s.smax + (unit & 1) * 2 * cs * MT;
-        float* ssum = s.ssum + (unit & 1) * 2 * cs * MT;
-        const bool live = row < t.count;
-        const int pos = t.start + (live ? row : 0);
-        const int pnv = live ? a.pnv[pos] - seg0 : 0;            // the pair's valid slots in this segment
-        const float c = live ? a.qinv[pos] * a.qscale : 0.f;
-        const int c0 = rank * ns + half * hw;                    // first slot of this warp's columns
-        float v[64];
-        float mx = a.softmax ? -CUDART_INF_F : 0.f;
-        if (mine) {
-          for (int k0 = 0; k0 < nkb; k0 += kpc, ++acc) {
-            const uint32_t buf = acc % RS_ACC;
-            done(*s.abort_flag || mbar_wait_bounded(&s.s_full[buf], (acc / RS_ACC) & 1));
+        if (unit > 0 && !(ok = mbar_wait_bounded(s.o_empty, (unit - 1) & 1))) break;
+        tc_fence_after();
+        if (rank * ns < nv) {
+          for (int k0 = 0; k0 < nkb && ok; k0 += kpc, ++acc) {
+            const uint32_t buf = acc % RS_ACC, use = acc / RS_ACC;
+            if (use > 0 && !(ok = mbar_wait_bounded(&s.s_empty[buf], (use - 1) & 1))) break;
             tc_fence_after();
-            const uint32_t at = tl + buf * (uint32_t)ns + (uint32_t)(half * hw);
-            float x[64];
-            if (hw == 64) {
-              tc_ld64(at, x);
-            } else {
-              tc_ld32(at, x);
+            const int k1 = min(nkb, k0 + kpc);
+            for (int kb = k0; kb < k1; ++kb) {
+              if (!(ok = mbar_wait_bounded(&s.full[ring.st], ring.phase))) break;
+              tc_fence_after();
+              const uint64_t da = dk + (st0 + ring.st * (C::stage / 16)), db = da + AROWS * 8;
 #pragma unroll
-              for (int i = 32; i < 64; ++i) x[i] = 0.f;
+              for (int ks = 0; ks < 4; ++ks)
+                tc_mma<0>(taddr + buf * (uint32_t)ns, da + ks * 2, db + ks * 2, id_s, kb > k0 || ks > 0);
+              tc_commit(&s.empty[ring.st]);
+              ring.next(C::stages);
             }
-#pragma unroll
-            for (int i = 0; i < 64; ++i) v[i] = k0 == 0 ? x[i] : v[i] + x[i];
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s.s_empty[buf]);
+            if (!ok) break;
+            tc_commit(&s.s_full[buf]);
           }
-          if (TERMS == 2) {
-            if (term == 1)
-#pragma unroll
-              for (int i = 0; i < 64; ++i)
-                if (i < hw) xch[i * 32 + lane] = v[i];
-            fence_proxy_async_smem();  // before another CTA's copy may land on the scratch
-            tc_fence_before();         // before the read product may overwrite the scores
-            named_bar_sync(2 + half * CQ + quarter % CQ, 64);
-            if (term == 0)
-#pragma unroll
-              for (int i = 0; i < 64; ++i)
-                if (i < hw) v[i] += xch[i * 32 + lane];
+          if (!ok) break;
+        }
+        // every CTA's block of P is here (and this CTA's softmax warps have read the scores)
+        if (!(ok = mbar_wait_cluster(s.p_full, unit & 1))) break;
+        tc_fence_after();
+        for (int b = 0; b < (nv + RS_VROWS - 1) / RS_VROWS && ok; ++b) {
+          const int left = nv - b * RS_VROWS, steps = min(RS_VROWS / 16, (left + 15) / 16);
+          // slots [b * 32, b * 32 + 32) of P: half a block of 64
+          const uint64_t dp = dk + (p0 + (b / 2) * (C::pblk / 16) + (b & 1) * 4);
+          for (int h = 0; h < my_boxes; h += 4) {
+            const int n = min(4, my_boxes - h);
+            if (!(ok = mbar_wait_bounded(&s.full[ring.st], ring.phase))) break;
+            tc_fence_after();
+            if (left < steps * 16) {  // rows of V behind the last valid slot: zeros (0 * NaN would not be 0)
+              unsigned char* base = s.stages + ring.st * C::stage;
+              for (int i = 0; i < n; ++i)
+                for (int c = left * 8; c < steps * 16 * 8; ++c)
+                  *reinterpret_cast<uint4*>(base + i * RS_VROWS * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+              fence_proxy_async_smem();
+            }
+            const uint64_t dx = dv + (st0 + ring.st * (C::stage / 16));
+            const uint32_t id = umma_idesc(FMT, FMT, 128, n * 64, 1);
+            for (int ks = 0; ks < steps; ++ks)
+              tc_mma<0>(taddr + (uint32_t)h * 64, dp + ks * 2, dx + ks * 128, id, b > 0 || ks > 0);
+            tc_commit(&s.empty[ring.st]);
+            ring.next(C::stages);
           }
         }
-        if (term == 0) {
-          if (mine) {
+        if (!ok) break;
+        tc_commit(s.o_full);
+        ++unit;
+      }
+      if (!ok) *s.abort_flag = 1;
+    }
+    __syncwarp();
+  } else if ((warp & 3) < C::quarters) {
+    // --------------------------------------------------------------------------------------------- softmax, epilogue
+    const int quarter = warp & 3, half = warp >> 2;
+    const int term = SAME ? lane >> 4 : quarter / CQ;                        // 0: hi rows
+    const int row = SAME ? lane & 15 : (quarter % CQ) * 32 + lane;           // pair of the tile
+    const bool does = SAME || term == 0;                                     // this warp does the softmax
+    const uint32_t tl = taddr + ((uint32_t)(quarter * 32) << 16);
+    const int hw = ns / 2;                                                   // score columns of this warp
+    const int pair_bar = 2 + half * CQ + quarter % CQ;                       // a hi warp and its lo warp
+    // scratch of the lo -> hi hand-over: the block of P that belongs to another CTA (no copy reads it, and none
+    // arrives before this CTA's maxima of the unit are out): [columns][rows of a pair of warps]
+    float* xch = reinterpret_cast<float*>(s.p + (size_t)((rank + 1 + half) % cs) * blk_bytes) + (quarter % CQ) * 32 * ns;
+    uint32_t unit = 0, acc = 0;
+    // A wait that runs out sets the abort flag; from then on nothing is waited for, and the warps run through their
+    // units on whatever is there, so that the named barriers they share stay matched.
+    auto done = [&](bool arrived) {
+      if (!arrived) *s.abort_flag = 1;
+    };
+    for (int u = cluster; u < n_units; u += n_clusters) {
+      const SharedTile t = a.tiles[u / a.segs];
+      const int seg = u % a.segs, seg0 = seg * a.seg_rows;
+      const int nv = min(t.nv - seg0, a.seg_rows);
+      if (nv <= 0) continue;
+      const bool mine = rank * ns < nv;
+      float* smax = s.smax + (unit & 1) * 2 * cs * MT;
+      float* ssum = s.ssum + (unit & 1) * 16 * MT;
+      const bool live = row < t.count;
+      const int pos = t.start + (live ? row : 0);
+      const int pnv = live ? a.pnv[pos] - seg0 : 0;            // the pair's valid slots in this segment
+      const float c = live ? a.qinv[pos] * a.qscale : 0.f;
+      const int c0 = rank * ns + half * hw;                    // first slot of this warp's columns
+      float v[64];
+      float mx = a.softmax ? -CUDART_INF_F : 0.f;
+      if (mine) {
+        for (int k0 = 0; k0 < nkb; k0 += kpc, ++acc) {
+          const uint32_t buf = acc % RS_ACC;
+          done(*s.abort_flag || mbar_wait_bounded(&s.s_full[buf], (acc / RS_ACC) & 1));
+          tc_fence_after();
+          const uint32_t at = tl + buf * (uint32_t)ns + (uint32_t)(half * hw);
+          float x[64];
+          if (hw == 64) {
+            tc_ld64(at, x);
+          } else {
+            tc_ld32(at, x);
 #pragma unroll
-            for (int i = 0; i < 64; ++i) {
-              v[i] *= c;
-              if (i < hw && c0 + i < pnv) mx = fmaxf(mx, a.softmax ? v[i] : fabsf(v[i]));
-            }
+            for (int i = 32; i < 64; ++i) x[i] = 0.f;
           }
-          // the rows' maxima to every CTA of the cluster
-          for (int r = 0; r < cs; ++r) st_cluster_f32(cluster_map(&smax[(rank * 2 + half) * MT + row], r), mx);
+#pragma unroll
+          for (int i = 0; i < 64; ++i) v[i] = k0 == 0 ? x[i] : v[i] + x[i];
+          tc_fence_before();
           __syncwarp();
-          if (lane < cs) mbar_arrive_cluster(cluster_map(s.stat, lane));
-          done(*s.abort_flag || mbar_wait_cluster(s.stat, unit & 1));
-          float m = a.softmax ? -CUDART_INF_F : 0.f;
-          for (int r = 0; r < 2 * cs; ++r) m = fmaxf(m, smax[r * MT + row]);
-          float l = 0.f;
-          if (mine) {
-            const float lin = a.softmax ? 0.f : f16_range_scale(m);
+          if (lane == 0) mbar_arrive(&s.s_empty[buf]);
+        }
+        if (SAME) {
 #pragma unroll
-            for (int i = 0; i < 64; ++i) {
-              float p = 0.f;
-              if (i < hw && c0 + i < pnv)
-                p = a.softmax ? RS_P_SCALE * (TERMS == 2 ? exp2f(v[i] - m) : pf_exp2(v[i] - m)) : v[i] * lin;
-              l += p;
-              v[i] = p;
+          for (int i = 0; i < 64; ++i)
+            if (i < hw) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 16);
+        } else if (TERMS == 2) {
+          if (term == 1)
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+              if (i < hw) xch[i * 32 + lane] = v[i];
+          fence_proxy_async_smem();  // before another CTA's copy may land on the scratch
+          tc_fence_before();         // before the read product may overwrite the scores
+          named_bar_sync(pair_bar, 64);
+          if (term == 0)
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+              if (i < hw) v[i] += xch[i * 32 + lane];
+        }
+      }
+      if (does) {
+        // t = scores * scale; masked slots -inf (softmax) or 0 (linear read). A row whose every score is masked gets
+        // max -inf and then NaN weights: it has no slot in this segment, so nothing reads them.
+        const int lim = min(pnv - c0, hw);
+        if (mine && a.softmax) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) {
+            v[i] = i < lim ? v[i] * c : -CUDART_INF_F;
+            mx = fmaxf(mx, v[i]);
+          }
+        } else if (mine) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) {
+            v[i] = i < lim ? v[i] * c : 0.f;
+            mx = fmaxf(mx, fabsf(v[i]));
+          }
+        }
+        // the rows' maxima to every CTA of the cluster
+        if (!SAME || lane < 16)
+          for (int r = 0; r < cs; ++r) st_cluster_f32(cluster_map(&smax[(rank * 2 + half) * MT + row], r), mx);
+        __syncwarp();
+        if (lane < cs) mbar_arrive_cluster(cluster_map(s.stat, lane));
+        done(*s.abort_flag || mbar_wait_cluster(s.stat, unit & 1));
+        float m = a.softmax ? -CUDART_INF_F : 0.f;
+        for (int r = 0; r < 2 * cs; ++r) m = fmaxf(m, smax[r * MT + row]);
+        float l[2] = {0.f, 0.f};  // sums of 32 columns each, whatever the shape: it changes no bit of a result
+        if (mine) {
+          if (a.softmax) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int i = g * 32; i < g * 32 + 32; ++i) {
+                v[i] = RS_P_SCALE * pf_exp2(v[i] - m);
+                l4[i & 3] += v[i];
+              }
+              l[g] = (l4[0] + l4[1]) + (l4[2] + l4[3]);
             }
-            // this row's P in 16 bits: block (c0 / 64), 16-byte chunk j of row r at chunk j ^ (r % 8)
-            unsigned char* blk = s.p + (size_t)(c0 >> 6) * RS_PBLK;
-            const int j0 = (c0 & 63) >> 3;
+          } else {
+            const float lin = f16_range_scale(m);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              if (j * 8 < hw) {
-                uint32_t hi[4], lo[4];
+            for (int i = 0; i < 64; ++i) v[i] *= lin;
+          }
+          // this row's P in 16 bits: block (c0 / 64), 16-byte chunk j of A row r at chunk j ^ (r % 8)
+          unsigned char* blk = s.p + (size_t)(c0 >> 6) * C::pblk;
+          const int j0 = (c0 & 63) >> 3;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  float r0, r1, q0, q1;
-                  hi[e] = pack2<T>(v[j * 8 + 2 * e], v[j * 8 + 2 * e + 1], r0, r1);
-                  if (TERMS == 2) lo[e] = pack2<T>(v[j * 8 + 2 * e] - r0, v[j * 8 + 2 * e + 1] - r1, q0, q1);
-                }
-                const int ch = (j0 + j) ^ (row & 7);
-                *reinterpret_cast<uint4*>(blk + row * 128 + ch * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          for (int j = 0; j < 8; ++j) {
+            if (j * 8 < hw) {
+              uint32_t hi[4], lo[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float x = v[j * 8 + 2 * e], y = v[j * 8 + 2 * e + 1];
+                float2 r, r2;
+                hi[e] = rs_pack(T{}, x, y, r);
+                if (TERMS == 2) lo[e] = rs_pack(T{}, x - r.x, y - r.y, r2);
+              }
+              const int ch = (j0 + j) ^ (row & 7);  // (MT is a multiple of 8: the same for the lo row)
+              const uint4 h4 = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+              if (SAME) {  // lanes 0-15 hold the hi rows, 16-31 the lo rows of the same pairs
+                const uint4 l4 = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                *reinterpret_cast<uint4*>(blk + lane * 128 + ch * 16) = term ? l4 : h4;
+              } else {
+                *reinterpret_cast<uint4*>(blk + row * 128 + ch * 16) = h4;
                 if (TERMS == 2)
                   *reinterpret_cast<uint4*>(blk + (MT + row) * 128 + ch * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
               }
             }
-            fence_proxy_async_smem();
           }
-          tc_fence_before();
-          named_bar_sync(1, 32 * CW);
-          if (warp == 4 && lane == 0) {  // quarter 0, half 0
-            // the other CTAs' blocks are still to come; then this CTA's block to them
-            const int n_work = min(cs, (nv + ns - 1) / ns);
-            mbar_arrive_expect_tx(s.p_full, (uint32_t)(n_work - (mine ? 1 : 0)) * blk_bytes);
-            if (mine && !*s.abort_flag)
-              for (int r = 1; r < cs; ++r) {
-                const uint32_t to = (uint32_t)((rank + r) % cs);
-                unsigned char* src = s.p + (size_t)rank * blk_bytes;
-                bulk_s2s(cluster_map(src, to), src, blk_bytes, cluster_map(s.p_full, to));
-              }
-          }
-          for (int r = 0; r < cs; ++r) st_cluster_f32(cluster_map(&ssum[(rank * 2 + half) * MT + row], r), l);
-          __syncwarp();
-          if (lane < cs) mbar_arrive_cluster(cluster_map(s.sums, lane));
-        }
-        // ------------------------------------------------------------------------------------- epilogue
-        float coef = 0.f;
-        if (term == 0) {
-          done(*s.abort_flag || mbar_wait_cluster(s.sums, unit & 1));
-          float m = a.softmax ? -CUDART_INF_F : 0.f, l = 0.f;
-          for (int r = 0; r < 2 * cs; ++r) {
-            m = fmaxf(m, smax[r * MT + row]);
-            l += ssum[r * MT + row];
-          }
-          if (a.softmax) coef = l != 0.f ? 1.f / l : 0.f;
-          else coef = pnv + seg0 > 0 ? rsqrtf((float)(pnv + seg0)) / f16_range_scale(m) : 0.f;
-          if (live && rank == 0 && half == 0) a.ml[(int64_t)pos * a.segs + seg] = make_float2(m, l);
-        }
-        done(*s.abort_flag || mbar_wait_bounded(s.o_full, unit & 1));
-        tc_fence_after();
-        const int cols = my_boxes * 64, pass = 32;
-        float* dst = a.part + ((int64_t)pos * a.segs + seg) * a.d_s + x0;
-        // the two halves of the warps take alternate passes of 32 columns
-        for (int q0 = half * pass; q0 < cols; q0 += 2 * pass) {
-          float o[32];
-          tc_ld32(tl + (uint32_t)q0, o);
-          if (TERMS == 2) {
-            if (term == 1)
-#pragma unroll
-              for (int i = 0; i < 32; ++i) xch[i * 32 + lane] = o[i];
-            named_bar_sync(2 + half * CQ + quarter % CQ, 64);
-            if (term == 0)
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] += xch[i * 32 + lane];
-            named_bar_sync(2 + half * CQ + quarter % CQ, 64);
-          }
-          if (term == 0 && live) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              if (x0 + q0 + i < a.d_s)
-                *reinterpret_cast<float4*>(dst + q0 + i) =
-                    make_float4(o[i] * coef, o[i + 1] * coef, o[i + 2] * coef, o[i + 3] * coef);
-          }
+          fence_proxy_async_smem();
         }
         tc_fence_before();
+        named_bar_sync(1, 32 * CW);
+        if (warp == 0 && lane == 0) {
+          // the other CTAs' blocks are still to come; then this CTA's block to them
+          const int n_work = min(cs, (nv + ns - 1) / ns);
+          mbar_arrive_expect_tx(s.p_full, (uint32_t)(n_work - (mine ? 1 : 0)) * blk_bytes);
+          if (mine && !*s.abort_flag)
+            for (int r = 1; r < cs; ++r) {
+              const uint32_t to = (uint32_t)((rank + r) % cs);
+              unsigned char* src = s.p + (size_t)rank * blk_bytes;
+              bulk_s2s(cluster_map(src, to), src, blk_bytes, cluster_map(s.p_full, to));
+            }
+        }
         __syncwarp();
-        if (lane == 0) mbar_arrive(s.o_empty);
-        ++unit;
+        if (!SAME || lane < 16)
+          for (int r = 0; r < cs; ++r) {
+            const uint32_t to = cluster_map(&ssum[(c0 >> 5) * MT + row], r);
+            st_cluster_f32(to, l[0]);
+            if (hw == 64) st_cluster_f32(to + MT * 4, l[1]);
+          }
+        __syncwarp();
+        if (lane < cs) mbar_arrive_cluster(cluster_map(s.sums, lane));
       }
+      // ------------------------------------------------------------------------------------- epilogue
+      float coef = 0.f;
+      if (does) {
+        done(*s.abort_flag || mbar_wait_cluster(s.sums, unit & 1));
+        float m = a.softmax ? -CUDART_INF_F : 0.f, l = 0.f;
+        for (int r = 0; r < 2 * cs; ++r) m = fmaxf(m, smax[r * MT + row]);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) l += ssum[r * MT + row];
+        if (a.softmax) coef = l != 0.f ? 1.f / l : 0.f;
+        else coef = pnv + seg0 > 0 ? rsqrtf((float)(pnv + seg0)) / f16_range_scale(m) : 0.f;
+        if (live && rank == 0 && half == 0 && (!SAME || term == 0))
+          a.ml[(int64_t)pos * a.segs + seg] = make_float2(m, l);
+      }
+      done(*s.abort_flag || mbar_wait_bounded(s.o_full, unit & 1));
+      tc_fence_after();
+      float* dst = a.part + ((int64_t)pos * a.segs + seg) * a.d_s + x0;
+      // the two halves of the warps take alternate boxes of 64 columns. The lo rows' parts go through the scratch: two
+      // buffers in turn where it holds two (one barrier a box then separates a write from the read two boxes before)
+      for (int b = half, turn = 0; b < my_boxes; b += 2, turn ^= 1) {
+        float o[64];
+        tc_ld64(tl + (uint32_t)b * 64, o);
+        if (SAME) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) o[i] += __shfl_xor_sync(0xffffffffu, o[i], 16);
+        } else if (TERMS == 2) {
+          float* x = xch + (ns == 128 ? turn * 64 * 32 : 0);
+          if (term == 1)
+#pragma unroll
+            for (int i = 0; i < 64; ++i) x[i * 32 + lane] = o[i];
+          named_bar_sync(pair_bar, 64);
+          if (term == 0)
+#pragma unroll
+            for (int i = 0; i < 64; ++i) o[i] += x[i * 32 + lane];
+          if (ns != 128) named_bar_sync(pair_bar, 64);
+        }
+        if (does && live) {
+#pragma unroll
+          for (int i = 0; i < 64; i += 4)
+            if (x0 + b * 64 + i < a.d_s && (!SAME || (i >> 5) == term))  // SAME: a pair's two lanes store a half each
+              *reinterpret_cast<float4*>(dst + b * 64 + i) =
+                  make_float4(o[i] * coef, o[i + 1] * coef, o[i + 2] * coef, o[i + 3] * coef);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s.o_empty);
+      ++unit;
     }
   }
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // no CTA leaves while another may still write to its shared memory
   tc_fence_after();
-  if (warp == 1) tc_dealloc(taddr, 512);
+  if (warp == C::mma) tc_dealloc(taddr, (uint32_t)a.tmem_cols);
 }
 
 // ----------------------------------------------------------------------------------------------------- combine
-// r[row] = sum_j wk[row, j] * (the pair's segments, merged by their maxima and sums), in the order of j.
+// r[row] = sum_j wk[row, j] * (the pair's segments, merged by their maxima and sums). One CTA per (row, 128 columns):
+// 8 groups of 32 threads take the routed chunks j = group, group + 8, ..., and their sums are added in the order of the
+// groups, so the result depends on nothing but the row.
+constexpr int RC_GROUPS = 8;
 template <typename TO>
-__global__ void __launch_bounds__(256) shared_combine_kernel(const SharedArgs a, TO* __restrict__ r) {
-  pdl_wait();
+__global__ void __launch_bounds__(32 * RC_GROUPS) shared_combine_kernel(const SharedArgs a, TO* __restrict__ r) {
+  __shared__ float4 sum[RC_GROUPS][32];
   const int64_t row = blockIdx.x;
   const int64_t lib = row / a.rows_per_lib;
-  const int x = (blockIdx.y * 256 + threadIdx.x) * 4;
-  if (x >= a.d_s) return;
+  const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
+  const int x = (blockIdx.y * 32 + lane) * 4;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int j = 0; j < a.k; ++j) {
+  for (int j = grp; j < a.k; j += RC_GROUPS) {
     const int64_t pair = row * a.k + j;
     const int page = a.page[pair];
     if (page < 0) continue;
     const int64_t pos = a.cnt[page] + a.rank[pair];
-    const int nv = min(a.n_valid[lib * a.C + a.idx[pair]], a.page_rows);
-    const int segs = (nv + a.seg_rows - 1) / a.seg_rows;
     const float w = a.wk[pair];
     const float* p = a.part + pos * a.segs * a.d_s + x;
+    int segs = 1;
     float m = -CUDART_INF_F, z = 0.f;
-    if (a.softmax && segs > 1) {
-      for (int g = 0; g < segs; ++g) m = fmaxf(m, a.ml[pos * a.segs + g].x);
-      for (int g = 0; g < segs; ++g) {
-        const float2 ml = a.ml[pos * a.segs + g];
-        z += exp2f(ml.x - m) * ml.y;
+    if (a.segs > 1) {
+      const int nv = min(a.n_valid[lib * a.C + a.idx[pair]], a.page_rows);
+      segs = (nv + a.seg_rows - 1) / a.seg_rows;
+      if (a.softmax) {
+        for (int g = 0; g < segs; ++g) m = fmaxf(m, a.ml[pos * a.segs + g].x);
+        for (int g = 0; g < segs; ++g) {
+          const float2 ml = a.ml[pos * a.segs + g];
+          z += exp2f(ml.x - m) * ml.y;
+        }
       }
     }
     for (int g = 0; g < segs; ++g) {
       float f = w;
-      if (a.softmax && segs > 1) {
+      if (a.softmax && a.segs > 1) {
         const float2 ml = a.ml[pos * a.segs + g];
         f *= exp2f(ml.x - m) * ml.y / z;
       }
-      const float4 v = *reinterpret_cast<const float4*>(p + (int64_t)g * a.d_s);
-      acc.x = fmaf(f, v.x, acc.x);
-      acc.y = fmaf(f, v.y, acc.y);
-      acc.z = fmaf(f, v.z, acc.z);
-      acc.w = fmaf(f, v.w, acc.w);
+      if (x < a.d_s) {
+        const float4 v = *reinterpret_cast<const float4*>(p + (int64_t)g * a.d_s);
+        acc.x = fmaf(f, v.x, acc.x);
+        acc.y = fmaf(f, v.y, acc.y);
+        acc.z = fmaf(f, v.z, acc.z);
+        acc.w = fmaf(f, v.w, acc.w);
+      }
     }
+  }
+  sum[grp][lane] = acc;
+  __syncthreads();
+  if (grp != 0 || x >= a.d_s) return;
+  const int n = min(a.k, RC_GROUPS);
+  for (int g = 1; g < n; ++g) {
+    const float4 v = sum[g][lane];
+    acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
   }
   TO* o = r + row * a.d_s + x;
   o[0] = from_f32<TO>(acc.x);

@@ -660,7 +660,7 @@ int plan_build(int n_chunks, int d_s, int page_rows, BuildPlan* p) {
 
 // ------------------------------------------------------------------------------------------------ shared read plan
 struct SharedPlan {
-  int terms, cs, ns, slab, seg_rows, segs, mt;
+  int terms, arows, cs, ns, slab, tmem_cols, seg_rows, segs, mt;
   int64_t n_pairs, max_tiles;
   size_t cnt, pair, tiles, q, part, ml, total;  // bytes of each workspace part
 };
@@ -674,16 +674,20 @@ int plan_shared(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows, 
   if (!elem_size(out_dtype)) return fail(XENCB_EINVAL, "read_shared: out_dtype %d unknown", out_dtype);
   if (d_s % 8 != 0 || d_s > RS_SLAB * RS_MAX_CS)
     return fail(XENCB_ENOTSUP, "read_shared: d_s=%d must be a multiple of 8, at most %d", d_s, RS_SLAB * RS_MAX_CS);
-  if (n_rows > INT32_MAX / k || 2 * n_rows * k + RS_AROWS > INT32_MAX)
+  if (n_rows > INT32_MAX / k || 2 * n_rows * k + 64 > INT32_MAX)
     return fail(XENCB_ENOTSUP, "read_shared: %lld rows x %d routed chunks are too many", (long long)n_rows, k);
   if (n_pages * (int64_t)page_rows + 1024 > INT32_MAX)
     return fail(XENCB_ENOTSUP, "read_shared: the slot pool is too large for 32-bit TMA coordinates");
   p->n_pairs = n_rows * k;
   p->terms = out_dtype == XENCB_F32 ? 2 : 1;
-  p->mt = RS_AROWS / p->terms;
-  p->cs = d_s <= 4 * RS_SLAB ? 4 : 8;
+  // Few pairs a page on average (a tile of 32 / terms holds them): the shape with two CTAs per SM.
+  const bool few = d_s <= 4 * RS_SLAB && p->n_pairs <= n_pages * (32 / p->terms);
+  p->arows = few ? 32 : 64;
+  p->mt = p->arows / p->terms;
+  p->cs = few || d_s > 4 * RS_SLAB ? 8 : 4;
   p->slab = (int)align_up((size_t)(d_s + p->cs - 1) / p->cs, 64);
   p->ns = 512 / p->cs;
+  p->tmem_cols = few ? 256 : 512;  // >= slab and >= RS_ACC * ns; two CTAs of the first shape share an SM's 512
   p->seg_rows = 512;
   p->segs = (page_rows + p->seg_rows - 1) / p->seg_rows;
   if (p->n_pairs * p->segs > INT32_MAX)
@@ -701,7 +705,7 @@ int plan_shared(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows, 
 
 // Clusters of the read kernel that fit the device at once, per device, cluster size and kernel.
 template <typename K>
-int shared_clusters(K kern, int cs, int* out) {
+int shared_clusters(K kern, int cs, int threads, size_t smem, int* out) {
   static std::mutex mu;
   static std::unordered_map<const void*, int> known[kMaxDev][RS_MAX_CS + 1];
   int dev = 0;
@@ -715,8 +719,8 @@ int shared_clusters(K kern, int cs, int* out) {
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)cs);
-  cfg.blockDim = dim3(RS_THREADS);
-  cfg.dynamicSmemBytes = RS_SMEM;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = (unsigned)cs;
@@ -732,20 +736,22 @@ int shared_clusters(K kern, int cs, int* out) {
   return XENCB_OK;
 }
 
-template <typename T, int TERMS>
+template <typename T, int TERMS, int AROWS>
 int run_shared(const void* q, int q_dtype, const SharedPlan& p, SharedArgs a, const void* slots, const void* vslots,
                void* q16, int64_t n_rows, void* r_out, int out_dtype, int sms, cudaStream_t st) {
   const CUtensorMapDataType dt =
       std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const uint64_t d = (uint64_t)a.d_s, pool_rows = (uint64_t)a.n_pages * a.page_rows;
-  CUtensorMap mq, mk, mv;
+  using Shape = RsShape<AROWS>;
+  CUtensorMap mq, mq8, mk, mv;
   int rc = tensor_map_2d(&mq, dt, 2, q16, d, (uint64_t)TERMS * p.n_pairs, d * 2, 64, (uint32_t)p.mt);
+  if (!rc) rc = tensor_map_2d(&mq8, dt, 2, q16, d, (uint64_t)TERMS * p.n_pairs, d * 2, 64, 8);
   if (!rc) rc = tensor_map_2d(&mk, dt, 2, slots, d, pool_rows, d * 2, 64, (uint32_t)p.ns);
-  if (!rc) rc = tensor_map_2d(&mv, dt, 2, vslots ? vslots : slots, d, pool_rows, d * 2, 64, 64);
-  auto kern = shared_read_kernel<T, TERMS>;
-  if (!rc) rc = ensure_smem(kern, (int)RS_SMEM);
+  if (!rc) rc = tensor_map_2d(&mv, dt, 2, vslots ? vslots : slots, d, pool_rows, d * 2, 64, RS_VROWS);
+  auto kern = shared_read_kernel<T, TERMS, AROWS>;
+  if (!rc) rc = ensure_smem(kern, (int)Shape::smem);
   int n_clusters = 0;
-  if (!rc) rc = shared_clusters(kern, p.cs, &n_clusters);
+  if (!rc) rc = shared_clusters(kern, p.cs, Shape::threads, Shape::smem, &n_clusters);
   if (rc) return rc;
   n_clusters = (int)std::min<int64_t>(n_clusters, p.max_tiles * p.segs);
   if (p.n_pairs <= 4096) {
@@ -775,8 +781,8 @@ int run_shared(const void* q, int q_dtype, const SharedPlan& p, SharedArgs a, co
   XENCB_CHECK_LAUNCH("shared_split launch");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(n_clusters * p.cs));
-  cfg.blockDim = dim3(RS_THREADS);
-  cfg.dynamicSmemBytes = RS_SMEM;
+  cfg.blockDim = dim3(Shape::threads);
+  cfg.dynamicSmemBytes = Shape::smem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -784,9 +790,9 @@ int run_shared(const void* q, int q_dtype, const SharedPlan& p, SharedArgs a, co
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  (void)cudaLaunchKernelEx(&cfg, kern, mq, mk, mv, a);
+  (void)cudaLaunchKernelEx(&cfg, kern, mq, mq8, mk, mv, a);
   XENCB_CHECK_LAUNCH("shared_read launch");
-  const dim3 grid((unsigned)n_rows, (unsigned)((a.d_s + 1023) / 1024));
+  const dim3 grid((unsigned)n_rows, (unsigned)((a.d_s + 127) / 128));
   switch (out_dtype) {
     case XENCB_F32: shared_combine_kernel<float><<<grid, 256, 0, st>>>(a, static_cast<float*>(r_out)); break;
     case XENCB_F16: shared_combine_kernel<__half><<<grid, 256, 0, st>>>(a, static_cast<__half*>(r_out)); break;
@@ -1584,15 +1590,17 @@ int xencb_read_shared(const void* q, int q_dtype, int64_t n_rows, int d_s, const
   a.part = reinterpret_cast<float*>(take(p.part));
   a.ml = reinterpret_cast<float2*>(take(p.ml));
   a.segs = p.segs; a.seg_rows = p.seg_rows; a.cs = p.cs; a.ns = p.ns; a.slab = p.slab;
+  a.tmem_cols = p.tmem_cols;
   a.softmax = read_softmax ? 1 : 0;
   a.qscale = read_softmax ? read_temp * 1.4426950408889634f : 1.f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (slots_dtype == XENCB_F16)
-    return p.terms == 2 ? run_shared<__half, 2>(q, q_dtype, p, a, slots, vslots, q16, n_rows, r_out, out_dtype, di.sms, st)
-                        : run_shared<__half, 1>(q, q_dtype, p, a, slots, vslots, q16, n_rows, r_out, out_dtype, di.sms, st);
-  return p.terms == 2
-             ? run_shared<__nv_bfloat16, 2>(q, q_dtype, p, a, slots, vslots, q16, n_rows, r_out, out_dtype, di.sms, st)
-             : run_shared<__nv_bfloat16, 1>(q, q_dtype, p, a, slots, vslots, q16, n_rows, r_out, out_dtype, di.sms, st);
+  auto run = [&](auto t) {
+    using T = decltype(t);
+    auto go = [&](auto kern) { return kern(q, q_dtype, p, a, slots, vslots, q16, n_rows, r_out, out_dtype, di.sms, st); };
+    if (p.arows == 32) return p.terms == 2 ? go(run_shared<T, 2, 32>) : go(run_shared<T, 1, 32>);
+    return p.terms == 2 ? go(run_shared<T, 2, 64>) : go(run_shared<T, 1, 64>);
+  };
+  return slots_dtype == XENCB_F16 ? run(__half{}) : run(__nv_bfloat16{});
 }
 
 // ------------------------------------------------------------------------------------------------ project_out
