@@ -104,6 +104,7 @@ __device__ __forceinline__ uint32_t pg_word_mask(int i, int n_pages) {
 __global__ void __launch_bounds__(PG_THREADS) pages_fork_plan_kernel(const PagePlanArgs a) {
   extern __shared__ uint32_t pg_bits[];
   __shared__ int sh[32];
+  pdl_trigger();  // (the copy kernel waits for this grid before it reads the list)
   const int n_words = (a.n_pages + 31) / 32;
   pg_mark_live(a, pg_bits, n_words, false);
   // entries that need a fresh page, in (child, chunk) order: each thread owns a contiguous range
@@ -166,6 +167,7 @@ __global__ void __launch_bounds__(PG_THREADS) pages_fork_plan_kernel(const PageP
 __global__ void __launch_bounds__(PG_THREADS) pages_compact_plan_kernel(const PagePlanArgs a) {
   extern __shared__ uint32_t pg_bits[];
   __shared__ int sh[32];
+  pdl_trigger();  // (the copy kernel waits for this grid before it reads the list)
   const int n_words = (a.n_pages + 31) / 32;
   pg_mark_live(a, pg_bits, n_words, true);
   const int wper = (n_words + PG_THREADS - 1) / PG_THREADS;
@@ -221,34 +223,51 @@ __global__ void __launch_bounds__(PG_THREADS) pages_compact_plan_kernel(const Pa
 struct PagePools {
   char* base[PG_POOLS];
   int64_t row_bytes[PG_POOLS];
-  int n;
+  int first[PG_POOLS + 1];  // first slice of each pool's page in a move's list of slices
+  int slices;
   int page_rows;
 };
 
 // Copies the listed pages in every pool: the first `rows` rows of page src, then zeros to the end of the page. V is
 // the unit of the accesses: 16 bytes where every pool's pages are 16-byte aligned, else 2 bytes (every slot type has
-// at least two).
+// at least two). A work item is a slice of one page of one pool, PG_UNROLL units a thread with every load in flight
+// before the first store; the pages are read and written once, so both bypass L1.
+constexpr int PG_COPY_THREADS = 256;
+constexpr int PG_UNROLL = 8;
+
+template <typename V> __device__ __forceinline__ V pg_zero();
+template <> __device__ __forceinline__ uint4 pg_zero<uint4>() { return make_uint4(0u, 0u, 0u, 0u); }
+template <> __device__ __forceinline__ uint16_t pg_zero<uint16_t>() { return 0; }
+
 template <typename V>
-__global__ void __launch_bounds__(256) pages_copy_kernel(const PagePools pools, const PageMove* __restrict__ moves,
-                                                         const int* __restrict__ n_moves) {
-  const int n = *n_moves;
-  for (int64_t w = blockIdx.x; w < (int64_t)n * pools.n; w += gridDim.x) {
-    const PageMove mv = moves[w / pools.n];
-    const int k = (int)(w % pools.n);
+__global__ void __launch_bounds__(PG_COPY_THREADS) pages_copy_kernel(const PagePools pools,
+                                                                     const PageMove* __restrict__ moves,
+                                                                     const int* __restrict__ n_moves) {
+  constexpr int SLICE = PG_COPY_THREADS * PG_UNROLL * (int)sizeof(V);
+  pdl_wait();
+  const int64_t n = (int64_t)*n_moves * pools.slices;
+  for (int64_t w = blockIdx.x; w < n; w += gridDim.x) {
+    const PageMove mv = moves[w / pools.slices];
+    int sl = (int)(w % pools.slices), k = 0;
+    while (sl >= pools.first[k + 1]) ++k;
+    sl -= pools.first[k];
     const int64_t page_bytes = pools.row_bytes[k] * pools.page_rows;
     const int64_t keep = pools.row_bytes[k] * mv.rows;
     const char* src = pools.base[k] + mv.src * page_bytes;
     char* dst = pools.base[k] + mv.dst * page_bytes;
-    for (int64_t i = (int64_t)threadIdx.x * sizeof(V); i < page_bytes; i += blockDim.x * sizeof(V)) {
-      V v{};
-      if (i + (int64_t)sizeof(V) <= keep) {
-        v = *reinterpret_cast<const V*>(src + i);
-      } else if (i < keep) {  // the unit that holds the last valid bytes
-        v = *reinterpret_cast<const V*>(src + i);
-        for (int b = 0; b < (int)sizeof(V); ++b)
-          if (i + b >= keep) reinterpret_cast<char*>(&v)[b] = 0;
-      }
-      *reinterpret_cast<V*>(dst + i) = v;
+    const int64_t at = (int64_t)sl * SLICE + threadIdx.x * sizeof(V);
+    V v[PG_UNROLL];
+#pragma unroll
+    for (int i = 0; i < PG_UNROLL; ++i) {
+      const int64_t o = at + (int64_t)i * PG_COPY_THREADS * sizeof(V);
+      v[i] = o < keep ? __ldcs(reinterpret_cast<const V*>(src + o)) : pg_zero<V>();
+    }
+#pragma unroll
+    for (int i = 0; i < PG_UNROLL; ++i) {
+      const int64_t o = at + (int64_t)i * PG_COPY_THREADS * sizeof(V);
+      if (o < keep && o + (int64_t)sizeof(V) > keep)  // the unit that holds the last valid bytes
+        for (int b = (int)(keep - o); b < (int)sizeof(V); ++b) reinterpret_cast<char*>(&v[i])[b] = 0;
+      if (o < page_bytes) __stcs(reinterpret_cast<V*>(dst + o), v[i]);
     }
   }
 }

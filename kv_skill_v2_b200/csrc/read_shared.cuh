@@ -35,31 +35,25 @@
 
 namespace xencb {
 
-constexpr int RS_MAX_CS = 8;      // CTAs per cluster: 4 or 8
+constexpr int RS_AROWS = 64;      // rows of the A operands that carry data (TERMS * MT; the MMA's M is 128 whatever they
+                                  // are, and the other rows are not looked at)
+constexpr int RS_CS = 8;          // CTAs per cluster
+constexpr int RS_NS = 64;         // slots whose scores a CTA computes
+constexpr int RS_SEG = RS_CS * RS_NS;  // slots of a unit
+constexpr int RS_HW = RS_NS / 2;  // score columns of a softmax warp
 constexpr int RS_SLAB = 512;      // columns of d_s per CTA at most (TMEM)
+constexpr int RS_AHEAD_SLAB = 256;  // up to here the scores have TMEM columns of their own
 constexpr int RS_VROWS = 32;      // slots per stage of the read product
-constexpr int RS_ACC = 4;         // score accumulators in TMEM (ns columns each)
+constexpr int RS_ACC = 4;         // score accumulators in TMEM
 constexpr int RS_CHUNK = 2;       // TERMS = 2: k-blocks per accumulator (8 accumulation steps)
-constexpr float RS_P_SCALE = 16384.f;         // P is scaled by 2^14
-
-// The kernel's shapes. AROWS: rows of the A operands that carry data (TERMS * MT pairs; the MMA's M is 128 whatever
-// they are, the other rows are not looked at).
-//   32: clusters of 8, two CTAs per SM (256 TMEM columns each): one unit's softmax and epilogue run under the other's
-//       loads. For pages that few rows read: the tile of Q is small beside the page's.
-//   64: one CTA per SM with a deeper ring: each page is fetched for twice the pairs.
-template <int AROWS>
-struct RsShape {
-  static constexpr int quarters = AROWS / 32;               // TMEM lane quarters that carry data
-  static constexpr int stage = AROWS == 32 ? 16384 : 24576;  // scores: A tile + B tile; read: 4 boxes of 32 x 64
-  static constexpr int stages = AROWS == 32 ? 4 : 6;
-  static constexpr int pblk = AROWS * 128;                  // P of 64 slots: one 128-byte swizzle row per A row
-  static constexpr int producer = quarters, mma = quarters + 1;  // warps; 0..quarters-1 and 4.. do the softmax
-  static constexpr int threads = 32 * (4 + quarters);
-  static constexpr int ctas = AROWS == 32 ? 2 : 1;          // per SM
-  static constexpr int stat_floats = 2 * 2 * RS_MAX_CS * AROWS;  // [2][2 * cs][MT]
-  static constexpr size_t smem =
-      1024 + 8 * pblk + (size_t)stages * stage + 2 * stat_floats * 4 + (2 * stages + 2 * RS_ACC + 5) * 8 + 16;
-};
+constexpr float RS_P_SCALE = 16384.f;     // P is scaled by 2^14
+constexpr int RS_STAGE = 16384;   // scores: 64 rows of Q + 64 slots of K; read: 4 boxes of 32 slots x 64 columns
+constexpr int RS_STAGES = 9;
+constexpr int RS_PBLK = RS_AROWS * 128;   // P of 64 slots: one 128-byte swizzle row per A row
+constexpr int RS_STAT = 2 * 2 * RS_CS * RS_AROWS;  // floats: [2][16][MT]
+constexpr int RS_THREADS = 192;   // warps 0, 1, 4, 5: softmax and epilogue (TMEM lanes 0-63); 2: producer; 3: MMA
+constexpr size_t RS_SMEM = 1024 + 8 * RS_PBLK + (size_t)RS_STAGES * RS_STAGE + 2 * RS_STAT * 4 +
+                           (2 * RS_STAGES + 2 * RS_ACC + 5) * 8 + 16;
 
 struct __align__(16) SharedTile {
   int page, start, count, nv;  // pairs [start, start + count) in grouped order; nv: the page's most valid slots
@@ -84,7 +78,9 @@ struct SharedArgs {
   int* pnv;        // [n_pairs] by position: valid slots
   float* qinv;     // [n_pairs] by position: 1 / (the row's power-of-two scale)
   // read
-  int segs, seg_rows, cs, ns, slab, tmem_cols;
+  int segs, slab;
+  int ahead;       // the next unit's scores run before this unit's read (slab <= RS_AHEAD_SLAB)
+  int v3d;         // V's map is 3-D: [64 columns][slots][blocks of 64 columns] (d_s a multiple of 64)
   float qscale;    // read_temp * log2(e), or 1
   int softmax;
   float* part;     // [n_pairs][segs][d_s], normalised per segment
@@ -178,26 +174,29 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const SharedArgs a, i
   rs_scan(a, mt);
 }
 
-// Each pair's q row in 16 bits at the pair's grouped position: hi terms [n_pairs, d_s], then (TERMS = 2) lo terms.
+// Each pair's q row in 16 bits at the pair's grouped position: hi terms [n_pairs, d_s], then (TERMS = 2) lo terms. One
+// CTA per row and up to 8 of its routed chunks; the row stays in registers (d_s <= 4096: two pieces of 8 a thread).
+constexpr int RS_SPLIT_THREADS = 256;
 template <typename TQ, typename T, int TERMS>
-__global__ void __launch_bounds__(256) shared_split_kernel(const TQ* __restrict__ q, const SharedArgs a,
-                                                           T* __restrict__ out) {
+__global__ void __launch_bounds__(RS_SPLIT_THREADS) shared_split_kernel(const TQ* __restrict__ q, const SharedArgs a,
+                                                                        T* __restrict__ out) {
   __shared__ float red[8];
-  const int64_t pair = blockIdx.x;
-  const int page = a.page[pair];
-  if (page < 0) return;
-  const int64_t row = pair / a.k;
-  const int pos = a.cnt[page] + a.rank[pair];
+  const int64_t row = blockIdx.x;
   const TQ* src = q + row * a.d_s;
-  float s = 1.f;
-  if (sizeof(T) == 2 && std::is_same<T, __half>::value) {  // f16's range: the row's largest value to [2^14, 2^15)
-    float mx = 0.f;
-    for (int i = threadIdx.x * 8; i < a.d_s; i += 256 * 8) {
-      float v[8];
-      load8_f32<TQ>(src + i, v);
+  float v[2][8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(v[e]));
-    }
+  for (int p = 0; p < 2; ++p) {
+    const int i = (p * RS_SPLIT_THREADS + threadIdx.x) * 8;
+    if (i < a.d_s) load8_f32<TQ>(src + i, v[p]);
+  }
+  float s = 1.f;
+  if (std::is_same<T, __half>::value) {  // f16's range: the row's largest value to [2^14, 2^15)
+    float mx = 0.f;
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+      if ((p * RS_SPLIT_THREADS + threadIdx.x) * 8 < a.d_s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(v[p][e]));
     mx = warp_max(mx);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = mx;
     __syncthreads();
@@ -206,27 +205,47 @@ __global__ void __launch_bounds__(256) shared_split_kernel(const TQ* __restrict_
     for (int w = 1; w < 8; ++w) mx = fmaxf(mx, red[w]);
     s = f16_range_scale(mx);
   }
-  for (int i = threadIdx.x * 8; i < a.d_s; i += 256 * 8) {
-    float v[8];
-    load8_f32<TQ>(src + i, v);
-    alignas(16) T hi[8], lo[8];
+  alignas(16) T hi[2][8], lo[2][8];
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      hi[e] = from_f32<T>(v[e] * s);
-      lo[e] = from_f32<T>(v[e] * s - to_f32(hi[e]));
+      hi[p][e] = from_f32<T>(v[p][e] * s);
+      if (TERMS == 2) lo[p][e] = from_f32<T>(v[p][e] * s - to_f32(hi[p][e]));
     }
-    *reinterpret_cast<uint4*>(out + (int64_t)pos * a.d_s + i) = *reinterpret_cast<const uint4*>(hi);
-    if (TERMS == 2)
-      *reinterpret_cast<uint4*>(out + ((int64_t)a.n_pairs + pos) * a.d_s + i) = *reinterpret_cast<const uint4*>(lo);
-  }
-  if (threadIdx.x == 0) {
-    const int64_t lib = row / a.rows_per_lib;
-    a.pnv[pos] = min(a.n_valid[lib * a.C + a.idx[pair]], a.page_rows);
-    a.qinv[pos] = 1.f / s;
+  const int64_t lib = row / a.rows_per_lib;
+  const int j1 = min(a.k, (int)(blockIdx.y + 1) * 8);
+  for (int j = blockIdx.y * 8; j < j1; ++j) {
+    const int64_t pair = row * a.k + j;
+    const int page = a.page[pair];
+    if (page < 0) continue;
+    const int pos = a.cnt[page] + a.rank[pair];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int i = (p * RS_SPLIT_THREADS + threadIdx.x) * 8;
+      if (i >= a.d_s) continue;
+      *reinterpret_cast<uint4*>(out + (int64_t)pos * a.d_s + i) = *reinterpret_cast<const uint4*>(hi[p]);
+      if (TERMS == 2)
+        *reinterpret_cast<uint4*>(out + ((int64_t)a.n_pairs + pos) * a.d_s + i) =
+            *reinterpret_cast<const uint4*>(lo[p]);
+    }
+    if (threadIdx.x == 0) {
+      a.pnv[pos] = min(a.n_valid[lib * a.C + a.idx[pair]], a.page_rows);
+      a.qinv[pos] = 1.f / s;
+    }
   }
 }
 
 // ----------------------------------------------------------------------------------------------------- cluster PTX
+// 3-D tiled TMA load (no multicast): the innermost coordinate must be 16-byte aligned.
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
 // True in one thread of a converged warp. The compiler issues TMA and MMA instructions of an elected thread from
 // uniform registers; under `lane == 0` each cost about 150 cycles to issue, which bound the kernel (one stage of three
 // copies 770 cycles, whatever its bytes).
@@ -311,17 +330,15 @@ struct RsRing {
   }
 };
 
-template <int AROWS>
 __device__ __forceinline__ RsSmem rs_smem(unsigned char* base) {
-  using C = RsShape<AROWS>;
   RsSmem s;
   s.p = base;
-  s.stages = base + 8 * C::pblk;
-  s.smax = reinterpret_cast<float*>(s.stages + C::stages * C::stage);
-  s.ssum = s.smax + C::stat_floats;
-  s.full = reinterpret_cast<uint64_t*>(s.ssum + C::stat_floats);
-  s.empty = s.full + C::stages;
-  s.s_full = s.empty + C::stages;
+  s.stages = base + 8 * RS_PBLK;
+  s.smax = reinterpret_cast<float*>(s.stages + RS_STAGES * RS_STAGE);
+  s.ssum = s.smax + RS_STAT;
+  s.full = reinterpret_cast<uint64_t*>(s.ssum + RS_STAT);
+  s.empty = s.full + RS_STAGES;
+  s.s_full = s.empty + RS_STAGES;
   s.s_empty = s.s_full + RS_ACC;
   s.p_full = s.s_empty + RS_ACC;
   s.o_full = s.p_full + 1;
@@ -333,36 +350,48 @@ __device__ __forceinline__ RsSmem rs_smem(unsigned char* base) {
   return s;
 }
 
-template <typename T, int TERMS, int AROWS>
-__global__ void __launch_bounds__(RsShape<AROWS>::threads, RsShape<AROWS>::ctas)
+// A unit of this cluster: a tile and one segment of its page. Every warp walks the same list.
+struct RsUnit {
+  int u;  // >= n_units: none
+  SharedTile t;
+  int seg0, nv;  // first slot, valid slots (of the pair with most) in the segment
+  __device__ __forceinline__ void find(const SharedArgs& a, int first, int n_units, int step) {
+    for (u = first; u < n_units; u += step) {
+      t = a.tiles[u / a.segs];
+      seg0 = (u % a.segs) * RS_SEG;
+      nv = min(t.nv - seg0, RS_SEG);
+      if (nv > 0) return;
+    }
+  }
+};
+
+template <typename T, int TERMS>
+__global__ void __launch_bounds__(RS_THREADS, 1)
     shared_read_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_q8,
                        const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        const SharedArgs a) {
-  using C = RsShape<AROWS>;
-  constexpr int MT = AROWS / TERMS;                 // pairs per tile
+  constexpr int MT = RS_AROWS / TERMS;                // pairs per tile
   constexpr int FMT = std::is_same<T, __half>::value ? UMMA_F16 : UMMA_BF16;
-  constexpr bool SAME = AROWS == 32 && TERMS == 2;  // a pair's hi and lo rows are lanes i and i + 16 of one warp
-  constexpr int CQ = SAME ? 1 : C::quarters / TERMS;  // quarters of the hi terms
-  constexpr int CW = 2 * CQ, AW = 2 * C::quarters;    // warps that do the softmax (two column halves); that read TMEM
+  constexpr int CQ = 2 / TERMS;                       // TMEM lane quarters of the hi terms
+  constexpr int CW = 2 * CQ, AW = 4;                  // warps that do the softmax; that read TMEM
   extern __shared__ unsigned char rs_smem_raw[];
-  const RsSmem s = rs_smem<AROWS>(reinterpret_cast<unsigned char*>(
-      (reinterpret_cast<uintptr_t>(rs_smem_raw) + 1023) & ~uintptr_t(1023)));
+  const RsSmem s = rs_smem(reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(rs_smem_raw) + 1023) &
+                                                            ~uintptr_t(1023)));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int cs = a.cs, ns = a.ns;
   const int rank = (int)cluster_rank();
-  const int cluster = blockIdx.x / cs, n_clusters = gridDim.x / cs;
+  const int cluster = blockIdx.x / RS_CS, n_clusters = gridDim.x / RS_CS;
   const int nkb = (a.d_s + 63) / 64;
   const int kpc = TERMS == 2 ? RS_CHUNK : nkb;                     // k-blocks per score accumulator
   const int x0 = rank * a.slab;                                    // this CTA's columns of d_s
   const int my_boxes = max(0, min(a.slab, a.d_s - x0) + 63) / 64;  // in boxes of 64
-  const uint32_t blk_bytes = (uint32_t)(ns / 64) * C::pblk;        // this CTA's share of P
+  const uint32_t s_col = a.ahead ? RS_AHEAD_SLAB : 0;              // TMEM columns of the scores
 
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_q);
     prefetch_tensormap(&map_q8);
     prefetch_tensormap(&map_k);
     prefetch_tensormap(&map_v);
-    for (int i = 0; i < C::stages; ++i) {
+    for (int i = 0; i < RS_STAGES; ++i) {
       mbar_init(&s.full[i], 1);
       mbar_init(&s.empty[i], 1);
     }
@@ -373,13 +402,13 @@ __global__ void __launch_bounds__(RsShape<AROWS>::threads, RsShape<AROWS>::ctas)
     mbar_init(s.p_full, 1);
     mbar_init(s.o_full, 1);
     mbar_init(s.o_empty, AW);
-    mbar_init(s.stat, cs * CW);
-    mbar_init(s.sums, cs * CW);
+    mbar_init(s.stat, RS_CS * CW);
+    mbar_init(s.sums, RS_CS * CW);
     *s.abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == C::mma) {
-    tc_alloc(s.tmem, (uint32_t)a.tmem_cols);
+  if (warp == 3) {
+    tc_alloc(s.tmem, 512);
     tc_relinquish();
   }
   tc_fence_before();
@@ -389,274 +418,271 @@ __global__ void __launch_bounds__(RsShape<AROWS>::threads, RsShape<AROWS>::ctas)
   const uint32_t taddr = *s.tmem;
   pdl_wait();
   const int n_units = *a.n_tiles * a.segs;
+  RsUnit cur, nxt;
+  cur.find(a, cluster, n_units, n_clusters);
 
-  if (warp == C::producer) {
+  if (warp == 2) {
     // --------------------------------------------------------------------------------------------- producer
     if (elect_one()) {
       RsRing ring{0, 0};
       uint32_t used = 0;
       bool ok = true;
-      for (int u = cluster; u < n_units && ok; u += n_clusters) {
-        const SharedTile t = a.tiles[u / a.segs];
-        const int seg0 = (u % a.segs) * a.seg_rows;
-        const int nv = min(t.nv - seg0, a.seg_rows);
-        if (nv <= 0) continue;
-        const int y0 = t.page * a.page_rows + seg0;
-        if (rank * ns < nv) {
-          const bool few = t.count <= 8;  // eight rows of Q a term; what lies in the others is not looked at
-          const uint32_t tx = (uint32_t)((few ? 8 : MT) * TERMS + ns) * 128;
-          for (int kb = 0; kb < nkb && ok; ++kb) {
-            if (used >= C::stages) ok = mbar_wait_bounded(&s.empty[ring.st], ring.phase ^ 1);
-            if (!ok) break;
-            uint64_t* bar = &s.full[ring.st];
-            unsigned char* st = s.stages + ring.st * C::stage;
-            mbar_arrive_expect_tx(bar, tx);
-            tma_load_2d(st + AROWS * 128, &map_k, kb * 64, y0 + rank * ns, bar);
-            if (few) {
+      auto scores = [&](const RsUnit& w) {
+        if (w.u >= n_units || rank * RS_NS >= w.nv) return;
+        const int y = w.t.page * a.page_rows + w.seg0 + rank * RS_NS;
+        const bool few = w.t.count <= 8;  // eight rows of Q a term; what lies in the others is not looked at
+        const uint32_t tx = (uint32_t)((few ? 8 : MT) * TERMS + RS_NS) * 128;
+        for (int kb = 0; kb < nkb && ok; ++kb) {
+          if (used >= RS_STAGES) ok = mbar_wait_spin(&s.empty[ring.st], ring.phase ^ 1);
+          if (!ok) break;
+          uint64_t* bar = &s.full[ring.st];
+          unsigned char* st = s.stages + ring.st * RS_STAGE;
+          mbar_arrive_expect_tx(bar, tx);
+          tma_load_2d(st + RS_AROWS * 128, &map_k, kb * 64, y, bar);
+          if (few) {
 #pragma unroll
-              for (int x = 0; x < TERMS; ++x)
-                tma_load_2d(st + x * MT * 128, &map_q8, kb * 64, x * a.n_pairs + t.start, bar);
-            } else {
-#pragma unroll
-              for (int x = 0; x < TERMS; ++x)
-                tma_load_2d(st + x * MT * 128, &map_q, kb * 64, x * a.n_pairs + t.start, bar);
-            }
-            ring.next(C::stages);
-            ++used;
+            for (int x = 0; x < TERMS; ++x)
+              tma_load_2d(st + x * MT * 128, &map_q8, kb * 64, x * a.n_pairs + w.t.start, bar);
+          } else {
+            tma_load_3d(st, &map_q, kb * 64, w.t.start, 0, bar);
           }
+          ring.next(RS_STAGES);
+          ++used;
         }
-        for (int b = 0; b < (nv + RS_VROWS - 1) / RS_VROWS && ok; ++b)
+      };
+      auto values = [&](const RsUnit& w) {
+        const int y = w.t.page * a.page_rows + w.seg0;
+        for (int b = 0; b < (w.nv + RS_VROWS - 1) / RS_VROWS && ok; ++b)
           for (int h = 0; h < my_boxes; h += 4) {
             const int n = min(4, my_boxes - h);
-            if (used >= C::stages) ok = mbar_wait_bounded(&s.empty[ring.st], ring.phase ^ 1);
+            if (used >= RS_STAGES) ok = mbar_wait_spin(&s.empty[ring.st], ring.phase ^ 1);
             if (!ok) break;
             uint64_t* bar = &s.full[ring.st];
-            unsigned char* st = s.stages + ring.st * C::stage;
-            mbar_arrive_expect_tx(bar, (uint32_t)n * RS_VROWS * 128);
-            for (int i = 0; i < n; ++i)
-              tma_load_2d(st + i * RS_VROWS * 128, &map_v, x0 + (h + i) * 64, y0 + b * RS_VROWS, bar);
-            ring.next(C::stages);
+            unsigned char* st = s.stages + ring.st * RS_STAGE;
+            mbar_arrive_expect_tx(bar, (uint32_t)(a.v3d ? 4 : n) * RS_VROWS * 128);
+            if (a.v3d)  // four boxes of 64 columns in one copy (those past d_s arrive as zeros)
+              tma_load_3d(st, &map_v, 0, y + b * RS_VROWS, (x0 >> 6) + h, bar);
+            else
+              for (int i = 0; i < n; ++i)
+                tma_load_2d(st + i * RS_VROWS * 128, &map_v, x0 + (h + i) * 64, y + b * RS_VROWS, bar);
+            ring.next(RS_STAGES);
             ++used;
           }
+      };
+      scores(cur);
+      while (cur.u < n_units && ok) {
+        nxt.find(a, cur.u + n_clusters, n_units, n_clusters);
+        if (a.ahead) scores(nxt);
+        values(cur);
+        if (!a.ahead) scores(nxt);
+        cur = nxt;
       }
       if (!ok) *s.abort_flag = 1;
       // the copies in flight end before the CTA's shared memory goes away
-      for (uint32_t i = min(used, (uint32_t)C::stages); i > 0; --i) {
-        ring.back(C::stages);
+      for (uint32_t i = min(used, (uint32_t)RS_STAGES); i > 0; --i) {
+        ring.back(RS_STAGES);
         mbar_wait_bounded(&s.full[ring.st], ring.phase);
       }
     }
     __syncwarp();
-  } else if (warp == C::mma) {
+  } else if (warp == 3) {
     // --------------------------------------------------------------------------------------------- MMA issuer
     if (elect_one()) {
       RsRing ring{0, 0};
       uint32_t unit = 0, acc = 0;
       bool ok = true;
-      const uint32_t id_s = umma_idesc(FMT, FMT, 128, ns);
+      const uint32_t id_s = umma_idesc(FMT, FMT, 128, RS_NS);
       // operand descriptors: the constant part, and addresses in 16-byte units (14 bits: the address of a CTA's shared
       // memory carries its cluster rank above them)
       const uint64_t dk = umma_desc_k_sw128(0), dv = umma_desc_mn_sw128(0, RS_VROWS * 128);
       const uint32_t st0 = (smem_u32(s.stages) >> 4) & 0x3FFFu, p0 = (smem_u32(s.p) >> 4) & 0x3FFFu;
-      for (int u = cluster; u < n_units; u += n_clusters) {
-        const SharedTile t = a.tiles[u / a.segs];
-        const int nv = min(t.nv - (u % a.segs) * a.seg_rows, a.seg_rows);
-        if (nv <= 0) continue;
-        if (unit > 0 && !(ok = mbar_wait_bounded(s.o_empty, (unit - 1) & 1))) break;
-        tc_fence_after();
-        if (rank * ns < nv) {
-          for (int k0 = 0; k0 < nkb && ok; k0 += kpc, ++acc) {
-            const uint32_t buf = acc % RS_ACC, use = acc / RS_ACC;
-            if (use > 0 && !(ok = mbar_wait_bounded(&s.s_empty[buf], (use - 1) & 1))) break;
+      auto scores = [&](const RsUnit& w) {
+        if (w.u >= n_units || rank * RS_NS >= w.nv) return;
+        for (int k0 = 0; k0 < nkb && ok; k0 += kpc, ++acc) {
+          const uint32_t buf = acc % RS_ACC, use = acc / RS_ACC;
+          if (use > 0 && !(ok = mbar_wait_spin(&s.s_empty[buf], (use - 1) & 1))) break;
+          tc_fence_after();
+          const int k1 = min(nkb, k0 + kpc);
+          for (int kb = k0; kb < k1; ++kb) {
+            if (!(ok = mbar_wait_spin(&s.full[ring.st], ring.phase))) break;
             tc_fence_after();
-            const int k1 = min(nkb, k0 + kpc);
-            for (int kb = k0; kb < k1; ++kb) {
-              if (!(ok = mbar_wait_bounded(&s.full[ring.st], ring.phase))) break;
-              tc_fence_after();
-              const uint64_t da = dk + (st0 + ring.st * (C::stage / 16)), db = da + AROWS * 8;
+            const uint64_t da = dk + (st0 + ring.st * (RS_STAGE / 16)), db = da + RS_AROWS * 8;
 #pragma unroll
-              for (int ks = 0; ks < 4; ++ks)
-                tc_mma<0>(taddr + buf * (uint32_t)ns, da + ks * 2, db + ks * 2, id_s, kb > k0 || ks > 0);
-              tc_commit(&s.empty[ring.st]);
-              ring.next(C::stages);
-            }
-            if (!ok) break;
-            tc_commit(&s.s_full[buf]);
+            for (int ks = 0; ks < 4; ++ks)
+              tc_mma<0>(taddr + s_col + buf * RS_NS, da + ks * 2, db + ks * 2, id_s, kb > k0 || ks > 0);
+            tc_commit(&s.empty[ring.st]);
+            ring.next(RS_STAGES);
           }
           if (!ok) break;
+          tc_commit(&s.s_full[buf]);
         }
+      };
+      auto values = [&](const RsUnit& w) {
         // every CTA's block of P is here (and this CTA's softmax warps have read the scores)
-        if (!(ok = mbar_wait_cluster(s.p_full, unit & 1))) break;
+        if (!(ok = ok && mbar_wait_cluster(s.p_full, unit & 1))) return;
         tc_fence_after();
-        for (int b = 0; b < (nv + RS_VROWS - 1) / RS_VROWS && ok; ++b) {
-          const int left = nv - b * RS_VROWS, steps = min(RS_VROWS / 16, (left + 15) / 16);
+        for (int b = 0; b < (w.nv + RS_VROWS - 1) / RS_VROWS && ok; ++b) {
+          const int left = w.nv - b * RS_VROWS, steps = min(RS_VROWS / 16, (left + 15) / 16);
           // slots [b * 32, b * 32 + 32) of P: half a block of 64
-          const uint64_t dp = dk + (p0 + (b / 2) * (C::pblk / 16) + (b & 1) * 4);
+          const uint64_t dp = dk + (p0 + (b / 2) * (RS_PBLK / 16) + (b & 1) * 4);
           for (int h = 0; h < my_boxes; h += 4) {
             const int n = min(4, my_boxes - h);
-            if (!(ok = mbar_wait_bounded(&s.full[ring.st], ring.phase))) break;
+            if (!(ok = mbar_wait_spin(&s.full[ring.st], ring.phase))) break;
             tc_fence_after();
             if (left < steps * 16) {  // rows of V behind the last valid slot: zeros (0 * NaN would not be 0)
-              unsigned char* base = s.stages + ring.st * C::stage;
+              unsigned char* base = s.stages + ring.st * RS_STAGE;
               for (int i = 0; i < n; ++i)
                 for (int c = left * 8; c < steps * 16 * 8; ++c)
                   *reinterpret_cast<uint4*>(base + i * RS_VROWS * 128 + c * 16) = make_uint4(0, 0, 0, 0);
               fence_proxy_async_smem();
             }
-            const uint64_t dx = dv + (st0 + ring.st * (C::stage / 16));
+            const uint64_t dx = dv + (st0 + ring.st * (RS_STAGE / 16));
             const uint32_t id = umma_idesc(FMT, FMT, 128, n * 64, 1);
             for (int ks = 0; ks < steps; ++ks)
               tc_mma<0>(taddr + (uint32_t)h * 64, dp + ks * 2, dx + ks * 128, id, b > 0 || ks > 0);
             tc_commit(&s.empty[ring.st]);
-            ring.next(C::stages);
+            ring.next(RS_STAGES);
           }
         }
-        if (!ok) break;
-        tc_commit(s.o_full);
+        if (ok) tc_commit(s.o_full);
         ++unit;
+      };
+      // the epilogue of the unit before has read its sums: they may be overwritten, by the read or (where they share
+      // columns) by the scores
+      auto drained = [&](uint32_t units) {
+        if (units > 0 && ok) ok = mbar_wait_spin(s.o_empty, (units - 1) & 1);
+        tc_fence_after();
+      };
+      scores(cur);
+      while (cur.u < n_units && ok) {
+        nxt.find(a, cur.u + n_clusters, n_units, n_clusters);
+        if (a.ahead) {
+          scores(nxt);
+          drained(unit);
+          if (ok) values(cur);
+        } else {
+          values(cur);
+          if (nxt.u < n_units) drained(unit);
+          if (ok) scores(nxt);
+        }
+        cur = nxt;
       }
       if (!ok) *s.abort_flag = 1;
     }
     __syncwarp();
-  } else if ((warp & 3) < C::quarters) {
+  } else {
     // --------------------------------------------------------------------------------------------- softmax, epilogue
     const int quarter = warp & 3, half = warp >> 2;
-    const int term = SAME ? lane >> 4 : quarter / CQ;                        // 0: hi rows
-    const int row = SAME ? lane & 15 : (quarter % CQ) * 32 + lane;           // pair of the tile
-    const bool does = SAME || term == 0;                                     // this warp does the softmax
+    const int term = quarter / CQ;                                           // 0: hi rows, which do the softmax
+    const int row = (quarter % CQ) * 32 + lane;                              // pair of the tile
     const uint32_t tl = taddr + ((uint32_t)(quarter * 32) << 16);
-    const int hw = ns / 2;                                                   // score columns of this warp
-    const int pair_bar = 2 + half * CQ + quarter % CQ;                       // a hi warp and its lo warp
-    // scratch of the lo -> hi hand-over: the block of P that belongs to another CTA (no copy reads it, and none
-    // arrives before this CTA's maxima of the unit are out): [columns][rows of a pair of warps]
-    float* xch = reinterpret_cast<float*>(s.p + (size_t)((rank + 1 + half) % cs) * blk_bytes) + (quarter % CQ) * 32 * ns;
+    const int pair_bar = 2 + half;                                           // TERMS = 2: a hi warp and its lo warp
+    const int c0 = rank * RS_NS + half * RS_HW;                              // first slot of this warp's columns
+    // scratch of the lo -> hi hand-over, [32 columns][32 rows] twice: the block of P that belongs to another CTA (no
+    // copy reads it, and none arrives before this CTA's maxima of the unit are out)
+    float* xch = reinterpret_cast<float*>(s.p + (size_t)((rank + 1 + half) % RS_CS) * RS_PBLK);
     uint32_t unit = 0, acc = 0;
     // A wait that runs out sets the abort flag; from then on nothing is waited for, and the warps run through their
     // units on whatever is there, so that the named barriers they share stay matched.
     auto done = [&](bool arrived) {
       if (!arrived) *s.abort_flag = 1;
     };
-    for (int u = cluster; u < n_units; u += n_clusters) {
-      const SharedTile t = a.tiles[u / a.segs];
-      const int seg = u % a.segs, seg0 = seg * a.seg_rows;
-      const int nv = min(t.nv - seg0, a.seg_rows);
-      if (nv <= 0) continue;
-      const bool mine = rank * ns < nv;
-      float* smax = s.smax + (unit & 1) * 2 * cs * MT;
-      float* ssum = s.ssum + (unit & 1) * 16 * MT;
+    float v[RS_HW];
+    auto scores = [&](const RsUnit& w) {  // this warp's 32 columns of the scores, added up over the accumulators
+      if (w.u >= n_units || rank * RS_NS >= w.nv) return;
+      for (int k0 = 0; k0 < nkb; k0 += kpc, ++acc) {
+        const uint32_t buf = acc % RS_ACC;
+        done(*s.abort_flag || mbar_wait_spin(&s.s_full[buf], (acc / RS_ACC) & 1));
+        tc_fence_after();
+        float x[RS_HW];
+        tc_ld32(tl + s_col + buf * RS_NS + (uint32_t)(half * RS_HW), x);
+#pragma unroll
+        for (int i = 0; i < RS_HW; ++i) v[i] = k0 == 0 ? x[i] : v[i] + x[i];
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.s_empty[buf]);
+      }
+    };
+    scores(cur);
+    while (cur.u < n_units) {
+      nxt.find(a, cur.u + n_clusters, n_units, n_clusters);
+      const SharedTile t = cur.t;
+      const int seg = cur.u % a.segs, seg0 = cur.seg0, nv = cur.nv;
+      const bool mine = rank * RS_NS < nv;
+      float* smax = s.smax + (unit & 1) * 2 * RS_CS * MT;
+      float* ssum = s.ssum + (unit & 1) * 2 * RS_CS * MT;
       const bool live = row < t.count;
       const int pos = t.start + (live ? row : 0);
       const int pnv = live ? a.pnv[pos] - seg0 : 0;            // the pair's valid slots in this segment
-      const float c = live ? a.qinv[pos] * a.qscale : 0.f;
-      const int c0 = rank * ns + half * hw;                    // first slot of this warp's columns
-      float v[64];
-      float mx = a.softmax ? -CUDART_INF_F : 0.f;
-      if (mine) {
-        for (int k0 = 0; k0 < nkb; k0 += kpc, ++acc) {
-          const uint32_t buf = acc % RS_ACC;
-          done(*s.abort_flag || mbar_wait_bounded(&s.s_full[buf], (acc / RS_ACC) & 1));
-          tc_fence_after();
-          const uint32_t at = tl + buf * (uint32_t)ns + (uint32_t)(half * hw);
-          float x[64];
-          if (hw == 64) {
-            tc_ld64(at, x);
-          } else {
-            tc_ld32(at, x);
+      if (TERMS == 2 && mine) {
+        if (term == 1)
 #pragma unroll
-            for (int i = 32; i < 64; ++i) x[i] = 0.f;
-          }
+          for (int i = 0; i < RS_HW; ++i) xch[i * 32 + lane] = v[i];
+        fence_proxy_async_smem();  // before another CTA's copy may land on the scratch
+        named_bar_sync(pair_bar, 64);
+        if (term == 0)
 #pragma unroll
-          for (int i = 0; i < 64; ++i) v[i] = k0 == 0 ? x[i] : v[i] + x[i];
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s.s_empty[buf]);
-        }
-        if (SAME) {
-#pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (i < hw) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 16);
-        } else if (TERMS == 2) {
-          if (term == 1)
-#pragma unroll
-            for (int i = 0; i < 64; ++i)
-              if (i < hw) xch[i * 32 + lane] = v[i];
-          fence_proxy_async_smem();  // before another CTA's copy may land on the scratch
-          tc_fence_before();         // before the read product may overwrite the scores
-          named_bar_sync(pair_bar, 64);
-          if (term == 0)
-#pragma unroll
-            for (int i = 0; i < 64; ++i)
-              if (i < hw) v[i] += xch[i * 32 + lane];
-        }
+          for (int i = 0; i < RS_HW; ++i) v[i] += xch[i * 32 + lane];
       }
-      if (does) {
+      if (term == 0) {
         // t = scores * scale; masked slots -inf (softmax) or 0 (linear read). A row whose every score is masked gets
         // max -inf and then NaN weights: it has no slot in this segment, so nothing reads them.
-        const int lim = min(pnv - c0, hw);
+        const float c = live ? a.qinv[pos] * a.qscale : 0.f;
+        const int lim = pnv - c0;
+        float mx = a.softmax ? -CUDART_INF_F : 0.f;
         if (mine && a.softmax) {
 #pragma unroll
-          for (int i = 0; i < 64; ++i) {
+          for (int i = 0; i < RS_HW; ++i) {
             v[i] = i < lim ? v[i] * c : -CUDART_INF_F;
             mx = fmaxf(mx, v[i]);
           }
         } else if (mine) {
 #pragma unroll
-          for (int i = 0; i < 64; ++i) {
+          for (int i = 0; i < RS_HW; ++i) {
             v[i] = i < lim ? v[i] * c : 0.f;
             mx = fmaxf(mx, fabsf(v[i]));
           }
         }
         // the rows' maxima to every CTA of the cluster
-        if (!SAME || lane < 16)
-          for (int r = 0; r < cs; ++r) st_cluster_f32(cluster_map(&smax[(rank * 2 + half) * MT + row], r), mx);
+#pragma unroll
+        for (int r = 0; r < RS_CS; ++r) st_cluster_f32(cluster_map(&smax[(rank * 2 + half) * MT + row], r), mx);
         __syncwarp();
-        if (lane < cs) mbar_arrive_cluster(cluster_map(s.stat, lane));
+        if (lane < RS_CS) mbar_arrive_cluster(cluster_map(s.stat, lane));
         done(*s.abort_flag || mbar_wait_cluster(s.stat, unit & 1));
         float m = a.softmax ? -CUDART_INF_F : 0.f;
-        for (int r = 0; r < 2 * cs; ++r) m = fmaxf(m, smax[r * MT + row]);
-        float l[2] = {0.f, 0.f};  // sums of 32 columns each, whatever the shape: it changes no bit of a result
+#pragma unroll
+        for (int r = 0; r < 2 * RS_CS; ++r) m = fmaxf(m, smax[r * MT + row]);
+        float l = 0.f;
         if (mine) {
           if (a.softmax) {
+            float l4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              float l4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-              for (int i = g * 32; i < g * 32 + 32; ++i) {
-                v[i] = RS_P_SCALE * pf_exp2(v[i] - m);
-                l4[i & 3] += v[i];
-              }
-              l[g] = (l4[0] + l4[1]) + (l4[2] + l4[3]);
+            for (int i = 0; i < RS_HW; ++i) {
+              v[i] = RS_P_SCALE * pf_exp2(v[i] - m);
+              l4[i & 3] += v[i];
             }
+            l = (l4[0] + l4[1]) + (l4[2] + l4[3]);
           } else {
             const float lin = f16_range_scale(m);
 #pragma unroll
-            for (int i = 0; i < 64; ++i) v[i] *= lin;
+            for (int i = 0; i < RS_HW; ++i) v[i] *= lin;
           }
-          // this row's P in 16 bits: block (c0 / 64), 16-byte chunk j of A row r at chunk j ^ (r % 8)
-          unsigned char* blk = s.p + (size_t)(c0 >> 6) * C::pblk;
-          const int j0 = (c0 & 63) >> 3;
+          // this row's P in 16 bits: this CTA's block, 16-byte chunk j of A row r at chunk j ^ (r % 8)
+          unsigned char* blk = s.p + (size_t)rank * RS_PBLK;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (j * 8 < hw) {
-              uint32_t hi[4], lo[4];
+          for (int j = 0; j < RS_HW / 8; ++j) {
+            uint32_t hi[4], lo[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float x = v[j * 8 + 2 * e], y = v[j * 8 + 2 * e + 1];
-                float2 r, r2;
-                hi[e] = rs_pack(T{}, x, y, r);
-                if (TERMS == 2) lo[e] = rs_pack(T{}, x - r.x, y - r.y, r2);
-              }
-              const int ch = (j0 + j) ^ (row & 7);  // (MT is a multiple of 8: the same for the lo row)
-              const uint4 h4 = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-              if (SAME) {  // lanes 0-15 hold the hi rows, 16-31 the lo rows of the same pairs
-                const uint4 l4 = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                *reinterpret_cast<uint4*>(blk + lane * 128 + ch * 16) = term ? l4 : h4;
-              } else {
-                *reinterpret_cast<uint4*>(blk + row * 128 + ch * 16) = h4;
-                if (TERMS == 2)
-                  *reinterpret_cast<uint4*>(blk + (MT + row) * 128 + ch * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-              }
+            for (int e = 0; e < 4; ++e) {
+              const float x = v[j * 8 + 2 * e], y = v[j * 8 + 2 * e + 1];
+              float2 r, r2;
+              hi[e] = rs_pack(T{}, x, y, r);
+              if (TERMS == 2) lo[e] = rs_pack(T{}, x - r.x, y - r.y, r2);
             }
+            const int ch = (half * 4 + j) ^ (row & 7);  // (MT is a multiple of 8: the same for the lo row)
+            *reinterpret_cast<uint4*>(blk + row * 128 + ch * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if (TERMS == 2)
+              *reinterpret_cast<uint4*>(blk + (MT + row) * 128 + ch * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
           }
           fence_proxy_async_smem();
         }
@@ -664,95 +690,93 @@ __global__ void __launch_bounds__(RsShape<AROWS>::threads, RsShape<AROWS>::ctas)
         named_bar_sync(1, 32 * CW);
         if (warp == 0 && lane == 0) {
           // the other CTAs' blocks are still to come; then this CTA's block to them
-          const int n_work = min(cs, (nv + ns - 1) / ns);
-          mbar_arrive_expect_tx(s.p_full, (uint32_t)(n_work - (mine ? 1 : 0)) * blk_bytes);
+          const int n_work = min(RS_CS, (nv + RS_NS - 1) / RS_NS);
+          mbar_arrive_expect_tx(s.p_full, (uint32_t)(n_work - (mine ? 1 : 0)) * RS_PBLK);
           if (mine && !*s.abort_flag)
-            for (int r = 1; r < cs; ++r) {
-              const uint32_t to = (uint32_t)((rank + r) % cs);
-              unsigned char* src = s.p + (size_t)rank * blk_bytes;
-              bulk_s2s(cluster_map(src, to), src, blk_bytes, cluster_map(s.p_full, to));
+            for (int r = 1; r < RS_CS; ++r) {
+              const uint32_t to = (uint32_t)((rank + r) % RS_CS);
+              unsigned char* src = s.p + (size_t)rank * RS_PBLK;
+              bulk_s2s(cluster_map(src, to), src, RS_PBLK, cluster_map(s.p_full, to));
             }
         }
         __syncwarp();
-        if (!SAME || lane < 16)
-          for (int r = 0; r < cs; ++r) {
-            const uint32_t to = cluster_map(&ssum[(c0 >> 5) * MT + row], r);
-            st_cluster_f32(to, l[0]);
-            if (hw == 64) st_cluster_f32(to + MT * 4, l[1]);
-          }
+#pragma unroll
+        for (int r = 0; r < RS_CS; ++r) st_cluster_f32(cluster_map(&ssum[(rank * 2 + half) * MT + row], r), l);
         __syncwarp();
-        if (lane < cs) mbar_arrive_cluster(cluster_map(s.sums, lane));
+        if (lane < RS_CS) mbar_arrive_cluster(cluster_map(s.sums, lane));
       }
+      if (a.ahead) scores(nxt);
       // ------------------------------------------------------------------------------------- epilogue
       float coef = 0.f;
-      if (does) {
+      if (term == 0) {
         done(*s.abort_flag || mbar_wait_cluster(s.sums, unit & 1));
         float m = a.softmax ? -CUDART_INF_F : 0.f, l = 0.f;
-        for (int r = 0; r < 2 * cs; ++r) m = fmaxf(m, smax[r * MT + row]);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) l += ssum[r * MT + row];
+        for (int r = 0; r < 2 * RS_CS; ++r) {
+          m = fmaxf(m, smax[r * MT + row]);
+          l += ssum[r * MT + row];
+        }
         if (a.softmax) coef = l != 0.f ? 1.f / l : 0.f;
         else coef = pnv + seg0 > 0 ? rsqrtf((float)(pnv + seg0)) / f16_range_scale(m) : 0.f;
-        if (live && rank == 0 && half == 0 && (!SAME || term == 0))
-          a.ml[(int64_t)pos * a.segs + seg] = make_float2(m, l);
+        if (live && rank == 0 && half == 0) a.ml[(int64_t)pos * a.segs + seg] = make_float2(m, l);
       }
-      done(*s.abort_flag || mbar_wait_bounded(s.o_full, unit & 1));
+      done(*s.abort_flag || mbar_wait_spin(s.o_full, unit & 1));
       tc_fence_after();
       float* dst = a.part + ((int64_t)pos * a.segs + seg) * a.d_s + x0;
-      // the two halves of the warps take alternate boxes of 64 columns. The lo rows' parts go through the scratch: two
-      // buffers in turn where it holds two (one barrier a box then separates a write from the read two boxes before)
-      for (int b = half, turn = 0; b < my_boxes; b += 2, turn ^= 1) {
-        float o[64];
-        tc_ld64(tl + (uint32_t)b * 64, o);
-        if (SAME) {
-#pragma unroll
-          for (int i = 0; i < 64; ++i) o[i] += __shfl_xor_sync(0xffffffffu, o[i], 16);
-        } else if (TERMS == 2) {
-          float* x = xch + (ns == 128 ? turn * 64 * 32 : 0);
+      // the two halves of the warps take alternate passes of 32 columns. The lo rows' parts go through the scratch, its
+      // two buffers in turn: one barrier a pass separates a write from the read two passes before
+      for (int q0 = half * 32, turn = 0; q0 < my_boxes * 64; q0 += 64, turn ^= 1) {
+        float o[32];
+        tc_ld32(tl + (uint32_t)q0, o);
+        if (TERMS == 2) {
+          float* x = xch + turn * 32 * 32;
           if (term == 1)
 #pragma unroll
-            for (int i = 0; i < 64; ++i) x[i * 32 + lane] = o[i];
+            for (int i = 0; i < 32; ++i) x[i * 32 + lane] = o[i];
           named_bar_sync(pair_bar, 64);
           if (term == 0)
 #pragma unroll
-            for (int i = 0; i < 64; ++i) o[i] += x[i * 32 + lane];
-          if (ns != 128) named_bar_sync(pair_bar, 64);
+            for (int i = 0; i < 32; ++i) o[i] += x[i * 32 + lane];
         }
-        if (does && live) {
+        if (term == 0 && live) {
 #pragma unroll
-          for (int i = 0; i < 64; i += 4)
-            if (x0 + b * 64 + i < a.d_s && (!SAME || (i >> 5) == term))  // SAME: a pair's two lanes store a half each
-              *reinterpret_cast<float4*>(dst + b * 64 + i) =
+          for (int i = 0; i < 32; i += 4)
+            if (x0 + q0 + i < a.d_s)
+              *reinterpret_cast<float4*>(dst + q0 + i) =
                   make_float4(o[i] * coef, o[i + 1] * coef, o[i + 2] * coef, o[i + 3] * coef);
         }
       }
       tc_fence_before();
+      if (TERMS == 2) named_bar_sync(pair_bar, 64);  // the scratch is read before the next unit's scores go there
       __syncwarp();
       if (lane == 0) mbar_arrive(s.o_empty);
+      if (!a.ahead) scores(nxt);
       ++unit;
+      cur = nxt;
     }
   }
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // no CTA leaves while another may still write to its shared memory
   tc_fence_after();
-  if (warp == C::mma) tc_dealloc(taddr, (uint32_t)a.tmem_cols);
+  if (warp == 3) tc_dealloc(taddr, 512);
 }
 
 // ----------------------------------------------------------------------------------------------------- combine
-// r[row] = sum_j wk[row, j] * (the pair's segments, merged by their maxima and sums). One CTA per (row, 128 columns):
-// 8 groups of 32 threads take the routed chunks j = group, group + 8, ..., and their sums are added in the order of the
-// groups, so the result depends on nothing but the row.
-constexpr int RC_GROUPS = 8;
-template <typename TO>
-__global__ void __launch_bounds__(32 * RC_GROUPS) shared_combine_kernel(const SharedArgs a, TO* __restrict__ r) {
-  __shared__ float4 sum[RC_GROUPS][32];
+// r[row] = sum_j wk[row, j] * (the pair's segments, merged by their maxima and sums). G groups of threads take the
+// routed chunks j = group, group + G, ..., and their sums are added in the order of the groups, so the result depends
+// on nothing but the row. G = 1 for up to 8 routed chunks (256 threads, 1024 columns), else 8 (128 columns).
+template <typename TO, int G>
+__global__ void __launch_bounds__(256) shared_combine_kernel(const SharedArgs a, TO* __restrict__ r) {
+  constexpr int W = 256 / G;
+  __shared__ float4 sum[G > 1 ? G : 1][G > 1 ? W : 1];
   const int64_t row = blockIdx.x;
   const int64_t lib = row / a.rows_per_lib;
-  const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;
-  const int x = (blockIdx.y * 32 + lane) * 4;
+  const int lane = threadIdx.x % W, grp = threadIdx.x / W;
+  const int x = (blockIdx.y * W + lane) * 4;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int j = grp; j < a.k; j += RC_GROUPS) {
+#pragma unroll 4
+  for (int j = grp; j < a.k; j += G) {
     const int64_t pair = row * a.k + j;
     const int page = a.page[pair];
     if (page < 0) continue;
@@ -763,7 +787,7 @@ __global__ void __launch_bounds__(32 * RC_GROUPS) shared_combine_kernel(const Sh
     float m = -CUDART_INF_F, z = 0.f;
     if (a.segs > 1) {
       const int nv = min(a.n_valid[lib * a.C + a.idx[pair]], a.page_rows);
-      segs = (nv + a.seg_rows - 1) / a.seg_rows;
+      segs = (nv + RS_SEG - 1) / RS_SEG;
       if (a.softmax) {
         for (int g = 0; g < segs; ++g) m = fmaxf(m, a.ml[pos * a.segs + g].x);
         for (int g = 0; g < segs; ++g) {
@@ -787,19 +811,20 @@ __global__ void __launch_bounds__(32 * RC_GROUPS) shared_combine_kernel(const Sh
       }
     }
   }
-  sum[grp][lane] = acc;
-  __syncthreads();
-  if (grp != 0 || x >= a.d_s) return;
-  const int n = min(a.k, RC_GROUPS);
-  for (int g = 1; g < n; ++g) {
-    const float4 v = sum[g][lane];
-    acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+  if (G > 1) {
+    sum[grp][lane] = acc;
+    __syncthreads();
+    if (grp != 0) return;
+#pragma unroll
+    for (int g = 1; g < G; ++g) {
+      const float4 v = sum[g][lane];
+      acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+    }
   }
-  TO* o = r + row * a.d_s + x;
-  o[0] = from_f32<TO>(acc.x);
-  o[1] = from_f32<TO>(acc.y);
-  o[2] = from_f32<TO>(acc.z);
-  o[3] = from_f32<TO>(acc.w);
+  if (x >= a.d_s) return;
+  alignas(16) TO o[4] = {from_f32<TO>(acc.x), from_f32<TO>(acc.y), from_f32<TO>(acc.z), from_f32<TO>(acc.w)};
+  if (sizeof(TO) == 4) *reinterpret_cast<uint4*>(r + row * a.d_s + x) = *reinterpret_cast<const uint4*>(o);
+  else *reinterpret_cast<uint2*>(r + row * a.d_s + x) = *reinterpret_cast<const uint2*>(o);
 }
 
 }  // namespace xencb

@@ -247,6 +247,23 @@ int tensor_map_2d(CUtensorMap* map, CUtensorMapDataType dt, uint32_t esize, cons
   return XENCB_OK;
 }
 
+// A 3-D tensor map of 16-bit elements, 128-byte swizzle, OOB elements filled with zeros.
+int tensor_map_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, const uint64_t (&n)[3],
+                  const uint64_t (&stride)[2], const uint32_t (&boxn)[3]) {
+  CUtensorMap probe;
+  int rc = g_encode ? XENCB_OK : tensor_map_2d(&probe, dt, 2, base, n[0], n[1], stride[0], boxn[0], boxn[1]);
+  if (rc) return rc;
+  const cuuint64_t dims[3] = {n[0], n[1], n[2]};
+  const cuuint64_t strides[2] = {stride[0], stride[1]};
+  const cuuint32_t box[3] = {boxn[0], boxn[1], boxn[2]};
+  const cuuint32_t es[3] = {1, 1, 1};
+  const CUresult r = g_encode(map, dt, 3, const_cast<void*>(base), dims, strides, box, es,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(XENCB_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return XENCB_OK;
+}
+
 // part = split partials of X @ W^T. X: [M, K] of type TX; W: [N, K] float32 (nn.Linear layout).
 // `xbuf` (M*K float32, may be null when TX is float) stages a 16-bit X as float32 for the TMA path.
 template <typename TX>
@@ -320,7 +337,7 @@ int launch_gemm(const void* X, int64_t M, int K, const float* W, int N, int sms,
 // ------------------------------------------------------------------------------------------------ adapters
 // Extra workspace of a projection with adapters: one more split partial (behind the GEMM's) and t [n_rows, rank].
 size_t adapt_slice_bytes(int64_t M, int N) { return align_up((size_t)M * N * sizeof(float), 256); }
-size_t adapt_t_bytes(int64_t M, int rank) { return align_up((size_t)M * rank * sizeof(float), 256); }
+size_t adapt_t_bytes(int64_t M, int rank) { return align_up((size_t)M * rank * AD_MAX_SPLITS * sizeof(float), 256); }
 
 int check_adapters(const char* what, const AdaptArgs& ad, int dtype) {
   if (!ad.a || !ad.b || !ad.of) return fail(XENCB_EINVAL, "%s: adapt_a, adapt_b and adapter_of are required", what);
@@ -333,26 +350,63 @@ int check_adapters(const char* what, const AdaptArgs& ad, int dtype) {
   return XENCB_OK;
 }
 
+bool adapt_tiles(const AdaptArgs& ad) { return ad.rows_per_adapter >= AD_MIN_TILE; }
+
+int64_t adapt_tile_count(const AdaptArgs& ad) {
+  const int64_t groups = (ad.n_rows + ad.rows_per_adapter - 1) / ad.rows_per_adapter;
+  return groups * ((std::min(ad.rows_per_adapter, ad.n_rows) + AD_TILE_ROWS - 1) / AD_TILE_ROWS);
+}
+
+// The sizes of one call; splits of d_in so that the shrink's tiles cover the SMs about twice.
+void plan_adapters(AdaptArgs* ad, const void* x, int64_t M, int d_in, int d_out, int sms) {
+  ad->n_rows = M;
+  ad->d_in = d_in;
+  ad->d_out = d_out;
+  ad->rows_per_adapter = std::min(ad->rows_per_adapter, M);  // (one group: the tiles need not cover more rows)
+  ad->vec_in = d_in % 8 == 0 && aligned(x, 16) && aligned(ad->a, 16);
+  ad->vec_r = ad->r % 8 == 0 && aligned(ad->b, 16);
+  ad->splits = 1;
+  if (adapt_tiles(*ad)) {
+    const int64_t ctas = adapt_tile_count(*ad) * ((ad->r + AD_TILE_J - 1) / AD_TILE_J);
+    ad->splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(AD_MAX_SPLITS, d_in / 256), (2 * sms + ctas - 1) / ctas));
+  }
+}
+
 // t = x A^T, before the GEMM (the row split that follows reads only x).
 template <typename TX>
-int launch_adapt_shrink(const void* x, int64_t M, const AdaptArgs& ad, int dtype, cudaStream_t st) {
+int launch_adapt_shrink(const void* x, const AdaptArgs& ad, int dtype, cudaStream_t st) {
   const TX* xp = static_cast<const TX*>(x);
-  switch (dtype) {
-    case XENCB_F32: adapt_shrink_kernel<TX, float><<<(unsigned)M, 256, 0, st>>>(xp, ad); break;
-    case XENCB_F16: adapt_shrink_kernel<TX, __half><<<(unsigned)M, 256, 0, st>>>(xp, ad); break;
-    default: adapt_shrink_kernel<TX, __nv_bfloat16><<<(unsigned)M, 256, 0, st>>>(xp, ad); break;
-  }
+  auto go = [&](auto t) {
+    using TA = decltype(t);
+    if (adapt_tiles(ad))
+      launch_pdl(adapt_shrink_tile_kernel<TX, TA>,
+                 dim3((unsigned)adapt_tile_count(ad), (unsigned)((ad.r + AD_TILE_J - 1) / AD_TILE_J), (unsigned)ad.splits),
+                 dim3(128), 0, st, xp, ad);
+    else
+      launch_pdl(adapt_shrink_row_kernel<TX, TA>, dim3((unsigned)ad.n_rows, (unsigned)((ad.r + 7) / 8)), dim3(256), 0,
+                 st, xp, ad);
+  };
+  if (dtype == XENCB_F32) go(float{});
+  else if (dtype == XENCB_F16) go(__half{});
+  else go(__nv_bfloat16{});
   XENCB_CHECK_LAUNCH("adapt_shrink launch");
   return XENCB_OK;
 }
 
-int launch_adapt_expand(float* out, int64_t M, const AdaptArgs& ad, int dtype, cudaStream_t st) {
-  const dim3 grid((unsigned)M, (unsigned)((ad.d_out + 255) / 256));
-  switch (dtype) {
-    case XENCB_F32: adapt_expand_kernel<float><<<grid, 256, 0, st>>>(ad, out); break;
-    case XENCB_F16: adapt_expand_kernel<__half><<<grid, 256, 0, st>>>(ad, out); break;
-    default: adapt_expand_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(ad, out); break;
-  }
+int launch_adapt_expand(float* out, const AdaptArgs& ad, int dtype, cudaStream_t st) {
+  auto go = [&](auto t) {
+    using TA = decltype(t);
+    if (adapt_tiles(ad))
+      launch_pdl(adapt_expand_tile_kernel<TA>,
+                 dim3((unsigned)adapt_tile_count(ad), (unsigned)((ad.d_out + AD_TILE_N - 1) / AD_TILE_N)), dim3(128), 0,
+                 st, ad, out);
+    else
+      launch_pdl(adapt_expand_row_kernel<TA>, dim3((unsigned)ad.n_rows, (unsigned)((ad.d_out + 255) / 256)), dim3(256),
+                 0, st, ad, out);
+  };
+  if (dtype == XENCB_F32) go(float{});
+  else if (dtype == XENCB_F16) go(__half{});
+  else go(__nv_bfloat16{});
   XENCB_CHECK_LAUNCH("adapt_expand launch");
   return XENCB_OK;
 }
@@ -660,7 +714,7 @@ int plan_build(int n_chunks, int d_s, int page_rows, BuildPlan* p) {
 
 // ------------------------------------------------------------------------------------------------ shared read plan
 struct SharedPlan {
-  int terms, arows, cs, ns, slab, tmem_cols, seg_rows, segs, mt;
+  int terms, slab, segs, mt;
   int64_t n_pairs, max_tiles;
   size_t cnt, pair, tiles, q, part, ml, total;  // bytes of each workspace part
 };
@@ -672,24 +726,17 @@ int plan_shared(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows, 
   if (slots_dtype != XENCB_F16 && slots_dtype != XENCB_BF16)
     return fail(XENCB_ENOTSUP, "read_shared: the tensor-core read takes f16 / bf16 slots");
   if (!elem_size(out_dtype)) return fail(XENCB_EINVAL, "read_shared: out_dtype %d unknown", out_dtype);
-  if (d_s % 8 != 0 || d_s > RS_SLAB * RS_MAX_CS)
-    return fail(XENCB_ENOTSUP, "read_shared: d_s=%d must be a multiple of 8, at most %d", d_s, RS_SLAB * RS_MAX_CS);
+  if (d_s % 8 != 0 || d_s > RS_SLAB * RS_CS)
+    return fail(XENCB_ENOTSUP, "read_shared: d_s=%d must be a multiple of 8, at most %d", d_s, RS_SLAB * RS_CS);
   if (n_rows > INT32_MAX / k || 2 * n_rows * k + 64 > INT32_MAX)
     return fail(XENCB_ENOTSUP, "read_shared: %lld rows x %d routed chunks are too many", (long long)n_rows, k);
   if (n_pages * (int64_t)page_rows + 1024 > INT32_MAX)
     return fail(XENCB_ENOTSUP, "read_shared: the slot pool is too large for 32-bit TMA coordinates");
   p->n_pairs = n_rows * k;
   p->terms = out_dtype == XENCB_F32 ? 2 : 1;
-  // Few pairs a page on average (a tile of 32 / terms holds them): the shape with two CTAs per SM.
-  const bool few = d_s <= 4 * RS_SLAB && p->n_pairs <= n_pages * (32 / p->terms);
-  p->arows = few ? 32 : 64;
-  p->mt = p->arows / p->terms;
-  p->cs = few || d_s > 4 * RS_SLAB ? 8 : 4;
-  p->slab = (int)align_up((size_t)(d_s + p->cs - 1) / p->cs, 64);
-  p->ns = 512 / p->cs;
-  p->tmem_cols = few ? 256 : 512;  // >= slab and >= RS_ACC * ns; two CTAs of the first shape share an SM's 512
-  p->seg_rows = 512;
-  p->segs = (page_rows + p->seg_rows - 1) / p->seg_rows;
+  p->mt = RS_AROWS / p->terms;
+  p->slab = (int)align_up((size_t)(d_s + RS_CS - 1) / RS_CS, 64);
+  p->segs = (page_rows + RS_SEG - 1) / RS_SEG;
   if (p->n_pairs * p->segs > INT32_MAX)
     return fail(XENCB_ENOTSUP, "read_shared: page_rows=%d is too long for this many rows", page_rows);
   p->max_tiles = p->n_pairs / p->mt + std::min<int64_t>(n_pages, p->n_pairs) + 1;
@@ -703,55 +750,57 @@ int plan_shared(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows, 
   return XENCB_OK;
 }
 
-// Clusters of the read kernel that fit the device at once, per device, cluster size and kernel.
+// Clusters of the read kernel that fit the device at once, per device and kernel.
 template <typename K>
-int shared_clusters(K kern, int cs, int threads, size_t smem, int* out) {
+int shared_clusters(K kern, int* out) {
   static std::mutex mu;
-  static std::unordered_map<const void*, int> known[kMaxDev][RS_MAX_CS + 1];
+  static std::unordered_map<const void*, int> known[kMaxDev];
   int dev = 0;
   cudaGetDevice(&dev);
   std::lock_guard<std::mutex> lk(mu);
-  auto& m = known[dev][cs];
-  const auto itr = m.find(reinterpret_cast<const void*>(kern));
-  if (itr != m.end()) {
+  const auto itr = known[dev].find(reinterpret_cast<const void*>(kern));
+  if (itr != known[dev].end()) {
     *out = itr->second;
     return XENCB_OK;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)cs);
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.gridDim = dim3(RS_CS);
+  cfg.blockDim = dim3(RS_THREADS);
+  cfg.dynamicSmemBytes = RS_SMEM;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)cs;
+  at[0].val.clusterDim.x = RS_CS;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
   int n = 0;
   const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
   if (e != cudaSuccess) return cuda_fail(e, "read_shared: cudaOccupancyMaxActiveClusters");
-  if (n <= 0) return fail(XENCB_ENOTSUP, "read_shared: no cluster of %d CTAs fits this device", cs);
-  m[reinterpret_cast<const void*>(kern)] = n;
+  if (n <= 0) return fail(XENCB_ENOTSUP, "read_shared: no cluster of %d CTAs fits this device", RS_CS);
+  known[dev][reinterpret_cast<const void*>(kern)] = n;
   *out = n;
   return XENCB_OK;
 }
 
-template <typename T, int TERMS, int AROWS>
+template <typename T, int TERMS>
 int run_shared(const void* q, int q_dtype, const SharedPlan& p, SharedArgs a, const void* slots, const void* vslots,
                void* q16, int64_t n_rows, void* r_out, int out_dtype, int sms, cudaStream_t st) {
   const CUtensorMapDataType dt =
       std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const uint64_t d = (uint64_t)a.d_s, pool_rows = (uint64_t)a.n_pages * a.page_rows;
-  using Shape = RsShape<AROWS>;
   CUtensorMap mq, mq8, mk, mv;
-  int rc = tensor_map_2d(&mq, dt, 2, q16, d, (uint64_t)TERMS * p.n_pairs, d * 2, 64, (uint32_t)p.mt);
+  const uint64_t np = (uint64_t)p.n_pairs;
+  int rc = tensor_map_3d(&mq, dt, q16, {d, np, (uint64_t)TERMS}, {d * 2, np * d * 2}, {64, (uint32_t)p.mt, TERMS});
   if (!rc) rc = tensor_map_2d(&mq8, dt, 2, q16, d, (uint64_t)TERMS * p.n_pairs, d * 2, 64, 8);
-  if (!rc) rc = tensor_map_2d(&mk, dt, 2, slots, d, pool_rows, d * 2, 64, (uint32_t)p.ns);
-  if (!rc) rc = tensor_map_2d(&mv, dt, 2, vslots ? vslots : slots, d, pool_rows, d * 2, 64, RS_VROWS);
-  auto kern = shared_read_kernel<T, TERMS, AROWS>;
-  if (!rc) rc = ensure_smem(kern, (int)Shape::smem);
+  if (!rc) rc = tensor_map_2d(&mk, dt, 2, slots, d, pool_rows, d * 2, 64, RS_NS);
+  const void* v = vslots ? vslots : slots;
+  a.v3d = a.d_s % 64 == 0;
+  if (!rc && a.v3d) rc = tensor_map_3d(&mv, dt, v, {64, pool_rows, d / 64}, {d * 2, 128}, {64, RS_VROWS, 4});
+  if (!rc && !a.v3d) rc = tensor_map_2d(&mv, dt, 2, v, d, pool_rows, d * 2, 64, RS_VROWS);
+  auto kern = shared_read_kernel<T, TERMS>;
+  if (!rc) rc = ensure_smem(kern, (int)RS_SMEM);
   int n_clusters = 0;
-  if (!rc) rc = shared_clusters(kern, p.cs, Shape::threads, Shape::smem, &n_clusters);
+  if (!rc) rc = shared_clusters(kern, &n_clusters);
   if (rc) return rc;
   n_clusters = (int)std::min<int64_t>(n_clusters, p.max_tiles * p.segs);
   if (p.n_pairs <= 4096) {
@@ -766,38 +815,39 @@ int run_shared(const void* q, int q_dtype, const SharedPlan& p, SharedArgs a, co
     XENCB_CHECK_LAUNCH("shared_scan launch");
   }
   T* qo = static_cast<T*>(q16);
-  switch (q_dtype) {
-    case XENCB_F32:
-      shared_split_kernel<float, T, TERMS><<<(unsigned)p.n_pairs, 256, 0, st>>>(static_cast<const float*>(q), a, qo);
-      break;
-    case XENCB_F16:
-      shared_split_kernel<__half, T, TERMS><<<(unsigned)p.n_pairs, 256, 0, st>>>(static_cast<const __half*>(q), a, qo);
-      break;
-    default:
-      shared_split_kernel<__nv_bfloat16, T, TERMS>
-          <<<(unsigned)p.n_pairs, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(q), a, qo);
-      break;
-  }
+  const dim3 sgrid((unsigned)n_rows, (unsigned)((a.k + 7) / 8));
+  auto split = [&](auto t) {
+    using TQ = decltype(t);
+    shared_split_kernel<TQ, T, TERMS><<<sgrid, RS_SPLIT_THREADS, 0, st>>>(static_cast<const TQ*>(q), a, qo);
+  };
+  if (q_dtype == XENCB_F32) split(float{});
+  else if (q_dtype == XENCB_F16) split(__half{});
+  else split(__nv_bfloat16{});
   XENCB_CHECK_LAUNCH("shared_split launch");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(n_clusters * p.cs));
-  cfg.blockDim = dim3(Shape::threads);
-  cfg.dynamicSmemBytes = Shape::smem;
+  cfg.gridDim = dim3((unsigned)(n_clusters * RS_CS));
+  cfg.blockDim = dim3(RS_THREADS);
+  cfg.dynamicSmemBytes = RS_SMEM;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)p.cs;
+  at[0].val.clusterDim.x = RS_CS;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
   (void)cudaLaunchKernelEx(&cfg, kern, mq, mq8, mk, mv, a);
   XENCB_CHECK_LAUNCH("shared_read launch");
-  const dim3 grid((unsigned)n_rows, (unsigned)((a.d_s + 127) / 128));
-  switch (out_dtype) {
-    case XENCB_F32: shared_combine_kernel<float><<<grid, 256, 0, st>>>(a, static_cast<float*>(r_out)); break;
-    case XENCB_F16: shared_combine_kernel<__half><<<grid, 256, 0, st>>>(a, static_cast<__half*>(r_out)); break;
-    default: shared_combine_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a, static_cast<__nv_bfloat16*>(r_out)); break;
-  }
+  auto combine = [&](auto t) {
+    using TO = decltype(t);
+    TO* r = static_cast<TO*>(r_out);
+    if (a.k <= 8)
+      shared_combine_kernel<TO, 1><<<dim3((unsigned)n_rows, (unsigned)((a.d_s + 1023) / 1024)), 256, 0, st>>>(a, r);
+    else
+      shared_combine_kernel<TO, 8><<<dim3((unsigned)n_rows, (unsigned)((a.d_s + 127) / 128)), 256, 0, st>>>(a, r);
+  };
+  if (out_dtype == XENCB_F32) combine(float{});
+  else if (out_dtype == XENCB_F16) combine(__half{});
+  else combine(__nv_bfloat16{});
   XENCB_CHECK_LAUNCH("shared_combine launch");
   return XENCB_OK;
 }
@@ -884,13 +934,12 @@ static int project_in_impl(const void* h, int h_dtype, int64_t n_rows, int d_m, 
   AdaptArgs ad{};
   if (adapters) {
     ad = *adapters;
-    ad.d_in = d_m;
-    ad.d_out = d_s;
+    plan_adapters(&ad, h, n_rows, d_m, d_s, di.sms);
     ad.t = reinterpret_cast<float*>(ws + g_bytes + nq_bytes + rd_bytes);
     switch (h_dtype) {
-      case XENCB_F32: rc = launch_adapt_shrink<float>(h, n_rows, ad, adapt_dtype, st); break;
-      case XENCB_F16: rc = launch_adapt_shrink<__half>(h, n_rows, ad, adapt_dtype, st); break;
-      default: rc = launch_adapt_shrink<__nv_bfloat16>(h, n_rows, ad, adapt_dtype, st); break;
+      case XENCB_F32: rc = launch_adapt_shrink<float>(h, ad, adapt_dtype, st); break;
+      case XENCB_F16: rc = launch_adapt_shrink<__half>(h, ad, adapt_dtype, st); break;
+      default: rc = launch_adapt_shrink<__nv_bfloat16>(h, ad, adapt_dtype, st); break;
     }
     if (rc) return rc;
   }
@@ -908,7 +957,7 @@ static int project_in_impl(const void* h, int h_dtype, int64_t n_rows, int d_m, 
   }
   if (rc) return rc;
   if (adapters) {  // the low-rank term is one more split partial
-    rc = launch_adapt_expand(part + (size_t)gp.splits * n_rows * d_s, n_rows, ad, adapt_dtype, st);
+    rc = launch_adapt_expand(part + (size_t)gp.splits * n_rows * d_s, ad, adapt_dtype, st);
     if (rc) return rc;
     ++gp.splits;
   }
@@ -1589,16 +1638,14 @@ int xencb_read_shared(const void* q, int q_dtype, int64_t n_rows, int d_s, const
   void* q16 = take(p.q);
   a.part = reinterpret_cast<float*>(take(p.part));
   a.ml = reinterpret_cast<float2*>(take(p.ml));
-  a.segs = p.segs; a.seg_rows = p.seg_rows; a.cs = p.cs; a.ns = p.ns; a.slab = p.slab;
-  a.tmem_cols = p.tmem_cols;
+  a.segs = p.segs; a.slab = p.slab; a.ahead = p.slab <= RS_AHEAD_SLAB ? 1 : 0;
   a.softmax = read_softmax ? 1 : 0;
   a.qscale = read_softmax ? read_temp * 1.4426950408889634f : 1.f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto run = [&](auto t) {
     using T = decltype(t);
     auto go = [&](auto kern) { return kern(q, q_dtype, p, a, slots, vslots, q16, n_rows, r_out, out_dtype, di.sms, st); };
-    if (p.arows == 32) return p.terms == 2 ? go(run_shared<T, 2, 32>) : go(run_shared<T, 1, 32>);
-    return p.terms == 2 ? go(run_shared<T, 2, 64>) : go(run_shared<T, 1, 64>);
+    return p.terms == 2 ? go(run_shared<T, 2>) : go(run_shared<T, 1>);
   };
   return slots_dtype == XENCB_F16 ? run(__half{}) : run(__nv_bfloat16{});
 }
@@ -1651,16 +1698,15 @@ static int project_out_impl(const float* r, int64_t n_rows, int d_s, const float
   AdaptArgs ad{};
   if (adapters) {
     ad = *adapters;
-    ad.d_in = d_s;
-    ad.d_out = d_m;
+    plan_adapters(&ad, r, n_rows, d_s, d_m, di.sms);
     ad.t = reinterpret_cast<float*>(ws + g_bytes + d_bytes + np_bytes + rd_bytes);
-    rc = launch_adapt_shrink<float>(r, n_rows, ad, adapt_dtype, st);
+    rc = launch_adapt_shrink<float>(r, ad, adapt_dtype, st);
     if (rc) return rc;
   }
   rc = launch_gemm<float>(r, n_rows, d_s, w_out, d_m, di.sms, part, w_prep ? xbuf : nullptr, nullptr, st, &gp, w_prep);
   if (rc) return rc;
   if (adapters) {  // the low-rank term is one more split partial
-    rc = launch_adapt_expand(part + (size_t)gp.splits * n_rows * d_m, n_rows, ad, adapt_dtype, st);
+    rc = launch_adapt_expand(part + (size_t)gp.splits * n_rows * d_m, ad, adapt_dtype, st);
     if (rc) return rc;
     ++gp.splits;
   }
@@ -1731,7 +1777,9 @@ int xencb_project_in_adapted(const void* h, int h_dtype, int64_t n_rows, int d_m
                              const void* adapt_b, int adapt_dtype, const float* adapt_scale, int n_adapters, int rank,
                              const int32_t* adapter_of, int64_t rows_per_adapter, void* workspace,
                              size_t workspace_bytes, void* stream) {
-  const AdaptArgs ad{adapt_a, adapt_b, adapt_scale, adapter_of, rows_per_adapter, n_adapters, rank, 0, 0, nullptr};
+  AdaptArgs ad{};
+  ad.a = adapt_a; ad.b = adapt_b; ad.scale = adapt_scale; ad.of = adapter_of; ad.rows_per_adapter = rows_per_adapter;
+  ad.n = n_adapters; ad.r = rank;
   const int rc = check_adapters("project_in_adapted", ad, adapt_dtype);
   if (rc) return rc;
   return project_in_impl(h, h_dtype, n_rows, d_m, w_in, w_prep, b_in, d_s, flags, gate_w, gate_b, gate_b_dev, sel_w,
@@ -1751,7 +1799,9 @@ int xencb_project_out_adapted(const float* r, int64_t n_rows, int d_s, const flo
                               const void* adapt_a, const void* adapt_b, int adapt_dtype, const float* adapt_scale,
                               int n_adapters, int rank, const int32_t* adapter_of, int64_t rows_per_adapter,
                               void* workspace, size_t workspace_bytes, void* stream) {
-  const AdaptArgs ad{adapt_a, adapt_b, adapt_scale, adapter_of, rows_per_adapter, n_adapters, rank, 0, 0, nullptr};
+  AdaptArgs ad{};
+  ad.a = adapt_a; ad.b = adapt_b; ad.scale = adapt_scale; ad.of = adapter_of; ad.rows_per_adapter = rows_per_adapter;
+  ad.n = n_adapters; ad.r = rank;
   const int rc = check_adapters("project_out_adapted", ad, adapt_dtype);
   if (rc) return rc;
   return project_out_impl(r, n_rows, d_s, w_out, w_prep, b_out, d_m, scale, log_scale_dev, gate, sel_w, log_alpha,
@@ -1773,20 +1823,30 @@ static int check_pools(const char* what, void* const* pools, const int64_t* row_
 }
 
 static int launch_page_copies(void* const* pools, const int64_t* row_bytes, int n_pools, int page_rows,
-                              const PageMove* moves, const int* n_moves, int sms, cudaStream_t st) {
+                              int64_t max_moves, const PageMove* moves, const int* n_moves, int sms, cudaStream_t st) {
   for (int i0 = 0; i0 < n_pools; i0 += PG_POOLS) {
     PagePools pp{};
-    pp.n = std::min(PG_POOLS, n_pools - i0);
+    const int n = std::min(PG_POOLS, n_pools - i0);
     pp.page_rows = page_rows;
     bool vec = true;
-    for (int i = 0; i < pp.n; ++i) {
+    for (int i = 0; i < n; ++i) {
       pp.base[i] = static_cast<char*>(pools[i0 + i]);
       pp.row_bytes[i] = row_bytes[i0 + i];
       vec = vec && aligned(pools[i0 + i], 16) && pp.row_bytes[i] * page_rows % 16 == 0;
     }
-    const unsigned grid = (unsigned)(8 * sms);
-    if (vec) pages_copy_kernel<uint4><<<grid, 256, 0, st>>>(pp, moves, n_moves);
-    else pages_copy_kernel<uint16_t><<<grid, 256, 0, st>>>(pp, moves, n_moves);
+    const int64_t slice = (int64_t)PG_COPY_THREADS * PG_UNROLL * (vec ? 16 : 2);
+    int64_t slices = 0;
+    for (int i = 0; i < n; ++i) {
+      pp.first[i] = (int)slices;
+      slices += (pp.row_bytes[i] * page_rows + slice - 1) / slice;
+      if (slices > INT32_MAX) return fail(XENCB_ENOTSUP, "pages: the pools' pages are too large");
+    }
+    for (int i = n; i <= PG_POOLS; ++i) pp.first[i] = (int)slices;
+    pp.slices = (int)slices;
+    // (the first copy launch follows the plan kernel, later ones a copy that has read the same list)
+    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(8 * sms, max_moves * slices));
+    if (vec) launch_pdl(pages_copy_kernel<uint4>, dim3(grid), dim3(PG_COPY_THREADS), 0, st, pp, moves, n_moves);
+    else launch_pdl(pages_copy_kernel<uint16_t>, dim3(grid), dim3(PG_COPY_THREADS), 0, st, pp, moves, n_moves);
     XENCB_CHECK_LAUNCH("pages_copy launch");
   }
   return XENCB_OK;
@@ -1834,7 +1894,7 @@ int xencb_pages_fork(void* const* pools, const int64_t* row_bytes, int n_pools, 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   pages_fork_plan_kernel<<<1, PG_THREADS, smem, st>>>(a);
   XENCB_CHECK_LAUNCH("pages_fork_plan launch");
-  return launch_page_copies(pools, row_bytes, n_pools, page_rows, a.moves, a.n_moves, di.sms, st);
+  return launch_page_copies(pools, row_bytes, n_pools, page_rows, n_children * n_chunks, a.moves, a.n_moves, di.sms, st);
 }
 
 size_t xencb_pages_compact_workspace(int64_t n_pages) {
@@ -1875,7 +1935,7 @@ int xencb_pages_compact(void* const* pools, const int64_t* row_bytes, int n_pool
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   pages_compact_plan_kernel<<<1, PG_THREADS, smem, st>>>(a);
   XENCB_CHECK_LAUNCH("pages_compact_plan launch");
-  return launch_page_copies(pools, row_bytes, n_pools, page_rows, a.moves, a.n_moves, di.sms, st);
+  return launch_page_copies(pools, row_bytes, n_pools, page_rows, n_pages / 2 + 1, a.moves, a.n_moves, di.sms, st);
 }
 
 // ------------------------------------------------------------------------------------------------ selector
