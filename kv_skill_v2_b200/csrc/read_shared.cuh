@@ -5,24 +5,30 @@
 //   r[t] = sum_j wk[t, j] * softmax_n(read_temp * q_t . K_p[n]) @ V_p,   p = page_of[lib(t), idx[t, j]], n < n_valid
 //
 // The (row, routed chunk) pairs are grouped by page (count, scan, scatter); a tile is one page with up to MT of its
-// pairs, a unit one tile with up to 128 * cs of the page's slots. A cluster of cs CTAs computes a unit on the 5th
-// generation tensor cores:
-//   scores  CTA j: S[pairs, its slots] = Q . K^T over all of d_s (TMA tiles, f32 in TMEM);
-//   softmax rows' maxima exchanged through distributed shared memory, P = 2^(t - max) in 16 bits, CTA j's block of P
-//           sent to every CTA of the cluster (bulk copies between their shared memories, counted on an mbarrier);
-//   read    CTA j: O[pairs, its columns of d_s] = P . V (V as an MN-major operand), scaled by 1 / sum, stored per pair.
+// pairs, a unit one tile with up to 512 of the page's slots. A cluster of 4 CTAs (8 for d_s > 2048) computes a unit on
+// the 5th generation tensor cores, both products with the page as the 128-row operand and the pairs as its N:
+//   scores  CTA j: S^T[its slots, pairs] = K . Q^T over all of d_s (TMA tiles, f32 in TMEM);
+//   softmax the pairs' maxima exchanged through distributed shared memory, P = 2^(t - max) in 16 bits, CTA j's block of
+//           P sent to every CTA of the cluster (bulk copies between their shared memories, counted on an mbarrier);
+//   read    CTA j: O^T[its columns of d_s, pairs] = V^T . P^T (V as an MN-major operand), scaled by 1 / sum, stored per
+//           pair: a warp's lanes are consecutive columns, so the stores are whole lines.
 // The scores and the read walk the page differently (all columns of some slots, all slots of some columns), so the page
-// passes through shared memory twice, but its second pass comes from L2: a cluster holds one page at a time.
+// passes through shared memory twice, but its second pass comes from L2: a cluster holds one or two pages at a time.
+// The roles run one unit apart: the scores of the next unit are computed while this one's softmax and exchange run,
+// and the epilogue stores one unit while the next one's P is made.
 // shared_combine adds a row's pairs in the order of its routing: results do not depend on how pairs were grouped.
 //
-// Precision. The operands are 16-bit. TERMS = 2 (float32 outputs): q and P enter as hi + lo pairs stacked in the rows
-// of one MMA (hi above lo: the same instructions cover both), which keeps 22 bits with f16 slots and 16 with bf16;
-// the rows' halves are added in float32. TERMS = 1 (16-bit outputs): one rounding of q and of P, as the other
-// tensor-core reads do. q is scaled by a power of two per row and P by 2^14, so f16's range is no limit.
+// Why this orientation: with the pairs as the 128 rows (of which a tile fills 64) the read cost 290 cycles per
+// 16 slots x 256 columns (M = 128, N = 256, MN-major B), this way 2 x 81 (M = 128, N = 64).
+//
+// Precision. The operands are 16-bit. TERMS = 2 (float32 outputs): q and P enter as hi + lo pairs, two of the MMA's
+// N columns per pair, which keeps 22 bits with f16 slots and 16 with bf16; the halves are added in float32.
+// TERMS = 1 (16-bit outputs): one rounding of q and of P, as the other tensor-core reads do. q is scaled by a power of
+// two per row and P by 2^14, so f16's range is no limit.
 //
 // The tensor core's accumulator drops bits below its running value at every 16-term step, always towards zero; over
 // d_s = 2048 that is 128 steps, 1.2e-5 of a score near 1, which read_temp multiplies. With TERMS = 2 the scores are
-// therefore accumulated 128 columns of d_s at a time into a ring of TMEM buffers and added up in float32 registers.
+// therefore accumulated in four parts of d_s, in TMEM buffers of their own, and added up in float32 registers.
 //
 // Slots at or past n_valid never reach a result: their scores are masked, P is 0 there, and the rows of V behind the
 // tile's last valid slot are zeroed in shared memory (0 * NaN would not be 0).
@@ -35,25 +41,24 @@
 
 namespace xencb {
 
-constexpr int RS_AROWS = 64;      // rows of the A operands that carry data (TERMS * MT; the MMA's M is 128 whatever they
-                                  // are, and the other rows are not looked at)
-constexpr int RS_CS = 8;          // CTAs per cluster
-constexpr int RS_NS = 64;         // slots whose scores a CTA computes
-constexpr int RS_SEG = RS_CS * RS_NS;  // slots of a unit
-constexpr int RS_HW = RS_NS / 2;  // score columns of a softmax warp
-constexpr int RS_SLAB = 512;      // columns of d_s per CTA at most (TMEM)
-constexpr int RS_AHEAD_SLAB = 256;  // up to here the scores have TMEM columns of their own
-constexpr int RS_VROWS = 32;      // slots per stage of the read product
+constexpr int RS_N = 64;          // N of both products: TERMS * MT
+constexpr int RS_SEG = 512;       // slots of a unit
+constexpr int RS_MAX_CS = 8;      // CTAs per cluster: 4, or 8
+constexpr int RS_SLAB = 512;      // columns of d_s per CTA at most (4 x 64 TMEM columns)
+constexpr int RS_VROWS = 48;      // slots per stage of the read
 constexpr int RS_ACC = 4;         // score accumulators in TMEM
-constexpr int RS_CHUNK = 2;       // TERMS = 2: k-blocks per accumulator (8 accumulation steps)
+constexpr int RS_S_COL = 256;     // their first TMEM column (the read's sums lie below)
 constexpr float RS_P_SCALE = 16384.f;     // P is scaled by 2^14
-constexpr int RS_STAGE = 16384;   // scores: 64 rows of Q + 64 slots of K; read: 4 boxes of 32 slots x 64 columns
-constexpr int RS_STAGES = 9;
-constexpr int RS_PBLK = RS_AROWS * 128;   // P of 64 slots: one 128-byte swizzle row per A row
-constexpr int RS_STAT = 2 * 2 * RS_CS * RS_AROWS;  // floats: [2][16][MT]
-constexpr int RS_THREADS = 192;   // warps 0, 1, 4, 5: softmax and epilogue (TMEM lanes 0-63); 2: producer; 3: MMA
+constexpr int RS_KTILE = 128 * 128;       // K tile of a stage: up to 128 slots x 64 columns; Q's 64 rows behind it
+constexpr int RS_STAGE = RS_KTILE + RS_N * 128;  // scores; the read: 4 boxes of 48 slots x 64 columns
+constexpr int RS_STAGES = 6;
+constexpr int RS_PBLK = RS_N * 128;       // P of 64 slots: one 128-byte swizzle row per N row
+constexpr int RS_STAT = 2 * 16 * RS_N;    // floats: [2][16 groups of 32 slots][MT]
+constexpr int RS_SM_WARPS = 8;            // softmax: 4 TMEM lane quarters (32 slots each) x 2 halves of the pairs
+constexpr int RS_THREADS = 32 * 14;       // 0-7 softmax, 8-11 epilogue, 12 producer, 13 MMA
 constexpr size_t RS_SMEM = 1024 + 8 * RS_PBLK + (size_t)RS_STAGES * RS_STAGE + 2 * RS_STAT * 4 +
-                           (2 * RS_STAGES + 2 * RS_ACC + 5) * 8 + 16;
+                           (2 * RS_STAGES + 2 * RS_ACC + 6) * 8 + 16;
+static_assert(4 * RS_VROWS * 128 <= RS_STAGE, "a stage of the read fits");
 
 struct __align__(16) SharedTile {
   int page, start, count, nv;  // pairs [start, start + count) in grouped order; nv: the page's most valid slots
@@ -78,8 +83,7 @@ struct SharedArgs {
   int* pnv;        // [n_pairs] by position: valid slots
   float* qinv;     // [n_pairs] by position: 1 / (the row's power-of-two scale)
   // read
-  int segs, slab;
-  int ahead;       // the next unit's scores run before this unit's read (slab <= RS_AHEAD_SLAB)
+  int segs, cs, ns, slab;  // segments of a page; CTAs per cluster, slots and columns of d_s per CTA
   int v3d;         // V's map is 3-D: [64 columns][slots][blocks of 64 columns] (d_s a multiple of 64)
   float qscale;    // read_temp * log2(e), or 1
   int softmax;
@@ -295,25 +299,13 @@ __device__ __forceinline__ void bulk_s2s(uint32_t dst_cluster, const void* src, 
       : "memory");
 }
 
-// Two floats rounded to 16 bits in one instruction (x in the low half), and the rounded values.
-__device__ __forceinline__ uint32_t rs_pack(__half, float x, float y, float2& r) {
-  const __half2 h = __floats2half2_rn(x, y);
-  r = __half22float2(h);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t rs_pack(__nv_bfloat16, float x, float y, float2& r) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-  r = __bfloat1622float2(h);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // ----------------------------------------------------------------------------------------------------- read
 struct RsSmem {
-  unsigned char* p;       // [8 blocks][pblk]
+  unsigned char* p;       // [8 blocks of 64 slots][RS_PBLK]
   unsigned char* stages;  // the ring
-  float* smax;            // [2][2 * cs][MT]: by the parity of the unit (a CTA without scores may lag a unit behind)
-  float* ssum;            // [2][16][MT]: per 32 slots
-  uint64_t *full, *empty, *s_full, *s_empty, *p_full, *o_full, *o_empty, *stat, *sums;
+  float* smax;            // [2][16][MT]: by the parity of the unit, per 32 slots
+  float* ssum;            // [2][16][MT]
+  uint64_t *full, *empty, *s_full, *s_empty, *p_full, *o_full, *o_empty, *stat, *sums, *seen;
   uint32_t* tmem;
   volatile int* abort_flag;
 };
@@ -345,7 +337,8 @@ __device__ __forceinline__ RsSmem rs_smem(unsigned char* base) {
   s.o_empty = s.o_full + 1;
   s.stat = s.o_empty + 1;
   s.sums = s.stat + 1;
-  s.tmem = reinterpret_cast<uint32_t*>(s.sums + 1);
+  s.seen = s.sums + 1;
+  s.tmem = reinterpret_cast<uint32_t*>(s.seen + 1);
   s.abort_flag = reinterpret_cast<volatile int*>(s.tmem + 1);
   return s;
 }
@@ -365,26 +358,47 @@ struct RsUnit {
   }
 };
 
+// Reduction over a warp's 32 lanes of N values a lane (N = 16 or 32): lane l returns the reduced value l % N. Each
+// step exchanges half of the values that are left: N - 1 shuffles (one more for N = 16) in place of 5 N.
+template <int N, typename F>
+__device__ __forceinline__ float rs_reduce(const float (&v)[N], int lane, F op) {
+  float a[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) a[i] = v[i];
+#pragma unroll
+  for (int o = N / 2; o > 0; o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float send = up ? a[i] : a[i + o], keep = up ? a[i + o] : a[i];
+      a[i] = op(keep, __shfl_xor_sync(0xffffffffu, send, o));
+    }
+  }
+  if (N == 16) a[0] = op(a[0], __shfl_xor_sync(0xffffffffu, a[0], 16));
+  return a[0];
+}
+
 template <typename T, int TERMS>
 __global__ void __launch_bounds__(RS_THREADS, 1)
     shared_read_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_q8,
                        const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        const SharedArgs a) {
-  constexpr int MT = RS_AROWS / TERMS;                // pairs per tile
+  constexpr int MT = RS_N / TERMS;                    // pairs per tile
+  constexpr int PP = MT / 2;                          // pairs of a softmax warp
   constexpr int FMT = std::is_same<T, __half>::value ? UMMA_F16 : UMMA_BF16;
-  constexpr int CQ = 2 / TERMS;                       // TMEM lane quarters of the hi terms
-  constexpr int CW = 2 * CQ, AW = 4;                  // warps that do the softmax; that read TMEM
   extern __shared__ unsigned char rs_smem_raw[];
   const RsSmem s = rs_smem(reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(rs_smem_raw) + 1023) &
                                                             ~uintptr_t(1023)));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cs = a.cs, ns = a.ns;
   const int rank = (int)cluster_rank();
-  const int cluster = blockIdx.x / RS_CS, n_clusters = gridDim.x / RS_CS;
+  const int cluster = blockIdx.x / cs, n_clusters = gridDim.x / cs;
   const int nkb = (a.d_s + 63) / 64;
-  const int kpc = TERMS == 2 ? RS_CHUNK : nkb;                     // k-blocks per score accumulator
+  const int kpc = TERMS == 2 ? max(2, (nkb + RS_ACC - 1) / RS_ACC) : nkb;  // k-blocks per score accumulator
   const int x0 = rank * a.slab;                                    // this CTA's columns of d_s
   const int my_boxes = max(0, min(a.slab, a.d_s - x0) + 63) / 64;  // in boxes of 64
-  const uint32_t s_col = a.ahead ? RS_AHEAD_SLAB : 0;              // TMEM columns of the scores
+  const int quarters = ns / 32;                                    // of the TMEM lanes hold slots
+  const int sm_warps = 2 * quarters;
 
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_q);
@@ -397,17 +411,18 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
     }
     for (int i = 0; i < RS_ACC; ++i) {
       mbar_init(&s.s_full[i], 1);
-      mbar_init(&s.s_empty[i], AW);
+      mbar_init(&s.s_empty[i], sm_warps);
     }
     mbar_init(s.p_full, 1);
     mbar_init(s.o_full, 1);
-    mbar_init(s.o_empty, AW);
-    mbar_init(s.stat, RS_CS * CW);
-    mbar_init(s.sums, RS_CS * CW);
+    mbar_init(s.o_empty, 4);
+    mbar_init(s.stat, cs * sm_warps);
+    mbar_init(s.sums, cs * sm_warps);
+    mbar_init(s.seen, 4);
     *s.abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 3) {
+  if (warp == 13) {
     tc_alloc(s.tmem, 512);
     tc_relinquish();
   }
@@ -420,31 +435,36 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
   const int n_units = *a.n_tiles * a.segs;
   RsUnit cur, nxt;
   cur.find(a, cluster, n_units, n_clusters);
+  // A wait that runs out sets the abort flag; from then on the softmax and epilogue warps wait for nothing and run
+  // through their units on whatever is there, so that the named barrier stays matched.
+  auto done = [&](bool arrived) {
+    if (!arrived) *s.abort_flag = 1;
+  };
 
-  if (warp == 2) {
+  if (warp == 12) {
     // --------------------------------------------------------------------------------------------- producer
     if (elect_one()) {
       RsRing ring{0, 0};
       uint32_t used = 0;
       bool ok = true;
       auto scores = [&](const RsUnit& w) {
-        if (w.u >= n_units || rank * RS_NS >= w.nv) return;
-        const int y = w.t.page * a.page_rows + w.seg0 + rank * RS_NS;
+        if (w.u >= n_units || rank * ns >= w.nv) return;
+        const int y = w.t.page * a.page_rows + w.seg0 + rank * ns;
         const bool few = w.t.count <= 8;  // eight rows of Q a term; what lies in the others is not looked at
-        const uint32_t tx = (uint32_t)((few ? 8 : MT) * TERMS + RS_NS) * 128;
+        const uint32_t tx = (uint32_t)((few ? 8 : MT) * TERMS + ns) * 128;
         for (int kb = 0; kb < nkb && ok; ++kb) {
           if (used >= RS_STAGES) ok = mbar_wait_spin(&s.empty[ring.st], ring.phase ^ 1);
           if (!ok) break;
           uint64_t* bar = &s.full[ring.st];
           unsigned char* st = s.stages + ring.st * RS_STAGE;
           mbar_arrive_expect_tx(bar, tx);
-          tma_load_2d(st + RS_AROWS * 128, &map_k, kb * 64, y, bar);
+          tma_load_2d(st, &map_k, kb * 64, y, bar);
           if (few) {
 #pragma unroll
             for (int x = 0; x < TERMS; ++x)
-              tma_load_2d(st + x * MT * 128, &map_q8, kb * 64, x * a.n_pairs + w.t.start, bar);
+              tma_load_2d(st + RS_KTILE + x * MT * 128, &map_q8, kb * 64, x * a.n_pairs + w.t.start, bar);
           } else {
-            tma_load_3d(st, &map_q, kb * 64, w.t.start, 0, bar);
+            tma_load_3d(st + RS_KTILE, &map_q, kb * 64, w.t.start, 0, bar);
           }
           ring.next(RS_STAGES);
           ++used;
@@ -472,9 +492,8 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
       scores(cur);
       while (cur.u < n_units && ok) {
         nxt.find(a, cur.u + n_clusters, n_units, n_clusters);
-        if (a.ahead) scores(nxt);
+        scores(nxt);
         values(cur);
-        if (!a.ahead) scores(nxt);
         cur = nxt;
       }
       if (!ok) *s.abort_flag = 1;
@@ -485,19 +504,20 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
       }
     }
     __syncwarp();
-  } else if (warp == 3) {
+  } else if (warp == 13) {
     // --------------------------------------------------------------------------------------------- MMA issuer
     if (elect_one()) {
       RsRing ring{0, 0};
       uint32_t unit = 0, acc = 0;
       bool ok = true;
-      const uint32_t id_s = umma_idesc(FMT, FMT, 128, RS_NS);
+      const uint32_t id_s = umma_idesc(FMT, FMT, 128, RS_N);
+      const uint32_t id_o = umma_idesc(FMT, FMT, 128, RS_N) | (1u << 15);  // A (V) is MN-major
       // operand descriptors: the constant part, and addresses in 16-byte units (14 bits: the address of a CTA's shared
       // memory carries its cluster rank above them)
       const uint64_t dk = umma_desc_k_sw128(0), dv = umma_desc_mn_sw128(0, RS_VROWS * 128);
       const uint32_t st0 = (smem_u32(s.stages) >> 4) & 0x3FFFu, p0 = (smem_u32(s.p) >> 4) & 0x3FFFu;
       auto scores = [&](const RsUnit& w) {
-        if (w.u >= n_units || rank * RS_NS >= w.nv) return;
+        if (w.u >= n_units || rank * ns >= w.nv) return;
         for (int k0 = 0; k0 < nkb && ok; k0 += kpc, ++acc) {
           const uint32_t buf = acc % RS_ACC, use = acc / RS_ACC;
           if (use > 0 && !(ok = mbar_wait_spin(&s.s_empty[buf], (use - 1) & 1))) break;
@@ -506,10 +526,10 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
           for (int kb = k0; kb < k1; ++kb) {
             if (!(ok = mbar_wait_spin(&s.full[ring.st], ring.phase))) break;
             tc_fence_after();
-            const uint64_t da = dk + (st0 + ring.st * (RS_STAGE / 16)), db = da + RS_AROWS * 8;
+            const uint64_t da = dk + (st0 + ring.st * (RS_STAGE / 16)), db = da + RS_KTILE / 16;
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
-              tc_mma<0>(taddr + s_col + buf * RS_NS, da + ks * 2, db + ks * 2, id_s, kb > k0 || ks > 0);
+              tc_mma<0>(taddr + RS_S_COL + buf * RS_N, da + ks * 2, db + ks * 2, id_s, kb > k0 || ks > 0);
             tc_commit(&s.empty[ring.st]);
             ring.next(RS_STAGES);
           }
@@ -518,13 +538,8 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
         }
       };
       auto values = [&](const RsUnit& w) {
-        // every CTA's block of P is here (and this CTA's softmax warps have read the scores)
-        if (!(ok = ok && mbar_wait_cluster(s.p_full, unit & 1))) return;
-        tc_fence_after();
         for (int b = 0; b < (w.nv + RS_VROWS - 1) / RS_VROWS && ok; ++b) {
           const int left = w.nv - b * RS_VROWS, steps = min(RS_VROWS / 16, (left + 15) / 16);
-          // slots [b * 32, b * 32 + 32) of P: half a block of 64
-          const uint64_t dp = dk + (p0 + (b / 2) * (RS_PBLK / 16) + (b & 1) * 4);
           for (int h = 0; h < my_boxes; h += 4) {
             const int n = min(4, my_boxes - h);
             if (!(ok = mbar_wait_spin(&s.full[ring.st], ring.phase))) break;
@@ -537,9 +552,14 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
               fence_proxy_async_smem();
             }
             const uint64_t dx = dv + (st0 + ring.st * (RS_STAGE / 16));
-            const uint32_t id = umma_idesc(FMT, FMT, 128, n * 64, 1);
-            for (int ks = 0; ks < steps; ++ks)
-              tc_mma<0>(taddr + (uint32_t)h * 64, dp + ks * 2, dx + ks * 128, id, b > 0 || ks > 0);
+            for (int ks = 0; ks < steps; ++ks) {
+              const int slot = b * RS_VROWS + ks * 16;  // its 16 slots of P lie in one block of 64
+              const uint64_t dp = dk + (p0 + (slot >> 6) * (RS_PBLK / 16) + ((slot & 63) >> 3));
+              // columns [128 t, 128 t + 128) of the slab: two boxes (the second may be stale: lanes nobody reads)
+              for (int t = 0; t < (n + 1) / 2; ++t)
+                tc_mma<0>(taddr + (uint32_t)(h / 2 + t) * RS_N, dx + t * (2 * RS_VROWS * 128 / 16) + ks * 128, dp, id_o,
+                          b > 0 || ks > 0);
+            }
             tc_commit(&s.empty[ring.st]);
             ring.next(RS_STAGES);
           }
@@ -547,210 +567,201 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
         if (ok) tc_commit(s.o_full);
         ++unit;
       };
-      // the epilogue of the unit before has read its sums: they may be overwritten, by the read or (where they share
-      // columns) by the scores
-      auto drained = [&](uint32_t units) {
-        if (units > 0 && ok) ok = mbar_wait_spin(s.o_empty, (units - 1) & 1);
-        tc_fence_after();
-      };
       scores(cur);
       while (cur.u < n_units && ok) {
         nxt.find(a, cur.u + n_clusters, n_units, n_clusters);
-        if (a.ahead) {
-          scores(nxt);
-          drained(unit);
-          if (ok) values(cur);
-        } else {
-          values(cur);
-          if (nxt.u < n_units) drained(unit);
-          if (ok) scores(nxt);
-        }
+        scores(nxt);
+        // the epilogue of the unit before has read its sums, and every CTA's block of P is here
+        if (ok && unit > 0) ok = mbar_wait_spin(s.o_empty, (unit - 1) & 1);
+        if (ok) ok = mbar_wait_cluster(s.p_full, unit & 1);
+        tc_fence_after();
+        if (ok) values(cur);
         cur = nxt;
       }
       if (!ok) *s.abort_flag = 1;
     }
     __syncwarp();
-  } else {
-    // --------------------------------------------------------------------------------------------- softmax, epilogue
+  } else if (warp < RS_SM_WARPS) {
+    // --------------------------------------------------------------------------------------------- softmax
+    // Lane = slot, registers = this warp's pairs.
     const int quarter = warp & 3, half = warp >> 2;
-    const int term = quarter / CQ;                                           // 0: hi rows, which do the softmax
-    const int row = (quarter % CQ) * 32 + lane;                              // pair of the tile
-    const uint32_t tl = taddr + ((uint32_t)(quarter * 32) << 16);
-    const int pair_bar = 2 + half;                                           // TERMS = 2: a hi warp and its lo warp
-    const int c0 = rank * RS_NS + half * RS_HW;                              // first slot of this warp's columns
-    // scratch of the lo -> hi hand-over, [32 columns][32 rows] twice: the block of P that belongs to another CTA (no
-    // copy reads it, and none arrives before this CTA's maxima of the unit are out)
-    float* xch = reinterpret_cast<float*>(s.p + (size_t)((rank + 1 + half) % RS_CS) * RS_PBLK);
-    uint32_t unit = 0, acc = 0;
-    // A wait that runs out sets the abort flag; from then on nothing is waited for, and the warps run through their
-    // units on whatever is there, so that the named barriers they share stay matched.
-    auto done = [&](bool arrived) {
-      if (!arrived) *s.abort_flag = 1;
-    };
-    float v[RS_HW];
-    auto scores = [&](const RsUnit& w) {  // this warp's 32 columns of the scores, added up over the accumulators
-      if (w.u >= n_units || rank * RS_NS >= w.nv) return;
-      for (int k0 = 0; k0 < nkb; k0 += kpc, ++acc) {
-        const uint32_t buf = acc % RS_ACC;
-        done(*s.abort_flag || mbar_wait_spin(&s.s_full[buf], (acc / RS_ACC) & 1));
-        tc_fence_after();
-        float x[RS_HW];
-        tc_ld32(tl + s_col + buf * RS_NS + (uint32_t)(half * RS_HW), x);
+    if (quarter < quarters) {
+      const uint32_t tl = taddr + ((uint32_t)(quarter * 32) << 16) + RS_S_COL + (uint32_t)(half * PP);
+      const int slot0 = rank * ns + quarter * 32;              // lane 0's slot of the segment
+      const int group = slot0 >> 5;                            // 32 slots: their entry of smax and ssum
+      // P: this CTA's block of the slot; 16-byte chunk j of row r at chunk j ^ (r % 8)
+      const int in_blk = (quarter * 32 + lane) & 63;
+      unsigned char* const pcol = s.p + (size_t)(rank * (ns / 64) + (quarter >> 1)) * RS_PBLK + (in_blk & 7) * 2;
+      uint32_t unit = 0, acc = 0;
+      float v[PP];
+      auto scores = [&](const RsUnit& w) {
+        if (w.u >= n_units || rank * ns >= w.nv) return;
+        for (int k0 = 0; k0 < nkb; k0 += kpc, ++acc) {
+          const uint32_t buf = acc % RS_ACC;
+          done(*s.abort_flag || mbar_wait_spin(&s.s_full[buf], (acc / RS_ACC) & 1));
+          tc_fence_after();
+          float x[PP];
+          if constexpr (TERMS == 2) {
+            float y[PP];
+            tc_ld16(tl + buf * RS_N, x);
+            tc_ld16(tl + buf * RS_N + MT, y);
 #pragma unroll
-        for (int i = 0; i < RS_HW; ++i) v[i] = k0 == 0 ? x[i] : v[i] + x[i];
-        tc_fence_before();
+            for (int i = 0; i < PP; ++i) x[i] += y[i];
+          } else {
+            tc_ld32(tl + buf * RS_N, x);
+          }
+#pragma unroll
+          for (int i = 0; i < PP; ++i) v[i] = k0 == 0 ? x[i] : v[i] + x[i];
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s.s_empty[buf]);
+        }
+      };
+      scores(cur);
+      while (cur.u < n_units) {
+        nxt.find(a, cur.u + n_clusters, n_units, n_clusters);
+        const SharedTile t = cur.t;
+        const bool mine = rank * ns < cur.nv;
+        const int count = t.count - half * PP;                 // this warp's pairs of the tile (may be <= 0)
+        float* smax = s.smax + (unit & 1) * 16 * MT + half * PP;
+        float* ssum = s.ssum + (unit & 1) * 16 * MT + half * PP;
+        // lane i holds pair i's valid slots (from this warp's first) and scale
+        const int me = lane & (PP - 1);
+        const int pos = t.start + half * PP + me;
+        const int lim = me < count ? a.pnv[pos] - cur.seg0 - slot0 : 0;
+        const float c = me < count ? a.qinv[pos] * a.qscale : 0.f;
+        // t = scores * scale; masked slots -inf (softmax) or 0 (linear read). A pair whose every score is masked gets max
+        // -inf and then NaN weights: it has no slot in this segment, so nothing reads them.
+        const float none = a.softmax ? -CUDART_INF_F : 0.f;
+        float mx = none;
+        if (mine) {
+          float w[PP];
+#pragma unroll
+          for (int i = 0; i < PP; ++i) {
+            const float ci = __shfl_sync(0xffffffffu, c, i);
+            const int li = __shfl_sync(0xffffffffu, lim, i);
+            v[i] = lane < li ? v[i] * ci : none;
+            w[i] = a.softmax ? v[i] : fabsf(v[i]);
+          }
+          mx = rs_reduce<PP>(w, lane, [](float p, float q) { return fmaxf(p, q); });
+        }
+        // the read of the unit before is done with P, and its epilogue with the maxima and sums two units back
+        if (unit > 0) {
+          done(*s.abort_flag || mbar_wait_spin(s.o_full, (unit - 1) & 1));
+          done(*s.abort_flag || mbar_wait_spin(s.seen, (unit - 1) & 1));
+        }
+        // the pairs' maxima over these 32 slots to every CTA of the cluster
+        if (lane < PP)
+          for (int r = 0; r < cs; ++r) st_cluster_f32(cluster_map(&smax[group * MT + lane], r), mx);
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s.s_empty[buf]);
+        if (lane < cs) mbar_arrive_cluster(cluster_map(s.stat, lane));
+        done(*s.abort_flag || mbar_wait_cluster(s.stat, unit & 1));
+        float l = 0.f;
+        if (mine) {
+          float m = none;
+#pragma unroll
+          for (int g = 0; g < 16; ++g) m = fmaxf(m, smax[g * MT + me]);
+          const float lin = a.softmax ? 0.f : f16_range_scale(m);
+#pragma unroll
+          for (int i = 0; i < PP; ++i) {
+            if (i < count) {
+              const float mi = __shfl_sync(0xffffffffu, a.softmax ? m : lin, i);
+              v[i] = a.softmax ? RS_P_SCALE * pf_exp2(v[i] - mi) : v[i] * mi;
+              const int r = half * PP + i;
+              unsigned char* at = pcol + r * 128 + (((in_blk >> 3) ^ (r & 7)) << 4);
+              const T hi = from_f32<T>(v[i]);
+              *reinterpret_cast<T*>(at) = hi;
+              if (TERMS == 2) *reinterpret_cast<T*>(at + MT * 128) = from_f32<T>(v[i] - to_f32(hi));
+            }
+          }
+          fence_proxy_async_smem();
+          if (a.softmax) l = rs_reduce<PP>(v, lane, [](float p, float q) { return p + q; });
+        }
+        named_bar_sync(1, 32 * sm_warps);
+        if (warp == 0 && lane == 0) {
+          // the other CTAs' blocks are still to come; then this CTA's block to them
+          const uint32_t bytes = (uint32_t)(ns / 64) * RS_PBLK;
+          const int n_work = min(cs, (cur.nv + ns - 1) / ns);
+          mbar_arrive_expect_tx(s.p_full, (uint32_t)(n_work - (mine ? 1 : 0)) * bytes);
+          if (mine && !*s.abort_flag)
+            for (int r = 1; r < cs; ++r) {
+              const uint32_t to = (uint32_t)((rank + r) % cs);
+              unsigned char* src = s.p + (size_t)rank * bytes;
+              bulk_s2s(cluster_map(src, to), src, bytes, cluster_map(s.p_full, to));
+            }
+        }
+        __syncwarp();
+        if (lane < PP)
+          for (int r = 0; r < cs; ++r) st_cluster_f32(cluster_map(&ssum[group * MT + lane], r), l);
+        __syncwarp();
+        if (lane < cs) mbar_arrive_cluster(cluster_map(s.sums, lane));
+        scores(nxt);
+        ++unit;
+        cur = nxt;
       }
-    };
-    scores(cur);
+    }
+  } else {
+    // --------------------------------------------------------------------------------------------- epilogue
+    // Lane = column of d_s, registers = pairs.
+    const int quarter = warp & 3;
+    uint32_t unit = 0;
     while (cur.u < n_units) {
       nxt.find(a, cur.u + n_clusters, n_units, n_clusters);
       const SharedTile t = cur.t;
-      const int seg = cur.u % a.segs, seg0 = cur.seg0, nv = cur.nv;
-      const bool mine = rank * RS_NS < nv;
-      float* smax = s.smax + (unit & 1) * 2 * RS_CS * MT;
-      float* ssum = s.ssum + (unit & 1) * 2 * RS_CS * MT;
-      const bool live = row < t.count;
-      const int pos = t.start + (live ? row : 0);
-      const int pnv = live ? a.pnv[pos] - seg0 : 0;            // the pair's valid slots in this segment
-      if (TERMS == 2 && mine) {
-        if (term == 1)
+      const int seg = cur.u % a.segs;
+      const float* smax = s.smax + (unit & 1) * 16 * MT;
+      const float* ssum = s.ssum + (unit & 1) * 16 * MT;
+      done(*s.abort_flag || mbar_wait_cluster(s.sums, unit & 1));
+      float coef[MT / 32];  // lane i: pairs i and (TERMS = 1) 32 + i
 #pragma unroll
-          for (int i = 0; i < RS_HW; ++i) xch[i * 32 + lane] = v[i];
-        fence_proxy_async_smem();  // before another CTA's copy may land on the scratch
-        named_bar_sync(pair_bar, 64);
-        if (term == 0)
-#pragma unroll
-          for (int i = 0; i < RS_HW; ++i) v[i] += xch[i * 32 + lane];
-      }
-      if (term == 0) {
-        // t = scores * scale; masked slots -inf (softmax) or 0 (linear read). A row whose every score is masked gets
-        // max -inf and then NaN weights: it has no slot in this segment, so nothing reads them.
-        const float c = live ? a.qinv[pos] * a.qscale : 0.f;
-        const int lim = pnv - c0;
-        float mx = a.softmax ? -CUDART_INF_F : 0.f;
-        if (mine && a.softmax) {
-#pragma unroll
-          for (int i = 0; i < RS_HW; ++i) {
-            v[i] = i < lim ? v[i] * c : -CUDART_INF_F;
-            mx = fmaxf(mx, v[i]);
-          }
-        } else if (mine) {
-#pragma unroll
-          for (int i = 0; i < RS_HW; ++i) {
-            v[i] = i < lim ? v[i] * c : 0.f;
-            mx = fmaxf(mx, fabsf(v[i]));
-          }
-        }
-        // the rows' maxima to every CTA of the cluster
-#pragma unroll
-        for (int r = 0; r < RS_CS; ++r) st_cluster_f32(cluster_map(&smax[(rank * 2 + half) * MT + row], r), mx);
-        __syncwarp();
-        if (lane < RS_CS) mbar_arrive_cluster(cluster_map(s.stat, lane));
-        done(*s.abort_flag || mbar_wait_cluster(s.stat, unit & 1));
-        float m = a.softmax ? -CUDART_INF_F : 0.f;
-#pragma unroll
-        for (int r = 0; r < 2 * RS_CS; ++r) m = fmaxf(m, smax[r * MT + row]);
-        float l = 0.f;
-        if (mine) {
-          if (a.softmax) {
-            float l4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < RS_HW; ++i) {
-              v[i] = RS_P_SCALE * pf_exp2(v[i] - m);
-              l4[i & 3] += v[i];
-            }
-            l = (l4[0] + l4[1]) + (l4[2] + l4[3]);
-          } else {
-            const float lin = f16_range_scale(m);
-#pragma unroll
-            for (int i = 0; i < RS_HW; ++i) v[i] *= lin;
-          }
-          // this row's P in 16 bits: this CTA's block, 16-byte chunk j of A row r at chunk j ^ (r % 8)
-          unsigned char* blk = s.p + (size_t)rank * RS_PBLK;
-#pragma unroll
-          for (int j = 0; j < RS_HW / 8; ++j) {
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x = v[j * 8 + 2 * e], y = v[j * 8 + 2 * e + 1];
-              float2 r, r2;
-              hi[e] = rs_pack(T{}, x, y, r);
-              if (TERMS == 2) lo[e] = rs_pack(T{}, x - r.x, y - r.y, r2);
-            }
-            const int ch = (half * 4 + j) ^ (row & 7);  // (MT is a multiple of 8: the same for the lo row)
-            *reinterpret_cast<uint4*>(blk + row * 128 + ch * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            if (TERMS == 2)
-              *reinterpret_cast<uint4*>(blk + (MT + row) * 128 + ch * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-          }
-          fence_proxy_async_smem();
-        }
-        tc_fence_before();
-        named_bar_sync(1, 32 * CW);
-        if (warp == 0 && lane == 0) {
-          // the other CTAs' blocks are still to come; then this CTA's block to them
-          const int n_work = min(RS_CS, (nv + RS_NS - 1) / RS_NS);
-          mbar_arrive_expect_tx(s.p_full, (uint32_t)(n_work - (mine ? 1 : 0)) * RS_PBLK);
-          if (mine && !*s.abort_flag)
-            for (int r = 1; r < RS_CS; ++r) {
-              const uint32_t to = (uint32_t)((rank + r) % RS_CS);
-              unsigned char* src = s.p + (size_t)rank * RS_PBLK;
-              bulk_s2s(cluster_map(src, to), src, RS_PBLK, cluster_map(s.p_full, to));
-            }
-        }
-        __syncwarp();
-#pragma unroll
-        for (int r = 0; r < RS_CS; ++r) st_cluster_f32(cluster_map(&ssum[(rank * 2 + half) * MT + row], r), l);
-        __syncwarp();
-        if (lane < RS_CS) mbar_arrive_cluster(cluster_map(s.sums, lane));
-      }
-      if (a.ahead) scores(nxt);
-      // ------------------------------------------------------------------------------------- epilogue
-      float coef = 0.f;
-      if (term == 0) {
-        done(*s.abort_flag || mbar_wait_cluster(s.sums, unit & 1));
+      for (int g = 0; g < MT / 32; ++g) {
+        const int i = g * 32 + lane;
         float m = a.softmax ? -CUDART_INF_F : 0.f, l = 0.f;
 #pragma unroll
-        for (int r = 0; r < 2 * RS_CS; ++r) {
-          m = fmaxf(m, smax[r * MT + row]);
-          l += ssum[r * MT + row];
+        for (int e = 0; e < 16; ++e) {
+          m = fmaxf(m, smax[e * MT + i]);
+          l += ssum[e * MT + i];
         }
-        if (a.softmax) coef = l != 0.f ? 1.f / l : 0.f;
-        else coef = pnv + seg0 > 0 ? rsqrtf((float)(pnv + seg0)) / f16_range_scale(m) : 0.f;
-        if (live && rank == 0 && half == 0) a.ml[(int64_t)pos * a.segs + seg] = make_float2(m, l);
+        coef[g] = 0.f;
+        if (i < t.count) {
+          const int64_t pos = t.start + i;
+          if (a.softmax) coef[g] = l != 0.f ? 1.f / l : 0.f;
+          else coef[g] = rsqrtf((float)a.pnv[pos]) / f16_range_scale(m);
+          if (rank == 0 && warp == 8) a.ml[pos * a.segs + seg] = make_float2(m, l);
+        }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s.seen);
       done(*s.abort_flag || mbar_wait_spin(s.o_full, unit & 1));
       tc_fence_after();
-      float* dst = a.part + ((int64_t)pos * a.segs + seg) * a.d_s + x0;
-      // the two halves of the warps take alternate passes of 32 columns. The lo rows' parts go through the scratch, its
-      // two buffers in turn: one barrier a pass separates a write from the read two passes before
-      for (int q0 = half * 32, turn = 0; q0 < my_boxes * 64; q0 += 64, turn ^= 1) {
-        float o[32];
-        tc_ld32(tl + (uint32_t)q0, o);
-        if (TERMS == 2) {
-          float* x = xch + turn * 32 * 32;
-          if (term == 1)
+      for (int b = 0; b < (my_boxes + 1) / 2; ++b) {
+        const int x = b * 128 + quarter * 32 + lane;  // column of the slab
+        const bool in = x < a.slab && x0 + x < a.d_s;
+        float* dst = a.part + ((int64_t)t.start * a.segs + seg) * a.d_s + x0 + x;
+        const uint32_t at = taddr + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * RS_N);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i * 32 + lane] = o[i];
-          named_bar_sync(pair_bar, 64);
-          if (term == 0)
+        for (int g = 0; g < MT / 32; ++g) {
+          if (g * 32 >= t.count) break;
+          float o[32];
+          tc_ld32(at + g * 32, o);
+          if constexpr (TERMS == 2) {
+            float y[32];
+            tc_ld32(at + 32, y);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] += x[i * 32 + lane];
-        }
-        if (term == 0 && live) {
+            for (int i = 0; i < 32; ++i) o[i] += y[i];
+          }
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            if (x0 + q0 + i < a.d_s)
-              *reinterpret_cast<float4*>(dst + q0 + i) =
-                  make_float4(o[i] * coef, o[i + 1] * coef, o[i + 2] * coef, o[i + 3] * coef);
+          for (int i = 0; i < 32; ++i) {
+            if (g * 32 + i < t.count) {
+              const float ci = __shfl_sync(0xffffffffu, coef[g], i);
+              if (in) dst[(int64_t)(g * 32 + i) * a.segs * a.d_s] = o[i] * ci;
+            }
+          }
         }
       }
       tc_fence_before();
-      if (TERMS == 2) named_bar_sync(pair_bar, 64);  // the scratch is read before the next unit's scores go there
       __syncwarp();
       if (lane == 0) mbar_arrive(s.o_empty);
-      if (!a.ahead) scores(nxt);
       ++unit;
       cur = nxt;
     }
@@ -759,7 +770,7 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
   __syncthreads();
   cluster_sync_all();  // no CTA leaves while another may still write to its shared memory
   tc_fence_after();
-  if (warp == 3) tc_dealloc(taddr, 512);
+  if (warp == 13) tc_dealloc(taddr, 512);
 }
 
 // ----------------------------------------------------------------------------------------------------- combine

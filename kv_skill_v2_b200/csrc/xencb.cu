@@ -714,7 +714,7 @@ int plan_build(int n_chunks, int d_s, int page_rows, BuildPlan* p) {
 
 // ------------------------------------------------------------------------------------------------ shared read plan
 struct SharedPlan {
-  int terms, slab, segs, mt;
+  int terms, cs, ns, slab, segs, mt;
   int64_t n_pairs, max_tiles;
   size_t cnt, pair, tiles, q, part, ml, total;  // bytes of each workspace part
 };
@@ -726,16 +726,18 @@ int plan_shared(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows, 
   if (slots_dtype != XENCB_F16 && slots_dtype != XENCB_BF16)
     return fail(XENCB_ENOTSUP, "read_shared: the tensor-core read takes f16 / bf16 slots");
   if (!elem_size(out_dtype)) return fail(XENCB_EINVAL, "read_shared: out_dtype %d unknown", out_dtype);
-  if (d_s % 8 != 0 || d_s > RS_SLAB * RS_CS)
-    return fail(XENCB_ENOTSUP, "read_shared: d_s=%d must be a multiple of 8, at most %d", d_s, RS_SLAB * RS_CS);
+  if (d_s % 8 != 0 || d_s > RS_SLAB * RS_MAX_CS)
+    return fail(XENCB_ENOTSUP, "read_shared: d_s=%d must be a multiple of 8, at most %d", d_s, RS_SLAB * RS_MAX_CS);
   if (n_rows > INT32_MAX / k || 2 * n_rows * k + 64 > INT32_MAX)
     return fail(XENCB_ENOTSUP, "read_shared: %lld rows x %d routed chunks are too many", (long long)n_rows, k);
   if (n_pages * (int64_t)page_rows + 1024 > INT32_MAX)
     return fail(XENCB_ENOTSUP, "read_shared: the slot pool is too large for 32-bit TMA coordinates");
   p->n_pairs = n_rows * k;
   p->terms = out_dtype == XENCB_F32 ? 2 : 1;
-  p->mt = RS_AROWS / p->terms;
-  p->slab = (int)align_up((size_t)(d_s + RS_CS - 1) / RS_CS, 64);
+  p->mt = RS_N / p->terms;
+  p->cs = d_s <= 4 * RS_SLAB ? 4 : 8;
+  p->ns = RS_SEG / p->cs;
+  p->slab = (int)align_up((size_t)(d_s + p->cs - 1) / p->cs, 64);
   p->segs = (page_rows + RS_SEG - 1) / RS_SEG;
   if (p->n_pairs * p->segs > INT32_MAX)
     return fail(XENCB_ENOTSUP, "read_shared: page_rows=%d is too long for this many rows", page_rows);
@@ -750,34 +752,35 @@ int plan_shared(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows, 
   return XENCB_OK;
 }
 
-// Clusters of the read kernel that fit the device at once, per device and kernel.
+// Clusters of the read kernel that fit the device at once, per device, cluster size and kernel.
 template <typename K>
-int shared_clusters(K kern, int* out) {
+int shared_clusters(K kern, int cs, int* out) {
   static std::mutex mu;
-  static std::unordered_map<const void*, int> known[kMaxDev];
+  static std::unordered_map<const void*, int> known[kMaxDev][RS_MAX_CS + 1];
   int dev = 0;
   cudaGetDevice(&dev);
   std::lock_guard<std::mutex> lk(mu);
-  const auto itr = known[dev].find(reinterpret_cast<const void*>(kern));
-  if (itr != known[dev].end()) {
+  auto& seen = known[dev][cs];
+  const auto itr = seen.find(reinterpret_cast<const void*>(kern));
+  if (itr != seen.end()) {
     *out = itr->second;
     return XENCB_OK;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(RS_CS);
+  cfg.gridDim = dim3((unsigned)cs);
   cfg.blockDim = dim3(RS_THREADS);
   cfg.dynamicSmemBytes = RS_SMEM;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = RS_CS;
+  at[0].val.clusterDim.x = (unsigned)cs;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
   int n = 0;
   const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
   if (e != cudaSuccess) return cuda_fail(e, "read_shared: cudaOccupancyMaxActiveClusters");
-  if (n <= 0) return fail(XENCB_ENOTSUP, "read_shared: no cluster of %d CTAs fits this device", RS_CS);
-  known[dev][reinterpret_cast<const void*>(kern)] = n;
+  if (n <= 0) return fail(XENCB_ENOTSUP, "read_shared: no cluster of %d CTAs fits this device", cs);
+  seen[reinterpret_cast<const void*>(kern)] = n;
   *out = n;
   return XENCB_OK;
 }
@@ -792,7 +795,7 @@ int run_shared(const void* q, int q_dtype, const SharedPlan& p, SharedArgs a, co
   const uint64_t np = (uint64_t)p.n_pairs;
   int rc = tensor_map_3d(&mq, dt, q16, {d, np, (uint64_t)TERMS}, {d * 2, np * d * 2}, {64, (uint32_t)p.mt, TERMS});
   if (!rc) rc = tensor_map_2d(&mq8, dt, 2, q16, d, (uint64_t)TERMS * p.n_pairs, d * 2, 64, 8);
-  if (!rc) rc = tensor_map_2d(&mk, dt, 2, slots, d, pool_rows, d * 2, 64, RS_NS);
+  if (!rc) rc = tensor_map_2d(&mk, dt, 2, slots, d, pool_rows, d * 2, 64, (uint32_t)p.ns);
   const void* v = vslots ? vslots : slots;
   a.v3d = a.d_s % 64 == 0;
   if (!rc && a.v3d) rc = tensor_map_3d(&mv, dt, v, {64, pool_rows, d / 64}, {d * 2, 128}, {64, RS_VROWS, 4});
@@ -800,7 +803,7 @@ int run_shared(const void* q, int q_dtype, const SharedPlan& p, SharedArgs a, co
   auto kern = shared_read_kernel<T, TERMS>;
   if (!rc) rc = ensure_smem(kern, (int)RS_SMEM);
   int n_clusters = 0;
-  if (!rc) rc = shared_clusters(kern, &n_clusters);
+  if (!rc) rc = shared_clusters(kern, p.cs, &n_clusters);
   if (rc) return rc;
   n_clusters = (int)std::min<int64_t>(n_clusters, p.max_tiles * p.segs);
   if (p.n_pairs <= 4096) {
@@ -825,13 +828,13 @@ int run_shared(const void* q, int q_dtype, const SharedPlan& p, SharedArgs a, co
   else split(__nv_bfloat16{});
   XENCB_CHECK_LAUNCH("shared_split launch");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(n_clusters * RS_CS));
+  cfg.gridDim = dim3((unsigned)(n_clusters * p.cs));
   cfg.blockDim = dim3(RS_THREADS);
   cfg.dynamicSmemBytes = RS_SMEM;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = RS_CS;
+  at[0].val.clusterDim.x = (unsigned)p.cs;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
@@ -1638,7 +1641,7 @@ int xencb_read_shared(const void* q, int q_dtype, int64_t n_rows, int d_s, const
   void* q16 = take(p.q);
   a.part = reinterpret_cast<float*>(take(p.part));
   a.ml = reinterpret_cast<float2*>(take(p.ml));
-  a.segs = p.segs; a.slab = p.slab; a.ahead = p.slab <= RS_AHEAD_SLAB ? 1 : 0;
+  a.segs = p.segs; a.cs = p.cs; a.ns = p.ns; a.slab = p.slab;
   a.softmax = read_softmax ? 1 : 0;
   a.qscale = read_softmax ? read_temp * 1.4426950408889634f : 1.f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
