@@ -16,6 +16,9 @@
 // passes through shared memory twice, but its second pass comes from L2: a cluster holds one or two pages at a time.
 // The roles run one unit apart: the scores of the next unit are computed while this one's softmax and exchange run,
 // and the epilogue stores one unit while the next one's P is made.
+// A unit of few pairs (8, or 16 for 16-bit results) takes its read product on the softmax warps instead, with mma.sync:
+// one 16-row tile holds all of its pairs, hi and lo together, and the tensor core's MN-major operand is read at about
+// 27 bytes a cycle (162 cycles per 16 slots x 128 columns), which ldmatrix is not.
 // shared_combine adds a row's pairs in the order of its routing: results do not depend on how pairs were grouped.
 //
 // Why this orientation: with the pairs as the 128 rows (of which a tile fills 64) the read cost 290 cycles per
@@ -55,9 +58,11 @@ constexpr int RS_STAGES = 6;
 constexpr int RS_PBLK = RS_N * 128;       // P of 64 slots: one 128-byte swizzle row per N row
 constexpr int RS_STAT = 2 * 16 * RS_N;    // floats: [2][16 groups of 32 slots][MT]
 constexpr int RS_SM_WARPS = 8;            // softmax: 4 TMEM lane quarters (32 slots each) x 2 halves of the pairs
+constexpr int RS_FEW = 16;                // N rows of a unit whose read runs on the softmax warps
 constexpr int RS_THREADS = 32 * 14;       // 0-7 softmax, 8-11 epilogue, 12 producer, 13 MMA
 constexpr size_t RS_SMEM = 1024 + 8 * RS_PBLK + (size_t)RS_STAGES * RS_STAGE + 2 * RS_STAT * 4 +
-                           (2 * RS_STAGES + 2 * RS_ACC + 6) * 8 + 16;
+                           (2 * RS_STAGES + 2 * RS_ACC + 9) * 8 + 16;
+static_assert(RS_STAGES % 2 == 0, "a stage of V goes to the same four warps each time round the ring");
 static_assert(4 * RS_VROWS * 128 <= RS_STAGE, "a stage of the read fits");
 
 struct __align__(16) SharedTile {
@@ -305,7 +310,9 @@ struct RsSmem {
   unsigned char* stages;  // the ring
   float* smax;            // [2][16][MT]: by the parity of the unit, per 32 slots
   float* ssum;            // [2][16][MT]
-  uint64_t *full, *empty, *s_full, *s_empty, *p_full, *o_full, *o_empty, *stat, *sums, *seen;
+  // p_full and sums: [0] units whose read runs on the tensor core, [1] units of few pairs. Each has one set of waiters,
+  // which sees every phase.
+  uint64_t *full, *empty, *s_full, *s_empty, *p_full, *o_full, *o_empty, *stat, *sums, *seen, *v_done;
   uint32_t* tmem;
   volatile int* abort_flag;
 };
@@ -315,6 +322,11 @@ struct RsRing {
   uint32_t st, phase;
   __device__ __forceinline__ void next(uint32_t n) {
     if (++st == n) { st = 0; phase ^= 1; }
+  }
+  __device__ __forceinline__ void skip(uint32_t by, uint32_t n) {
+    st += by;
+    phase ^= (st / n) & 1;
+    st %= n;
   }
   __device__ __forceinline__ void back(uint32_t n) {
     if (st == 0) { st = n; phase ^= 1; }
@@ -333,12 +345,13 @@ __device__ __forceinline__ RsSmem rs_smem(unsigned char* base) {
   s.s_full = s.empty + RS_STAGES;
   s.s_empty = s.s_full + RS_ACC;
   s.p_full = s.s_empty + RS_ACC;
-  s.o_full = s.p_full + 1;
+  s.o_full = s.p_full + 2;
   s.o_empty = s.o_full + 1;
   s.stat = s.o_empty + 1;
   s.sums = s.stat + 1;
-  s.seen = s.sums + 1;
-  s.tmem = reinterpret_cast<uint32_t*>(s.seen + 1);
+  s.seen = s.sums + 2;
+  s.v_done = s.seen + 1;
+  s.tmem = reinterpret_cast<uint32_t*>(s.v_done + 1);
   s.abort_flag = reinterpret_cast<volatile int*>(s.tmem + 1);
   return s;
 }
@@ -413,12 +426,15 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
       mbar_init(&s.s_full[i], 1);
       mbar_init(&s.s_empty[i], sm_warps);
     }
-    mbar_init(s.p_full, 1);
+    mbar_init(&s.p_full[0], 1);
+    mbar_init(&s.p_full[1], 1);
     mbar_init(s.o_full, 1);
     mbar_init(s.o_empty, 4);
     mbar_init(s.stat, cs * sm_warps);
-    mbar_init(s.sums, cs * sm_warps);
+    mbar_init(&s.sums[0], cs * sm_warps);
+    mbar_init(&s.sums[1], cs * sm_warps);
     mbar_init(s.seen, 4);
+    mbar_init(s.v_done, RS_SM_WARPS);
     *s.abort_flag = 0;
     fence_mbar_init();
   }
@@ -435,6 +451,10 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
   const int n_units = *a.n_tiles * a.segs;
   RsUnit cur, nxt;
   cur.find(a, cluster, n_units, n_clusters);
+  // few pairs: the read runs on the softmax warps (which are all there with 128 slots a CTA)
+  auto is_few = [&](const RsUnit& w) { return w.t.count * TERMS <= RS_FEW && ns == 128; };
+  auto s_stages = [&](const RsUnit& w) { return w.u < n_units && rank * ns < w.nv ? nkb : 0; };
+  auto v_stages = [&](const RsUnit& w) { return (w.nv + RS_VROWS - 1) / RS_VROWS * ((my_boxes + 3) / 4); };
   // A wait that runs out sets the abort flag; from then on the softmax and epilogue warps wait for nothing and run
   // through their units on whatever is there, so that the named barrier stays matched.
   auto done = [&](bool arrived) {
@@ -508,7 +528,7 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
     // --------------------------------------------------------------------------------------------- MMA issuer
     if (elect_one()) {
       RsRing ring{0, 0};
-      uint32_t unit = 0, acc = 0;
+      uint32_t big = 0, few = 0, acc = 0;  // units whose read runs here, and on the softmax warps
       bool ok = true;
       const uint32_t id_s = umma_idesc(FMT, FMT, 128, RS_N);
       const uint32_t id_o = umma_idesc(FMT, FMT, 128, RS_N) | (1u << 15);  // A (V) is MN-major
@@ -565,17 +585,25 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
           }
         }
         if (ok) tc_commit(s.o_full);
-        ++unit;
       };
       scores(cur);
       while (cur.u < n_units && ok) {
         nxt.find(a, cur.u + n_clusters, n_units, n_clusters);
         scores(nxt);
-        // the epilogue of the unit before has read its sums, and every CTA's block of P is here
-        if (ok && unit > 0) ok = mbar_wait_spin(s.o_empty, (unit - 1) & 1);
-        if (ok) ok = mbar_wait_cluster(s.p_full, unit & 1);
-        tc_fence_after();
-        if (ok) values(cur);
+        if (is_few(cur)) {
+          // the softmax warps take these stages: a wait for a later use of a stage is one for a parity, so it may only
+          // begin when every use before it is complete
+          if (ok) ok = mbar_wait_spin(s.v_done, few & 1);
+          ++few;
+          ring.skip(v_stages(cur), RS_STAGES);
+        } else {
+          // the epilogue of the last such unit has read its sums, and every CTA's block of P is here
+          if (ok && big > 0) ok = mbar_wait_spin(s.o_empty, (big - 1) & 1);
+          if (ok) ok = mbar_wait_cluster(&s.p_full[0], big & 1);
+          tc_fence_after();
+          if (ok) values(cur);
+          ++big;
+        }
         cur = nxt;
       }
       if (!ok) *s.abort_flag = 1;
@@ -592,7 +620,9 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
       // P: this CTA's block of the slot; 16-byte chunk j of row r at chunk j ^ (r % 8)
       const int in_blk = (quarter * 32 + lane) & 63;
       unsigned char* const pcol = s.p + (size_t)(rank * (ns / 64) + (quarter >> 1)) * RS_PBLK + (in_blk & 7) * 2;
-      uint32_t unit = 0, acc = 0;
+      uint32_t unit = 0, big = 0, acc = 0;
+      bool was_big = false;
+      RsRing ring{0, 0};
       float v[PP];
       auto scores = [&](const RsUnit& w) {
         if (w.u >= n_units || rank * ns >= w.nv) return;
@@ -617,11 +647,91 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
           if (lane == 0) mbar_arrive(&s.s_empty[buf]);
         }
       };
+      // The read of a unit of few pairs: O[16 rows, 64 columns] of this warp = P . V, the rows being the pairs' hi rows, then
+      // their lo rows (TERMS = 2), or 16 pairs. Warp w takes the w-th 64 columns of the slab; the four warps of a stage
+      // hand it back together.
+      auto read_few = [&](const RsUnit& w, uint32_t un, uint32_t nth, RsRing rg) {
+        done(*s.abort_flag || mbar_wait_cluster(&s.p_full[1], nth & 1));
+        const int hgroups = (my_boxes + 3) / 4, hg = warp >> 2;
+        if (hg >= hgroups) {  // no columns: but every phase of the barriers is waited for
+          done(*s.abort_flag || mbar_wait_cluster(&s.sums[1], nth & 1));
+          if (lane == 0) mbar_arrive(s.v_done);
+          return;
+        }
+        const int mtx = lane >> 3, r8 = lane & 7;
+        const int prow = TERMS == 2 ? (mtx & 1) * MT + r8 : (mtx & 1) * 8 + r8;  // (prow % 8 == r8)
+        const uint32_t pa = smem_u32(s.p) + prow * 128;
+        const uint32_t vrow = (uint32_t)(warp & 3) * (RS_VROWS * 128) + (r8 + (mtx & 1) * 8) * 128;
+        float acc_o[8][4];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc_o[i][0] = acc_o[i][1] = acc_o[i][2] = acc_o[i][3] = 0.f;
+        rg.skip(hg, RS_STAGES);
+        for (int b = 0; b < (w.nv + RS_VROWS - 1) / RS_VROWS; ++b) {
+          done(*s.abort_flag || mbar_wait_spin(&s.full[rg.st], rg.phase));
+          const uint32_t va = smem_u32(s.stages) + rg.st * RS_STAGE + vrow;
+          const int left = w.nv - b * RS_VROWS;
+#pragma unroll
+          for (int ks = 0; ks < RS_VROWS / 16; ++ks) {
+            if (ks * 16 >= left) break;
+            const int slot = b * RS_VROWS + ks * 16;
+            uint32_t a0, a1, a2, a3;
+            ldsm_x4(pa + (slot >> 6) * RS_PBLK + (((((slot & 63) >> 3) + (mtx >> 1)) ^ r8) << 4), a0, a1, a2, a3);
+            uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;  // rows of V behind the last valid slot: zeros
+            const int over = left - ks * 16;
+            if (over < 16) {
+              const int k = (lane & 3) * 2;
+              keep0 = (k < over ? 0xffffu : 0u) | (k + 1 < over ? 0xffff0000u : 0u);
+              keep1 = (k + 8 < over ? 0xffffu : 0u) | (k + 9 < over ? 0xffff0000u : 0u);
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              uint32_t b0, b1, b2, b3;
+              ldsm_x4_t(va + ks * 2048 + (((n * 2 + (mtx >> 1)) ^ r8) << 4), b0, b1, b2, b3);
+              mma16816<T>(acc_o[2 * n], a0, a1, a2, a3, b0 & keep0, b1 & keep1);
+              mma16816<T>(acc_o[2 * n + 1], a0, a1, a2, a3, b2 & keep0, b3 & keep1);
+            }
+          }
+          named_bar_sync(2 + hg, 128);
+          if ((warp & 3) == 0 && lane == 0 && !*s.abort_flag) mbar_arrive(&s.empty[rg.st]);
+          rg.skip(hgroups, RS_STAGES);
+        }
+        if (lane == 0) mbar_arrive(s.v_done);
+        done(*s.abort_flag || mbar_wait_cluster(&s.sums[1], nth & 1));
+        const int seg = w.u % a.segs, pair = lane >> 2;
+        const float* smax = s.smax + (un & 1) * 16 * MT;
+        const float* ssum = s.ssum + (un & 1) * 16 * MT;
+#pragma unroll
+        for (int g = 0; g < (TERMS == 2 ? 1 : 2); ++g) {
+          const int i = pair + 8 * g;
+          if (i >= w.t.count) continue;
+          float m = a.softmax ? -CUDART_INF_F : 0.f, l = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            m = fmaxf(m, smax[e * MT + i]);
+            l += ssum[e * MT + i];
+          }
+          const int64_t pos = w.t.start + i;
+          float coef;
+          if (a.softmax) coef = l != 0.f ? 1.f / l : 0.f;
+          else coef = rsqrtf((float)a.pnv[pos]) / f16_range_scale(m);
+          if (rank == 0 && warp == 0 && (lane & 3) == 0) a.ml[pos * a.segs + seg] = make_float2(m, l);
+          float* dst = a.part + (pos * a.segs + seg) * a.d_s + x0;
+#pragma unroll
+          for (int n = 0; n < 8; ++n) {
+            const int x = warp * 64 + n * 8 + (lane & 3) * 2;
+            const float o0 = TERMS == 2 ? acc_o[n][0] + acc_o[n][2] : acc_o[n][2 * g];
+            const float o1 = TERMS == 2 ? acc_o[n][1] + acc_o[n][3] : acc_o[n][2 * g + 1];
+            if (x < a.slab && x0 + x < a.d_s) *reinterpret_cast<float2*>(dst + x) = make_float2(o0 * coef, o1 * coef);
+          }
+        }
+      };
       scores(cur);
+      ring.skip(s_stages(cur), RS_STAGES);
       while (cur.u < n_units) {
         nxt.find(a, cur.u + n_clusters, n_units, n_clusters);
         const SharedTile t = cur.t;
         const bool mine = rank * ns < cur.nv;
+        const bool few = is_few(cur);
         const int count = t.count - half * PP;                 // this warp's pairs of the tile (may be <= 0)
         float* smax = s.smax + (unit & 1) * 16 * MT + half * PP;
         float* ssum = s.ssum + (unit & 1) * 16 * MT + half * PP;
@@ -646,9 +756,9 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
           mx = rs_reduce<PP>(w, lane, [](float p, float q) { return fmaxf(p, q); });
         }
         // the read of the unit before is done with P, and its epilogue with the maxima and sums two units back
-        if (unit > 0) {
-          done(*s.abort_flag || mbar_wait_spin(s.o_full, (unit - 1) & 1));
-          done(*s.abort_flag || mbar_wait_spin(s.seen, (unit - 1) & 1));
+        if (was_big) {
+          done(*s.abort_flag || mbar_wait_spin(s.o_full, (big - 1) & 1));
+          done(*s.abort_flag || mbar_wait_spin(s.seen, (big - 1) & 1));
         }
         // the pairs' maxima over these 32 slots to every CTA of the cluster
         if (lane < PP)
@@ -661,11 +771,13 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
           float m = none;
 #pragma unroll
           for (int g = 0; g < 16; ++g) m = fmaxf(m, smax[g * MT + me]);
-          const float lin = a.softmax ? 0.f : f16_range_scale(m);
+          const float ml = a.softmax ? m : f16_range_scale(m);
 #pragma unroll
-          for (int i = 0; i < PP; ++i) {
-            if (i < count) {
-              const float mi = __shfl_sync(0xffffffffu, a.softmax ? m : lin, i);
+          for (int g = 0; g < PP; g += 8) {
+            if (g >= count) break;
+#pragma unroll
+            for (int i = g; i < g + 8; ++i) {  // (rows behind the last pair are written and not looked at)
+              const float mi = __shfl_sync(0xffffffffu, ml, i);
               v[i] = a.softmax ? RS_P_SCALE * pf_exp2(v[i] - mi) : v[i] * mi;
               const int r = half * PP + i;
               unsigned char* at = pcol + r * 128 + (((in_blk >> 3) ^ (r & 7)) << 4);
@@ -682,20 +794,25 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
           // the other CTAs' blocks are still to come; then this CTA's block to them
           const uint32_t bytes = (uint32_t)(ns / 64) * RS_PBLK;
           const int n_work = min(cs, (cur.nv + ns - 1) / ns);
-          mbar_arrive_expect_tx(s.p_full, (uint32_t)(n_work - (mine ? 1 : 0)) * bytes);
+          mbar_arrive_expect_tx(&s.p_full[few], (uint32_t)(n_work - (mine ? 1 : 0)) * bytes);
           if (mine && !*s.abort_flag)
             for (int r = 1; r < cs; ++r) {
               const uint32_t to = (uint32_t)((rank + r) % cs);
               unsigned char* src = s.p + (size_t)rank * bytes;
-              bulk_s2s(cluster_map(src, to), src, bytes, cluster_map(s.p_full, to));
+              bulk_s2s(cluster_map(src, to), src, bytes, cluster_map(&s.p_full[few], to));
             }
         }
         __syncwarp();
         if (lane < PP)
           for (int r = 0; r < cs; ++r) st_cluster_f32(cluster_map(&ssum[group * MT + lane], r), l);
         __syncwarp();
-        if (lane < cs) mbar_arrive_cluster(cluster_map(s.sums, lane));
-        scores(nxt);
+        if (lane < cs) mbar_arrive_cluster(cluster_map(&s.sums[few], lane));
+        ring.skip(s_stages(nxt), RS_STAGES);
+        scores(nxt);  // (and with them every stage before this unit's V has been used: see v_done)
+        if (few) read_few(cur, unit, unit - big, ring);
+        else ++big;
+        ring.skip(v_stages(cur), RS_STAGES);
+        was_big = !few;
         ++unit;
         cur = nxt;
       }
@@ -704,14 +821,19 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
     // --------------------------------------------------------------------------------------------- epilogue
     // Lane = column of d_s, registers = pairs.
     const int quarter = warp & 3;
-    uint32_t unit = 0;
+    uint32_t unit = 0, big = 0;
     while (cur.u < n_units) {
       nxt.find(a, cur.u + n_clusters, n_units, n_clusters);
       const SharedTile t = cur.t;
       const int seg = cur.u % a.segs;
+      if (is_few(cur)) {
+        ++unit;
+        cur = nxt;
+        continue;
+      }
       const float* smax = s.smax + (unit & 1) * 16 * MT;
       const float* ssum = s.ssum + (unit & 1) * 16 * MT;
-      done(*s.abort_flag || mbar_wait_cluster(s.sums, unit & 1));
+      done(*s.abort_flag || mbar_wait_cluster(&s.sums[0], big & 1));
       float coef[MT / 32];  // lane i: pairs i and (TERMS = 1) 32 + i
 #pragma unroll
       for (int g = 0; g < MT / 32; ++g) {
@@ -732,11 +854,12 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(s.seen);
-      done(*s.abort_flag || mbar_wait_spin(s.o_full, unit & 1));
+      done(*s.abort_flag || mbar_wait_spin(s.o_full, big & 1));
       tc_fence_after();
       for (int b = 0; b < (my_boxes + 1) / 2; ++b) {
         const int x = b * 128 + quarter * 32 + lane;  // column of the slab
         const bool in = x < a.slab && x0 + x < a.d_s;
+        const int64_t pair_stride = (int64_t)a.segs * a.d_s;
         float* dst = a.part + ((int64_t)t.start * a.segs + seg) * a.d_s + x0 + x;
         const uint32_t at = taddr + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * RS_N);
 #pragma unroll
@@ -750,11 +873,14 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] += y[i];
           }
+          float* d = dst + (int64_t)(g * 32) * pair_stride;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (g * 32 + i < t.count) {
-              const float ci = __shfl_sync(0xffffffffu, coef[g], i);
-              if (in) dst[(int64_t)(g * 32 + i) * a.segs * a.d_s] = o[i] * ci;
+          for (int i8 = 0; i8 < 32; i8 += 8) {
+            if (g * 32 + i8 >= t.count) break;
+#pragma unroll
+            for (int i = i8; i < i8 + 8; ++i, d += pair_stride) {
+              const float x = o[i] * __shfl_sync(0xffffffffu, coef[g], i);
+              if (in && g * 32 + i < t.count) *d = x;
             }
           }
         }
@@ -762,6 +888,7 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(s.o_empty);
+      ++big;
       ++unit;
       cur = nxt;
     }

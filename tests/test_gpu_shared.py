@@ -283,3 +283,20 @@ def test_refusals(dev):
             ops.read_shared(q[:, :d].contiguous(), p, idx, wk, rows_per_lib=4)
     with pytest.raises(RuntimeError):
         ops.read_shared(q.cpu(), pages, idx, wk, rows_per_lib=4)
+
+
+@pytest.mark.parametrize("d_s,page_rows", [(2048, 512), (1024, 300), (256, 130)])
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+def test_pages_of_few_and_of_many_pairs_in_turn(dev, d_s, page_rows, out):
+    """Each cluster meets units of both kinds, several of them, in a random order."""
+    from kv_skill_v2_b200 import ops
+    C, R = 220, 260
+    pages, q, idx, wk = make(dev, 21, rows=R, shared=C, k=6, page_rows=page_rows, d_s=d_s)
+    g = torch.Generator(device=dev).manual_seed(5)
+    busy = torch.randperm(C, generator=g, device=dev)[:60]
+    many = torch.rand(R, 6, generator=g, device=dev) < 0.7  # most pairs go to a few pages
+    idx = torch.where(many, busy[torch.randint(0, 60, (R, 6), generator=g, device=dev)].to(torch.int32), idx)
+    idx = idx.contiguous()
+    got = ops.read_shared(q, pages, idx, wk, rows_per_lib=R, out_dtype=out)
+    check(got, pages, q, idx, wk, R, out)
+    assert ops.device_status(dev) == 0
