@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
     mbar_init(&s.sums[0], cs * sm_warps);
     mbar_init(&s.sums[1], cs * sm_warps);
     mbar_init(s.seen, 4);
-    mbar_init(s.v_done, RS_SM_WARPS);
+    mbar_init(s.v_done, RS_SM_WARPS + 1);  // and the MMA thread, so that it sees every phase
     *s.abort_flag = 0;
     fence_mbar_init();
   }
@@ -457,8 +457,11 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
   auto v_stages = [&](const RsUnit& w) { return (w.nv + RS_VROWS - 1) / RS_VROWS * ((my_boxes + 3) / 4); };
   // A wait that runs out sets the abort flag; from then on the softmax and epilogue warps wait for nothing and run
   // through their units on whatever is there, so that the named barrier stays matched.
+  // The lanes of a warp may leave a wait one after the other: they meet again here, as the tensor-memory loads, mma.sync,
+  // ldmatrix and barriers that follow need a converged warp.
   auto done = [&](bool arrived) {
     if (!arrived) *s.abort_flag = 1;
+    __syncwarp();
   };
 
   if (warp == 12) {
@@ -593,6 +596,7 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
         if (is_few(cur)) {
           // the softmax warps take these stages: a wait for a later use of a stage is one for a parity, so it may only
           // begin when every use before it is complete
+          mbar_arrive(s.v_done);
           if (ok) ok = mbar_wait_spin(s.v_done, few & 1);
           ++few;
           ring.skip(v_stages(cur), RS_STAGES);
@@ -645,6 +649,7 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&s.s_empty[buf]);
+          __syncwarp();
         }
       };
       // The read of a unit of few pairs: O[16 rows, 64 columns] of this warp = P . V, the rows being the pairs' hi rows, then
@@ -691,8 +696,10 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
               mma16816<T>(acc_o[2 * n + 1], a0, a1, a2, a3, b2 & keep0, b3 & keep1);
             }
           }
+          __syncwarp();
           named_bar_sync(2 + hg, 128);
           if ((warp & 3) == 0 && lane == 0 && !*s.abort_flag) mbar_arrive(&s.empty[rg.st]);
+          __syncwarp();
           rg.skip(hgroups, RS_STAGES);
         }
         if (lane == 0) mbar_arrive(s.v_done);
@@ -789,6 +796,7 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
           fence_proxy_async_smem();
           if (a.softmax) l = rs_reduce<PP>(v, lane, [](float p, float q) { return p + q; });
         }
+        __syncwarp();
         named_bar_sync(1, 32 * sm_warps);
         if (warp == 0 && lane == 0) {
           // the other CTAs' blocks are still to come; then this CTA's block to them
@@ -854,6 +862,7 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(s.seen);
+      __syncwarp();
       done(*s.abort_flag || mbar_wait_spin(s.o_full, big & 1));
       tc_fence_after();
       for (int b = 0; b < (my_boxes + 1) / 2; ++b) {
@@ -893,6 +902,7 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
       cur = nxt;
     }
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // no CTA leaves while another may still write to its shared memory
