@@ -169,10 +169,14 @@ __global__ void __launch_bounds__(256) shared_count_kernel(const SharedArgs a) {
   rs_count(a, (int64_t)blockIdx.x * blockDim.x + threadIdx.x, (int64_t)gridDim.x * blockDim.x);
 }
 
-__global__ void __launch_bounds__(1024) shared_scan_kernel(const SharedArgs a, int mt) { rs_scan(a, mt); }
+__global__ void __launch_bounds__(1024) shared_scan_kernel(const SharedArgs a, int mt) {
+  pdl_trigger();  // (the split reads q, which no kernel from here on writes, and waits before anything else)
+  rs_scan(a, mt);
+}
 
 // Few pairs: the whole plan in one CTA.
 __global__ void __launch_bounds__(1024) shared_plan_kernel(const SharedArgs a, int mt) {
+  pdl_trigger();
   for (int p = threadIdx.x; p < a.n_pages; p += 1024) {
     a.cnt[p] = 0;
     a.nvmax[p] = 0;
@@ -190,6 +194,7 @@ template <typename TQ, typename T, int TERMS>
 __global__ void __launch_bounds__(RS_SPLIT_THREADS) shared_split_kernel(const TQ* __restrict__ q, const SharedArgs a,
                                                                         T* __restrict__ out) {
   __shared__ float red[8];
+  pdl_trigger();
   const int64_t row = blockIdx.x;
   const TQ* src = q + row * a.d_s;
   float v[2][8];
@@ -222,6 +227,7 @@ __global__ void __launch_bounds__(RS_SPLIT_THREADS) shared_split_kernel(const TQ
       hi[p][e] = from_f32<T>(v[p][e] * s);
       if (TERMS == 2) lo[p][e] = from_f32<T>(v[p][e] * s - to_f32(hi[p][e]));
     }
+  pdl_wait();  // the plan
   const int64_t lib = row / a.rows_per_lib;
   const int j1 = min(a.k, (int)(blockIdx.y + 1) * 8);
   for (int j = blockIdx.y * 8; j < j1; ++j) {
@@ -903,6 +909,7 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
     }
   }
   __syncwarp();
+  pdl_trigger();
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // no CTA leaves while another may still write to its shared memory
@@ -918,6 +925,7 @@ template <typename TO, int G>
 __global__ void __launch_bounds__(256) shared_combine_kernel(const SharedArgs a, TO* __restrict__ r) {
   constexpr int W = 256 / G;
   __shared__ float4 sum[G > 1 ? G : 1][G > 1 ? W : 1];
+  pdl_wait();
   const int64_t row = blockIdx.x;
   const int64_t lib = row / a.rows_per_lib;
   const int lane = threadIdx.x % W, grp = threadIdx.x / W;

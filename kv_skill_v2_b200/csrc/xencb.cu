@@ -821,7 +821,7 @@ int run_shared(const void* q, int q_dtype, const SharedPlan& p, SharedArgs a, co
   const dim3 sgrid((unsigned)n_rows, (unsigned)((a.k + 7) / 8));
   auto split = [&](auto t) {
     using TQ = decltype(t);
-    shared_split_kernel<TQ, T, TERMS><<<sgrid, RS_SPLIT_THREADS, 0, st>>>(static_cast<const TQ*>(q), a, qo);
+    launch_pdl(shared_split_kernel<TQ, T, TERMS>, sgrid, dim3(RS_SPLIT_THREADS), 0, st, static_cast<const TQ*>(q), a, qo);
   };
   if (q_dtype == XENCB_F32) split(float{});
   else if (q_dtype == XENCB_F16) split(__half{});
@@ -832,21 +832,25 @@ int run_shared(const void* q, int q_dtype, const SharedPlan& p, SharedArgs a, co
   cfg.blockDim = dim3(RS_THREADS);
   cfg.dynamicSmemBytes = RS_SMEM;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = (unsigned)p.cs;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
   (void)cudaLaunchKernelEx(&cfg, kern, mq, mq8, mk, mv, a);
   XENCB_CHECK_LAUNCH("shared_read launch");
   auto combine = [&](auto t) {
     using TO = decltype(t);
     TO* r = static_cast<TO*>(r_out);
     if (a.k <= 8)
-      shared_combine_kernel<TO, 1><<<dim3((unsigned)n_rows, (unsigned)((a.d_s + 1023) / 1024)), 256, 0, st>>>(a, r);
+      launch_pdl(shared_combine_kernel<TO, 1>, dim3((unsigned)n_rows, (unsigned)((a.d_s + 1023) / 1024)), dim3(256), 0,
+                 st, a, r);
     else
-      shared_combine_kernel<TO, 8><<<dim3((unsigned)n_rows, (unsigned)((a.d_s + 127) / 128)), 256, 0, st>>>(a, r);
+      launch_pdl(shared_combine_kernel<TO, 8>, dim3((unsigned)n_rows, (unsigned)((a.d_s + 127) / 128)), dim3(256), 0, st,
+                 a, r);
   };
   if (out_dtype == XENCB_F32) combine(float{});
   else if (out_dtype == XENCB_F16) combine(__half{});

@@ -83,6 +83,8 @@ class ExternalSkillInjector:
         # entry keeps its source tensor alive so the key cannot be reused by another tensor
         self.gemm_f16x3 = True
         self._wprep: dict = {}
+        # low-rank adapters of the requests of a batch (set_adapters)
+        self._adapters: Optional[tuple] = None
         self._attach()
 
     def _active(self) -> bool:
@@ -114,6 +116,34 @@ class ExternalSkillInjector:
 
     def load(self, skill: KVSkill) -> None:
         self.skill = skill
+
+    def set_adapters(self, adapters_in: Optional[ops.Adapters] = None, adapters_out: Optional[ops.Adapters] = None,
+                     adapter_of: Optional[torch.Tensor] = None) -> None:
+        """Low-rank adapters beside the interface's maps (a ModelInterface with a full-rank A, or a LinearInterface):
+        adapters_in beside d_m -> d_s, adapters_out beside d_s -> d_m; adapter_of [B] int32 on the device names the one
+        of each batch row (negative: none). Without arguments they are taken off."""
+        if adapters_in is None and adapters_out is None:
+            self._adapters = None
+        else:
+            if adapter_of is None:
+                raise ValueError("set_adapters: adapter_of is required")
+            self._adapters = (adapters_in, adapters_out, adapter_of)
+
+    def _adapter_args(self, which: int, rows: int) -> dict:
+        """project_in's (which 0) or project_out's (1) adapter arguments for `rows` rows; empty without adapters."""
+        if self._adapters is None or self._adapters[which] is None:
+            return {}
+        of = self._adapters[2]
+        if of.numel() == 0 or rows % of.numel():
+            raise ValueError(f"set_adapters: adapter_of has {of.numel()} entries, the batch {rows} rows")
+        return {"adapters": self._adapters[which], "adapter_of": of, "rows_per_adapter": rows // of.numel()}
+
+    def _adapter_key(self) -> tuple:
+        if self._adapters is None:
+            return ()
+        a, b, of = self._adapters
+        ts = [x for ad in (a, b) if ad is not None for x in (ad.a, ad.b, ad.scale) if x is not None] + [of]
+        return tuple((x.data_ptr(), tuple(x.shape), x.dtype) for x in ts) + (a is None, b is None)
 
     # subclasses provide _branch (delta in float32) and _inject (h + delta, rel)
 
@@ -196,9 +226,10 @@ class XEncInjector(ExternalSkillInjector):
         if sel_fuse is not None:
             sel_w = sel_fuse.u.weight.detach().float().to(h2.device)
             sel_b = sel_fuse.u.bias.detach().float().to(h2.device)
+        more = self._adapter_args(0, h2.shape[0])
         if isinstance(itf, LinearInterface):
             W = _on(itf.w_in.detach(), h2).float()
-            q, _, _, z = ops.project_in(h2, W, sel_w=sel_w, sel_b=sel_b, w_prep=self._prep(W))
+            q, _, _, z = ops.project_in(h2, W, sel_w=sel_w, sel_b=sel_b, w_prep=self._prep(W), **more)
             return q, None, None, z
         p = itf._pos[li]
         gate_w = _on(itf.gate_w.detach(), h2).float()
@@ -210,8 +241,10 @@ class XEncInjector(ExternalSkillInjector):
             Wf = _f32_on(W, h2)
             q, g, _, z = ops.project_in(h2, Wf, None if b is None else _on(b.detach(), h2).float(),
                                         gate_w=gate_w, gate_b=gate_b, sel_w=sel_w, sel_b=sel_b,
-                                        w_prep=self._prep(Wf))
+                                        w_prep=self._prep(Wf), **more)
             return q, g, gain, z
+        if more:
+            raise NotImplementedError("adapters need a full-rank query map (this interface's A is low-rank)")
         # low-rank A: rms_norm + first map (gate and selector logits on the normed input), then map + L2
         x = h2
         g = z = None
@@ -232,6 +265,8 @@ class XEncInjector(ExternalSkillInjector):
         """(q, gate | None, log_gain | None, idx, wk, w) from the fused input projection + routing of decode rows,
         or None when the interface's query map is not one linear layer (low-rank A: two projections)."""
         itf = self.itf
+        if self._adapters is not None and self._adapters[0] is not None:
+            return None  # the projection with adapters, then the routing
         if isinstance(itf, LinearInterface):
             W = _on(itf.w_in.detach(), h2).float()
             q, _, _, idx, wk, w, _ = ops.project_in_route(
@@ -292,6 +327,7 @@ class XEncInjector(ExternalSkillInjector):
         lead = h.shape[:-1]
         W, b = self._write_weights(h2)
         wp = self._prep(W)
+        more = self._adapter_args(1, h2.shape[0])
         pm = self._pos_mask(h) if inject else None
         if extra is not None:  # a tensor calibration gain: fold into the per-row gate
             g = (g if g is not None else torch.ones(r.shape[0], device=r.device)) * extra.reshape(-1).float()
@@ -300,11 +336,11 @@ class XEncInjector(ExternalSkillInjector):
             _, h_new, rel = ops.project_out(r, W, h2, b_out=b, scale=float(self.gain_scale) * float(scale),
                                             log_scale=log_scale, gate=g, sel_w=sel_col, log_alpha=log_alpha,
                                             pos_mask=pm, want_delta=False,
-                                            h_out=h_new, want_rel=True, w_prep=wp)
+                                            h_out=h_new, want_rel=True, w_prep=wp, **more)
             return h_new.view(h.shape), rel
         delta, _, _ = ops.project_out(r, W, h2.float() if h2.dtype != torch.float32 else h2, b_out=b,
                                       scale=float(self.gain_scale) * float(scale), log_scale=log_scale, gate=g,
-                                      sel_w=sel_col, log_alpha=log_alpha, want_delta=True, w_prep=wp)
+                                      sel_w=sel_col, log_alpha=log_alpha, want_delta=True, w_prep=wp, **more)
         return delta.view(*lead, -1)
 
     def _duck_finish(self, h, hn, r, gcal, li, inject, selector=None):
@@ -335,8 +371,12 @@ class XEncInjector(ExternalSkillInjector):
 
 class LibraryInjector(XEncInjector):
     def __init__(self, model, interface, read_softmax: bool = True, read_temp: float = 12.0, route_temp: float = 10.0,
-                 top_k: int = 0, selector=None, read_fp32: bool = True, slot_dtype="auto", cuda_graphs: bool = True):
+                 top_k: int = 0, selector=None, read_fp32: bool = True, slot_dtype="auto", cuda_graphs: bool = True,
+                 share_pages: bool = False):
         self.lib = None
+        # read every page once for all rows that read it (ops.read_shared): for batches whose Libraries name the same
+        # pages (PagedLibrary.fork), many requests on one document, and prompts with top-k routing
+        self.share_pages = bool(share_pages)
         # per-(layer, shape) CUDA graphs of the fused hook path (see _run_lib); cleared whenever the Library changes
         self.cuda_graphs = bool(cuda_graphs)
         self._graphs: dict = {}
@@ -534,7 +574,7 @@ class LibraryInjector(XEncInjector):
         pages = self._pages(li, h)
         base = (li, tuple(h.shape), tuple(h.stride()), h.dtype, h.device, id(pages), float(self.gain_scale),
                 self.top_k, float(self.read_temp), float(self.route_temp), bool(self.read_softmax),
-                self._weights_key(), bool(self.gemm_f16x3))
+                self._weights_key(), bool(self.gemm_f16x3), self.share_pages, self._adapter_key())
         ent = self._graphs.get((base, h.data_ptr()))
         if ent is None:
             ent = self._graphs.get((base, None))
@@ -550,7 +590,7 @@ class LibraryInjector(XEncInjector):
                 # the entry keeps the prepared weights it captured alive
                 self._graphs[(base, h.data_ptr() if on_buffer else None)] = (
                     graph, None if on_buffer else h_static, h_new_s, rel_s, self.last_route, pages,
-                    list(self._wprep.values()))
+                    (list(self._wprep.values()), self._adapters))
                 # the captured step has not run yet: this call's routing is the eager run's
                 self.last_route = route_eager
                 return out
@@ -605,8 +645,13 @@ class LibraryInjector(XEncInjector):
             idx, wk, w, _ = ops.route(q, pages.S, rows_per_lib=rpl, top_k=self.top_k, route_temp=self.route_temp,
                                       n_chunks_of=pages.n_chunks_of, row_w=sel_col)
         # with a selector most rows read nothing at most depths: the sparse plan spreads the live rows' work
+        if not self._fast_interface() and self._adapters is not None:
+            raise NotImplementedError("adapters need a ModelInterface or a LinearInterface")
         if self.record_attn or self.force_attn is not None:
             r = self._read_with_diagnostics(h, li, q, pages, idx, wk, rpl, sparse=sel_col is not None)
+        elif self.share_pages and ops.shared_supported(pages):
+            r = ops.read_shared(q, pages, idx, wk, rows_per_lib=rpl, read_temp=self.read_temp,
+                                read_softmax=self.read_softmax)
         else:
             r = ops.read_decode(q, pages, idx, wk, rows_per_lib=rpl, read_temp=self.read_temp,
                                 read_softmax=self.read_softmax, sparse=sel_col is not None)

@@ -265,6 +265,98 @@ class PagedLibrary:
             self._pages[li] = p
         return p
 
+    # ------------------------------------------------------------------ forking, freeing, compacting
+    def _tables(self):
+        """(pools, page_of, n_valid, n_chunks_of) when every layer has the same page table, as the builders lay it out."""
+        first = self._pages[self.layers[0]]
+        pools, seen = [], set()
+        for li in self.layers:
+            p = self._pages[li]
+            for a, b, what in ((p.page_of, first.page_of, "page_of"), (p.n_valid, first.n_valid, "n_valid"),
+                               (p.n_chunks_of, first.n_chunks_of, "n_chunks_of")):
+                if (a is None) != (b is None) or (a is not None and a is not b and not torch.equal(a, b)):
+                    raise ValueError(f"layer {li} has another {what} than layer {self.layers[0]}: its pages cannot be "
+                                     "moved together")
+            for pool in (p.slots, p.vslots):
+                if pool is not None and pool.data_ptr() not in seen:
+                    seen.add(pool.data_ptr())
+                    pools.append(pool)
+        return pools, first.page_of, first.n_valid, first.n_chunks_of
+
+    def _with_tables(self, page_of, n_valid, n_chunks_of, rows, pools=None) -> "PagedLibrary":
+        """This one with new tables; `rows` picks each new row's summary keys, `pools` maps old pools to new ones."""
+        pools = pools or {}
+        pages = {}
+        for li, p in self._pages.items():
+            slots = pools.get(p.slots.data_ptr(), p.slots)
+            v = None if p.vslots is None else pools.get(p.vslots.data_ptr(), p.vslots)
+            S = p.S if rows is None else p.S.index_select(0, rows)
+            pages[li] = Pages(slots=slots, page_of=page_of, n_valid=n_valid, S=S, n_chunks_of=n_chunks_of, vslots=v)
+        return PagedLibrary(pages, depths=self.depths)
+
+    def _rows(self, rows) -> torch.Tensor:
+        dev = next(iter(self._pages.values())).device
+        rows = torch.as_tensor(rows, dtype=torch.int64)
+        if rows.dim() != 1 or rows.numel() == 0 or int(rows.min()) < 0 or int(rows.max()) >= self.n_lib:
+            raise ValueError(f"rows must be a non-empty list of Libraries 0..{self.n_lib - 1}, got {rows.tolist()}")
+        return rows.to(dev)
+
+    def select(self, rows) -> "PagedLibrary":
+        """The Libraries `rows`, in that order and sharing this one's pools: the batch a step reads. Fork and compact
+        on the PagedLibrary that holds every row: a page that none of its rows names counts as free."""
+        _, page_of, n_valid, nco = self._tables()
+        r = self._rows(rows)
+        return self._with_tables(page_of.index_select(0, r).contiguous(), n_valid.index_select(0, r).contiguous(),
+                                 None if nco is None else nco.index_select(0, r).contiguous(), r)
+
+    def drop(self, rows) -> "PagedLibrary":
+        """Without the Libraries `rows`: the pages only they named are free for the next fork."""
+        gone = set(self._rows(rows).tolist())
+        return self.select([i for i in range(self.n_lib) if i not in gone])
+
+    def reserve(self, pages: int) -> "PagedLibrary":
+        """The same Libraries in pools with `pages` more (zeroed) pages, for forks to take."""
+        pools, page_of, n_valid, nco = self._tables()
+        if int(pages) < 0:
+            raise ValueError(f"reserve: pages={pages} must not be negative")
+        new = {}
+        for pool in pools:
+            big = torch.zeros(pool.shape[0] + int(pages), *pool.shape[1:], dtype=pool.dtype, device=pool.device)
+            big[:pool.shape[0]].copy_(pool)
+            new[pool.data_ptr()] = big
+        return self._with_tables(page_of, n_valid, nco, None, new)
+
+    def fork(self, parents, own_from=None) -> "PagedLibrary":
+        """These Libraries and, behind them, one fork of each of `parents`. A fork shares its parent's pages for the
+        chunks below own_from (an int, or one per fork; default: all of them) and has pages of its own, holding copies,
+        for the rest, so that they can be rewritten for one request alone. RuntimeError when the pools have too few free
+        pages (reserve). Reads one integer back from the device."""
+        from .ops import pages_fork
+
+        pools, page_of, n_valid, nco = self._tables()
+        r = self._rows(parents)
+        m = r.numel()
+        own = torch.as_tensor(self.n_chunks if own_from is None else own_from, dtype=torch.int32)
+        if own.dim() > 1 or (own.dim() == 1 and own.numel() != m) or bool((own < 0).any()):
+            raise ValueError(f"fork: own_from must be one chunk number, or one for each of {m} forks")
+        own = own.expand(m).contiguous().to(page_of.device)
+        page_of, n_valid = page_of.contiguous(), n_valid.contiguous()
+        child, missing = pages_fork(pools, page_of, n_valid, r.to(torch.int32), own, n_chunks_of=nco)
+        if int(missing):
+            raise RuntimeError(f"fork: the pools have {int(missing)} free pages too few (PagedLibrary.reserve)")
+        rows = torch.cat([torch.arange(self.n_lib, device=r.device), r])
+        return self._with_tables(torch.cat([page_of, child]), n_valid.index_select(0, rows).contiguous(),
+                                 None if nco is None else nco.index_select(0, rows).contiguous(), rows)
+
+    def compact(self):
+        """(the same Libraries with their pages moved to the front of the pools, the number n of pages in use): pages
+        [n, P) are free. The pools are this one's, so this PagedLibrary and any select() of it must no longer be read."""
+        from .ops import pages_compact
+
+        pools, page_of, n_valid, nco = self._tables()
+        table, n_live = pages_compact(pools, page_of.contiguous(), n_valid.contiguous(), n_chunks_of=nco)
+        return self._with_tables(table, n_valid, nco, None), int(n_live)
+
     @staticmethod
     def from_libraries(libs: list, device, slot_dtype=torch.float16) -> "PagedLibrary":
         """Stack Libraries with the same layers and d_s; library b serves batch row b. When any Library is

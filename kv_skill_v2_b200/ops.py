@@ -19,11 +19,13 @@ _DT = {torch.float32: N.F32, torch.float16: N.F16, torch.bfloat16: N.BF16}
 
 
 def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()  # (the bindings' argument types make it a void*)
 
 
 def _stream(dev: torch.device):
-    return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+    """The raw current stream of `dev` (the same handle as torch.cuda.current_stream(dev).cuda_stream, without
+    building the Stream object: about 4 us of a call)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index if dev.index is not None else torch.cuda.current_device())
 
 
 def _cuda(what: str, *ts) -> torch.device:
@@ -629,6 +631,12 @@ def read_shared(q: torch.Tensor, pages: Pages, idx: torch.Tensor, wk: torch.Tens
     return r
 
 
+def shared_supported(pages: Pages) -> bool:
+    """Whether read_shared takes this slot pool (f16 / bf16 slots, d_s % 8 == 0, d_s <= 4096)."""
+    return N.lib().xencb_read_shared_workspace(1, 1, pages.d_s, pages.slots.shape[0], pages.page_rows,
+                                               _hdt(pages.slots, "slots"), N.F32) > 0
+
+
 def multi_supported(pages: Pages, n_rows: int, rows_per_lib: int) -> bool:
     """Whether read_multi takes this slot pool (f16 / bf16 slots, d_s % 16 == 0, the stages fit on chip)."""
     if pages.slots.dtype not in (torch.float16, torch.bfloat16) or pages.d_s % 16:
@@ -824,8 +832,9 @@ def _pool_args(what: str, pools, page_of: torch.Tensor, n_valid: torch.Tensor, n
     dev = _cuda(what, *pools, page_of, n_valid, n_chunks_of)
     P, N_rows = pools[0].shape[:2]
     for p in pools:
-        _hdt(p, f"{what}: pool")
-        if p.dim() != 3 or not p.is_contiguous() or tuple(p.shape[:2]) != (P, N_rows):
+        if p.dtype not in _DT:
+            raise ValueError(f"{what}: pool dtype {p.dtype} not supported (float32 / float16 / bfloat16)")
+        if p.dim() != 3 or p.shape[0] != P or p.shape[1] != N_rows or not p.is_contiguous():
             raise ValueError(f"{what}: pools must be contiguous [pages, page_rows, d] tensors with the same pages, got "
                              f"{tuple(p.shape)} beside {tuple(pools[0].shape)}")
     for name, t in (("page_of", page_of), ("n_valid", n_valid)):
@@ -857,9 +866,9 @@ def pages_fork(pools, page_of: torch.Tensor, n_valid: torch.Tensor, parents: tor
     n_lib, C = page_of.shape
     m = int(parents.numel())
     child = torch.empty(m, C, dtype=torch.int32, device=dev)
-    missing = torch.zeros(1, dtype=torch.int32, device=dev)
     if m == 0:
-        return child, missing
+        return child, torch.zeros(1, dtype=torch.int32, device=dev)
+    missing = torch.empty(1, dtype=torch.int32, device=dev)
     with _on_device(dev):
         ws = _workspace(N.lib().xencb_pages_fork_workspace(m, C), dev)
         N.call("xencb_pages_fork", ptrs, sizes, len(ptrs), P, page_rows, _ptr(page_of), _ptr(n_valid), C,

@@ -1,0 +1,190 @@
+"""Many requests over shared documents, as a server runs them: Libraries forked for requests, their pages compacted, the
+batch read with every shared page fetched once, and an adapter of its own per request -- against the definition in 64
+bits, and against itself after pages moved (results do not depend on where a page lies)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests._fixtures import TOL, TinyReader, rel_err
+
+pytestmark = pytest.mark.gpu
+
+D_M, D_S, LAYER = 96, 64, 1
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    return torch.device("cuda:0")
+
+
+def _library(dev, seed=0, n_lib=3, C=5, rows=20, ragged=True, untied=False):
+    from kv_skill_v2_b200 import PagedLibrary
+    g = torch.Generator(device=dev).manual_seed(seed)
+    pools = {li: torch.nn.functional.normalize(torch.randn(n_lib * C, rows, D_S, generator=g, device=dev), dim=-1).half()
+             for li in (LAYER, 3)}
+    vals = {li: torch.randn_like(p) for li, p in pools.items()} if untied else None
+    page_of = torch.randperm(n_lib * C, generator=g, device=dev).view(n_lib, C).to(torch.int32)
+    n_valid = torch.randint(1, rows + 1, (n_lib, C), generator=g, device=dev, dtype=torch.int32)
+    nco = torch.tensor([C, C - 2, C - 1], dtype=torch.int32, device=dev)[:n_lib] if ragged else None
+    return PagedLibrary.from_pool(pools, page_of, n_valid, nco, layer_vslots=vals)
+
+
+def _content(lib, li, row, c):
+    p = lib.pages(li)
+    return p.slots[int(p.page_of[row, c]), :int(p.n_valid[row, c])]
+
+
+def _chunks(lib, row):
+    nco = lib.pages(LAYER).n_chunks_of
+    return lib.n_chunks if nco is None else int(nco[row])
+
+
+@pytest.mark.parametrize("ragged,untied", [(False, False), (True, False), (True, True)])
+def test_fork_drop_compact_keep_every_library(dev, ragged, untied):
+    lib = _library(dev, ragged=ragged, untied=untied)
+    before = {(li, r, c): _content(lib, li, r, c).clone() for li in lib.layers for r in range(3)
+              for c in range(_chunks(lib, r))}
+    with pytest.raises(RuntimeError, match="free pages too few"):
+        lib.fork([0, 0, 0, 0, 0, 0, 0, 0], own_from=0)
+    lib = lib.reserve(8)
+    parents, own = [0, 1, 0, 2], [5, 2, 3, 4]
+    lib = lib.fork(parents, own)
+    assert lib.n_lib == 7
+    origin = [0, 1, 2] + parents
+
+    def same(lib, origin):
+        for i, o in enumerate(origin):
+            for li in lib.layers:
+                for c in range(_chunks(lib, i)):
+                    assert torch.equal(_content(lib, li, i, c), before[li, o, c])
+
+    same(lib, origin)
+    t = lib.pages(LAYER).page_of
+    taken = {int(t[r, c]) for r in range(3) for c in range(_chunks(lib, r))}  # (entries past a Library's chunks name nothing)
+    for i, (par, o) in enumerate(zip(parents, own)):
+        n = _chunks(lib, par)
+        assert torch.equal(t[3 + i, :min(o, n)], t[par, :min(o, n)])
+        assert not set(t[3 + i, o:n].tolist()) & taken
+    # rewriting a fork's own chunk reaches nobody else
+    p = lib.pages(LAYER)
+    mine = int(p.page_of[5, 4]) if _chunks(lib, 5) == 5 else int(p.page_of[5, 3])
+    kept = p.slots[mine].clone()
+    p.slots[mine].fill_(0.25)
+    same(lib.select([0, 1, 2, 3, 4, 6]), [0, 1, 2, 0, 1, 2])
+    p.slots[mine].copy_(kept)
+    lib = lib.drop([1, 4])
+    lib, n = lib.compact()
+    origin = [0, 2, 0, 0, 2]
+    same(lib, origin)
+    live = set()
+    for i in range(lib.n_lib):
+        live |= set(lib.pages(LAYER).page_of[i, :_chunks(lib, i)].tolist())
+    assert live == set(range(n))
+    with pytest.raises(ValueError):
+        lib.select([9])
+    with pytest.raises(ValueError):
+        lib.fork([0], own_from=[1, 2])
+
+
+def _reference(h, W_in, W_out, lib, li, ad_in, ad_out, of, top_k, route_temp, read_temp):
+    """delta of every token in 64 bits (single linear maps, no gate)."""
+    out = torch.zeros(h.shape, dtype=torch.float64, device=h.device)
+    p = lib.pages(li)
+    for b in range(h.shape[0]):
+        x = h[b].double()
+        x = x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + 1e-6)
+        q = x @ W_in.double()
+        a = int(of[b])
+        if a >= 0:
+            q = q + ad_in.scale[a].double() * (x @ ad_in.a[a].double().t()) @ ad_in.b[a].double().t()
+        q = q / (q.norm(dim=-1, keepdim=True) + 1e-6)
+        n = _chunks(lib, b)
+        logits = q @ p.S[b, :n].double().t() * route_temp
+        k = top_k if 0 < top_k < n else n
+        top, idx = logits.topk(k, dim=-1)
+        w = torch.softmax(top, -1)
+        r = torch.zeros(q.shape, dtype=torch.float64, device=h.device)
+        for t in range(q.shape[0]):
+            for j in range(k):
+                K = _content(lib, li, b, int(idx[t, j])).double()
+                r[t] += w[t, j] * (torch.softmax(read_temp * K @ q[t], 0) @ K)
+        y = r @ W_out.double()
+        if a >= 0:
+            y = y + ad_out.scale[a].double() * (r @ ad_out.a[a].double().t()) @ ad_out.b[a].double().t()
+        out[b] = y
+    return out
+
+
+@pytest.mark.parametrize("T", [1, 5, 70])
+@pytest.mark.parametrize("graphs", [True, False])
+def test_requests_with_adapters_over_forked_libraries(dev, T, graphs):
+    from kv_skill_v2_b200 import LibraryInjector, ops
+    from kv_skill_v2_b200.interface import LinearInterface
+    g = torch.Generator(device=dev).manual_seed(3)
+    W_in = torch.randn(D_M, D_S, generator=g, device=dev) * D_M ** -0.5
+    W_out = torch.randn(D_S, D_M, generator=g, device=dev) * 0.2
+    whole = _library(dev, seed=4).reserve(6).fork([0, 0, 1, 2], own_from=[4, 3, 2, 9])
+    lib = whole.select([3, 4, 5, 6, 0])
+    B = lib.n_lib
+    of = torch.tensor([2, -1, 0, 2, 1], dtype=torch.int32, device=dev)
+
+    def adapters(d_in, d_out):
+        return ops.Adapters(a=torch.randn(3, 4, d_in, generator=g, device=dev) * d_in ** -0.5,
+                            b=torch.randn(3, d_out, 4, generator=g, device=dev) * 0.2,
+                            scale=torch.rand(3, generator=g, device=dev) + 0.5)
+
+    ad_in, ad_out = adapters(D_M, D_S), adapters(D_S, D_M)
+    reader = TinyReader(D_M, 4).to(dev)
+    itf = LinearInterface(W_in, W_out, [LAYER]).to(dev).requires_grad_(False)
+    inj = LibraryInjector(reader, itf, top_k=2, cuda_graphs=graphs, share_pages=True)
+    inj.load_library(lib)
+    inj.set_adapters(ad_in, ad_out, of)
+    h = torch.randn(B, T, D_M, generator=g, device=dev)
+    with torch.no_grad():
+        want = _reference(h, W_in, W_out, lib, LAYER, ad_in, ad_out, of, 2, 10.0, 12.0)
+        for _ in range(3):  # eager, captured, replayed
+            got, _ = inj._inject(h, LAYER)
+            assert rel_err(got - h, want) <= TOL
+        first = got.clone()
+        # another assignment of adapters, in place and then as another tensor
+        of.copy_(of.flip(0))
+        want2 = _reference(h, W_in, W_out, lib, LAYER, ad_in, ad_out, of, 2, 10.0, 12.0)
+        assert rel_err(inj._inject(h, LAYER)[0] - h, want2) <= TOL
+        inj.set_adapters(ad_in, ad_out, of.flip(0).contiguous())
+        assert torch.equal(inj._inject(h, LAYER)[0], first)
+        # the pages move: the same bits
+        moved, _ = whole.compact()
+        inj.load_library(moved.select([3, 4, 5, 6, 0]))
+        assert torch.equal(inj._inject(h, LAYER)[0], first)
+        # without adapters and page sharing: the path of read_decode
+        inj.set_adapters()
+        inj.share_pages = False
+        plain, _ = inj._inject(h, LAYER)
+        none = torch.full((B,), -1, dtype=torch.int32, device=dev)
+        ref = _reference(h, W_in, W_out, moved.select([3, 4, 5, 6, 0]), LAYER, ad_in, ad_out, none, 2, 10.0, 12.0)
+        assert rel_err(plain - h, ref) <= TOL
+    assert ops.device_status(dev) == 0
+    inj.detach()
+
+
+def test_adapter_refusals(dev):
+    from kv_skill_v2_b200 import LibraryInjector, make_interface, ops
+    reader = TinyReader(D_M, 4).to(dev)
+    low = make_interface(D_M, D_S, [LAYER], rank=8).to(dev).requires_grad_(False)
+    inj = LibraryInjector(reader, low, top_k=2)
+    inj.load_library(_library(dev, ragged=False))
+    ad = ops.Adapters(a=torch.zeros(1, 2, D_M, device=dev), b=torch.zeros(1, D_S, 2, device=dev))
+    with pytest.raises(ValueError):
+        inj.set_adapters(ad)
+    inj.set_adapters(ad, None, torch.zeros(3, dtype=torch.int32, device=dev))
+    h = torch.randn(3, 1, D_M, device=dev)
+    with torch.no_grad(), pytest.raises(NotImplementedError):
+        inj._inject(h, LAYER)
+    inj.set_adapters(ad, None, torch.zeros(2, dtype=torch.int32, device=dev))
+    with torch.no_grad(), pytest.raises(ValueError):
+        inj._inject(h, LAYER)
+    inj.detach()

@@ -1,0 +1,72 @@
+"""Refusals of the shared read, the page operators and the adapters that need no GPU."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+from kv_skill_v2_b200 import _native as N
+from kv_skill_v2_b200 import ops
+
+
+def _pages(d=64):
+    return ops.Pages(slots=torch.zeros(2, 4, d, dtype=torch.float16), page_of=torch.zeros(1, 2, dtype=torch.int32),
+                     n_valid=torch.ones(1, 2, dtype=torch.int32), S=torch.zeros(1, 2, d))
+
+
+def test_cpu_tensors_are_refused():
+    q, idx, wk = torch.zeros(1, 64), torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, 1)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.read_shared(q, _pages(), idx, wk, rows_per_lib=1)
+    p = _pages()
+    one = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.pages_fork([p.slots], p.page_of, p.n_valid, one, one)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.pages_compact([p.slots], p.page_of, p.n_valid)
+    with pytest.raises(ValueError, match="at least one pool"):
+        ops.pages_compact([], p.page_of, p.n_valid)
+    ad = ops.Adapters(torch.zeros(1, 2, 64), torch.zeros(1, 64, 2))
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.project_in(torch.zeros(1, 64), torch.zeros(64, 64), adapters=ad, adapter_of=one)
+
+
+def test_read_shared_shapes():
+    """The workspace query (host only) tells which shapes the kernel takes."""
+    size = N.lib().xencb_read_shared_workspace
+    for d in (8, 64, 200, 2048, 2560, 4096):
+        assert size(4, 2, d, 10, 512, N.F16, N.F32) >= size(4, 2, d, 10, 512, N.F16, N.BF16) > 0
+    for bad in ((4, 2, 60, 10, 512, N.F16, N.F32), (4, 2, 4104, 10, 512, N.F16, N.F32),
+                (4, 2, 64, 10, 512, N.F32, N.F32), (4, 2, 64, 10, 512, N.F16, 7), (0, 2, 64, 10, 512, N.F16, N.F32),
+                (4, 0, 64, 10, 512, N.F16, N.F32), (1 << 31, 64, 64, 10, 512, N.F16, N.F32),
+                (4, 2, 64, 1 << 24, 512, N.F16, N.F32)):
+        assert size(*bad) == 0
+    assert ops.shared_supported(_pages()) and not ops.shared_supported(_pages(60))
+
+
+def _call(fn, *args):
+    return getattr(N.lib(), fn)(*args)
+
+
+def test_page_operators_refuse_bad_arguments():
+    one, buf = ctypes.c_void_p(256), (ctypes.c_void_p * 1)(256)
+    row = (ctypes.c_int64 * 1)(16)
+
+    def compact(pools=buf, rows=row, n=1, pages=4, page_rows=2, table=one, C=2, n_lib=1, ws=one, ws_bytes=1 << 20):
+        return _call("xencb_pages_compact", pools, rows, n, pages, page_rows, table, one, C, None, n_lib, one, one, ws,
+                     ws_bytes, None)
+
+    def fork(m=1, parents=one, ws_bytes=1 << 20, C=2):
+        return _call("xencb_pages_fork", buf, row, 1, 4, 2, one, one, C, None, 1, parents, one, m, one, one, one,
+                     ws_bytes, None)
+
+    assert compact(pools=None) == N.EINVAL and compact(n=0) == N.EINVAL and compact(pages=0) == N.EINVAL
+    assert compact(rows=(ctypes.c_int64 * 1)(3)) == N.EINVAL and compact(table=None) == N.EINVAL
+    assert compact(pages=(1 << 20) + 1) == N.ENOTSUP and compact(C=0) == N.EINVAL
+    assert compact(C=1 << 20, n_lib=1 << 12) == N.ENOTSUP
+    assert compact(ws=ctypes.c_void_p(264)) == N.EINVAL and compact(ws_bytes=8) == N.EINVAL
+    assert fork(m=0) == N.EINVAL and fork(parents=None) == N.EINVAL and fork(ws_bytes=8) == N.EINVAL
+    assert fork(m=1 << 20, C=1 << 12) == N.ENOTSUP
+    assert N.lib().xencb_pages_fork_workspace(0, 4) == 0 and N.lib().xencb_pages_compact_workspace(0) == 0
