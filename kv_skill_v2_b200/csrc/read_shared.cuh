@@ -273,11 +273,12 @@ __device__ __forceinline__ bool elect_one() {
       : "=r"(p));
   return p != 0;
 }
-__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+// A 4-byte store to a CTA of the cluster that counts its bytes on that CTA's barrier: the value and its arrival in one
+// trip, where a store, a release and an arrival took 1 us more.
+__device__ __forceinline__ void st_async_f32(uint32_t addr, float v, uint32_t bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.u32 [%0], %1, [%2];" ::"r"(addr),
+               "r"(__float_as_uint(v)), "r"(bar)
+               : "memory");
 }
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
@@ -436,9 +437,9 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
     mbar_init(&s.p_full[1], 1);
     mbar_init(s.o_full, 1);
     mbar_init(s.o_empty, 4);
-    mbar_init(s.stat, cs * sm_warps);
-    mbar_init(&s.sums[0], cs * sm_warps);
-    mbar_init(&s.sums[1], cs * sm_warps);
+    mbar_init(s.stat, 1);  // and the bytes of cs * sm_warps * PP values (sums too)
+    mbar_init(&s.sums[0], 1);
+    mbar_init(&s.sums[1], 1);
     mbar_init(s.seen, 4);
     mbar_init(s.v_done, RS_SM_WARPS + 1);  // and the MMA thread, so that it sees every phase
     *s.abort_flag = 0;
@@ -626,6 +627,7 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
     if (quarter < quarters) {
       const uint32_t tl = taddr + ((uint32_t)(quarter * 32) << 16) + RS_S_COL + (uint32_t)(half * PP);
       const int slot0 = rank * ns + quarter * 32;              // lane 0's slot of the segment
+      const int nth_warp = half * quarters + quarter;          // of the sm_warps
       const int group = slot0 >> 5;                            // 32 slots: their entry of smax and ssum
       // P: this CTA's block of the slot; 16-byte chunk j of row r at chunk j ^ (r % 8)
       const int in_blk = (quarter * 32 + lane) & 63;
@@ -774,10 +776,11 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
           done(*s.abort_flag || mbar_wait_spin(s.seen, (big - 1) & 1));
         }
         // the pairs' maxima over these 32 slots to every CTA of the cluster
+        const uint32_t stat_bytes = (uint32_t)(cs * sm_warps * PP * 4);
+        if (nth_warp == 0 && lane == 0) mbar_arrive_expect_tx(s.stat, stat_bytes);
         if (lane < PP)
-          for (int r = 0; r < cs; ++r) st_cluster_f32(cluster_map(&smax[group * MT + lane], r), mx);
-        __syncwarp();
-        if (lane < cs) mbar_arrive_cluster(cluster_map(s.stat, lane));
+          for (int r = 0; r < cs; ++r)
+            st_async_f32(cluster_map(&smax[group * MT + lane], r), mx, cluster_map(s.stat, r));
         done(*s.abort_flag || mbar_wait_cluster(s.stat, unit & 1));
         float l = 0.f;
         if (mine) {
@@ -804,23 +807,28 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
         }
         __syncwarp();
         named_bar_sync(1, 32 * sm_warps);
-        if (warp == 0 && lane == 0) {
-          // the other CTAs' blocks are still to come; then this CTA's block to them
+        if (elect_one()) {
           const uint32_t bytes = (uint32_t)(ns / 64) * RS_PBLK;
-          const int n_work = min(cs, (cur.nv + ns - 1) / ns);
-          mbar_arrive_expect_tx(&s.p_full[few], (uint32_t)(n_work - (mine ? 1 : 0)) * bytes);
+          if (nth_warp == 0) {
+            // the other CTAs' blocks and sums are still to come
+            const int n_work = min(cs, (cur.nv + ns - 1) / ns);
+            mbar_arrive_expect_tx(&s.p_full[few], (uint32_t)(n_work - (mine ? 1 : 0)) * bytes);
+            mbar_arrive_expect_tx(&s.sums[few], stat_bytes);
+          }
+          // this CTA's block to the others: each warp takes every sm_warps-th of them
+          unsigned char* src = s.p + (size_t)rank * bytes;
           if (mine && !*s.abort_flag)
-            for (int r = 1; r < cs; ++r) {
-              const uint32_t to = (uint32_t)((rank + r) % cs);
-              unsigned char* src = s.p + (size_t)rank * bytes;
-              bulk_s2s(cluster_map(src, to), src, bytes, cluster_map(&s.p_full[few], to));
-            }
+            for (int r = nth_warp; r < cs; r += sm_warps)
+              if (r > 0) {
+                const uint32_t to = (uint32_t)((rank + r) % cs);
+                bulk_s2s(cluster_map(src, to), src, bytes, cluster_map(&s.p_full[few], to));
+              }
         }
         __syncwarp();
         if (lane < PP)
-          for (int r = 0; r < cs; ++r) st_cluster_f32(cluster_map(&ssum[group * MT + lane], r), l);
+          for (int r = 0; r < cs; ++r)
+            st_async_f32(cluster_map(&ssum[group * MT + lane], r), l, cluster_map(&s.sums[few], r));
         __syncwarp();
-        if (lane < cs) mbar_arrive_cluster(cluster_map(&s.sums[few], lane));
         ring.skip(s_stages(nxt), RS_STAGES);
         scores(nxt);  // (and with them every stage before this unit's V has been used: see v_done)
         if (few) read_few(cur, unit, unit - big, ring);
