@@ -31,7 +31,7 @@
 //
 // The tensor core's accumulator drops bits below its running value at every 16-term step, always towards zero; over
 // d_s = 2048 that is 128 steps, 1.2e-5 of a score near 1, which read_temp multiplies. With TERMS = 2 the scores are
-// therefore accumulated in four parts of d_s, in TMEM buffers of their own, and added up in float32 registers.
+// therefore accumulated 128 columns of d_s at a time into a ring of TMEM buffers and added up in float32 registers.
 //
 // Slots at or past n_valid never reach a result: their scores are masked, P is 0 there, and the rows of V behind the
 // tile's last valid slot are zeroed in shared memory (0 * NaN would not be 0).
@@ -48,24 +48,23 @@ constexpr int RS_N = 64;          // N of both products: TERMS * MT
 constexpr int RS_SEG = 512;       // slots of a unit
 constexpr int RS_MAX_CS = 8;      // CTAs per cluster: 4, or 8
 constexpr int RS_SLAB = 512;      // columns of d_s per CTA at most (4 x 64 TMEM columns)
-constexpr int RS_VROWS = 32;      // slots per stage of the read
+constexpr int RS_VROWS = 48;      // slots per stage of the read
 constexpr int RS_ACC = 4;         // score accumulators in TMEM
+constexpr int RS_CHUNK = 2;       // TERMS = 2: k-blocks per accumulator (8 accumulation steps)
 constexpr int RS_S_COL = 256;     // their first TMEM column (the read's sums lie below)
 constexpr float RS_P_SCALE = 16384.f;     // P is scaled by 2^14
 constexpr int RS_KTILE = 128 * 128;       // K tile of a stage: up to 128 slots x 64 columns; Q's 64 rows behind it
-// Two rings, so that a page's second pass (from L2) streams beside the next page's first (from HBM).
-constexpr int RS_SSTAGE = RS_KTILE + RS_N * 128;
-constexpr int RS_SSTAGES = 3;
-constexpr int RS_VSTAGE = 4 * RS_VROWS * 128;    // 4 boxes of 32 slots x 64 columns
-constexpr int RS_VSTAGES = 4;
+constexpr int RS_STAGE = RS_KTILE + RS_N * 128;  // scores; the read: 4 boxes of 48 slots x 64 columns
+constexpr int RS_STAGES = 6;
 constexpr int RS_PBLK = RS_N * 128;       // P of 64 slots: one 128-byte swizzle row per N row
 constexpr int RS_STAT = 2 * 16 * RS_N;    // floats: [2][16 groups of 32 slots][MT]
 constexpr int RS_SM_WARPS = 8;            // softmax: 4 TMEM lane quarters (32 slots each) x 2 halves of the pairs
 constexpr int RS_FEW = 16;                // N rows of a unit whose read runs on the softmax warps
-constexpr int RS_THREADS = 32 * 15;       // 0-7 softmax, 8-11 epilogue, 12 and 14 producers, 13 MMA
-constexpr size_t RS_SMEM = 1024 + 8 * RS_PBLK + (size_t)RS_SSTAGES * RS_SSTAGE + (size_t)RS_VSTAGES * RS_VSTAGE +
-                           2 * RS_STAT * 4 + (2 * RS_SSTAGES + 2 * RS_VSTAGES + 2 * RS_ACC + 9) * 8 + 16;
-static_assert(RS_VSTAGES % 2 == 0, "a stage of V goes to the same four warps each time round the ring");
+constexpr int RS_THREADS = 32 * 14;       // 0-7 softmax, 8-11 epilogue, 12 producer, 13 MMA
+constexpr size_t RS_SMEM = 1024 + 8 * RS_PBLK + (size_t)RS_STAGES * RS_STAGE + 2 * RS_STAT * 4 +
+                           (2 * RS_STAGES + 2 * RS_ACC + 9) * 8 + 16;
+static_assert(RS_STAGES % 2 == 0, "a stage of V goes to the same four warps each time round the ring");
+static_assert(4 * RS_VROWS * 128 <= RS_STAGE, "a stage of the read fits");
 
 struct __align__(16) SharedTile {
   int page, start, count, nv;  // pairs [start, start + count) in grouped order; nv: the page's most valid slots
@@ -302,29 +301,6 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t pa
       : "memory");
   return ok != 0;
 }
-// Whether the phase of this parity is complete, without waiting.
-__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ bool mbar_test_cluster(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
 // Bounded wait for a barrier that other CTAs of the cluster arrive on.
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity) {
   if (mbar_try_wait_cluster(bar, parity)) return true;
@@ -348,13 +324,12 @@ __device__ __forceinline__ void bulk_s2s(uint32_t dst_cluster, const void* src, 
 // ----------------------------------------------------------------------------------------------------- read
 struct RsSmem {
   unsigned char* p;       // [8 blocks of 64 slots][RS_PBLK]
-  unsigned char* sst;     // the scores' ring
-  unsigned char* vst;     // the read's ring
+  unsigned char* stages;  // the ring
   float* smax;            // [2][16][MT]: by the parity of the unit, per 32 slots
   float* ssum;            // [2][16][MT]
   // p_full and sums: [0] units whose read runs on the tensor core, [1] units of few pairs. Each has one set of waiters,
   // which sees every phase.
-  uint64_t *full, *empty, *vfull, *vempty, *s_full, *s_empty, *p_full, *o_full, *o_empty, *stat, *sums, *seen, *v_done;
+  uint64_t *full, *empty, *s_full, *s_empty, *p_full, *o_full, *o_empty, *stat, *sums, *seen, *v_done;
   uint32_t* tmem;
   volatile int* abort_flag;
 };
@@ -379,15 +354,12 @@ struct RsRing {
 __device__ __forceinline__ RsSmem rs_smem(unsigned char* base) {
   RsSmem s;
   s.p = base;
-  s.sst = base + 8 * RS_PBLK;
-  s.vst = s.sst + RS_SSTAGES * RS_SSTAGE;
-  s.smax = reinterpret_cast<float*>(s.vst + RS_VSTAGES * RS_VSTAGE);
+  s.stages = base + 8 * RS_PBLK;
+  s.smax = reinterpret_cast<float*>(s.stages + RS_STAGES * RS_STAGE);
   s.ssum = s.smax + RS_STAT;
   s.full = reinterpret_cast<uint64_t*>(s.ssum + RS_STAT);
-  s.empty = s.full + RS_SSTAGES;
-  s.vfull = s.empty + RS_SSTAGES;
-  s.vempty = s.vfull + RS_VSTAGES;
-  s.s_full = s.vempty + RS_VSTAGES;
+  s.empty = s.full + RS_STAGES;
+  s.s_full = s.empty + RS_STAGES;
   s.s_empty = s.s_full + RS_ACC;
   s.p_full = s.s_empty + RS_ACC;
   s.o_full = s.p_full + 2;
@@ -452,7 +424,7 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
   const int rank = (int)cluster_rank();
   const int cluster = blockIdx.x / cs, n_clusters = gridDim.x / cs;
   const int nkb = (a.d_s + 63) / 64;
-  const int kpc = TERMS == 2 ? max(2, (nkb + RS_ACC - 1) / RS_ACC) : nkb;  // k-blocks per score accumulator
+  const int kpc = TERMS == 2 ? RS_CHUNK : nkb;                     // k-blocks per score accumulator
   const int x0 = rank * a.slab;                                    // this CTA's columns of d_s
   const int my_boxes = max(0, min(a.slab, a.d_s - x0) + 63) / 64;  // in boxes of 64
   const int quarters = ns / 32;                                    // of the TMEM lanes hold slots
@@ -463,13 +435,9 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
     prefetch_tensormap(&map_q8);
     prefetch_tensormap(&map_k);
     prefetch_tensormap(&map_v);
-    for (int i = 0; i < RS_SSTAGES; ++i) {
+    for (int i = 0; i < RS_STAGES; ++i) {
       mbar_init(&s.full[i], 1);
       mbar_init(&s.empty[i], 1);
-    }
-    for (int i = 0; i < RS_VSTAGES; ++i) {
-      mbar_init(&s.vfull[i], 1);
-      mbar_init(&s.vempty[i], 1);
     }
     for (int i = 0; i < RS_ACC; ++i) {
       mbar_init(&s.s_full[i], 1);
@@ -502,6 +470,7 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
   cur.find(a, cluster, n_units, n_clusters);
   // few pairs: the read runs on the softmax warps (which are all there with 128 slots a CTA)
   auto is_few = [&](const RsUnit& w) { return w.t.count * TERMS <= RS_FEW && ns == 128; };
+  auto s_stages = [&](const RsUnit& w) { return w.u < n_units && rank * ns < w.nv ? nkb : 0; };
   auto v_stages = [&](const RsUnit& w) { return (w.nv + RS_VROWS - 1) / RS_VROWS * ((my_boxes + 3) / 4); };
   // A wait that runs out sets the abort flag; from then on the softmax and epilogue warps wait for nothing and run
   // through their units on whatever is there, so that the named barrier stays matched.
@@ -513,82 +482,75 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
   };
 
   if (warp == 12) {
-    // --------------------------------------------------------------------------------------------- producer: K and Q
+    // --------------------------------------------------------------------------------------------- producer
     if (elect_one()) {
       // The clusters hold a page each that is to be read again and one that is arriving, about the size of L2: K's
       // lines are kept, V's pass (the second of a tied page) lets them go.
-      const uint64_t keep = policy_evict_last();
+      const uint64_t keep = policy_evict_last(), let_go = policy_evict_first();
       RsRing ring{0, 0};
       uint32_t used = 0;
       bool ok = true;
-      for (; cur.u < n_units && ok; cur.find(a, cur.u + n_clusters, n_units, n_clusters)) {
-        if (rank * ns >= cur.nv) continue;
-        const int y = cur.t.page * a.page_rows + cur.seg0 + rank * ns;
-        const bool few = cur.t.count <= 8;  // eight rows of Q a term; what lies in the others is not looked at
+      auto scores = [&](const RsUnit& w) {
+        if (w.u >= n_units || rank * ns >= w.nv) return;
+        const int y = w.t.page * a.page_rows + w.seg0 + rank * ns;
+        const bool few = w.t.count <= 8;  // eight rows of Q a term; what lies in the others is not looked at
         const uint32_t tx = (uint32_t)((few ? 8 : MT) * TERMS + ns) * 128;
-        for (int kb = 0; kb < nkb; ++kb) {
-          if (used >= RS_SSTAGES) ok = mbar_wait_spin(&s.empty[ring.st], ring.phase ^ 1);
+        for (int kb = 0; kb < nkb && ok; ++kb) {
+          if (used >= RS_STAGES) ok = mbar_wait_spin(&s.empty[ring.st], ring.phase ^ 1);
           if (!ok) break;
           uint64_t* bar = &s.full[ring.st];
-          unsigned char* st = s.sst + ring.st * RS_SSTAGE;
+          unsigned char* st = s.stages + ring.st * RS_STAGE;
           mbar_arrive_expect_tx(bar, tx);
           tma_load_2d_hint(st, &map_k, kb * 64, y, bar, keep);
           if (few) {
 #pragma unroll
             for (int x = 0; x < TERMS; ++x)
-              tma_load_2d(st + RS_KTILE + x * MT * 128, &map_q8, kb * 64, x * a.n_pairs + cur.t.start, bar);
+              tma_load_2d(st + RS_KTILE + x * MT * 128, &map_q8, kb * 64, x * a.n_pairs + w.t.start, bar);
           } else {
-            tma_load_3d(st + RS_KTILE, &map_q, kb * 64, cur.t.start, 0, bar);
+            tma_load_3d(st + RS_KTILE, &map_q, kb * 64, w.t.start, 0, bar);
           }
-          ring.next(RS_SSTAGES);
+          ring.next(RS_STAGES);
           ++used;
         }
-      }
-      if (!ok) *s.abort_flag = 1;
-      // the copies in flight end before the CTA's shared memory goes away
-      for (uint32_t i = min(used, (uint32_t)RS_SSTAGES); i > 0; --i) {
-        ring.back(RS_SSTAGES);
-        mbar_wait_bounded(&s.full[ring.st], ring.phase);
-      }
-    }
-    __syncwarp();
-  } else if (warp == 14) {
-    // --------------------------------------------------------------------------------------------- producer: V
-    if (elect_one()) {
-      const uint64_t let_go = policy_evict_first();
-      RsRing ring{0, 0};
-      uint32_t used = 0;
-      bool ok = true;
-      for (; cur.u < n_units && ok; cur.find(a, cur.u + n_clusters, n_units, n_clusters)) {
-        const int y = cur.t.page * a.page_rows + cur.seg0;
-        for (int b = 0; b < (cur.nv + RS_VROWS - 1) / RS_VROWS && ok; ++b)
+      };
+      auto values = [&](const RsUnit& w) {
+        const int y = w.t.page * a.page_rows + w.seg0;
+        for (int b = 0; b < (w.nv + RS_VROWS - 1) / RS_VROWS && ok; ++b)
           for (int h = 0; h < my_boxes; h += 4) {
             const int n = min(4, my_boxes - h);
-            if (used >= RS_VSTAGES) ok = mbar_wait_spin(&s.vempty[ring.st], ring.phase ^ 1);
+            if (used >= RS_STAGES) ok = mbar_wait_spin(&s.empty[ring.st], ring.phase ^ 1);
             if (!ok) break;
-            uint64_t* bar = &s.vfull[ring.st];
-            unsigned char* st = s.vst + ring.st * RS_VSTAGE;
+            uint64_t* bar = &s.full[ring.st];
+            unsigned char* st = s.stages + ring.st * RS_STAGE;
             mbar_arrive_expect_tx(bar, (uint32_t)(a.v3d ? 4 : n) * RS_VROWS * 128);
             if (a.v3d)  // four boxes of 64 columns in one copy (those past d_s arrive as zeros)
               tma_load_3d_hint(st, &map_v, 0, y + b * RS_VROWS, (x0 >> 6) + h, bar, let_go);
             else
               for (int i = 0; i < n; ++i)
                 tma_load_2d_hint(st + i * RS_VROWS * 128, &map_v, x0 + (h + i) * 64, y + b * RS_VROWS, bar, let_go);
-            ring.next(RS_VSTAGES);
+            ring.next(RS_STAGES);
             ++used;
           }
+      };
+      scores(cur);
+      while (cur.u < n_units && ok) {
+        nxt.find(a, cur.u + n_clusters, n_units, n_clusters);
+        scores(nxt);
+        values(cur);
+        cur = nxt;
       }
       if (!ok) *s.abort_flag = 1;
-      for (uint32_t i = min(used, (uint32_t)RS_VSTAGES); i > 0; --i) {
-        ring.back(RS_VSTAGES);
-        mbar_wait_bounded(&s.vfull[ring.st], ring.phase);
+      // the copies in flight end before the CTA's shared memory goes away
+      for (uint32_t i = min(used, (uint32_t)RS_STAGES); i > 0; --i) {
+        ring.back(RS_STAGES);
+        mbar_wait_bounded(&s.full[ring.st], ring.phase);
       }
     }
     __syncwarp();
   } else if (warp == 13) {
     // --------------------------------------------------------------------------------------------- MMA issuer
     if (elect_one()) {
-      RsRing rs{0, 0}, rv{0, 0};
+      RsRing ring{0, 0};
       uint32_t big = 0, few = 0, acc = 0;  // units whose read runs here, and on the softmax warps
       bool ok = true;
       const uint32_t id_s = umma_idesc(FMT, FMT, 128, RS_N);
@@ -596,115 +558,74 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
       // operand descriptors: the constant part, and addresses in 16-byte units (14 bits: the address of a CTA's shared
       // memory carries its cluster rank above them)
       const uint64_t dk = umma_desc_k_sw128(0), dv = umma_desc_mn_sw128(0, RS_VROWS * 128);
-      const uint32_t s0 = (smem_u32(s.sst) >> 4) & 0x3FFFu, v0 = (smem_u32(s.vst) >> 4) & 0x3FFFu;
-      const uint32_t p0 = (smem_u32(s.p) >> 4) & 0x3FFFu;
-      // One stage at a time of the next unit's scores and of this unit's read, whichever has its operands: the two
-      // rings stream side by side, and neither product waits for the other's exchange.
-      int s_kb = 0, s_end = 0;                    // k-blocks of the scores
-      int v_b = 0, v_h = 0, v_end = 0, v_nv = 0;  // 32-slot blocks and box groups of the read
-      bool p_here = false;
-      auto start_scores = [&](const RsUnit& w) {
-        s_kb = 0;
-        s_end = w.u < n_units && rank * ns < w.nv ? nkb : 0;
-      };
-      auto step_scores = [&]() -> bool {
-        const uint32_t buf = acc % RS_ACC, use = acc / RS_ACC;
-        const int in = s_kb % kpc;
-        if (in == 0 && use > 0 && !mbar_test(&s.s_empty[buf], (use - 1) & 1)) return false;
-        if (!mbar_test(&s.full[rs.st], rs.phase)) return false;
-        tc_fence_after();
-        const uint64_t da = dk + (s0 + rs.st * (RS_SSTAGE / 16)), db = da + RS_KTILE / 16;
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-          tc_mma<0>(taddr + RS_S_COL + buf * RS_N, da + ks * 2, db + ks * 2, id_s, in > 0 || ks > 0);
-        tc_commit(&s.empty[rs.st]);
-        rs.next(RS_SSTAGES);
-        ++s_kb;
-        if (in == kpc - 1 || s_kb == s_end) {
-          tc_commit(&s.s_full[buf]);
-          ++acc;
-        }
-        return true;
-      };
-      auto step_read = [&]() -> bool {
-        if (!p_here) {
-          // the epilogue of the last such unit has read its sums, and every CTA's block of P is here
-          if (big > 0 && !mbar_test(s.o_empty, (big - 1) & 1)) return false;
-          if (!mbar_test_cluster(&s.p_full[0], big & 1)) return false;
-          p_here = true;
-        }
-        if (v_b < v_end) {
-          if (!mbar_test(&s.vfull[rv.st], rv.phase)) return false;
+      const uint32_t st0 = (smem_u32(s.stages) >> 4) & 0x3FFFu, p0 = (smem_u32(s.p) >> 4) & 0x3FFFu;
+      auto scores = [&](const RsUnit& w) {
+        if (w.u >= n_units || rank * ns >= w.nv) return;
+        for (int k0 = 0; k0 < nkb && ok; k0 += kpc, ++acc) {
+          const uint32_t buf = acc % RS_ACC, use = acc / RS_ACC;
+          if (use > 0 && !(ok = mbar_wait_spin(&s.s_empty[buf], (use - 1) & 1))) break;
           tc_fence_after();
-          const int n = min(4, my_boxes - v_h);
-          const int left = v_nv - v_b * RS_VROWS, steps = min(RS_VROWS / 16, (left + 15) / 16);
-          if (left < steps * 16) {  // rows of V behind the last valid slot: zeros (0 * NaN would not be 0)
-            unsigned char* base = s.vst + rv.st * RS_VSTAGE;
-            for (int i = 0; i < n; ++i)
-              for (int c = left * 8; c < steps * 16 * 8; ++c)
-                *reinterpret_cast<uint4*>(base + i * RS_VROWS * 128 + c * 16) = make_uint4(0, 0, 0, 0);
-            fence_proxy_async_smem();
+          const int k1 = min(nkb, k0 + kpc);
+          for (int kb = k0; kb < k1; ++kb) {
+            if (!(ok = mbar_wait_spin(&s.full[ring.st], ring.phase))) break;
+            tc_fence_after();
+            const uint64_t da = dk + (st0 + ring.st * (RS_STAGE / 16)), db = da + RS_KTILE / 16;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+              tc_mma<0>(taddr + RS_S_COL + buf * RS_N, da + ks * 2, db + ks * 2, id_s, kb > k0 || ks > 0);
+            tc_commit(&s.empty[ring.st]);
+            ring.next(RS_STAGES);
           }
-          const uint64_t dx = dv + (v0 + rv.st * (RS_VSTAGE / 16));
-          // slots [32 b, 32 b + 32) of P: half a block of 64
-          const uint64_t dp = dk + (p0 + (v_b >> 1) * (RS_PBLK / 16) + (v_b & 1) * 4);
-          for (int ks = 0; ks < steps; ++ks)
-            // columns [128 t, 128 t + 128) of the slab: two boxes (the second may be stale: lanes nobody reads)
-            for (int t = 0; t < (n + 1) / 2; ++t)
-              tc_mma<0>(taddr + (uint32_t)(v_h / 2 + t) * RS_N, dx + t * (2 * RS_VROWS * 128 / 16) + ks * 128,
-                        dp + ks * 2, id_o, v_b > 0 || ks > 0);
-          tc_commit(&s.vempty[rv.st]);
-          rv.next(RS_VSTAGES);
-          v_h += 4;
-          if (v_h >= my_boxes) {
-            v_h = 0;
-            ++v_b;
-          }
+          if (!ok) break;
+          tc_commit(&s.s_full[buf]);
         }
-        return true;
       };
-      auto run = [&](bool read) {  // the scores started, and the read of a unit of many pairs
-        bool r_done = !read;
-        long long t0 = clock64();
-        for (uint32_t idle = 0; s_kb < s_end || !r_done;) {
-          bool moved = false;
-          if (s_kb < s_end) moved = step_scores();
-          if (!r_done && step_read()) {
-            moved = true;
-            r_done = v_b >= v_end;
-            if (r_done) tc_commit(s.o_full);
-          }
-          if (moved) {
-            idle = 0;
-          } else if ((++idle & 255u) == 0u) {
-            if (idle == 256u) t0 = clock64();
-            else if (clock64() - t0 > XENCB_WAIT_CYCLES) {
-              flag_error(XENCB_DEV_TIMEOUT);
-              ok = false;
-              return;
+      auto values = [&](const RsUnit& w) {
+        for (int b = 0; b < (w.nv + RS_VROWS - 1) / RS_VROWS && ok; ++b) {
+          const int left = w.nv - b * RS_VROWS, steps = min(RS_VROWS / 16, (left + 15) / 16);
+          for (int h = 0; h < my_boxes; h += 4) {
+            const int n = min(4, my_boxes - h);
+            if (!(ok = mbar_wait_spin(&s.full[ring.st], ring.phase))) break;
+            tc_fence_after();
+            if (left < steps * 16) {  // rows of V behind the last valid slot: zeros (0 * NaN would not be 0)
+              unsigned char* base = s.stages + ring.st * RS_STAGE;
+              for (int i = 0; i < n; ++i)
+                for (int c = left * 8; c < steps * 16 * 8; ++c)
+                  *reinterpret_cast<uint4*>(base + i * RS_VROWS * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+              fence_proxy_async_smem();
             }
+            const uint64_t dx = dv + (st0 + ring.st * (RS_STAGE / 16));
+            for (int ks = 0; ks < steps; ++ks) {
+              const int slot = b * RS_VROWS + ks * 16;  // its 16 slots of P lie in one block of 64
+              const uint64_t dp = dk + (p0 + (slot >> 6) * (RS_PBLK / 16) + ((slot & 63) >> 3));
+              // columns [128 t, 128 t + 128) of the slab: two boxes (the second may be stale: lanes nobody reads)
+              for (int t = 0; t < (n + 1) / 2; ++t)
+                tc_mma<0>(taddr + (uint32_t)(h / 2 + t) * RS_N, dx + t * (2 * RS_VROWS * 128 / 16) + ks * 128, dp, id_o,
+                          b > 0 || ks > 0);
+            }
+            tc_commit(&s.empty[ring.st]);
+            ring.next(RS_STAGES);
           }
         }
+        if (ok) tc_commit(s.o_full);
       };
-      start_scores(cur);
-      run(false);
+      scores(cur);
       while (cur.u < n_units && ok) {
         nxt.find(a, cur.u + n_clusters, n_units, n_clusters);
-        start_scores(nxt);
+        scores(nxt);
         if (is_few(cur)) {
-          run(false);
-          // the softmax warps take V's stages: a wait for a later use of a stage is one for a parity, so it may only
+          // the softmax warps take these stages: a wait for a later use of a stage is one for a parity, so it may only
           // begin when every use before it is complete
           mbar_arrive(s.v_done);
           if (ok) ok = mbar_wait_spin(s.v_done, few & 1);
           ++few;
-          rv.skip(v_stages(cur), RS_VSTAGES);
+          ring.skip(v_stages(cur), RS_STAGES);
         } else {
-          v_b = v_h = 0;
-          v_end = my_boxes > 0 ? (cur.nv + RS_VROWS - 1) / RS_VROWS : 0;
-          v_nv = cur.nv;
-          p_here = false;
-          run(true);
+          // the epilogue of the last such unit has read its sums, and every CTA's block of P is here
+          if (ok && big > 0) ok = mbar_wait_spin(s.o_empty, (big - 1) & 1);
+          if (ok) ok = mbar_wait_cluster(&s.p_full[0], big & 1);
+          tc_fence_after();
+          if (ok) values(cur);
           ++big;
         }
         cur = nxt;
@@ -752,9 +673,10 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
           __syncwarp();
         }
       };
-      // The read of a unit of few pairs: O[16 rows, 64 columns] of this warp = P . V, the rows being the pairs' hi rows, then
-      // their lo rows (TERMS = 2), or 16 pairs. Warp w takes the w-th 64 columns of the slab; the four warps of a stage
-      // hand it back together.
+      // The read of a unit of few pairs: O^T[64 columns, N] of this warp = V^T . P^T with N = 8 or 16: four pairs' hi rows
+      // and their lo rows (TERMS = 2) or 8 pairs to a tile of 8. Warp w takes the w-th 64 columns of the slab; the four
+      // warps of a stage hand it back together. mma.sync bounds it (a tile of 16 x 8 x 16 takes 32 cycles of a
+      // scheduler): the columns as its 16 rows need half the products that the pairs as its rows did.
       auto read_few = [&](const RsUnit& w, uint32_t un, uint32_t nth, RsRing rg) {
         done(*s.abort_flag || mbar_wait_cluster(&s.p_full[1], nth & 1));
         const int hgroups = (my_boxes + 3) / 4, hg = warp >> 2;
@@ -763,24 +685,31 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
           if (lane == 0) mbar_arrive(s.v_done);
           return;
         }
+        const bool two = w.t.count * TERMS > 8;
         const int mtx = lane >> 3, r8 = lane & 7;
-        const int prow = TERMS == 2 ? (mtx & 1) * MT + r8 : (mtx & 1) * 8 + r8;  // (prow % 8 == r8)
+        // P: matrices (tile 0, slots 0-7), (tile 0, 8-15), (tile 1, 0-7), (tile 1, 8-15); row r8 of a tile
+        const int pair_of = TERMS == 2 ? (mtx >> 1) * 4 + (r8 & 3) : (mtx >> 1) * 8 + r8;
+        const int prow = TERMS == 2 ? (r8 >> 2) * MT + pair_of : pair_of;
         const uint32_t pa = smem_u32(s.p) + prow * 128;
-        const uint32_t vrow = (uint32_t)(warp & 3) * (RS_VROWS * 128) + (r8 + (mtx & 1) * 8) * 128;
-        float acc_o[8][4];
+        // V: matrices (slots 0-7, columns 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15), transposed
+        const uint32_t vrow = (uint32_t)(warp & 3) * (RS_VROWS * 128) + (r8 + (mtx >> 1) * 8) * 128;
+        float acc_o[4][2][4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc_o[i][0] = acc_o[i][1] = acc_o[i][2] = acc_o[i][3] = 0.f;
-        rg.skip(hg, RS_VSTAGES);
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) acc_o[i][x][0] = acc_o[i][x][1] = acc_o[i][x][2] = acc_o[i][x][3] = 0.f;
+        rg.skip(hg, RS_STAGES);
         for (int b = 0; b < (w.nv + RS_VROWS - 1) / RS_VROWS; ++b) {
-          done(*s.abort_flag || mbar_wait_spin(&s.vfull[rg.st], rg.phase));
-          const uint32_t va = smem_u32(s.vst) + rg.st * RS_VSTAGE + vrow;
+          done(*s.abort_flag || mbar_wait_spin(&s.full[rg.st], rg.phase));
+          const uint32_t va = smem_u32(s.stages) + rg.st * RS_STAGE + vrow;
           const int left = w.nv - b * RS_VROWS;
 #pragma unroll
           for (int ks = 0; ks < RS_VROWS / 16; ++ks) {
             if (ks * 16 >= left) break;
             const int slot = b * RS_VROWS + ks * 16;
-            uint32_t a0, a1, a2, a3;
-            ldsm_x4(pa + (slot >> 6) * RS_PBLK + (((((slot & 63) >> 3) + (mtx >> 1)) ^ r8) << 4), a0, a1, a2, a3);
+            uint32_t p[4];
+            ldsm_x4(pa + (slot >> 6) * RS_PBLK + (((((slot & 63) >> 3) + (mtx & 1)) ^ (prow & 7)) << 4), p[0], p[1],
+                    p[2], p[3]);
             uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;  // rows of V behind the last valid slot: zeros
             const int over = left - ks * 16;
             if (over < 16) {
@@ -789,50 +718,67 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
               keep1 = (k + 8 < over ? 0xffffu : 0u) | (k + 9 < over ? 0xffff0000u : 0u);
             }
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              uint32_t b0, b1, b2, b3;
-              ldsm_x4_t(va + ks * 2048 + (((n * 2 + (mtx >> 1)) ^ r8) << 4), b0, b1, b2, b3);
-              mma16816<T>(acc_o[2 * n], a0, a1, a2, a3, b0 & keep0, b1 & keep1);
-              mma16816<T>(acc_o[2 * n + 1], a0, a1, a2, a3, b2 & keep0, b3 & keep1);
+            for (int m = 0; m < 4; ++m) {
+              uint32_t a0, a1, a2, a3;
+              ldsm_x4_t(va + ks * 2048 + (((m * 2 + (mtx & 1)) ^ r8) << 4), a0, a1, a2, a3);
+              a0 &= keep0; a1 &= keep0; a2 &= keep1; a3 &= keep1;
+              mma16816<T>(acc_o[m][0], a0, a1, a2, a3, p[0], p[1]);
+              if (two) mma16816<T>(acc_o[m][1], a0, a1, a2, a3, p[2], p[3]);
             }
           }
           __syncwarp();
           named_bar_sync(2 + hg, 128);
-          if ((warp & 3) == 0 && lane == 0 && !*s.abort_flag) mbar_arrive(&s.vempty[rg.st]);
+          if ((warp & 3) == 0 && lane == 0 && !*s.abort_flag) mbar_arrive(&s.empty[rg.st]);
           __syncwarp();
-          rg.skip(hgroups, RS_VSTAGES);
+          rg.skip(hgroups, RS_STAGES);
         }
         if (lane == 0) mbar_arrive(s.v_done);
         done(*s.abort_flag || mbar_wait_cluster(&s.sums[1], nth & 1));
-        const int seg = w.u % a.segs, pair = lane >> 2;
+        const int seg = w.u % a.segs;
         const float* smax = s.smax + (un & 1) * 16 * MT;
         const float* ssum = s.ssum + (un & 1) * 16 * MT;
-#pragma unroll
-        for (int g = 0; g < (TERMS == 2 ? 1 : 2); ++g) {
-          const int i = pair + 8 * g;
-          if (i >= w.t.count) continue;
+        // lane i: pair i's coefficient
+        float coef = 0.f;
+        if (lane < w.t.count) {
           float m = a.softmax ? -CUDART_INF_F : 0.f, l = 0.f;
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            m = fmaxf(m, smax[e * MT + i]);
-            l += ssum[e * MT + i];
+            m = fmaxf(m, smax[e * MT + lane]);
+            l += ssum[e * MT + lane];
           }
-          const int64_t pos = w.t.start + i;
-          float coef;
+          const int64_t pos = w.t.start + lane;
           if (a.softmax) coef = l != 0.f ? 1.f / l : 0.f;
           else coef = rsqrtf((float)a.pnv[pos]) / f16_range_scale(m);
-          if (rank == 0 && warp == 0 && (lane & 3) == 0) a.ml[pos * a.segs + seg] = make_float2(m, l);
-          float* dst = a.part + (pos * a.segs + seg) * a.d_s + x0;
+          if (rank == 0 && warp == 0) a.ml[pos * a.segs + seg] = make_float2(m, l);
+        }
+        __syncwarp();
 #pragma unroll
-          for (int n = 0; n < 8; ++n) {
-            const int x = warp * 64 + n * 8 + (lane & 3) * 2;
-            const float o0 = TERMS == 2 ? acc_o[n][0] + acc_o[n][2] : acc_o[n][2 * g];
-            const float o1 = TERMS == 2 ? acc_o[n][1] + acc_o[n][3] : acc_o[n][2 * g + 1];
-            if (x < a.slab && x0 + x < a.d_s) *reinterpret_cast<float2*>(dst + x) = make_float2(o0 * coef, o1 * coef);
+        for (int x = 0; x < 2; ++x) {
+          if (x == 1 && !two) break;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {  // this lane's N = 2 (lane % 4) + e
+            const int n = (lane & 3) * 2 + e;
+            const int pr = TERMS == 2 ? x * 4 + (n & 3) : x * 8 + n;
+            const float ci = __shfl_sync(0xffffffffu, coef, pr);
+            float* dst = a.part + ((int64_t)(w.t.start + pr) * a.segs + seg) * a.d_s + x0;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              float lo = acc_o[m][x][e], hi = acc_o[m][x][2 + e];  // columns (lane / 4) and 8 further
+              if (TERMS == 2) {  // the lo rows' parts lie two lanes further
+                lo += __shfl_xor_sync(0xffffffffu, lo, 2);
+                hi += __shfl_xor_sync(0xffffffffu, hi, 2);
+              }
+              const int c = warp * 64 + m * 16 + (lane >> 2);
+              if (pr < w.t.count && (TERMS == 1 || (lane & 2) == 0)) {
+                if (c < a.slab && x0 + c < a.d_s) dst[c] = lo * ci;
+                if (c + 8 < a.slab && x0 + c + 8 < a.d_s) dst[c + 8] = hi * ci;
+              }
+            }
           }
         }
       };
       scores(cur);
+      ring.skip(s_stages(cur), RS_STAGES);
       while (cur.u < n_units) {
         nxt.find(a, cur.u + n_clusters, n_units, n_clusters);
         const SharedTile t = cur.t;
@@ -920,10 +866,11 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
           for (int r = 0; r < cs; ++r)
             st_async_f32(cluster_map(&ssum[group * MT + lane], r), l, cluster_map(&s.sums[few], r));
         __syncwarp();
+        ring.skip(s_stages(nxt), RS_STAGES);
+        scores(nxt);  // (and with them every stage before this unit's V has been used: see v_done)
         if (few) read_few(cur, unit, unit - big, ring);
         else ++big;
-        ring.skip(v_stages(cur), RS_VSTAGES);
-        scores(nxt);
+        ring.skip(v_stages(cur), RS_STAGES);
         was_big = !few;
         ++unit;
         cur = nxt;
