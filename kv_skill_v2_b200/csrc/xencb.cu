@@ -166,13 +166,13 @@ struct GemmPlan {
   size_t part_bytes;
 };
 
-GemmPlan plan_gemm_tc(int64_t M, int N, int K, int sms) {
+GemmPlan plan_gemm_tc(int64_t M, int N, int K, int sms, int min_splits = 1) {
   GemmPlan p;
   p.tc = true;
   const int64_t tiles = ((N + TC_BM - 1) / TC_BM) * ((M + TC_BN - 1) / TC_BN);
   const int kblocks = (K + TC_BK - 1) / TC_BK;
   int64_t s = sms / tiles;  // one CTA per SM (the stage ring takes most of the shared memory)
-  if (s < 1) s = 1;
+  if (s < min_splits) s = min_splits;
   if (s > kblocks) s = kblocks;
   p.kps = (int)((kblocks + s - 1) / s) * TC_BK;
   p.splits = (K + p.kps - 1) / p.kps;
@@ -268,14 +268,14 @@ int tensor_map_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, co
 // `xbuf` (M*K float32, may be null when TX is float) stages a 16-bit X as float32 for the TMA path.
 template <typename TX>
 int launch_gemm(const void* X, int64_t M, int K, const float* W, int N, int sms, float* part, float* xbuf,
-                int* row_done, cudaStream_t st, GemmPlan* used, const void* w_prep = nullptr) {
+                int* row_done, cudaStream_t st, GemmPlan* used, const void* w_prep = nullptr, int min_splits = 1) {
   // 3xF16 (weights split once by xencb_weights_prep, X split here with a power-of-two scale per row) whenever the
   // prepared weights are given: half the MMAs of 3xTF32, and no per-k-block split of W
   const bool f16x3 = w_prep != nullptr;
   if (f16x3 && K % 8 == 0 && aligned(w_prep, 256) && aligned(X, 16) && xbuf && M <= INT32_MAX / 2 &&
       N <= INT32_MAX / 2 && wprep_pairs(N, K) * 2 * H3_BM <= INT32_MAX) {
     const bool two = M > H3_BN;  // more than one row tile: two CTAs per SM (see gemm_f16x3.cuh)
-    const GemmPlan p = plan_gemm_tc(M, N, K, (two ? 2 : 1) * sms);
+    const GemmPlan p = plan_gemm_tc(M, N, K, (two ? 2 : 1) * sms, min_splits);
     __half* xs = reinterpret_cast<__half*>(xbuf);  // [X_hi; X_lo]: 2 M K halves = M K floats of staging
     float* x_inv = reinterpret_cast<float*>(reinterpret_cast<char*>(xbuf) + align_up((size_t)M * K * sizeof(float), 256));
     launch_pdl(split_rows_f16x2_kernel<TX>, dim3((unsigned)M), dim3(SR_THREADS), 0, st, static_cast<const TX*>(X), M,
@@ -303,7 +303,7 @@ int launch_gemm(const void* X, int64_t M, int K, const float* W, int N, int sms,
   }
   const bool tc_ok = (K % 4 == 0) && aligned(W, 16) && (std::is_same<TX, float>::value ? aligned(X, 16) : xbuf != nullptr);
   if (tc_ok) {
-    const GemmPlan p = plan_gemm_tc(M, N, K, sms);
+    const GemmPlan p = plan_gemm_tc(M, N, K, sms, min_splits);
     const float* xf = static_cast<const float*>(X);
     if (!std::is_same<TX, float>::value) {
       const int64_t n = M * (int64_t)K;
@@ -337,6 +337,16 @@ int launch_gemm(const void* X, int64_t M, int K, const float* W, int N, int sms,
 // ------------------------------------------------------------------------------------------------ adapters
 // Extra workspace of a projection with adapters: one more split partial (behind the GEMM's) and t [n_rows, rank].
 size_t adapt_slice_bytes(int64_t M, int N) { return align_up((size_t)M * N * sizeof(float), 256); }
+// A projection with adapters splits d_in at least every AD_KPS columns: the tensor core's accumulator loses about
+// 2^-24 of its value at every 16-column step, towards zero, and 2048 rows x 5120 columns in one run were 6.6e-6 off
+// (1.4e-6 in splits of 1280); the row kernels add the splits in float32.
+int adapt_min_splits(int K) { return (K + AD_KPS - 1) / AD_KPS; }
+// Bytes a call's partials take beyond gemm_part_bytes: the low-rank slice, and the splits above where there are more.
+size_t adapt_part_extra(int64_t M, int N, int K, int sms) {
+  const size_t have = gemm_part_bytes(M, N, K, sms);
+  const size_t want = align_up((size_t)(adapt_min_splits(K) + 1) * M * N * sizeof(float), 256);
+  return adapt_slice_bytes(M, N) + (want > have ? want - have : 0);
+}
 size_t adapt_t_bytes(int64_t M, int rank) { return align_up((size_t)M * rank * AD_MAX_SPLITS * sizeof(float), 256); }
 
 int check_adapters(const char* what, const AdaptArgs& ad, int dtype) {
@@ -922,7 +932,7 @@ static int project_in_impl(const void* h, int h_dtype, int64_t n_rows, int d_m, 
   int rc = device_info(&di);
   if (rc) return rc;
   const int nch = (d_s + PIN_CHUNK - 1) / PIN_CHUNK;
-  const size_t slice = adapters ? adapt_slice_bytes(n_rows, d_s) : 0;
+  const size_t slice = adapters ? adapt_part_extra(n_rows, d_s, d_m, di.sms) : 0;
   const size_t g_bytes = gemm_ws_bytes(n_rows, d_s, d_m, di.sms, true) + slice;
   const size_t nq_bytes = align_up((size_t)n_rows * nch * sizeof(float), 256);
   const size_t rd_bytes = align_up((size_t)n_rows * sizeof(int), 256);
@@ -939,6 +949,7 @@ static int project_in_impl(const void* h, int h_dtype, int64_t n_rows, int d_m, 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   GemmPlan gp;
   AdaptArgs ad{};
+  const int min_splits = adapters ? adapt_min_splits(d_m) : 1;
   if (adapters) {
     ad = *adapters;
     plan_adapters(&ad, h, n_rows, d_m, d_s, di.sms);
@@ -953,13 +964,14 @@ static int project_in_impl(const void* h, int h_dtype, int64_t n_rows, int d_m, 
   switch (h_dtype) {
     case XENCB_F32:
       rc = launch_gemm<float>(h, n_rows, d_m, w_in, d_s, di.sms, part, w_prep ? xbuf : nullptr, row_done, st, &gp,
-                              w_prep);
+                              w_prep, min_splits);
       break;
     case XENCB_F16:
-      rc = launch_gemm<__half>(h, n_rows, d_m, w_in, d_s, di.sms, part, xbuf, row_done, st, &gp, w_prep);
+      rc = launch_gemm<__half>(h, n_rows, d_m, w_in, d_s, di.sms, part, xbuf, row_done, st, &gp, w_prep, min_splits);
       break;
     default:
-      rc = launch_gemm<__nv_bfloat16>(h, n_rows, d_m, w_in, d_s, di.sms, part, xbuf, row_done, st, &gp, w_prep);
+      rc = launch_gemm<__nv_bfloat16>(h, n_rows, d_m, w_in, d_s, di.sms, part, xbuf, row_done, st, &gp, w_prep,
+                                      min_splits);
       break;
   }
   if (rc) return rc;
@@ -1684,7 +1696,7 @@ static int project_out_impl(const float* r, int64_t n_rows, int d_s, const float
   int rc = device_info(&di);
   if (rc) return rc;
   const int nch = (d_m + PIN_CHUNK - 1) / PIN_CHUNK;
-  const size_t slice = adapters ? adapt_slice_bytes(n_rows, d_m) : 0;
+  const size_t slice = adapters ? adapt_part_extra(n_rows, d_m, d_s, di.sms) : 0;
   const size_t g_bytes = gemm_ws_bytes(n_rows, d_m, d_s, di.sms, false) + slice;
   const size_t d_bytes = align_up((size_t)n_rows * d_m * sizeof(float), 256);
   const size_t np_bytes = align_up((size_t)n_rows * nch * 3 * sizeof(float), 256);
@@ -1710,7 +1722,8 @@ static int project_out_impl(const float* r, int64_t n_rows, int d_s, const float
     rc = launch_adapt_shrink<float>(r, ad, adapt_dtype, st);
     if (rc) return rc;
   }
-  rc = launch_gemm<float>(r, n_rows, d_s, w_out, d_m, di.sms, part, w_prep ? xbuf : nullptr, nullptr, st, &gp, w_prep);
+  rc = launch_gemm<float>(r, n_rows, d_s, w_out, d_m, di.sms, part, w_prep ? xbuf : nullptr, nullptr, st, &gp, w_prep,
+                          adapters ? adapt_min_splits(d_s) : 1);
   if (rc) return rc;
   if (adapters) {  // the low-rank term is one more split partial
     rc = launch_adapt_expand(part + (size_t)gp.splits * n_rows * d_m, ad, adapt_dtype, st);
@@ -1774,7 +1787,9 @@ int xencb_project_out(const float* r, int64_t n_rows, int d_s, const float* w_ou
 // ------------------------------------------------------------------------------------------------ with adapters
 size_t xencb_project_in_adapted_workspace(int64_t n_rows, int d_m, int d_s, int rank) {
   const size_t base = xencb_project_in_workspace(n_rows, d_m, d_s);
-  return base && rank > 0 ? base + adapt_slice_bytes(n_rows, d_s) + adapt_t_bytes(n_rows, rank) : 0;
+  DevInfo di;
+  if (!base || rank <= 0 || device_info(&di)) return 0;
+  return base + adapt_part_extra(n_rows, d_s, d_m, di.sms) + adapt_t_bytes(n_rows, rank);
 }
 
 int xencb_project_in_adapted(const void* h, int h_dtype, int64_t n_rows, int d_m, const float* w_in, const void* w_prep,
@@ -1796,7 +1811,9 @@ int xencb_project_in_adapted(const void* h, int h_dtype, int64_t n_rows, int d_m
 
 size_t xencb_project_out_adapted_workspace(int64_t n_rows, int d_s, int d_m, int rank) {
   const size_t base = xencb_project_out_workspace(n_rows, d_s, d_m);
-  return base && rank > 0 ? base + adapt_slice_bytes(n_rows, d_m) + adapt_t_bytes(n_rows, rank) : 0;
+  DevInfo di;
+  if (!base || rank <= 0 || device_info(&di)) return 0;
+  return base + adapt_part_extra(n_rows, d_m, d_s, di.sms) + adapt_t_bytes(n_rows, rank);
 }
 
 int xencb_project_out_adapted(const float* r, int64_t n_rows, int d_s, const float* w_out, const void* w_prep,
@@ -1851,7 +1868,7 @@ static int launch_page_copies(void* const* pools, const int64_t* row_bytes, int 
     for (int i = n; i <= PG_POOLS; ++i) pp.first[i] = (int)slices;
     pp.slices = (int)slices;
     // (the first copy launch follows the plan kernel, later ones a copy that has read the same list)
-    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(8 * sms, max_moves * slices));
+    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(64 * (int64_t)sms, max_moves * slices));
     if (vec) launch_pdl(pages_copy_kernel<uint4>, dim3(grid), dim3(PG_COPY_THREADS), 0, st, pp, moves, n_moves);
     else launch_pdl(pages_copy_kernel<uint16_t>, dim3(grid), dim3(PG_COPY_THREADS), 0, st, pp, moves, n_moves);
     XENCB_CHECK_LAUNCH("pages_copy launch");
