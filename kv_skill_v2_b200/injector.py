@@ -125,6 +125,8 @@ class ExternalSkillInjector:
         if adapters_in is None and adapters_out is None:
             self._adapters = None
         else:
+            if not self._fast_interface():
+                raise NotImplementedError("adapters need a ModelInterface or a LinearInterface")
             if adapter_of is None:
                 raise ValueError("set_adapters: adapter_of is required")
             self._adapters = (adapters_in, adapters_out, adapter_of)
@@ -344,6 +346,8 @@ class XEncInjector(ExternalSkillInjector):
         return delta.view(*lead, -1)
 
     def _duck_finish(self, h, hn, r, gcal, li, inject, selector=None):
+        if self._adapters is not None:
+            raise NotImplementedError("adapters need a ModelInterface or a LinearInterface")
         lead = h.shape[:-1]
         itf = self.itf
         hn3 = hn.view(*lead, -1)
@@ -645,8 +649,6 @@ class LibraryInjector(XEncInjector):
             idx, wk, w, _ = ops.route(q, pages.S, rows_per_lib=rpl, top_k=self.top_k, route_temp=self.route_temp,
                                       n_chunks_of=pages.n_chunks_of, row_w=sel_col)
         # with a selector most rows read nothing at most depths: the sparse plan spreads the live rows' work
-        if not self._fast_interface() and self._adapters is not None:
-            raise NotImplementedError("adapters need a ModelInterface or a LinearInterface")
         if self.record_attn or self.force_attn is not None:
             r = self._read_with_diagnostics(h, li, q, pages, idx, wk, rpl, sparse=sel_col is not None)
         elif self.share_pages and ops.shared_supported(pages):

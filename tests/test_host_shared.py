@@ -9,6 +9,7 @@ import torch
 
 from kv_skill_v2_b200 import _native as N
 from kv_skill_v2_b200 import ops
+from tests._fixtures import TinyReader
 
 
 def _pages(d=64):
@@ -70,3 +71,38 @@ def test_page_operators_refuse_bad_arguments():
     assert fork(m=0) == N.EINVAL and fork(parents=None) == N.EINVAL and fork(ws_bytes=8) == N.EINVAL
     assert fork(m=1 << 20, C=1 << 12) == N.ENOTSUP
     assert N.lib().xencb_pages_fork_workspace(0, 4) == 0 and N.lib().xencb_pages_compact_workspace(0) == 0
+
+
+class _OwnInterface:
+    """An interface object of the caller's: query, gate, gain and write only."""
+
+    d_s, inject_layers = 16, [0]
+
+    def query(self, hn):
+        return hn[..., :16]
+
+    def gate(self, hn, li):
+        return hn[..., :1]
+
+    def gain(self, li):
+        return 1.0
+
+    def write(self, r):
+        return r
+
+
+@pytest.mark.parametrize("kind", ["XEncInjector", "LibraryInjector"])
+def test_adapters_need_a_known_interface(kind):
+    """An interface that the kernels do not see refuses adapters, rather than leaving them out."""
+    import kv_skill_v2_b200 as pkg
+
+    inj = getattr(pkg, kind)(TinyReader(32, 2), _OwnInterface())
+    ad = pkg.ops.Adapters(a=torch.zeros(1, 2, 32), b=torch.zeros(1, 16, 2))
+    with pytest.raises(NotImplementedError):
+        inj.set_adapters(ad, None, torch.zeros(1, dtype=torch.int32))
+    inj._adapters = (ad, None, torch.zeros(1, dtype=torch.int32))  # (an interface exchanged after set_adapters)
+    with pytest.raises(NotImplementedError):
+        inj._duck_finish(torch.zeros(1, 1, 32), torch.zeros(1, 32), torch.zeros(1, 16), 1.0, 0, False)
+    inj.set_adapters()
+    assert inj._adapters is None
+    inj.detach()
