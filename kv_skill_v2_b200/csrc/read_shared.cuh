@@ -34,7 +34,8 @@
 // therefore accumulated 128 columns of d_s at a time into a ring of TMEM buffers and added up in float32 registers.
 //
 // Slots at or past n_valid never reach a result: their scores are masked, P is 0 there, and the rows of V behind the
-// tile's last valid slot are zeroed in shared memory (0 * NaN would not be 0).
+// tile's last valid slot are zeroed in shared memory (0 * NaN would not be 0). Pairs of one page with different n_valid
+// share a tile: slots between theirs are multiplied by 0 for the shorter ones, so those have to be finite.
 #pragma once
 
 #include <math_constants.h>
