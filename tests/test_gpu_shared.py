@@ -300,3 +300,21 @@ def test_pages_of_few_and_of_many_pairs_in_turn(dev, d_s, page_rows, out):
     got = ops.read_shared(q, pages, idx, wk, rows_per_lib=R, out_dtype=out)
     check(got, pages, q, idx, wk, R, out)
     assert ops.device_status(dev) == 0
+
+
+@pytest.mark.parametrize("slots,out", [(torch.float16, torch.float32), (torch.bfloat16, torch.float32),
+                                       (torch.float16, torch.bfloat16)])
+@pytest.mark.parametrize("d_s,page_rows", [(2048, 512), (1024, 300), (256, 1100)])
+def test_the_tail_of_a_page_gives_the_same_bits(dev, d_s, page_rows, slots, out):
+    """A page's last few pairs take another form of the read, and which pairs those are is up to the order of the
+    count: the result is the same to the bit, run after run and with a row alone."""
+    from kv_skill_v2_b200 import ops
+    R = 69  # 64 + 5, 2 * 32 + 5
+    pages, q, idx, wk = make(dev, 31, rows=R, shared=3, k=0, page_rows=page_rows, d_s=d_s, slots=slots)
+    whole = ops.read_shared(q, pages, idx, wk, rows_per_lib=R, out_dtype=out)
+    for _ in range(5):
+        assert torch.equal(whole, ops.read_shared(q, pages, idx, wk, rows_per_lib=R, out_dtype=out))
+    for row in (0, 33, 68):
+        one = ops.read_shared(q[row:row + 1].contiguous(), pages, idx[row:row + 1].contiguous(),
+                              wk[row:row + 1].contiguous(), rows_per_lib=1, out_dtype=out)
+        assert torch.equal(whole[row:row + 1], one)
