@@ -8,6 +8,8 @@ Public API, mirroring the reference's xenc package for this path:
     ModelInterface, LinearInterface, make_interface, EncoderLens, interface_param_groups,
     save_interface, load_interface, count_params (xenc/interface.py)
     DEPTHS, CAND, rho_layer_map, injection_layers, for_reader, KVSkill (xenc/__init__.py, xenc/depth_skill.py)
+Beyond it, for many requests over shared documents: PagedLibrary.fork / drop / select / reserve / compact,
+LibraryInjector(share_pages=True), set_adapters with ops.Adapters.
 The compute runs in libxencb.so (include/xencb.h), hand-written CUDA for sm_100a; `ops` exposes one
 function per C-ABI entry point.
 """
