@@ -10,8 +10,8 @@
 // costs the same however few rows it holds, so it is taken from 16 rows per adapter on.
 //
 // Measured beside the projection (d_in 4096 -> 2048): 64 rows with 64 adapters of rank 16, shrink 10.6 us and expand
-// 5.3 us of a call of 31 us (the GEMM 11.6 us); 2048 rows of 4 adapters of rank 32 (5120 -> 2048), shrink 78 us and
-// expand 26 us of 366 us; by rows the same took 159 and 249 us.
+// 5.3 us of a call of 31 us (the GEMM 11.6 us); 2048 rows of 4 adapters of rank 32 (5120 -> 2048), shrink 19 us
+// (78 us with float32 multiplications) and expand 27 us of 267 us; by rows the same took 159 and 249 us.
 #pragma once
 
 #include "gemm_f16x3.cuh"
@@ -191,6 +191,63 @@ __global__ void __launch_bounds__(128) adapt_shrink_tile_kernel(const TX* __rest
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (ty * 4 + i < rows && tx * 4 + j < nj) t[(row0 + ty * 4 + i) * p.r + j0 + tx * 4 + j] = acc[i][j];
+}
+
+// The same with mma.sync where x and A have one 16-bit type and 16-byte rows (products exact, sums in float32): a warp
+// takes 16 rows x 32 ranks. The order of a dot product's terms is free, so lane l holds 8 consecutive columns of its rows
+// (one 16-byte load from global memory, nothing staged) and the four lanes of a row make two k-steps of them. The tensor
+// core's sums, which lose up to 2^-24 a step towards zero, are added up in float32 every 128 columns.
+template <typename T>
+__global__ void __launch_bounds__(128) adapt_shrink_mma_kernel(const T* __restrict__ x, const AdaptArgs p) {
+  pdl_trigger();
+  pdl_wait();
+  int64_t row0;
+  int rows;
+  ad_tile(p, blockIdx.x, row0, rows);
+  const int w0 = (threadIdx.x >> 5) * 16;  // this warp's first row of the tile
+  if (rows <= w0) return;
+  const int ad = ad_of(p, row0);
+  if (ad < 0) return;
+  const int lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3;
+  const int j0 = blockIdx.y * AD_TILE_J, nj = min(AD_TILE_J, p.r - j0);
+  const int steps = (p.d_in + AD_BK - 1) / AD_BK, per = (steps + p.splits - 1) / p.splits;
+  const int kb = blockIdx.z * per * AD_BK, ke = min(p.d_in, kb + per * AD_BK);
+  const bool in0 = w0 + r < rows, in1 = w0 + r + 8 < rows;
+  const T* x0 = x + (row0 + w0 + r) * p.d_in + q * 8;
+  const T* x1 = x0 + 8 * (int64_t)p.d_in;
+  const T* ar = static_cast<const T*>(p.a) + ((int64_t)ad * p.r + j0 + r) * p.d_in + q * 8;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  float sum[4][4] = {};
+  for (int k0 = kb; k0 < ke; k0 += 4 * AD_BK) {
+    float acc[4][4] = {};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int k = k0 + u * AD_BK;
+      const bool in = k + q * 8 < ke;  // (d_in is a multiple of 8, and so is every split's end)
+      const uint4 a0 = in && in0 ? *reinterpret_cast<const uint4*>(x0 + k) : zero;
+      const uint4 a1 = in && in1 ? *reinterpret_cast<const uint4*>(x1 + k) : zero;
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const uint4 b = in && n * 8 + r < nj ? *reinterpret_cast<const uint4*>(ar + (int64_t)n * 8 * p.d_in + k) : zero;
+        mma16816<T>(acc[n], a0.x, a1.x, a0.y, a1.y, b.x, b.y);
+        mma16816<T>(acc[n], a0.z, a1.z, a0.w, a1.w, b.z, b.w);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[n][e] += acc[n][e];
+  }
+  float* t = p.t + ((int64_t)blockIdx.z * p.n_rows + row0 + w0 + r) * p.r + j0;
+#pragma unroll
+  for (int n = 0; n < 4; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int j = n * 8 + q * 2 + e;
+      if (j >= nj) continue;
+      if (in0) t[j] = sum[n][e];
+      if (in1) t[8 * (int64_t)p.r + j] = sum[n][2 + e];
+    }
 }
 
 // out[row][n] = s_a sum_j (sum_z t[z][row][j]) B[a][n][j]: 64 rows x 128 columns a CTA of 128 threads, 8 x 8 outputs.

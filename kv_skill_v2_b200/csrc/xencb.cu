@@ -388,10 +388,14 @@ int launch_adapt_shrink(const void* x, const AdaptArgs& ad, int dtype, cudaStrea
   const TX* xp = static_cast<const TX*>(x);
   auto go = [&](auto t) {
     using TA = decltype(t);
+    const dim3 tiles((unsigned)adapt_tile_count(ad), (unsigned)((ad.r + AD_TILE_J - 1) / AD_TILE_J), (unsigned)ad.splits);
+    if constexpr (std::is_same<TX, TA>::value && sizeof(TX) == 2)
+      if (adapt_tiles(ad) && ad.vec_in) {
+        launch_pdl(adapt_shrink_mma_kernel<TX>, tiles, dim3(128), 0, st, xp, ad);
+        return;
+      }
     if (adapt_tiles(ad))
-      launch_pdl(adapt_shrink_tile_kernel<TX, TA>,
-                 dim3((unsigned)adapt_tile_count(ad), (unsigned)((ad.r + AD_TILE_J - 1) / AD_TILE_J), (unsigned)ad.splits),
-                 dim3(128), 0, st, xp, ad);
+      launch_pdl(adapt_shrink_tile_kernel<TX, TA>, tiles, dim3(128), 0, st, xp, ad);
     else
       launch_pdl(adapt_shrink_row_kernel<TX, TA>, dim3((unsigned)ad.n_rows, (unsigned)((ad.r + 7) / 8)), dim3(256), 0,
                  st, xp, ad);

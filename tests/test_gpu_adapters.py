@@ -180,3 +180,19 @@ def test_captured_calls_with_their_own_workspaces(dev):
         graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(q1, eager) and not torch.equal(q2, eager)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("R,rpa,n,rank,d_in,d_out", [(16, 16, 1, 1, 8, 64), (200, 70, 3, 33, 2056, 256),
+                                                     (130, 17, 9, 40, 1000, 132), (64, 64, 1, 256, 5120, 128)])
+def test_tiles_of_one_16_bit_type(dev, dtype, R, rpa, n, rank, d_in, d_out):
+    """Rows and adapters of one 16-bit type, in tiles of rows that end inside a warp's 16 and ranks inside its 32."""
+    from kv_skill_v2_b200 import ops
+    s = _inputs(dev, 41, R, rpa, n, rank, d_in, d_out, dtype, dtype)
+    ad = ops.Adapters(a=s["a"], b=s["b"], scale=s["scale"])
+    q = ops.project_in(s["h"], s["w"], l2=False, rms=False, adapters=ad, adapter_of=s["of"], rows_per_adapter=rpa)[0]
+    of = s["of"].long().repeat_interleave(rpa)[:R]
+    low = torch.einsum("tk,trk->tr", s["h"].double(), s["a"].double()[of.clamp(min=0)])
+    low = torch.einsum("tr,tnr->tn", low, s["b"].double()[of.clamp(min=0)]) * s["scale"].double()[of.clamp(min=0)][:, None]
+    want = s["h"].double() @ s["w"].double().t() + low * (of >= 0)[:, None]
+    assert float((q.double() - want).abs().max()) <= TOL * float(want.abs().max())
