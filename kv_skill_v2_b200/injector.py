@@ -145,7 +145,7 @@ class ExternalSkillInjector:
             return ()
         a, b, of = self._adapters
         ts = [x for ad in (a, b) if ad is not None for x in (ad.a, ad.b, ad.scale) if x is not None] + [of]
-        return tuple((x.data_ptr(), tuple(x.shape), x.dtype) for x in ts) + (a is None, b is None)
+        return tuple((x.data_ptr(), tuple(x.shape), x.stride(), x.dtype) for x in ts) + (a is None, b is None)
 
     # subclasses provide _branch (delta in float32) and _inject (h + delta, rel)
 

@@ -106,3 +106,17 @@ def test_adapters_need_a_known_interface(kind):
     inj.set_adapters()
     assert inj._adapters is None
     inj.detach()
+
+
+def test_a_captured_step_is_keyed_by_the_adapters_layout():
+    """Adapters of one address, shape and type but other strides are other adapters to a captured step."""
+    from kv_skill_v2_b200 import LibraryInjector, make_interface
+
+    inj = LibraryInjector(TinyReader(16, 2), make_interface(16, 16, [0]))
+    a, of = torch.zeros(1, 16, 16), torch.zeros(1, dtype=torch.int32)
+    keys = set()
+    for x in (a, a.transpose(1, 2)):
+        inj.set_adapters(ops.Adapters(a=x, b=a), None, of)
+        keys.add(inj._adapter_key())
+    assert len(keys) == 2
+    inj.detach()
