@@ -264,11 +264,11 @@ XENCB_API int xencb_read_prefill(const float* q, int64_t n_rows, int d_s, const 
 /* Shared read: the result of xencb_read_decode with every page fetched once for all query rows that read it, whichever
  * Libraries they belong to (Libraries whose tables name the same pages, many rows of one Library, prompts with top-k
  * routing; xenc/injector.py:239-245, 263-265). The (row, routed chunk) pairs are grouped by page on the device and
- * each page is read by up to 64 of them at once on the tensor cores (32 for float32 results).
+ * each page is read by up to 64 of them at once on the tensor cores (32 for float32 results or bf16 slots).
  *   q       [n_rows, d_s] of q_dtype
  *   r_out   [n_rows, d_s] of out_dtype. XENCB_F32: q and the softmax weights enter the tensor cores as pairs of
- *           16-bit values (22 bits with f16 slots, 16 with bf16). XENCB_F16 / XENCB_BF16: one rounding of each, and
- *           one of the result.
+ *           16-bit values (22 bits with f16 slots, 16 with bf16). XENCB_F16 / XENCB_BF16: one rounding of the result
+ *           and, with f16 slots, one of each.
  *   idx, wk as xencb_route writes them; a chunk may appear more than once in a row; entries with idx < 0 or
  *           wk == 0 are skipped, a row without any gives 0. idx >= n_chunks or a page outside the pool is skipped and
  *           flagged (XENCB_DEV_BADPAGE).

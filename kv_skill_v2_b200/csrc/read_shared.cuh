@@ -16,7 +16,7 @@
 // passes through shared memory twice, but its second pass comes from L2: a cluster holds one or two pages at a time.
 // The roles run one unit apart: the scores of the next unit are computed while this one's softmax and exchange run,
 // and the epilogue stores one unit while the next one's P is made.
-// A unit of few pairs (8, or 16 for 16-bit results) takes its read product on the softmax warps instead, with mma.sync:
+// A unit of few pairs (16 / TERMS) takes its read product on the softmax warps instead, with mma.sync:
 // one 16-row tile holds all of its pairs, hi and lo together, and the tensor core's MN-major operand is read at about
 // 27 bytes a cycle (162 cycles per 16 slots x 128 columns), which ldmatrix is not.
 // shared_combine adds a row's pairs in the order of its routing: results do not depend on how pairs were grouped.
@@ -24,9 +24,10 @@
 // Why this orientation: with the pairs as the 128 rows (of which a tile fills 64) the read cost 290 cycles per
 // 16 slots x 256 columns (M = 128, N = 256, MN-major B), this way 2 x 81 (M = 128, N = 64).
 //
-// Precision. The operands are 16-bit. TERMS = 2 (float32 outputs): q and P enter as hi + lo pairs, two of the MMA's
+// Precision. The operands are 16-bit. TERMS = 2 (float32 outputs, bf16 slots): q and P enter as hi + lo pairs, two of the MMA's
 // N columns per pair, which keeps 22 bits with f16 slots and 16 with bf16; the halves are added in float32.
-// TERMS = 1 (16-bit outputs): one rounding of q and of P, as the other tensor-core reads do. q is scaled by a power of
+// bf16 slots take it for 16-bit outputs too: one rounding of q and P to 8 bits added half of the result's own rounding.
+// TERMS = 1 (16-bit outputs of f16 slots): one rounding of q and of P, to 11 bits. q is scaled by a power of
 // two per row and P by 2^14, so f16's range is no limit.
 //
 // The tensor core's accumulator drops bits below its running value at every 16-term step, always towards zero; over

@@ -747,7 +747,8 @@ int plan_shared(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows, 
   if (n_pages * (int64_t)page_rows + 1024 > INT32_MAX)
     return fail(XENCB_ENOTSUP, "read_shared: the slot pool is too large for 32-bit TMA coordinates");
   p->n_pairs = n_rows * k;
-  p->terms = out_dtype == XENCB_F32 ? 2 : 1;
+  // bf16 operands keep 8 bits of q and P, which shows beside one rounding of the result (2.6e-3 against 1.7e-3)
+  p->terms = out_dtype == XENCB_F32 || slots_dtype == XENCB_BF16 ? 2 : 1;
   p->mt = RS_N / p->terms;
   p->cs = d_s <= 4 * RS_SLAB ? 4 : 8;
   p->ns = RS_SEG / p->cs;

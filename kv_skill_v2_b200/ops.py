@@ -597,10 +597,10 @@ def read_shared(q: torch.Tensor, pages: Pages, idx: torch.Tensor, wk: torch.Tens
     tables name the same pages (forks of a document), many rows on one document, prompts with top-k routing.
 
     q [R, d_s] float32 / float16 / bfloat16; idx, wk [R, k] as route gives them. out_dtype float32: 22 bits of q and of
-    the softmax weights (16 with bfloat16 slots); float16 / bfloat16: each rounded once, and the result. Slots that no row
-    reads may hold anything; where Libraries name one page with different n_valid, the values that any of them reads must
-    be finite (a weight of 0 multiplies them for the others). The workspace holds 8 d_s bytes per routed pair and 512
-    slots of its page (q in 16 bits, the page's partial result), so long prompts want a top_k. Raises
+    the softmax weights (16 with bfloat16 slots); float16 / bfloat16: the result rounded once (and, with float16 slots, q
+    and the weights). Slots that no row reads may hold anything; where Libraries name one page with different n_valid, the
+    values that any of them reads must be finite (a weight of 0 multiplies them for the others). The workspace holds up to
+    8 d_s bytes per routed pair and 512 slots of its page, so long prompts want a top_k. Raises
     NotImplementedError for float32 slots and d_s above 4096 or not a multiple of 8 (use read_decode)."""
     dev = _cuda("read_shared", q, pages.slots, pages.page_of, pages.n_valid, idx, wk)
     q = q.contiguous()
