@@ -49,12 +49,13 @@ __host__ __device__ inline int64_t wprep_pairs(int64_t n, int64_t k) {
   return ((n + H3_BM - 1) / H3_BM) * ((k + H3_BK - 1) / H3_BK);
 }
 
-// 2^e with max * 2^e in [2^14, 2^15) (e = 0 for max 0 or non-finite): exact power-of-two scale into f16 range.
+// 2^e with max * 2^e in [2^14, 2^15) (e = 0 for max 0 or non-finite): exact power-of-two scale into f16 range. It stops
+// at 2^126: 2^127 has no normal reciprocal, and 2^128, which a max below 2^-112 asks for, is no float at all.
 __device__ __forceinline__ float f16_range_scale(float mx) {
   if (!(mx > 0.f) || !isfinite(mx)) return 1.f;
   int ex;
   frexpf(mx, &ex);  // mx = f * 2^ex, f in [0.5, 1)
-  return ldexpf(1.f, 15 - ex);
+  return ldexpf(1.f, min(15 - ex, 126));
 }
 
 template <typename T>

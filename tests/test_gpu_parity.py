@@ -833,3 +833,23 @@ def test_attention_diagnostics_against_reference(dev, name):
             inj._branch(torch.from_numpy(base["h"]).to(dev), li)
     inj.detach()
     _status_clean(dev)
+
+
+@pytest.mark.parametrize("small", ["rows", "weights"])
+@pytest.mark.parametrize("size", [1e-30, 1e-34, 1e-36])
+def test_projection_gemm_f16x3_near_the_smallest_floats(dev, small, size):
+    """Rows (or a weight) so small that 2^15 over their largest value is no float32: the scale stops at 2^126, and every
+    value from 2^-126 up is still a normal f16 or two. Outputs stay above 2^-126, so the bar is the GEMM's 1e-5."""
+    from kv_skill_v2_b200 import ops
+    g = torch.Generator(device=dev).manual_seed(11)
+    R, d_s, d_m = 70, 512, 264
+    r = torch.randn(R, d_s, generator=g, device=dev)
+    W = torch.randn(d_m, d_s, generator=g, device=dev)
+    r, W = (r * size, W) if small == "rows" else (r, W * size)
+    r[5] = 0.0
+    r[:, ::9] = 0.0
+    h = torch.zeros(R, d_m, device=dev)
+    d, _, _ = ops.project_out(r, W, h, w_prep=ops.weights_prep(W), prefer_prep=True)
+    ref = r.double() / size @ W.double().t() if small == "rows" else r.double() @ (W.double() / size).t()
+    assert torch.isfinite(d).all() and rel_err(d.double() / size, ref) < 1e-5
+    assert (d[5] == 0).all()

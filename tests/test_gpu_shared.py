@@ -318,3 +318,24 @@ def test_the_tail_of_a_page_gives_the_same_bits(dev, d_s, page_rows, slots, out)
         one = ops.read_shared(q[row:row + 1].contiguous(), pages, idx[row:row + 1].contiguous(),
                               wk[row:row + 1].contiguous(), rows_per_lib=1, out_dtype=out)
         assert torch.equal(whole[row:row + 1], one)
+
+
+@pytest.mark.parametrize("slots", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("softmax,size,temp", [(True, 1e-34, TEMP), (True, 1e-36, TEMP), (True, 1e-34, TEMP / 1e-34),
+                                               (False, 1e-34, TEMP), (False, 1e-30, TEMP)])
+def test_queries_near_the_smallest_floats(dev, slots, out, softmax, size, temp):
+    """2^15 over the row's largest value is no float32 from 2^-112 down: the row's scale stops at 2^126. The linear read
+    is compared in units of `size` (its bound has an absolute part); its coefficient 1 / (2^126 sqrt(n)) keeps 20 bits,
+    half a step of which (2^-21) is below the bound's 2^-23 (d_s / 16)."""
+    from kv_skill_v2_b200 import ops
+    pages, q, idx, wk = make(dev, 14, rows=40, shared=5, k=3, page_rows=90, d_s=512, slots=slots)
+    q = q * size
+    q[:, ::7] = 0.0
+    q[3] = 0.0
+    got = ops.read_shared(q, pages, idx, wk, rows_per_lib=40, read_temp=temp, read_softmax=softmax, out_dtype=out)
+    if softmax:
+        check(got, pages, q, idx, wk, 40, out, temp=temp)
+    else:
+        check(got.double() / size, pages, q.double() / size, idx, wk, 40, out, softmax=False, norm=False)
+    assert ops.device_status(dev) == 0
