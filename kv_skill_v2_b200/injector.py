@@ -131,14 +131,18 @@ class ExternalSkillInjector:
                 raise ValueError("set_adapters: adapter_of is required")
             self._adapters = (adapters_in, adapters_out, adapter_of)
 
-    def _adapter_args(self, which: int, rows: int) -> dict:
-        """project_in's (which 0) or project_out's (1) adapter arguments for `rows` rows; empty without adapters."""
+    def _adapter_args(self, which: int, h: torch.Tensor) -> dict:
+        """project_in's (which 0) or project_out's (1) adapter arguments for the rows of h [B, T, d] or [B, d]; empty
+        without adapters. An adapter_of of another length is an earlier batch's: it would give the tokens of one request
+        to several adapters. (One entry serves a single sequence [T, d] too.)"""
         if self._adapters is None or self._adapters[which] is None:
             return {}
         of = self._adapters[2]
-        if of.numel() == 0 or rows % of.numel():
-            raise ValueError(f"set_adapters: adapter_of has {of.numel()} entries, the batch {rows} rows")
-        return {"adapters": self._adapters[which], "adapter_of": of, "rows_per_adapter": rows // of.numel()}
+        n, rows = of.numel(), h.numel() // h.shape[-1]
+        B = h.shape[0] if h.dim() > 1 else 1
+        if n == 0 or (n != B and not (n == 1 and h.dim() <= 2)):
+            raise ValueError(f"set_adapters: adapter_of has {n} entries, the batch {tuple(h.shape)} {B} rows")
+        return {"adapters": self._adapters[which], "adapter_of": of, "rows_per_adapter": rows // n}
 
     def _adapter_key(self) -> tuple:
         if self._adapters is None:
@@ -218,8 +222,10 @@ class XEncInjector(ExternalSkillInjector):
     def _fast_interface(self) -> bool:
         return isinstance(self.itf, (ModelInterface, LinearInterface))
 
-    def _query(self, h2: torch.Tensor, li: int, sel_fuse: Optional[LayerSelector] = None):
-        """(q [R, d_s], gate [R] | None, log_gain | None, z | None) for rows h2 [R, d_m] (fast interfaces).
+    def _query(self, h2: torch.Tensor, li: int, sel_fuse: Optional[LayerSelector] = None,
+               h: Optional[torch.Tensor] = None):
+        """(q [R, d_s], gate [R] | None, log_gain | None, z | None) for rows h2 [R, d_m] (fast interfaces); h is the
+        batch whose rows these are (adapters are per batch row).
 
         The per-layer parameters (gate_b[pos], log_gain[pos]) stay on the device and are read by the kernels, so
         the hook path has no host reads and can be captured in a CUDA graph."""
@@ -228,7 +234,7 @@ class XEncInjector(ExternalSkillInjector):
         if sel_fuse is not None:
             sel_w = sel_fuse.u.weight.detach().float().to(h2.device)
             sel_b = sel_fuse.u.bias.detach().float().to(h2.device)
-        more = self._adapter_args(0, h2.shape[0])
+        more = self._adapter_args(0, h2 if h is None else h)
         if isinstance(itf, LinearInterface):
             W = _on(itf.w_in.detach(), h2).float()
             q, _, _, z = ops.project_in(h2, W, sel_w=sel_w, sel_b=sel_b, w_prep=self._prep(W), **more)
@@ -314,7 +320,7 @@ class XEncInjector(ExternalSkillInjector):
         lead, d_m = h.shape[:-1], h.shape[-1]
         h2 = h.reshape(-1, d_m)
         if self._fast_interface():
-            q, g, log_gain, _ = self._query(h2, li)
+            q, g, log_gain, _ = self._query(h2, li, h=h)
             r = self._skill_read(q, li)
             r, gcal = self._calibrate(r, li)
             return self._finish(h, h2, r, g, gcal if not isinstance(gcal, torch.Tensor) else 1.0, li, inject,
@@ -329,7 +335,7 @@ class XEncInjector(ExternalSkillInjector):
         lead = h.shape[:-1]
         W, b = self._write_weights(h2)
         wp = self._prep(W)
-        more = self._adapter_args(1, h2.shape[0])
+        more = self._adapter_args(1, h)
         pm = self._pos_mask(h) if inject else None
         if extra is not None:  # a tensor calibration gain: fold into the per-row gate
             g = (g if g is not None else torch.ones(r.shape[0], device=r.device)) * extra.reshape(-1).float()
@@ -637,7 +643,7 @@ class LibraryInjector(XEncInjector):
             q, g, log_gain, idx, wk, w = routed
         else:
             if self._fast_interface():
-                q, g, log_gain, z = self._query(h2, li, sel_fuse=sel if fuse_sel else None)
+                q, g, log_gain, z = self._query(h2, li, sel_fuse=sel if fuse_sel else None, h=h)
             else:
                 hn = ops.rms_norm(h2)
                 q = self.itf.query(hn.view(*lead, -1)).reshape(-1, self.itf.d_s).float().contiguous()

@@ -415,7 +415,7 @@ class TopKLibraryInjector(LibraryInjector):
             idx = idx[:1]
         idx = _on(idx, h2)
         if self._fast_interface():
-            q, g, log_gain, _ = self._query(h2, li)
+            q, g, log_gain, _ = self._query(h2, li, h=h)
         else:
             hn = ops.rms_norm(h2)
             q = self.itf.query(hn.view(*lead, -1)).reshape(-1, self.itf.d_s).float().contiguous()

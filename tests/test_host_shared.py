@@ -120,3 +120,40 @@ def test_a_captured_step_is_keyed_by_the_adapters_layout():
         keys.add(inj._adapter_key())
     assert len(keys) == 2
     inj.detach()
+
+
+@pytest.mark.parametrize("entries,shape", [(4, (2, 2, 32)), (4, (8, 1, 32)), (4, (1, 64, 32)), (1, (3, 2, 32)),
+                                           (0, (2, 1, 32)), (2, (4, 32)), (8, (2, 4, 32))])
+@pytest.mark.parametrize("which", [0, 1])
+def test_an_adapter_of_of_another_batch_is_refused(entries, shape, which):
+    """Whatever divides the rows: the entries belong to batch rows."""
+    from kv_skill_v2_b200 import LibraryInjector, PagedLibrary
+    from kv_skill_v2_b200.interface import LinearInterface
+
+    itf = LinearInterface(torch.zeros(32, 16), torch.zeros(16, 32), [0]).requires_grad_(False)
+    ad = ops.Adapters(a=torch.zeros(1, 2, 32), b=torch.zeros(1, 16, 2))
+    out = ops.Adapters(a=torch.zeros(1, 2, 16), b=torch.zeros(1, 32, 2))
+    inj = LibraryInjector(TinyReader(32, 2), itf)
+    inj.load_library(PagedLibrary({0: _pages(16)}))
+    inj.set_adapters(ad if which == 0 else None, out if which else None, torch.zeros(entries, dtype=torch.int32))
+    h = torch.zeros(shape)
+    with torch.no_grad(), pytest.raises(ValueError, match="adapter_of"):
+        if which == 0:
+            inj._inject(h, 0)
+        else:  # (the read before it needs a GPU)
+            inj._finish(h, h.reshape(-1, 32), torch.zeros(h.numel() // 32, 16), None, 1.0, 0, True)
+    inj.detach()
+
+
+@pytest.mark.parametrize("entries,shape,each", [(2, (2, 2, 32), 2), (8, (8, 1, 32), 1), (1, (1, 64, 32), 64),
+                                                (4, (4, 32), 1), (1, (5, 32), 5), (1, (32,), 1)])
+def test_adapter_of_per_batch_row(entries, shape, each):
+    from kv_skill_v2_b200 import LibraryInjector
+    from kv_skill_v2_b200.interface import LinearInterface
+
+    inj = LibraryInjector(TinyReader(32, 2), LinearInterface(torch.zeros(32, 16), torch.zeros(16, 32), [0]))
+    inj.set_adapters(ops.Adapters(a=torch.zeros(1, 2, 32), b=torch.zeros(1, 16, 2)), None,
+                     torch.zeros(entries, dtype=torch.int32))
+    assert inj._adapter_args(0, torch.zeros(shape))["rows_per_adapter"] == each
+    assert inj._adapter_args(1, torch.zeros(shape)) == {}
+    inj.detach()
