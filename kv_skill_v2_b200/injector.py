@@ -65,6 +65,8 @@ def _needs_grad(*objs) -> bool:
 
 # graphs of the fused hook path captured directly on a caller's input buffer, per (layer, shape, ...)
 _PTR_GRAPHS = 4
+# settings of set_adapters whose captured steps are kept (the current one and the ones captured before it)
+_ADAPTER_SETS = 4
 
 class ExternalSkillInjector:
     """Forward-hook plumbing for a reader model (the deltaskill base class the reference subclasses)."""
@@ -597,6 +599,7 @@ class LibraryInjector(XEncInjector):
                 graph = torch.cuda.CUDAGraph()
                 with torch.cuda.graph(graph):
                     h_new_s, rel_s = self._run_lib_eager(h_static, li, inject, sel)
+                self._drop_stale_graphs()
                 # the entry keeps the prepared weights it captured alive
                 self._graphs[(base, h.data_ptr() if on_buffer else None)] = (
                     graph, None if on_buffer else h_static, h_new_s, rel_s, self.last_route, pages,
@@ -610,6 +613,16 @@ class LibraryInjector(XEncInjector):
         graph.replay()
         self.last_route = route_s
         return h_new_s.clone(), rel_s.clone()
+
+    def _drop_stale_graphs(self) -> None:
+        """Forget the captured steps (with their workspaces) of all but the last _ADAPTER_SETS settings of set_adapters:
+        requests that join and leave bring new tensors, and an entry keeps the ones it was captured with. Called before
+        an entry is added; nothing that it drops is running, as beginning a capture waits for the device."""
+        now = self._adapter_key()
+        sets = [k for k in dict.fromkeys(key[0][-1] for key in self._graphs) if k != now]
+        old = set(sets[:max(0, len(sets) - (_ADAPTER_SETS - 1))])
+        if old:
+            self._graphs = {k: v for k, v in self._graphs.items() if k[0][-1] not in old}
 
     def _run_lib_eager(self, h: torch.Tensor, li: int, inject: bool, sel: Optional[LayerSelector]):
         self._check_diagnostics()

@@ -188,3 +188,37 @@ def test_adapter_refusals(dev):
     with torch.no_grad(), pytest.raises(ValueError):
         inj._inject(h, LAYER)
     inj.detach()
+
+
+def test_captured_steps_of_earlier_adapters_do_not_pile_up(dev):
+    """Requests join and leave: every step brings other adapter tensors."""
+    from kv_skill_v2_b200 import LibraryInjector, ops
+    from kv_skill_v2_b200.interface import LinearInterface
+    g = torch.Generator(device=dev).manual_seed(8)
+    W_in = torch.randn(D_M, D_S, generator=g, device=dev) * D_M ** -0.5
+    W_out = torch.randn(D_S, D_M, generator=g, device=dev) * 0.2
+    lib = _library(dev, seed=9, ragged=False)
+    itf = LinearInterface(W_in, W_out, [LAYER]).to(dev).requires_grad_(False)
+    inj = LibraryInjector(TinyReader(D_M, 4).to(dev), itf, top_k=2)
+    inj.load_library(lib)
+    h = torch.randn(3, 1, D_M, generator=g, device=dev)
+    kept, sizes = [], []
+    with torch.no_grad():
+        inj._inject(h, LAYER)
+        plain = inj._inject(h, LAYER)[0]
+        for step in range(24):
+            ad = ops.Adapters(a=torch.randn(2, 4, D_M, generator=g, device=dev) * D_M ** -0.5,
+                              b=torch.randn(2, D_S, 4, generator=g, device=dev) * 0.2, scale=torch.ones(2, device=dev))
+            of = torch.randint(-1, 2, (3,), generator=g, device=dev, dtype=torch.int32)
+            inj.set_adapters(ad, None, of)
+            kept.append(ad)  # (the caller keeps them: no address comes back)
+            for _ in range(2):
+                got = inj._inject(h, LAYER)[0]
+            want = _reference(h, W_in, W_out, lib, LAYER, ad, ops.Adapters(a=torch.zeros(2, 1, D_S, device=dev),
+                              b=torch.zeros(2, D_M, 1, device=dev), scale=torch.zeros(2, device=dev)), of, 2, 10.0, 12.0)
+            assert rel_err(got - h, want) <= TOL
+            sizes.append(len(inj._graphs))
+        inj.set_adapters()
+        assert torch.equal(inj._inject(h, LAYER)[0], plain)
+    assert max(sizes) <= 8 and max(sizes[12:]) == max(sizes[:12]), sizes
+    inj.detach()
