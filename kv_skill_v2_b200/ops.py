@@ -602,6 +602,10 @@ def read_shared(q: torch.Tensor, pages: Pages, idx: torch.Tensor, wk: torch.Tens
     values that any of them reads must be finite (a weight of 0 multiplies them for the others). The workspace holds up to
     8 d_s bytes per routed pair and 512 slots of its page, so long prompts want a top_k. Raises
     NotImplementedError for float32 slots and d_s above 4096 or not a multiple of 8 (use read_decode)."""
+    # the kernels index both tables as dense [n_lib, C] int32
+    for name, t in (("page_of", pages.page_of), ("n_valid", pages.n_valid)):
+        if t.dtype != torch.int32 or t.dim() != 2 or t.shape != pages.page_of.shape or not t.is_contiguous():
+            raise ValueError(f"read_shared: {name} must be a contiguous int32 [n_lib, C] tensor")
     dev = _cuda("read_shared", q, pages.slots, pages.page_of, pages.n_valid, idx, wk)
     q = q.contiguous()
     wk = _f32(wk, "wk")

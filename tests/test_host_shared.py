@@ -157,3 +157,15 @@ def test_adapter_of_per_batch_row(entries, shape, each):
     assert inj._adapter_args(0, torch.zeros(shape))["rows_per_adapter"] == each
     assert inj._adapter_args(1, torch.zeros(shape)) == {}
     inj.detach()
+
+
+def test_read_shared_refuses_other_tables():
+    """page_of and n_valid are read as dense int32 [n_lib, C]: any other layout would be misread, or read past its end."""
+    q, idx, wk = torch.zeros(2, 64), torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, 1)
+    t = torch.zeros(2, 3, dtype=torch.int32)
+    for page_of, n_valid in ((t.long(), t), (t, t.long()), (t, t[:1]), (t, t[:, :2].contiguous()), (t.t().contiguous().t(), t),
+                             (t, t.t().contiguous().t()), (t[0], t[0]), (t.expand(4, 2, 3)[0].repeat(1, 2)[:, ::2], t)):
+        p = ops.Pages(slots=torch.zeros(2, 4, 64, dtype=torch.float16), page_of=page_of, n_valid=n_valid,
+                      S=torch.zeros(2, 3, 64))
+        with pytest.raises(ValueError, match="contiguous int32"):
+            ops.read_shared(q, p, idx, wk, rows_per_lib=1)
