@@ -67,6 +67,10 @@ def _needs_grad(*objs) -> bool:
 _PTR_GRAPHS = 4
 # settings of set_adapters whose captured steps are kept (the current one and the ones captured before it)
 _ADAPTER_SETS = 4
+# a captured step keeps its workspace, so shared reads that need more than this run eagerly. One hooked step (4096 -> 2048
+# -> 4096, 64 pages of 512) takes, eager and captured, 147 and 116 us with 4 MB of it (64 rows, top-4), 124 and 126 with
+# 34 MB (32 rows, all chunks), 482 and 481 with 34 MB (512 rows, top-4): from there the device hides the launches
+_GRAPH_WORKSPACE = 32 << 20
 
 class ExternalSkillInjector:
     """Forward-hook plumbing for a reader model (the deltaskill base class the reference subclasses)."""
@@ -536,6 +540,15 @@ class LibraryInjector(XEncInjector):
                 and self.force_attn is None and not torch.is_grad_enabled()
                 and not torch.cuda.is_current_stream_capturing())
 
+    def _large_shared_read(self, h: torch.Tensor, li: int) -> bool:
+        """Whether this call's shared read takes more workspace than a captured step may keep."""
+        if not self.share_pages:
+            return False
+        pages = self._pages(li, h)
+        k = self.top_k if 0 < self.top_k < pages.n_chunks else pages.n_chunks
+        need = ops.shared_workspace(pages, h.numel() // h.shape[-1], k)
+        return need > _GRAPH_WORKSPACE or (need == 0 and ops.shared_supported(pages))  # (0: more rows than one call takes)
+
     def _check_diagnostics(self) -> None:
         if self.training_attn and torch.is_grad_enabled():
             raise NotImplementedError("training_attn keeps the attention for a training loss (autograd); the xencb "
@@ -574,7 +587,7 @@ class LibraryInjector(XEncInjector):
 
     def _run_lib(self, h: torch.Tensor, li: int, inject: bool, sel: Optional[LayerSelector]):
         self._check_diagnostics()
-        if not self._graphable(h, inject, sel):
+        if not self._graphable(h, inject, sel) or self._large_shared_read(h, li):
             return self._run_lib_eager(h, li, inject, sel)
         # CUDA-graph replay: the first call for a (layer, shape, dtype, Library view) runs eagerly (which also
         # validates and sizes the workspaces), then captures the same launches on static buffers; later calls

@@ -590,9 +590,32 @@ def read_prefill(q: torch.Tensor, pages: Pages, w: torch.Tensor, *, rows_per_lib
     return out
 
 
+# Workspace of one launch of read_shared: 64 K routed pairs of d_s 2048, 1000 rows on every page of a 64-page document. A
+# fetch serves 32 (64) pairs, so slices cost little: 4096 rows on all of 64 pages of 512 x 2048 take 6550 us at once
+# (4.3 GB), 6850 us in slices of at most 1 GiB, 7130 us of 512 MiB; 16384 rows of top-4 routing 1743, 1811 and 1923 us.
+SHARED_WORKSPACE = 1 << 30
+
+
+def shared_slices(n_rows: int, rows_per_lib: int, size, limit: int) -> list:
+    """Row ranges [(r0, r1), ...] of a read_shared call whose workspaces size(rows) (bytes; 0: too many rows for one call)
+    stay within `limit`, or of one row: whole Libraries where one fits, else even parts of one Library each."""
+    fit = n_rows
+    while fit > 1 and not 0 < size(fit) <= limit:
+        fit = (fit + 1) // 2
+    if fit >= n_rows:
+        return [(0, n_rows)]
+    if fit >= rows_per_lib:
+        step = fit // rows_per_lib * rows_per_lib
+        return [(r, min(r + step, n_rows)) for r in range(0, n_rows, step)]
+    parts = -(-rows_per_lib // fit)
+    step = -(-rows_per_lib // parts)
+    return [(r, min(r + step, lib + rows_per_lib, n_rows)) for lib in range(0, n_rows, rows_per_lib)
+            for r in range(lib, min(lib + rows_per_lib, n_rows), step)]
+
+
 def read_shared(q: torch.Tensor, pages: Pages, idx: torch.Tensor, wk: torch.Tensor, *, rows_per_lib: int,
-                read_temp: float = 12.0, read_softmax: bool = True,
-                out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+                read_temp: float = 12.0, read_softmax: bool = True, out_dtype: torch.dtype = torch.float32,
+                max_workspace: int = SHARED_WORKSPACE) -> torch.Tensor:
     """r [R, d_s]: the read of read_decode with every page fetched once for all rows that read it -- Libraries whose
     tables name the same pages (forks of a document), many rows on one document, prompts with top-k routing.
 
@@ -600,7 +623,8 @@ def read_shared(q: torch.Tensor, pages: Pages, idx: torch.Tensor, wk: torch.Tens
     the softmax weights (16 with bfloat16 slots); float16 / bfloat16: the result rounded once (and, with float16 slots, q
     and the weights). Slots that no row reads may hold anything; where Libraries name one page with different n_valid, the
     values that any of them reads must be finite (a weight of 0 multiplies them for the others). The workspace holds up to
-    8 d_s bytes per routed pair and 512 slots of its page, so long prompts want a top_k. Raises
+    8 d_s bytes per routed pair and 512 slots of its page; rows whose pairs would take more than max_workspace bytes of it
+    are read in slices, with the same bits. Raises
     NotImplementedError for float32 slots and d_s above 4096 or not a multiple of 8 (use read_decode)."""
     # the kernels index both tables as dense [n_lib, C] int32
     for name, t in (("page_of", pages.page_of), ("n_valid", pages.n_valid)):
@@ -621,27 +645,43 @@ def read_shared(q: torch.Tensor, pages: Pages, idx: torch.Tensor, wk: torch.Tens
         raise ValueError("read_shared: idx must be int32 [R, k] matching wk")
     if out_dtype not in _DT:
         raise ValueError(f"read_shared: out_dtype {out_dtype} not supported (float32 / float16 / bfloat16)")
-    k = int(idx.shape[1])
+    k, rpl = int(idx.shape[1]), int(rows_per_lib)
+    if rpl <= 0 or -(-R // rpl) > pages.n_lib:
+        raise ValueError(f"read_shared: {R} rows, {rpl} per Library, need more than {pages.n_lib} Libraries")
     idx = idx.contiguous()
     r = torch.empty(R, d_s, dtype=out_dtype, device=dev)
     dt, odt = _hdt(slots, "slots"), _DT[out_dtype]
-    P, page_rows = slots.shape[0], pages.page_rows
+    P, page_rows, C = slots.shape[0], pages.page_rows, pages.n_chunks
     with _on_device(dev):
-        ws_bytes = N.lib().xencb_read_shared_workspace(R, k, d_s, P, page_rows, dt, odt)
-        if ws_bytes == 0:
-            N.check(N.EINVAL if min(R, k) <= 0 else N.ENOTSUP, "read_shared_workspace")
+        size = lambda rows: N.lib().xencb_read_shared_workspace(rows, k, d_s, P, page_rows, dt, odt)
+        parts, ws_bytes = [(0, R)], size(R)
+        if not 0 < ws_bytes <= max_workspace:
+            if size(min(R, 1)) == 0:
+                N.check(N.EINVAL if min(R, k) <= 0 else N.ENOTSUP, "read_shared_workspace")
+            parts = shared_slices(R, rpl, size, max_workspace)
+            ws_bytes = max(size(n) for n in {r1 - r0 for r0, r1 in parts})
         ws = _workspace(ws_bytes, dev)
-        N.call("xencb_read_shared", _ptr(q), _hdt(q, "q"), R, d_s, _ptr(slots), _ptr(_vpool(pages)), dt, P,
-               page_rows * d_s, page_rows, _ptr(pages.page_of), _ptr(pages.n_valid), pages.n_chunks, int(rows_per_lib),
-               pages.n_lib, _ptr(idx), _ptr(wk), k, float(read_temp), int(bool(read_softmax)), _ptr(r), odt, _ptr(ws),
-               ws.numel(), _stream(dev))
+        at = lambda t, row: t.data_ptr() + row * t.stride(0) * t.element_size()
+        for r0, r1 in parts:
+            lib, rows = r0 // rpl, r1 - r0
+            libs = -(-rows // rpl)
+            N.call("xencb_read_shared", at(q, r0), _hdt(q, "q"), rows, d_s, _ptr(slots), _ptr(_vpool(pages)), dt, P,
+                   page_rows * d_s, page_rows, at(pages.page_of, lib), at(pages.n_valid, lib), C, rpl, libs, at(idx, r0),
+                   at(wk, r0), k, float(read_temp), int(bool(read_softmax)), at(r, r0), odt, _ptr(ws), ws.numel(),
+                   _stream(dev))
     return r
+
+
+def shared_workspace(pages: Pages, n_rows: int, k: int, out_dtype: torch.dtype = torch.float32) -> int:
+    """Bytes of workspace for n_rows rows of k routed chunks in one read_shared call; 0: this pool, or so many rows in one
+    call, it does not take."""
+    return N.lib().xencb_read_shared_workspace(n_rows, k, pages.d_s, pages.slots.shape[0], pages.page_rows,
+                                               _hdt(pages.slots, "slots"), _DT[out_dtype])
 
 
 def shared_supported(pages: Pages) -> bool:
     """Whether read_shared takes this slot pool (f16 / bf16 slots, d_s % 8 == 0, d_s <= 4096)."""
-    return N.lib().xencb_read_shared_workspace(1, 1, pages.d_s, pages.slots.shape[0], pages.page_rows,
-                                               _hdt(pages.slots, "slots"), N.F32) > 0
+    return shared_workspace(pages, 1, 1) > 0
 
 
 def multi_supported(pages: Pages, n_rows: int, rows_per_lib: int) -> bool:

@@ -222,3 +222,35 @@ def test_captured_steps_of_earlier_adapters_do_not_pile_up(dev):
         assert torch.equal(inj._inject(h, LAYER)[0], plain)
     assert max(sizes) <= 8 and max(sizes[12:]) == max(sizes[:12]), sizes
     inj.detach()
+
+
+@pytest.mark.parametrize("top_k", [0, 2])
+def test_a_prompt_over_shared_pages_keeps_no_workspace(dev, monkeypatch, top_k):
+    """A shared read above the workspace limits runs in slices and is not captured; the rows are the same."""
+    import kv_skill_v2_b200.injector as module
+    from kv_skill_v2_b200 import LibraryInjector, ops
+    from kv_skill_v2_b200.interface import LinearInterface
+    g = torch.Generator(device=dev).manual_seed(12)
+    W_in = torch.randn(D_M, D_S, generator=g, device=dev) * D_M ** -0.5
+    W_out = torch.randn(D_S, D_M, generator=g, device=dev) * 0.2
+    lib = _library(dev, seed=13, ragged=False)
+    inj = LibraryInjector(TinyReader(D_M, 4).to(dev), LinearInterface(W_in, W_out, [LAYER]).to(dev).requires_grad_(False),
+                          top_k=top_k, share_pages=True)
+    inj.load_library(lib)
+    h = torch.randn(3, 200, D_M, generator=g, device=dev)
+    with torch.no_grad():
+        whole = inj._inject(h, LAYER)[0]
+        assert torch.equal(inj._inject(h, LAYER)[0], whole) and len(inj._graphs) == 1
+        need = ops.shared_workspace(lib.pages(LAYER), 600, top_k or 5)
+        monkeypatch.setattr(module, "_GRAPH_WORKSPACE", need - 1)
+        monkeypatch.setattr(ops.read_shared, "__kwdefaults__", {**ops.read_shared.__kwdefaults__, "max_workspace": need // 4})
+        inj._graphs.clear()
+        before = torch.cuda.memory_allocated()
+        for _ in range(3):
+            again = inj._inject(h, LAYER)[0]
+        assert torch.equal(again, whole) and not inj._graphs
+        torch.cuda.synchronize()
+        assert torch.cuda.memory_allocated() - before <= 3 * h.numel() * 4
+        inj._inject(h[:, :20].contiguous(), LAYER)
+        assert len(inj._graphs) == 1  # (a smaller step is captured as before)
+    inj.detach()

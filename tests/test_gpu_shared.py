@@ -339,3 +339,25 @@ def test_queries_near_the_smallest_floats(dev, slots, out, softmax, size, temp):
     else:
         check(got.double() / size, pages, q.double() / size, idx, wk, 40, out, softmax=False, norm=False)
     assert ops.device_status(dev) == 0
+
+
+@pytest.mark.parametrize("case", [dict(rows=70, shared=5, k=3, page_rows=200, d_s=256),
+                                  dict(n_lib=7, rows=9, shared=3, private=2, k=0, page_rows=600, d_s=128),
+                                  dict(n_lib=3, rows=41, shared=4, private=1, k=4, page_rows=90, d_s=512)])
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+def test_slices_give_the_same_bits(dev, case, out):
+    """A workspace limit cuts the rows into slices: within Libraries, at their borders, down to one row each."""
+    from kv_skill_v2_b200 import ops
+    rows = case["rows"]
+    pages, q, idx, wk = make(dev, 16, **case)
+    whole = ops.read_shared(q, pages, idx, wk, rows_per_lib=rows, out_dtype=out)
+    need = ops.shared_workspace(pages, q.shape[0], idx.shape[1], out)
+    for limit in (need // 2, need // 5, need // 30, 1):
+        got = ops.read_shared(q, pages, idx, wk, rows_per_lib=rows, out_dtype=out, max_workspace=limit)
+        assert torch.equal(got, whole)
+    # a last Library that is cut, and more rows than Libraries
+    cut = ops.read_shared(q[:-2], pages, idx[:-2], wk[:-2], rows_per_lib=rows, out_dtype=out, max_workspace=need // 5)
+    assert torch.equal(cut, whole[:-2])
+    with pytest.raises(ValueError):
+        ops.read_shared(q, pages, idx, wk, rows_per_lib=rows - 1, out_dtype=out, max_workspace=need // 5)
+    assert ops.device_status(dev) == 0

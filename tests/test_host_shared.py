@@ -169,3 +169,36 @@ def test_read_shared_refuses_other_tables():
                       S=torch.zeros(2, 3, 64))
         with pytest.raises(ValueError, match="contiguous int32"):
             ops.read_shared(q, p, idx, wk, rows_per_lib=1)
+
+
+def test_slices_of_a_shared_read():
+    """Every row once and in order, no slice above the limit unless it is one row, and none that holds parts of two
+    Libraries."""
+    import random
+
+    rng = random.Random(0)
+    for _ in range(2000):
+        rpl, n, per = rng.randint(1, 40), rng.randint(1, 200), rng.randint(1, 50)
+        limit, most = rng.randint(1, 3000), rng.choice([10 ** 9, rng.randint(1, 50)])
+
+        def size(rows):
+            return 0 if rows > most else 7 + per * rows
+
+        parts = ops.shared_slices(n, rpl, size, limit)
+        assert [r for a, b in parts for r in range(a, b)] == list(range(n))
+        for a, b in parts:
+            assert 0 < size(b - a) <= limit or b - a == 1
+            assert a // rpl == (b - 1) // rpl or a % rpl == 0
+        if 0 < size(n) <= limit:
+            assert parts == [(0, n)]
+
+
+def test_a_dense_prompt_over_shared_pages_is_sliced():
+    """4 x 2048 tokens on 64 chunks of 512 x 2048 would take 8.6 GB in one call."""
+    p = ops.Pages(slots=torch.zeros(1, 1, 1).half().expand(64, 512, 2048), page_of=torch.zeros(4, 64, dtype=torch.int32),
+                  n_valid=torch.ones(4, 64, dtype=torch.int32), S=torch.zeros(4, 64, 1))
+    assert ops.shared_workspace(p, 4 * 2048, 64) > 8 << 30
+    for rows, rpl in ((4 * 2048, 2048), (8 * 4096, 4096), (64, 1)):
+        parts = ops.shared_slices(rows, rpl, lambda n: ops.shared_workspace(p, n, 64), ops.SHARED_WORKSPACE)
+        assert max(ops.shared_workspace(p, b - a, 64) for a, b in parts) <= ops.SHARED_WORKSPACE
+        assert len(parts) <= 1 + 2 * ops.shared_workspace(p, rows, 64) // ops.SHARED_WORKSPACE
