@@ -41,7 +41,8 @@
 //
 // Slots at or past n_valid never reach a result: their scores are masked, P is 0 there, and the rows of V behind the
 // tile's last valid slot are zeroed in shared memory (0 * NaN would not be 0). Pairs of one page with different n_valid
-// share a tile: slots between theirs are multiplied by 0 for the shorter ones, so those have to be finite.
+// share a tile: slots between theirs are multiplied by 0 for the shorter ones. The plan therefore looks those rows of V
+// over, and a page where one is not finite gives each of its pairs a tile of its own.
 #pragma once
 
 #include <math_constants.h>
@@ -74,7 +75,7 @@ static_assert(RS_STAGES % 2 == 0, "a stage of V goes to the same four warps each
 static_assert(4 * RS_VROWS * 128 <= RS_STAGE, "a stage of the read fits");
 
 struct __align__(16) SharedTile {
-  int page, start, count, nv;  // pairs [start, start + count) in grouped order; nv: the page's most valid slots
+  int page, start, count, nv;  // pairs [start, start + count) in grouped order; nv: their most valid slots
 };
 
 struct SharedArgs {
@@ -102,6 +103,10 @@ struct SharedArgs {
   int softmax;
   float* part;     // [n_pairs][segs][d_s], normalised per segment
   float2* ml;      // [n_pairs][segs]: (max, sum)
+  // plan: pages whose readers disagree on n_valid
+  int* nvgap;         // [n_pages]: page_rows less the page's fewest valid slots; -1 - its first tile: one pair a tile
+  const uint16_t* v;  // the value pool's bits
+  uint32_t v_exp;     // the exponent bits of its type
 };
 
 // ----------------------------------------------------------------------------------------------------- plan
@@ -129,9 +134,43 @@ __device__ __forceinline__ void rs_count(const SharedArgs& a, int64_t first, int
       } else {
         a.rank[i] = atomicAdd(&a.cnt[page], 1);
         atomicMax(&a.nvmax[page], nv);
+        if (nv < a.page_rows) atomicMax(&a.nvgap[page], a.page_rows - nv);
       }
     }
     a.page[i] = page;
+  }
+}
+
+// Pages whose readers disagree on n_valid: are the rows of V that only some of them read finite? One CTA of 1024 threads
+// reads them, 64 KB in flight; as a rule they are the few rows that one fork has appended.
+__device__ __forceinline__ void rs_check_rows(const SharedArgs& a) {
+  __shared__ int next;
+  for (int p = 0;;) {
+    __syncthreads();
+    if (threadIdx.x == 0) next = a.n_pages;
+    __syncthreads();
+    for (int i = p + (int)threadIdx.x; i < a.n_pages; i += 1024)
+      if (a.nvmax[i] > a.page_rows - a.nvgap[i]) {
+        atomicMin(&next, i);
+        break;
+      }
+    __syncthreads();
+    p = next;
+    if (p >= a.n_pages) return;
+    const int64_t first = ((int64_t)p * a.page_rows + a.page_rows - a.nvgap[p]) * a.d_s;
+    const int64_t last = ((int64_t)p * a.page_rows + a.nvmax[p]) * a.d_s;
+    const uint32_t e0 = a.v_exp, e1 = a.v_exp << 16;
+    bool bad = false;
+#pragma unroll 4
+    for (int64_t i = first + threadIdx.x * 8; i < last; i += 1024 * 8) {
+      const uint4 u = *reinterpret_cast<const uint4*>(a.v + i);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int x = 0; x < 4; ++x) bad |= (w[x] & e0) == e0 || (w[x] & e1) == e1;
+    }
+    bad = __syncthreads_or(bad);
+    if (threadIdx.x == 0 && bad) a.nvgap[p] = -1;
+    ++p;
   }
 }
 
@@ -142,10 +181,18 @@ __device__ __forceinline__ void rs_scan(const SharedArgs& a, int mt) {
   const int per = (a.n_pages + 1023) / 1024;
   const int p0 = min(a.n_pages, (int)threadIdx.x * per), p1 = min(a.n_pages, p0 + per);
   int pos = 0, tiles = 0;
+  bool differ = false;
   for (int p = p0; p < p1; ++p) {
     const int c = a.cnt[p];
     pos += c;
     tiles += (c + mt - 1) / mt;
+    differ |= a.nvmax[p] > a.page_rows - a.nvgap[p];
+  }
+  differ = __syncthreads_or(differ);
+  if (differ) {
+    rs_check_rows(a);
+    tiles = 0;
+    for (int p = p0; p < p1; ++p) tiles += a.nvgap[p] < 0 ? a.cnt[p] : (a.cnt[p] + mt - 1) / mt;
   }
   int ip = pos, it = tiles;
 #pragma unroll
@@ -168,8 +215,22 @@ __device__ __forceinline__ void rs_scan(const SharedArgs& a, int mt) {
   for (int p = p0; p < p1; ++p) {
     const int c = a.cnt[p];
     a.cnt[p] = at;
-    for (int s = 0; s < c; s += mt) a.tiles[tile++] = SharedTile{p, at + s, min(mt, c - s), a.nvmax[p]};
+    int step = mt;
+    if (differ && a.nvgap[p] < 0) {
+      step = 1;
+      a.nvgap[p] = -1 - tile;
+    }
+    for (int s = 0; s < c; s += step) a.tiles[tile++] = SharedTile{p, at + s, min(step, c - s), a.nvmax[p]};
     at += c;
+  }
+  if (differ) {  // a pair that has its tile for itself: its own valid slots
+    __syncthreads();
+    for (int64_t i = threadIdx.x; i < a.n_pairs; i += 1024) {
+      const int page = a.page[i];
+      if (page < 0 || a.nvgap[page] >= 0) continue;
+      const int64_t lib = i / a.k / a.rows_per_lib;
+      a.tiles[-1 - a.nvgap[page] + a.rank[i]].nv = min(a.n_valid[lib * a.C + a.idx[i]], a.page_rows);
+    }
   }
 }
 
@@ -188,6 +249,7 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const SharedArgs a, i
   for (int p = threadIdx.x; p < a.n_pages; p += 1024) {
     a.cnt[p] = 0;
     a.nvmax[p] = 0;
+    a.nvgap[p] = 0;
   }
   __syncthreads();
   rs_count(a, threadIdx.x, 1024);

@@ -621,15 +621,15 @@ def read_shared(q: torch.Tensor, pages: Pages, idx: torch.Tensor, wk: torch.Tens
 
     q [R, d_s] float32 / float16 / bfloat16; idx, wk [R, k] as route gives them. out_dtype float32: 22 bits of q and of
     the softmax weights (16 with bfloat16 slots); float16 / bfloat16: the result rounded once (and, with float16 slots, q
-    and the weights). Slots that no row reads may hold anything; where Libraries name one page with different n_valid, the
-    values that any of them reads must be finite (a weight of 0 multiplies them for the others). The workspace holds up to
-    8 d_s bytes per routed pair and 512 slots of its page; rows whose pairs would take more than max_workspace bytes of it
-    are read in slices, with the same bits. Raises
-    NotImplementedError for float32 slots and d_s above 4096 or not a multiple of 8 (use read_decode)."""
+    and the weights). Slots that a row does not read may hold anything. The workspace holds up to 8 d_s bytes per routed
+    pair and 512 slots of its page; rows whose pairs would take more than max_workspace bytes of it are read in slices,
+    with the same bits. Raises NotImplementedError for float32 slots and d_s above 4096 or not a multiple of 8 (use
+    read_decode)."""
     # the kernels index both tables as dense [n_lib, C] int32
-    for name, t in (("page_of", pages.page_of), ("n_valid", pages.n_valid)):
-        if t.dtype != torch.int32 or t.dim() != 2 or t.shape != pages.page_of.shape or not t.is_contiguous():
-            raise ValueError(f"read_shared: {name} must be a contiguous int32 [n_lib, C] tensor")
+    po, nv = pages.page_of, pages.n_valid
+    if po.dtype is not torch.int32 or nv.dtype is not torch.int32 or po.dim() != 2 or nv.shape != po.shape \
+            or not po.is_contiguous() or not nv.is_contiguous():
+        raise ValueError("read_shared: page_of and n_valid must be contiguous int32 [n_lib, C] tensors")
     dev = _cuda("read_shared", q, pages.slots, pages.page_of, pages.n_valid, idx, wk)
     q = q.contiguous()
     wk = _f32(wk, "wk")
@@ -661,14 +661,14 @@ def read_shared(q: torch.Tensor, pages: Pages, idx: torch.Tensor, wk: torch.Tens
             parts = shared_slices(R, rpl, size, max_workspace)
             ws_bytes = max(size(n) for n in {r1 - r0 for r0, r1 in parts})
         ws = _workspace(ws_bytes, dev)
-        at = lambda t, row: t.data_ptr() + row * t.stride(0) * t.element_size()
+        q_at, r_at, po_at, nv_at, idx_at, wk_at = (t.data_ptr() for t in (q, r, po, nv, idx, wk))
+        q_row, r_row = d_s * q.element_size(), d_s * r.element_size()
         for r0, r1 in parts:
             lib, rows = r0 // rpl, r1 - r0
-            libs = -(-rows // rpl)
-            N.call("xencb_read_shared", at(q, r0), _hdt(q, "q"), rows, d_s, _ptr(slots), _ptr(_vpool(pages)), dt, P,
-                   page_rows * d_s, page_rows, at(pages.page_of, lib), at(pages.n_valid, lib), C, rpl, libs, at(idx, r0),
-                   at(wk, r0), k, float(read_temp), int(bool(read_softmax)), at(r, r0), odt, _ptr(ws), ws.numel(),
-                   _stream(dev))
+            N.call("xencb_read_shared", q_at + r0 * q_row, _hdt(q, "q"), rows, d_s, _ptr(slots), _ptr(_vpool(pages)), dt, P,
+                   page_rows * d_s, page_rows, po_at + lib * C * 4, nv_at + lib * C * 4, C, rpl, -(-rows // rpl),
+                   idx_at + r0 * k * 4, wk_at + r0 * k * 4, k, float(read_temp), int(bool(read_softmax)),
+                   r_at + r0 * r_row, odt, _ptr(ws), ws_bytes, _stream(dev))
     return r
 
 

@@ -361,3 +361,32 @@ def test_slices_give_the_same_bits(dev, case, out):
     with pytest.raises(ValueError):
         ops.read_shared(q, pages, idx, wk, rows_per_lib=rows - 1, out_dtype=out, max_workspace=need // 5)
     assert ops.device_status(dev) == 0
+
+
+@pytest.mark.parametrize("d_s,page_rows", [(256, 100), (2048, 300), (2560, 90), (256, 700)])
+@pytest.mark.parametrize("slots", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("softmax", [True, False])
+def test_a_slot_that_is_not_finite_reaches_only_its_readers(dev, d_s, page_rows, slots, softmax):
+    """Libraries that name one page with different n_valid: NaN in the slots that only some of them read."""
+    from kv_skill_v2_b200 import ops
+    n_lib, rows = 5, 8
+    pages, q, idx, wk = make(dev, 15, n_lib=n_lib, rows=rows, shared=3, k=0, page_rows=page_rows, d_s=d_s, slots=slots,
+                             full=True)
+    few = page_rows * 2 // 3
+    pages.n_valid[:3] = few
+    pages.n_valid[4] = few - 20
+    pages.slots[pages.page_of[0, 1].long(), few:] = float("nan")
+    r = ops.read_shared(q, pages, idx, wk, rows_per_lib=rows, read_softmax=softmax)
+    keep = torch.arange(n_lib * rows, device=dev) // rows != 3
+    assert torch.isnan(r[~keep]).all()
+    want, mag_s, mag_p = reference(pages, q, idx, wk, rows, softmax)
+    e, u = 2.0 ** -23, 2 * HALF[slots] ** 2
+    bound = (u + e * (d_s / 16 + 4)) * mag_s + (u + e * 40) * mag_p + 2.0 ** -24 * want.abs() + 1e-30
+    assert ((r.double() - want).abs() <= bound)[keep].all()
+    # the same bits as from a call that nobody else is part of
+    one = ops.Pages(slots=pages.slots, page_of=pages.page_of[4:5].contiguous(),
+                    n_valid=pages.n_valid[4:5].contiguous(), S=pages.S[4:5])
+    at = slice(4 * rows, 5 * rows)
+    alone = ops.read_shared(q[at].contiguous(), one, idx[at].contiguous(), wk[at].contiguous(), rows_per_lib=rows,
+                            read_softmax=softmax)
+    assert torch.equal(r[at], alone)
