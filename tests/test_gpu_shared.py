@@ -390,3 +390,21 @@ def test_a_slot_that_is_not_finite_reaches_only_its_readers(dev, d_s, page_rows,
     alone = ops.read_shared(q[at].contiguous(), one, idx[at].contiguous(), wk[at].contiguous(), rows_per_lib=rows,
                             read_softmax=softmax)
     assert torch.equal(r[at], alone)
+
+
+def test_a_slot_that_is_not_finite_among_many_pairs(dev):
+    """The same where the plan takes several launches (more than 4096 pairs) and pages have several tiles; the page of
+    another chunk only has another length."""
+    from kv_skill_v2_b200 import ops
+    n_lib, rows = 5, 300
+    pages, q, idx, wk = make(dev, 17, n_lib=n_lib, rows=rows, shared=6, k=3, page_rows=80, d_s=64, full=True)
+    pages.n_valid[:2, 1] = 50
+    pages.n_valid[2, 4] = 60
+    pages.slots[pages.page_of[0, 1].long(), 70, 5] = float("inf")
+    r = ops.read_shared(q, pages, idx, wk, rows_per_lib=rows)
+    reads = ((idx == 1) & (torch.arange(n_lib * rows, device=dev) // rows >= 2)[:, None]).any(1)
+    want, mag_s, mag_p = reference(pages, q, idx, wk, rows)
+    bound = (2.0 ** -21 + 2.0 ** -23 * 8) * mag_s + (2.0 ** -21 + 2.0 ** -23 * 13) * mag_p + 2.0 ** -24 * want.abs() + 1e-30
+    assert ((r.double() - want).abs() <= bound)[~reads].all() and torch.isfinite(r[~reads]).all()
+    assert not torch.isfinite(r[reads]).all(-1).any()
+    assert ops.device_status(dev) == 0
