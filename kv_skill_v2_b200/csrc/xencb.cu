@@ -1670,12 +1670,9 @@ int xencb_read_shared(const void* q, int q_dtype, int64_t n_rows, int d_s, const
   a.softmax = read_softmax ? 1 : 0;
   a.qscale = read_softmax ? read_temp * 1.4426950408889634f : 1.f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto run = [&](auto t) {
-    using T = decltype(t);
-    auto go = [&](auto kern) { return kern(q, q_dtype, p, a, slots, vslots, q16, n_rows, r_out, out_dtype, di.sms, st); };
-    return p.terms == 2 ? go(run_shared<T, 2>) : go(run_shared<T, 1>);
-  };
-  return slots_dtype == XENCB_F16 ? run(__half{}) : run(__nv_bfloat16{});
+  auto go = [&](auto run) { return run(q, q_dtype, p, a, slots, vslots, q16, n_rows, r_out, out_dtype, di.sms, st); };
+  if (slots_dtype == XENCB_BF16) return go(run_shared<__nv_bfloat16, 2>);  // (plan_shared: bf16 slots always take two terms)
+  return p.terms == 2 ? go(run_shared<__half, 2>) : go(run_shared<__half, 1>);
 }
 
 // ------------------------------------------------------------------------------------------------ project_out
