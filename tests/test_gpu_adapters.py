@@ -196,3 +196,60 @@ def test_tiles_of_one_16_bit_type(dev, dtype, R, rpa, n, rank, d_in, d_out):
     low = torch.einsum("tr,tnr->tn", low, s["b"].double()[of.clamp(min=0)]) * s["scale"].double()[of.clamp(min=0)][:, None]
     want = s["h"].double() @ s["w"].double().t() + low * (of >= 0)[:, None]
     assert float((q.double() - want).abs().max()) <= TOL * float(want.abs().max())
+
+
+# Plans that would run all of d_in in one split, and are given one per 1280 columns: many output tiles, long rows.
+FORCED = [(2048, 512, 4, 32, 2600, 2048), (1999, 512, 4, 7, 5120, 2048), (1100, 1, 5, 16, 2568, 4096)]
+
+
+@pytest.mark.parametrize("R,rpa,n,rank,d_in,d_out", FORCED)
+@pytest.mark.parametrize("prepared", [True, False])
+@pytest.mark.parametrize("h_dtype", [torch.bfloat16, torch.float32])
+def test_long_rows_with_many_output_tiles(dev, R, rpa, n, rank, d_in, d_out, prepared, h_dtype):
+    """Both projections, called through the C entries with exactly the workspace that the query gives and a guard behind
+    it. 2-norm: the accumulator loses up to 2^-23 of itself at each product it adds, always towards zero, half of that on
+    average. 1280 columns are 80 steps of three products (3xF16; 160 steps as 3xTF32), over which the running sum grows
+    like a square root, 2/3 of its end on average: 240 x 2^-24 x 2/3 = 1e-5 (2e-5). The loss is in proportion to the
+    columns of a split, so rows without an adapter are at most 0.6 as far off as in the plain projection's one split of
+    them all (a third or a quarter, and the operands' own 1e-7)."""
+    from kv_skill_v2_b200 import _native as N
+    from kv_skill_v2_b200 import ops
+    s = _inputs(dev, R + d_in, R, rpa, n, rank, d_in, d_out, h_dtype, torch.bfloat16)
+    s["of"][0] = -1
+    prep = ops.weights_prep(s["w"]) if prepared else None
+    want = _ref(s["h"], s, rpa)
+    y = torch.empty(R, d_out, device=dev)
+    ptr, st = ops._ptr, ops._stream(dev)
+    adapt = (ptr(s["a"]), ptr(s["b"]), N.BF16, ptr(s["scale"]), n, rank, ptr(s["of"]), rpa)
+    guard = 32 << 20
+
+    def workspace(size):
+        assert size > 0
+        ws = torch.full((size + guard,), 0x5A, dtype=torch.uint8, device=dev)
+        return ws, size
+
+    def judge(ws, size):
+        torch.cuda.synchronize()
+        assert (ws[size:] == 0x5A).all()
+        assert float((y.double() - want).norm() / want.norm()) <= (1e-5 if prepared else 2e-5)
+        _close(y, want, torch.float32)
+
+    ws, size = workspace(N.lib().xencb_project_in_adapted_workspace(R, d_in, d_out, rank))
+    N.call("xencb_project_in_adapted", ptr(s["h"]), ops._hdt(s["h"], "h"), R, d_in, ptr(s["w"]), ptr(prep), None, d_out, 0,
+           None, 0.0, None, None, None, 0, 1e-6, ptr(y), None, None, None, *adapt, ptr(ws), size, st)
+    judge(ws, size)
+    if prepared:
+        plain = ops.project_in(s["h"], s["w"], w_prep=prep, rms=False, l2=False)[0].double()
+        bare = s["h"].double() @ s["w"].double().t()
+        none = torch.full_like(s["of"], -1)
+        split = ops.project_in(s["h"], s["w"], w_prep=prep, rms=False, l2=False, adapter_of=none, rows_per_adapter=rpa,
+                               adapters=ops.Adapters(s["a"], s["b"], s["scale"]))[0].double()
+        assert float((split - bare).norm()) <= 0.6 * float((plain - bare).norm())
+    if h_dtype == torch.float32:
+        y.fill_(7.0)
+        zero = torch.zeros(R, d_out, device=dev)
+        ws, size = workspace(N.lib().xencb_project_out_adapted_workspace(R, d_in, d_out, rank))
+        N.call("xencb_project_out_adapted", ptr(s["h"]), R, d_in, ptr(s["w"]), ptr(prep), None, d_out, 1.0, None, None,
+               None, 0.0, None, None, ptr(zero), N.F32, ptr(y), None, None, *adapt, ptr(ws), size, st)
+        judge(ws, size)
+    assert ops.device_status(dev) == 0
