@@ -6,12 +6,17 @@
 // and the gate, as the GEMM's partials do, and is float32 throughout.
 //
 // Two forms of each. Rows: one CTA per row (decode: every row has its own adapter, and the adapters' bytes bound it).
-// Tiles: 64 rows of one adapter at a time, A and B read once a tile (prompts; the multiplications bound it). A tile
-// costs the same however few rows it holds, so it is taken from 16 rows per adapter on.
+// Tiles: 64 rows of one adapter at a time, A and B read once a tile (prompts; the multiplications bound it), from
+// AD_MIN_TILE rows per adapter on. Both forms, us a call of project_in (4096 -> 2048, 512 rows; rows / tiles):
+//   rows per adapter             4          8          16         64
+//   bf16 rows, rank 16         86 / 133   86 / 100   86 / 84    86 / 88
+//   bf16 rows, rank 64        258 / 205  254 / 145  252 / 111  250 / 109
+//   float32 rows, rank 16      88 / 211   88 / 153   88 / 115   88 / 143
+//   float32 rows, rank 64     260 / 358  256 / 238  254 / 168  256 / 166
 //
 // Measured beside the projection (d_in 4096 -> 2048): 64 rows with 64 adapters of rank 16, shrink 10.6 us and expand
 // 5.3 us of a call of 31 us (the GEMM 11.6 us); 2048 rows of 4 adapters of rank 32 (5120 -> 2048), shrink 19 us
-// (78 us with float32 multiplications) and expand 27 us of 267 us; by rows the same took 159 and 249 us.
+// (78 us with float32 multiplications) and expand 27 us of 264 us; by rows the same took 159 and 249 us.
 #pragma once
 
 #include "gemm_f16x3.cuh"

@@ -23,13 +23,17 @@ __device__ unsigned int g_dev_status = 0;
 __device__ __forceinline__ void flag_error(unsigned int bits) { atomicOr(&g_dev_status, bits); }
 
 // Programmatic dependent launch (the kernels the host launches with programmatic stream serialisation: the read
-// merge, the row split, the 3xF16 GEMM, the projection row kernels and the fused decode router). pdl_wait()
+// merge, the row split, the 3xF16 GEMM, the projection row kernels, the fused decode router, the adapters' shrink and
+// expand, the shared read's split, read and combine, and the page copies). pdl_wait()
 // returns once the grid before this one in the stream has completed and its writes are visible (a no-op for a
 // plain launch). Before it such a kernel only reads, and only data that no kernel still running can be writing:
-// the GEMM's weight tiles and the router's summary keys (Library data), and the row kernels' hidden-state rows
-// (they start after the GEMM has passed its own wait, so the kernel that wrote h has completed). Nothing is written
-// before the wait. pdl_trigger() lets the next grid be scheduled; the row split and the row kernels issue it first
-// thing (their successors' early work is such a read), the others after their wait.
+// the GEMM's weight tiles and the router's summary keys (Library data), the row kernels' hidden-state rows
+// (they start after the GEMM has passed its own wait, so the kernel that wrote h has completed; with an expand in
+// between, that starts after the GEMM's wait and they after it), and the shared read's q (its plan is a plain launch,
+// so whatever wrote q has completed). Nothing is written before the wait. pdl_trigger() lets the next grid be scheduled.
+// The GEMM issues it after its wait, which the row kernels' early reads rest on, and the shared read at its end; the row
+// split, the row kernels, the adapters' kernels, the shared read's plan and split and the page plans issue it first thing
+// (their successors' early work is such a read, or none).
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

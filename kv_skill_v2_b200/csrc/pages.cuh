@@ -232,7 +232,7 @@ struct PagePools {
 // the unit of the accesses: 16 bytes where every pool's pages are 16-byte aligned, else 2 bytes (every slot type has
 // at least two). A work item is a slice of one page of one pool, PG_UNROLL units a thread with every load in flight
 // before the first store; the pages are read and written once, so both bypass L1. HBM bounds it: 64 pages of 2 MiB in
-// four pools (0.94 GB read and written) 171 us with the plan, 5.5 TB/s, 0.84 of a plain copy's rate. 16 KiB slices on
+// four pools (0.94 GB read and written) 171 to 181 us with the plan, 5.2 to 5.5 TB/s, 0.79 to 0.84 of a plain copy's rate. 16 KiB slices on
 // up to 64 CTAs per SM, most of which take a few slices: 8 units a thread on 8 CTAs per SM took 206 us.
 constexpr int PG_COPY_THREADS = 256;
 constexpr int PG_UNROLL = 4;

@@ -14,20 +14,28 @@
 //           pair: a warp's lanes are consecutive columns, so the stores are whole lines.
 // The scores and the read walk the page differently (all columns of some slots, all slots of some columns), so the page
 // passes through shared memory twice, but its second pass comes from L2: a cluster holds one or two pages at a time.
-// The roles run one unit apart: the scores of the next unit are computed while this one's softmax and exchange run,
-// and the epilogue stores one unit while the next one's P is made.
-// A unit of few pairs (16 / TERMS) takes its read product on the softmax warps instead, with mma.sync:
-// one 16-row tile holds all of its pairs, hi and lo together, and the tensor core's MN-major operand is read at about
-// 27 bytes a cycle (162 cycles per 16 slots x 128 columns), which ldmatrix is not.
+// The roles run one unit apart: the scores of the next unit are computed while this one's softmax and exchange run (with
+// TERMS = 2 a quarter of them: the RS_ACC accumulators are drained by the softmax warps), and the epilogue stores one
+// unit while the next one's P is made.
+// A unit of few pairs (16 / TERMS) takes its read product on the softmax warps instead, with mma.sync: one 16-row tile
+// holds all of its pairs, hi and lo together.
 // shared_combine adds a row's pairs in the order of its routing: results do not depend on how pairs were grouped.
 //
-// Measured (f16 slots, d_s 2048, pages of 512): 64 rows of top-4 routing on 64 pages 68 us a call, the read 54 us (2.5 TB/s
-// of pages; two pages a cluster one after the other bound it); 32 forks with 48 common and 16 own pages each, dense, 424
-// and 364 us (3.2 TB/s; V's shared-memory reads); 4096 rows of top-4 routing to bf16 280 and 213 us (0.32 PFLOP/s; the
-// same), 20 us the split and 40 us the combine. Through read_decode's plan every pair reads its page again.
+// Measured (f16 slots, d_s 2048, pages of 512): 64 rows of top-4 routing on 64 pages 69 us a call, the read 54 us (2.5 TB/s
+// of pages); 32 forks with 48 common and 16 own pages each, dense, 424 and 364 us (3.2 TB/s); 4096 rows of top-4 routing
+// to bf16 281 and 205-213 us (0.32 PFLOP/s), 20 us the split and 40 us the combine. Beside read_decode, which reads a page
+// again for every pair: 79 against 114 us at 4 readers a page (64 rows), 81 against 364 at 16, 477 against 5560 at 256
+// (float32 results), but 71 against 44 at 1.6 and 127 against 73 where no page is shared: it pays from about 3 readers.
 //
-// Why this orientation: with the pairs as the 128 rows (of which a tile fills 64) the read cost 290 cycles per
-// 16 slots x 256 columns (M = 128, N = 256, MN-major B), this way 2 x 81 (M = 128, N = 64).
+// What bounds it, by cycle counts of the roles: a unit takes 37k cycles in both regimes. Few pairs: the scores of the next
+// unit (18-20k, of them 2-5k waits for accumulators and 3-5k for stages) and the read of few pairs (18k) follow one
+// another, as the same warps serve both. Many pairs: the next scores (15-17k, half of it waits for stages) and the read
+// (21k, 1k of waits) follow one another on the MMA thread. The read's 128 products leave it at 158 cycles each, as its
+// loops have no constant length; the product itself (M 128, N 64, K 16, V MN-major) takes 73 to 84 cycles alone, the
+// scores' (both operands K-major) 48. With loops of constant length the read took 13.7k cycles.
+//
+// Why the page is the 128-row operand: with the pairs as the 128 rows (of which a tile fills 64) the read cost 290 cycles
+// per 16 slots x 256 columns (M = 128, N = 256, MN-major B), this way two products.
 //
 // Precision. The operands are 16-bit. TERMS = 2 (float32 outputs, bf16 slots): q and P enter as hi + lo pairs, two of the MMA's
 // N columns per pair, which keeps 22 bits with f16 slots and 16 with bf16; the halves are added in float32.
@@ -745,7 +753,8 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
       // The read of a unit of few pairs: O^T[64 columns, N] of this warp = V^T . P^T with N = 8 or 16: four pairs' hi rows
       // and their lo rows (TERMS = 2) or 8 pairs to a tile of 8. Warp w takes the w-th 64 columns of the slab; the four
       // warps of a stage hand it back together. mma.sync bounds it (a tile of 16 x 8 x 16 takes 32 cycles of a
-      // scheduler): the columns as its 16 rows need half the products that the pairs as its rows did.
+      // scheduler; 18k cycles a unit of 512 slots): the columns as its 16 rows need half the products that the pairs as its
+      // rows did.
       auto read_few = [&](const RsUnit& w, uint32_t un, uint32_t nth, RsRing rg) {
         done(*s.abort_flag || mbar_wait_cluster(&s.p_full[1], nth & 1));
         const int hgroups = (my_boxes + 3) / 4, hg = warp >> 2;

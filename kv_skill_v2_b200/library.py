@@ -330,7 +330,8 @@ class PagedLibrary:
         """These Libraries and, behind them, one fork of each of `parents`. A fork shares its parent's pages for the
         chunks below own_from (an int, or one per fork; default: all of them) and has pages of its own, holding copies,
         for the rest, so that they can be rewritten for one request alone. RuntimeError when the pools have too few free
-        pages (reserve). Reads one integer back from the device."""
+        pages (reserve). Reads one integer back from the device. Fork from the newest: a page that no row of this
+        PagedLibrary names counts as free, also where another fork of it, or one made from a select(), has taken it."""
         from .ops import pages_fork
 
         pools, page_of, n_valid, nco = self._tables()
