@@ -49,8 +49,11 @@
 //
 // Slots at or past n_valid never reach a result: their scores are masked, P is 0 there, and the rows of V behind the
 // tile's last valid slot are zeroed in shared memory (0 * NaN would not be 0). Pairs of one page with different n_valid
-// share a tile: slots between theirs are multiplied by 0 for the shorter ones. The plan therefore looks those rows of V
-// over, and a page where one is not finite gives each of its pairs a tile of its own.
+// share a tile: slots between theirs are multiplied by 0 for the shorter ones. Such a page is therefore planned twice, in
+// tiles as any other and, behind all of these, with a tile for each of its pairs; the split looks over the rows of V that
+// only some of its readers read, and the read takes the pairs one by one if a value there is not finite. Where all of 64
+// pages of 512 slots differ in 4 (256) rows, 64 rows of top-4 routing take 108 (154) us in place of 81, 4096 rows 488 (495)
+// in place of 481; with an infinity on each of them 214 (243) and 9500 (8400).
 #pragma once
 
 #include <math_constants.h>
@@ -85,6 +88,9 @@ static_assert(4 * RS_VROWS * 128 <= RS_STAGE, "a stage of the read fits");
 struct __align__(16) SharedTile {
   int page, start, count, nv;  // pairs [start, start + count) in grouped order; nv: their most valid slots
 };
+// flags beside `start` (there are fewer than 2^30 pairs) of a page whose readers disagree on n_valid: a tile of all of
+// them, and one of a single pair
+constexpr int RS_MIXED = 1 << 30, RS_SINGLE = -2147483647 - 1;
 
 struct SharedArgs {
   // plan inputs
@@ -111,8 +117,11 @@ struct SharedArgs {
   int softmax;
   float* part;     // [n_pairs][segs][d_s], normalised per segment
   float2* ml;      // [n_pairs][segs]: (max, sum)
-  // plan: pages whose readers disagree on n_valid
-  int* nvgap;         // [n_pages]: page_rows less the page's fewest valid slots; -1 - its first tile: one pair a tile
+  // pages whose readers disagree on n_valid ("mixed")
+  int* nvgap;         // [n_pages]: page_rows less the page's fewest valid slots; after the split -1: not all finite
+  int* n_mixed;       // their number; the number of their single tiles, which lie behind all others; 1: these are read
+  int* mixed;         // [n_pages]: the mixed pages
+  int* single;        // [n_pages]: the first of a mixed page's single tiles, -1: not mixed
   const uint16_t* v;  // the value pool's bits
   uint32_t v_exp;     // the exponent bits of its type
 };
@@ -149,39 +158,6 @@ __device__ __forceinline__ void rs_count(const SharedArgs& a, int64_t first, int
   }
 }
 
-// Pages whose readers disagree on n_valid: are the rows of V that only some of them read finite? One CTA of 1024 threads
-// reads them, 64 KB in flight; as a rule they are the few rows that one fork has appended.
-__device__ __forceinline__ void rs_check_rows(const SharedArgs& a) {
-  __shared__ int next;
-  for (int p = 0;;) {
-    __syncthreads();
-    if (threadIdx.x == 0) next = a.n_pages;
-    __syncthreads();
-    for (int i = p + (int)threadIdx.x; i < a.n_pages; i += 1024)
-      if (a.nvmax[i] > a.page_rows - a.nvgap[i]) {
-        atomicMin(&next, i);
-        break;
-      }
-    __syncthreads();
-    p = next;
-    if (p >= a.n_pages) return;
-    const int64_t first = ((int64_t)p * a.page_rows + a.page_rows - a.nvgap[p]) * a.d_s;
-    const int64_t last = ((int64_t)p * a.page_rows + a.nvmax[p]) * a.d_s;
-    const uint32_t e0 = a.v_exp, e1 = a.v_exp << 16;
-    bool bad = false;
-#pragma unroll 4
-    for (int64_t i = first + threadIdx.x * 8; i < last; i += 1024 * 8) {
-      const uint4 u = *reinterpret_cast<const uint4*>(a.v + i);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int x = 0; x < 4; ++x) bad |= (w[x] & e0) == e0 || (w[x] & e1) == e1;
-    }
-    bad = __syncthreads_or(bad);
-    if (threadIdx.x == 0 && bad) a.nvgap[p] = -1;
-    ++p;
-  }
-}
-
 // One CTA of 1024 threads: positions of the pages' first pairs (into cnt) and the tiles of mt pairs.
 __device__ __forceinline__ void rs_scan(const SharedArgs& a, int mt) {
   __shared__ int sh_pos[32], sh_tile[32];
@@ -189,18 +165,10 @@ __device__ __forceinline__ void rs_scan(const SharedArgs& a, int mt) {
   const int per = (a.n_pages + 1023) / 1024;
   const int p0 = min(a.n_pages, (int)threadIdx.x * per), p1 = min(a.n_pages, p0 + per);
   int pos = 0, tiles = 0;
-  bool differ = false;
   for (int p = p0; p < p1; ++p) {
     const int c = a.cnt[p];
     pos += c;
     tiles += (c + mt - 1) / mt;
-    differ |= a.nvmax[p] > a.page_rows - a.nvgap[p];
-  }
-  differ = __syncthreads_or(differ);
-  if (differ) {
-    rs_check_rows(a);
-    tiles = 0;
-    for (int p = p0; p < p1; ++p) tiles += a.nvgap[p] < 0 ? a.cnt[p] : (a.cnt[p] + mt - 1) / mt;
   }
   int ip = pos, it = tiles;
 #pragma unroll
@@ -218,27 +186,19 @@ __device__ __forceinline__ void rs_scan(const SharedArgs& a, int mt) {
     if (lane >= o) { wp += yp; wt += yt; }
   }
   if (threadIdx.x == 1023) *a.n_tiles = wt;
+  const int all = __shfl_sync(0xffffffffu, wt, 31);
   int at = ip - pos + __shfl_sync(0xffffffffu, wp - wp0, wid);
   int tile = it - tiles + __shfl_sync(0xffffffffu, wt - wt0, wid);
   for (int p = p0; p < p1; ++p) {
     const int c = a.cnt[p];
     a.cnt[p] = at;
-    int step = mt;
-    if (differ && a.nvgap[p] < 0) {
-      step = 1;
-      a.nvgap[p] = -1 - tile;
-    }
-    for (int s = 0; s < c; s += step) a.tiles[tile++] = SharedTile{p, at + s, min(step, c - s), a.nvmax[p]};
+    const int nv = a.nvmax[p];
+    const bool mixed = nv > a.page_rows - a.nvgap[p];
+    for (int s = 0; s < c; s += mt)
+      a.tiles[tile++] = SharedTile{p, (at + s) | (mixed ? RS_MIXED : 0), min(mt, c - s), nv};
+    if (mixed) a.mixed[atomicAdd(a.n_mixed, 1)] = p;
+    a.single[p] = mixed ? all + atomicAdd(a.n_mixed + 1, c) : -1;  // (the split writes these tiles)
     at += c;
-  }
-  if (differ) {  // a pair that has its tile for itself: its own valid slots
-    __syncthreads();
-    for (int64_t i = threadIdx.x; i < a.n_pairs; i += 1024) {
-      const int page = a.page[i];
-      if (page < 0 || a.nvgap[page] >= 0) continue;
-      const int64_t lib = i / a.k / a.rows_per_lib;
-      a.tiles[-1 - a.nvgap[page] + a.rank[i]].nv = min(a.n_valid[lib * a.C + a.idx[i]], a.page_rows);
-    }
   }
 }
 
@@ -254,6 +214,7 @@ __global__ void __launch_bounds__(1024) shared_scan_kernel(const SharedArgs a, i
 // Few pairs: the whole plan in one CTA.
 __global__ void __launch_bounds__(1024) shared_plan_kernel(const SharedArgs a, int mt) {
   pdl_trigger();
+  if (threadIdx.x < 3) a.n_mixed[threadIdx.x] = 0;
   for (int p = threadIdx.x; p < a.n_pages; p += 1024) {
     a.cnt[p] = 0;
     a.nvmax[p] = 0;
@@ -265,12 +226,37 @@ __global__ void __launch_bounds__(1024) shared_plan_kernel(const SharedArgs a, i
   rs_scan(a, mt);
 }
 
+// Are the rows of V that only some readers of a mixed page read finite? The grid takes 16 rows at a time.
+__device__ __forceinline__ void rs_check_mixed(const SharedArgs& a, int n, int threads) {
+  const int per = (a.page_rows + 15) / 16;
+  const int64_t step = (int64_t)gridDim.x * gridDim.y;
+  for (int64_t w = (int64_t)blockIdx.y * gridDim.x + blockIdx.x; w < (int64_t)n * per; w += step) {
+    const int page = a.mixed[w / per], gap = *reinterpret_cast<volatile int*>(&a.nvgap[page]);
+    if (gap < 0) continue;  // (found already)
+    const int lo = a.page_rows - gap + (int)(w % per) * 16, hi = min(lo + 16, a.nvmax[page]);
+    const uint16_t* v = a.v + ((int64_t)page * a.page_rows + lo) * a.d_s;
+    const uint32_t e0 = a.v_exp, e1 = a.v_exp << 16;
+    bool bad = false;
+#pragma unroll 4
+    for (int i = (int)threadIdx.x * 8; i < (hi - lo) * a.d_s; i += threads * 8) {
+      const uint4 u = *reinterpret_cast<const uint4*>(v + i);
+      const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bad |= (x[e] & e0) == e0 || (x[e] & e1) == e1;
+    }
+    if (bad) {
+      a.nvgap[page] = -1;
+      a.n_mixed[2] = 1;
+    }
+  }
+}
+
 // Each pair's q row in 16 bits at the pair's grouped position: hi terms [n_pairs, d_s], then (TERMS = 2) lo terms. One
 // CTA per row and up to 8 of its routed chunks; the row stays in registers (d_s <= 4096: two pieces of 8 a thread).
 constexpr int RS_SPLIT_THREADS = 256;
 template <typename TQ, typename T, int TERMS>
-__global__ void __launch_bounds__(RS_SPLIT_THREADS) shared_split_kernel(const TQ* __restrict__ q, const SharedArgs a,
-                                                                        T* __restrict__ out) {
+__global__ void __launch_bounds__(RS_SPLIT_THREADS, TERMS == 1 ? 8 : std::is_same<T, __half>::value ? 5 : 6)
+    shared_split_kernel(const TQ* __restrict__ q, const SharedArgs a, T* __restrict__ out) {
   __shared__ float red[8];
   pdl_trigger();
   const int64_t row = blockIdx.x;
@@ -306,6 +292,7 @@ __global__ void __launch_bounds__(RS_SPLIT_THREADS) shared_split_kernel(const TQ
       if (TERMS == 2) lo[p][e] = from_f32<T>(v[p][e] * s - to_f32(hi[p][e]));
     }
   pdl_wait();  // the plan
+  const int n_mixed = *a.n_mixed;
   const int64_t lib = row / a.rows_per_lib;
   const int j1 = min(a.k, (int)(blockIdx.y + 1) * 8);
   for (int j = blockIdx.y * 8; j < j1; ++j) {
@@ -323,10 +310,14 @@ __global__ void __launch_bounds__(RS_SPLIT_THREADS) shared_split_kernel(const TQ
             *reinterpret_cast<const uint4*>(lo[p]);
     }
     if (threadIdx.x == 0) {
-      a.pnv[pos] = min(a.n_valid[lib * a.C + a.idx[pair]], a.page_rows);
+      const int nv = min(a.n_valid[lib * a.C + a.idx[pair]], a.page_rows);
+      a.pnv[pos] = nv;
       a.qinv[pos] = 1.f / s;
+      const int single = n_mixed ? a.single[page] : -1;
+      if (single >= 0) a.tiles[single + a.rank[pair]] = SharedTile{page, pos | RS_SINGLE, 1, nv};
     }
   }
+  if (n_mixed) rs_check_mixed(a, n_mixed, RS_SPLIT_THREADS);
 }
 
 // ----------------------------------------------------------------------------------------------------- cluster PTX
@@ -458,6 +449,10 @@ struct RsUnit {
   __device__ __forceinline__ void find(const SharedArgs& a, int first, int n_units, int step) {
     for (u = first; u < n_units; u += step) {
       t = a.tiles[u / a.segs];
+      if (t.start & (RS_MIXED | RS_SINGLE)) {  // one form or the other
+        if ((a.nvgap[t.page] < 0) != ((t.start & RS_SINGLE) != 0)) continue;
+        t.start &= ~(RS_MIXED | RS_SINGLE);
+      }
       seg0 = (u % a.segs) * RS_SEG;
       nv = min(t.nv - seg0, RS_SEG);
       if (nv > 0) return;
@@ -542,7 +537,7 @@ __global__ void __launch_bounds__(RS_THREADS, 1)
   tc_fence_after();
   const uint32_t taddr = *s.tmem;
   pdl_wait();
-  const int n_units = *a.n_tiles * a.segs;
+  const int n_units = (*a.n_tiles + (a.n_mixed[2] ? a.n_mixed[1] : 0)) * a.segs;
   RsUnit cur, nxt;
   cur.find(a, cluster, n_units, n_clusters);
   // few pairs: the read runs on the softmax warps (which are all there with 128 slots a CTA)

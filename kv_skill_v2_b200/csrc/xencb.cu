@@ -754,10 +754,11 @@ int plan_shared(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows, 
   p->ns = RS_SEG / p->cs;
   p->slab = (int)align_up((size_t)(d_s + p->cs - 1) / p->cs, 64);
   p->segs = (page_rows + RS_SEG - 1) / RS_SEG;
-  if (p->n_pairs * p->segs > INT32_MAX)
+  // full tiles, a tail a page, and a tile for each pair of pages whose readers disagree on n_valid
+  p->max_tiles = p->n_pairs + p->n_pairs / p->mt + std::min<int64_t>(n_pages, p->n_pairs) + 1;
+  if (p->max_tiles * p->segs > INT32_MAX)
     return fail(XENCB_ENOTSUP, "read_shared: page_rows=%d is too long for this many rows", page_rows);
-  p->max_tiles = p->n_pairs;  // (a page may give every pair a tile of its own)
-  p->cnt = align_up((size_t)n_pages * 12, 256);
+  p->cnt = align_up((size_t)n_pages * 20 + 12, 256);
   p->pair = align_up((size_t)p->n_pairs * 4, 256);
   p->tiles = align_up((size_t)p->max_tiles * sizeof(SharedTile), 256);
   p->q = align_up((size_t)p->terms * p->n_pairs * d_s * 2, 256);
@@ -821,12 +822,12 @@ int run_shared(const void* q, int q_dtype, const SharedPlan& p, SharedArgs a, co
   if (!rc) rc = shared_clusters(kern, p.cs, &n_clusters);
   if (rc) return rc;
   n_clusters = (int)std::min<int64_t>(
-      n_clusters, (p.n_pairs / p.mt + std::min<int64_t>(a.n_pages, p.n_pairs) + 1) * p.segs);  // (full tiles, and a tail a page)
+      n_clusters, (p.max_tiles - p.n_pairs) * p.segs);  // (the single tiles are for pages that few calls have)
   if (p.n_pairs <= 4096) {
     shared_plan_kernel<<<1, 1024, 0, st>>>(a, p.mt);
     XENCB_CHECK_LAUNCH("shared_plan launch");
   } else {
-    const cudaError_t e = cudaMemsetAsync(a.cnt, 0, (size_t)a.n_pages * 12, st);
+    const cudaError_t e = cudaMemsetAsync(a.cnt, 0, (size_t)a.n_pages * 12 + 12, st);
     if (e != cudaSuccess) return cuda_fail(e, "read_shared: memset");
     shared_count_kernel<<<(unsigned)std::min<int64_t>((p.n_pairs + 255) / 256, 4 * sms), 256, 0, st>>>(a);
     XENCB_CHECK_LAUNCH("shared_count launch");
@@ -1655,6 +1656,9 @@ int xencb_read_shared(const void* q, int q_dtype, int64_t n_rows, int d_s, const
   a.cnt = reinterpret_cast<int*>(take(p.cnt));
   a.nvmax = a.cnt + n_pages;
   a.nvgap = a.nvmax + n_pages;
+  a.n_mixed = a.nvgap + n_pages;
+  a.mixed = a.n_mixed + 3;
+  a.single = a.mixed + n_pages;
   a.v = static_cast<const uint16_t*>(vslots ? vslots : slots);
   a.v_exp = slots_dtype == XENCB_F16 ? 0x7c00u : 0x7f80u;
   a.page = reinterpret_cast<int*>(take(p.pair));
