@@ -317,9 +317,10 @@ class XEncInjector(ExternalSkillInjector):
         return r, gcal
 
     def _check_forward_only(self, h: torch.Tensor) -> None:
-        if _needs_grad(h, self.itf if isinstance(self.itf, nn.Module) else None):
+        adapters = [t for ad in (self._adapters or ())[:2] if ad is not None for t in (ad.a, ad.b, ad.scale)]
+        if _needs_grad(h, self.itf if isinstance(self.itf, nn.Module) else None, *adapters):
             raise RuntimeError("the xencb Library read is forward-only (no autograd); run the reader under "
-                               "torch.no_grad() / torch.inference_mode(), or freeze the interface")
+                               "torch.no_grad() / torch.inference_mode(), or freeze the interface (and its adapters)")
 
     def _run(self, h: torch.Tensor, li: int, inject: bool):
         """Single-skill branch. inject=False -> delta (float32); inject=True -> (h + delta, rel)."""

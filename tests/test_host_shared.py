@@ -202,3 +202,24 @@ def test_a_dense_prompt_over_shared_pages_is_sliced():
         parts = ops.shared_slices(rows, rpl, lambda n: ops.shared_workspace(p, n, 64), ops.SHARED_WORKSPACE)
         assert max(ops.shared_workspace(p, b - a, 64) for a, b in parts) <= ops.SHARED_WORKSPACE
         assert len(parts) <= 1 + 2 * ops.shared_workspace(p, rows, 64) // ops.SHARED_WORKSPACE
+
+
+@pytest.mark.parametrize("which", ["a", "b", "scale"])
+@pytest.mark.parametrize("side", [0, 1])
+def test_adapters_that_need_gradients_are_refused(which, side):
+    """As an interface that needs them is: the kernels would leave the adapters out of the graph."""
+    from kv_skill_v2_b200 import LibraryInjector, PagedLibrary
+    from kv_skill_v2_b200.interface import LinearInterface
+
+    itf = LinearInterface(torch.zeros(32, 16), torch.zeros(16, 32), [0]).requires_grad_(False)
+    inj = LibraryInjector(TinyReader(32, 2), itf)
+    inj.load_library(PagedLibrary({0: _pages(16)}))
+    d_in, d_out = ((32, 16), (16, 32))[side]
+    ad = ops.Adapters(a=torch.zeros(1, 2, d_in), b=torch.zeros(1, d_out, 2), scale=torch.ones(1))
+    getattr(ad, which).requires_grad_()
+    inj.set_adapters(*((ad, None), (None, ad))[side], torch.zeros(1, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="forward-only"):
+        inj._inject(torch.zeros(1, 1, 32), 0)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
+        inj._inject(torch.zeros(1, 1, 32), 0)
+    inj.detach()
