@@ -23,7 +23,7 @@
 //
 // Measured (f16 slots, d_s 2048, pages of 512): 64 rows of top-4 routing on 64 pages 69 us a call, the read 54 us (2.5 TB/s
 // of pages); 32 forks with 48 common and 16 own pages each, dense, 424 and 364 us (3.2 TB/s); 4096 rows of top-4 routing
-// to bf16 281 and 205-213 us (0.32 PFLOP/s), 20 us the split and 40 us the combine. Beside read_decode, which reads a page
+// to bf16 283 and 205-213 us (0.32 PFLOP/s), 22 us the split and 40 us the combine. Beside read_decode, which reads a page
 // again for every pair: 79 against 114 us at 4 readers a page (64 rows), 81 against 364 at 16, 477 against 5560 at 256
 // (float32 results), but 71 against 44 at 1.6 and 127 against 73 where no page is shared: it pays from about 3 readers.
 //
