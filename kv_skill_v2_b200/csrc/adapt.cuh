@@ -15,8 +15,8 @@
 //   float32 rows, rank 64     260 / 358  256 / 238  254 / 168  256 / 166
 //
 // Measured beside the projection (d_in 4096 -> 2048): 64 rows with 64 adapters of rank 16, shrink 10.6 us and expand
-// 5.3 us of a call of 31 us (the GEMM 11.6 us); 2048 rows of 4 adapters of rank 32 (5120 -> 2048), shrink 19 us
-// (78 us with float32 multiplications) and expand 27 us of 264 us; by rows the same took 159 and 249 us.
+// 5.3 us of a call of 32.5 us (the GEMM 12.4 us); 2048 rows of 4 adapters of rank 32 (5120 -> 2048), shrink 19 us
+// (78 us with float32 multiplications) and expand 27 us of 266 us; by rows the same took 159 and 249 us.
 #pragma once
 
 #include "gemm_f16x3.cuh"

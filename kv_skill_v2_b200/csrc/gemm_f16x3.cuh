@@ -18,7 +18,12 @@
 // run of the prepared weight, so a CTA's k-blocks are one sequential stream) and the boxes X_hi, X_lo [64 x 64],
 // all 128-byte-swizzled, into a 4- or 2-stage ring (weights with L2 evict-last); warp 1 lane 0 issues 4 k-steps
 // x 3 tcgen05.mma kind::f16 (f32 accumulate in TMEM) per k-block and commits each stage back to the producer;
-// warps 2-5 read the accumulator (tcgen05.ld), undo the scales and store the split partial. Weight rows past N
+// warps 2-5 read the accumulator (tcgen05.ld), undo the scales and store the split partial. The accumulator drops bits
+// below its running value at every product it adds, towards zero: three times a k-step. APART (the projections with
+// adapters) gives the two small products an accumulator of their own, which the epilogue adds, so that only hi*hi is
+// left to lose: 1.9e-6 -> 6.5e-7 of the result over 512 columns a split, 4.6e-6 -> 1.6e-6 over 1280 (64 rows, 4096 ->
+// 2048: the kernel 11.7 -> 12.4 us; 2048 rows, 5120 -> 2048: 149.6 -> 150.2, as W_hi times X_hi and X_lo is one product
+// of N = 128). Weight rows past N
 // and columns past K are zeros in the prepared tiles; X boxes that run past M read rows of the other half of
 // the stacked pair or zeros, which only reach outputs m >= M (not stored). Every barrier wait is bounded; TMEM
 // is freed on every path.
@@ -173,13 +178,14 @@ __global__ void __launch_bounds__(SR_THREADS) split_rows_f16x2_kernel(const T* _
   }
 }
 
-template <int STAGES, int MINB>
+template <int STAGES, int MINB, bool APART = false>
 __global__ void __launch_bounds__(H3_THREADS, MINB) gemm_f16x3_kernel(const __grid_constant__ CUtensorMap map_w,
                                                                    const __grid_constant__ CUtensorMap map_x,
                                                                    int64_t M, int N, int K, int kps,
                                                                    const float* __restrict__ w_inv_scale,
                                                                    const float* __restrict__ x_inv_scale,
                                                                    float* __restrict__ part, int* __restrict__ row_done) {
+  constexpr uint32_t TMEM_COLS = (APART ? 2 : 1) * H3_TMEM_COLS;
   extern __shared__ unsigned char h3_smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(h3_smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * H3_STAGE);
@@ -202,7 +208,7 @@ __global__ void __launch_bounds__(H3_THREADS, MINB) gemm_f16x3_kernel(const __gr
     prefetch_tensormap(&map_x);
   }
   if (warp == 1) {
-    tc_alloc(tmem_slot, H3_TMEM_COLS);
+    tc_alloc(tmem_slot, TMEM_COLS);
     tc_relinquish();
   }
   if (threadIdx.x == 0) {
@@ -265,6 +271,7 @@ __global__ void __launch_bounds__(H3_THREADS, MINB) gemm_f16x3_kernel(const __gr
     // ------------------------------------------------------------------------------------------- MMA issuer
     if (lane == 0) {
       constexpr uint32_t idesc = umma_idesc(UMMA_F16, UMMA_F16, H3_BM, H3_BN);
+      constexpr uint32_t idesc2 = umma_idesc(UMMA_F16, UMMA_F16, H3_BM, 2 * H3_BN);
       for (int kb = 0; kb < nkb; ++kb) {
         const int s = kb % STAGES;
         if (!mbar_wait_spin(&full[s], (kb / STAGES) & 1) || *abort_flag) { *abort_flag = 1; break; }
@@ -274,9 +281,14 @@ __global__ void __launch_bounds__(H3_THREADS, MINB) gemm_f16x3_kernel(const __gr
 #pragma unroll
         for (int ks = 0; ks < H3_BK / 16; ++ks) {  // 16 f16 per UMMA k-step: 32 bytes along the swizzle row
           const uint32_t off = ks * 32;
-          tc_mma<0>(taddr, umma_desc_k_sw128(wh + off), umma_desc_k_sw128(xh + off), idesc, kb > 0 || ks > 0);
-          tc_mma<0>(taddr, umma_desc_k_sw128(wh + off), umma_desc_k_sw128(xl + off), idesc, true);
-          tc_mma<0>(taddr, umma_desc_k_sw128(wl + off), umma_desc_k_sw128(xh + off), idesc, true);
+          if constexpr (APART) {  // X_lo's box lies behind X_hi's: one product for both, 64 columns each
+            tc_mma<0>(taddr, umma_desc_k_sw128(wh + off), umma_desc_k_sw128(xh + off), idesc2, kb > 0 || ks > 0);
+            tc_mma<0>(taddr + H3_BN, umma_desc_k_sw128(wl + off), umma_desc_k_sw128(xh + off), idesc, true);
+          } else {
+            tc_mma<0>(taddr, umma_desc_k_sw128(wh + off), umma_desc_k_sw128(xh + off), idesc, kb > 0 || ks > 0);
+            tc_mma<0>(taddr, umma_desc_k_sw128(wh + off), umma_desc_k_sw128(xl + off), idesc, true);
+            tc_mma<0>(taddr, umma_desc_k_sw128(wl + off), umma_desc_k_sw128(xh + off), idesc, true);
+          }
         }
         tc_commit(&sfree[s]);  // the stage is free once these MMAs have read it
       }
@@ -297,7 +309,15 @@ __global__ void __launch_bounds__(H3_THREADS, MINB) gemm_f16x3_kernel(const __gr
     tc_fence_after();
     for (int c = 0; c < rows; c += 32) {
       float v[32];
-      tc_ld32(taddr + ((uint32_t)(q * 32) << 16) + (uint32_t)c, v);
+      const uint32_t at = taddr + ((uint32_t)(q * 32) << 16) + (uint32_t)c;
+      if constexpr (APART) {
+        float u[32];
+        tc_ld32_two(at, at + H3_BN, v, u);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] += u[i];
+      } else {
+        tc_ld32(at, v);
+      }
       const float xs = c == 0 ? xs0 : xs1;
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
@@ -308,7 +328,7 @@ __global__ void __launch_bounds__(H3_THREADS, MINB) gemm_f16x3_kernel(const __gr
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tc_dealloc(taddr, H3_TMEM_COLS);
+  if (warp == 1) tc_dealloc(taddr, TMEM_COLS);
 }
 
 }  // namespace xencb

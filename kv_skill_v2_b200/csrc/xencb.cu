@@ -268,7 +268,8 @@ int tensor_map_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, co
 // `xbuf` (M*K float32, may be null when TX is float) stages a 16-bit X as float32 for the TMA path.
 template <typename TX>
 int launch_gemm(const void* X, int64_t M, int K, const float* W, int N, int sms, float* part, float* xbuf,
-                int* row_done, cudaStream_t st, GemmPlan* used, const void* w_prep = nullptr, int min_splits = 1) {
+                int* row_done, cudaStream_t st, GemmPlan* used, const void* w_prep = nullptr, int min_splits = 1,
+                bool apart = false) {
   // 3xF16 (weights split once by xencb_weights_prep, X split here with a power-of-two scale per row) whenever the
   // prepared weights are given: half the MMAs of 3xTF32, and no per-k-block split of W
   const bool f16x3 = w_prep != nullptr;
@@ -290,7 +291,8 @@ int launch_gemm(const void* X, int64_t M, int K, const float* W, int N, int sms,
     rc = tensor_map_2d(&mx, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, xs, (uint64_t)K, 2 * (uint64_t)M, (uint64_t)K * 2,
                        H3_BK, H3_BN);
     if (rc) return rc;
-    auto kern = two ? gemm_f16x3_kernel<2, 2> : gemm_f16x3_kernel<4, 1>;
+    auto kern = apart ? (two ? gemm_f16x3_kernel<2, 2, true> : gemm_f16x3_kernel<4, 1, true>)
+                      : (two ? gemm_f16x3_kernel<2, 2> : gemm_f16x3_kernel<4, 1>);
     const size_t h3s = h3_smem(two ? 2 : 4);
     rc = ensure_smem(kern, (int)h3s);
     if (rc) return rc;
@@ -337,9 +339,10 @@ int launch_gemm(const void* X, int64_t M, int K, const float* W, int N, int sms,
 // ------------------------------------------------------------------------------------------------ adapters
 // Extra workspace of a projection with adapters: one more split partial (behind the GEMM's) and t [n_rows, rank].
 size_t adapt_slice_bytes(int64_t M, int N) { return align_up((size_t)M * N * sizeof(float), 256); }
-// A projection with adapters splits d_in at least every AD_KPS columns: the tensor core's accumulator loses about
-// 2^-24 of its value at every 16-column step, towards zero, and 2048 rows x 5120 columns in one run were 6.6e-6 off
-// (1.4e-6 in splits of 1280); the row kernels add the splits in float32.
+// A projection with adapters splits d_in at least every AD_KPS columns, and keeps the 3xF16 GEMM's small products apart:
+// the tensor core's accumulator loses about 2^-24 of its value at every product, towards zero, and 2048 rows x 5120
+// columns in one run were 6.6e-6 off after the L2 norm (1.7e-6 in splits of 1280, 0.8e-6 with the small products apart);
+// the row kernels add the splits in float32.
 int adapt_min_splits(int K) { return (K + AD_KPS - 1) / AD_KPS; }
 // Bytes a call's partials take beyond gemm_part_bytes: the low-rank slice, and the splits above where there are more.
 size_t adapt_part_extra(int64_t M, int N, int K, int sms) {
@@ -971,14 +974,15 @@ static int project_in_impl(const void* h, int h_dtype, int64_t n_rows, int d_m, 
   switch (h_dtype) {
     case XENCB_F32:
       rc = launch_gemm<float>(h, n_rows, d_m, w_in, d_s, di.sms, part, w_prep ? xbuf : nullptr, row_done, st, &gp,
-                              w_prep, min_splits);
+                              w_prep, min_splits, adapters != nullptr);
       break;
     case XENCB_F16:
-      rc = launch_gemm<__half>(h, n_rows, d_m, w_in, d_s, di.sms, part, xbuf, row_done, st, &gp, w_prep, min_splits);
+      rc = launch_gemm<__half>(h, n_rows, d_m, w_in, d_s, di.sms, part, xbuf, row_done, st, &gp, w_prep, min_splits,
+                               adapters != nullptr);
       break;
     default:
       rc = launch_gemm<__nv_bfloat16>(h, n_rows, d_m, w_in, d_s, di.sms, part, xbuf, row_done, st, &gp, w_prep,
-                                      min_splits);
+                                      min_splits, adapters != nullptr);
       break;
   }
   if (rc) return rc;
@@ -1733,7 +1737,7 @@ static int project_out_impl(const float* r, int64_t n_rows, int d_s, const float
     if (rc) return rc;
   }
   rc = launch_gemm<float>(r, n_rows, d_s, w_out, d_m, di.sms, part, w_prep ? xbuf : nullptr, nullptr, st, &gp, w_prep,
-                          adapters ? adapt_min_splits(d_s) : 1);
+                          adapters ? adapt_min_splits(d_s) : 1, adapters != nullptr);
   if (rc) return rc;
   if (adapters) {  // the low-rank term is one more split partial
     rc = launch_adapt_expand(part + (size_t)gp.splits * n_rows * d_m, ad, adapt_dtype, st);

@@ -253,3 +253,21 @@ def test_long_rows_with_many_output_tiles(dev, R, rpa, n, rank, d_in, d_out, pre
                None, 0.0, None, None, ptr(zero), N.F32, ptr(y), None, None, *adapt, ptr(ws), size, st)
         judge(ws, size)
     assert ops.device_status(dev) == 0
+
+
+@pytest.mark.parametrize("R,d_in,d_out", [(2048, 5120, 2048), (1999, 2600, 2048), (64, 2048, 4096), (5, 3440, 1544),
+                                          (1, 4096, 2048), (130, 1280, 4096)])
+def test_only_the_large_products_lose_to_the_accumulator(dev, R, d_in, d_out):
+    """2-norm of float32 results with prepared weights. hi*hi alone is summed in the accumulator that holds the result, 80
+    steps at most in a split of 1280 columns, each of which loses half of 2^-23 of a running sum on average, 2/3 of its end
+    (it grows like a square root): 80 x 2^-24 x 2/3 = 3.2e-6. The operands' 22 bits and the float32 additions stay below
+    2e-7 beside it."""
+    from kv_skill_v2_b200 import ops
+    s = _inputs(dev, R + d_in, R, 1, 3, 4, d_in, d_out, torch.float32, torch.bfloat16)
+    x = s["h"] / s["h"].norm(dim=-1, keepdim=True)
+    want = _ref(x, s, 1)
+    more = dict(w_prep=ops.weights_prep(s["w"]), adapters=ops.Adapters(s["a"], s["b"], s["scale"]), adapter_of=s["of"])
+    steps = min(80, -(-d_in // 16))
+    for got in (ops.project_out(x, s["w"], torch.zeros(R, d_out, device=dev), **more)[0],
+                ops.project_in(x, s["w"], rms=False, l2=False, **more)[0]):
+        assert float((got.double() - want).norm() / want.norm()) <= steps * 2.0 ** -24 * 2 / 3 + 2e-7
