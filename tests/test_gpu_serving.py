@@ -254,3 +254,93 @@ def test_a_prompt_over_shared_pages_keeps_no_workspace(dev, monkeypatch, top_k):
         inj._inject(h[:, :20].contiguous(), LAYER)
         assert len(inj._graphs) == 1  # (a smaller step is captured as before)
     inj.detach()
+
+
+def _merged(itf, ad_in, ad_out, a):
+    """A copy of the interface whose maps hold adapter a (negative: none)."""
+    import copy
+    m = copy.deepcopy(itf)
+    if a >= 0:
+        with torch.no_grad():
+            m.A.weight += ad_in.scale[a] * ad_in.b[a] @ ad_in.a[a]
+            m.B.weight += ad_out.scale[a] * ad_out.b[a] @ ad_out.a[a]
+    return m
+
+
+def _model_interface(dev, g, layers):
+    from kv_skill_v2_b200 import ModelInterface
+    itf = ModelInterface(D_M, D_S, layers)
+    with torch.no_grad():
+        itf.A.weight.copy_(torch.randn(D_S, D_M, generator=g, device=dev) * D_M ** -0.5)
+        itf.B.weight.copy_(torch.randn(D_M, D_S, generator=g, device=dev) * 0.2)
+        itf.gate_w.copy_(torch.randn(D_M, generator=g, device=dev) * 0.1)
+        itf.gate_b.copy_(torch.randn(len(layers), generator=g, device=dev))
+        itf.log_gain.copy_(torch.randn(len(layers), generator=g, device=dev) * 0.3)
+    ads = [ops_adapters(dev, g, d_in, d_out) for d_in, d_out in ((D_M, D_S), (D_S, D_M))]
+    return itf.to(dev).requires_grad_(False), ads
+
+
+def ops_adapters(dev, g, d_in, d_out):
+    from kv_skill_v2_b200 import ops
+    return ops.Adapters(a=torch.randn(3, 4, d_in, generator=g, device=dev) * d_in ** -0.5,
+                        b=torch.randn(3, d_out, 4, generator=g, device=dev) * 0.2,
+                        scale=torch.rand(3, generator=g, device=dev) + 0.5)
+
+
+@pytest.mark.parametrize("selector", [False, True])
+@pytest.mark.parametrize("T", [1, 90])
+def test_a_hooked_reader_with_adapters_is_one_of_merged_weights(dev, T, selector):
+    """ModelInterface (gate, gain) at two depths, with and without a LayerSelector, over forks that share pages: each
+    request's tokens come out as from a reader whose interface holds its adapter in the weights."""
+    from kv_skill_v2_b200 import LayerSelector, LibraryInjector, ops
+    g = torch.Generator(device=dev).manual_seed(21)
+    layers = [LAYER, 3]
+    itf, (ad_in, ad_out) = _model_interface(dev, g, layers)
+    lib = _library(dev, seed=22).reserve(4).fork([0, 2, 0], own_from=[4, 3, 9]).select([3, 4, 5, 1])
+    sel = None
+    if selector:
+        sel = LayerSelector(D_M, layers, k=1, alpha_init=0.05).to(dev).requires_grad_(False)
+        sel.u.weight.copy_(torch.randn(sel.u.weight.shape, generator=g, device=dev))
+    of = torch.tensor([1, -1, 2, 1], dtype=torch.int32, device=dev)
+    reader = TinyReader(D_M, 5).to(dev).eval().requires_grad_(False)
+    x = torch.randn(4, T, D_M, generator=g, device=dev)
+    inj = LibraryInjector(reader, itf, top_k=2, selector=sel, share_pages=True)
+    inj.load_library(lib)
+    inj.set_adapters(ad_in, ad_out, of)
+    with torch.no_grad():
+        for _ in range(2):
+            got = reader(x)
+        inj.detach()
+        bare = reader(x)
+        for b in range(4):
+            one = LibraryInjector(reader, _merged(itf, ad_in, ad_out, int(of[b])), top_k=2, selector=sel)
+            one.load_library(lib.select([b]))
+            want = reader(x[b:b + 1])
+            one.detach()
+            assert rel_err(got[b:b + 1] - bare[b:b + 1], want - bare[b:b + 1]) <= 2 * TOL  # (both are within TOL)
+    assert ops.device_status(dev) == 0
+
+
+def test_a_single_skill_with_adapters_is_one_of_merged_weights(dev):
+    from kv_skill_v2_b200 import KVSkill, XEncInjector
+    g = torch.Generator(device=dev).manual_seed(23)
+    itf, (ad_in, ad_out) = _model_interface(dev, g, [LAYER])
+    K = torch.nn.functional.normalize(torch.randn(50, D_S, generator=g, device=dev), dim=-1).half().float()
+    reader = TinyReader(D_M, 4).to(dev)
+    h = torch.randn(3, 7, D_M, generator=g, device=dev)
+    of = torch.tensor([2, -1, 0], dtype=torch.int32, device=dev)
+
+    def branch(interface, rows, **adapters):
+        inj = XEncInjector(reader, interface)
+        inj.load(KVSkill({LAYER: K}, {LAYER: K}, D_S))
+        if adapters:
+            inj.set_adapters(**adapters)
+        with torch.no_grad():
+            out = inj._branch(rows, LAYER)
+        inj.detach()
+        return out
+
+    got = branch(itf, h, adapters_in=ad_in, adapters_out=ad_out, adapter_of=of)
+    for b in range(3):
+        want = branch(_merged(itf, ad_in, ad_out, int(of[b])), h[b:b + 1])
+        assert rel_err(got[b:b + 1], want) <= 2 * TOL
