@@ -273,7 +273,8 @@ XENCB_API int xencb_read_prefill(const float* q, int64_t n_rows, int d_s, const 
  *           wk == 0 are skipped, a row without any gives 0. idx >= n_chunks or a page outside the pool is skipped and
  *           flagged (XENCB_DEV_BADPAGE).
  * A page's Libraries may disagree on its n_valid; slots at or past a row's own n_valid may hold anything (a value there
- * that is not finite, which another row reads, costs that page its sharing). Chunks with n_valid 0 contribute 0.
+ * that is not finite, which another row reads, costs that page its sharing). Chunks with n_valid 0 contribute 0. A row
+ * whose own valid keys hold an infinity is NaN, also where the score's limit has a weight.
  * f16 / bf16 slots, d_s a multiple of 8 up to 4096, a dense pool (page_stride == page_rows * d_s), any page_rows; else
  * XENCB_ENOTSUP. The result does not depend on how the pairs are grouped. Workspace:
  * xencb_read_shared_workspace bytes, 256-byte aligned. */
