@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define XENCB_ABI_VERSION 7
+#define XENCB_ABI_VERSION 8
 
 #if defined(__GNUC__)
 #define XENCB_API __attribute__((visibility("default")))
@@ -378,6 +378,31 @@ XENCB_API int xencb_project_out_adapted(const float* r, int64_t n_rows, int d_s,
                                         const float* adapt_scale, int n_adapters, int rank,
                                         const int32_t* adapter_of, int64_t rows_per_adapter, void* workspace,
                                         size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * The projections in 8-bit floating point. No counterpart in the reference.
+ * A matrix [n, k] in 8 bits: x8 [n, 128 * ceil(k / 128)] e4m3 bytes (zeros behind column k) and scale [n, ceil(k / 128)]
+ * bytes e + 127: x8 = round_to_nearest_even(x * 2^-e) with e the smallest integer for which the largest finite value of
+ * the row's block of 128 columns is at most 448 * 2^e (0 for a block of zeros). Values that are not finite become NaN.
+ * xencb_quant8 writes it from x (float32 / float16 / bfloat16); x8 16-byte aligned. A weight is laid out once.
+ * xencb_project_in8 / xencb_project_out8 are xencb_project_in / xencb_project_out with the product
+ *   y[r, n] = sum over blocks b of 2^(e_x[r, b] + e_w[n, b]) * sum_{k in b} x8[r, k] w8[n, k]
+ * in place of x @ W^T, accumulated in float32; the rows (h as it is given, r) are quantised in the call. Everything else,
+ * 1/rms and the gate among it, comes from the rows in full. Any d_m (d_s) on the input side; outputs as there. A row
+ * that holds a value that is not finite comes out as NaN. */
+XENCB_API int xencb_quant8(const void* x, int dtype, int64_t n, int k, void* x8, void* scale, void* stream);
+XENCB_API size_t xencb_project_in8_workspace(int64_t n_rows, int d_m, int d_s);
+XENCB_API int xencb_project_in8(const void* h, int h_dtype, int64_t n_rows, int d_m, const void* w8,
+                                const void* w_scale, const float* b_in, int d_s, int flags, const float* gate_w,
+                                float gate_b, const float* gate_b_dev, const float* sel_w, const float* sel_b,
+                                int n_cand, float rms_eps, float* q_out, float* gate_out, float* rstd_out,
+                                float* z_out, void* workspace, size_t workspace_bytes, void* stream);
+XENCB_API size_t xencb_project_out8_workspace(int64_t n_rows, int d_s, int d_m);
+XENCB_API int xencb_project_out8(const float* r, int64_t n_rows, int d_s, const void* w8, const void* w_scale,
+                                 const float* b_out, int d_m, float scale, const float* log_scale_dev,
+                                 const float* gate, const float* sel_w, float log_alpha, const float* log_alpha_dev,
+                                 const float* pos_mask, const void* h, int h_dtype, void* delta_out, void* h_out,
+                                 float* rel_out, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------------------
  * Page operators of pools that several Libraries share (no counterpart in the reference, whose Library owns its

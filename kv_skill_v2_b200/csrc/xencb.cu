@@ -18,6 +18,7 @@
 #include "project.cuh"
 #include "gemm_tc.cuh"
 #include "gemm_f16x3.cuh"
+#include "gemm_f8.cuh"
 #include "read_decode.cuh"
 #include "read_decode_mma.cuh"
 #include "read_multi.cuh"
@@ -333,6 +334,88 @@ int launch_gemm(const void* X, int64_t M, int K, const float* W, int N, int sms,
                                                            row_done);
   XENCB_CHECK_LAUNCH("gemm_simt launch");
   *used = p;
+  return XENCB_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ 8-bit GEMM
+// A weight in 8 bits: [N, 128 ceil(K / 128)] e4m3 and [N, ceil(K / 128)] exponents + 127.
+struct Weight8 {
+  const void* w;
+  const uint8_t* scale;
+};
+
+struct F8Plan {
+  int bn, nb, bps, sx_stride;
+  GemmPlan gp;
+  size_t x8_bytes, sx_bytes, total;
+};
+
+// BN = 64 and 128 where all rows fit one tile (the split CTAs stream the weights); more rows take 256 at a time, so that a
+// weight tile is fetched a quarter as often.
+F8Plan plan_f8(int64_t M, int N, int K, int sms) {
+  F8Plan p;
+  p.bn = M <= 64 ? 64 : M <= 128 ? 128 : 256;
+  p.nb = (K + F8_BK - 1) / F8_BK;
+  const int64_t tiles = ((int64_t)(N + F8_BM - 1) / F8_BM) * ((M + p.bn - 1) / p.bn);
+  const int64_t s = std::min<int64_t>(std::max<int64_t>(1, sms / tiles), p.nb);
+  // (blocks b0 .. b0 + bps - 1 lie in at most (bps + 6) / 4 words of scale factors)
+  p.bps = std::min((int)((p.nb + s - 1) / s), 4 * f8_max_words(p.bn) - 6);
+  p.gp.tc = true;
+  p.gp.kps = p.bps * F8_BK;
+  p.gp.splits = (p.nb + p.bps - 1) / p.bps;
+  p.gp.part_bytes = align_up((size_t)p.gp.splits * (size_t)M * (size_t)N * sizeof(float), 256);
+  p.sx_stride = (p.nb + 3) / 4 * 4;
+  p.x8_bytes = align_up((size_t)M * p.nb * F8_BK, 256);
+  p.sx_bytes = align_up((size_t)M * p.sx_stride, 256);
+  p.total = p.gp.part_bytes + p.x8_bytes + p.sx_bytes;
+  return p;
+}
+
+template <typename T>
+int launch_quant_f8(const void* x, int64_t M, int K, void* x8, uint8_t* scale, int stride, int sms, cudaStream_t st) {
+  const int64_t n = M * ((K + F8_BK - 1) / F8_BK);
+  const int vec = K % 4 == 0 && aligned(x, 4 * sizeof(T));
+  const unsigned grid = (unsigned)std::min<int64_t>((n + F8Q_WARPS - 1) / F8Q_WARPS, 16 * (int64_t)sms);
+  launch_pdl(quant_f8_kernel<T>, dim3(grid), dim3(32 * F8Q_WARPS), 0, st, static_cast<const T*>(x), M, K, vec,
+             static_cast<uint8_t*>(x8), scale, stride);
+  XENCB_CHECK_LAUNCH("quant_f8 launch");
+  return XENCB_OK;
+}
+
+template <int BN>
+int run_gemm_f8(const CUtensorMap& mw, const CUtensorMap& mx, const F8Args& a, int splits, cudaStream_t st) {
+  auto kern = gemm_f8_kernel<BN>;
+  int rc = ensure_smem(kern, (int)f8_smem(BN));
+  if (rc) return rc;
+  const dim3 grid((a.N + F8_BM - 1) / F8_BM, (unsigned)((a.M + BN - 1) / BN), splits);
+  launch_pdl(kern, grid, dim3(F8_THREADS), f8_smem(BN), st, mw, mx, a);
+  XENCB_CHECK_LAUNCH("gemm_f8 launch");
+  return XENCB_OK;
+}
+
+// part = split partials of X @ W^T with both in 8 bits. ws: p.total bytes (the partials first).
+template <typename TX>
+int launch_gemm_f8(const void* X, int64_t M, int K, const Weight8& w, int N, int sms, const F8Plan& p, char* ws,
+                   int* row_done, cudaStream_t st) {
+  uint8_t* x8 = reinterpret_cast<uint8_t*>(ws + p.gp.part_bytes);
+  uint8_t* sx = x8 + p.x8_bytes;
+  int rc = launch_quant_f8<TX>(X, M, K, x8, sx, p.sx_stride, sms, st);
+  if (rc) return rc;
+  const uint64_t kp = (uint64_t)p.nb * F8_BK;
+  CUtensorMap mw, mx;
+  rc = tensor_map_2d(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w.w, kp, (uint64_t)N, kp, F8_BK, F8_BM);
+  if (!rc) rc = tensor_map_2d(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x8, kp, (uint64_t)M, kp, F8_BK, (uint32_t)p.bn);
+  if (rc) return rc;
+  const F8Args a{M, N, p.nb, p.bps, w.scale, sx, p.sx_stride, reinterpret_cast<float*>(ws), row_done};
+  if (p.bn == 64) return run_gemm_f8<64>(mw, mx, a, p.gp.splits, st);
+  if (p.bn == 128) return run_gemm_f8<128>(mw, mx, a, p.gp.splits, st);
+  return run_gemm_f8<256>(mw, mx, a, p.gp.splits, st);
+}
+
+int check_weight8(const char* what, const Weight8& w, int64_t M, int N) {
+  if (!w.w || !w.scale) return fail(XENCB_EINVAL, "%s: the 8-bit weight and its scales are required", what);
+  if (!aligned(w.w, 16)) return fail(XENCB_EINVAL, "%s: the 8-bit weight must be 16-byte aligned", what);
+  if (M > INT32_MAX / 2 || N > INT32_MAX / 2) return fail(XENCB_ENOTSUP, "%s: too many rows", what);
   return XENCB_OK;
 }
 
@@ -921,10 +1004,11 @@ static int project_in_impl(const void* h, int h_dtype, int64_t n_rows, int d_m, 
                            const float* gate_b_dev, const float* sel_w, const float* sel_b, int n_cand, float rms_eps,
                            float* q_out, float* gate_out, float* rstd_out, float* z_out, void* workspace,
                            size_t workspace_bytes, void* stream, const RouteFuse* rf,
-                           const AdaptArgs* adapters = nullptr, int adapt_dtype = 0) {
+                           const AdaptArgs* adapters = nullptr, int adapt_dtype = 0, const Weight8* w8 = nullptr) {
   if (flags & ~(XENCB_PIN_RMS | XENCB_PIN_L2)) return fail(XENCB_EINVAL, "project_in: unknown flags 0x%x", flags);
-  if (!h || (!w_in && !w_prep) || !q_out) return fail(XENCB_EINVAL, "project_in: h, w_in (or w_prep) and q_out are required");
-  if (!w_in && (d_m % 8 != 0 || !aligned(w_prep, 256)))
+  if (!h || (!w_in && !w_prep && !w8) || !q_out)
+    return fail(XENCB_EINVAL, "project_in: h, w_in (or w_prep) and q_out are required");
+  if (!w_in && !w8 && (d_m % 8 != 0 || !aligned(w_prep, 256)))
     return fail(XENCB_EINVAL, "project_in: without w_in, w_prep must be 256-byte aligned and d_m %% 8 == 0");
   if (n_rows <= 0 || d_m <= 0 || d_s <= 0)
     return fail(XENCB_EINVAL, "project_in: n_rows=%lld d_m=%d d_s=%d must be positive", (long long)n_rows, d_m, d_s);
@@ -942,8 +1026,10 @@ static int project_in_impl(const void* h, int h_dtype, int64_t n_rows, int d_m, 
   int rc = device_info(&di);
   if (rc) return rc;
   const int nch = (d_s + PIN_CHUNK - 1) / PIN_CHUNK;
+  if (w8 && (rc = check_weight8("project_in8", *w8, n_rows, d_s))) return rc;
+  const F8Plan p8 = w8 ? plan_f8(n_rows, d_s, d_m, di.sms) : F8Plan{};
   const size_t slice = adapters ? adapt_part_extra(n_rows, d_s, d_m, di.sms) : 0;
-  const size_t g_bytes = gemm_ws_bytes(n_rows, d_s, d_m, di.sms, true) + slice;
+  const size_t g_bytes = w8 ? p8.total : gemm_ws_bytes(n_rows, d_s, d_m, di.sms, true) + slice;
   const size_t nq_bytes = align_up((size_t)n_rows * nch * sizeof(float), 256);
   const size_t rd_bytes = align_up((size_t)n_rows * sizeof(int), 256);
   const size_t need = g_bytes + nq_bytes + rd_bytes + (adapters ? adapt_t_bytes(n_rows, adapters->r) : 0);
@@ -971,7 +1057,14 @@ static int project_in_impl(const void* h, int h_dtype, int64_t n_rows, int d_m, 
     }
     if (rc) return rc;
   }
-  switch (h_dtype) {
+  if (w8) {
+    gp = p8.gp;
+    switch (h_dtype) {
+      case XENCB_F32: rc = launch_gemm_f8<float>(h, n_rows, d_m, *w8, d_s, di.sms, p8, ws, row_done, st); break;
+      case XENCB_F16: rc = launch_gemm_f8<__half>(h, n_rows, d_m, *w8, d_s, di.sms, p8, ws, row_done, st); break;
+      default: rc = launch_gemm_f8<__nv_bfloat16>(h, n_rows, d_m, *w8, d_s, di.sms, p8, ws, row_done, st); break;
+    }
+  } else switch (h_dtype) {
     case XENCB_F32:
       rc = launch_gemm<float>(h, n_rows, d_m, w_in, d_s, di.sms, part, w_prep ? xbuf : nullptr, row_done, st, &gp,
                               w_prep, min_splits, adapters != nullptr);
@@ -1698,9 +1791,10 @@ static int project_out_impl(const float* r, int64_t n_rows, int d_s, const float
                             const float* sel_w, float log_alpha, const float* log_alpha_dev, const float* pos_mask,
                             const void* h, int h_dtype, void* delta_out, void* h_out, float* rel_out, void* workspace,
                             size_t workspace_bytes, void* stream, const AdaptArgs* adapters = nullptr,
-                            int adapt_dtype = 0) {
-  if (!r || (!w_out && !w_prep) || !h) return fail(XENCB_EINVAL, "project_out: r, w_out (or w_prep) and h are required");
-  if (!w_out && (d_s % 8 != 0 || !aligned(w_prep, 256)))
+                            int adapt_dtype = 0, const Weight8* w8 = nullptr) {
+  if (!r || (!w_out && !w_prep && !w8) || !h)
+    return fail(XENCB_EINVAL, "project_out: r, w_out (or w_prep) and h are required");
+  if (!w_out && !w8 && (d_s % 8 != 0 || !aligned(w_prep, 256)))
     return fail(XENCB_EINVAL, "project_out: without w_out, w_prep must be 256-byte aligned and d_s %% 8 == 0");
   if (n_rows <= 0 || d_m <= 0 || d_s <= 0) return fail(XENCB_EINVAL, "project_out: sizes must be positive");
   if (!elem_size(h_dtype)) return fail(XENCB_EINVAL, "project_out: h_dtype %d unknown", h_dtype);
@@ -1710,8 +1804,10 @@ static int project_out_impl(const float* r, int64_t n_rows, int d_s, const float
   int rc = device_info(&di);
   if (rc) return rc;
   const int nch = (d_m + PIN_CHUNK - 1) / PIN_CHUNK;
+  if (w8 && (rc = check_weight8("project_out8", *w8, n_rows, d_m))) return rc;
+  const F8Plan p8 = w8 ? plan_f8(n_rows, d_m, d_s, di.sms) : F8Plan{};
   const size_t slice = adapters ? adapt_part_extra(n_rows, d_m, d_s, di.sms) : 0;
-  const size_t g_bytes = gemm_ws_bytes(n_rows, d_m, d_s, di.sms, false) + slice;
+  const size_t g_bytes = w8 ? p8.total : gemm_ws_bytes(n_rows, d_m, d_s, di.sms, false) + slice;
   const size_t d_bytes = align_up((size_t)n_rows * d_m * sizeof(float), 256);
   const size_t np_bytes = align_up((size_t)n_rows * nch * 3 * sizeof(float), 256);
   const size_t rd_bytes = align_up((size_t)n_rows * sizeof(int), 256);
@@ -1736,8 +1832,13 @@ static int project_out_impl(const float* r, int64_t n_rows, int d_s, const float
     rc = launch_adapt_shrink<float>(r, ad, adapt_dtype, st);
     if (rc) return rc;
   }
-  rc = launch_gemm<float>(r, n_rows, d_s, w_out, d_m, di.sms, part, w_prep ? xbuf : nullptr, nullptr, st, &gp, w_prep,
-                          adapters ? adapt_min_splits(d_s) : 1, adapters != nullptr);
+  if (w8) {
+    gp = p8.gp;
+    rc = launch_gemm_f8<float>(r, n_rows, d_s, *w8, d_m, di.sms, p8, ws, nullptr, st);
+  } else {
+    rc = launch_gemm<float>(r, n_rows, d_s, w_out, d_m, di.sms, part, w_prep ? xbuf : nullptr, nullptr, st, &gp, w_prep,
+                            adapters ? adapt_min_splits(d_s) : 1, adapters != nullptr);
+  }
   if (rc) return rc;
   if (adapters) {  // the low-rank term is one more split partial
     rc = launch_adapt_expand(part + (size_t)gp.splits * n_rows * d_m, ad, adapt_dtype, st);
@@ -1845,6 +1946,62 @@ int xencb_project_out_adapted(const float* r, int64_t n_rows, int d_s, const flo
   return project_out_impl(r, n_rows, d_s, w_out, w_prep, b_out, d_m, scale, log_scale_dev, gate, sel_w, log_alpha,
                           log_alpha_dev, pos_mask, h, h_dtype, delta_out, h_out, rel_out, workspace, workspace_bytes,
                           stream, &ad, adapt_dtype);
+}
+
+// ------------------------------------------------------------------------------------------------ 8-bit projections
+int xencb_quant8(const void* x, int dtype, int64_t n, int k, void* x8, void* scale, void* stream) {
+  if (!x || !x8 || !scale) return fail(XENCB_EINVAL, "quant8: x, x8 and scale are required");
+  if (n <= 0 || k <= 0) return fail(XENCB_EINVAL, "quant8: n=%lld k=%d must be positive", (long long)n, k);
+  if (!elem_size(dtype)) return fail(XENCB_EINVAL, "quant8: dtype %d unknown", dtype);
+  if (!aligned(x8, 16)) return fail(XENCB_EINVAL, "quant8: x8 must be 16-byte aligned");
+  DevInfo di;
+  const int rc = device_info(&di);
+  if (rc) return rc;
+  uint8_t* s = static_cast<uint8_t*>(scale);
+  const int nb = (k + F8_BK - 1) / F8_BK;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case XENCB_F32: return launch_quant_f8<float>(x, n, k, x8, s, nb, di.sms, st);
+    case XENCB_F16: return launch_quant_f8<__half>(x, n, k, x8, s, nb, di.sms, st);
+    default: return launch_quant_f8<__nv_bfloat16>(x, n, k, x8, s, nb, di.sms, st);
+  }
+}
+
+size_t xencb_project_in8_workspace(int64_t n_rows, int d_m, int d_s) {
+  DevInfo di;
+  if (n_rows <= 0 || d_m <= 0 || d_s <= 0 || device_info(&di)) return 0;
+  const int nch = (d_s + PIN_CHUNK - 1) / PIN_CHUNK;
+  return plan_f8(n_rows, d_s, d_m, di.sms).total + align_up((size_t)n_rows * nch * sizeof(float), 256) +
+         align_up((size_t)n_rows * sizeof(int), 256);
+}
+
+int xencb_project_in8(const void* h, int h_dtype, int64_t n_rows, int d_m, const void* w8, const void* w_scale,
+                      const float* b_in, int d_s, int flags, const float* gate_w, float gate_b, const float* gate_b_dev,
+                      const float* sel_w, const float* sel_b, int n_cand, float rms_eps, float* q_out, float* gate_out,
+                      float* rstd_out, float* z_out, void* workspace, size_t workspace_bytes, void* stream) {
+  const Weight8 w{w8, static_cast<const uint8_t*>(w_scale)};
+  return project_in_impl(h, h_dtype, n_rows, d_m, nullptr, nullptr, b_in, d_s, flags, gate_w, gate_b, gate_b_dev, sel_w,
+                         sel_b, n_cand, rms_eps, q_out, gate_out, rstd_out, z_out, workspace, workspace_bytes, stream,
+                         nullptr, nullptr, 0, &w);
+}
+
+size_t xencb_project_out8_workspace(int64_t n_rows, int d_s, int d_m) {
+  DevInfo di;
+  if (n_rows <= 0 || d_m <= 0 || d_s <= 0 || device_info(&di)) return 0;
+  const int nch = (d_m + PIN_CHUNK - 1) / PIN_CHUNK;
+  return plan_f8(n_rows, d_m, d_s, di.sms).total + align_up((size_t)n_rows * d_m * sizeof(float), 256) +
+         align_up((size_t)n_rows * nch * 3 * sizeof(float), 256) + align_up((size_t)n_rows * sizeof(int), 256);
+}
+
+int xencb_project_out8(const float* r, int64_t n_rows, int d_s, const void* w8, const void* w_scale, const float* b_out,
+                       int d_m, float scale, const float* log_scale_dev, const float* gate, const float* sel_w,
+                       float log_alpha, const float* log_alpha_dev, const float* pos_mask, const void* h, int h_dtype,
+                       void* delta_out, void* h_out, float* rel_out, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  const Weight8 w{w8, static_cast<const uint8_t*>(w_scale)};
+  return project_out_impl(r, n_rows, d_s, nullptr, nullptr, b_out, d_m, scale, log_scale_dev, gate, sel_w, log_alpha,
+                          log_alpha_dev, pos_mask, h, h_dtype, delta_out, h_out, rel_out, workspace, workspace_bytes,
+                          stream, nullptr, 0, &w);
 }
 
 // ------------------------------------------------------------------------------------------------ pages

@@ -117,6 +117,60 @@ def weights_prep(w: torch.Tensor) -> torch.Tensor:
 
 
 @dataclass
+class Weights8:
+    """A projection weight [n, k] in 8-bit floating point, a power of two for each row's block of 128 columns.
+
+    w      [n, 128 * ceil(k / 128)] torch.float8_e4m3fn, zeros behind column k
+    scale  [n, ceil(k / 128)] uint8 (or torch.float8_e8m0fnu): e + 127 of the block's factor 2^e
+    k      the weight's columns"""
+
+    w: torch.Tensor
+    scale: torch.Tensor
+    k: int
+
+    @property
+    def shape(self) -> tuple:
+        return (int(self.w.shape[0]), int(self.k))
+
+
+def weights_fp8(w: torch.Tensor) -> Weights8:
+    """A weight [n, k] (float32 / float16 / bfloat16) in 8 bits, for project_in / project_out: each row's block of 128
+    columns times the smallest power of two that brings its largest value to at most 448, rounded to nearest even."""
+    dev = _cuda("weights_fp8", w)
+    if w.dim() != 2 or w.numel() == 0:
+        raise ValueError(f"weights_fp8: w must be a non-empty [n, k] matrix, got {tuple(w.shape)}")
+    w = w.detach().contiguous()
+    dt = _hdt(w, "w")
+    n, k = w.shape
+    nb = -(-k // 128)
+    out = torch.empty(n, nb * 128, dtype=torch.float8_e4m3fn, device=dev)
+    scale = torch.empty(n, nb, dtype=torch.uint8, device=dev)
+    with _on_device(dev):
+        N.call("xencb_quant8", _ptr(w), dt, n, k, _ptr(out), _ptr(scale), _stream(dev))
+    return Weights8(w=out, scale=scale, k=k)
+
+
+def _weights8(what: str, dev, w: Weights8, d_in: int, adapters):
+    """(n, w, scale), checked; a row of d_in values is to be multiplied with it."""
+    if adapters is not None:
+        raise NotImplementedError(f"{what}: adapters beside an 8-bit weight")
+    if _cuda(what, w.w, w.scale) != dev:
+        raise RuntimeError(f"{what}: the weight is on {w.w.device}, the rows on {dev}")
+    k, nb = int(w.k), -(-int(w.k) // 128)
+    if w.w.dtype != torch.float8_e4m3fn or w.w.dim() != 2 or k <= 0 or w.w.shape[1] != nb * 128 \
+            or not w.w.is_contiguous() or w.w.data_ptr() % 16:
+        raise ValueError(f"{what}: an 8-bit weight of {k} columns is a contiguous, 16-byte aligned float8_e4m3fn "
+                         f"[n, {nb * 128}] tensor, got {w.w.dtype} {tuple(w.w.shape)}")
+    if w.scale.dtype not in (torch.uint8, torch.float8_e8m0fnu) or tuple(w.scale.shape) != (w.w.shape[0], nb) \
+            or not w.scale.is_contiguous():
+        raise ValueError(f"{what}: the scales must be contiguous uint8 (or float8_e8m0fnu) [{w.w.shape[0]}, {nb}], got "
+                         f"{w.scale.dtype} {tuple(w.scale.shape)}")
+    if k != d_in:
+        raise ValueError(f"{what}: the weight has {k} columns, the rows {d_in}")
+    return int(w.w.shape[0]), w.w, w.scale
+
+
+@dataclass
 class Adapters:
     """Low-rank adapters of one projection, one per request (or per group of requests).
 
@@ -154,7 +208,7 @@ def _adapter_args(what: str, dev, ad: Adapters, of: Optional[torch.Tensor], rows
     return ad.a.contiguous(), ad.b.contiguous(), _hdt(ad.a, "adapters"), scale, n, r, of.contiguous(), rpa
 
 
-def project_in(h2: torch.Tensor, w_in: torch.Tensor, b_in=None, *, rms: bool = True, l2: bool = True,
+def project_in(h2: torch.Tensor, w_in, b_in=None, *, rms: bool = True, l2: bool = True,
                gate_w=None, gate_b=0.0, sel_w=None, sel_b=None, eps: float = 1e-6,
                w_prep: Optional[torch.Tensor] = None, prefer_prep: bool = False,
                adapters: Optional[Adapters] = None, adapter_of: Optional[torch.Tensor] = None,
@@ -166,14 +220,23 @@ def project_in(h2: torch.Tensor, w_in: torch.Tensor, b_in=None, *, rms: bool = T
     GEMM as 3xF16 on the f16 tensor cores (same accuracy as 3xTF32, half its MMAs); prefer_prep=True passes only
     the prepared form (w_in then only gives the shape).
     adapters: low-rank adapters added to w_in, adapter_of [ceil(R / rows_per_adapter)] int32 the one of each group of
-    rows_per_adapter rows (negative: none)."""
-    dev = _cuda("project_in", h2, w_in, b_in, gate_w, sel_w, sel_b)
+    rows_per_adapter rows (negative: none).
+    w_in may be a Weights8: the rows are then put into 8 bits too (blocks of 128 columns of h2 as it is given, so 1/rms, the
+    gate and the selector's logits stay what they are), and the products are accumulated in float32. A row with a value
+    that is not finite gives NaN."""
+    w8 = w_in if isinstance(w_in, Weights8) else None
+    dev = _cuda("project_in", h2, None if w8 else w_in, b_in, gate_w, sel_w, sel_b)
     h2 = h2.contiguous()
-    w_in = _f32(w_in, "w_in")
     R, d_m = h2.shape
-    d_s = w_in.shape[0]
-    if w_in.shape[1] != d_m:
-        raise ValueError(f"w_in is {tuple(w_in.shape)}, expected [d_s, {d_m}] (nn.Linear layout)")
+    if w8 is not None:
+        if w_prep is not None:
+            raise ValueError("project_in: w_prep is the prepared form of a float32 weight")
+        d_s, w8_w, w8_s = _weights8("project_in", dev, w8, d_m, adapters)
+    else:
+        w_in = _f32(w_in, "w_in")
+        d_s = w_in.shape[0]
+        if w_in.shape[1] != d_m:
+            raise ValueError(f"w_in is {tuple(w_in.shape)}, expected [d_s, {d_m}] (nn.Linear layout)")
     q = torch.empty(R, d_s, dtype=torch.float32, device=dev)
     gate = torch.empty(R, dtype=torch.float32, device=dev) if gate_w is not None else None
     rstd = torch.empty(R, dtype=torch.float32, device=dev)
@@ -185,6 +248,12 @@ def project_in(h2: torch.Tensor, w_in: torch.Tensor, b_in=None, *, rms: bool = T
     sel_w, sel_b = _f32(sel_w, "sel_w"), _f32(sel_b, "sel_b")
     gb, gb_dev = _dev_scalar(gate_b, "gate_b")
     with _on_device(dev):
+        if w8 is not None:
+            ws = _workspace(N.lib().xencb_project_in8_workspace(R, d_m, d_s), dev)
+            N.call("xencb_project_in8", _ptr(h2), _hdt(h2, "h"), R, d_m, _ptr(w8_w), _ptr(w8_s), _ptr(b_in), d_s, flags,
+                   _ptr(gate_w), gb, _ptr(gb_dev), _ptr(sel_w), _ptr(sel_b), n_cand, eps, _ptr(q), _ptr(gate),
+                   _ptr(rstd), _ptr(z), _ptr(ws), ws.numel(), _stream(dev))
+            return q, gate, rstd, z
         w_arg = None if (prefer_prep and w_prep is not None) else w_in
         if adapters is not None:
             a, b, dt, scale, n, r, of, rpa = _adapter_args("project_in", dev, adapters, adapter_of, rows_per_adapter,
@@ -303,7 +372,7 @@ def project_in_route_lse(h2: torch.Tensor, w_in: torch.Tensor, b_in=None, *, S: 
     return q, w, header_out
 
 
-def project_out(r: torch.Tensor, w_out: torch.Tensor, h2: torch.Tensor, *, b_out=None, scale: float = 1.0,
+def project_out(r: torch.Tensor, w_out, h2: torch.Tensor, *, b_out=None, scale: float = 1.0,
                 log_scale: Optional[torch.Tensor] = None, gate=None, sel_w=None, log_alpha=0.0, pos_mask=None,
                 want_delta: bool = True, h_out: Optional[torch.Tensor] = None, want_rel: bool = False,
                 w_prep: Optional[torch.Tensor] = None, prefer_prep: bool = False,
@@ -316,13 +385,19 @@ def project_out(r: torch.Tensor, w_out: torch.Tensor, h2: torch.Tensor, *, b_out
     log_scale is a one-element device tensor or None);
     d *= pos_mask; delta = d in h2's dtype; h_out = h2 + delta; rel = ||delta|| / (||h2|| + 1e-6).
     w_prep: weights_prep(w_out) for the 3xF16 GEMM. adapters, adapter_of, rows_per_adapter: as in project_in, added
-    to w_out."""
-    dev = _cuda("project_out", r, w_out, h2, b_out, gate, sel_w, pos_mask, h_out)
+    to w_out. w_out may be a Weights8: r is then put into 8 bits too, as in project_in."""
+    w8 = w_out if isinstance(w_out, Weights8) else None
+    dev = _cuda("project_out", r, None if w8 else w_out, h2, b_out, gate, sel_w, pos_mask, h_out)
     r = _f32(r, "r")
-    w_out = _f32(w_out, "w_out")
     h2 = h2.contiguous()
     R, d_s = r.shape
-    d_m = w_out.shape[0]
+    if w8 is not None:
+        if w_prep is not None:
+            raise ValueError("project_out: w_prep is the prepared form of a float32 weight")
+        d_m, w8_w, w8_s = _weights8("project_out", dev, w8, d_s, adapters)
+    else:
+        w_out = _f32(w_out, "w_out")
+        d_m = w_out.shape[0]
     if w_out.shape[1] != d_s or h2.shape != (R, d_m):
         raise ValueError(f"project_out: r {tuple(r.shape)}, w_out {tuple(w_out.shape)}, h {tuple(h2.shape)}")
     delta = torch.empty_like(h2) if want_delta else None
@@ -334,6 +409,12 @@ def project_out(r: torch.Tensor, w_out: torch.Tensor, h2: torch.Tensor, *, b_out
     la, la_dev = _dev_scalar(log_alpha, "log_alpha")
     ls_dev = None if log_scale is None else _dev_scalar(log_scale, "log_scale")[1]
     with _on_device(dev):
+        if w8 is not None:
+            ws = _workspace(N.lib().xencb_project_out8_workspace(R, d_s, d_m), dev)
+            N.call("xencb_project_out8", _ptr(r), R, d_s, _ptr(w8_w), _ptr(w8_s), _ptr(b_out), d_m, float(scale),
+                   _ptr(ls_dev), _ptr(gate), _ptr(sel_w), la, _ptr(la_dev), _ptr(pos_mask), _ptr(h2), _hdt(h2, "h"),
+                   _ptr(delta), _ptr(h_out), _ptr(rel), _ptr(ws), ws.numel(), _stream(dev))
+            return delta, h_out, rel
         w_arg = None if (prefer_prep and w_prep is not None) else w_out
         if adapters is not None:
             a, b, dt, ad_scale, n, rk, of, rpa = _adapter_args("project_out", dev, adapters, adapter_of,
