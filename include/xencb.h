@@ -433,6 +433,31 @@ XENCB_API int xencb_pages_compact(void* const* pools, const int64_t* row_bytes, 
                                   const int32_t* n_chunks_of, int64_t n_lib, int32_t* page_of_out,
                                   int32_t* n_live_out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Eviction: of every page that some table names, the rows with the largest mass stay, in their order, at the front; the
+ * same rows in every pool. mass [n_pages, page_rows] float32 is what read_mass accumulates (NaN counts as the smallest).
+ * rows(p) = the most rows of page p that some entry reads (n_valid); rank = a row's place among those by mass, the
+ * largest first, ties to the lower row.
+ *   per_library 0  keep [n_lib, n_chunks] (NULL: keep_all everywhere): page p keeps its rows with rank <
+ *                  min(rows(p), new_rows, max(keep, floor)), keep the largest of the entries that name the page
+ *   per_library 1  keep [n_lib] (NULL: keep_all) is a budget for a whole Library: every page keeps its `floor` heaviest
+ *                  rows; what those of them that the Library reads leave of its budget goes to the heaviest other rows
+ *                  that it reads, rank < new_rows, ties to the lower chunk, then to the lower row. A row stays if some
+ *                  Library keeps it.
+ * pools_out[i] is a pool of [n_pages, new_rows] rows (rows behind those that stay, and pages that no table names, become
+ * zeros), or pools[i] itself with new_rows = page_rows: in place, where the rows that went become zeros, and rows that no
+ * table read and pages that none names stay as they were.
+ * n_valid_out [n_lib, n_chunks]: the rows of each entry that stay (those before its own n_valid). A Library that reads
+ * fewer rows of a page than another may be left with none. mass_out [n_pages, new_rows] and kept_out [n_pages, new_rows]:
+ * the mass and the old row of each row that stays; 0 and -1 behind them. page_rows at most 4096. The table itself does not
+ * change. */
+XENCB_API size_t xencb_pages_evict_workspace(int64_t n_pages, int page_rows, int per_library);
+XENCB_API int xencb_pages_evict(const void* const* pools, void* const* pools_out, const int64_t* row_bytes, int n_pools,
+                                int64_t n_pages, int page_rows, int new_rows, const int32_t* page_of,
+                                const int32_t* n_valid, int n_chunks, const int32_t* n_chunks_of, int64_t n_lib,
+                                const float* mass, const int32_t* keep, int keep_all, int per_library, int floor,
+                                int32_t* n_valid_out, float* mass_out, int32_t* kept_out, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------------------------------------------------
  * LayerSelector weights from logits. Replaces LayerSelector._weights_from_logits (xenc/selector.py:59-67),
  * forward value: top-k of z (ties to the lower index), softmax over the kept (or 1/k when

@@ -89,6 +89,9 @@ SIGNATURES: dict = {
     "xencb_pages_fork": (_i, [_p, _p, _i, _i64, _i, _p, _p, _i, _p, _i64, _p, _p, _i64, _p, _p, _p, _sz, _p]),
     "xencb_pages_compact_workspace": (_sz, [_i64]),
     "xencb_pages_compact": (_i, [_p, _p, _i, _i64, _i, _p, _p, _i, _p, _i64, _p, _p, _p, _sz, _p]),
+    "xencb_pages_evict_workspace": (_sz, [_i64, _i, _i]),
+    "xencb_pages_evict": (_i, [_p, _p, _p, _i, _i64, _i, _i, _p, _p, _i, _p, _i64, _p, _p, _i, _i, _i, _p, _p, _p, _p, _sz,
+                               _p]),
     "xencb_selector_weights": (_i, [_p, _i64, _i, _i, _i, _p, _p]),
     "xencb_selector_logits": (_i, [_p, _i, _i64, _i, _p, _p, _i, _i, _f, _p, _p]),
     "xencb_selector_apply": (_i, [_p, _i, _p, _i, _i64, _i, _p, _i, _i, _f, _p, _p]),

@@ -29,6 +29,7 @@
 #include "attn.cuh"
 #include "exchange.cuh"
 #include "pages.cuh"
+#include "evict.cuh"
 #include "adapt.cuh"
 #include "read_shared.cuh"
 
@@ -2131,6 +2132,104 @@ int xencb_pages_compact(void* const* pools, const int64_t* row_bytes, int n_pool
   pages_compact_plan_kernel<<<1, PG_THREADS, smem, st>>>(a);
   XENCB_CHECK_LAUNCH("pages_compact_plan launch");
   return launch_page_copies(pools, row_bytes, n_pools, page_rows, n_pages / 2 + 1, a.moves, a.n_moves, di.sms, st);
+}
+
+size_t xencb_pages_evict_workspace(int64_t n_pages, int page_rows, int per_library) {
+  if (n_pages <= 0 || page_rows <= 0 || page_rows > EV_MAX_ROWS || n_pages > PG_MAX_PAGES) return 0;
+  const size_t lists = 3 * pages_list_bytes(n_pages);
+  if (!per_library) return lists;
+  return lists + align_up((size_t)n_pages * page_rows * sizeof(uint16_t), 256) +
+         align_up((size_t)n_pages * ((page_rows + 31) / 32) * sizeof(uint32_t), 256);
+}
+
+int xencb_pages_evict(const void* const* pools, void* const* pools_out, const int64_t* row_bytes, int n_pools,
+                      int64_t n_pages, int page_rows, int new_rows, const int32_t* page_of, const int32_t* n_valid,
+                      int n_chunks, const int32_t* n_chunks_of, int64_t n_lib, const float* mass, const int32_t* keep,
+                      int keep_all, int per_library, int floor, int32_t* n_valid_out, float* mass_out,
+                      int32_t* kept_out, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!pools_out) return fail(XENCB_EINVAL, "pages_evict: pools_out is required (pools: in place)");
+  int rc = check_pools("pages_evict", const_cast<void* const*>(reinterpret_cast<const void* const*>(pools)), row_bytes,
+                       n_pools, n_pages, page_rows);
+  if (!rc) rc = check_pools("pages_evict", pools_out, row_bytes, n_pools, n_pages, page_rows);
+  if (rc) return rc;
+  if (!page_of || !n_valid || !mass || !n_valid_out || !mass_out || !kept_out)
+    return fail(XENCB_EINVAL, "pages_evict: page_of, n_valid, mass and the outputs are required");
+  if (n_chunks <= 0 || n_lib <= 0) return fail(XENCB_EINVAL, "pages_evict: n_lib and n_chunks must be positive");
+  if (n_lib > INT32_MAX / n_chunks) return fail(XENCB_ENOTSUP, "pages_evict: the table is too large");
+  if (page_rows > EV_MAX_ROWS)
+    return fail(XENCB_ENOTSUP, "pages_evict: page_rows=%d, at most %d are supported", page_rows, EV_MAX_ROWS);
+  if (new_rows <= 0 || new_rows > page_rows)
+    return fail(XENCB_EINVAL, "pages_evict: new_rows=%d must be 1 .. page_rows=%d", new_rows, page_rows);
+  if (floor < 0) return fail(XENCB_EINVAL, "pages_evict: floor=%d must not be negative", floor);
+  int inplace = 0;
+  for (int i = 0; i < n_pools; ++i) inplace += pools_out[i] == pools[i];
+  if (inplace && (inplace != n_pools || new_rows != page_rows))
+    return fail(XENCB_EINVAL, "pages_evict: in place, every pool is its own output and new_rows is page_rows");
+  const size_t need = xencb_pages_evict_workspace(n_pages, page_rows, per_library);
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < need)
+    return fail(XENCB_EINVAL, "pages_evict: workspace needs %zu bytes, 256-byte aligned (got %zu)", need,
+                workspace_bytes);
+  DevInfo di;
+  rc = device_info(&di);
+  if (rc) return rc;
+  char* ws = static_cast<char*>(workspace);
+  const size_t list = pages_list_bytes(n_pages);
+  EvictArgs a{};
+  a.page_of = page_of; a.n_valid = n_valid; a.n_chunks_of = n_chunks_of; a.n_lib = n_lib; a.C = n_chunks;
+  a.n_pages = (int)n_pages; a.page_rows = page_rows; a.new_rows = new_rows; a.mass = mass; a.keep = keep;
+  a.keep_all = keep_all; a.per_library = per_library ? 1 : 0; a.floor = floor;
+  a.n_valid_out = n_valid_out; a.mass_out = mass_out; a.kept = kept_out;
+  a.rows = reinterpret_cast<int*>(ws);
+  a.most = reinterpret_cast<int*>(ws + list);
+  a.count = reinterpret_cast<int*>(ws + 2 * list);
+  a.words = (page_rows + 31) / 32;
+  if (per_library) {
+    a.rank = reinterpret_cast<uint16_t*>(ws + 3 * list);
+    a.bits = reinterpret_cast<uint32_t*>(ws + 3 * list + align_up((size_t)n_pages * page_rows * sizeof(uint16_t), 256));
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  evict_plan_kernel<<<1, PG_THREADS, 0, st>>>(a);
+  XENCB_CHECK_LAUNCH("evict_plan launch");
+  int n2 = 64;
+  while (n2 < page_rows) n2 *= 2;
+  launch_pdl(evict_rank_kernel, dim3((unsigned)n_pages), dim3((unsigned)std::min(1024, std::max(64, n2 / 2))),
+             (size_t)n2 * 8, st, a, n2);
+  XENCB_CHECK_LAUNCH("evict_rank launch");
+  if (per_library) {
+    launch_pdl(evict_budget_kernel, dim3((unsigned)n_lib), dim3(PG_THREADS), 0, st, a);
+    XENCB_CHECK_LAUNCH("evict_budget launch");
+    launch_pdl(evict_list_kernel, dim3((unsigned)n_pages), dim3(256), 0, st, a);
+    XENCB_CHECK_LAUNCH("evict_list launch");
+  }
+  for (int i0 = 0; i0 < n_pools; i0 += PG_POOLS) {
+    EvictPools pp{};
+    const int n = std::min(PG_POOLS, n_pools - i0);
+    bool vec = true;
+    for (int i = 0; i < n; ++i) {
+      pp.src[i] = static_cast<const char*>(pools[i0 + i]);
+      pp.dst[i] = static_cast<char*>(pools_out[i0 + i]);
+      pp.row_bytes[i] = row_bytes[i0 + i];
+      vec = vec && aligned(pp.src[i], 16) && aligned(pp.dst[i], 16) && pp.row_bytes[i] % 16 == 0;
+    }
+    const int64_t unit = vec ? 16 : 2;
+    int64_t slices = 0;
+    for (int i = 0; i < n; ++i) {
+      pp.first[i] = (int)slices;
+      const int64_t row = pp.row_bytes[i] / unit;
+      if (row * page_rows > INT32_MAX) return fail(XENCB_ENOTSUP, "pages_evict: the pools' pages are too large");
+      slices += inplace ? (row + EV_THREADS - 1) / EV_THREADS
+                        : (row * new_rows + EV_THREADS * EV_UNROLL - 1) / (EV_THREADS * EV_UNROLL);
+      if (slices > INT32_MAX) return fail(XENCB_ENOTSUP, "pages_evict: the pools' pages are too large");
+    }
+    for (int i = n; i <= PG_POOLS; ++i) pp.first[i] = (int)slices;
+    pp.slices = (int)slices;
+    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(64 * (int64_t)di.sms, n_pages * slices));
+    auto go = [&](auto kern) { launch_pdl(kern, dim3(grid), dim3(EV_THREADS), 0, st, a, pp); };
+    if (inplace) vec ? go(evict_inplace_kernel<uint4>) : go(evict_inplace_kernel<uint16_t>);
+    else vec ? go(evict_gather_kernel<uint4>) : go(evict_gather_kernel<uint16_t>);
+    XENCB_CHECK_LAUNCH("evict move launch");
+  }
+  return XENCB_OK;
 }
 
 // ------------------------------------------------------------------------------------------------ selector

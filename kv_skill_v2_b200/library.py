@@ -358,6 +358,39 @@ class PagedLibrary:
         table, n_live = pages_compact(pools, page_of.contiguous(), n_valid.contiguous(), n_chunks_of=nco)
         return self._with_tables(table, n_valid, nco, None), int(n_live)
 
+    def evict(self, mass, keep, *, per_library: bool = False, floor: int = 1, page_rows: Optional[int] = None):
+        """(these Libraries without the slots that received least attention, the mass [P, rows] of those that stay).
+
+        mass: a [P, page_rows] tensor as ops.read_mass gives it, or one per layer ({layer: tensor}, as a LibraryInjector
+        with record_mass holds them): these are added up, so that a token's slots stay or go at every depth alike. keep,
+        per_library, floor as in ops.pages_evict. page_rows: new pools with pages of that many rows, the old ones are free
+        once nothing refers to them; None: within these pools, and then this PagedLibrary and any select() of it must no
+        longer be read. The summary keys stay as they are, so the routing does not change. Evict on the PagedLibrary that
+        holds every row, as for fork and compact. Rows that the Libraries read differ in number only where a page is shared by
+        Libraries with different n_valid; RuntimeError where one of them would be left with an empty chunk (new pools only).
+        Reads one flag back from the device in that case."""
+        from .ops import pages_evict
+
+        pools, page_of, n_valid, nco = self._tables()
+        page_of, n_valid = page_of.contiguous(), n_valid.contiguous()
+        if isinstance(mass, dict):
+            if not mass:
+                raise ValueError("evict: mass of at least one layer is required")
+            mass = torch.stack([mass[li] for li in sorted(mass)]).sum(0)
+        nv, new_mass, _, new = pages_evict(pools, page_of, n_valid, mass.contiguous(), keep, n_chunks_of=nco,
+                                           per_library=per_library, floor=floor, page_rows=page_rows)
+        if page_rows is not None and bool(((nv == 0) & (n_valid > 0) & self._live(page_of, nco)).any()):
+            raise RuntimeError("evict: a Library would be left with an empty chunk (a page that it shares with one that "
+                               "reads more of its rows, or keep = floor = 0)")
+        renamed = {p.data_ptr(): q for p, q in zip(pools, new)}
+        return self._with_tables(page_of, nv, nco, None, renamed), new_mass
+
+    def _live(self, page_of, n_chunks_of) -> torch.Tensor:
+        """[n_lib, C] bool: the entries of the table that are chunks."""
+        if n_chunks_of is None:
+            return torch.ones_like(page_of, dtype=torch.bool)
+        return torch.arange(page_of.shape[1], device=page_of.device).view(1, -1) < n_chunks_of.view(-1, 1)
+
     @staticmethod
     def from_libraries(libs: list, device, slot_dtype=torch.float16) -> "PagedLibrary":
         """Stack Libraries with the same layers and d_s; library b serves batch row b. When any Library is

@@ -1023,6 +1023,58 @@ def pages_compact(pools, page_of: torch.Tensor, n_valid: torch.Tensor, *,
     return out, n_live
 
 
+def pages_evict(pools, page_of: torch.Tensor, n_valid: torch.Tensor, mass: torch.Tensor, keep, *,
+                n_chunks_of: Optional[torch.Tensor] = None, per_library: bool = False, floor: int = 1,
+                page_rows: Optional[int] = None):
+    """(n_valid [n_lib, C] int32, mass [P, rows] float32, kept [P, rows] int32, pools): the rows of every page with the
+    largest mass stay, in their order, at the front of the page, the same rows in every pool.
+
+    mass [P, page_rows] float32: what read_mass accumulates (NaN counts as the smallest; ties stay with the lower row).
+    keep: rows to keep of each chunk (an int, or int32 [n_lib, C] on the device; a page keeps the most that an entry which
+    names it asks for), at least `floor`; with per_library the rows to keep of each whole Library (an int, or int32
+    [n_lib]): every page keeps its `floor` heaviest rows, the rest of the budget goes to the Library's heaviest others (ties:
+    the lower chunk), and a row stays if some Library keeps it.
+    page_rows: the rows of a page of the new pools that are returned (a page keeps no more than that), which hold zeros behind
+    the rows that stay and in pages that no table names. None: the rows move within the given pools, which are returned; rows
+    that went become zeros.
+    n_valid are the new counts for the same page_of (a Library that reads fewer rows of a shared page than another may be
+    left with none of it); kept the old row of each row that stays, -1 behind them. Nothing is read back by the host."""
+    pools = list(pools)
+    dev, ptrs, sizes, P, N_rows = _pool_args("pages_evict", pools, page_of, n_valid, n_chunks_of)
+    if _cuda("pages_evict", mass) != dev:
+        raise RuntimeError(f"pages_evict: mass on {mass.device}, pools on {dev}")
+    if mass.dtype != torch.float32 or tuple(mass.shape) != (P, N_rows) or not mass.is_contiguous():
+        raise ValueError(f"pages_evict: mass must be a contiguous float32 [{P}, {N_rows}] tensor")
+    n_lib, C = page_of.shape
+    keep_all = 0
+    if isinstance(keep, torch.Tensor):
+        shape = (n_lib,) if per_library else (n_lib, C)
+        if _cuda("pages_evict", keep) != dev:
+            raise RuntimeError(f"pages_evict: keep on {keep.device}, pools on {dev}")
+        if keep.dtype != torch.int32 or tuple(keep.shape) != shape or not keep.is_contiguous():
+            raise ValueError(f"pages_evict: keep must be an int or a contiguous int32 {list(shape)} tensor")
+    else:
+        keep_all, keep = min(max(int(keep), 0), 2**31 - 1), None
+    rows = N_rows if page_rows is None else int(page_rows)
+    if not 0 < rows <= N_rows:
+        raise ValueError(f"pages_evict: page_rows={rows} must be 1 .. {N_rows}")
+    if int(floor) < 0:
+        raise ValueError(f"pages_evict: floor={floor} must not be negative")
+    if N_rows > 4096:
+        raise NotImplementedError(f"pages_evict: pages of {N_rows} rows, at most 4096 are supported")
+    out = pools if page_rows is None else [torch.empty(P, rows, p.shape[2], dtype=p.dtype, device=dev) for p in pools]
+    optrs = (ctypes.c_void_p * len(out))(*[p.data_ptr() for p in out])
+    nv = torch.empty_like(n_valid)
+    new_mass = torch.empty(P, rows, dtype=torch.float32, device=dev)
+    kept = torch.empty(P, rows, dtype=torch.int32, device=dev)
+    with _on_device(dev):
+        ws = _workspace(N.lib().xencb_pages_evict_workspace(P, N_rows, int(bool(per_library))), dev)
+        N.call("xencb_pages_evict", ptrs, optrs, sizes, len(ptrs), P, N_rows, rows, _ptr(page_of), _ptr(n_valid), C,
+               _ptr(n_chunks_of), n_lib, _ptr(mass), _ptr(keep), keep_all, int(bool(per_library)), min(int(floor), N_rows),
+               _ptr(nv), _ptr(new_mass), _ptr(kept), _ptr(ws), ws.numel(), _stream(dev))
+    return nv, new_mass, kept, out
+
+
 # ------------------------------------------------------------------------------------------------ D8 top-k read
 _POOL = {"max": 0, "mean": 1}
 
