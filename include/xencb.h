@@ -287,6 +287,22 @@ XENCB_API int xencb_read_shared(const void* q, int q_dtype, int64_t n_rows, int 
                                 float read_temp, int read_softmax, void* r_out, int out_dtype, void* workspace,
                                 size_t workspace_bytes, void* stream);
 
+/* Attention mass: what every slot of the pool receives from a batch of rows, the column sums of the weights of the softmax
+ * read (xenc/injector.py:239-245; the linear read has none):
+ *   mass[p, n] = decay * prior[p, n] + sum over rows t and routed chunks j with page_of[lib(t), idx[t, j]] = p and
+ *                n < n_valid[lib(t), idx[t, j]] of wk[t, j] * softmax over n of (read_temp * q[t] . slots[p, n])
+ * Arguments as xencb_read_shared's; prior [n_pages, page_rows] or NULL (0; decay is then not used); mass [n_pages,
+ * page_rows] float32, may be prior itself. Every page is written. Float32 q takes part with 22 bits (16 with bf16 slots), a
+ * 16-bit q exactly. The sums are added in the order of the rows: the same call gives the same bits. Slots at or past
+ * n_valid may hold anything. f16 / bf16 slots, d_s a multiple of 8, page_rows at most 2048. */
+XENCB_API size_t xencb_read_mass_workspace(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows,
+                                           int slots_dtype, int q_dtype);
+XENCB_API int xencb_read_mass(const void* q, int q_dtype, int64_t n_rows, int d_s, const void* slots, int slots_dtype,
+                              int64_t n_pages, int64_t page_stride, int page_rows, const int32_t* page_of,
+                              const int32_t* n_valid, int n_chunks, int64_t rows_per_lib, int64_t n_lib,
+                              const int32_t* idx, const float* wk, int k, float read_temp, const float* prior,
+                              float decay, float* mass, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Dense routing of one chunk shard of a Library (the routing softmax of xenc/injector.py:220-229 with top_k = 0,
  * regrouped by shard): w_out [n_rows, n_chunks] = e^(l_c - max_c l_c) with l = route_temp * q . S_c, and
  * header_out [n_rows, 4] = (max_c l_c, sum_c e^(l_c - max), 0, 0). Feeding w_out to xencb_read_multi gives the

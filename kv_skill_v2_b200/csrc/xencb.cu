@@ -32,6 +32,7 @@
 #include "evict.cuh"
 #include "adapt.cuh"
 #include "read_shared.cuh"
+#include "mass.cuh"
 
 // Scratch of xencb_read_decode_noalloc: a fixed device array, so that entry point never allocates.
 static __device__ __align__(256) unsigned char g_noalloc_scratch[XENCB_NOALLOC_SCRATCH_BYTES];
@@ -855,9 +856,9 @@ int plan_shared(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows, 
   return XENCB_OK;
 }
 
-// Clusters of the read kernel that fit the device at once, per device, cluster size and kernel.
+// Clusters of a kernel that fit the device at once, per device, cluster size and kernel.
 template <typename K>
-int shared_clusters(K kern, int cs, int* out) {
+int shared_clusters(K kern, int cs, int threads, size_t smem, int* out) {
   static std::mutex mu;
   static std::unordered_map<const void*, int> known[kMaxDev][RS_MAX_CS + 1];
   int dev = 0;
@@ -871,8 +872,8 @@ int shared_clusters(K kern, int cs, int* out) {
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)cs);
-  cfg.blockDim = dim3(RS_THREADS);
-  cfg.dynamicSmemBytes = RS_SMEM;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = (unsigned)cs;
@@ -881,8 +882,8 @@ int shared_clusters(K kern, int cs, int* out) {
   cfg.numAttrs = 1;
   int n = 0;
   const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
-  if (e != cudaSuccess) return cuda_fail(e, "read_shared: cudaOccupancyMaxActiveClusters");
-  if (n <= 0) return fail(XENCB_ENOTSUP, "read_shared: no cluster of %d CTAs fits this device", cs);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaOccupancyMaxActiveClusters");
+  if (n <= 0) return fail(XENCB_ENOTSUP, "no cluster of %d CTAs fits this device", cs);
   seen[reinterpret_cast<const void*>(kern)] = n;
   *out = n;
   return XENCB_OK;
@@ -906,7 +907,7 @@ int run_shared(const void* q, int q_dtype, const SharedPlan& p, SharedArgs a, co
   auto kern = shared_read_kernel<T, TERMS>;
   if (!rc) rc = ensure_smem(kern, (int)RS_SMEM);
   int n_clusters = 0;
-  if (!rc) rc = shared_clusters(kern, p.cs, &n_clusters);
+  if (!rc) rc = shared_clusters(kern, p.cs, RS_THREADS, RS_SMEM, &n_clusters);
   if (rc) return rc;
   n_clusters = (int)std::min<int64_t>(
       n_clusters, (p.max_tiles - p.n_pairs) * p.segs);  // (the single tiles are for pages that few calls have)
@@ -960,6 +961,99 @@ int run_shared(const void* q, int q_dtype, const SharedPlan& p, SharedArgs a, co
   else if (out_dtype == XENCB_F16) combine(__half{});
   else combine(__nv_bfloat16{});
   XENCB_CHECK_LAUNCH("shared_combine launch");
+  return XENCB_OK;
+}
+// ------------------------------------------------------------------------------------------------ attention mass plan
+struct MassPlan {
+  int terms, cs, per;
+  int64_t n_pairs, max_tiles;
+  size_t pages, pair, tiles, q, rinv, part, total;
+};
+
+int plan_mass(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows, int slots_dtype, int q_dtype, MassPlan* p) {
+  if (n_rows <= 0 || k <= 0 || d_s <= 0 || n_pages <= 0 || page_rows <= 0)
+    return fail(XENCB_EINVAL, "read_mass: sizes must be positive");
+  if (slots_dtype != XENCB_F16 && slots_dtype != XENCB_BF16)
+    return fail(XENCB_ENOTSUP, "read_mass: the tensor cores take f16 / bf16 slots");
+  if (!elem_size(q_dtype)) return fail(XENCB_EINVAL, "read_mass: q_dtype %d unknown", q_dtype);
+  if (d_s % 8 != 0) return fail(XENCB_ENOTSUP, "read_mass: d_s=%d must be a multiple of 8", d_s);
+  if (page_rows > MS_N * MS_MAX_CS)
+    return fail(XENCB_ENOTSUP, "read_mass: page_rows=%d, at most %d are supported", page_rows, MS_N * MS_MAX_CS);
+  if (n_rows > (INT32_MAX - 64) / k || n_pages * (int64_t)page_rows + 1024 > INT32_MAX)
+    return fail(XENCB_ENOTSUP, "read_mass: too many rows, routed chunks or pages");
+  p->n_pairs = n_rows * k;
+  // a 16-bit q is one product where the slots' type holds it (bf16's 8 bits fit f16)
+  p->terms = q_dtype == XENCB_F32 || (q_dtype == XENCB_F16 && slots_dtype == XENCB_BF16) ? 2 : 1;
+  p->cs = (page_rows + MS_N - 1) / MS_N;
+  p->per = (int)align_up((size_t)(page_rows + p->cs - 1) / p->cs, 16);
+  p->max_tiles = p->n_pairs / MS_M + std::min<int64_t>(n_pages, p->n_pairs);
+  p->pages = align_up((size_t)n_pages * 4, 256);
+  p->pair = align_up((size_t)p->n_pairs * 4, 256);
+  p->tiles = align_up((size_t)p->max_tiles * sizeof(MassTile), 256);
+  p->q = align_up((size_t)p->terms * n_rows * d_s * 2, 256);
+  p->rinv = align_up((size_t)n_rows * 4, 256);
+  p->part = align_up((size_t)p->max_tiles * page_rows * 4, 256);
+  p->total = 4 * p->pages + 4 * p->pair + p->tiles + 256 + p->q + p->rinv + p->part;
+  return XENCB_OK;
+}
+
+template <typename T, int TERMS>
+int run_mass(const void* q, int q_dtype, const MassPlan& p, const MassArgs& a, const void* slots, void* q16, int sms,
+             cudaStream_t st) {
+  const CUtensorMapDataType dt =
+      std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const uint64_t d = (uint64_t)a.d_s;
+  CUtensorMap mk;
+  int rc = tensor_map_2d(&mk, dt, 2, slots, d, (uint64_t)a.n_pages * a.page_rows, d * 2, 64, (uint32_t)p.per);
+  auto kern = mass_scores_kernel<T, TERMS>;
+  const size_t smem = ms_smem(TERMS, p.cs);
+  if (!rc) rc = ensure_smem(kern, (int)smem);
+  int n_clusters = 0;
+  if (!rc) rc = shared_clusters(kern, p.cs, MS_THREADS, smem, &n_clusters);
+  if (rc) return rc;
+  // the softmax warps wait for the registers that the others give up: the launch must have as many
+  static const int regs = [&] {
+    cudaFuncAttributes fa;
+    return cudaFuncGetAttributes(&fa, kern) == cudaSuccess ? fa.numRegs * MS_THREADS : 0;
+  }();
+  if (regs < MS_REGS) return fail(XENCB_ENOTSUP, "read_mass: built with %d registers a CTA, %d are needed", regs, MS_REGS);
+  n_clusters = (int)std::min<int64_t>(n_clusters, p.max_tiles);
+  const int counted = p.n_pairs > MS_ONE_CTA;
+  if (counted) {
+    const cudaError_t e = cudaMemsetAsync(a.cnt, 0, 2 * p.pages, st);
+    if (e != cudaSuccess) return cuda_fail(e, "read_mass: memset");
+    mass_count_kernel<<<(unsigned)std::min<int64_t>((p.n_pairs + 255) / 256, 4 * sms), 256, 0, st>>>(a);
+    XENCB_CHECK_LAUNCH("mass_count launch");
+  }
+  T* qo = static_cast<T*>(q16);
+  const unsigned pgrid = 1 + (unsigned)((a.n_rows + 3) / 4);
+  auto prep = [&](auto t) {
+    using TQ = decltype(t);
+    mass_prep_kernel<TQ, T, TERMS><<<pgrid, MS_PREP_THREADS, 0, st>>>(a, static_cast<const TQ*>(q), qo, counted);
+  };
+  if (q_dtype == XENCB_F32) prep(float{});
+  else if (q_dtype == XENCB_F16) prep(__half{});
+  else prep(__nv_bfloat16{});
+  XENCB_CHECK_LAUNCH("mass_prep launch");
+  launch_pdl(mass_order_kernel, dim3((unsigned)a.n_pages), dim3(MS_ORDER_THREADS), 0, st, a);
+  XENCB_CHECK_LAUNCH("mass_order launch");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(n_clusters * p.cs));
+  cfg.blockDim = dim3(MS_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)p.cs;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  (void)cudaLaunchKernelEx(&cfg, kern, mk, a);
+  XENCB_CHECK_LAUNCH("mass_scores launch");
+  launch_pdl(mass_combine_kernel, dim3((unsigned)a.n_pages, (unsigned)((a.page_rows + 255) / 256)), dim3(256), 0, st, a);
+  XENCB_CHECK_LAUNCH("mass_combine launch");
   return XENCB_OK;
 }
 }  // namespace
@@ -1775,6 +1869,70 @@ int xencb_read_shared(const void* q, int q_dtype, int64_t n_rows, int d_s, const
   auto go = [&](auto run) { return run(q, q_dtype, p, a, slots, vslots, q16, n_rows, r_out, out_dtype, di.sms, st); };
   if (slots_dtype == XENCB_BF16) return go(run_shared<__nv_bfloat16, 2>);  // (plan_shared: bf16 slots always take two terms)
   return p.terms == 2 ? go(run_shared<__half, 2>) : go(run_shared<__half, 1>);
+}
+
+// ------------------------------------------------------------------------------------------------ read_mass
+size_t xencb_read_mass_workspace(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows, int slots_dtype,
+                                 int q_dtype) {
+  MassPlan p;
+  return plan_mass(n_rows, k, d_s, n_pages, page_rows, slots_dtype, q_dtype, &p) ? 0 : p.total;
+}
+
+int xencb_read_mass(const void* q, int q_dtype, int64_t n_rows, int d_s, const void* slots, int slots_dtype,
+                    int64_t n_pages, int64_t page_stride, int page_rows, const int32_t* page_of, const int32_t* n_valid,
+                    int n_chunks, int64_t rows_per_lib, int64_t n_lib, const int32_t* idx, const float* wk, int k,
+                    float read_temp, const float* prior, float decay, float* mass, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  if (!q || !slots || !page_of || !n_valid || !idx || !wk || !mass)
+    return fail(XENCB_EINVAL, "read_mass: q, slots, page_of, n_valid, idx, wk and mass are required");
+  if (n_chunks <= 0 || rows_per_lib <= 0 || n_lib <= 0) return fail(XENCB_EINVAL, "read_mass: sizes must be positive");
+  MassPlan p;
+  int rc = plan_mass(n_rows, k, d_s, n_pages, page_rows, slots_dtype, q_dtype, &p);
+  if (rc) return rc;
+  if ((n_rows + rows_per_lib - 1) / rows_per_lib > n_lib)
+    return fail(XENCB_EINVAL, "read_mass: %lld rows need more than %lld Libraries", (long long)n_rows, (long long)n_lib);
+  if (page_stride != (int64_t)page_rows * d_s)
+    return fail(XENCB_ENOTSUP, "read_mass: the slot pool must be dense ([pages, page_rows, d_s])");
+  if (!aligned(slots, 16) || !aligned(q, 16))
+    return fail(XENCB_EINVAL, "read_mass: slots and q must be 16-byte aligned");
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < p.total)
+    return fail(XENCB_EINVAL, "read_mass: workspace needs %zu bytes, 256-byte aligned (got %zu)", p.total,
+                workspace_bytes);
+  DevInfo di;
+  rc = device_info(&di);
+  if (rc) return rc;
+  char* ws = static_cast<char*>(workspace);
+  auto take = [&](size_t bytes) {
+    char* at = ws;
+    ws += bytes;
+    return at;
+  };
+  MassArgs a{};
+  a.page_of = page_of; a.n_valid = n_valid; a.idx = idx; a.wk = wk; a.n_rows = n_rows; a.rows_per_lib = rows_per_lib;
+  a.n_lib = n_lib; a.k = k; a.C = n_chunks; a.n_pages = (int)n_pages; a.page_rows = page_rows; a.d_s = d_s;
+  a.n_pairs = (int)p.n_pairs;
+  a.cnt = reinterpret_cast<int*>(take(p.pages));
+  a.nvmax = reinterpret_cast<int*>(take(p.pages));
+  a.start = reinterpret_cast<int*>(take(p.pages));
+  a.tile0 = reinterpret_cast<int*>(take(p.pages));
+  a.page = reinterpret_cast<int*>(take(p.pair));
+  a.prow = reinterpret_cast<int*>(take(p.pair));
+  a.pnv = reinterpret_cast<int*>(take(p.pair));
+  a.pw = reinterpret_cast<float*>(take(p.pair));
+  a.tiles = reinterpret_cast<MassTile*>(take(p.tiles));
+  a.n_tiles = reinterpret_cast<int*>(take(256));
+  void* q16 = take(p.q);
+  a.q16 = q16;
+  a.rinv = reinterpret_cast<float*>(take(p.rinv));
+  a.part = reinterpret_cast<float*>(take(p.part));
+  a.cs = p.cs; a.per = p.per;
+  a.qscale = read_temp * 1.4426950408889634f;
+  a.prior = prior; a.decay = decay; a.mass = mass;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto go = [&](auto run) { return run(q, q_dtype, p, a, slots, q16, di.sms, st); };
+  if (slots_dtype == XENCB_BF16)
+    return p.terms == 2 ? go(run_mass<__nv_bfloat16, 2>) : go(run_mass<__nv_bfloat16, 1>);
+  return p.terms == 2 ? go(run_mass<__half, 2>) : go(run_mass<__half, 1>);
 }
 
 // ------------------------------------------------------------------------------------------------ project_out

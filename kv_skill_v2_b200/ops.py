@@ -753,6 +753,50 @@ def read_shared(q: torch.Tensor, pages: Pages, idx: torch.Tensor, wk: torch.Tens
     return r
 
 
+def read_mass(q: torch.Tensor, pages: Pages, idx: torch.Tensor, wk: torch.Tensor, *, rows_per_lib: int,
+              read_temp: float = 12.0, mass: Optional[torch.Tensor] = None, decay: float = 1.0,
+              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """mass [P, page_rows] float32: the attention that every slot of the pool receives from these rows, added to decay times
+    what it had before (`mass`, None: nothing): the sum over rows and routed chunks of wk * softmax(read_temp * q . K) over the
+    chunk's valid slots, the weights with which the softmax read multiplies the values. What pages_evict goes by.
+
+    q [R, d_s] float32 / float16 / bfloat16; idx, wk [R, k] as route gives them; a page that several Libraries name gets
+    the attention of all of them. out: where to write it (may be `mass` itself). float32 q takes part with 22 bits (16 with
+    bfloat16 slots), a 16-bit q exactly; the same call gives the same bits. Slots at or past n_valid may hold anything.
+    Raises NotImplementedError for float32 slots, d_s not a multiple of 8 and pages of more than 2048 rows."""
+    po, nv = pages.page_of, pages.n_valid
+    if po.dtype is not torch.int32 or nv.dtype is not torch.int32 or po.dim() != 2 or nv.shape != po.shape \
+            or not po.is_contiguous() or not nv.is_contiguous():
+        raise ValueError("read_mass: page_of and n_valid must be contiguous int32 [n_lib, C] tensors")
+    dev = _cuda("read_mass", q, pages.slots, po, nv, idx, wk, mass, out)
+    slots = pages.slots
+    if q.dim() != 2 or not slots.is_contiguous() or slots.shape[-1] != q.shape[1]:
+        raise ValueError(f"read_mass: q must be [R, {slots.shape[-1]}], the slot pool contiguous [P, page_rows, "
+                         f"{slots.shape[-1]}]; got {tuple(q.shape)}")
+    q, wk, idx = q.contiguous(), _f32(wk, "wk"), idx.contiguous()
+    R, d_s = q.shape
+    if idx.dtype != torch.int32 or idx.dim() != 2 or idx.shape != wk.shape or idx.shape[0] != R:
+        raise ValueError("read_mass: idx must be int32 [R, k] matching wk")
+    P, page_rows, k, rpl = slots.shape[0], pages.page_rows, int(idx.shape[1]), int(rows_per_lib)
+    if rpl <= 0 or -(-R // rpl) > pages.n_lib:
+        raise ValueError(f"read_mass: {R} rows, {rpl} per Library, need more than {pages.n_lib} Libraries")
+    for name, t in (("mass", mass), ("out", out)):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (P, page_rows) or not t.is_contiguous()):
+            raise ValueError(f"read_mass: {name} must be a contiguous float32 [{P}, {page_rows}] tensor")
+    if out is None:
+        out = torch.empty(P, page_rows, dtype=torch.float32, device=dev)
+    sdt, qdt = _hdt(slots, "slots"), _hdt(q, "q")
+    with _on_device(dev):
+        ws_bytes = N.lib().xencb_read_mass_workspace(R, k, d_s, P, page_rows, sdt, qdt)
+        if ws_bytes == 0:
+            N.check(N.EINVAL if min(R, k) <= 0 else N.ENOTSUP, "read_mass_workspace")
+        ws = _workspace(ws_bytes, dev)
+        N.call("xencb_read_mass", _ptr(q), qdt, R, d_s, _ptr(slots), sdt, P, page_rows * d_s, page_rows, _ptr(po), _ptr(nv),
+               pages.n_chunks, rpl, pages.n_lib, _ptr(idx), _ptr(wk), k, float(read_temp), _ptr(mass), float(decay),
+               _ptr(out), _ptr(ws), ws_bytes, _stream(dev))
+    return out
+
+
 def shared_workspace(pages: Pages, n_rows: int, k: int, out_dtype: torch.dtype = torch.float32) -> int:
     """Bytes of workspace for n_rows rows of k routed chunks in one read_shared call; 0: this pool, or so many rows in one
     call, it does not take."""
