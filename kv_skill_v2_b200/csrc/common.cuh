@@ -286,6 +286,12 @@ __device__ __forceinline__ uint32_t pack2(float x, float y, float& rx, float& ry
   return (uint32_t)ux | ((uint32_t)uy << 16);
 }
 
+// A group of four warps gives registers up, or waits for as many as others of its CTA have given up.
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+
 __device__ __forceinline__ void named_bar_sync(int id, int nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }

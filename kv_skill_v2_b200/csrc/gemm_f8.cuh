@@ -15,7 +15,8 @@
 // every output of their row.
 #pragma once
 
-#include "gemm_f16x3.cuh"
+#include "project.cuh"
+#include "read_shared.cuh"
 
 namespace xencb {
 
@@ -24,7 +25,7 @@ constexpr int F8_BK = 128;   // columns of a block: one scale factor a row, one 
 constexpr int F8_THREADS = 32 * 6;
 __host__ __device__ constexpr int f8_stage(int bn) { return (F8_BM + bn) * F8_BK; }
 __host__ __device__ constexpr int f8_stages(int bn) { return bn == 64 ? 8 : bn == 128 ? 6 : 4; }
-__host__ __device__ constexpr size_t f8_smem(int bn) { return 1024 + (size_t)f8_stages(bn) * f8_stage(bn) + 256; }
+__host__ __device__ constexpr size_t f8_smem(int bn) { return 1024 + (size_t)f8_stages(bn) * f8_stage(bn) + 1024; }
 // columns of tensor memory: BN of the accumulator, then per word of four blocks 4 of W's factors and BN / 32 of X's
 __host__ __device__ constexpr int f8_word_cols(int bn) { return 4 + bn / 32; }
 __host__ __device__ constexpr int f8_max_words(int bn) { return (512 - bn) / f8_word_cols(bn); }
@@ -33,24 +34,14 @@ __host__ __device__ constexpr int f8_max_words(int bn) { return (512 - bn) / f8_
 __device__ __forceinline__ float f8_exp2i(int e) { return e > -127 ? __int_as_float((e + 127) << 23) : __int_as_float(1 << 22); }
 
 // ------------------------------------------------------------------------------------------------ to 8 bits
-// One warp per (row, block): lane l holds columns 4 l .. 4 l + 3. x8 rows are kp = 128 ceil(K / 128) bytes, zeros behind
-// column K; scale[row * stride + b] = e + 127.
+// 8 values of a row from column k on (zeros behind column K); vec: 16-byte aligned rows of a multiple of 8 columns.
 template <typename T>
-__device__ __forceinline__ void f8_load4(const T* __restrict__ row, int k, int K, bool vec, float* v) {
-  if (vec && k + 4 <= K) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 a = *reinterpret_cast<const float4*>(row + k);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    } else {
-      const uint2 u = *reinterpret_cast<const uint2*>(row + k);
-      T t[4];
-      memcpy(t, &u, 8);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = to_f32(t[i]);
-    }
+__device__ __forceinline__ void f8_load8(const T* __restrict__ row, int k, int K, bool vec, float* v) {
+  if (vec && k < K) {
+    load8_f32<T>(row + k, v);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = k + i < K ? to_f32(row[k + i]) : 0.f;
+    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? to_f32(row[k + i]) : 0.f;
   }
 }
 
@@ -74,29 +65,77 @@ __device__ __forceinline__ uint32_t f8_pack4(const float* v, float s) {
   return u;
 }
 
-constexpr int F8Q_WARPS = 8;
+// What the projection takes of a row besides its 8-bit form (project_in): 1/rms and the gate.
+struct F8RowStats {
+  int rms;
+  float eps;
+  const float* gate_w;  // [K] or null
+  float gate_b;
+  const float* gate_b_dev;
+  float* rstd;          // [M]; null: no statistics
+  float* gate;          // [M] or null
+};
+
+// One CTA per row, 16 threads a block of 128 columns (8 values each, F8Q_UNROLL blocks' loads in flight). x8 rows are
+// kp = 128 ceil(K / 128) bytes, zeros behind column K; scale[row * stride + b] = e + 127.
+constexpr int F8Q_THREADS = 256;
+constexpr int F8Q_UNROLL = 4;
 
 template <typename T>
-__global__ void __launch_bounds__(32 * F8Q_WARPS) quant_f8_kernel(const T* __restrict__ x, int64_t M, int K, int vec,
-                                                                  uint8_t* __restrict__ x8,
-                                                                  uint8_t* __restrict__ scale, int stride) {
+__global__ void __launch_bounds__(F8Q_THREADS) quant_f8_kernel(const T* __restrict__ x, int K, int vec,
+                                                               uint8_t* __restrict__ x8, uint8_t* __restrict__ scale,
+                                                               int stride, const F8RowStats st) {
+  __shared__ float2 red[32];
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int nb = (K + F8_BK - 1) / F8_BK;
-  const int64_t n = M * nb, step = (int64_t)gridDim.x * F8Q_WARPS;
-  for (int64_t i = (int64_t)blockIdx.x * F8Q_WARPS + (threadIdx.x >> 5); i < n; i += step) {
-    const int64_t m = i / nb;
-    const int b = (int)(i - m * nb);
-    float v[4];
-    f8_load4<T>(x + m * K, b * F8_BK + lane * 4, K, vec, v);
-    float mx = 0.f;
+  const int64_t m = blockIdx.x;
+  const T* row = x + m * K;
+  const int kp = (K + F8_BK - 1) / F8_BK * F8_BK;
+  float ss = 0.f, gd = 0.f;
+  for (int k0 = 0; k0 < kp; k0 += F8Q_THREADS * 8 * F8Q_UNROLL) {
+    float v[F8Q_UNROLL][8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) mx = fmaxf(mx, isfinite(v[j]) ? fabsf(v[j]) : 0.f);
-    const int e = f8_exponent(warp_max(mx));
-    const uint32_t u = f8_pack4(v, f8_exp2i(-e));
-    reinterpret_cast<uint32_t*>(x8 + (m * nb + b) * F8_BK)[lane] = u;
-    if (lane == 0) scale[m * stride + b] = (uint8_t)(e + 127);
+    for (int u = 0; u < F8Q_UNROLL; ++u) {
+      const int k = k0 + (u * F8Q_THREADS + (int)threadIdx.x) * 8;
+      if (k < kp) f8_load8<T>(row, k, K, vec, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < F8Q_UNROLL; ++u) {
+      const int k = k0 + (u * F8Q_THREADS + (int)threadIdx.x) * 8;
+      if (k0 + u * F8Q_THREADS * 8 >= kp) break;
+      float mx = 0.f;
+      if (k < kp) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) mx = fmaxf(mx, isfinite(v[u][j]) ? fabsf(v[u][j]) : 0.f);
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      if (k >= kp) continue;
+      const int e = f8_exponent(mx);
+      const float s = f8_exp2i(-e);
+      uint2 p;
+      p.x = f8_pack4(v[u], s);
+      p.y = f8_pack4(v[u] + 4, s);
+      *reinterpret_cast<uint2*>(x8 + m * kp + k) = p;
+      if ((threadIdx.x & 15) == 0) scale[m * stride + k / F8_BK] = (uint8_t)(e + 127);
+      if (st.rstd) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          ss = fmaf(v[u][j], v[u][j], ss);
+          if (st.gate_w && k + j < K) gd = fmaf(v[u][j], __ldg(st.gate_w + k + j), gd);
+        }
+      }
+    }
+  }
+  if (!st.rstd) return;
+  const float2 t = block_sum2(ss, gd, red);
+  if (threadIdx.x == 0) {
+    const float rstd = st.rms ? rsqrtf(t.x / (float)K + st.eps) : 1.f;
+    st.rstd[m] = rstd;
+    if (st.gate) {
+      const float gb = st.gate_b_dev ? __ldg(st.gate_b_dev) : st.gate_b;
+      st.gate[m] = 1.f / (1.f + expf(-(t.y * rstd + gb)));
+    }
   }
 }
 
@@ -125,8 +164,9 @@ __device__ __forceinline__ void tc_st1(uint32_t taddr, uint32_t v) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(v) : "memory");
 }
 
-// Scale bytes of blocks 4 w .. 4 w + 3 of a row (1 behind the last).
-__device__ __forceinline__ uint32_t f8_scale_word(const uint8_t* __restrict__ s, int nb, int w) {
+// Scale bytes of blocks 4 w .. 4 w + 3 of a row (1 behind the last); words: the row is a whole number of aligned words.
+__device__ __forceinline__ uint32_t f8_scale_word(const uint8_t* __restrict__ s, int nb, int w, bool words) {
+  if (words) return __ldg(reinterpret_cast<const uint32_t*>(s) + w);
   uint32_t u = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) u |= (w * 4 + i < nb ? (uint32_t)s[w * 4 + i] : 127u) << (8 * i);
@@ -137,8 +177,9 @@ struct F8Args {
   int64_t M;
   int N, nb, bps;  // blocks of K, blocks per split
   const uint8_t* sw;  // [N, nb]
-  const uint8_t* sx;  // [M, sx_stride]
+  const uint8_t* sx;  // [M, sx_stride], rows of aligned words
   int sx_stride;
+  int sw_words;       // W's rows too
   float* part;
   int* row_done;
 };
@@ -153,8 +194,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_f8_kernel(const __grid_con
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE);
   uint64_t* sfree = full + STAGES;
   uint64_t* done = sfree + STAGES;
-  uint64_t* sf_ready = done + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sf_ready + 1);
+  uint64_t* sf_ready = done + 1;  // one per word of scale factors
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sf_ready + f8_max_words(BN));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -171,7 +212,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_f8_kernel(const __grid_con
       mbar_init(&sfree[i], 1);
     }
     mbar_init(done, 1);
-    mbar_init(sf_ready, 4);
+    for (int i = 0; i < f8_max_words(BN); ++i) mbar_init(&sf_ready[i], 4);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -222,11 +263,15 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_f8_kernel(const __grid_con
           mbar_wait_bounded(&full[kb % STAGES], (kb / STAGES) & 1);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      bool ok = nkb > 0 && mbar_wait_spin(sf_ready, 0);
-      tc_fence_after();
+    if (elect_one()) {
+      bool ok = nkb > 0;
+      int ready = -1;
       for (int kb = 0; kb < nkb && ok; ++kb) {
         const int s = kb % STAGES;
+        if ((b0 + kb) / 4 - w0 != ready) {
+          ready = (b0 + kb) / 4 - w0;
+          if (!(ok = mbar_wait_spin(&sf_ready[ready], 0))) break;
+        }
         if (!mbar_wait_spin(&full[s], (kb / STAGES) & 1) || *abort_flag) { ok = false; break; }
         tc_fence_after();
         const uint32_t sb = smem_u32(smem + s * STAGE);
@@ -242,6 +287,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_f8_kernel(const __grid_con
       if (!ok) *abort_flag = 1;
       tc_commit(done);
     }
+    __syncwarp();
   } else {
     const int q = warp & 3;  // TMEM lane quarter of this warp
     const uint32_t tl = taddr + ((uint32_t)(q * 32) << 16);
@@ -252,20 +298,21 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_f8_kernel(const __grid_con
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int n = n0 + j * 32 + lane;
-        u[j] = n < a.N ? f8_scale_word(a.sw + (int64_t)n * a.nb, a.nb, w0 + w) : 0x7f7f7f7fu;
+        u[j] = n < a.N ? f8_scale_word(a.sw + (int64_t)n * a.nb, a.nb, w0 + w, a.sw_words) : 0x7f7f7f7fu;
       }
 #pragma unroll
       for (int j = 0; j < BN / 32; ++j) {
         const int64_t m = m0 + j * 32 + lane;
-        u[4 + j] = m < a.M ? f8_scale_word(a.sx + m * a.sx_stride, a.nb, w0 + w) : 0x7f7f7f7fu;
+        u[4 + j] = m < a.M ? f8_scale_word(a.sx + m * a.sx_stride, a.nb, w0 + w, true) : 0x7f7f7f7fu;
       }
 #pragma unroll
       for (int j = 0; j < f8_word_cols(BN); ++j) tc_st1(tl + BN + w * f8_word_cols(BN) + j, u[j]);
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sf_ready[w]);
+      __syncwarp();
     }
-    tc_wait_st();
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(sf_ready);
     const int n = n0 + q * 32 + lane;
     float* out = a.part + (int64_t)blockIdx.z * a.M * a.N;
     const int rows = (int)min((int64_t)BN, a.M - m0);
@@ -286,6 +333,313 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_f8_kernel(const __grid_con
     __syncwarp();
     tc_dealloc(taddr, 512);
   }
+}
+
+// ------------------------------------------------------------------------------------------------ many rows
+// The same product with the rows of X as the 128-row operand and 256 output features as N, for calls that fill the device
+// with such tiles: a thread of the epilogue holds 128 outputs of one row, so the projection's elementwise end is done
+// where the product is and no partials are written. Persistent: 8 epilogue warps take the accumulator into registers and
+// give it back before they store, so that the next tile's products run meanwhile; they also bring the next tile's scale
+// factors (two sets of them in tensor memory).
+//   project_in   q = y * rstd + b; the row's sum of squares by pieces of 128 columns, for f8_norm_kernel
+//   project_out  delta = scale * gate * (y + b) * mask in h's type, h + delta; sums of squares of delta and h for the mag term
+constexpr int FR_BM = 128, FR_BN = 256, FR_STAGES = 4;
+constexpr int FR_STAGE = (FR_BM + FR_BN) * F8_BK;
+constexpr int FR_WORD_COLS = FR_BM / 32 + FR_BN / 32;
+constexpr int FR_MAX_WORDS = (512 - FR_BN) / 2 / FR_WORD_COLS;  // two sets
+constexpr int FR_EPI = 8;
+constexpr int FR_THREADS = 32 * (4 + FR_EPI);
+constexpr size_t FR_SMEM = 1024 + (size_t)FR_STAGES * FR_STAGE + 256;
+constexpr int FR_REGS_LOW = 88, FR_REGS_HIGH = 208;
+constexpr int FR_REGS = 4 * 32 * FR_REGS_LOW + 32 * FR_EPI * FR_REGS_HIGH;
+
+struct F8RowsArgs {
+  int64_t M;
+  int N, nb, tiles_n;
+  int64_t tiles;
+  const uint8_t* sw;
+  int sw_words;
+  const uint8_t* sx;
+  int sx_stride;
+  const float* mul;   // [M]: 1/rms, or the gate; null: 1
+  const float* bias;  // [N] or null
+  float scale;        // project_out
+  const float* log_scale_dev;
+  const float* pos_mask;
+  const void* h;      // [M, N] for out2
+  void* out;          // q, or delta (or null)
+  void* out2;         // h + delta, or null
+  float2* sums;       // [M, 2 tiles_n]: sums of squares of q, or of (delta, h); null: none
+  int vec;            // 32-byte stores: N and the bases allow them
+};
+
+// 32 bytes of a thread
+__device__ __forceinline__ void st_global_32(void* p, const uint32_t* u) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]),
+               "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+               : "memory");
+}
+__device__ __forceinline__ void ld_global_32(const void* p, uint32_t* u) {
+  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
+               : "l"(p));
+}
+
+template <typename TO, bool OUT>
+__global__ void __launch_bounds__(FR_THREADS, 1) gemm_f8_rows_kernel(const __grid_constant__ CUtensorMap map_x,
+                                                                     const __grid_constant__ CUtensorMap map_w,
+                                                                     const F8RowsArgs a) {
+  extern __shared__ unsigned char fr_smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(fr_smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + FR_STAGES * FR_STAGE);
+  uint64_t* empty = full + FR_STAGES;
+  uint64_t* acc_full = empty + FR_STAGES;
+  uint64_t* acc_empty = acc_full + 1;
+  uint64_t* sf_full = acc_empty + 1;  // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sf_full + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int words = (a.nb + 3) / 4;
+
+  if (threadIdx.x == 0) {
+    prefetch_tensormap(&map_x);
+    prefetch_tensormap(&map_w);
+    for (int i = 0; i < FR_STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, FR_EPI);
+    mbar_init(&sf_full[0], FR_EPI);
+    mbar_init(&sf_full[1], FR_EPI);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tc_alloc(tmem_slot, 512);
+    tc_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t taddr = *tmem_slot;
+  pdl_wait();
+  pdl_trigger();
+
+  if (warp < 4) {
+    regs_dec<FR_REGS_LOW>();
+    if (warp == 0) {
+      if (elect_one()) {
+        const uint64_t keep = policy_evict_last();
+        RsRing ring{0, 0};
+        uint32_t used = 0;
+        bool ok = true;
+        for (int64_t t = blockIdx.x; t < a.tiles && ok; t += gridDim.x) {
+          const int m0 = (int)(t / a.tiles_n) * FR_BM, n0 = (int)(t % a.tiles_n) * FR_BN;
+          for (int kb = 0; kb < a.nb; ++kb) {
+            if (used >= FR_STAGES && !(ok = mbar_wait_spin(&empty[ring.st], ring.phase ^ 1))) break;
+            unsigned char* st = smem + ring.st * FR_STAGE;
+            mbar_arrive_expect_tx(&full[ring.st], FR_STAGE);
+            tma_load_2d(st, &map_x, kb * F8_BK, m0, &full[ring.st]);
+            tma_load_2d_hint(st + FR_BM * F8_BK, &map_w, kb * F8_BK, n0, &full[ring.st], keep);
+            ring.next(FR_STAGES);
+            ++used;
+          }
+        }
+        if (!ok) {  // the copies in flight end before the CTA's shared memory goes away
+          *abort_flag = 1;
+          for (uint32_t i = min(used, (uint32_t)FR_STAGES); i > 0; --i) {
+            ring.back(FR_STAGES);
+            mbar_wait_bounded(&full[ring.st], ring.phase);
+          }
+        }
+      }
+      __syncwarp();
+    } else if (warp == 1) {
+      if (elect_one()) {
+        RsRing ring{0, 0};
+        bool ok = true;
+        uint32_t i = 0;
+        for (int64_t t = blockIdx.x; t < a.tiles && ok; t += gridDim.x, ++i) {
+          if (!(ok = mbar_wait_spin(&sf_full[i & 1], (i >> 1) & 1))) break;
+          if (i > 0 && !(ok = mbar_wait_spin(acc_empty, (i - 1) & 1))) break;
+          tc_fence_after();
+          const uint32_t sf = taddr + FR_BN + (i & 1) * (FR_MAX_WORDS * FR_WORD_COLS);
+          for (int kb = 0; kb < a.nb; ++kb) {
+            if (!(ok = mbar_wait_spin(&full[ring.st], ring.phase))) break;
+            tc_fence_after();
+            const uint32_t sb = smem_u32(smem + ring.st * FR_STAGE);
+            const uint32_t sa = sf + (kb >> 2) * FR_WORD_COLS;
+            const uint32_t idesc = f8_idesc(FR_BN, 0) | ((uint32_t)(kb & 3) << 4) | ((uint32_t)(kb & 3) << 29);
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+              tc_mma_mx8(taddr, umma_desc_k_sw128(sb + ks * 32), umma_desc_k_sw128(sb + FR_BM * F8_BK + ks * 32), idesc,
+                         sa, sa + FR_BM / 32, kb > 0 || ks > 0);
+            tc_commit(&empty[ring.st]);
+            ring.next(FR_STAGES);
+          }
+          if (ok) tc_commit(acc_full);
+        }
+        if (!ok) *abort_flag = 1;
+      }
+      __syncwarp();
+    }
+  } else {
+    regs_inc<FR_REGS_HIGH>();
+    const int q = warp & 3, half = (warp - 4) >> 2;
+    const uint32_t tl = taddr + ((uint32_t)(q * 32) << 16);
+    auto done = [&](bool arrived) {
+      if (!arrived) *abort_flag = 1;
+      __syncwarp();
+    };
+    // the scale words of tile t: row 32 j + lane in column j, in every lane quarter; the two warps of a quarter take turns
+    auto scales = [&](int64_t t, uint32_t i) {
+      const int64_t m0 = t / a.tiles_n * FR_BM;
+      const int n0 = (int)(t % a.tiles_n) * FR_BN;
+      const uint32_t at = tl + FR_BN + (i & 1) * (FR_MAX_WORDS * FR_WORD_COLS);
+      for (int w = half; w < words; w += 2) {
+        uint32_t u[FR_WORD_COLS];
+#pragma unroll
+        for (int j = 0; j < FR_BM / 32; ++j) {
+          const int64_t m = m0 + j * 32 + lane;
+          u[j] = m < a.M ? f8_scale_word(a.sx + m * a.sx_stride, a.nb, w, true) : 0x7f7f7f7fu;
+        }
+#pragma unroll
+        for (int j = 0; j < FR_BN / 32; ++j) {
+          const int n = n0 + j * 32 + lane;
+          u[FR_BM / 32 + j] = n < a.N ? f8_scale_word(a.sw + (int64_t)n * a.nb, a.nb, w, a.sw_words) : 0x7f7f7f7fu;
+        }
+#pragma unroll
+        for (int j = 0; j < FR_WORD_COLS; ++j) tc_st1(at + w * FR_WORD_COLS + j, u[j]);
+      }
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sf_full[i & 1]);
+      __syncwarp();
+    };
+    if (blockIdx.x < a.tiles) scales(blockIdx.x, 0);
+    const float ls = a.log_scale_dev ? expf(__ldg(a.log_scale_dev)) : 1.f;
+    uint32_t i = 0;
+    for (int64_t t = blockIdx.x; t < a.tiles; t += gridDim.x, ++i) {
+      // (the products of the tile before, which used this set, are done: its accumulator was waited for)
+      if (t + gridDim.x < a.tiles) scales(t + gridDim.x, i + 1);
+      const int64_t m = t / a.tiles_n * FR_BM + q * 32 + lane;
+      const int n0 = (int)(t % a.tiles_n) * FR_BN + half * 128;
+      const bool in = m < a.M;
+      float mul = in && a.mul ? a.mul[m] : 1.f;
+      if (OUT) mul *= a.scale * ls;
+      const float pm = OUT && a.pos_mask && in ? a.pos_mask[m] : 1.f;
+      done(*abort_flag || mbar_wait_spin(acc_full, i & 1));
+      tc_fence_after();
+      float v[128];
+#pragma unroll
+      for (int g = 0; g < 128; g += 32) tc_ld32(tl + half * 128 + g, v + g);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty);
+      __syncwarp();
+      if (*abort_flag) {
+#pragma unroll
+        for (int g = 0; g < 128; ++g) v[g] = 0.f;
+      }
+      float s0 = 0.f, s1 = 0.f;
+      if (in) {
+        TO* o = a.out ? static_cast<TO*>(a.out) + m * a.N + n0 : nullptr;
+        TO* o2 = OUT && a.out2 ? static_cast<TO*>(a.out2) + m * a.N + n0 : nullptr;
+        const TO* h = OUT && (a.out2 || a.sums) ? static_cast<const TO*>(a.h) + m * a.N + n0 : nullptr;
+        constexpr int PER = 32 / sizeof(TO);  // values of a 32-byte store
+#pragma unroll
+        for (int g = 0; g < 128; g += PER) {
+          alignas(32) TO x[PER], hx[PER];
+          const bool vec = a.vec && n0 + g + PER <= a.N;
+          if (OUT && h) {
+            if (vec) {
+              ld_global_32(h + g, reinterpret_cast<uint32_t*>(hx));
+            } else {
+#pragma unroll
+              for (int e = 0; e < PER; ++e) hx[e] = n0 + g + e < a.N ? h[g + e] : from_f32<TO>(0.f);
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < PER; ++e) {
+            const float b = a.bias && n0 + g + e < a.N ? __ldg(a.bias + n0 + g + e) : 0.f;
+            float y = OUT ? mul * (v[g + e] + b) : v[g + e] * mul + b;
+            if (OUT && a.pos_mask) y *= pm;
+            x[e] = from_f32<TO>(y);
+            if (n0 + g + e < a.N) {
+              const float r = to_f32(x[e]);
+              s0 = fmaf(r, r, s0);
+              if (OUT && h) {
+                const float hv = to_f32(hx[e]);
+                s1 = fmaf(hv, hv, s1);
+              }
+            }
+          }
+          if (o) {
+            if (vec) {
+              st_global_32(o + g, reinterpret_cast<const uint32_t*>(x));
+            } else {
+#pragma unroll
+              for (int e = 0; e < PER; ++e)
+                if (n0 + g + e < a.N) o[g + e] = x[e];
+            }
+          }
+          if (OUT && o2) {
+#pragma unroll
+            for (int e = 0; e < PER; ++e) hx[e] = from_f32<TO>(to_f32(hx[e]) + to_f32(x[e]));
+            if (vec) {
+              st_global_32(o2 + g, reinterpret_cast<const uint32_t*>(hx));
+            } else {
+#pragma unroll
+              for (int e = 0; e < PER; ++e)
+                if (n0 + g + e < a.N) o2[g + e] = hx[e];
+            }
+          }
+        }
+        if (a.sums) a.sums[m * 2 * a.tiles_n + (t % a.tiles_n) * 2 + half] = make_float2(s0, s1);
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tc_dealloc(taddr, 512);
+}
+
+// q /= ||q|| + 1e-6, one CTA per row.
+__global__ void __launch_bounds__(256) f8_norm_kernel(float* __restrict__ q, int N, const float2* __restrict__ sums,
+                                                      int n_sums) {
+  pdl_trigger();
+  pdl_wait();
+  const int64_t m = blockIdx.x;
+  float t = 0.f;
+  for (int i = 0; i < n_sums; ++i) t += sums[m * n_sums + i].x;
+  const float den = sqrtf(t) + 1e-6f;
+  float4* row = reinterpret_cast<float4*>(q + m * N);
+#pragma unroll 4
+  for (int i = threadIdx.x; i < N / 4; i += 256) {
+    float4 v = row[i];
+    v.x /= den; v.y /= den; v.z /= den; v.w /= den;
+    row[i] = v;
+  }
+}
+
+// The mag term ||delta|| / (||h|| + 1e-6) of every row.
+__global__ void __launch_bounds__(256) f8_rel_kernel(int64_t M, const float2* __restrict__ sums, int n_sums,
+                                                     float* __restrict__ rel) {
+  pdl_trigger();
+  pdl_wait();
+  const int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (m >= M) return;
+  float d = 0.f, h = 0.f;
+  for (int i = 0; i < n_sums; ++i) {
+    const float2 t = sums[m * n_sums + i];
+    d += t.x;
+    h += t.y;
+  }
+  rel[m] = sqrtf(d) / (sqrtf(h) + 1e-6f);
 }
 
 }  // namespace xencb

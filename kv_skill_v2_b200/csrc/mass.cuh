@@ -251,11 +251,6 @@ __device__ __forceinline__ void ms_copies_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-template <int N>
-__device__ __forceinline__ void ms_regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void ms_regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-
 struct MsSmem {
   unsigned char* stages;
   float* stat;   // [2][2 cs][128][2]: by the parity of the tile, maximum and sum of each pair's half of a CTA's slots
@@ -324,7 +319,7 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
 
   // The softmax keeps 128 sums a thread: the other warps give registers up (their sum stays below the launch's).
   if (warp < 4) {
-    ms_regs_dec<MS_REGS_LOW>();
+    regs_dec<MS_REGS_LOW>();
     if (warp == 0) {
       // --------------------------------------------------------------------------------------------- slots
       if (elect_one()) {
@@ -436,7 +431,7 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
     }
   } else {
     // --------------------------------------------------------------------------------------------- softmax
-    ms_regs_inc<MS_REGS_HIGH>();
+    regs_inc<MS_REGS_HIGH>();
     const int quarter = warp & 3, half = (warp - 2 - MS_PRODUCERS) >> 2;
     const int r = quarter * 32 + lane;               // pair of the tile = TMEM lane
     const uint32_t tl = taddr + ((uint32_t)(quarter * 32) << 16) + half * 128;

@@ -344,16 +344,20 @@ int launch_gemm(const void* X, int64_t M, int K, const float* W, int N, int sms,
 struct Weight8 {
   const void* w;
   const uint8_t* scale;
+  int words(int nb) const { return nb % 4 == 0 && reinterpret_cast<uintptr_t>(scale) % 4 == 0; }
 };
 
 struct F8Plan {
   int bn, nb, bps, sx_stride;
+  bool rows;  // gemm_f8_rows_kernel, where the call's arguments allow it
   GemmPlan gp;
-  size_t x8_bytes, sx_bytes, total;
+  size_t out_bytes, x8_bytes, sx_bytes, rstd_bytes, total;
 };
 
-// BN = 64 and 128 where all rows fit one tile (the split CTAs stream the weights); more rows take 256 at a time, so that a
-// weight tile is fetched a quarter as often.
+// Calls with tiles of 128 rows and 256 output features for half of the device take gemm_f8_rows_kernel (2048 rows, 5120 ->
+// 2048: %ROWS%); it keeps two tiles' scale factors in tensor memory, blocks of up to 40. The others split K: BN = 64
+// and 128 where all rows fit one tile (the CTAs stream the weights), 256 where they do not, so that a weight tile is
+// fetched a quarter as often.
 F8Plan plan_f8(int64_t M, int N, int K, int sms) {
   F8Plan p;
   p.bn = M <= 64 ? 64 : M <= 128 ? 128 : 256;
@@ -367,21 +371,33 @@ F8Plan plan_f8(int64_t M, int N, int K, int sms) {
   p.gp.splits = (p.nb + p.bps - 1) / p.bps;
   p.gp.part_bytes = align_up((size_t)p.gp.splits * (size_t)M * (size_t)N * sizeof(float), 256);
   p.sx_stride = (p.nb + 3) / 4 * 4;
+  const int64_t tiles_n = (N + FR_BN - 1) / FR_BN;
+  p.rows = (p.nb + 3) / 4 <= FR_MAX_WORDS && 2 * tiles_n * ((M + FR_BM - 1) / FR_BM) >= sms;
+  p.out_bytes = std::max(p.gp.part_bytes, p.rows ? align_up((size_t)M * 2 * tiles_n * sizeof(float2), 256) : 0);
   p.x8_bytes = align_up((size_t)M * p.nb * F8_BK, 256);
   p.sx_bytes = align_up((size_t)M * p.sx_stride, 256);
-  p.total = p.gp.part_bytes + p.x8_bytes + p.sx_bytes;
+  p.rstd_bytes = align_up((size_t)M * sizeof(float), 256);
+  p.total = p.out_bytes + p.x8_bytes + p.sx_bytes + p.rstd_bytes;
   return p;
 }
 
 template <typename T>
-int launch_quant_f8(const void* x, int64_t M, int K, void* x8, uint8_t* scale, int stride, int sms, cudaStream_t st) {
-  const int64_t n = M * ((K + F8_BK - 1) / F8_BK);
-  const int vec = K % 4 == 0 && aligned(x, 4 * sizeof(T));
-  const unsigned grid = (unsigned)std::min<int64_t>((n + F8Q_WARPS - 1) / F8Q_WARPS, 16 * (int64_t)sms);
-  launch_pdl(quant_f8_kernel<T>, dim3(grid), dim3(32 * F8Q_WARPS), 0, st, static_cast<const T*>(x), M, K, vec,
-             static_cast<uint8_t*>(x8), scale, stride);
+int launch_quant_f8(const void* x, int64_t M, int K, void* x8, uint8_t* scale, int stride, const F8RowStats& stats,
+                    cudaStream_t st) {
+  const int vec = K % 8 == 0 && aligned(x, 16);
+  launch_pdl(quant_f8_kernel<T>, dim3((unsigned)M), dim3(F8Q_THREADS), 0, st, static_cast<const T*>(x), K, vec,
+             static_cast<uint8_t*>(x8), scale, stride, stats);
   XENCB_CHECK_LAUNCH("quant_f8 launch");
   return XENCB_OK;
+}
+
+int launch_quant_f8(const void* x, int dtype, int64_t M, int K, void* x8, uint8_t* scale, int stride,
+                    const F8RowStats& stats, cudaStream_t st) {
+  switch (dtype) {
+    case XENCB_F32: return launch_quant_f8<float>(x, M, K, x8, scale, stride, stats, st);
+    case XENCB_F16: return launch_quant_f8<__half>(x, M, K, x8, scale, stride, stats, st);
+    default: return launch_quant_f8<__nv_bfloat16>(x, M, K, x8, scale, stride, stats, st);
+  }
 }
 
 template <int BN>
@@ -395,23 +411,50 @@ int run_gemm_f8(const CUtensorMap& mw, const CUtensorMap& mx, const F8Args& a, i
   return XENCB_OK;
 }
 
-// part = split partials of X @ W^T with both in 8 bits. ws: p.total bytes (the partials first).
-template <typename TX>
-int launch_gemm_f8(const void* X, int64_t M, int K, const Weight8& w, int N, int sms, const F8Plan& p, char* ws,
+// part (at the front of ws, p.total bytes) = split partials of X @ W^T with both in 8 bits.
+int launch_gemm_f8(const void* X, int dtype, int64_t M, int K, const Weight8& w, int N, const F8Plan& p, char* ws,
                    int* row_done, cudaStream_t st) {
-  uint8_t* x8 = reinterpret_cast<uint8_t*>(ws + p.gp.part_bytes);
+  uint8_t* x8 = reinterpret_cast<uint8_t*>(ws + p.out_bytes);
   uint8_t* sx = x8 + p.x8_bytes;
-  int rc = launch_quant_f8<TX>(X, M, K, x8, sx, p.sx_stride, sms, st);
+  int rc = launch_quant_f8(X, dtype, M, K, x8, sx, p.sx_stride, F8RowStats{}, st);
   if (rc) return rc;
   const uint64_t kp = (uint64_t)p.nb * F8_BK;
   CUtensorMap mw, mx;
   rc = tensor_map_2d(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w.w, kp, (uint64_t)N, kp, F8_BK, F8_BM);
   if (!rc) rc = tensor_map_2d(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x8, kp, (uint64_t)M, kp, F8_BK, (uint32_t)p.bn);
   if (rc) return rc;
-  const F8Args a{M, N, p.nb, p.bps, w.scale, sx, p.sx_stride, reinterpret_cast<float*>(ws), row_done};
+  const F8Args a{M, N, p.nb, p.bps, w.scale, sx, p.sx_stride, w.words(p.nb), reinterpret_cast<float*>(ws), row_done};
   if (p.bn == 64) return run_gemm_f8<64>(mw, mx, a, p.gp.splits, st);
   if (p.bn == 128) return run_gemm_f8<128>(mw, mx, a, p.gp.splits, st);
   return run_gemm_f8<256>(mw, mx, a, p.gp.splits, st);
+}
+
+// X (in 8 bits already, behind p.out_bytes of ws) times W with the projection's end in the product's epilogue. a: mul,
+// bias, scale, log_scale_dev, pos_mask, h, out, out2 and sums are set.
+template <typename TO, bool OUT>
+int launch_gemm_f8_rows(int64_t M, const Weight8& w, int N, int sms, const F8Plan& p, char* ws, F8RowsArgs a,
+                        cudaStream_t st) {
+  uint8_t* x8 = reinterpret_cast<uint8_t*>(ws + p.out_bytes);
+  const uint64_t kp = (uint64_t)p.nb * F8_BK;
+  CUtensorMap mw, mx;
+  int rc = tensor_map_2d(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x8, kp, (uint64_t)M, kp, F8_BK, FR_BM);
+  if (!rc) rc = tensor_map_2d(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w.w, kp, (uint64_t)N, kp, F8_BK, FR_BN);
+  if (rc) return rc;
+  auto kern = gemm_f8_rows_kernel<TO, OUT>;
+  if ((rc = ensure_smem(kern, (int)FR_SMEM))) return rc;
+  // the epilogue warps wait for the registers that the others give up: the launch must have as many
+  static const int regs = [&] {
+    cudaFuncAttributes fa;
+    return cudaFuncGetAttributes(&fa, kern) == cudaSuccess ? fa.numRegs * FR_THREADS : 0;
+  }();
+  if (regs < FR_REGS) return fail(XENCB_ENOTSUP, "gemm_f8: built with %d registers a CTA, %d are needed", regs, FR_REGS);
+  a.M = M; a.N = N; a.nb = p.nb; a.tiles_n = (N + FR_BN - 1) / FR_BN;
+  a.tiles = a.tiles_n * ((M + FR_BM - 1) / FR_BM);
+  a.sw = w.scale; a.sw_words = w.words(p.nb); a.sx = x8 + p.x8_bytes; a.sx_stride = p.sx_stride;
+  a.vec = (size_t)N * sizeof(TO) % 32 == 0 && aligned(a.out, 32) && aligned(a.out2, 32) && aligned(a.h, 32);
+  launch_pdl(kern, dim3((unsigned)std::min<int64_t>(sms, a.tiles)), dim3(FR_THREADS), FR_SMEM, st, mx, mw, a);
+  XENCB_CHECK_LAUNCH("gemm_f8_rows launch");
+  return XENCB_OK;
 }
 
 int check_weight8(const char* what, const Weight8& w, int64_t M, int N) {
@@ -1152,13 +1195,26 @@ static int project_in_impl(const void* h, int h_dtype, int64_t n_rows, int d_m, 
     }
     if (rc) return rc;
   }
+  if (w8 && p8.rows && !sel_w) {
+    float* rstd = rstd_out ? rstd_out : reinterpret_cast<float*>(ws + p8.out_bytes + p8.x8_bytes + p8.sx_bytes);
+    uint8_t* x8 = reinterpret_cast<uint8_t*>(ws + p8.out_bytes);
+    const F8RowStats stats{(flags & XENCB_PIN_RMS) ? 1 : 0, rms_eps, gate_w, gate_b, gate_b_dev, rstd,
+                           gate_w ? gate_out : nullptr};
+    rc = launch_quant_f8(h, h_dtype, n_rows, d_m, x8, x8 + p8.x8_bytes, p8.sx_stride, stats, st);
+    if (rc) return rc;
+    F8RowsArgs a{};
+    a.mul = rstd; a.bias = b_in; a.out = q_out;
+    a.sums = (flags & XENCB_PIN_L2) ? reinterpret_cast<float2*>(ws) : nullptr;
+    rc = launch_gemm_f8_rows<float, false>(n_rows, *w8, d_s, di.sms, p8, ws, a, st);
+    if (rc || !a.sums) return rc;
+    launch_pdl(f8_norm_kernel, dim3((unsigned)n_rows), dim3(256), 0, st, q_out, d_s, (const float2*)a.sums,
+               2 * ((d_s + FR_BN - 1) / FR_BN));
+    XENCB_CHECK_LAUNCH("f8_norm launch");
+    return XENCB_OK;
+  }
   if (w8) {
     gp = p8.gp;
-    switch (h_dtype) {
-      case XENCB_F32: rc = launch_gemm_f8<float>(h, n_rows, d_m, *w8, d_s, di.sms, p8, ws, row_done, st); break;
-      case XENCB_F16: rc = launch_gemm_f8<__half>(h, n_rows, d_m, *w8, d_s, di.sms, p8, ws, row_done, st); break;
-      default: rc = launch_gemm_f8<__nv_bfloat16>(h, n_rows, d_m, *w8, d_s, di.sms, p8, ws, row_done, st); break;
-    }
+    rc = launch_gemm_f8(h, h_dtype, n_rows, d_m, *w8, d_s, p8, ws, row_done, st);
   } else switch (h_dtype) {
     case XENCB_F32:
       rc = launch_gemm<float>(h, n_rows, d_m, w_in, d_s, di.sms, part, w_prep ? xbuf : nullptr, row_done, st, &gp,
@@ -1991,9 +2047,27 @@ static int project_out_impl(const float* r, int64_t n_rows, int d_s, const float
     rc = launch_adapt_shrink<float>(r, ad, adapt_dtype, st);
     if (rc) return rc;
   }
+  if (w8 && p8.rows && !sel_w) {
+    uint8_t* x8 = reinterpret_cast<uint8_t*>(ws + p8.out_bytes);
+    rc = launch_quant_f8(r, XENCB_F32, n_rows, d_s, x8, x8 + p8.x8_bytes, p8.sx_stride, F8RowStats{}, st);
+    if (rc) return rc;
+    F8RowsArgs a{};
+    a.mul = gate; a.bias = b_out; a.scale = scale; a.log_scale_dev = log_scale_dev; a.pos_mask = pos_mask; a.h = h;
+    a.out = delta_out; a.out2 = h_out; a.sums = rel_out ? reinterpret_cast<float2*>(ws) : nullptr;
+    switch (h_dtype) {
+      case XENCB_F32: rc = launch_gemm_f8_rows<float, true>(n_rows, *w8, d_m, di.sms, p8, ws, a, st); break;
+      case XENCB_F16: rc = launch_gemm_f8_rows<__half, true>(n_rows, *w8, d_m, di.sms, p8, ws, a, st); break;
+      default: rc = launch_gemm_f8_rows<__nv_bfloat16, true>(n_rows, *w8, d_m, di.sms, p8, ws, a, st); break;
+    }
+    if (rc || !rel_out) return rc;
+    launch_pdl(f8_rel_kernel, dim3((unsigned)((n_rows + 255) / 256)), dim3(256), 0, st, n_rows, (const float2*)a.sums,
+               2 * ((d_m + FR_BN - 1) / FR_BN), rel_out);
+    XENCB_CHECK_LAUNCH("f8_rel launch");
+    return XENCB_OK;
+  }
   if (w8) {
     gp = p8.gp;
-    rc = launch_gemm_f8<float>(r, n_rows, d_s, *w8, d_m, di.sms, p8, ws, nullptr, st);
+    rc = launch_gemm_f8(r, XENCB_F32, n_rows, d_s, *w8, d_m, p8, ws, nullptr, st);
   } else {
     rc = launch_gemm<float>(r, n_rows, d_s, w_out, d_m, di.sms, part, w_prep ? xbuf : nullptr, nullptr, st, &gp, w_prep,
                             adapters ? adapt_min_splits(d_s) : 1, adapters != nullptr);
@@ -2116,14 +2190,9 @@ int xencb_quant8(const void* x, int dtype, int64_t n, int k, void* x8, void* sca
   DevInfo di;
   const int rc = device_info(&di);
   if (rc) return rc;
-  uint8_t* s = static_cast<uint8_t*>(scale);
-  const int nb = (k + F8_BK - 1) / F8_BK;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  switch (dtype) {
-    case XENCB_F32: return launch_quant_f8<float>(x, n, k, x8, s, nb, di.sms, st);
-    case XENCB_F16: return launch_quant_f8<__half>(x, n, k, x8, s, nb, di.sms, st);
-    default: return launch_quant_f8<__nv_bfloat16>(x, n, k, x8, s, nb, di.sms, st);
-  }
+  if (n > INT32_MAX) return fail(XENCB_ENOTSUP, "quant8: too many rows");
+  return launch_quant_f8(x, dtype, n, k, x8, static_cast<uint8_t*>(scale), (k + F8_BK - 1) / F8_BK, F8RowStats{},
+                         static_cast<cudaStream_t>(stream));
 }
 
 size_t xencb_project_in8_workspace(int64_t n_rows, int d_m, int d_s) {

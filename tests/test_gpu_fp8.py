@@ -99,6 +99,7 @@ def test_weights_fp8_not_finite():
     (63, 520, 256, torch.bfloat16), (64, 4096, 2048, torch.float16), (65, 777, 260, torch.float32),
     (127, 384, 516, torch.bfloat16), (128, 1024, 512, torch.float32), (129, 1024, 1024, torch.bfloat16),
     (300, 512, 2048, torch.float32), (513, 2048, 384, torch.float16), (1000, 5120, 640, torch.bfloat16),
+    (2048, 5120, 2048, torch.bfloat16), (1111, 700, 2052, torch.float32), (19000, 130, 132, torch.float16),
     (4, 40000, 8, torch.float32), (200, 12000, 16, torch.bfloat16), (3, 256, 7000, torch.float32)])
 def test_project_in(R, d_in, d_out, dtype):
     h, W = rows(R, d_in, 3, dtype=dtype), rows(d_out, d_in, 4) * d_in ** -0.5
@@ -114,6 +115,11 @@ def test_project_in(R, d_in, d_out, dtype):
     # what does not go through the 8-bit product is what it is with a float32 weight, bit for bit
     _, gate32, rstd32, z32 = ops.project_in(h, W, b, gate_w=gate_w, gate_b=0.3, sel_w=sel_w)
     assert torch.equal(gate, gate32) and torch.equal(rstd, rstd32) and torch.equal(z, z32)
+    # without a selector calls of many rows take 1/rms and the gate in another order of float32 sums
+    q2, gate2, rstd2, _ = ops.project_in(h, w8, b, gate_w=gate_w, gate_b=0.3)
+    assert rel(q2, y / (y.norm(dim=-1, keepdim=True) + 1e-6)) < TOL
+    assert rel(rstd2, rs[:, 0]) < 1e-6
+    assert rel(gate2, torch.sigmoid((hd @ gate_w.double()) * rs[:, 0] + 0.3)) < TOL
     raw = ops.project_in(h, w8, rms=False, l2=False)[0]
     assert rel(raw, values(h) @ values(W).t()) < TOL
 
@@ -121,7 +127,8 @@ def test_project_in(R, d_in, d_out, dtype):
 @pytest.mark.parametrize("R,d_in,d_out,dtype", [
     (1, 2048, 4096, torch.bfloat16), (5, 328, 1000, torch.float32), (64, 2048, 4096, torch.float16), (70, 96, 512, torch.float32),
     (128, 640, 260, torch.bfloat16), (257, 2048, 1024, torch.bfloat16), (700, 1032, 512, torch.float32),
-    (2, 128, 8192, torch.float32)])
+    (2, 128, 8192, torch.float32), (2048, 2048, 4096, torch.bfloat16), (1500, 520, 2052, torch.float16),
+    (10001, 264, 260, torch.float32)])
 def test_project_out(R, d_in, d_out, dtype):
     r, W = rows(R, d_in, 6), rows(d_out, d_in, 7) * d_in ** -0.5
     g = gen(8)
