@@ -45,24 +45,21 @@ __device__ __forceinline__ void f8_load8(const T* __restrict__ row, int k, int K
   }
 }
 
-// The exponent of a block whose largest finite value is mx: mx = m 2^x with m in [1/2, 1), 448 = (7/8) 2^9.
-__device__ __forceinline__ int f8_exponent(float mx) {
-  if (!(mx > 0.f)) return 0;
-  int x;
-  const float m = frexpf(mx, &x);
-  return max(-127, min(127, x - 9 + (m > 0.875f ? 1 : 0)));
+// The exponent of a block whose largest value has the bits mx (finite): mx = m 2^x with m in [1/2, 1), 448 = (7/8) 2^9.
+// Values below 2^-126 have x <= -126: they get the smallest exponent.
+__device__ __forceinline__ int f8_exponent(uint32_t mx) {
+  if (mx == 0u) return 0;
+  return max(-127, min(127, (int)(mx >> 23) - 126 - 9 + ((mx & 0x7fffffu) > 0x600000u ? 1 : 0)));
 }
 
-// Four values as e4m3 bytes (round to nearest even); what is not finite as NaN.
+__device__ __forceinline__ uint32_t f8_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// Four values as e4m3 bytes (round to nearest even).
 __device__ __forceinline__ uint32_t f8_pack4(const float* v, float s) {
   uint16_t lo, hi;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(v[1] * s), "f"(v[0] * s));
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(v[3] * s), "f"(v[2] * s));
-  uint32_t u = (uint32_t)lo | ((uint32_t)hi << 16);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (!isfinite(v[i])) u |= 0x7fu << (8 * i);
-  return u;
+  return (uint32_t)lo | ((uint32_t)hi << 16);
 }
 
 // What the projection takes of a row besides its 8-bit form (project_in): 1/rms and the gate.
@@ -103,19 +100,36 @@ __global__ void __launch_bounds__(F8Q_THREADS) quant_f8_kernel(const T* __restri
     for (int u = 0; u < F8Q_UNROLL; ++u) {
       const int k = k0 + (u * F8Q_THREADS + (int)threadIdx.x) * 8;
       if (k0 + u * F8Q_THREADS * 8 >= kp) break;
-      float mx = 0.f;
+      uint32_t mx = 0u;
       if (k < kp) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) mx = fmaxf(mx, isfinite(v[u][j]) ? fabsf(v[u][j]) : 0.f);
+        for (int j = 0; j < 8; ++j) mx = max(mx, f8_bits(v[u][j]));
       }
+      uint32_t top = mx;
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const bool odd = __any_sync(0xffffffffu, mx >= 0x7f800000u);  // a value of the warp that is not finite
+      if (odd) {  // the largest finite one decides
+        uint32_t fin = 0u;
+        if (k < kp) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) fin = max(fin, f8_bits(v[u][j]) < 0x7f800000u ? f8_bits(v[u][j]) : 0u);
+        }
+        top = fin;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      }
       if (k >= kp) continue;
-      const int e = f8_exponent(mx);
+      const int e = f8_exponent(top);
       const float s = f8_exp2i(-e);
       uint2 p;
       p.x = f8_pack4(v[u], s);
       p.y = f8_pack4(v[u] + 4, s);
+      if (odd) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (f8_bits(v[u][j]) >= 0x7f800000u) (j < 4 ? p.x : p.y) |= 0x7fu << (8 * (j & 3));
+      }
       *reinterpret_cast<uint2*>(x8 + m * kp + k) = p;
       if ((threadIdx.x & 15) == 0) scale[m * stride + k / F8_BK] = (uint8_t)(e + 127);
       if (st.rstd) {
@@ -528,8 +542,7 @@ __global__ void __launch_bounds__(FR_THREADS, 1) gemm_f8_rows_kernel(const __gri
       const int n0 = (int)(t % a.tiles_n) * FR_BN + half * 128;
       const bool in = m < a.M;
       float mul = in && a.mul ? a.mul[m] : 1.f;
-      if (OUT) mul *= a.scale * ls;
-      const float pm = OUT && a.pos_mask && in ? a.pos_mask[m] : 1.f;
+      if (OUT) mul *= a.scale * ls * (a.pos_mask && in ? a.pos_mask[m] : 1.f);
       done(*abort_flag || mbar_wait_spin(acc_full, i & 1));
       tc_fence_after();
       float v[128];
@@ -543,36 +556,47 @@ __global__ void __launch_bounds__(FR_THREADS, 1) gemm_f8_rows_kernel(const __gri
 #pragma unroll
         for (int g = 0; g < 128; ++g) v[g] = 0.f;
       }
-      float s0 = 0.f, s1 = 0.f;
       if (in) {
         TO* o = a.out ? static_cast<TO*>(a.out) + m * a.N + n0 : nullptr;
         TO* o2 = OUT && a.out2 ? static_cast<TO*>(a.out2) + m * a.N + n0 : nullptr;
         const TO* h = OUT && (a.out2 || a.sums) ? static_cast<const TO*>(a.h) + m * a.N + n0 : nullptr;
         constexpr int PER = 32 / sizeof(TO);  // values of a 32-byte store
+        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+        // (one test a group for what a call has: a test for each value took the epilogue from 96 to 172 us, 16384 rows
+        // 2048 -> 4096)
 #pragma unroll
         for (int g = 0; g < 128; g += PER) {
+          if (n0 + g >= a.N) break;
+          const bool whole = n0 + g + PER <= a.N, vec = a.vec && whole;
+          if (a.bias) {
+#pragma unroll
+            for (int e = 0; e < PER; ++e) {
+              const float b = whole || n0 + g + e < a.N ? __ldg(a.bias + n0 + g + e) : 0.f;
+              v[g + e] = OUT ? mul * (v[g + e] + b) : fmaf(v[g + e], mul, b);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < PER; ++e) v[g + e] *= mul;
+          }
           alignas(32) TO x[PER], hx[PER];
-          const bool vec = a.vec && n0 + g + PER <= a.N;
+#pragma unroll
+          for (int e = 0; e < PER; ++e) x[e] = from_f32<TO>(v[g + e]);
           if (OUT && h) {
             if (vec) {
               ld_global_32(h + g, reinterpret_cast<uint32_t*>(hx));
             } else {
 #pragma unroll
-              for (int e = 0; e < PER; ++e) hx[e] = n0 + g + e < a.N ? h[g + e] : from_f32<TO>(0.f);
+              for (int e = 0; e < PER; ++e) hx[e] = whole || n0 + g + e < a.N ? h[g + e] : from_f32<TO>(0.f);
             }
           }
+          if (a.sums) {
 #pragma unroll
-          for (int e = 0; e < PER; ++e) {
-            const float b = a.bias && n0 + g + e < a.N ? __ldg(a.bias + n0 + g + e) : 0.f;
-            float y = OUT ? mul * (v[g + e] + b) : v[g + e] * mul + b;
-            if (OUT && a.pos_mask) y *= pm;
-            x[e] = from_f32<TO>(y);
-            if (n0 + g + e < a.N) {
-              const float r = to_f32(x[e]);
-              s0 = fmaf(r, r, s0);
-              if (OUT && h) {
+            for (int e = 0; e < PER; ++e) {
+              const float r = whole || n0 + g + e < a.N ? to_f32(x[e]) : 0.f;
+              s0[e & 3] = fmaf(r, r, s0[e & 3]);
+              if (OUT) {
                 const float hv = to_f32(hx[e]);
-                s1 = fmaf(hv, hv, s1);
+                s1[e & 3] = fmaf(hv, hv, s1[e & 3]);
               }
             }
           }
@@ -582,7 +606,7 @@ __global__ void __launch_bounds__(FR_THREADS, 1) gemm_f8_rows_kernel(const __gri
             } else {
 #pragma unroll
               for (int e = 0; e < PER; ++e)
-                if (n0 + g + e < a.N) o[g + e] = x[e];
+                if (whole || n0 + g + e < a.N) o[g + e] = x[e];
             }
           }
           if (OUT && o2) {
@@ -593,11 +617,13 @@ __global__ void __launch_bounds__(FR_THREADS, 1) gemm_f8_rows_kernel(const __gri
             } else {
 #pragma unroll
               for (int e = 0; e < PER; ++e)
-                if (n0 + g + e < a.N) o2[g + e] = hx[e];
+                if (whole || n0 + g + e < a.N) o2[g + e] = hx[e];
             }
           }
         }
-        if (a.sums) a.sums[m * 2 * a.tiles_n + (t % a.tiles_n) * 2 + half] = make_float2(s0, s1);
+        if (a.sums) 
+          a.sums[m * 2 * a.tiles_n + (t % a.tiles_n) * 2 + half] =
+              make_float2((s0[0] + s0[1]) + (s0[2] + s0[3]), (s1[0] + s1[1]) + (s1[2] + s1[3]));
       }
     }
   }
@@ -614,15 +640,23 @@ __global__ void __launch_bounds__(256) f8_norm_kernel(float* __restrict__ q, int
   pdl_trigger();
   pdl_wait();
   const int64_t m = blockIdx.x;
-  float t = 0.f;
-  for (int i = 0; i < n_sums; ++i) t += sums[m * n_sums + i].x;
-  const float den = sqrtf(t) + 1e-6f;
+  const int lane = threadIdx.x & 31;
   float4* row = reinterpret_cast<float4*>(q + m * N);
-#pragma unroll 4
-  for (int i = threadIdx.x; i < N / 4; i += 256) {
-    float4 v = row[i];
-    v.x /= den; v.y /= den; v.z /= den; v.w /= den;
-    row[i] = v;
+  constexpr int HELD = 2;
+  float4 v[HELD];
+#pragma unroll
+  for (int h = 0; h < HELD; ++h)
+    if (h * 256 + threadIdx.x < N / 4) v[h] = row[h * 256 + threadIdx.x];
+  float t = 0.f;  // (every warp adds the pieces in the same order)
+  for (int i = lane; i < n_sums; i += 32) t += sums[m * n_sums + i].x;
+  const float den = sqrtf(warp_sum(t)) + 1e-6f;
+#pragma unroll
+  for (int h = 0; h < HELD; ++h)
+    if (h * 256 + threadIdx.x < N / 4)
+      row[h * 256 + threadIdx.x] = make_float4(v[h].x / den, v[h].y / den, v[h].z / den, v[h].w / den);
+  for (int i = HELD * 256 + threadIdx.x; i < N / 4; i += 256) {
+    const float4 w = row[i];
+    row[i] = make_float4(w.x / den, w.y / den, w.z / den, w.w / den);
   }
 }
 

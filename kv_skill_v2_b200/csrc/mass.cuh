@@ -6,9 +6,10 @@
 // the column sums of the weights with which the read (xenc/injector.py:239-245) multiplies the values. The (row, routed
 // chunk) pairs are grouped by page in the order of their rows; a tile is one page with up to 128 of its pairs.
 //
-//   mass_prep    q in 16 bits, a power of two per row (f16's range); CTA 0 counts the pairs of each page and lays out the
-//                tiles
-//   mass_order   a CTA per page lists its pairs in order, so that sums do not depend on the order of atomics
+//   mass_plan    counts the pairs of each page and lays out the tiles (one CTA; more than MS_ONE_CTA pairs are counted by a
+//                grid before). Calls of up to MS_DIRECT pairs do without: every page has room for all of them
+//   mass_rows    a CTA per page lists its pairs in order, so that sums do not depend on the order of atomics; a CTA per row
+//                brings q into 16 bits, a power of two per row (f16's range)
 //   mass_scores  a cluster of ceil(page_rows / 256) CTAs per tile, each with up to 256 of the page's slots:
 //                S[pairs, slots] = Q . K^T on the tensor cores (pairs as the 128-row operand), chunk softmax, column sums
 //   mass_combine a page's tiles added in order, with the prior
@@ -33,21 +34,25 @@ namespace xencb {
 constexpr int MS_M = 128;         // pairs of a tile
 constexpr int MS_N = 256;         // slots of a CTA at most
 constexpr int MS_MAX_CS = 8;      // CTAs per cluster: pages of up to 2048 slots
-constexpr int MS_CHUNK = 2;       // blocks of 64 columns per accumulator
+constexpr int MS_CHUNK = 4;       // blocks of 64 columns per accumulator
 constexpr int MS_ATILE = MS_M * 128;
 constexpr int MS_BTILE = MS_N * 128;
-constexpr int MS_PRODUCERS = 2;   // warps that bring Q
+constexpr int MS_PRODUCERS = 4;   // warps that bring Q
 constexpr int MS_EPI = 8;         // softmax warps: 4 TMEM lane quarters x 2 halves of the slots
-constexpr int MS_THREADS = 32 * (2 + MS_PRODUCERS + MS_EPI);
-constexpr int MS_REGS_LOW = 88, MS_REGS_HIGH = 208;  // registers of a thread of the first four warps, and of the others
-constexpr int MS_REGS = 4 * 32 * MS_REGS_LOW + 32 * MS_EPI * MS_REGS_HIGH;
-static_assert(2 + MS_PRODUCERS == 4, "the softmax warps begin a group of four");
-constexpr int MS_ONE_CTA = 16384;  // pairs that one CTA counts
+constexpr int MS_LOW = 8;         // warps before the softmax: 0 slots, 1 MMA, 4 .. 7 Q
+constexpr int MS_THREADS = 32 * (MS_LOW + MS_EPI);
+constexpr int MS_REGS_LOW = 56, MS_REGS_HIGH = 200;  // registers of a thread of these warps, and of the others
+constexpr int MS_REGS = 32 * (MS_LOW * MS_REGS_LOW + MS_EPI * MS_REGS_HIGH);
+constexpr int MS_FEW = 64;        // pairs of a tile whose hi and lo rows fit one 128-row operand
+constexpr int MS_ONE_CTA = 2048;  // pairs that one CTA counts
+constexpr int MS_DIRECT = 512;    // pairs of a call without a plan
+constexpr int MS_XPITCH = 17;     // 16 columns of the lo rows' sums on their way to the hi rows' lanes
 __host__ __device__ constexpr int ms_stage(int terms) { return terms * MS_ATILE + MS_BTILE; }
 // stages of the ring: what the maxima and sums of cs CTAs (two generations, two halves of the slots each) leave
 __host__ __device__ constexpr int ms_stages(int terms, int cs) { return (cs <= 4 ? 1 : 0) + (terms == 2 ? 2 : 3); }
 __host__ __device__ constexpr size_t ms_smem(int terms, int cs) {
-  return 1024 + (size_t)ms_stages(terms, cs) * ms_stage(terms) + (size_t)cs * 4 * MS_M * 8 + 4 * MS_N * 4 + 256;
+  return 1024 + (size_t)ms_stages(terms, cs) * ms_stage(terms) + (size_t)cs * 4 * MS_M * 8 + 4 * MS_N * 4 +
+         (terms == 2 ? 2 * MS_FEW * MS_XPITCH * 4 : 0) + 256;
 }
 
 struct __align__(16) MassTile {
@@ -59,19 +64,22 @@ struct MassArgs {
   const int32_t* n_valid;  // [n_lib, C]
   const int32_t* idx;      // [R, k]
   const float* wk;         // [R, k]
-  int64_t n_rows, rows_per_lib, n_lib;
-  int k, C, n_pages, page_rows, d_s, n_pairs;
+  int64_t n_rows;
+  int rows_per_lib, k, C, n_pages, page_rows, d_s, n_pairs;
   // plan
   int* cnt;       // [n_pages]: pairs per page
   int* nvmax;     // [n_pages]
   int* start;     // [n_pages]: the page's first place
-  int* tile0;     // [n_pages]: its first tile
+  int* tile0;     // [n_pages]: its first tile of more than MS_FEW pairs
+  int* few;       // [n_pages]: its tile of fewer, -1: none
   int* page;      // [n_pairs]: page of a pair, -1: reads nothing
   int* prow;      // [n_pairs] by place: row of q
   int* pnv;       // [n_pairs] by place: valid slots
   float* pw;      // [n_pairs] by place: weight
   MassTile* tiles;
   int* n_tiles;
+  int direct;     // no plan: page p's pairs from place p * n_pairs on, its j-th tile is tile j * n_pages + p
+  int slots;      // of the list of tiles (those without pairs are skipped)
   // rows
   float* rinv;    // [R]: 1 / (the row's power of two)
   const void* q16;  // [terms, R, d_s]
@@ -84,161 +92,224 @@ struct MassArgs {
   float* mass;
 };
 
-__device__ __forceinline__ void ms_count(const MassArgs& a, int64_t first, int64_t step) {
-  for (int64_t i = first; i < a.n_pairs; i += step) {
-    const int64_t row = i / a.k;
-    const int64_t lib = row / a.rows_per_lib;
-    const int c = a.idx[i];
-    int page = -1;
-    if (c >= 0 && a.wk[i] != 0.f) {
-      if (c < a.C) page = a.page_of[lib * a.C + c];
-      if (page < 0 || page >= a.n_pages) {
-        flag_error(XENCB_DEV_BADPAGE);
-        page = -1;
-      }
-    }
+// The page that pair i reads and its valid slots; -1: none. Bad tables are flagged where `flag` is set.
+__device__ __forceinline__ int ms_page(const MassArgs& a, int i, bool flag, int* nv) {
+  const int c = a.idx[i];
+  if (c < 0 || a.wk[i] == 0.f) return -1;
+  const int64_t at = (int64_t)((unsigned)i / (unsigned)a.k / (unsigned)a.rows_per_lib) * a.C + c;
+  const int page = c < a.C ? a.page_of[at] : -1;
+  if (page < 0 || page >= a.n_pages) {
+    if (flag) flag_error(XENCB_DEV_BADPAGE);
+    return -1;
+  }
+  const int n = a.n_valid[at];
+  if (flag && n > a.page_rows) flag_error(XENCB_DEV_CLAMPED);
+  *nv = min(n, a.page_rows);
+  return n > 0 ? page : -1;
+}
+
+__device__ __forceinline__ void ms_count(const MassArgs& a, unsigned first, unsigned step) {
+  for (unsigned i = first; i < (unsigned)a.n_pairs; i += step) {
+    int nv;
+    const int page = ms_page(a, i, true, &nv);
     if (page >= 0) {
-      const int nv = a.n_valid[lib * a.C + c];
-      if (nv > a.page_rows) flag_error(XENCB_DEV_CLAMPED);
-      if (nv <= 0) {
-        page = -1;
-      } else {
-        atomicAdd(&a.cnt[page], 1);
-        atomicMax(&a.nvmax[page], min(nv, a.page_rows));
-      }
+      atomicAdd(&a.cnt[page], 1);
+      atomicMax(&a.nvmax[page], nv);
     }
     a.page[i] = page;
   }
 }
 
 __global__ void __launch_bounds__(256) mass_count_kernel(const MassArgs a) {
-  ms_count(a, (int64_t)blockIdx.x * blockDim.x + threadIdx.x, (int64_t)gridDim.x * blockDim.x);
+  ms_count(a, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
 }
 
-// First places and tiles of the pages, by one CTA of 1024 threads.
-__device__ __forceinline__ void ms_scan(const MassArgs& a) {
+// First places and tiles of the pages, by one CTA of 1024 threads. The tiles of few pairs, which take half as long, lie
+// behind all others: the clusters take the tiles in turn.
+constexpr int MS_PLAN_THREADS = 1024;
+__global__ void __launch_bounds__(MS_PLAN_THREADS) mass_plan_kernel(const MassArgs a, int counted) {
   __shared__ int sh[32];
-  const int per = (a.n_pages + 1023) / 1024;
-  const int p0 = min(a.n_pages, (int)threadIdx.x * per), p1 = min(a.n_pages, p0 + per);
-  int pos = 0, tiles = 0;
-  for (int p = p0; p < p1; ++p) {
-    pos += a.cnt[p];
-    tiles += (a.cnt[p] + MS_M - 1) / MS_M;
+  pdl_trigger();
+  if (!counted) {
+    for (int p = threadIdx.x; p < a.n_pages; p += MS_PLAN_THREADS) {
+      a.cnt[p] = 0;
+      a.nvmax[p] = 0;
+    }
+    __syncthreads();
+    ms_count(a, threadIdx.x, MS_PLAN_THREADS);
+    __syncthreads();
   }
-  int all;
+  const int per = (a.n_pages + MS_PLAN_THREADS - 1) / MS_PLAN_THREADS;
+  const int p0 = min(a.n_pages, (int)threadIdx.x * per), p1 = min(a.n_pages, p0 + per);
+  int pos = 0, big = 0, few = 0;
+  for (int p = p0; p < p1; ++p) {
+    const int c = a.cnt[p], left = c % MS_M;
+    pos += c;
+    big += c / MS_M + (left > MS_FEW);
+    few += left > 0 && left <= MS_FEW;
+  }
+  int all, n_big, n_few;
   int at = pg_scan(pos, sh, &all);
-  int tile = pg_scan(tiles, sh, &all);
-  if (threadIdx.x == 0) *a.n_tiles = all;
+  int tb = pg_scan(big, sh, &n_big);
+  int tf = pg_scan(few, sh, &n_few) + n_big;
+  if (threadIdx.x == 0) *a.n_tiles = n_big + n_few;
   for (int p = p0; p < p1; ++p) {
     const int c = a.cnt[p];
     a.start[p] = at;
-    a.tile0[p] = tile;
-    for (int s = 0; s < c; s += MS_M) a.tiles[tile++] = MassTile{p, at + s, min(MS_M, c - s), a.nvmax[p]};
+    a.tile0[p] = tb;
+    a.few[p] = -1;
+    for (int s = 0; s < c; s += MS_M) {
+      const int n = min(MS_M, c - s);
+      if (n <= MS_FEW) a.few[p] = tf;
+      a.tiles[n <= MS_FEW ? tf++ : tb++] = MassTile{p, at + s, n, a.nvmax[p]};
+    }
     at += c;
   }
 }
 
-// CTA 0: the plan (counted: the counts are there already). The others: four rows of q each, 256 threads a row.
-constexpr int MS_PREP_THREADS = 1024;
-template <typename TQ, typename T, int TERMS>
-__global__ void __launch_bounds__(MS_PREP_THREADS) mass_prep_kernel(const MassArgs a, const TQ* __restrict__ q,
-                                                                    T* __restrict__ out, int counted) {
-  __shared__ float red[32];
-  pdl_trigger();
-  if (blockIdx.x == 0) {
-    if (!counted) {
-      for (int p = threadIdx.x; p < a.n_pages; p += MS_PREP_THREADS) {
-        a.cnt[p] = 0;
-        a.nvmax[p] = 0;
+constexpr int MS_ROWS_THREADS = 256;
+constexpr int MS_ROWS_IDS = 16;  // pairs a thread looks at in one round
+
+// Exclusive count over the CTA's threads; *total gets the sum. `sh` holds a round's sums of the warps.
+__device__ __forceinline__ int ms_scan(int c, int* sh, int* total) {
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  int incl = c;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  __syncthreads();
+  if (lane == 31) sh[wid] = incl;
+  __syncthreads();
+  int before = incl - c, all = 0;
+#pragma unroll
+  for (int w = 0; w < MS_ROWS_THREADS / 32; ++w) {
+    before += w < wid ? sh[w] : 0;
+    all += sh[w];
+  }
+  *total = all;
+  return before;
+}
+
+// The pairs of page p in the order of their rows.
+__device__ __forceinline__ void ms_order(const MassArgs& a, int p) {
+  __shared__ int sh[MS_ROWS_THREADS / 32];
+  __shared__ int nv_most;
+  if (threadIdx.x == 0) nv_most = 0;
+  const int n = a.direct ? a.n_pairs : a.cnt[p];
+  const int64_t start = a.direct ? (int64_t)p * a.n_pairs : a.start[p];
+  int found = 0;
+  const int ids = a.direct ? MS_DIRECT / MS_ROWS_THREADS : MS_ROWS_IDS;  // pairs of a thread in one round
+  for (int64_t i0 = 0; i0 < a.n_pairs && found < n; i0 += MS_ROWS_THREADS * ids) {
+    const int64_t i = i0 + threadIdx.x * ids;
+    uint32_t hit = 0;
+    if (a.direct) {
+#pragma unroll
+      for (int e = 0; e < MS_DIRECT / MS_ROWS_THREADS; ++e) {
+        int nv;
+        if (i + e < a.n_pairs) hit |= (uint32_t)(ms_page(a, (int)i + e, p == 0, &nv) == p) << e;
       }
-      __syncthreads();
-      ms_count(a, threadIdx.x, MS_PREP_THREADS);
-      __syncthreads();
+    } else {
+      int id[MS_ROWS_IDS];
+#pragma unroll
+      for (int e = 0; e < MS_ROWS_IDS; e += 4) {
+        if (i + e + 4 <= a.n_pairs) {
+          *reinterpret_cast<int4*>(id + e) = *reinterpret_cast<const int4*>(a.page + i + e);
+        } else {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) id[e + x] = i + e + x < a.n_pairs ? a.page[i + e + x] : -1;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < MS_ROWS_IDS; ++e) hit |= (uint32_t)(id[e] == p) << e;
     }
-    ms_scan(a);
+    int round;
+    int64_t place = start + found + ms_scan(__popc(hit), sh, &round);
+    found += round;
+    for (; hit; hit &= hit - 1, ++place) {
+      const unsigned j = (unsigned)i + __ffs(hit) - 1, row = j / (unsigned)a.k;
+      const int nv = min(a.n_valid[(int64_t)(row / (unsigned)a.rows_per_lib) * a.C + a.idx[j]], a.page_rows);
+      a.prow[place] = (int)row;
+      a.pnv[place] = nv;
+      a.pw[place] = a.wk[j];
+      if (a.direct) atomicMax(&nv_most, nv);
+    }
+  }
+  if (!a.direct) return;
+  __syncthreads();
+  const int per = a.slots / a.n_pages;
+  if (threadIdx.x < per) {
+    const int s = threadIdx.x * MS_M;
+    a.tiles[threadIdx.x * a.n_pages + p] = MassTile{p, (int)(start + s), max(0, min(MS_M, found - s)), nv_most};
+  }
+  if (threadIdx.x == 0) a.cnt[p] = found;
+}
+
+// CTAs 0 .. n_pages - 1: a page's pairs; the others: a row of q each.
+template <typename TQ, typename T, int TERMS>
+__global__ void __launch_bounds__(MS_ROWS_THREADS) mass_rows_kernel(const MassArgs a, const TQ* __restrict__ q,
+                                                                    T* __restrict__ out) {
+  __shared__ float red[MS_ROWS_THREADS / 32];
+  pdl_trigger();
+  if ((int)blockIdx.x < a.n_pages) {
+    pdl_wait();
+    ms_order(a, blockIdx.x);
     return;
   }
-  const int grp = threadIdx.x >> 8, t = threadIdx.x & 255;
-  const int64_t row = ((int64_t)blockIdx.x - 1) * 4 + grp;
-  const bool in = row < a.n_rows;
+  // (q may be read before the wait: the plan is a plain launch, so whatever wrote q has completed)
+  const int64_t row = (int64_t)blockIdx.x - a.n_pages;
   const TQ* src = q + row * a.d_s;
+  constexpr int STEP = MS_ROWS_THREADS * 8, HELD = 2;  // the first HELD pieces stay in registers
+  float v[HELD][8];
+  float mx = 0.f;
+#pragma unroll
+  for (int h = 0; h < HELD; ++h) {
+    const int i = h * STEP + threadIdx.x * 8;
+    if (i < a.d_s) {
+      load8_f32<TQ>(src + i, v[h]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(v[h][e]));
+    }
+  }
   float s = 1.f;
   if (std::is_same<T, __half>::value) {  // f16's range: the row's largest value to [2^14, 2^15)
-    float mx = 0.f;
-    if (in)
-      for (int i = t * 8; i < a.d_s; i += 256 * 8) {
-        float v[8];
-        load8_f32<TQ>(src + i, v);
+    for (int i = HELD * STEP + threadIdx.x * 8; i < a.d_s; i += STEP) {
+      float w[8];
+      load8_f32<TQ>(src + i, w);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(v[e]));
-      }
+      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(w[e]));
+    }
     mx = warp_max(mx);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = mx;
     __syncthreads();
-    mx = red[grp * 8];
+    mx = red[0];
 #pragma unroll
-    for (int w = 1; w < 8; ++w) mx = fmaxf(mx, red[grp * 8 + w]);
+    for (int w = 1; w < MS_ROWS_THREADS / 32; ++w) mx = fmaxf(mx, red[w]);
     s = f16_range_scale(mx);
   }
-  if (!in) return;
-  if (t == 0) a.rinv[row] = 1.f / s;
-  for (int i = t * 8; i < a.d_s; i += 256 * 8) {
-    float v[8];
-    load8_f32<TQ>(src + i, v);
+  pdl_wait();
+  if (threadIdx.x == 0) a.rinv[row] = 1.f / s;
+  auto emit = [&](int i, const float* w) {
     alignas(16) T hi[8], lo[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      hi[e] = from_f32<T>(v[e] * s);
-      if (TERMS == 2) lo[e] = from_f32<T>(v[e] * s - to_f32(hi[e]));
+      hi[e] = from_f32<T>(w[e] * s);
+      if (TERMS == 2) lo[e] = from_f32<T>(w[e] * s - to_f32(hi[e]));
     }
     *reinterpret_cast<uint4*>(out + row * a.d_s + i) = *reinterpret_cast<const uint4*>(hi);
     if (TERMS == 2)
       *reinterpret_cast<uint4*>(out + (a.n_rows + row) * a.d_s + i) = *reinterpret_cast<const uint4*>(lo);
+  };
+#pragma unroll
+  for (int h = 0; h < HELD; ++h) {
+    const int i = h * STEP + threadIdx.x * 8;
+    if (i < a.d_s) emit(i, v[h]);
   }
-}
-
-// One CTA per page: its pairs in the order of their rows.
-constexpr int MS_ORDER_THREADS = 256;
-__global__ void __launch_bounds__(MS_ORDER_THREADS) mass_order_kernel(const MassArgs a) {
-  __shared__ int sh[MS_ORDER_THREADS / 32];
-  pdl_trigger();
-  pdl_wait();
-  const int p = blockIdx.x, n = a.cnt[p], start = a.start[p];
-  if (n == 0) return;
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  int found = 0;
-  for (int64_t i0 = 0; i0 < a.n_pairs && found < n; i0 += MS_ORDER_THREADS * 4) {
-    const int64_t i = i0 + threadIdx.x * 4;
-    int hit[4], c = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      hit[e] = i + e < a.n_pairs && a.page[i + e] == p;
-      c += hit[e];
-    }
-    int incl = c;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += y;
-    }
-    __syncthreads();
-    if (lane == 31) sh[wid] = incl;
-    __syncthreads();
-    int at = found + incl - c;
-#pragma unroll
-    for (int w = 0; w < MS_ORDER_THREADS / 32; ++w) {
-      at += w < wid ? sh[w] : 0;
-      found += sh[w];
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (hit[e]) {
-        const int64_t row = (i + e) / a.k;
-        const int place = start + at++;
-        a.prow[place] = (int)row;
-        a.pnv[place] = min(a.n_valid[row / a.rows_per_lib * a.C + a.idx[i + e]], a.page_rows);
-        a.pw[place] = a.wk[i + e];
-      }
+  for (int i = HELD * STEP + threadIdx.x * 8; i < a.d_s; i += STEP) {
+    float w[8];
+    load8_f32<TQ>(src + i, w);
+    emit(i, w);
   }
 }
 
@@ -255,6 +326,7 @@ struct MsSmem {
   unsigned char* stages;
   float* stat;   // [2][2 cs][128][2]: by the parity of the tile, maximum and sum of each pair's half of a CTA's slots
   float* cols;   // [4][256]: column sums of the lane quarters
+  float* xch;    // [2][64][MS_XPITCH]: sums of the lo rows of few pairs
   uint64_t *full, *empty, *s_full, *s_empty, *st;
   uint32_t* tmem;
   volatile int* abort_flag;
@@ -271,7 +343,8 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
   s.stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ms_smem_raw) + 1023) & ~uintptr_t(1023));
   s.stat = reinterpret_cast<float*>(s.stages + n_st * STAGE);
   s.cols = s.stat + cs * 4 * MS_M * 2;
-  s.full = reinterpret_cast<uint64_t*>(s.cols + 4 * MS_N);
+  s.xch = s.cols + 4 * MS_N;
+  s.full = reinterpret_cast<uint64_t*>(s.xch + (TERMS == 2 ? 2 * MS_FEW * MS_XPITCH : 0));
   s.empty = s.full + 4;
   s.s_full = s.empty + 4;
   s.s_empty = s.s_full + 2;
@@ -311,14 +384,15 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
   tc_fence_after();
   const uint32_t taddr = *s.tmem;
   pdl_wait();
-  const int n_tiles = *a.n_tiles;
+  const int n_tiles = a.direct ? a.slots : *a.n_tiles;
+  auto stacked = [](const MassTile& t) { return TERMS == 2 && t.count <= MS_FEW; };
   auto done = [&](bool arrived) {
     if (!arrived) *s.abort_flag = 1;
     __syncwarp();
   };
 
   // The softmax keeps 128 sums a thread: the other warps give registers up (their sum stays below the launch's).
-  if (warp < 4) {
+  if (warp < MS_LOW) {
     regs_dec<MS_REGS_LOW>();
     if (warp == 0) {
       // --------------------------------------------------------------------------------------------- slots
@@ -328,7 +402,7 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
         bool ok = true;
         for (int t = cluster; t < n_tiles && ok; t += n_clusters) {
           const MassTile tile = a.tiles[t];
-          if (seg0 >= tile.nv) continue;
+          if (tile.count == 0 || seg0 >= tile.nv) continue;
           const int y = tile.page * a.page_rows + seg0;
           for (int kb = 0; kb < nkb; ++kb) {
             if (used >= (uint32_t)n_st && !(ok = mbar_wait_spin(&s.empty[ring.st], ring.phase ^ 1))) break;
@@ -355,7 +429,9 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
         bool ok = true;
         const uint32_t idesc = umma_idesc(FMT, FMT, MS_M, a.per);
         for (int t = cluster; t < n_tiles && ok; t += n_clusters) {
-          if (seg0 >= a.tiles[t].nv) continue;
+          const MassTile tile = a.tiles[t];
+          if (tile.count == 0 || seg0 >= tile.nv) continue;
+          const int terms = stacked(tile) ? 1 : TERMS;
           for (int k0 = 0; k0 < nkb && ok; k0 += MS_CHUNK, ++acc) {
             const uint32_t buf = acc & 1, use = acc >> 1;
             if (use > 0 && !(ok = mbar_wait_spin(&s.s_empty[buf], (use - 1) & 1))) break;
@@ -370,7 +446,7 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
               for (int ks = 0; ks < 4; ++ks)
   #pragma unroll
                 for (int x = 0; x < TERMS; ++x)
-                  tc_mma<0>(taddr + buf * MS_N, umma_desc_k_sw128(st + x * MS_ATILE + ks * 32),
+                  if (x < terms) tc_mma<0>(taddr + buf * MS_N, umma_desc_k_sw128(st + x * MS_ATILE + ks * 32),
                             umma_desc_k_sw128(bk + ks * 32), idesc, kb > k0 || ks > 0 || x > 0);
               tc_commit(&s.empty[ring.st]);
               ring.next(n_st);
@@ -381,11 +457,11 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
         if (!ok) *s.abort_flag = 1;
       }
       __syncwarp();
-    } else {
+    } else if (warp >= 4) {
       // --------------------------------------------------------------------------------------------- rows of Q
       // Eight lanes a row (16 bytes each: chunk j of row r at chunk j ^ (r % 8)), 4 MS_PRODUCERS rows at a time.
       constexpr int STEP = 4 * MS_PRODUCERS, PASSES = MS_M / STEP;
-      const int t0 = threadIdx.x - 64;
+      const int t0 = threadIdx.x - 128;
       const int sub = t0 >> 3, ch = t0 & 7;
       const char* q = static_cast<const char*>(a.q16);
       const int64_t row_bytes = (int64_t)a.d_s * 2, lo = a.n_rows * row_bytes;
@@ -394,7 +470,8 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
       bool ok = true;
       for (int t = cluster; t < n_tiles && ok; t += n_clusters) {
         const MassTile tile = a.tiles[t];
-        if (seg0 >= tile.nv) continue;
+        if (tile.count == 0 || seg0 >= tile.nv) continue;
+        const uint32_t lo_at = stacked(tile) ? MS_FEW * 128 : MS_ATILE;
         int rows[PASSES];
   #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
@@ -417,7 +494,7 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
               const char* src = q + rows[i] * row_bytes + (in ? col * 2 : 0);
               const uint32_t dst = st + r * 128 + ((ch ^ (r & 7)) << 4);
               ms_copy16(dst, src, in ? 16 : 0);
-              if (TERMS == 2) ms_copy16(dst + MS_ATILE, src + lo, in ? 16 : 0);
+              if (TERMS == 2) ms_copy16(dst + lo_at, src + lo, in ? 16 : 0);
             }
           }
           ms_copies_arrive(&s.full[ring.st]);
@@ -432,15 +509,17 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
   } else {
     // --------------------------------------------------------------------------------------------- softmax
     regs_inc<MS_REGS_HIGH>();
-    const int quarter = warp & 3, half = (warp - 2 - MS_PRODUCERS) >> 2;
+    const int quarter = warp & 3, half = (warp - MS_LOW) >> 2;
     const int r = quarter * 32 + lane;               // pair of the tile = TMEM lane
     const uint32_t tl = taddr + ((uint32_t)(quarter * 32) << 16) + half * 128;
     const int n0 = seg0 + half * 128;                // first slot of this warp
     const int width = max(0, min(128, a.per - half * 128));
     uint32_t acc = 0, gen = 0;
-    for (int t = cluster; t < n_tiles; t += n_clusters, ++gen) {
+    for (int t = cluster; t < n_tiles; t += n_clusters) {
       const MassTile tile = a.tiles[t];
-      const bool here = r < tile.count, any = quarter * 32 < tile.count;
+      if (tile.count == 0) continue;
+      const bool few = stacked(tile), here = r < tile.count, any = quarter * 32 < tile.count;
+      const bool drain = (few ? quarter & 1 : quarter) * 32 < tile.count && width > 0;  // this warp's lanes hold sums
       int nv = 0;
       float w = 0.f, c = 0.f;
       if (here) {
@@ -457,7 +536,7 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
           const uint32_t buf = acc & 1;
           done(*s.abort_flag || mbar_wait_spin(&s.s_full[buf], (acc >> 1) & 1));
           tc_fence_after();
-          if (any && width > 0) {
+          if (drain) {
 #pragma unroll
             for (int g = 0; g < 128; g += 32) {
               float x[32];
@@ -472,20 +551,50 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
           __syncwarp();
         }
       }
+      if (TERMS == 2 && few && drain) {  // the lo rows' sums, 64 lanes further, to those of the hi rows
+        float* x = s.xch + (half * MS_FEW + (quarter & 1) * 32 + lane) * MS_XPITCH;
+#pragma unroll
+        for (int g = 0; g < 128; g += 16) {
+          if (quarter >= 2) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = v[g + i];
+          }
+          named_bar_sync(2 + half * 2 + (quarter & 1), 64);
+          if (quarter < 2) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[g + i] += x[i];
+          }
+          named_bar_sync(2 + half * 2 + (quarter & 1), 64);
+        }
+      }
       // e^(score - max) of this half, its maximum and sum
       float m = -CUDART_INF_F, l = 0.f;
+      {
+        float mx[4] = {m, m, m, m}, sum[4] = {0.f, 0.f, 0.f, 0.f};  // (four chains: the warps are few)
+        if (__all_sync(0xffffffffu, nv == 128)) {
 #pragma unroll
-      for (int i = 0; i < 128; ++i) {
-        v[i] *= c;
-        if (i < nv) m = fmaxf(m, v[i]);
-      }
+          for (int i = 0; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i] * c);
+          m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 #pragma unroll
-      for (int i = 0; i < 128; ++i) {
-        v[i] = i < nv ? pf_exp2(v[i] - m) : 0.f;
-        l += v[i];
+          for (int i = 0; i < 128; ++i) {
+            v[i] = pf_exp2(fmaf(v[i], c, -m));
+            sum[i & 3] += v[i];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 128; ++i)
+            if (i < nv) mx[i & 3] = fmaxf(mx[i & 3], v[i] * c);
+          m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+#pragma unroll
+          for (int i = 0; i < 128; ++i) {
+            v[i] = i < nv ? pf_exp2(fmaf(v[i], c, -m)) : 0.f;
+            sum[i & 3] += v[i];
+          }
+        }
+        l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
       }
       float* stat = s.stat + (size_t)(gen & 1) * cs * 2 * MS_M * 2;
-      if (threadIdx.x == 32 * (2 + MS_PRODUCERS)) mbar_arrive_expect_tx(&s.st[gen & 1], (uint32_t)cs * 2 * MS_M * 8);
+      if (threadIdx.x == 32 * MS_LOW) mbar_arrive_expect_tx(&s.st[gen & 1], (uint32_t)cs * 2 * MS_M * 8);
       {
         float* mine = stat + ((rank * 2 + half) * MS_M + r) * 2;
         for (int to = 0; to < cs; ++to) {
@@ -507,12 +616,12 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
       for (int g = 0; g < 128; g += 32) {
         float x[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) x[i] = g + i < nv ? v[g + i] * f : 0.f;
+        for (int i = 0; i < 32; ++i) x[i] = g + i < nv ? v[g + i] * f : 0.f;  // (not 0 * NaN)
         const float sum = any ? rs_reduce<32>(x, lane, [](float p, float q) { return p + q; }) : 0.f;
         s.cols[quarter * MS_N + half * 128 + g + lane] = sum;
       }
       named_bar_sync(1, 32 * MS_EPI);
-      const int col = (int)threadIdx.x - 32 * (2 + MS_PRODUCERS);
+      const int col = (int)threadIdx.x - 32 * MS_LOW;
       if (col < a.per && seg0 + col < a.page_rows) {
         float sum = s.cols[col];
 #pragma unroll
@@ -520,6 +629,7 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
         a.part[(int64_t)t * a.page_rows + seg0 + col] = sum;
       }
       named_bar_sync(1, 32 * MS_EPI);
+      ++gen;
     }
   }
   __syncwarp();
@@ -538,9 +648,17 @@ __global__ void __launch_bounds__(256) mass_combine_kernel(const MassArgs a) {
   if (n >= a.page_rows) return;
   const int64_t at = (int64_t)p * a.page_rows + n;
   float v = a.prior ? a.decay * a.prior[at] : 0.f;
-  const int tiles = (a.cnt[p] + MS_M - 1) / MS_M;
-  const float* part = a.part + (int64_t)a.tile0[p] * a.page_rows + n;
-  for (int t = 0; t < tiles; ++t) v += part[(int64_t)t * a.page_rows];
+  const int c = a.cnt[p];
+  if (a.direct) {
+    const float* part = a.part + (int64_t)p * a.page_rows + n;
+    for (int t = 0; t * MS_M < c; ++t) v += part[(int64_t)t * a.n_pages * a.page_rows];
+  } else {
+    const int big = c / MS_M + (c % MS_M > MS_FEW);
+    const float* part = a.part + (int64_t)a.tile0[p] * a.page_rows + n;
+#pragma unroll 4
+    for (int t = 0; t < big; ++t) v += part[(int64_t)t * a.page_rows];
+    if (c > 0 && a.few[p] >= 0) v += a.part[(int64_t)a.few[p] * a.page_rows + n];
+  }
   a.mass[at] = v;
 }
 

@@ -1008,9 +1008,9 @@ int run_shared(const void* q, int q_dtype, const SharedPlan& p, SharedArgs a, co
 }
 // ------------------------------------------------------------------------------------------------ attention mass plan
 struct MassPlan {
-  int terms, cs, per;
+  int terms, cs, per, direct;
   int64_t n_pairs, max_tiles;
-  size_t pages, pair, tiles, q, rinv, part, total;
+  size_t pages, pair, place, tiles, q, rinv, part, total;
 };
 
 int plan_mass(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows, int slots_dtype, int q_dtype, MassPlan* p) {
@@ -1022,21 +1022,25 @@ int plan_mass(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows, in
   if (d_s % 8 != 0) return fail(XENCB_ENOTSUP, "read_mass: d_s=%d must be a multiple of 8", d_s);
   if (page_rows > MS_N * MS_MAX_CS)
     return fail(XENCB_ENOTSUP, "read_mass: page_rows=%d, at most %d are supported", page_rows, MS_N * MS_MAX_CS);
-  if (n_rows > (INT32_MAX - 64) / k || n_pages * (int64_t)page_rows + 1024 > INT32_MAX)
+  if (n_rows > (INT32_MAX - 64) / k || n_rows + n_pages > INT32_MAX || n_pages * (int64_t)page_rows + 1024 > INT32_MAX)
     return fail(XENCB_ENOTSUP, "read_mass: too many rows, routed chunks or pages");
   p->n_pairs = n_rows * k;
   // a 16-bit q is one product where the slots' type holds it (bf16's 8 bits fit f16)
   p->terms = q_dtype == XENCB_F32 || (q_dtype == XENCB_F16 && slots_dtype == XENCB_BF16) ? 2 : 1;
   p->cs = (page_rows + MS_N - 1) / MS_N;
   p->per = (int)align_up((size_t)(page_rows + p->cs - 1) / p->cs, 16);
-  p->max_tiles = p->n_pairs / MS_M + std::min<int64_t>(n_pages, p->n_pairs);
+  // few pairs over few pages: no plan, but room in every page for all of them
+  const int64_t most = (p->n_pairs + MS_M - 1) / MS_M;
+  p->direct = p->n_pairs <= MS_DIRECT && n_pages * most <= 4096;
+  p->max_tiles = p->direct ? n_pages * most : p->n_pairs / MS_M + std::min<int64_t>(n_pages, p->n_pairs);
   p->pages = align_up((size_t)n_pages * 4, 256);
   p->pair = align_up((size_t)p->n_pairs * 4, 256);
+  p->place = p->direct ? align_up((size_t)p->n_pairs * n_pages * 4, 256) : p->pair;
   p->tiles = align_up((size_t)p->max_tiles * sizeof(MassTile), 256);
   p->q = align_up((size_t)p->terms * n_rows * d_s * 2, 256);
   p->rinv = align_up((size_t)n_rows * 4, 256);
   p->part = align_up((size_t)p->max_tiles * page_rows * 4, 256);
-  p->total = 4 * p->pages + 4 * p->pair + p->tiles + 256 + p->q + p->rinv + p->part;
+  p->total = 5 * p->pages + p->pair + 3 * p->place + p->tiles + 256 + p->q + p->rinv + p->part;
   return XENCB_OK;
 }
 
@@ -1068,18 +1072,23 @@ int run_mass(const void* q, int q_dtype, const MassPlan& p, const MassArgs& a, c
     mass_count_kernel<<<(unsigned)std::min<int64_t>((p.n_pairs + 255) / 256, 4 * sms), 256, 0, st>>>(a);
     XENCB_CHECK_LAUNCH("mass_count launch");
   }
+  if (!p.direct) {
+    mass_plan_kernel<<<1, MS_PLAN_THREADS, 0, st>>>(a, counted);
+    XENCB_CHECK_LAUNCH("mass_plan launch");
+  }
   T* qo = static_cast<T*>(q16);
-  const unsigned pgrid = 1 + (unsigned)((a.n_rows + 3) / 4);
-  auto prep = [&](auto t) {
+  const dim3 rgrid((unsigned)(a.n_pages + a.n_rows));
+  auto rows = [&](auto t) {
     using TQ = decltype(t);
-    mass_prep_kernel<TQ, T, TERMS><<<pgrid, MS_PREP_THREADS, 0, st>>>(a, static_cast<const TQ*>(q), qo, counted);
+    auto rk = mass_rows_kernel<TQ, T, TERMS>;
+    // (its rows are read before the plan is waited for: it may only follow the plan so closely)
+    if (p.direct) rk<<<rgrid, MS_ROWS_THREADS, 0, st>>>(a, static_cast<const TQ*>(q), qo);
+    else launch_pdl(rk, rgrid, dim3(MS_ROWS_THREADS), 0, st, a, static_cast<const TQ*>(q), qo);
   };
-  if (q_dtype == XENCB_F32) prep(float{});
-  else if (q_dtype == XENCB_F16) prep(__half{});
-  else prep(__nv_bfloat16{});
-  XENCB_CHECK_LAUNCH("mass_prep launch");
-  launch_pdl(mass_order_kernel, dim3((unsigned)a.n_pages), dim3(MS_ORDER_THREADS), 0, st, a);
-  XENCB_CHECK_LAUNCH("mass_order launch");
+  if (q_dtype == XENCB_F32) rows(float{});
+  else if (q_dtype == XENCB_F16) rows(__half{});
+  else rows(__nv_bfloat16{});
+  XENCB_CHECK_LAUNCH("mass_rows launch");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(n_clusters * p.cs));
   cfg.blockDim = dim3(MS_THREADS);
@@ -1964,17 +1973,20 @@ int xencb_read_mass(const void* q, int q_dtype, int64_t n_rows, int d_s, const v
     return at;
   };
   MassArgs a{};
-  a.page_of = page_of; a.n_valid = n_valid; a.idx = idx; a.wk = wk; a.n_rows = n_rows; a.rows_per_lib = rows_per_lib;
-  a.n_lib = n_lib; a.k = k; a.C = n_chunks; a.n_pages = (int)n_pages; a.page_rows = page_rows; a.d_s = d_s;
+  a.page_of = page_of; a.n_valid = n_valid; a.idx = idx; a.wk = wk; a.n_rows = n_rows;
+  a.rows_per_lib = (int)std::min<int64_t>(rows_per_lib, INT32_MAX);
+  a.k = k; a.C = n_chunks; a.n_pages = (int)n_pages; a.page_rows = page_rows; a.d_s = d_s;
   a.n_pairs = (int)p.n_pairs;
   a.cnt = reinterpret_cast<int*>(take(p.pages));
   a.nvmax = reinterpret_cast<int*>(take(p.pages));
   a.start = reinterpret_cast<int*>(take(p.pages));
   a.tile0 = reinterpret_cast<int*>(take(p.pages));
+  a.few = reinterpret_cast<int*>(take(p.pages));
   a.page = reinterpret_cast<int*>(take(p.pair));
-  a.prow = reinterpret_cast<int*>(take(p.pair));
-  a.pnv = reinterpret_cast<int*>(take(p.pair));
-  a.pw = reinterpret_cast<float*>(take(p.pair));
+  a.prow = reinterpret_cast<int*>(take(p.place));
+  a.pnv = reinterpret_cast<int*>(take(p.place));
+  a.pw = reinterpret_cast<float*>(take(p.place));
+  a.direct = p.direct; a.slots = (int)p.max_tiles;
   a.tiles = reinterpret_cast<MassTile*>(take(p.tiles));
   a.n_tiles = reinterpret_cast<int*>(take(256));
   void* q16 = take(p.q);
