@@ -2375,10 +2375,9 @@ int xencb_pages_compact(void* const* pools, const int64_t* row_bytes, int n_pool
 
 size_t xencb_pages_evict_workspace(int64_t n_pages, int page_rows, int per_library) {
   if (n_pages <= 0 || page_rows <= 0 || page_rows > EV_MAX_ROWS || n_pages > PG_MAX_PAGES) return 0;
-  const size_t lists = 3 * pages_list_bytes(n_pages);
-  if (!per_library) return lists;
-  return lists + align_up((size_t)n_pages * page_rows * sizeof(uint16_t), 256) +
-         align_up((size_t)n_pages * ((page_rows + 31) / 32) * sizeof(uint32_t), 256);
+  const size_t lists = 2 * pages_list_bytes(n_pages) +
+                       align_up((size_t)n_pages * ((page_rows + 31) / 32) * sizeof(uint32_t), 256);
+  return lists + (per_library ? align_up((size_t)n_pages * page_rows * sizeof(uint32_t), 256) : 0);
 }
 
 int xencb_pages_evict(const void* const* pools, void* const* pools_out, const int64_t* row_bytes, int n_pools,
@@ -2420,25 +2419,35 @@ int xencb_pages_evict(const void* const* pools, void* const* pools_out, const in
   a.n_valid_out = n_valid_out; a.mass_out = mass_out; a.kept = kept_out;
   a.rows = reinterpret_cast<int*>(ws);
   a.most = reinterpret_cast<int*>(ws + list);
-  a.count = reinterpret_cast<int*>(ws + 2 * list);
   a.words = (page_rows + 31) / 32;
-  if (per_library) {
-    a.rank = reinterpret_cast<uint16_t*>(ws + 3 * list);
-    a.bits = reinterpret_cast<uint32_t*>(ws + 3 * list + align_up((size_t)n_pages * page_rows * sizeof(uint16_t), 256));
-  }
+  a.bits = reinterpret_cast<uint32_t*>(ws + 2 * list);
+  a.keys = reinterpret_cast<uint32_t*>(ws + 2 * list + align_up((size_t)n_pages * a.words * sizeof(uint32_t), 256));
+  // short tables are looked through by every page's CTA (one launch less); a million entries in all take about 10 us
+  a.direct = n_lib * n_chunks <= 1024 && n_lib * n_chunks * n_pages <= (1 << 20);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  evict_plan_kernel<<<1, PG_THREADS, 0, st>>>(a);
-  XENCB_CHECK_LAUNCH("evict_plan launch");
+  if (!a.direct) {
+    evict_plan_kernel<<<1, PG_THREADS, 0, st>>>(a);
+    XENCB_CHECK_LAUNCH("evict_plan launch");
+  }
   int n2 = 64;
   while (n2 < page_rows) n2 *= 2;
-  launch_pdl(evict_rank_kernel, dim3((unsigned)n_pages), dim3((unsigned)std::min(1024, std::max(64, n2 / 2))),
-             (size_t)n2 * 8, st, a, n2);
+  const dim3 rthreads((unsigned)std::min(1024, n2 <= EV_COUNTED ? n2 : n2 / 2));
+  const size_t rsmem = (size_t)n2 * (n2 <= EV_COUNTED ? 4 : 8);
+  if (a.direct) evict_rank_kernel<<<(unsigned)n_pages, rthreads, rsmem, st>>>(a, n2);
+  else launch_pdl(evict_rank_kernel, dim3((unsigned)n_pages), rthreads, rsmem, st, a, n2);
   XENCB_CHECK_LAUNCH("evict_rank launch");
   if (per_library) {
-    launch_pdl(evict_budget_kernel, dim3((unsigned)n_lib), dim3(PG_THREADS), 0, st, a);
+    const int pitch = a.words * 32;
+    const int64_t cache = (int64_t)n_chunks * pitch * 4;
+    const dim3 bgrid((unsigned)n_lib), bthreads(PG_THREADS);
+    if (cache <= 200 * 1024) {
+      rc = ensure_smem(evict_budget_kernel<true>, (int)cache);
+      if (rc) return rc;
+      launch_pdl(evict_budget_kernel<true>, bgrid, bthreads, (size_t)cache, st, a, pitch);
+    } else {
+      launch_pdl(evict_budget_kernel<false>, bgrid, bthreads, 0, st, a, pitch);
+    }
     XENCB_CHECK_LAUNCH("evict_budget launch");
-    launch_pdl(evict_list_kernel, dim3((unsigned)n_pages), dim3(256), 0, st, a);
-    XENCB_CHECK_LAUNCH("evict_list launch");
   }
   for (int i0 = 0; i0 < n_pools; i0 += PG_POOLS) {
     EvictPools pp{};
@@ -2462,6 +2471,7 @@ int xencb_pages_evict(const void* const* pools, void* const* pools_out, const in
     }
     for (int i = n; i <= PG_POOLS; ++i) pp.first[i] = (int)slices;
     pp.slices = (int)slices;
+    pp.outputs = i0 == 0;
     const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(64 * (int64_t)di.sms, n_pages * slices));
     auto go = [&](auto kern) { launch_pdl(kern, dim3(grid), dim3(EV_THREADS), 0, st, a, pp); };
     if (inplace) vec ? go(evict_inplace_kernel<uint4>) : go(evict_inplace_kernel<uint16_t>);

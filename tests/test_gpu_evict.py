@@ -139,6 +139,14 @@ def test_many_chunks_of_one_library():
         check(*a, 2000 + 777 * seed, [2000 + 777 * seed], per_library=True, M=60)
 
 
+@pytest.mark.parametrize("per_library", [False, True])
+def test_long_tables(per_library):
+    # too long for every page's CTA to look through, and too many rows of a Library for shared memory
+    a = case(45, 4, 300, 1250, 200, 8, [F16])
+    k = 9000 if per_library else 37
+    check(*a, k, [k] * 4 if per_library else [[k] * 300] * 4, per_library=per_library, M=90)
+
+
 def test_a_chunk_without_rows_and_a_page_outside_the_pool():
     pools, page_of, n_valid, mass = case(50, 2, 4, 12, 20, 16, [F16])
     n_valid[1, 2] = 0
