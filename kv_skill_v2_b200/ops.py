@@ -8,6 +8,7 @@ device. There is no CPU path: a CPU tensor raises RuntimeError.
 from __future__ import annotations
 
 import ctypes
+import functools
 from dataclasses import dataclass
 from typing import Optional
 
@@ -33,13 +34,16 @@ def _cuda(what: str, *ts) -> torch.device:
     for t in ts:
         if t is None:
             continue
+        d = t.device
+        if d == dev:
+            continue
         if not t.is_cuda:
-            raise RuntimeError(f"{what}: xencb kernels run on CUDA tensors only (got a {t.device} tensor); "
+            raise RuntimeError(f"{what}: xencb kernels run on CUDA tensors only (got a {d} tensor); "
                                "the Library read has no CPU path")
         if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise RuntimeError(f"{what}: tensors on {dev} and {t.device}")
+            dev = d
+        else:
+            raise RuntimeError(f"{what}: tensors on {dev} and {d}")
     return dev
 
 
@@ -65,7 +69,7 @@ class _on_device:
         self.prev = None
 
     def __enter__(self):
-        cur = torch.cuda.current_device()
+        cur = torch._C._cuda_getDevice()  # (torch.cuda.current_device() without its look whether CUDA is initialised)
         if cur != self.dev:
             self.prev = cur
             torch.cuda.set_device(self.dev)
@@ -77,6 +81,17 @@ class _on_device:
 
 def _workspace(nbytes: int, dev: torch.device) -> torch.Tensor:
     return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=dev)
+
+
+@functools.lru_cache(maxsize=4096)
+def _known_bytes(dev_index: int, query: str, *args) -> int:
+    return getattr(N.lib(), query)(*args)
+
+
+def _workspace_bytes(dev: torch.device, query: str, *args) -> int:
+    """A workspace query's answer, asked once per device and shape; 0 (the shape is refused) is asked again, so that the
+    library's message is this call's."""
+    return _known_bytes(dev.index, query, *args) or getattr(N.lib(), query)(*args)
 
 
 # ------------------------------------------------------------------------------------------------ rms / project
@@ -150,24 +165,29 @@ def weights_fp8(w: torch.Tensor) -> Weights8:
     return Weights8(w=out, scale=scale, k=k)
 
 
-def _weights8(what: str, dev, w: Weights8, d_in: int, adapters):
-    """(n, w, scale), checked; a row of d_in values is to be multiplied with it."""
+def _weights8(what: str, dev, w8: Weights8, d_in: int, w_prep, adapters):
+    """(n, address, address of the scales), checked; a row of d_in values is to be multiplied with it."""
     if adapters is not None:
         raise NotImplementedError(f"{what}: adapters beside an 8-bit weight")
-    if _cuda(what, w.w, w.scale) != dev:
-        raise RuntimeError(f"{what}: the weight is on {w.w.device}, the rows on {dev}")
-    k, nb = int(w.k), -(-int(w.k) // 128)
-    if w.w.dtype != torch.float8_e4m3fn or w.w.dim() != 2 or k <= 0 or w.w.shape[1] != nb * 128 \
-            or not w.w.is_contiguous() or w.w.data_ptr() % 16:
+    if w_prep is not None:
+        raise ValueError(f"{what}: w_prep is the prepared form of a float32 weight")
+    w, scale, k = w8.w, w8.scale, w8.k
+    if w.device != dev or scale.device != dev:
+        if not (w.is_cuda and scale.is_cuda):
+            _cuda(what, w, scale)
+        raise RuntimeError(f"{what}: the weight is on {w.device}, its scales on {scale.device}, the rows on {dev}")
+    nb = -(-k // 128)
+    n, at = w.shape[0] if w.dim() == 2 else 0, w.data_ptr()
+    if w.dtype is not torch.float8_e4m3fn or k <= 0 or w.shape != (n, nb * 128) or not w.is_contiguous() or at % 16:
         raise ValueError(f"{what}: an 8-bit weight of {k} columns is a contiguous, 16-byte aligned float8_e4m3fn "
-                         f"[n, {nb * 128}] tensor, got {w.w.dtype} {tuple(w.w.shape)}")
-    if w.scale.dtype not in (torch.uint8, torch.float8_e8m0fnu) or tuple(w.scale.shape) != (w.w.shape[0], nb) \
-            or not w.scale.is_contiguous():
-        raise ValueError(f"{what}: the scales must be contiguous uint8 (or float8_e8m0fnu) [{w.w.shape[0]}, {nb}], got "
-                         f"{w.scale.dtype} {tuple(w.scale.shape)}")
+                         f"[n, {nb * 128}] tensor, got {w.dtype} {tuple(w.shape)}")
+    if (scale.dtype is not torch.uint8 and scale.dtype is not torch.float8_e8m0fnu) or scale.shape != (n, nb) \
+            or not scale.is_contiguous():
+        raise ValueError(f"{what}: the scales must be contiguous uint8 (or float8_e8m0fnu) [{n}, {nb}], got "
+                         f"{scale.dtype} {tuple(scale.shape)}")
     if k != d_in:
         raise ValueError(f"{what}: the weight has {k} columns, the rows {d_in}")
-    return int(w.w.shape[0]), w.w, w.scale
+    return n, at, scale.data_ptr()
 
 
 @dataclass
@@ -229,9 +249,7 @@ def project_in(h2: torch.Tensor, w_in, b_in=None, *, rms: bool = True, l2: bool 
     h2 = h2.contiguous()
     R, d_m = h2.shape
     if w8 is not None:
-        if w_prep is not None:
-            raise ValueError("project_in: w_prep is the prepared form of a float32 weight")
-        d_s, w8_w, w8_s = _weights8("project_in", dev, w8, d_m, adapters)
+        d_s, w8_at, w8_scale = _weights8("project_in", dev, w8, d_m, w_prep, adapters)
     else:
         w_in = _f32(w_in, "w_in")
         d_s = w_in.shape[0]
@@ -249,8 +267,8 @@ def project_in(h2: torch.Tensor, w_in, b_in=None, *, rms: bool = True, l2: bool 
     gb, gb_dev = _dev_scalar(gate_b, "gate_b")
     with _on_device(dev):
         if w8 is not None:
-            ws = _workspace(N.lib().xencb_project_in8_workspace(R, d_m, d_s), dev)
-            N.call("xencb_project_in8", _ptr(h2), _hdt(h2, "h"), R, d_m, _ptr(w8_w), _ptr(w8_s), _ptr(b_in), d_s, flags,
+            ws = _workspace(_workspace_bytes(dev, "xencb_project_in8_workspace", R, d_m, d_s), dev)
+            N.call("xencb_project_in8", _ptr(h2), _hdt(h2, "h"), R, d_m, w8_at, w8_scale, _ptr(b_in), d_s, flags,
                    _ptr(gate_w), gb, _ptr(gb_dev), _ptr(sel_w), _ptr(sel_b), n_cand, eps, _ptr(q), _ptr(gate),
                    _ptr(rstd), _ptr(z), _ptr(ws), ws.numel(), _stream(dev))
             return q, gate, rstd, z
@@ -392,9 +410,7 @@ def project_out(r: torch.Tensor, w_out, h2: torch.Tensor, *, b_out=None, scale: 
     h2 = h2.contiguous()
     R, d_s = r.shape
     if w8 is not None:
-        if w_prep is not None:
-            raise ValueError("project_out: w_prep is the prepared form of a float32 weight")
-        d_m, w8_w, w8_s = _weights8("project_out", dev, w8, d_s, adapters)
+        d_m, w8_at, w8_scale = _weights8("project_out", dev, w8, d_s, w_prep, adapters)
     else:
         w_out = _f32(w_out, "w_out")
         d_m = w_out.shape[0]
@@ -410,8 +426,8 @@ def project_out(r: torch.Tensor, w_out, h2: torch.Tensor, *, b_out=None, scale: 
     ls_dev = None if log_scale is None else _dev_scalar(log_scale, "log_scale")[1]
     with _on_device(dev):
         if w8 is not None:
-            ws = _workspace(N.lib().xencb_project_out8_workspace(R, d_s, d_m), dev)
-            N.call("xencb_project_out8", _ptr(r), R, d_s, _ptr(w8_w), _ptr(w8_s), _ptr(b_out), d_m, float(scale),
+            ws = _workspace(_workspace_bytes(dev, "xencb_project_out8_workspace", R, d_s, d_m), dev)
+            N.call("xencb_project_out8", _ptr(r), R, d_s, w8_at, w8_scale, _ptr(b_out), d_m, float(scale),
                    _ptr(ls_dev), _ptr(gate), _ptr(sel_w), la, _ptr(la_dev), _ptr(pos_mask), _ptr(h2), _hdt(h2, "h"),
                    _ptr(delta), _ptr(h_out), _ptr(rel), _ptr(ws), ws.numel(), _stream(dev))
             return delta, h_out, rel
@@ -787,7 +803,7 @@ def read_mass(q: torch.Tensor, pages: Pages, idx: torch.Tensor, wk: torch.Tensor
         out = torch.empty(P, page_rows, dtype=torch.float32, device=dev)
     sdt, qdt = _hdt(slots, "slots"), _hdt(q, "q")
     with _on_device(dev):
-        ws_bytes = N.lib().xencb_read_mass_workspace(R, k, d_s, P, page_rows, sdt, qdt)
+        ws_bytes = _workspace_bytes(dev, "xencb_read_mass_workspace", R, k, d_s, P, page_rows, sdt, qdt)
         if ws_bytes == 0:
             N.check(N.EINVAL if min(R, k) <= 0 else N.ENOTSUP, "read_mass_workspace")
         ws = _workspace(ws_bytes, dev)
@@ -1112,7 +1128,7 @@ def pages_evict(pools, page_of: torch.Tensor, n_valid: torch.Tensor, mass: torch
     new_mass = torch.empty(P, rows, dtype=torch.float32, device=dev)
     kept = torch.empty(P, rows, dtype=torch.int32, device=dev)
     with _on_device(dev):
-        ws = _workspace(N.lib().xencb_pages_evict_workspace(P, N_rows, int(bool(per_library))), dev)
+        ws = _workspace(_workspace_bytes(dev, "xencb_pages_evict_workspace", P, N_rows, int(bool(per_library))), dev)
         N.call("xencb_pages_evict", ptrs, optrs, sizes, len(ptrs), P, N_rows, rows, _ptr(page_of), _ptr(n_valid), C,
                _ptr(n_chunks_of), n_lib, _ptr(mass), _ptr(keep), keep_all, int(bool(per_library)), min(int(floor), N_rows),
                _ptr(nv), _ptr(new_mass), _ptr(kept), _ptr(ws), ws.numel(), _stream(dev))
