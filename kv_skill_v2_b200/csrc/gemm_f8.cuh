@@ -11,8 +11,9 @@
 //
 // gemm_f8_kernel: D[n][m] (128 output features = UMMA M, BN rows of X = UMMA N). Warp 0 loads W8 and X8 tiles of 128 bytes
 // a row by TMA into a ring, warp 1 issues four products a block, warps 2-5 bring the scale factors into tensor memory and
-// store the split partial (a warp's lanes are consecutive columns). Values that are not finite become NaN, and so does
-// every output of their row.
+// store the split partial (a warp's lanes are consecutive columns). Up to 8 rows warps 2-5 bring X's tiles into 8 bits
+// themselves (TX its type; every band of 128 features does it again), a launch less: %FUSED%. Values
+// that are not finite become NaN, and so does every output of their row.
 #pragma once
 
 #include "project.cuh"
@@ -62,6 +63,41 @@ __device__ __forceinline__ uint32_t f8_pack4(const float* v, float s) {
   return (uint32_t)lo | ((uint32_t)hi << 16);
 }
 
+// 8 consecutive values of a lane as e4m3 bytes, and the exponent of their block, which 16 consecutive lanes hold (all 32
+// take part; `in`: this lane has values).
+__device__ __forceinline__ uint2 f8_quant8(const float* v, bool in, int* e) {
+  uint32_t mx = 0u;
+  if (in) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mx = max(mx, f8_bits(v[j]));
+  }
+  uint32_t top = mx;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const bool odd = __any_sync(0xffffffffu, mx >= 0x7f800000u);  // a value of the warp that is not finite
+  if (odd) {  // the largest finite one decides
+    top = 0u;
+    if (in) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, f8_bits(v[j]) < 0x7f800000u ? f8_bits(v[j]) : 0u);
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  }
+  uint2 p = make_uint2(0u, 0u);
+  *e = f8_exponent(top);
+  if (!in) return p;
+  const float s = f8_exp2i(-*e);
+  p.x = f8_pack4(v, s);
+  p.y = f8_pack4(v + 4, s);
+  if (odd) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (f8_bits(v[j]) >= 0x7f800000u) (j < 4 ? p.x : p.y) |= 0x7fu << (8 * (j & 3));
+  }
+  return p;
+}
+
 // What the projection takes of a row besides its 8-bit form (project_in): 1/rms and the gate.
 struct F8RowStats {
   int rms;
@@ -100,36 +136,9 @@ __global__ void __launch_bounds__(F8Q_THREADS) quant_f8_kernel(const T* __restri
     for (int u = 0; u < F8Q_UNROLL; ++u) {
       const int k = k0 + (u * F8Q_THREADS + (int)threadIdx.x) * 8;
       if (k0 + u * F8Q_THREADS * 8 >= kp) break;
-      uint32_t mx = 0u;
-      if (k < kp) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) mx = max(mx, f8_bits(v[u][j]));
-      }
-      uint32_t top = mx;
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const bool odd = __any_sync(0xffffffffu, mx >= 0x7f800000u);  // a value of the warp that is not finite
-      if (odd) {  // the largest finite one decides
-        uint32_t fin = 0u;
-        if (k < kp) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) fin = max(fin, f8_bits(v[u][j]) < 0x7f800000u ? f8_bits(v[u][j]) : 0u);
-        }
-        top = fin;
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      }
+      int e;
+      const uint2 p = f8_quant8(v[u], k < kp, &e);
       if (k >= kp) continue;
-      const int e = f8_exponent(top);
-      const float s = f8_exp2i(-e);
-      uint2 p;
-      p.x = f8_pack4(v[u], s);
-      p.y = f8_pack4(v[u] + 4, s);
-      if (odd) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (f8_bits(v[u][j]) >= 0x7f800000u) (j < 4 ? p.x : p.y) |= 0x7fu << (8 * (j & 3));
-      }
       *reinterpret_cast<uint2*>(x8 + m * kp + k) = p;
       if ((threadIdx.x & 15) == 0) scale[m * stride + k / F8_BK] = (uint8_t)(e + 127);
       if (st.rstd) {
@@ -196,13 +205,23 @@ struct F8Args {
   int sw_words;       // W's rows too
   float* part;
   int* row_done;
+  const void* x;  // TX [M, K]: the rows as they are
+  int K, vec;
 };
 
-template <int BN>
+// X's factors lie behind W's: a word of four blocks like W's, or (TX) a word of one block, in BN / 32 columns.
+constexpr int F8_FUSED_ROWS = 8;
+constexpr int F8_MAX_FUSED = 120;  // blocks of a split then
+
+template <int BN, typename TX>
 __global__ void __launch_bounds__(F8_THREADS, 1) gemm_f8_kernel(const __grid_constant__ CUtensorMap map_w,
                                                                 const __grid_constant__ CUtensorMap map_x,
                                                                 const F8Args a) {
   constexpr int STAGES = f8_stages(BN), STAGE = f8_stage(BN);
+  constexpr bool FUSED = !std::is_void<TX>::value;
+  static_assert(!FUSED || BN == 64, "two columns of X's factors a block");
+  constexpr int WCOLS = FUSED ? 4 : f8_word_cols(BN);
+  __shared__ uint8_t xs_sh[FUSED ? 8 * F8_FUSED_ROWS : 1];
   extern __shared__ unsigned char f8_smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(f8_smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE);
@@ -217,12 +236,13 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_f8_kernel(const __grid_con
   const int64_t m0 = (int64_t)blockIdx.y * BN;
   const int b0 = blockIdx.z * a.bps, b1 = min(a.nb, b0 + a.bps);
   const int nkb = max(0, b1 - b0), w0 = b0 / 4;
+  const int words = nkb > 0 ? (b1 - 1) / 4 - w0 + 1 : 0;
 
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_w);
     prefetch_tensormap(&map_x);
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&full[i], 1);
+      mbar_init(&full[i], FUSED ? 5 : 1);
       mbar_init(&sfree[i], 1);
     }
     mbar_init(done, 1);
@@ -252,7 +272,7 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_f8_kernel(const __grid_con
     if (lane == 0) {
       const uint64_t keep = policy_evict_last();
       for (int kb = 0; kb < npre; ++kb) {
-        mbar_arrive_expect_tx(&full[kb], STAGE);
+        mbar_arrive_expect_tx(&full[kb], FUSED ? F8_BM * F8_BK : STAGE);
         tma_load_2d_hint(smem + kb * STAGE, &map_w, (b0 + kb) * F8_BK, n0, &full[kb], keep);
       }
       pdl_wait();
@@ -265,10 +285,10 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_f8_kernel(const __grid_con
         if (use > 0 && (!mbar_wait_spin(&sfree[s], (use - 1) & 1) || *abort_flag)) { *abort_flag = 1; break; }
         unsigned char* st = smem + s * STAGE;
         if (kb >= npre) {
-          mbar_arrive_expect_tx(&full[s], STAGE);
+          mbar_arrive_expect_tx(&full[s], FUSED ? F8_BM * F8_BK : STAGE);
           tma_load_2d_hint(st, &map_w, (b0 + kb) * F8_BK, n0, &full[s], keep);
         }
-        tma_load_2d(st + F8_BM * F8_BK, &map_x, (b0 + kb) * F8_BK, (int)m0, &full[s]);
+        if (!FUSED) tma_load_2d(st + F8_BM * F8_BK, &map_x, (b0 + kb) * F8_BK, (int)m0, &full[s]);
         used = kb + 1;
       }
       // after a wait that ran out: the copies in flight end before the CTA's shared memory goes away
@@ -290,12 +310,14 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_f8_kernel(const __grid_con
         tc_fence_after();
         const uint32_t sb = smem_u32(smem + s * STAGE);
         const int b = b0 + kb, word = b / 4 - w0;
-        const uint32_t sa = taddr + BN + word * f8_word_cols(BN);
-        const uint32_t idesc = f8_idesc(BN, 0) | ((uint32_t)(b & 3) << 4) | ((uint32_t)(b & 3) << 29);
+        if (FUSED) fence_proxy_async_smem();  // X's tile was written by this CTA's threads
+        const uint32_t sa = taddr + BN + word * WCOLS;
+        const uint32_t sx = FUSED ? taddr + BN + words * WCOLS + kb * (BN / 32) : sa + 4;
+        const uint32_t idesc = f8_idesc(BN, 0) | (FUSED ? 0u : (uint32_t)(b & 3) << 4) | ((uint32_t)(b & 3) << 29);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)  // 32 columns: 32 bytes along the swizzle row
           tc_mma_mx8(taddr, umma_desc_k_sw128(sb + ks * 32), umma_desc_k_sw128(sb + F8_BM * F8_BK + ks * 32), idesc, sa,
-                     sa + 4, kb > 0 || ks > 0);
+                     sx, kb > 0 || ks > 0);
         tc_commit(&sfree[s]);
       }
       if (!ok) *abort_flag = 1;
@@ -305,40 +327,109 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_f8_kernel(const __grid_con
   } else {
     const int q = warp & 3;  // TMEM lane quarter of this warp
     const uint32_t tl = taddr + ((uint32_t)(q * 32) << 16);
+    const int rows = (int)min((int64_t)BN, a.M - m0);
+    // FUSED: thread t holds 8 values of row t / 16 in each of 8 blocks; the first are on their way before W's factors
+    const int t = threadIdx.x - 64, xr = t >> 4, xk = (t & 15) * 8;
+    float v[FUSED ? 8 : 1][8];
+    auto load = [&](int kb) {
+      if constexpr (FUSED) {
+        const TX* x = static_cast<const TX*>(a.x) + (m0 + xr) * a.K;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+          if (xr < rows && kb + i < nkb) f8_load8<TX>(x, (b0 + kb + i) * F8_BK + xk, a.K, a.vec, v[i]);
+        }
+      }
+    };
+    if (FUSED && nkb > 0) load(0);
     // scale words: row 32 j + lane in column j, the same in every lane quarter
-    const int words = nkb > 0 ? (b1 - 1) / 4 - w0 + 1 : 0;
     for (int w = 0; w < words; ++w) {
-      uint32_t u[f8_word_cols(BN)];
+      uint32_t u[WCOLS];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int n = n0 + j * 32 + lane;
         u[j] = n < a.N ? f8_scale_word(a.sw + (int64_t)n * a.nb, a.nb, w0 + w, a.sw_words) : 0x7f7f7f7fu;
       }
 #pragma unroll
-      for (int j = 0; j < BN / 32; ++j) {
+      for (int j = 0; j < WCOLS - 4; ++j) {
         const int64_t m = m0 + j * 32 + lane;
         u[4 + j] = m < a.M ? f8_scale_word(a.sx + m * a.sx_stride, a.nb, w0 + w, true) : 0x7f7f7f7fu;
       }
 #pragma unroll
-      for (int j = 0; j < f8_word_cols(BN); ++j) tc_st1(tl + BN + w * f8_word_cols(BN) + j, u[j]);
+      for (int j = 0; j < WCOLS; ++j) tc_st1(tl + BN + w * WCOLS + j, u[j]);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sf_ready[w]);
       __syncwarp();
     }
+    if constexpr (FUSED) {
+      static_assert(!FUSED || STAGES == 8, "a round of 8 blocks fills the ring");
+      for (int kb = 0; kb < nkb; kb += 8) {
+        const int n = min(8, nkb - kb);
+        if (kb > 0) {
+          for (int i = 0; i < n; ++i)
+            if (!*abort_flag && !mbar_wait_spin(&sfree[i], (kb / 8 - 1) & 1)) *abort_flag = 1;
+          __syncwarp();
+        }
+        // (the eight blocks' reductions side by side)
+        uint32_t top[8], any = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          top[i] = 0u;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) top[i] = max(top[i], f8_bits(v[i][j]));
+          any = max(any, top[i]);
+        }
+        const bool odd = __any_sync(0xffffffffu, any >= 0x7f800000u);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) top[i] = max(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {  // 16-byte chunk c of row r at chunk c ^ (r % 8)
+          int e = f8_exponent(top[i]);
+          uint2 p;
+          if (odd) {
+            p = f8_quant8(v[i], true, &e);
+          } else {
+            const float sc = f8_exp2i(-e);
+            p = make_uint2(f8_pack4(v[i], sc), f8_pack4(v[i] + 4, sc));
+          }
+          if (xr < rows && i < n) {
+            unsigned char* tile = smem + i * STAGE + F8_BM * F8_BK;
+            *reinterpret_cast<uint2*>(tile + xr * F8_BK + (((xk >> 4) ^ xr) << 4) + (xk & 8)) = p;
+            if ((t & 15) == 0) xs_sh[i * F8_FUSED_ROWS + xr] = (uint8_t)(e + 127);
+          }
+        }
+        if (kb + 8 < nkb) load(kb + 8);
+        fence_proxy_async_smem();
+        named_bar_sync(1, 128);
+        for (int i = 0; i < n; ++i) {
+          const uint32_t at = tl + BN + words * WCOLS + (kb + i) * (BN / 32);
+          tc_st1(at, lane < rows ? xs_sh[i * F8_FUSED_ROWS + lane] : 127u);
+          tc_st1(at + 1, 127u);
+        }
+        tc_wait_st();
+        tc_fence_before();
+        named_bar_sync(1, 128);  // (every warp has read the bytes; the next round writes them)
+        if (lane == 0)
+          for (int i = 0; i < n; ++i) mbar_arrive(&full[i]);
+        __syncwarp();
+      }
+    }
     const int n = n0 + q * 32 + lane;
     float* out = a.part + (int64_t)blockIdx.z * a.M * a.N;
-    const int rows = (int)min((int64_t)BN, a.M - m0);
     const bool ok = nkb > 0 && mbar_wait_bounded(done, 0) && !*abort_flag;
     __syncwarp();
     tc_fence_after();
     for (int c = 0; c < rows; c += 32) {
-      float v[32];
-      tc_ld32(tl + (uint32_t)c, v);
+      float y[32];
+      tc_ld32(tl + (uint32_t)c, y);
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        if (c + i < rows && n < a.N) out[(m0 + c + i) * a.N + n] = ok ? v[i] : 0.f;
+        if (c + i < rows && n < a.N) out[(m0 + c + i) * a.N + n] = ok ? y[i] : 0.f;
     }
   }
   tc_fence_before();

@@ -12,7 +12,8 @@
 //                brings q into 16 bits, a power of two per row (f16's range)
 //   mass_scores  a cluster of ceil(page_rows / 256) CTAs per tile, each with up to 256 of the page's slots:
 //                S[pairs, slots] = Q . K^T on the tensor cores (pairs as the 128-row operand), chunk softmax, column sums
-//   mass_combine a page's tiles added in order, with the prior
+//                (all a page's tiles, in their order and with the prior, are added up by the CTA that finishes its part of
+//                the page last; pages that nothing reads are mass_rows')
 //
 // In mass_scores the slots arrive by TMA, the pairs' rows of Q by 16-byte asynchronous copies (128 rows anywhere in the
 // batch, so no row is copied in memory for each of its pairs). A pair is a TMEM lane, so the maximum and the sum of its
@@ -56,7 +57,8 @@ __host__ __device__ constexpr size_t ms_smem(int terms, int cs) {
 }
 
 struct __align__(16) MassTile {
-  int page, start, count, nv;  // pairs [start, start + count) in grouped order; nv: the most valid slots of the page
+  int page, start, count, nv;    // pairs [start, start + count) in grouped order; nv: the most valid slots of the page
+  int total, base, stride, few;  // tiles of the page: base + j * stride for j < total, the last one `few` if that is not -1
 };
 
 struct MassArgs {
@@ -70,8 +72,7 @@ struct MassArgs {
   int* cnt;       // [n_pages]: pairs per page
   int* nvmax;     // [n_pages]
   int* start;     // [n_pages]: the page's first place
-  int* tile0;     // [n_pages]: its first tile of more than MS_FEW pairs
-  int* few;       // [n_pages]: its tile of fewer, -1: none
+  int* done;      // [n_pages, cs]: tiles that are finished
   int* page;      // [n_pairs]: page of a pair, -1: reads nothing
   int* prow;      // [n_pairs] by place: row of q
   int* pnv;       // [n_pairs] by place: valid slots
@@ -156,12 +157,11 @@ __global__ void __launch_bounds__(MS_PLAN_THREADS) mass_plan_kernel(const MassAr
   for (int p = p0; p < p1; ++p) {
     const int c = a.cnt[p];
     a.start[p] = at;
-    a.tile0[p] = tb;
-    a.few[p] = -1;
+    const int left = c % MS_M, total = (c + MS_M - 1) / MS_M, base = tb;
+    const int few = left > 0 && left <= MS_FEW ? tf++ : -1;
     for (int s = 0; s < c; s += MS_M) {
       const int n = min(MS_M, c - s);
-      if (n <= MS_FEW) a.few[p] = tf;
-      a.tiles[n <= MS_FEW ? tf++ : tb++] = MassTile{p, at + s, n, a.nvmax[p]};
+      a.tiles[few >= 0 && n < MS_M ? few : tb++] = MassTile{p, at + s, n, a.nvmax[p], total, base, 1, few};
     }
     at += c;
   }
@@ -197,6 +197,7 @@ __device__ __forceinline__ void ms_order(const MassArgs& a, int p) {
   __shared__ int sh[MS_ROWS_THREADS / 32];
   __shared__ int nv_most;
   if (threadIdx.x == 0) nv_most = 0;
+  if (threadIdx.x < a.cs) a.done[p * a.cs + threadIdx.x] = 0;
   const int n = a.direct ? a.n_pairs : a.cnt[p];
   const int64_t start = a.direct ? (int64_t)p * a.n_pairs : a.start[p];
   int found = 0;
@@ -236,14 +237,19 @@ __device__ __forceinline__ void ms_order(const MassArgs& a, int p) {
       if (a.direct) atomicMax(&nv_most, nv);
     }
   }
+  if (found == 0)
+    for (int i = threadIdx.x; i < a.page_rows; i += MS_ROWS_THREADS) {
+      const int64_t at = (int64_t)p * a.page_rows + i;
+      a.mass[at] = a.prior ? a.decay * a.prior[at] : 0.f;
+    }
   if (!a.direct) return;
   __syncthreads();
-  const int per = a.slots / a.n_pages;
+  const int per = a.slots / a.n_pages, total = (found + MS_M - 1) / MS_M;
   if (threadIdx.x < per) {
     const int s = threadIdx.x * MS_M;
-    a.tiles[threadIdx.x * a.n_pages + p] = MassTile{p, (int)(start + s), max(0, min(MS_M, found - s)), nv_most};
+    a.tiles[threadIdx.x * a.n_pages + p] =
+        MassTile{p, (int)(start + s), max(0, min(MS_M, found - s)), nv_most, total, p, a.n_pages, -1};
   }
-  if (threadIdx.x == 0) a.cnt[p] = found;
 }
 
 // CTAs 0 .. n_pages - 1: a page's pairs; the others: a row of q each.
@@ -329,7 +335,7 @@ struct MsSmem {
   float* xch;    // [2][64][MS_XPITCH]: sums of the lo rows of few pairs
   uint64_t *full, *empty, *s_full, *s_empty, *st;
   uint32_t* tmem;
-  volatile int* abort_flag;
+  volatile int *abort_flag, *last;
 };
 
 template <typename T, int TERMS>
@@ -351,6 +357,7 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
   s.st = s.s_empty + 2;
   s.tmem = reinterpret_cast<uint32_t*>(s.st + 2);
   s.abort_flag = reinterpret_cast<volatile int*>(s.tmem + 1);
+  s.last = s.abort_flag + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank();
   const int cluster = blockIdx.x / cs, n_clusters = gridDim.x / cs;
@@ -622,12 +629,32 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
       }
       named_bar_sync(1, 32 * MS_EPI);
       const int col = (int)threadIdx.x - 32 * MS_LOW;
-      if (col < a.per && seg0 + col < a.page_rows) {
-        float sum = s.cols[col];
+      const bool mine = col < a.per && seg0 + col < a.page_rows;
+      float sum = 0.f;
+      if (mine) {
+        sum = s.cols[col];
 #pragma unroll
         for (int g = 1; g < 4; ++g) sum += s.cols[g * MS_N + col];
-        a.part[(int64_t)t * a.page_rows + seg0 + col] = sum;
       }
+      const int64_t at = (int64_t)tile.page * a.page_rows + seg0 + col;
+      bool last = tile.total == 1;
+      if (!last) {
+        if (mine) a.part[(int64_t)t * a.page_rows + seg0 + col] = sum;
+        __threadfence();
+        named_bar_sync(1, 32 * MS_EPI);  // (the CTA's part of the tile is written; the column sums are read)
+        if (col == 0) *s.last = atomicAdd(&a.done[tile.page * cs + rank], 1) == tile.total - 1;
+        named_bar_sync(1, 32 * MS_EPI);
+        last = *s.last;
+        if (last && mine) {
+          __threadfence();
+          sum = 0.f;
+          for (int j = 0; j < tile.total; ++j) {
+            const int tj = j == tile.total - 1 && tile.few >= 0 ? tile.few : tile.base + j * tile.stride;
+            sum += __ldcg(a.part + (int64_t)tj * a.page_rows + seg0 + col);
+          }
+        }
+      }
+      if (last && mine) a.mass[at] = a.prior ? fmaf(a.decay, a.prior[at], sum) : sum;
       named_bar_sync(1, 32 * MS_EPI);
       ++gen;
     }
@@ -639,27 +666,6 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
   cluster_sync_all();  // no CTA leaves while another may still write to its shared memory
   tc_fence_after();
   if (warp == 1) tc_dealloc(taddr, 512);
-}
-
-// mass = decay * prior + a page's tiles in order. Grid (n_pages, ceil(page_rows / 256)).
-__global__ void __launch_bounds__(256) mass_combine_kernel(const MassArgs a) {
-  pdl_wait();
-  const int p = blockIdx.x, n = blockIdx.y * 256 + threadIdx.x;
-  if (n >= a.page_rows) return;
-  const int64_t at = (int64_t)p * a.page_rows + n;
-  float v = a.prior ? a.decay * a.prior[at] : 0.f;
-  const int c = a.cnt[p];
-  if (a.direct) {
-    const float* part = a.part + (int64_t)p * a.page_rows + n;
-    for (int t = 0; t * MS_M < c; ++t) v += part[(int64_t)t * a.n_pages * a.page_rows];
-  } else {
-    const int big = c / MS_M + (c % MS_M > MS_FEW);
-    const float* part = a.part + (int64_t)a.tile0[p] * a.page_rows + n;
-#pragma unroll 4
-    for (int t = 0; t < big; ++t) v += part[(int64_t)t * a.page_rows];
-    if (c > 0 && a.few[p] >= 0) v += a.part[(int64_t)a.few[p] * a.page_rows + n];
-  }
-  a.mass[at] = v;
 }
 
 }  // namespace xencb

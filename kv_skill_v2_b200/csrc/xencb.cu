@@ -365,7 +365,7 @@ F8Plan plan_f8(int64_t M, int N, int K, int sms) {
   const int64_t tiles = ((int64_t)(N + F8_BM - 1) / F8_BM) * ((M + p.bn - 1) / p.bn);
   const int64_t s = std::min<int64_t>(std::max<int64_t>(1, sms / tiles), p.nb);
   // (blocks b0 .. b0 + bps - 1 lie in at most (bps + 6) / 4 words of scale factors)
-  p.bps = std::min((int)((p.nb + s - 1) / s), 4 * f8_max_words(p.bn) - 6);
+  p.bps = std::min((int)((p.nb + s - 1) / s), M <= F8_FUSED_ROWS ? F8_MAX_FUSED : 4 * f8_max_words(p.bn) - 6);
   p.gp.tc = true;
   p.gp.kps = p.bps * F8_BK;
   p.gp.splits = (p.nb + p.bps - 1) / p.bps;
@@ -400,9 +400,9 @@ int launch_quant_f8(const void* x, int dtype, int64_t M, int K, void* x8, uint8_
   }
 }
 
-template <int BN>
+template <int BN, typename TX>
 int run_gemm_f8(const CUtensorMap& mw, const CUtensorMap& mx, const F8Args& a, int splits, cudaStream_t st) {
-  auto kern = gemm_f8_kernel<BN>;
+  auto kern = gemm_f8_kernel<BN, TX>;
   int rc = ensure_smem(kern, (int)f8_smem(BN));
   if (rc) return rc;
   const dim3 grid((a.N + F8_BM - 1) / F8_BM, (unsigned)((a.M + BN - 1) / BN), splits);
@@ -416,17 +416,25 @@ int launch_gemm_f8(const void* X, int dtype, int64_t M, int K, const Weight8& w,
                    int* row_done, cudaStream_t st) {
   uint8_t* x8 = reinterpret_cast<uint8_t*>(ws + p.out_bytes);
   uint8_t* sx = x8 + p.x8_bytes;
-  int rc = launch_quant_f8(X, dtype, M, K, x8, sx, p.sx_stride, F8RowStats{}, st);
-  if (rc) return rc;
   const uint64_t kp = (uint64_t)p.nb * F8_BK;
   CUtensorMap mw, mx;
-  rc = tensor_map_2d(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w.w, kp, (uint64_t)N, kp, F8_BK, F8_BM);
+  int rc = tensor_map_2d(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, w.w, kp, (uint64_t)N, kp, F8_BK, F8_BM);
+  if (rc) return rc;
+  F8Args a{M, N, p.nb, p.bps, w.scale, sx, p.sx_stride, w.words(p.nb), reinterpret_cast<float*>(ws), row_done,
+           X, K, K % 8 == 0 && aligned(X, 16)};
+  if (M <= F8_FUSED_ROWS) {  // (X's map is not used)
+    switch (dtype) {
+      case XENCB_F32: return run_gemm_f8<64, float>(mw, mw, a, p.gp.splits, st);
+      case XENCB_F16: return run_gemm_f8<64, __half>(mw, mw, a, p.gp.splits, st);
+      default: return run_gemm_f8<64, __nv_bfloat16>(mw, mw, a, p.gp.splits, st);
+    }
+  }
+  rc = launch_quant_f8(X, dtype, M, K, x8, sx, p.sx_stride, F8RowStats{}, st);
   if (!rc) rc = tensor_map_2d(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, x8, kp, (uint64_t)M, kp, F8_BK, (uint32_t)p.bn);
   if (rc) return rc;
-  const F8Args a{M, N, p.nb, p.bps, w.scale, sx, p.sx_stride, w.words(p.nb), reinterpret_cast<float*>(ws), row_done};
-  if (p.bn == 64) return run_gemm_f8<64>(mw, mx, a, p.gp.splits, st);
-  if (p.bn == 128) return run_gemm_f8<128>(mw, mx, a, p.gp.splits, st);
-  return run_gemm_f8<256>(mw, mx, a, p.gp.splits, st);
+  if (p.bn == 64) return run_gemm_f8<64, void>(mw, mx, a, p.gp.splits, st);
+  if (p.bn == 128) return run_gemm_f8<128, void>(mw, mx, a, p.gp.splits, st);
+  return run_gemm_f8<256, void>(mw, mx, a, p.gp.splits, st);
 }
 
 // X (in 8 bits already, behind p.out_bytes of ws) times W with the projection's end in the product's epilogue. a: mul,
@@ -1040,7 +1048,7 @@ int plan_mass(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows, in
   p->q = align_up((size_t)p->terms * n_rows * d_s * 2, 256);
   p->rinv = align_up((size_t)n_rows * 4, 256);
   p->part = align_up((size_t)p->max_tiles * page_rows * 4, 256);
-  p->total = 5 * p->pages + p->pair + 3 * p->place + p->tiles + 256 + p->q + p->rinv + p->part;
+  p->total = (3 + p->cs) * p->pages + p->pair + 3 * p->place + p->tiles + 256 + p->q + p->rinv + p->part;
   return XENCB_OK;
 }
 
@@ -1104,8 +1112,6 @@ int run_mass(const void* q, int q_dtype, const MassPlan& p, const MassArgs& a, c
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   (void)cudaLaunchKernelEx(&cfg, kern, mk, a);
   XENCB_CHECK_LAUNCH("mass_scores launch");
-  launch_pdl(mass_combine_kernel, dim3((unsigned)a.n_pages, (unsigned)((a.page_rows + 255) / 256)), dim3(256), 0, st, a);
-  XENCB_CHECK_LAUNCH("mass_combine launch");
   return XENCB_OK;
 }
 }  // namespace
@@ -1980,8 +1986,7 @@ int xencb_read_mass(const void* q, int q_dtype, int64_t n_rows, int d_s, const v
   a.cnt = reinterpret_cast<int*>(take(p.pages));
   a.nvmax = reinterpret_cast<int*>(take(p.pages));
   a.start = reinterpret_cast<int*>(take(p.pages));
-  a.tile0 = reinterpret_cast<int*>(take(p.pages));
-  a.few = reinterpret_cast<int*>(take(p.pages));
+  a.done = reinterpret_cast<int*>(take(p.cs * p.pages));
   a.page = reinterpret_cast<int*>(take(p.pair));
   a.prow = reinterpret_cast<int*>(take(p.place));
   a.pnv = reinterpret_cast<int*>(take(p.place));
