@@ -111,7 +111,7 @@ struct F8RowStats {
 
 // One CTA per row, 16 threads a block of 128 columns (8 values each, F8Q_UNROLL blocks' loads in flight). x8 rows are
 // kp = 128 ceil(K / 128) bytes, zeros behind column K; scale[row * stride + b] = e + 127.
-constexpr int F8Q_THREADS = 256;
+constexpr int F8Q_THREADS = 128;
 constexpr int F8Q_UNROLL = 4;
 
 template <typename T>

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import struct
 from dataclasses import dataclass
 from typing import Optional
 
@@ -1013,27 +1014,35 @@ def library_build(rows: torch.Tensor, counts, *, page_rows: Optional[int] = None
 
 # ------------------------------------------------------------------------------------------------ pages
 def _pool_args(what: str, pools, page_of: torch.Tensor, n_valid: torch.Tensor, n_chunks_of):
-    """(device, pointer array, row-byte array, n_pages, page_rows) of pools that one page table describes."""
+    """(device, pool addresses, row bytes (host arrays), n_pages, page_rows) of pools that one page table describes."""
     pools = list(pools)
     if not pools:
         raise ValueError(f"{what}: at least one pool is required")
     dev = _cuda(what, *pools, page_of, n_valid, n_chunks_of)
     P, N_rows = pools[0].shape[:2]
+    ptrs, sizes = [], []
     for p in pools:
+        shape = p.shape
         if p.dtype not in _DT:
             raise ValueError(f"{what}: pool dtype {p.dtype} not supported (float32 / float16 / bfloat16)")
-        if p.dim() != 3 or p.shape[0] != P or p.shape[1] != N_rows or not p.is_contiguous():
+        if len(shape) != 3 or shape[0] != P or shape[1] != N_rows or not p.is_contiguous():
             raise ValueError(f"{what}: pools must be contiguous [pages, page_rows, d] tensors with the same pages, got "
-                             f"{tuple(p.shape)} beside {tuple(pools[0].shape)}")
+                             f"{tuple(shape)} beside {tuple(pools[0].shape)}")
+        ptrs.append(p.data_ptr())
+        sizes.append(shape[2] * p.element_size())
+    table = page_of.shape
     for name, t in (("page_of", page_of), ("n_valid", n_valid)):
-        if t.dtype != torch.int32 or t.dim() != 2 or t.shape != page_of.shape or not t.is_contiguous():
+        if t.dtype != torch.int32 or len(table) != 2 or t.shape != table or not t.is_contiguous():
             raise ValueError(f"{what}: {name} must be a contiguous int32 [n_lib, C] tensor")
-    if n_chunks_of is not None and (n_chunks_of.dtype != torch.int32 or n_chunks_of.numel() != page_of.shape[0]
+    if n_chunks_of is not None and (n_chunks_of.dtype != torch.int32 or n_chunks_of.numel() != table[0]
                                     or not n_chunks_of.is_contiguous()):
         raise ValueError(f"{what}: n_chunks_of must be a contiguous int32 [n_lib] tensor")
-    ptrs = (ctypes.c_void_p * len(pools))(*[p.data_ptr() for p in pools])
-    sizes = (ctypes.c_int64 * len(pools))(*[p.shape[2] * p.element_size() for p in pools])
-    return dev, ptrs, sizes, P, N_rows
+    return dev, _words(ptrs), _words(sizes), P, N_rows
+
+
+def _words(values) -> bytes:
+    """A host array of 64-bit words, as a pointer argument takes it."""
+    return struct.pack(f"{len(values)}Q", *values)
 
 
 def pages_fork(pools, page_of: torch.Tensor, n_valid: torch.Tensor, parents: torch.Tensor, own_from: torch.Tensor, *,
@@ -1059,7 +1068,7 @@ def pages_fork(pools, page_of: torch.Tensor, n_valid: torch.Tensor, parents: tor
     missing = torch.empty(1, dtype=torch.int32, device=dev)
     with _on_device(dev):
         ws = _workspace(N.lib().xencb_pages_fork_workspace(m, C), dev)
-        N.call("xencb_pages_fork", ptrs, sizes, len(ptrs), P, page_rows, _ptr(page_of), _ptr(n_valid), C,
+        N.call("xencb_pages_fork", ptrs, sizes, len(ptrs) // 8, P, page_rows, _ptr(page_of), _ptr(n_valid), C,
                _ptr(n_chunks_of), n_lib, _ptr(parents), _ptr(own_from), m, _ptr(child), _ptr(missing), _ptr(ws),
                ws.numel(), _stream(dev))
     return child, missing
@@ -1078,7 +1087,7 @@ def pages_compact(pools, page_of: torch.Tensor, n_valid: torch.Tensor, *,
     n_live = torch.empty(1, dtype=torch.int32, device=dev)
     with _on_device(dev):
         ws = _workspace(N.lib().xencb_pages_compact_workspace(P), dev)
-        N.call("xencb_pages_compact", ptrs, sizes, len(ptrs), P, page_rows, _ptr(page_of), _ptr(n_valid), C,
+        N.call("xencb_pages_compact", ptrs, sizes, len(ptrs) // 8, P, page_rows, _ptr(page_of), _ptr(n_valid), C,
                _ptr(n_chunks_of), n_lib, _ptr(out), _ptr(n_live), _ptr(ws), ws.numel(), _stream(dev))
     return out, n_live
 
@@ -1122,16 +1131,21 @@ def pages_evict(pools, page_of: torch.Tensor, n_valid: torch.Tensor, mass: torch
         raise ValueError(f"pages_evict: floor={floor} must not be negative")
     if N_rows > 4096:
         raise NotImplementedError(f"pages_evict: pages of {N_rows} rows, at most 4096 are supported")
-    out = pools if page_rows is None else [torch.empty(P, rows, p.shape[2], dtype=p.dtype, device=dev) for p in pools]
-    optrs = (ctypes.c_void_p * len(out))(*[p.data_ptr() for p in out])
+    if page_rows is None:
+        out, optrs = pools, ptrs
+    else:
+        out = [torch.empty((P, rows, p.shape[2]), dtype=p.dtype, device=dev) for p in pools]
+        optrs = _words([p.data_ptr() for p in out])
     nv = torch.empty_like(n_valid)
-    new_mass = torch.empty(P, rows, dtype=torch.float32, device=dev)
-    kept = torch.empty(P, rows, dtype=torch.int32, device=dev)
+    new_mass = torch.empty((P, rows), dtype=torch.float32, device=dev)
+    kept = torch.empty((P, rows), dtype=torch.int32, device=dev)
+    whole = int(bool(per_library))
     with _on_device(dev):
-        ws = _workspace(_workspace_bytes(dev, "xencb_pages_evict_workspace", P, N_rows, int(bool(per_library))), dev)
-        N.call("xencb_pages_evict", ptrs, optrs, sizes, len(ptrs), P, N_rows, rows, _ptr(page_of), _ptr(n_valid), C,
-               _ptr(n_chunks_of), n_lib, _ptr(mass), _ptr(keep), keep_all, int(bool(per_library)), min(int(floor), N_rows),
-               _ptr(nv), _ptr(new_mass), _ptr(kept), _ptr(ws), ws.numel(), _stream(dev))
+        ws_bytes = _workspace_bytes(dev, "xencb_pages_evict_workspace", P, N_rows, whole)
+        ws = _workspace(ws_bytes, dev)
+        N.call("xencb_pages_evict", ptrs, optrs, sizes, len(pools), P, N_rows, rows, page_of.data_ptr(), n_valid.data_ptr(),
+               C, _ptr(n_chunks_of), n_lib, mass.data_ptr(), _ptr(keep), keep_all, whole, min(int(floor), N_rows),
+               nv.data_ptr(), new_mass.data_ptr(), kept.data_ptr(), ws.data_ptr(), ws_bytes, _stream(dev))
     return nv, new_mass, kept, out
 
 
