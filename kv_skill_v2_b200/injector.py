@@ -88,6 +88,10 @@ class ExternalSkillInjector:
         # projection weights in the 3xF16 form (ops.weights_prep), keyed by storage, version and shape; each
         # entry keeps its source tensor alive so the key cannot be reused by another tensor
         self.gemm_f16x3 = True
+        # the projections in 8-bit floating point (ops.weights_fp8; rows quantised in the call): a quarter of the prepared
+        # weights' bytes and, for prompts, a fifth of the projections' time, at e4m3's precision. It moves the routing too, so it
+        # is the caller's choice. Not beside adapters
+        self.gemm_fp8 = False
         self._wprep: dict = {}
         # low-rank adapters of the requests of a batch (set_adapters)
         self._adapters: Optional[tuple] = None
@@ -219,6 +223,18 @@ class XEncInjector(ExternalSkillInjector):
         self._wprep[key] = (W, prep)
         return prep
 
+    def _weight(self, W: torch.Tensor):
+        """(weight, its prepared form or None) as project_in and project_out take them, for W [out, in] float32."""
+        if not self.gemm_fp8:
+            return W, self._prep(W)
+        key = (W.data_ptr(), W._version, tuple(W.shape), str(W.device), "fp8")
+        hit = self._wprep.get(key)
+        if hit is None:
+            if len(self._wprep) >= 64:
+                self._wprep.clear()
+            hit = self._wprep[key] = (W, ops.weights_fp8(W))
+        return hit[1], None
+
     def _weights_key(self) -> tuple:
         """Storage and version of every interface parameter (a captured step is valid only for these)."""
         itf = self.itf
@@ -244,7 +260,8 @@ class XEncInjector(ExternalSkillInjector):
         more = self._adapter_args(0, h2 if h is None else h)
         if isinstance(itf, LinearInterface):
             W = _on(itf.w_in.detach(), h2).float()
-            q, _, _, z = ops.project_in(h2, W, sel_w=sel_w, sel_b=sel_b, w_prep=self._prep(W), **more)
+            W, prep = self._weight(W)
+            q, _, _, z = ops.project_in(h2, W, sel_w=sel_w, sel_b=sel_b, w_prep=prep, **more)
             return q, None, None, z
         p = itf._pos[li]
         gate_w = _on(itf.gate_w.detach(), h2).float()
@@ -253,10 +270,10 @@ class XEncInjector(ExternalSkillInjector):
         lins = itf.query_weights()
         if len(lins) == 1:
             W, b = lins[0]
-            Wf = _f32_on(W, h2)
+            Wf, prep = self._weight(_f32_on(W, h2))
             q, g, _, z = ops.project_in(h2, Wf, None if b is None else _on(b.detach(), h2).float(),
                                         gate_w=gate_w, gate_b=gate_b, sel_w=sel_w, sel_b=sel_b,
-                                        w_prep=self._prep(Wf), **more)
+                                        w_prep=prep, **more)
             return q, g, gain, z
         if more:
             raise NotImplementedError("adapters need a full-rank query map (this interface's A is low-rank)")
@@ -265,12 +282,12 @@ class XEncInjector(ExternalSkillInjector):
         g = z = None
         for i, (W, b) in enumerate(lins):
             first, last = i == 0, i == len(lins) - 1
-            Wf = _f32_on(W, h2)
+            Wf, prep = self._weight(_f32_on(W, h2))
             x, g_i, _, z_i = ops.project_in(x, Wf,
                                             None if b is None else _on(b.detach(), h2).float(), rms=first, l2=last,
                                             gate_w=gate_w if first else None, gate_b=gate_b,
                                             sel_w=sel_w if first else None, sel_b=sel_b if first else None,
-                                            w_prep=self._prep(Wf))
+                                            w_prep=prep)
             if first:
                 g, z = g_i, z_i
         return x, g, gain, z
@@ -280,8 +297,8 @@ class XEncInjector(ExternalSkillInjector):
         """(q, gate | None, log_gain | None, idx, wk, w) from the fused input projection + routing of decode rows,
         or None when the interface's query map is not one linear layer (low-rank A: two projections)."""
         itf = self.itf
-        if self._adapters is not None and self._adapters[0] is not None:
-            return None  # the projection with adapters, then the routing
+        if self.gemm_fp8 or (self._adapters is not None and self._adapters[0] is not None):
+            return None  # the projection in 8 bits or with adapters, then the routing
         if isinstance(itf, LinearInterface):
             W = _on(itf.w_in.detach(), h2).float()
             q, _, _, idx, wk, w, _ = ops.project_in_route(
@@ -342,7 +359,7 @@ class XEncInjector(ExternalSkillInjector):
     def _finish(self, h, h2, r, g, scale, li, inject, sel_col=None, log_alpha=0.0, extra=None, log_scale=None):
         lead = h.shape[:-1]
         W, b = self._write_weights(h2)
-        wp = self._prep(W)
+        W, wp = self._weight(W)
         more = self._adapter_args(1, h)
         pm = self._pos_mask(h) if inject else None
         if extra is not None:  # a tensor calibration gain: fold into the per-row gate
@@ -408,6 +425,12 @@ class LibraryInjector(XEncInjector):
         self.last_route: Optional[torch.Tensor] = None
         self.record_attn = False
         self.last_attn: dict = {}
+        # record_mass: every softmax read adds the attention that its rows give to the Library's slots to slot_mass[layer]
+        # [pages, page_rows] (ops.read_mass), after mass_decay times what is there; PagedLibrary.evict goes by it. Rows
+        # whose position mask is 0 do not count
+        self.record_mass = False
+        self.mass_decay = 1.0
+        self.slot_mass: dict = {}
         self.force_attn = None
         self.force_norm_match = False
         self.training_attn = False
@@ -424,6 +447,7 @@ class LibraryInjector(XEncInjector):
 
     def load_library(self, lib) -> None:
         self._graphs.clear()
+        self.slot_mass = {}
         if lib.d_s != self.itf.d_s:
             raise ValueError(f"library d_s={lib.d_s} (encoder) != interface d_s={self.itf.d_s}")
         missing = set(self.itf.inject_layers) - set(lib.K)
@@ -453,6 +477,7 @@ class LibraryInjector(XEncInjector):
         self._graphs.clear()
         self.skill = None
         self.lib = None
+        self.slot_mass = {}
         self.mag_terms.clear()
         self.route_terms.clear()
         self.attn_terms.clear()
@@ -541,7 +566,7 @@ class LibraryInjector(XEncInjector):
         forward), a fast interface, no calibration or position mask, no attention diagnostics, no grad, not inside
         a user's capture."""
         return (self.cuda_graphs and inject and sel is None and self._fast_interface() and h.is_cuda
-                and self.calib is None and self.pos_mask is None and not self.record_attn
+                and self.calib is None and self.pos_mask is None and not self.record_attn and not self.record_mass
                 and self.force_attn is None and not torch.is_grad_enabled()
                 and not torch.cuda.is_current_stream_capturing())
 
@@ -553,6 +578,19 @@ class LibraryInjector(XEncInjector):
         k = self.top_k if 0 < self.top_k < pages.n_chunks else pages.n_chunks
         need = ops.shared_workspace(pages, h.numel() // h.shape[-1], k)
         return need > _GRAPH_WORKSPACE or (need == 0 and ops.shared_supported(pages))  # (0: more rows than one call takes)
+
+    def _add_mass(self, h: torch.Tensor, li: int, q: torch.Tensor, pages: ops.Pages, idx, wk, rpl: int) -> None:
+        """record_mass: this read's attention into slot_mass[li]."""
+        if not self.read_softmax:
+            raise ValueError("record_mass: the linear read has no attention weights")
+        if self.force_attn is not None:
+            raise ValueError("record_mass: force_attn replaces the read's attention")
+        pm = self._pos_mask(h)
+        if pm is not None:
+            wk = torch.where((pm != 0).view(-1, 1), wk, torch.zeros_like(wk))
+        mass = self.slot_mass.get(li)
+        self.slot_mass[li] = ops.read_mass(q, pages, idx, wk, rows_per_lib=rpl, read_temp=self.read_temp, mass=mass,
+                                           decay=self.mass_decay, out=mass)
 
     def _check_diagnostics(self) -> None:
         if self.training_attn and torch.is_grad_enabled():
@@ -604,7 +642,7 @@ class LibraryInjector(XEncInjector):
         pages = self._pages(li, h)
         base = (li, tuple(h.shape), tuple(h.stride()), h.dtype, h.device, id(pages), float(self.gain_scale),
                 self.top_k, float(self.read_temp), float(self.route_temp), bool(self.read_softmax),
-                self._weights_key(), bool(self.gemm_f16x3), self.share_pages, self._adapter_key())
+                self._weights_key(), bool(self.gemm_f16x3), bool(self.gemm_fp8), self.share_pages, self._adapter_key())
         ent = self._graphs.get((base, h.data_ptr()))
         if ent is None:
             ent = self._graphs.get((base, None))
@@ -685,6 +723,8 @@ class LibraryInjector(XEncInjector):
                 sel_col, log_alpha = sel_column()
             idx, wk, w, _ = ops.route(q, pages.S, rows_per_lib=rpl, top_k=self.top_k, route_temp=self.route_temp,
                                       n_chunks_of=pages.n_chunks_of, row_w=sel_col)
+        if self.record_mass:
+            self._add_mass(h, li, q, pages, idx, wk, rpl)
         # with a selector most rows read nothing at most depths: the sparse plan spreads the live rows' work
         if self.record_attn or self.force_attn is not None:
             r = self._read_with_diagnostics(h, li, q, pages, idx, wk, rpl, sparse=sel_col is not None)

@@ -401,6 +401,8 @@ class TopKLibraryInjector(LibraryInjector):
             return super()._run_lib(h, li, inject, sel)
         if self.force_attn is not None or self.training_attn:
             raise NotImplementedError("force_attn / training_attn are not served by the xencb top-k read")
+        if self.record_mass:
+            raise NotImplementedError("record_mass: the top-k read selects slots, it gives the others no attention")
         if self.tk._idx32 is None:
             raise RuntimeError("TopKLibraryInjector: no selection for this forward (the selection pass did not run)")
         self._check_forward_only(h)
