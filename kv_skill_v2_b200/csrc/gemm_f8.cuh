@@ -109,13 +109,36 @@ struct F8RowStats {
   float* gate;          // [M] or null
 };
 
-// One CTA per row, 16 threads a block of 128 columns (8 values each, F8Q_UNROLL blocks' loads in flight). x8 rows are
-// kp = 128 ceil(K / 128) bytes, zeros behind column K; scale[row * stride + b] = e + 127.
-constexpr int F8Q_THREADS = 128;
-constexpr int F8Q_UNROLL = 4;
+// One CTA per row, 16 threads a block of 128 columns (8 values each, four times as many of a thread on their way, held as
+// they came). x8 rows are kp = 128 ceil(K / 128) bytes, zeros behind column K; scale[row * stride + b] = e + 127.
+template <typename T> __host__ __device__ constexpr int f8q_threads() { return sizeof(T) == 4 ? 128 : 256; }
+
+// 8 values as they lie in memory.
+template <typename T> struct F8Raw {
+  uint4 u[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* __restrict__ row, int k, int K, bool vec) {
+    if (vec && k < K) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4*>(row + k)[i];
+    } else {
+      T t[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = k + i < K ? row[k + i] : from_f32<T>(0.f);
+      memcpy(u, t, sizeof(t));
+    }
+  }
+  __device__ __forceinline__ void values(float* v) const {
+    if constexpr (sizeof(T) == 4) {
+      unpack16<T>(u[0], v);
+      unpack16<T>(u[1], v + 4);
+    } else {
+      unpack16<T>(u[0], v);
+    }
+  }
+};
 
 template <typename T>
-__global__ void __launch_bounds__(F8Q_THREADS) quant_f8_kernel(const T* __restrict__ x, int K, int vec,
+__global__ void __launch_bounds__(f8q_threads<T>(), sizeof(T) == 4 ? 8 : 6) quant_f8_kernel(const T* __restrict__ x, int K, int vec,
                                                                uint8_t* __restrict__ x8, uint8_t* __restrict__ scale,
                                                                int stride, const F8RowStats st) {
   __shared__ float2 red[32];
@@ -125,27 +148,32 @@ __global__ void __launch_bounds__(F8Q_THREADS) quant_f8_kernel(const T* __restri
   const T* row = x + m * K;
   const int kp = (K + F8_BK - 1) / F8_BK * F8_BK;
   float ss = 0.f, gd = 0.f;
-  for (int k0 = 0; k0 < kp; k0 += F8Q_THREADS * 8 * F8Q_UNROLL) {
-    float v[F8Q_UNROLL][8];
+  constexpr int U = 4, STEP = f8q_threads<T>() * 8;
+  for (int k0 = 0; k0 < kp; k0 += STEP * U) {
+    F8Raw<T> raw[U];
 #pragma unroll
-    for (int u = 0; u < F8Q_UNROLL; ++u) {
-      const int k = k0 + (u * F8Q_THREADS + (int)threadIdx.x) * 8;
-      if (k < kp) f8_load8<T>(row, k, K, vec, v[u]);
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * STEP + (int)threadIdx.x * 8;
+      if (k < kp) raw[u].load(row, k, K, vec);
     }
 #pragma unroll
-    for (int u = 0; u < F8Q_UNROLL; ++u) {
-      const int k = k0 + (u * F8Q_THREADS + (int)threadIdx.x) * 8;
-      if (k0 + u * F8Q_THREADS * 8 >= kp) break;
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * STEP + (int)threadIdx.x * 8;
+      if (k0 + u * STEP >= kp) break;
+      float v[8];
+      raw[u].values(v);
       int e;
-      const uint2 p = f8_quant8(v[u], k < kp, &e);
+      const uint2 p = f8_quant8(v, k < kp, &e);
       if (k >= kp) continue;
       *reinterpret_cast<uint2*>(x8 + m * kp + k) = p;
       if ((threadIdx.x & 15) == 0) scale[m * stride + k / F8_BK] = (uint8_t)(e + 127);
       if (st.rstd) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          ss = fmaf(v[u][j], v[u][j], ss);
-          if (st.gate_w && k + j < K) gd = fmaf(v[u][j], __ldg(st.gate_w + k + j), gd);
+        for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
+        if (st.gate_w) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (k + j < K) gd = fmaf(v[j], __ldg(st.gate_w + k + j), gd);
         }
       }
     }

@@ -6,8 +6,8 @@
 // the column sums of the weights with which the read (xenc/injector.py:239-245) multiplies the values. The (row, routed
 // chunk) pairs are grouped by page in the order of their rows; a tile is one page with up to 128 of its pairs.
 //
-//   mass_plan    counts the pairs of each page and lays out the tiles (one CTA; more than MS_ONE_CTA pairs are counted by a
-//                grid before). Calls of up to MS_DIRECT pairs do without: every page has room for all of them
+//   mass_plan    counts the pairs of each page and lays out the tiles. Calls of up to MS_DIRECT pairs do without: every page
+//                has room for all of them
 //   mass_rows    a CTA per page lists its pairs in order, so that sums do not depend on the order of atomics; a CTA per row
 //                brings q into 16 bits, a power of two per row (f16's range)
 //   mass_scores  a cluster of ceil(page_rows / 256) CTAs per tile, each with up to 256 of the page's slots:
@@ -34,6 +34,7 @@ namespace xencb {
 
 constexpr int MS_M = 128;         // pairs of a tile
 constexpr int MS_N = 256;         // slots of a CTA at most
+constexpr int MS_MAX_CLUSTERS = 256;  // of a launch
 constexpr int MS_MAX_CS = 8;      // CTAs per cluster: pages of up to 2048 slots
 constexpr int MS_CHUNK = 4;       // blocks of 64 columns per accumulator
 constexpr int MS_ATILE = MS_M * 128;
@@ -121,55 +122,7 @@ __device__ __forceinline__ void ms_count(const MassArgs& a, unsigned first, unsi
   }
 }
 
-__global__ void __launch_bounds__(256) mass_count_kernel(const MassArgs a) {
-  ms_count(a, blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
-}
-
-// First places and tiles of the pages, by one CTA of 1024 threads. The tiles of few pairs, which take half as long, lie
-// behind all others: the clusters take the tiles in turn.
-constexpr int MS_PLAN_THREADS = 1024;
-__global__ void __launch_bounds__(MS_PLAN_THREADS) mass_plan_kernel(const MassArgs a, int counted) {
-  __shared__ int sh[32];
-  pdl_trigger();
-  if (!counted) {
-    for (int p = threadIdx.x; p < a.n_pages; p += MS_PLAN_THREADS) {
-      a.cnt[p] = 0;
-      a.nvmax[p] = 0;
-    }
-    __syncthreads();
-    ms_count(a, threadIdx.x, MS_PLAN_THREADS);
-    __syncthreads();
-  }
-  const int per = (a.n_pages + MS_PLAN_THREADS - 1) / MS_PLAN_THREADS;
-  const int p0 = min(a.n_pages, (int)threadIdx.x * per), p1 = min(a.n_pages, p0 + per);
-  int pos = 0, big = 0, few = 0;
-  for (int p = p0; p < p1; ++p) {
-    const int c = a.cnt[p], left = c % MS_M;
-    pos += c;
-    big += c / MS_M + (left > MS_FEW);
-    few += left > 0 && left <= MS_FEW;
-  }
-  int all, n_big, n_few;
-  int at = pg_scan(pos, sh, &all);
-  int tb = pg_scan(big, sh, &n_big);
-  int tf = pg_scan(few, sh, &n_few) + n_big;
-  if (threadIdx.x == 0) *a.n_tiles = n_big + n_few;
-  for (int p = p0; p < p1; ++p) {
-    const int c = a.cnt[p];
-    a.start[p] = at;
-    const int left = c % MS_M, total = (c + MS_M - 1) / MS_M, base = tb;
-    const int few = left > 0 && left <= MS_FEW ? tf++ : -1;
-    for (int s = 0; s < c; s += MS_M) {
-      const int n = min(MS_M, c - s);
-      a.tiles[few >= 0 && n < MS_M ? few : tb++] = MassTile{p, at + s, n, a.nvmax[p], total, base, 1, few};
-    }
-    at += c;
-  }
-}
-
-constexpr int MS_ROWS_THREADS = 256;
-constexpr int MS_ROWS_IDS = 16;  // pairs a thread looks at in one round
-
+constexpr int MS_THREADS_256 = 256;  // of the plan and of the rows
 // Exclusive count over the CTA's threads; *total gets the sum. `sh` holds a round's sums of the warps.
 __device__ __forceinline__ int ms_scan(int c, int* sh, int* total) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
@@ -184,13 +137,79 @@ __device__ __forceinline__ int ms_scan(int c, int* sh, int* total) {
   __syncthreads();
   int before = incl - c, all = 0;
 #pragma unroll
-  for (int w = 0; w < MS_ROWS_THREADS / 32; ++w) {
+  for (int w = 0; w < MS_THREADS_256 / 32; ++w) {
     before += w < wid ? sh[w] : 0;
     all += sh[w];
   }
   *total = all;
   return before;
 }
+
+// Counts the pairs; the CTA that ends last lays out places and tiles. The clusters take the tiles in turn (cluster c tiles
+// c, c + n_clusters, ...). Those of more than MS_FEW pairs come first; those of few pairs take about half as long: the
+// clusters that have one turn less than others get two of them before anybody else gets one, so some turns stay empty.
+constexpr int MS_PLAN_THREADS = MS_THREADS_256;
+__global__ void __launch_bounds__(MS_PLAN_THREADS) mass_plan_kernel(const MassArgs a, int n_clusters) {
+  __shared__ int sh[MS_PLAN_THREADS / 32];
+  __shared__ int last;
+  pdl_trigger();
+  if (gridDim.x == 1) {
+    for (int p = threadIdx.x; p < a.n_pages; p += MS_PLAN_THREADS) {
+      a.cnt[p] = 0;
+      a.nvmax[p] = 0;
+    }
+    __syncthreads();
+  }
+  ms_count(a, blockIdx.x * MS_PLAN_THREADS + threadIdx.x, gridDim.x * MS_PLAN_THREADS);
+  if (gridDim.x > 1) {
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(&a.nvmax[a.n_pages], 1) == (int)gridDim.x - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+  } else {
+    __syncthreads();
+  }
+  const int per = (a.n_pages + MS_PLAN_THREADS - 1) / MS_PLAN_THREADS;
+  const int p0 = min(a.n_pages, (int)threadIdx.x * per), p1 = min(a.n_pages, p0 + per);
+  int pos = 0, big = 0, few = 0;
+  for (int p = p0; p < p1; ++p) {
+    const int c = __ldcg(a.cnt + p), left = c % MS_M;
+    pos += c;
+    big += c / MS_M + (left > MS_FEW);
+    few += left > 0 && left <= MS_FEW;
+  }
+  int all, n_big, n_few;
+  int at = ms_scan(pos, sh, &all);
+  int tb = ms_scan(big, sh, &n_big);
+  int tf = ms_scan(few, sh, &n_few);
+  // the j-th tile of few pairs: `gap` clusters have a turn less, and get the first 2 gap of them
+  const int taken = n_big % n_clusters, gap = taken ? n_clusters - taken : 0, round = n_big - taken;  // (round: its first turn)
+  auto few_at = [&](int j) {
+    if (j < gap) return n_big + j;
+    if (j < 2 * gap) return round + n_clusters + taken + (j - gap);
+    return round + (gap ? 2 * n_clusters : 0) + (j - 2 * gap);
+  };
+  // (clusters without a hole in the second of these turns leave it empty)
+  if (n_few > gap)
+    for (int i = threadIdx.x; i < taken; i += MS_PLAN_THREADS) a.tiles[round + n_clusters + i].count = 0;
+  if (threadIdx.x == 0) *a.n_tiles = n_few > 0 ? few_at(n_few - 1) + 1 : n_big;
+  for (int p = p0; p < p1; ++p) {
+    const int c = __ldcg(a.cnt + p), nv = __ldcg(a.nvmax + p);
+    a.start[p] = at;
+    const int left = c % MS_M, total = (c + MS_M - 1) / MS_M, base = tb;
+    const int mine = left > 0 && left <= MS_FEW ? few_at(tf++) : -1;
+    for (int s = 0; s < c; s += MS_M) {
+      const int n = min(MS_M, c - s);
+      a.tiles[mine >= 0 && n < MS_M ? mine : tb++] = MassTile{p, at + s, n, nv, total, base, 1, mine};
+    }
+    at += c;
+  }
+}
+
+constexpr int MS_ROWS_THREADS = MS_THREADS_256;
+constexpr int MS_ROWS_IDS = 16;  // pairs a thread looks at in one round
 
 // The pairs of page p in the order of their rows.
 __device__ __forceinline__ void ms_order(const MassArgs& a, int p) {
@@ -263,7 +282,8 @@ __global__ void __launch_bounds__(MS_ROWS_THREADS) mass_rows_kernel(const MassAr
     ms_order(a, blockIdx.x);
     return;
   }
-  // (q may be read before the wait: the plan is a plain launch, so whatever wrote q has completed)
+  // (No wait: the plan is a plain launch, so whatever wrote q or used this workspace has completed, and it touches neither
+  // of the rows' outputs.)
   const int64_t row = (int64_t)blockIdx.x - a.n_pages;
   const TQ* src = q + row * a.d_s;
   constexpr int STEP = MS_ROWS_THREADS * 8, HELD = 2;  // the first HELD pieces stay in registers
@@ -294,7 +314,6 @@ __global__ void __launch_bounds__(MS_ROWS_THREADS) mass_rows_kernel(const MassAr
     for (int w = 1; w < MS_ROWS_THREADS / 32; ++w) mx = fmaxf(mx, red[w]);
     s = f16_range_scale(mx);
   }
-  pdl_wait();
   if (threadIdx.x == 0) a.rinv[row] = 1.f / s;
   auto emit = [&](int i, const float* w) {
     alignas(16) T hi[8], lo[8];
@@ -576,27 +595,16 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
       }
       // e^(score - max) of this half, its maximum and sum
       float m = -CUDART_INF_F, l = 0.f;
-      {
+      if (any) {
         float mx[4] = {m, m, m, m}, sum[4] = {0.f, 0.f, 0.f, 0.f};  // (four chains: the warps are few)
-        if (__all_sync(0xffffffffu, nv == 128)) {
 #pragma unroll
-          for (int i = 0; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i] * c);
-          m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        for (int i = 0; i < 128; ++i)
+          if (i < nv) mx[i & 3] = fmaxf(mx[i & 3], v[i] * c);
+        m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
 #pragma unroll
-          for (int i = 0; i < 128; ++i) {
-            v[i] = pf_exp2(fmaf(v[i], c, -m));
-            sum[i & 3] += v[i];
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (i < nv) mx[i & 3] = fmaxf(mx[i & 3], v[i] * c);
-          m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-#pragma unroll
-          for (int i = 0; i < 128; ++i) {
-            v[i] = i < nv ? pf_exp2(fmaf(v[i], c, -m)) : 0.f;
-            sum[i & 3] += v[i];
-          }
+        for (int i = 0; i < 128; ++i) {
+          v[i] = i < nv ? pf_exp2(fmaf(v[i], c, -m)) : 0.f;
+          sum[i & 3] += v[i];
         }
         l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
       }
@@ -621,10 +629,13 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
       // column sums over the warp's pairs, then over the lane quarters
 #pragma unroll
       for (int g = 0; g < 128; g += 32) {
-        float x[32];
+        float sum = 0.f;
+        if (any) {
+          float x[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) x[i] = g + i < nv ? v[g + i] * f : 0.f;  // (not 0 * NaN)
-        const float sum = any ? rs_reduce<32>(x, lane, [](float p, float q) { return p + q; }) : 0.f;
+          for (int i = 0; i < 32; ++i) x[i] = g + i < nv ? v[g + i] * f : 0.f;  // (not 0 * NaN)
+          sum = rs_reduce<32>(x, lane, [](float p, float q) { return p + q; });
+        }
         s.cols[quarter * MS_N + half * 128 + g + lane] = sum;
       }
       named_bar_sync(1, 32 * MS_EPI);
@@ -634,7 +645,7 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
       if (mine) {
         sum = s.cols[col];
 #pragma unroll
-        for (int g = 1; g < 4; ++g) sum += s.cols[g * MS_N + col];
+          for (int g = 1; g < 4; ++g) sum += s.cols[g * MS_N + col];
       }
       const int64_t at = (int64_t)tile.page * a.page_rows + seg0 + col;
       bool last = tile.total == 1;

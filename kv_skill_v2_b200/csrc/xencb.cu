@@ -385,7 +385,7 @@ template <typename T>
 int launch_quant_f8(const void* x, int64_t M, int K, void* x8, uint8_t* scale, int stride, const F8RowStats& stats,
                     cudaStream_t st) {
   const int vec = K % 8 == 0 && aligned(x, 16);
-  launch_pdl(quant_f8_kernel<T>, dim3((unsigned)M), dim3(F8Q_THREADS), 0, st, static_cast<const T*>(x), K, vec,
+  launch_pdl(quant_f8_kernel<T>, dim3((unsigned)M), dim3(f8q_threads<T>()), 0, st, static_cast<const T*>(x), K, vec,
              static_cast<uint8_t*>(x8), scale, stride, stats);
   XENCB_CHECK_LAUNCH("quant_f8 launch");
   return XENCB_OK;
@@ -1040,8 +1040,9 @@ int plan_mass(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows, in
   // few pairs over few pages: no plan, but room in every page for all of them
   const int64_t most = (p->n_pairs + MS_M - 1) / MS_M;
   p->direct = p->n_pairs <= MS_DIRECT && n_pages * most <= 4096;
-  p->max_tiles = p->direct ? n_pages * most : p->n_pairs / MS_M + std::min<int64_t>(n_pages, p->n_pairs);
-  p->pages = align_up((size_t)n_pages * 4, 256);
+  // (with a plan: two turns of at most 148 clusters may stay empty)
+  p->max_tiles = p->direct ? n_pages * most : p->n_pairs / MS_M + std::min<int64_t>(n_pages, p->n_pairs) + 2 * MS_MAX_CLUSTERS;
+  p->pages = align_up((size_t)(n_pages + 1) * 4, 256);
   p->pair = align_up((size_t)p->n_pairs * 4, 256);
   p->place = p->direct ? align_up((size_t)p->n_pairs * n_pages * 4, 256) : p->pair;
   p->tiles = align_up((size_t)p->max_tiles * sizeof(MassTile), 256);
@@ -1072,16 +1073,16 @@ int run_mass(const void* q, int q_dtype, const MassPlan& p, const MassArgs& a, c
     return cudaFuncGetAttributes(&fa, kern) == cudaSuccess ? fa.numRegs * MS_THREADS : 0;
   }();
   if (regs < MS_REGS) return fail(XENCB_ENOTSUP, "read_mass: built with %d registers a CTA, %d are needed", regs, MS_REGS);
-  n_clusters = (int)std::min<int64_t>(n_clusters, p.max_tiles);
-  const int counted = p.n_pairs > MS_ONE_CTA;
-  if (counted) {
-    const cudaError_t e = cudaMemsetAsync(a.cnt, 0, 2 * p.pages, st);
-    if (e != cudaSuccess) return cuda_fail(e, "read_mass: memset");
-    mass_count_kernel<<<(unsigned)std::min<int64_t>((p.n_pairs + 255) / 256, 4 * sms), 256, 0, st>>>(a);
-    XENCB_CHECK_LAUNCH("mass_count launch");
-  }
+  n_clusters = (int)std::min<int64_t>(std::min(n_clusters, MS_MAX_CLUSTERS), p.max_tiles);
   if (!p.direct) {
-    mass_plan_kernel<<<1, MS_PLAN_THREADS, 0, st>>>(a, counted);
+    // one CTA counts few pairs; more take a grid, whose counters are zeroed before
+    const unsigned pgrid = p.n_pairs <= MS_ONE_CTA ? 1u
+                                                   : (unsigned)std::min<int64_t>((p.n_pairs + MS_PLAN_THREADS - 1) / MS_PLAN_THREADS, 2 * sms);
+    if (pgrid > 1) {
+      const cudaError_t e = cudaMemsetAsync(a.cnt, 0, 2 * p.pages, st);
+      if (e != cudaSuccess) return cuda_fail(e, "read_mass: memset");
+    }
+    mass_plan_kernel<<<pgrid, MS_PLAN_THREADS, 0, st>>>(a, n_clusters);
     XENCB_CHECK_LAUNCH("mass_plan launch");
   }
   T* qo = static_cast<T*>(q16);
@@ -1089,7 +1090,7 @@ int run_mass(const void* q, int q_dtype, const MassPlan& p, const MassArgs& a, c
   auto rows = [&](auto t) {
     using TQ = decltype(t);
     auto rk = mass_rows_kernel<TQ, T, TERMS>;
-    // (its rows are read before the plan is waited for: it may only follow the plan so closely)
+    // (its rows are not held back by the plan: it may only follow the plan so closely)
     if (p.direct) rk<<<rgrid, MS_ROWS_THREADS, 0, st>>>(a, static_cast<const TQ*>(q), qo);
     else launch_pdl(rk, rgrid, dim3(MS_ROWS_THREADS), 0, st, a, static_cast<const TQ*>(q), qo);
   };
