@@ -354,10 +354,11 @@ struct F8Plan {
   size_t out_bytes, x8_bytes, sx_bytes, rstd_bytes, total;
 };
 
-// Calls with tiles of 128 rows and 256 output features for half of the device take gemm_f8_rows_kernel (2048 rows, 5120 ->
-// 2048: %ROWS%); it keeps two tiles' scale factors in tensor memory, blocks of up to 40. The others split K: BN = 64
-// and 128 where all rows fit one tile (the CTAs stream the weights), 256 where they do not, so that a weight tile is
-// fetched a quarter as often.
+// Calls with tiles of 128 rows and 256 output features for a quarter of the device take gemm_f8_rows_kernel (captured
+// in / out, this form against split K: 2048 -> 4096, 384 rows 19.2 / 14.5 us against 20.1 / 20.7; 4096 -> 2048, 600 rows
+// 25.7 / 21.1 against 27.1 / 26.6, 1024 rows 26.4 / 22.5 against 36.4 / 35.2); it keeps two tiles' scale factors in tensor
+// memory, blocks of up to 40. The others split K: BN = 64 and 128 where all rows fit one tile (the CTAs stream the
+// weights), 256 where they do not, so that a weight tile is fetched a quarter as often.
 F8Plan plan_f8(int64_t M, int N, int K, int sms) {
   F8Plan p;
   p.bn = M <= 64 ? 64 : M <= 128 ? 128 : 256;
@@ -372,7 +373,7 @@ F8Plan plan_f8(int64_t M, int N, int K, int sms) {
   p.gp.part_bytes = align_up((size_t)p.gp.splits * (size_t)M * (size_t)N * sizeof(float), 256);
   p.sx_stride = (p.nb + 3) / 4 * 4;
   const int64_t tiles_n = (N + FR_BN - 1) / FR_BN;
-  p.rows = (p.nb + 3) / 4 <= FR_MAX_WORDS && 2 * tiles_n * ((M + FR_BM - 1) / FR_BM) >= sms;
+  p.rows = (p.nb + 3) / 4 <= FR_MAX_WORDS && 4 * tiles_n * ((M + FR_BM - 1) / FR_BM) >= sms;
   p.out_bytes = std::max(p.gp.part_bytes, p.rows ? align_up((size_t)M * 2 * tiles_n * sizeof(float2), 256) : 0);
   p.x8_bytes = align_up((size_t)M * p.nb * F8_BK, 256);
   p.sx_bytes = align_up((size_t)M * p.sx_stride, 256);
