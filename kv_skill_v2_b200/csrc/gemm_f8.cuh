@@ -100,6 +100,7 @@ __device__ __forceinline__ uint2 f8_quant8(const float* v, bool in, int* e) {
 
 // What the projection takes of a row besides its 8-bit form (project_in): 1/rms and the gate.
 struct F8RowStats {
+  int weight;           // a weight, not rows: the products load one before their wait, so nothing may start before its end
   int rms;
   float eps;
   const float* gate_w;  // [K] or null
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(f8q_threads<T>(), sizeof(T) == 4 ? 8 : 6) quan
                                                                uint8_t* __restrict__ x8, uint8_t* __restrict__ scale,
                                                                int stride, const F8RowStats st) {
   __shared__ float2 red[32];
-  pdl_trigger();
+  if (!st.weight) pdl_trigger();
   pdl_wait();
   const int64_t m = blockIdx.x;
   const T* row = x + m * K;
@@ -286,7 +287,8 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_f8_kernel(const __grid_con
   __syncthreads();
   tc_fence_after();
   const uint32_t taddr = *tmem_slot;
-  // one stage of weights before the wait, as the 3xF16 GEMM does
+  // one stage of weights before the wait, as the 3xF16 GEMM does (xencb_quant8, which writes them, lets no grid start
+  // before its end)
   const int npre = min(nkb, 1);
   if (threadIdx.x != 0) {
     pdl_wait();

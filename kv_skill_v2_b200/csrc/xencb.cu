@@ -1215,7 +1215,7 @@ static int project_in_impl(const void* h, int h_dtype, int64_t n_rows, int d_m, 
   if (w8 && p8.rows && !sel_w) {
     float* rstd = rstd_out ? rstd_out : reinterpret_cast<float*>(ws + p8.out_bytes + p8.x8_bytes + p8.sx_bytes);
     uint8_t* x8 = reinterpret_cast<uint8_t*>(ws + p8.out_bytes);
-    const F8RowStats stats{(flags & XENCB_PIN_RMS) ? 1 : 0, rms_eps, gate_w, gate_b, gate_b_dev, rstd,
+    const F8RowStats stats{0, (flags & XENCB_PIN_RMS) ? 1 : 0, rms_eps, gate_w, gate_b, gate_b_dev, rstd,
                            gate_w ? gate_out : nullptr};
     rc = launch_quant_f8(h, h_dtype, n_rows, d_m, x8, x8 + p8.x8_bytes, p8.sx_stride, stats, st);
     if (rc) return rc;
@@ -2210,7 +2210,7 @@ int xencb_quant8(const void* x, int dtype, int64_t n, int k, void* x8, void* sca
   const int rc = device_info(&di);
   if (rc) return rc;
   if (n > INT32_MAX) return fail(XENCB_ENOTSUP, "quant8: too many rows");
-  return launch_quant_f8(x, dtype, n, k, x8, static_cast<uint8_t*>(scale), (k + F8_BK - 1) / F8_BK, F8RowStats{},
+  return launch_quant_f8(x, dtype, n, k, x8, static_cast<uint8_t*>(scale), (k + F8_BK - 1) / F8_BK, F8RowStats{1},
                          static_cast<cudaStream_t>(stream));
 }
 
@@ -2410,6 +2410,17 @@ int xencb_pages_evict(const void* const* pools, void* const* pools_out, const in
   for (int i = 0; i < n_pools; ++i) inplace += pools_out[i] == pools[i];
   if (inplace && (inplace != n_pools || new_rows != page_rows))
     return fail(XENCB_EINVAL, "pages_evict: in place, every pool is its own output and new_rows is page_rows");
+  if (mass_out == mass) return fail(XENCB_EINVAL, "pages_evict: mass_out must not be mass");
+  // nothing that is written may lie in a pool or in another output (rows move in no order)
+  const auto overlap = [&](const void* x, int64_t x_rows, int i, const void* y, int64_t y_rows, int j) {
+    const uintptr_t xa = reinterpret_cast<uintptr_t>(x), ya = reinterpret_cast<uintptr_t>(y);
+    return xa < ya + (uintptr_t)(n_pages * y_rows * row_bytes[j]) && ya < xa + (uintptr_t)(n_pages * x_rows * row_bytes[i]);
+  };
+  for (int i = 0; i < n_pools; ++i)
+    for (int j = 0; j < n_pools; ++j)
+      if ((!inplace && overlap(pools_out[i], new_rows, i, pools[j], page_rows, j)) ||
+          (j > i && overlap(pools_out[i], new_rows, i, pools_out[j], new_rows, j)))
+        return fail(XENCB_EINVAL, "pages_evict: output %d overlaps a pool or another output", i);
   const size_t need = xencb_pages_evict_workspace(n_pages, page_rows, per_library);
   if (!workspace || !aligned(workspace, 256) || workspace_bytes < need)
     return fail(XENCB_EINVAL, "pages_evict: workspace needs %zu bytes, 256-byte aligned (got %zu)", need,

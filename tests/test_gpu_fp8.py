@@ -159,6 +159,29 @@ def test_project_out(R, d_in, d_out, dtype):
     assert rel(delta, matched) < TOL + eps
 
 
+@pytest.mark.parametrize("R", [3, 8, 9, 20, 100, 129, 200])
+def test_many_blocks_and_no_split(R):
+    # 94 blocks in one split: several rounds of the ring's blocks, many words of scale factors
+    n, k = 148 * 128 - 4, 12000
+    h, w8 = rows(R, k, 40, dtype=torch.bfloat16), ops.weights_fp8(W := rows(n, k, 41) * k ** -0.5)
+    assert rel(ops.project_in(h, w8, rms=False, l2=False)[0], values(h) @ values(W).t()) < TOL
+
+
+@pytest.mark.parametrize("R", [1, 50, 2000])
+def test_a_weight_is_read_after_it_is_written(R):
+    # the products load weights before they wait for the launch before theirs: never before the weight is there
+    h, Ws = rows(R, 2048, 42, dtype=torch.bfloat16), [rows(4096, 2048, s) for s in (43, 44)]
+    want = [ops.project_in(h, ops.weights_fp8(W))[0] for W in Ws]
+    w8 = ops.weights_fp8(Ws[0])
+    torch.cuda.synchronize()
+    for i in range(20):
+        at = w8.w.data_ptr()
+        del w8
+        w8 = ops.weights_fp8(Ws[i & 1])  # the same memory as the weight before
+        q = ops.project_in(h, w8)[0]
+        assert w8.w.data_ptr() == at and torch.equal(q, want[i & 1])
+
+
 def test_a_row_that_is_not_finite_is_alone():
     h, W = rows(70, 512, 9), rows(256, 512, 10)
     w8 = ops.weights_fp8(W)
