@@ -464,8 +464,9 @@ XENCB_API int xencb_pages_compact(void* const* pools, const int64_t* row_bytes, 
  * table read and pages that none names stay as they were.
  * n_valid_out [n_lib, n_chunks]: the rows of each entry that stay (those before its own n_valid). A Library that reads
  * fewer rows of a page than another may be left with none. mass_out [n_pages, new_rows] and kept_out [n_pages, new_rows]:
- * the mass and the old row of each row that stays; 0 and -1 behind them. page_rows at most 4096. The table itself does not
- * change. */
+ * the mass and the old row of each row that stays; 0 and -1 behind them (mass_out is not mass). A page that a Library names
+ * twice counts twice in its budget. Outputs lie neither in the pools nor in each other. page_rows at most 4096. The table
+ * itself does not change. */
 XENCB_API size_t xencb_pages_evict_workspace(int64_t n_pages, int page_rows, int per_library);
 XENCB_API int xencb_pages_evict(const void* const* pools, void* const* pools_out, const int64_t* row_bytes, int n_pools,
                                 int64_t n_pages, int page_rows, int new_rows, const int32_t* page_of,

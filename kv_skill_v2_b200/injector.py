@@ -230,9 +230,12 @@ class XEncInjector(ExternalSkillInjector):
         key = (W.data_ptr(), W._version, tuple(W.shape), str(W.device), "fp8")
         hit = self._wprep.get(key)
         if hit is None:
+            w8 = ops.weights_fp8(W)
+            if W.is_cuda and torch.cuda.is_current_stream_capturing():
+                return w8, None  # (it is there after a replay only)
             if len(self._wprep) >= 64:
                 self._wprep.clear()
-            hit = self._wprep[key] = (W, ops.weights_fp8(W))
+            hit = self._wprep[key] = (W, w8)
         return hit[1], None
 
     def _weights_key(self) -> tuple:
@@ -589,6 +592,8 @@ class LibraryInjector(XEncInjector):
         if pm is not None:
             wk = torch.where((pm != 0).view(-1, 1), wk, torch.zeros_like(wk))
         mass = self.slot_mass.get(li)
+        if mass is None and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("record_mass: run the step once before it is captured (slot_mass is what replays add to)")
         self.slot_mass[li] = ops.read_mass(q, pages, idx, wk, rows_per_lib=rpl, read_temp=self.read_temp, mass=mass,
                                            decay=self.mass_decay, out=mass)
 

@@ -1102,7 +1102,7 @@ def pages_evict(pools, page_of: torch.Tensor, n_valid: torch.Tensor, mass: torch
     keep: rows to keep of each chunk (an int, or int32 [n_lib, C] on the device; a page keeps the most that an entry which
     names it asks for), at least `floor`; with per_library the rows to keep of each whole Library (an int, or int32
     [n_lib]): every page keeps its `floor` heaviest rows, the rest of the budget goes to the Library's heaviest others (ties:
-    the lower chunk), and a row stays if some Library keeps it.
+    the lower chunk; a page that it names twice counts twice), and a row stays if some Library keeps it.
     page_rows: the rows of a page of the new pools that are returned (a page keeps no more than that), which hold zeros behind
     the rows that stay and in pages that no table names. None: the rows move within the given pools, which are returned; rows
     that went become zeros.

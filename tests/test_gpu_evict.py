@@ -176,6 +176,40 @@ def test_captured_and_repeated():
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("per_library", [False, True])
+def test_one_library_one_page_twice_and_keeps_below_zero(per_library):
+    a = case(80, 1, 6, 7, 40, 24, [F16, F16])
+    a[1][0, 3] = a[1][0, 1]
+    k = 50 if per_library else 9
+    check(*a, k, [k] if per_library else [[k] * 6], per_library=per_library, M=30)
+    keep = torch.tensor([-3] if per_library else [[-1, 0, 5, -7, 40, 41]], dtype=torch.int32)
+    check(*a, keep.cuda(), keep.tolist(), per_library=per_library, floor=0)
+    check(*a, keep.cuda(), keep.tolist(), per_library=per_library, floor=40, M=12)
+
+
+def test_more_pools_than_one_launch_moves():
+    dtypes = [F16, BF16, F32] * 25
+    check(*case(81, 2, 3, 8, 20, 16, dtypes), 7, [[7] * 3] * 2, M=9)
+    check(*case(82, 2, 3, 8, 20, 16, dtypes), 7, [[7] * 3] * 2)
+
+
+def test_two_streams_at_once():
+    a, b = case(83, 4, 6, 40, 64, 256, [F16, F16]), case(84, 2, 30, 70, 128, 64, [F16])
+    run = [lambda x=x, k=k: ops.pages_evict(*x, k, per_library=True, page_rows=40) for x, k in ((a, 100), (b, 700))]
+    want = [r() for r in run]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        got = []
+        for s, r in zip(streams, run):
+            with torch.cuda.stream(s):
+                got.append(r())
+        torch.cuda.synchronize()
+        for w, g in zip(want, got):
+            for x, y in zip([*w[:3], *w[3]], [*g[:3], *g[3]]):
+                assert torch.equal(x, y)
+
+
 def test_refusals():
     pools, page_of, n_valid, mass = case(70, 2, 3, 9, 16, 8, [F16])
     with pytest.raises(ValueError, match="mass"):
@@ -194,6 +228,8 @@ def test_refusals():
         ops.pages_evict(pools, page_of, n_valid, mass, 3, floor=-1)
     with pytest.raises(RuntimeError, match="CUDA"):
         ops.pages_evict(pools, page_of, n_valid, mass.cpu(), 3)
+    with pytest.raises(ValueError, match="overlaps"):  # in place the same pool twice would move twice
+        ops.pages_evict([*pools, pools[0]], page_of, n_valid, mass, 3)
     big = torch.zeros(1, 4100, 8, dtype=F16, device="cuda")
     one = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
     with pytest.raises(NotImplementedError, match="4096"):

@@ -109,6 +109,48 @@ def test_reads_record_the_attention_of_their_slots(share, top_k):
     inj.detach()
 
 
+def test_a_captured_step_records():
+    lib = library(40)
+    inj = LibraryInjector(TinyReader(D_M, 5).cuda(), itf := interface(41), top_k=2)
+    inj.load_library(lib)
+    inj.record_mass = inj.gemm_fp8 = True
+    g = torch.Generator(device="cuda").manual_seed(42)
+    x, h = torch.zeros(3, 1, D_M, device="cuda"), torch.randn(3, 1, D_M, generator=g, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad():
+        with pytest.raises(RuntimeError, match="before it is captured"):  # nothing there yet that replays could add to
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                inj._inject(x, 1)
+        inj._inject(h, 1)
+        first = inj.slot_mass[1].clone()
+        with torch.cuda.graph(graph):
+            inj._inject(x, 1)
+    inj.slot_mass[1].zero_()
+    x.copy_(h)
+    for _ in range(3):
+        graph.replay()
+    close(inj.slot_mass[1], 3 * first.double(), 1e-6)
+    close(first, step(h, itf, lib, 1, 2, fp8=True)[1], 1e-3)
+    inj.detach()
+
+
+def test_a_weight_first_used_in_a_capture():
+    lib, itf = library(43), interface(44)
+    h = torch.randn(3, 2, D_M, generator=torch.Generator(device="cuda").manual_seed(45), device="cuda")
+    inj = LibraryInjector(TinyReader(D_M, 5).cuda(), itf, top_k=2)
+    inj.load_library(lib)
+    inj.gemm_fp8 = True
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad():
+        with torch.cuda.graph(graph):
+            got = inj._inject(h, 1)[0]
+        want = inj._inject(h, 1)[0].clone()  # before any replay: not with what the graph has yet to write
+        graph.replay()
+        assert torch.equal(got, want) and not torch.equal(want, h)
+        assert rel_err(want - h, step(h, itf, lib, 1, 2, fp8=True)[0]) <= 2e-2
+    inj.detach()
+
+
 def test_masked_positions_give_no_attention():
     """A padded batch: the position mask's zeros are not counted."""
     lib = library(4)

@@ -68,6 +68,24 @@ def test_evict_refuses_bad_arguments():
     assert call("xencb_pages_evict_workspace", 4, 8, 1) > call("xencb_pages_evict_workspace", 4, 8, 0) > 0
 
 
+def test_evict_refuses_outputs_that_overlap():
+    at = lambda *a: (ctypes.c_void_p * len(a))(*a)  # noqa: E731
+    row, p = (ctypes.c_int64 * 2)(16, 16), ctypes.c_void_p(1 << 30)
+
+    def evict(pools, out, new=4, mass=1 << 29):  # a workspace of 8 bytes ends the calls that get past the check
+        return call("xencb_pages_evict", pools, out, row, 2, 4, 8, new, p, p, 2, None, 1, ctypes.c_void_p(mass), None, 3, 0, 1,
+                    p, p, p, p, 8, None)
+
+    for bad in ((at(4096, 8192), at(4096 + 496, 16384)), (at(4096, 8192), at(8192, 4096)), (at(4096, 8192), at(1 << 20, 1 << 20)),
+                (at(4096, 8192), at(1 << 20, (1 << 20) + 240)), (at(4096, 8192), at(4096 - 240, 1 << 20))):
+        assert evict(*bad) == N.EINVAL and b"overlaps" in N.lib().xencb_last_error(), bad
+    for good in ((at(4096, 4096), at(4096 + 512, 4096 - 256)), (at(4096, 8192), at(1 << 20, (1 << 20) + 256))):
+        assert evict(*good) == N.EINVAL and b"workspace" in N.lib().xencb_last_error()
+    assert evict(at(4096, 4096), at(4096, 4096), new=8) == N.EINVAL and b"overlaps" in N.lib().xencb_last_error()
+    assert evict(at(4096, 4608), at(4096, 4608), new=8) == N.EINVAL and b"workspace" in N.lib().xencb_last_error()
+    assert evict(at(4096, 4608), at(4096, 4608), new=8, mass=1 << 30) == N.EINVAL and b"mass_out" in N.lib().xencb_last_error()
+
+
 def test_mass_and_8_bit_calls_refuse_bad_arguments():
     p = ctypes.c_void_p(256)
 
