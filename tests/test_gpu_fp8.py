@@ -100,7 +100,10 @@ def test_weights_fp8_not_finite():
     (127, 384, 516, torch.bfloat16), (128, 1024, 512, torch.float32), (129, 1024, 1024, torch.bfloat16),
     (300, 512, 2048, torch.float32), (513, 2048, 384, torch.float16), (1000, 5120, 640, torch.bfloat16),
     (2048, 5120, 2048, torch.bfloat16), (1111, 700, 2052, torch.float32), (19000, 130, 132, torch.float16),
-    (4, 40000, 8, torch.float32), (200, 12000, 16, torch.bfloat16), (3, 256, 7000, torch.float32)])
+    (4, 40000, 8, torch.float32), (200, 12000, 16, torch.bfloat16), (3, 256, 7000, torch.float32),
+    # 2, 3, 5, 6, 7 and 8 tiles of 256 features, several turns of a CTA, odd ends
+    (12345, 136, 260, torch.bfloat16), (9000, 130, 516, torch.float32), (4100, 1000, 1156, torch.float16),
+    (5000, 264, 1284, torch.bfloat16), (6001, 72, 1796, torch.float32), (2500, 512, 1800, torch.bfloat16)])
 def test_project_in(R, d_in, d_out, dtype):
     h, W = rows(R, d_in, 3, dtype=dtype), rows(d_out, d_in, 4) * d_in ** -0.5
     g = gen(5)
