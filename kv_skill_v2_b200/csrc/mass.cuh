@@ -22,8 +22,8 @@
 //
 // Precision. Float32 q enters as hi + lo in 16 bits, two products into one accumulator: 22 bits with f16 slots, 16 with
 // bf16. A 16-bit q is one product, exact (bf16 q fits f16's 11 bits, but for values 2^-28 below the row's largest). The
-// tensor core's accumulator drops bits below its running value, so it runs over MS_CHUNK blocks of 64 columns and is added
-// up in float32 registers.
+// tensor core's accumulator drops bits below its running value, so it runs over MS_CHUNK or MS_CHUNK_FEW blocks of 64 columns
+// and is added up in float32 registers.
 //
 // What bounds it. Few pairs a page: HBM, one pass over the slots (64 rows on 64 pages of 512 x 2048: 37 us a launch, 3.6
 // TB/s; 1024 pages with few pairs each run at 5.6 TB/s). Full tiles: 128 pairs x 512 slots x 2048 columns take 22.9 us of
@@ -43,6 +43,8 @@ constexpr int MS_N = 256;         // slots of a CTA at most
 constexpr int MS_MAX_CLUSTERS = 256;  // of a launch
 constexpr int MS_MAX_CS = 8;      // CTAs per cluster: pages of up to 2048 slots
 constexpr int MS_CHUNK = 4;       // blocks of 64 columns per accumulator
+constexpr int MS_CHUNK_FEW = 2;   // of calls of few pairs, whose errors no sum averages out (64 rows, top-4: 5.6e-7 -> 3.3e-7);
+                                  // it costs them nothing, prompts 3 % for the same error
 constexpr int MS_ATILE = MS_M * 128;
 constexpr int MS_BTILE = MS_N * 128;
 constexpr int MS_PRODUCERS = 4;   // warps that bring Q
@@ -386,7 +388,7 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank();
   const int cluster = blockIdx.x / cs, n_clusters = gridDim.x / cs;
-  const int nkb = (a.d_s + 63) / 64, n_chunk = (nkb + MS_CHUNK - 1) / MS_CHUNK;
+  const int nkb = (a.d_s + 63) / 64, chunk = a.direct ? MS_CHUNK_FEW : MS_CHUNK;
   const int seg0 = rank * a.per;
 
   if (threadIdx.x == 0) {
@@ -464,11 +466,11 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
           const MassTile tile = a.tiles[t];
           if (tile.count == 0 || seg0 >= tile.nv) continue;
           const int terms = stacked(tile) ? 1 : TERMS;
-          for (int k0 = 0; k0 < nkb && ok; k0 += MS_CHUNK, ++acc) {
+          for (int k0 = 0; k0 < nkb && ok; k0 += chunk, ++acc) {
             const uint32_t buf = acc & 1, use = acc >> 1;
             if (use > 0 && !(ok = mbar_wait_spin(&s.s_empty[buf], (use - 1) & 1))) break;
             tc_fence_after();
-            const int k1 = min(nkb, k0 + MS_CHUNK);
+            const int k1 = min(nkb, k0 + chunk);
             for (int kb = k0; kb < k1; ++kb) {
               if (!(ok = mbar_wait_spin(&s.full[ring.st], ring.phase))) break;
               fence_proxy_async_smem();  // Q was written by this CTA's threads
@@ -564,7 +566,7 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
 #pragma unroll
       for (int i = 0; i < 128; ++i) v[i] = 0.f;
       if (seg0 < tile.nv) {
-        for (int k = 0; k < n_chunk; ++k, ++acc) {
+        for (int k0 = 0; k0 < nkb; k0 += chunk, ++acc) {
           const uint32_t buf = acc & 1;
           done(*s.abort_flag || mbar_wait_spin(&s.s_full[buf], (acc >> 1) & 1));
           tc_fence_after();
