@@ -366,24 +366,39 @@ class PagedLibrary:
         per_library, floor as in ops.pages_evict. page_rows: new pools with pages of that many rows, the old ones are free
         once nothing refers to them; None: within these pools, and then this PagedLibrary and any select() of it must no
         longer be read. The summary keys stay as they are, so the routing does not change. Evict on the PagedLibrary that
-        holds every row, as for fork and compact. Rows that the Libraries read differ in number only where a page is shared by
-        Libraries with different n_valid; RuntimeError where one of them would be left with an empty chunk (new pools only).
-        Reads one flag back from the device in that case."""
+        holds every row, as for fork and compact.
+
+        Where a page is shared by Libraries with different n_valid, one of them may read none of the rows that stay; with
+        keep = floor = 0 nobody does. An empty chunk cannot be read: RuntimeError, and nothing has moved. One flag is read
+        back from the device to know it, so an eviction is not captured (ops.pages_evict, which leaves such chunks to its
+        caller, can be)."""
         from .ops import pages_evict
 
         pools, page_of, n_valid, nco = self._tables()
         page_of, n_valid = page_of.contiguous(), n_valid.contiguous()
+        if page_of.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("evict reads a flag back from the device and cannot be captured (ops.pages_evict can)")
         if isinstance(mass, dict):
             if not mass:
                 raise ValueError("evict: mass of at least one layer is required")
             mass = torch.stack([mass[li] for li in sorted(mass)]).sum(0)
-        nv, new_mass, _, new = pages_evict(pools, page_of, n_valid, mass.contiguous(), keep, n_chunks_of=nco,
-                                           per_library=per_library, floor=floor, page_rows=page_rows)
-        if page_rows is not None and bool(((nv == 0) & (n_valid > 0) & self._live(page_of, nco)).any()):
-            raise RuntimeError("evict: a Library would be left with an empty chunk (a page that it shares with one that "
-                               "reads more of its rows, or keep = floor = 0)")
+        mass = mass.contiguous()
+        how = dict(n_chunks_of=nco, per_library=per_library, floor=floor)
+        if page_rows is None:  # rows that moved are not to be had back: the counts first, with a pool that holds nothing
+            P, rows = pools[0].shape[:2]
+            blank = torch.empty(P, rows, 1, dtype=torch.float16, device=pools[0].device)
+            nv = pages_evict([blank], page_of, n_valid, mass, keep, page_rows=rows, **how)[0]
+            self._refuse_empty(nv, page_of, n_valid, nco)
+        nv, new_mass, _, new = pages_evict(pools, page_of, n_valid, mass, keep, page_rows=page_rows, **how)
+        if page_rows is not None:
+            self._refuse_empty(nv, page_of, n_valid, nco)
         renamed = {p.data_ptr(): q for p, q in zip(pools, new)}
         return self._with_tables(page_of, nv, nco, None, renamed), new_mass
+
+    def _refuse_empty(self, n_left, page_of, n_valid, n_chunks_of) -> None:
+        if bool(((n_left == 0) & (n_valid > 0) & self._live(page_of, n_chunks_of)).any()):
+            raise RuntimeError("evict: a Library would be left with an empty chunk (a page that it shares with one that "
+                               "reads more of its rows, or keep = floor = 0)")
 
     def _live(self, page_of, n_chunks_of) -> torch.Tensor:
         """[n_lib, C] bool: the entries of the table that are chunks."""
