@@ -1,4 +1,5 @@
-"""What a server does around a Library that shrinks: evictions that are refused leave it whole."""
+"""What a server does around a Library that shrinks: evictions that are refused leave it whole, one bad request does not
+spoil the attention that others recorded."""
 
 from __future__ import annotations
 
@@ -52,3 +53,53 @@ def test_an_eviction_is_not_captured():
             with torch.cuda.graph(torch.cuda.CUDAGraph()):
                 lib.evict(mass, 4, page_rows=new_rows)
     assert ops.device_status(DEV) == 0
+
+
+@pytest.mark.parametrize("share", [False, True])
+@pytest.mark.parametrize("top_k", [2, 0])
+@pytest.mark.parametrize("T", [1, 9])
+def test_a_request_that_is_not_finite_leaves_no_trace_in_the_mass(share, top_k, T):
+    """Three Libraries and forks that share their pages: one request of the batch goes wrong, then the next steps run."""
+    lib = library(1).reserve(4).fork([0, 2], own_from=[3, 2])
+    g = torch.Generator(device="cuda").manual_seed(50)
+    steps = [torch.randn(lib.n_lib, T, D_M, generator=g, device="cuda") for _ in range(3)]
+    bad = [x.clone() for x in steps]
+    bad[0][3, -1, 5], bad[1][0, 0] = float("nan"), float("inf")
+    live = [torch.ones(lib.n_lib, T, device="cuda") for _ in steps]
+    live[0][3, -1], live[1][0, 0] = 0, 0
+    got = []
+    for rows, masks in ((bad, None), (steps, live)):  # the same rows taken out by a position mask
+        inj = LibraryInjector(TinyReader(D_M, 5).cuda(), interface(2), top_k=top_k, share_pages=share)
+        inj.load_library(lib)
+        inj.record_mass, inj.mass_decay = True, 0.5
+        with torch.no_grad():
+            for i, h in enumerate(rows):
+                inj.pos_mask = None if masks is None else masks[i]
+                for li in LAYERS:
+                    inj._inject(h, li)
+        got.append(inj.slot_mass)
+        inj.detach()
+    for li in LAYERS:
+        assert bool(got[0][li].isfinite().all()) and float(got[0][li].sum()) > 0
+        assert torch.equal(got[0][li], got[1][li])
+    assert ops.device_status(DEV) == 0
+
+
+def test_summary_keys_that_are_not_finite_leave_no_trace_in_the_mass():
+    """The routing of one Library is NaN: it shares pages with a fork whose routing is not."""
+    lib = library(1).fork([0])
+    inj = LibraryInjector(TinyReader(D_M, 5).cuda(), interface(2), top_k=0)
+    inj.load_library(lib)
+    inj.record_mass = True
+    h = torch.randn(lib.n_lib, 4, D_M, generator=torch.Generator(device="cuda").manual_seed(51), device="cuda")
+    lib.pages(1).S[3, 1] = float("nan")
+    with torch.no_grad():
+        inj._inject(h, 1)
+    assert bool(inj.slot_mass[1].isfinite().all())
+    live = torch.ones(lib.n_lib, 4, device="cuda")
+    live[3] = 0
+    got, inj.slot_mass, inj.pos_mask = inj.slot_mass[1], {}, live
+    with torch.no_grad():
+        inj._inject(h, 1)
+    assert torch.equal(got, inj.slot_mass[1])
+    inj.detach()
