@@ -71,6 +71,26 @@ _ADAPTER_SETS = 4
 # -> 4096, 64 pages of 512) takes, eager and captured, 147 and 116 us with 4 MB of it (64 rows, top-4), 124 and 126 with
 # 34 MB (32 rows, all chunks), 482 and 481 with 34 MB (512 rows, top-4): from there the device hides the launches
 _GRAPH_WORKSPACE = 32 << 20
+_PREPARED = 64  # weights whose prepared forms an injector keeps
+
+
+class _Prepared:
+    """A prepared weight (ops.weights_prep, ops.weights_fp8) with its source, kept alive so that no other tensor can have
+    its address, the streams that have waited for it and whether a caller's capture reads it."""
+
+    def __init__(self, source: torch.Tensor, form, stream: int):
+        self.source, self.form, self.streams, self.captured = source, form, {stream}, False
+        self.written = torch.cuda.Event()
+        self.written.record(torch.cuda.current_stream(source.device))
+
+    def share(self, stream: int) -> None:
+        """The current stream, `stream`, reads it too."""
+        now = torch.cuda.current_stream(self.source.device)
+        now.wait_event(self.written)
+        for t in (self.form.w, self.form.scale) if isinstance(self.form, ops.Weights8) else (self.form,):
+            t.record_stream(now)
+        self.streams.add(stream)
+
 
 class ExternalSkillInjector:
     """Forward-hook plumbing for a reader model (the deltaskill base class the reference subclasses)."""
@@ -85,14 +105,15 @@ class ExternalSkillInjector:
         self.calib: Optional[dict] = None
         self.skill: Optional[KVSkill] = None
         self.pos_mask: Optional[torch.Tensor] = None  # [B, T] multiplier of delta (None: all positions)
-        # projection weights in the 3xF16 form (ops.weights_prep), keyed by storage, version and shape; each
-        # entry keeps its source tensor alive so the key cannot be reused by another tensor
+        # projection weights in the 3xF16 form (ops.weights_prep)
         self.gemm_f16x3 = True
         # the projections in 8-bit floating point (ops.weights_fp8; rows quantised in the call): a quarter of the prepared
         # weights' bytes and, for prompts, a fifth of the projections' time, at e4m3's precision. It moves the routing too, so it
         # is the caller's choice. Not beside adapters
         self.gemm_fp8 = False
+        # prepared weights by form, storage, version and shape (_prepared)
         self._wprep: dict = {}
+        self._capturing_hook = False
         # low-rank adapters of the requests of a batch (set_adapters)
         self._adapters: Optional[tuple] = None
         self._attach()
@@ -209,34 +230,39 @@ class XEncInjector(ExternalSkillInjector):
                                read_softmax=self.read_softmax)
 
     # ------------------------------------------------------------------ shared projection machinery
+    def _prepared(self, kind: str, W: torch.Tensor, make):
+        """make(W), kept with its source for later calls. What a capture makes is not kept (only replays write it), and
+        what a caller's own capture takes is never dropped (its replays read it). A call on another stream than the one
+        that made it waits for it."""
+        key = (kind, W.data_ptr(), W._version, tuple(W.shape), str(W.device))
+        hit = self._wprep.get(key)
+        capturing = W.is_cuda and torch.cuda.is_current_stream_capturing()
+        if hit is None:
+            form = make(W)
+            if capturing:
+                return form
+            if len(self._wprep) >= _PREPARED:
+                self._wprep.pop(next((k for k, e in self._wprep.items() if not e.captured), key), None)
+            self._wprep[key] = _Prepared(W, form, ops._stream(W.device))
+            return form
+        self._wprep[key] = self._wprep.pop(key)  # (the least lately used goes first)
+        if capturing:  # (torch.cuda.graph has waited for the device)
+            hit.captured = hit.captured or not self._capturing_hook
+        elif ops._stream(W.device) not in hit.streams:
+            hit.share(ops._stream(W.device))
+        return hit.form
+
     def _prep(self, W: torch.Tensor) -> Optional[torch.Tensor]:
         """W [out, in] float32 on the device in the 3xF16 form, or None (disabled, or in % 8 != 0)."""
         if not self.gemm_f16x3 or W.shape[-1] % 8 != 0 or not W.is_cuda:
             return None
-        key = (W.data_ptr(), W._version, tuple(W.shape), str(W.device))
-        hit = self._wprep.get(key)
-        if hit is not None:
-            return hit[1]
-        if len(self._wprep) >= 64:
-            self._wprep.clear()
-        prep = ops.weights_prep(W)
-        self._wprep[key] = (W, prep)
-        return prep
+        return self._prepared("f16x3", W, ops.weights_prep)
 
     def _weight(self, W: torch.Tensor):
         """(weight, its prepared form or None) as project_in and project_out take them, for W [out, in] float32."""
         if not self.gemm_fp8:
             return W, self._prep(W)
-        key = (W.data_ptr(), W._version, tuple(W.shape), str(W.device), "fp8")
-        hit = self._wprep.get(key)
-        if hit is None:
-            w8 = ops.weights_fp8(W)
-            if W.is_cuda and torch.cuda.is_current_stream_capturing():
-                return w8, None  # (it is there after a replay only)
-            if len(self._wprep) >= 64:
-                self._wprep.clear()
-            hit = self._wprep[key] = (W, w8)
-        return hit[1], None
+        return self._prepared("fp8", W, ops.weights_fp8), None
 
     def _weights_key(self) -> tuple:
         """Storage and version of every interface parameter (a captured step is valid only for these)."""
@@ -662,8 +688,12 @@ class LibraryInjector(XEncInjector):
                 route_eager = self.last_route
                 h_static = h.detach() if on_buffer else h.detach().clone()
                 graph = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(graph):
-                    h_new_s, rel_s = self._run_lib_eager(h_static, li, inject, sel)
+                self._capturing_hook = True
+                try:
+                    with torch.cuda.graph(graph):
+                        h_new_s, rel_s = self._run_lib_eager(h_static, li, inject, sel)
+                finally:
+                    self._capturing_hook = False
                 self._drop_stale_graphs()
                 # the entry keeps the prepared weights it captured alive
                 self._graphs[(base, h.data_ptr() if on_buffer else None)] = (

@@ -1,5 +1,5 @@
 """What a server does around a Library that shrinks: evictions that are refused leave it whole, one bad request does not
-spoil the attention that others recorded."""
+spoil the attention that others recorded, weights are prepared once for every stream and capture."""
 
 from __future__ import annotations
 
@@ -8,7 +8,7 @@ import torch
 
 from kv_skill_v2_b200 import LibraryInjector, ops
 from tests._fixtures import TinyReader
-from tests.test_gpu_shrink import D_M, DEV, LAYERS, interface, library
+from tests.test_gpu_shrink import D_M, D_S, DEV, LAYERS, interface, library
 
 pytestmark = pytest.mark.gpu
 
@@ -102,4 +102,68 @@ def test_summary_keys_that_are_not_finite_leave_no_trace_in_the_mass():
     with torch.no_grad():
         inj._inject(h, 1)
     assert torch.equal(got, inj.slot_mass[1])
+    inj.detach()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_weight_prepared_on_another_stream(fp8):
+    lib, h = library(60), torch.randn(3, 2, D_M, generator=torch.Generator(device="cuda").manual_seed(61), device="cuda")
+    outs = []
+    for late in (False, True):
+        inj = LibraryInjector(TinyReader(D_M, 5).cuda(), interface(62), top_k=2, cuda_graphs=False)
+        inj.load_library(lib)
+        inj.gemm_fp8 = fp8
+        one, two = torch.cuda.Stream(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.no_grad():
+            if late:  # the weights are written 20 ms from now, in memory that held NaN
+                with torch.cuda.stream(one):
+                    for n in (64 * 128, 96 * 128, 1 << 20):
+                        torch.full((n,), float("nan"), device="cuda")
+                    torch.cuda._sleep(40_000_000)
+                    inj._inject(h, 1)
+            with torch.cuda.stream(two):
+                outs.append(inj._inject(h, 1)[0])
+        torch.cuda.synchronize()
+        inj.detach()
+    assert torch.equal(outs[0], outs[1]) and not torch.equal(outs[0], h)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_weight_first_used_in_a_callers_capture(fp8):
+    lib, h = library(63), torch.randn(3, 2, D_M, generator=torch.Generator(device="cuda").manual_seed(64), device="cuda")
+    itf, outs = interface(65), []
+    for captured in (False, True):
+        inj = LibraryInjector(TinyReader(D_M, 5).cuda(), itf, top_k=2, cuda_graphs=False)
+        inj.load_library(lib)
+        inj.gemm_fp8 = fp8
+        graph = torch.cuda.CUDAGraph()
+        with torch.no_grad():
+            if captured:
+                with torch.cuda.graph(graph):
+                    inj._inject(h, 1)
+            outs.append(inj._inject(h, 1)[0])  # before any replay
+        inj.detach()
+    assert torch.equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_captured_step_keeps_its_weights(fp8):
+    """A caller's graph reads the prepared weights in place: others that come later do not push them out."""
+    lib, h = library(66), torch.randn(3, 2, D_M, generator=torch.Generator(device="cuda").manual_seed(67), device="cuda")
+    inj = LibraryInjector(TinyReader(D_M, 5).cuda(), interface(68), top_k=2, cuda_graphs=False)
+    inj.load_library(lib)
+    inj.gemm_fp8 = fp8
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad():
+        want = inj._inject(h, 1)[0]
+        with torch.cuda.graph(graph):
+            got = inj._inject(h, 1)[0]
+        others = [torch.full((D_S, D_M), float(i), device="cuda") for i in range(100)]
+        for W in others:
+            inj._weight(W)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+    assert torch.equal(got, want) and not torch.equal(want, h)
     inj.detach()
