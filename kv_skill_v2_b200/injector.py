@@ -475,7 +475,10 @@ class LibraryInjector(XEncInjector):
         self._graphs.clear()
         super().load(skill)
 
-    def load_library(self, lib) -> None:
+    def load_library(self, lib, slot_mass: Optional[dict] = None) -> None:
+        """lib is what the hooks read from here on. slot_mass: attention that was recorded over its pages ({layer: [pages,
+        page_rows] float32}, taken along by PagedLibrary.fork, compact and evict), to which record_mass goes on adding, in
+        place; pages that a reserve has added since have none. Without it recording starts anew."""
         self._graphs.clear()
         self.slot_mass = {}
         if lib.d_s != self.itf.d_s:
@@ -501,6 +504,17 @@ class LibraryInjector(XEncInjector):
                         raise ValueError(f"PagedLibrary layer {li}: a chunk has no valid slot (the softmax read is NaN)")
         else:
             raise TypeError(f"load_library expects a Library or PagedLibrary, got {type(lib).__name__}")
+        if slot_mass:
+            kept = {}
+            for li, m in slot_mass.items():
+                slots = (lib.pages(li, dev, self.slot_dtype) if isinstance(lib, Library) else lib.pages(li)).slots
+                P, N = slots.shape[:2]
+                if m.dtype != torch.float32 or m.dim() != 2 or m.shape[1] != N or m.shape[0] > P or not m.is_contiguous() \
+                        or m.device != slots.device:
+                    raise ValueError(f"slot_mass of layer {li} must be a contiguous float32 [{P}, {N}] tensor on "
+                                     f"{slots.device}, got {m.dtype} {list(m.shape)} on {m.device}")
+                kept[li] = m if m.shape[0] == P else nn.functional.pad(m, (0, 0, 0, P - m.shape[0]))
+            self.slot_mass = kept
         self.lib = lib
 
     def unload(self) -> None:

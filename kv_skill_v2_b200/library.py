@@ -326,15 +326,32 @@ class PagedLibrary:
             new[pool.data_ptr()] = big
         return self._with_tables(page_of, n_valid, nco, None, new)
 
-    def fork(self, parents, own_from=None) -> "PagedLibrary":
+    def _masses(self, mass) -> list:
+        """Recorded attention ([P, page_rows], or {layer: ...}) as pools of one float32 a row."""
+        if mass is None:
+            return []
+        first = self._pages[self.layers[0]]
+        out = []
+        for m in (mass.values() if isinstance(mass, dict) else [mass]):
+            if m.dtype != torch.float32 or tuple(m.shape) != tuple(first.slots.shape[:2]) or not m.is_contiguous() \
+                    or m.device != first.device:
+                raise ValueError(f"mass must be a contiguous float32 {list(first.slots.shape[:2])} tensor on {first.device}, "
+                                 f"got {m.dtype} {list(m.shape)} on {m.device}")
+            out.append(m.unsqueeze(-1))
+        return out
+
+    def fork(self, parents, own_from=None, mass=None) -> "PagedLibrary":
         """These Libraries and, behind them, one fork of each of `parents`. A fork shares its parent's pages for the
         chunks below own_from (an int, or one per fork; default: all of them) and has pages of its own, holding copies,
         for the rest, so that they can be rewritten for one request alone. RuntimeError when the pools have too few free
         pages (reserve). Reads one integer back from the device. Fork from the newest: a page that no row of this
-        PagedLibrary names counts as free, also where another fork of it, or one made from a select(), has taken it."""
+        PagedLibrary names counts as free, also where another fork of it, or one made from a select(), has taken it.
+        mass: attention recorded over these pages ([P, page_rows] float32, or one per layer as LibraryInjector.slot_mass):
+        a fork's own pages take their parents' on, in place. Without it they have what the free page had."""
         from .ops import pages_fork
 
         pools, page_of, n_valid, nco = self._tables()
+        masses = self._masses(mass)
         r = self._rows(parents)
         m = r.numel()
         own = torch.as_tensor(self.n_chunks if own_from is None else own_from, dtype=torch.int32)
@@ -345,21 +362,31 @@ class PagedLibrary:
         child, missing = pages_fork(pools, page_of, n_valid, r.to(torch.int32), own, n_chunks_of=nco)
         if int(missing):
             raise RuntimeError(f"fork: the pools have {int(missing)} free pages too few (PagedLibrary.reserve)")
+        if masses:  # (the same pages again; beside the slots their short rows would be the unit of every copy)
+            pages_fork(masses, page_of, n_valid, r.to(torch.int32), own, n_chunks_of=nco)
         rows = torch.cat([torch.arange(self.n_lib, device=r.device), r])
         return self._with_tables(torch.cat([page_of, child]), n_valid.index_select(0, rows).contiguous(),
                                  None if nco is None else nco.index_select(0, rows).contiguous(), rows)
 
-    def compact(self):
+    def compact(self, mass=None):
         """(the same Libraries with their pages moved to the front of the pools, the number n of pages in use): pages
-        [n, P) are free. The pools are this one's, so this PagedLibrary and any select() of it must no longer be read."""
+        [n, P) are free. The pools are this one's, so this PagedLibrary and any select() of it must no longer be read.
+        mass: attention recorded over these pages, as in fork; it moves with them, in place. What was recorded before a
+        compact and did not take part in it belongs to other pages than its numbers now say."""
         from .ops import pages_compact
 
         pools, page_of, n_valid, nco = self._tables()
-        table, n_live = pages_compact(pools, page_of.contiguous(), n_valid.contiguous(), n_chunks_of=nco)
+        masses = self._masses(mass)
+        page_of, n_valid = page_of.contiguous(), n_valid.contiguous()
+        table, n_live = pages_compact(pools, page_of, n_valid, n_chunks_of=nco)
+        if masses:  # (the same moves again, as in fork)
+            pages_compact(masses, page_of, n_valid, n_chunks_of=nco)
         return self._with_tables(table, n_valid, nco, None), int(n_live)
 
-    def evict(self, mass, keep, *, per_library: bool = False, floor: int = 1, page_rows: Optional[int] = None):
-        """(these Libraries without the slots that received least attention, the mass [P, rows] of those that stay).
+    def evict(self, mass, keep, *, per_library: bool = False, floor: int = 1, page_rows: Optional[int] = None,
+              per_layer: bool = False):
+        """(these Libraries without the slots that received least attention, the mass [P, rows] of those that stay; with
+        per_layer, and mass of each layer, {layer: [P, rows]}: what LibraryInjector.load_library takes on).
 
         mass: a [P, page_rows] tensor as ops.read_mass gives it, or one per layer ({layer: tensor}, as a LibraryInjector
         with record_mass holds them): these are added up, so that a token's slots stay or go at every depth alike. keep,
@@ -378,7 +405,10 @@ class PagedLibrary:
         page_of, n_valid = page_of.contiguous(), n_valid.contiguous()
         if page_of.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("evict reads a flag back from the device and cannot be captured (ops.pages_evict can)")
-        if isinstance(mass, dict):
+        layers = mass if isinstance(mass, dict) else None
+        if per_layer and layers is None:
+            raise ValueError("evict: per_layer takes the mass of each layer")
+        if layers is not None:
             if not mass:
                 raise ValueError("evict: mass of at least one layer is required")
             mass = torch.stack([mass[li] for li in sorted(mass)]).sum(0)
@@ -389,9 +419,12 @@ class PagedLibrary:
             blank = torch.empty(P, rows, 1, dtype=torch.float16, device=pools[0].device)
             nv = pages_evict([blank], page_of, n_valid, mass, keep, page_rows=rows, **how)[0]
             self._refuse_empty(nv, page_of, n_valid, nco)
-        nv, new_mass, _, new = pages_evict(pools, page_of, n_valid, mass, keep, page_rows=page_rows, **how)
+        nv, new_mass, kept, new = pages_evict(pools, page_of, n_valid, mass, keep, page_rows=page_rows, **how)
         if page_rows is not None:
             self._refuse_empty(nv, page_of, n_valid, nco)
+        if per_layer:
+            at = kept.clamp(min=0).long()
+            new_mass = {li: torch.where(kept >= 0, m.gather(1, at), 0.0) for li, m in layers.items()}
         renamed = {p.data_ptr(): q for p, q in zip(pools, new)}
         return self._with_tables(page_of, nv, nco, None, renamed), new_mass
 

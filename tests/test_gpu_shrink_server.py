@@ -1,5 +1,5 @@
 """What a server does around a Library that shrinks: evictions that are refused leave it whole, one bad request does not
-spoil the attention that others recorded, weights are prepared once for every stream and capture."""
+spoil the attention that others recorded, recorded attention goes with the pages when they are forked, moved or evicted."""
 
 from __future__ import annotations
 
@@ -8,7 +8,7 @@ import torch
 
 from kv_skill_v2_b200 import LibraryInjector, ops
 from tests._fixtures import TinyReader
-from tests.test_gpu_shrink import D_M, D_S, DEV, LAYERS, interface, library
+from tests.test_gpu_shrink import D_M, D_S, DEV, LAYERS, chunks, interface, library, step
 
 pytestmark = pytest.mark.gpu
 
@@ -166,4 +166,85 @@ def test_a_captured_step_keeps_its_weights(fp8):
         graph.replay()
         torch.cuda.synchronize()
     assert torch.equal(got, want) and not torch.equal(want, h)
+    inj.detach()
+
+
+def of_slots(lib):
+    """A mass that says which slot it belongs to, another for every layer."""
+    return {li: lib.pages(li).slots[..., li].float().contiguous() for li in LAYERS}
+
+
+def belongs(mass, lib):
+    """Every valid slot's mass is its own."""
+    for li in LAYERS:
+        p = lib.pages(li)
+        assert tuple(mass[li].shape) == tuple(p.slots.shape[:2])
+        for b in range(lib.n_lib):
+            for c in range(chunks(lib, b)):
+                page, nv = int(p.page_of[b, c]), int(p.n_valid[b, c])
+                assert nv > 0 and torch.equal(mass[li][page, :nv], p.slots[page, :nv, li].float())
+
+
+@pytest.mark.parametrize("new_rows", [None, 9])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_recorded_attention_goes_with_its_pages(new_rows, ragged):
+    """reserve, fork, drop, compact, evict and load_library, as requests join and leave."""
+    lib = library(70, ragged=ragged)
+    inj = LibraryInjector(TinyReader(D_M, 5).cuda(), interface(71), top_k=2)
+    mass = of_slots(lib)
+    lib = lib.reserve(9)
+    inj.load_library(lib, slot_mass=mass)
+    mass = inj.slot_mass
+    belongs(mass, lib)
+    held = {li: mass[li].data_ptr() for li in LAYERS}
+    for m in mass.values():
+        m[15:] = 7.0  # what is left in free pages by those that were there
+    lib = lib.fork([0, 2], own_from=[1, 2], mass=mass)
+    belongs(mass, lib)
+    lib = lib.drop([0, 1])
+    lib, n_live = lib.compact(mass=mass)
+    belongs(mass, lib)
+    assert n_live < 15 and {li: mass[li].data_ptr() for li in LAYERS} == held
+    lib, mass = lib.evict(mass, 8, page_rows=new_rows, per_layer=True)
+    belongs(mass, lib)
+    inj.load_library(lib, slot_mass=mass)
+    # recording goes on from there
+    inj.record_mass = True
+    h = torch.randn(lib.n_lib, 3, D_M, generator=torch.Generator(device="cuda").manual_seed(72), device="cuda")
+    before = mass[1].double()
+    with torch.no_grad():
+        inj._inject(h, 1)
+    want = before + step(h, inj.itf, lib, 1, 2)[1]
+    assert inj.slot_mass[1] is mass[1] and float((mass[1] - want).abs().max()) <= 1e-4 * float(want.abs().max())
+    inj.detach()
+
+
+def test_one_mass_for_all_layers_goes_with_its_pages():
+    lib = library(73, rows=203).reserve(4)  # 203 floats: rows of no 16 bytes
+    mass = of_slots(lib)[1]
+    lib = lib.fork([0], own_from=[3], mass=mass).drop([1])
+    lib, _ = lib.compact(mass=mass)
+    p = lib.pages(1)
+    for b in range(lib.n_lib):
+        for c in range(chunks(lib, b)):
+            page, nv = int(p.page_of[b, c]), int(p.n_valid[b, c])
+            assert torch.equal(mass[page, :nv], p.slots[page, :nv, 1].float())
+
+
+def test_masses_that_do_not_fit_are_refused():
+    lib = library(74).reserve(3)
+    P, N = lib.pages(1).slots.shape[:2]
+    inj = LibraryInjector(TinyReader(D_M, 5).cuda(), interface(75), top_k=2)
+    table, slots = lib.pages(1).page_of.clone(), lib.pages(1).slots.clone()
+    for bad in (torch.zeros(P - 1, N, device="cuda"), torch.zeros(P, N, device="cuda", dtype=torch.float64),
+                torch.zeros(N, P, device="cuda").t(), torch.zeros(P, N)):
+        for call in (lambda: lib.fork([0], own_from=4, mass=bad), lambda: lib.compact(mass={1: bad})):
+            with pytest.raises(ValueError, match="mass must be"):
+                call()
+    for bad in (torch.zeros(P + 1, N, device="cuda"), torch.zeros(P, N + 1, device="cuda"), torch.zeros(P, N, device="cuda").half()):
+        with pytest.raises(ValueError, match="slot_mass of layer 3"):
+            inj.load_library(lib, slot_mass={3: bad})
+    with pytest.raises(ValueError, match="each layer"):
+        lib.evict(torch.zeros(P, N, device="cuda"), 4, per_layer=True)
+    assert torch.equal(lib.pages(1).page_of, table) and torch.equal(lib.pages(1).slots, slots)
     inj.detach()
