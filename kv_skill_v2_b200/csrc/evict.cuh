@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(PG_THREADS) evict_budget_kernel(const EvictArg
   int n_first, n_others;
   pg_scan(first, sh, &n_first);
   pg_scan(others, sh, &n_others);
-  int left = (a.keep ? a.keep[lib] : a.keep_all) - n_first;
+  int left = max(0, a.keep ? a.keep[lib] : a.keep_all) - n_first;
   if (left <= 0 || n_others == 0) return;
   uint32_t last = 1u;  // the order of the last mass that stays
   bool cut = false;    // not all of that mass stay

@@ -187,6 +187,17 @@ def test_one_library_one_page_twice_and_keeps_below_zero(per_library):
     check(*a, keep.cuda(), keep.tolist(), per_library=per_library, floor=40, M=12)
 
 
+@pytest.mark.parametrize("per_library", [False, True])
+def test_the_least_keep_there_is(per_library):
+    # a budget below zero is one of nothing, also where the floor's rows would take it below what 32 bits hold
+    a = case(86, 3, 4, 12, 40, 24, [F16])
+    least = -2**31
+    keep = torch.full((3,) if per_library else (3, 4), least, dtype=torch.int32)
+    keep[1] = least + 3
+    for floor in (0, 2):
+        check(*a, keep.cuda(), keep.tolist(), per_library=per_library, floor=floor, M=30)
+
+
 def test_more_pools_than_one_launch_moves():
     dtypes = [F16, BF16, F32] * 25
     check(*case(81, 2, 3, 8, 20, 16, dtypes), 7, [[7] * 3] * 2, M=9)
