@@ -104,7 +104,6 @@ __device__ __forceinline__ uint2 f8_quant8(const float* v, bool in, int* e) {
 
 // What the projection takes of a row besides its 8-bit form (project_in): 1/rms and the gate.
 struct F8RowStats {
-  int weight;           // a weight, not rows: the products load one before their wait, so nothing may start before its end
   int rms;
   float eps;
   const float* gate_w;  // [K] or null
@@ -148,7 +147,7 @@ __global__ void __launch_bounds__(f8q_threads<T>(), sizeof(T) == 4 ? 8 : 6) quan
                                                                uint8_t* __restrict__ x8, uint8_t* __restrict__ scale,
                                                                int stride, const F8RowStats st) {
   __shared__ float2 red[32];
-  if (!st.weight) pdl_trigger();
+  pdl_trigger();
   pdl_wait();
   const int64_t m = blockIdx.x;
   const T* row = x + m * K;
@@ -292,37 +291,24 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_f8_kernel(const __grid_con
   __syncthreads();
   tc_fence_after();
   const uint32_t taddr = *tmem_slot;
-  // one stage of weights before the wait, as the 3xF16 GEMM does (xencb_quant8, which writes them, lets no grid start
-  // before its end)
-  const int npre = min(nkb, 1);
-  if (threadIdx.x != 0) {
-    pdl_wait();
-    pdl_trigger();
-  }
+  const uint64_t keep = policy_evict_last();
+  // The first weights are asked into L2 before the wait, and read behind it: what wrote them (xencb_quant8, a copy) may be
+  // the launch before this one.
+  if (threadIdx.x == 0 && nkb > 0) tma_prefetch_2d(&map_w, b0 * F8_BK, n0, keep);
+  pdl_wait();
+  pdl_trigger();
   if (a.row_done && blockIdx.x == 0 && blockIdx.z == 0)
-    for (int64_t i = m0 + threadIdx.x; i < min(a.M, m0 + BN); i += blockDim.x)
-      if (threadIdx.x != 0) a.row_done[i] = 0;
+    for (int64_t i = m0 + threadIdx.x; i < min(a.M, m0 + BN); i += blockDim.x) a.row_done[i] = 0;
 
   if (warp == 0) {
     if (lane == 0) {
-      const uint64_t keep = policy_evict_last();
-      for (int kb = 0; kb < npre; ++kb) {
-        mbar_arrive_expect_tx(&full[kb], FUSED ? F8_BM * F8_BK : STAGE);
-        tma_load_2d_hint(smem + kb * STAGE, &map_w, (b0 + kb) * F8_BK, n0, &full[kb], keep);
-      }
-      pdl_wait();
-      pdl_trigger();
-      if (a.row_done && blockIdx.x == 0 && blockIdx.z == 0)
-        for (int64_t i = m0; i < min(a.M, m0 + BN); i += blockDim.x) a.row_done[i] = 0;
       uint32_t used = 0;
       for (int kb = 0; kb < nkb; ++kb) {
         const int s = kb % STAGES, use = kb / STAGES;
         if (use > 0 && (!mbar_wait_spin(&sfree[s], (use - 1) & 1) || *abort_flag)) { *abort_flag = 1; break; }
         unsigned char* st = smem + s * STAGE;
-        if (kb >= npre) {
-          mbar_arrive_expect_tx(&full[s], FUSED ? F8_BM * F8_BK : STAGE);
-          tma_load_2d_hint(st, &map_w, (b0 + kb) * F8_BK, n0, &full[s], keep);
-        }
+        mbar_arrive_expect_tx(&full[s], FUSED ? F8_BM * F8_BK : STAGE);
+        tma_load_2d_hint(st, &map_w, (b0 + kb) * F8_BK, n0, &full[s], keep);
         if (!FUSED) tma_load_2d(st + F8_BM * F8_BK, &map_x, (b0 + kb) * F8_BK, (int)m0, &full[s]);
         used = kb + 1;
       }

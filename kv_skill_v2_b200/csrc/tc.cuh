@@ -210,6 +210,13 @@ __device__ __forceinline__ void tma_load_2d_hint(void* smem_dst, const CUtensorM
       : "memory");
 }
 
+// Asks L2 for the box of such a load. Nothing is read, so it may come before what writes the box is known to have ended.
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y, uint64_t policy) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile.L2::cache_hint [%0, {%1, %2}], %3;" ::"l"(map), "r"(x),
+               "r"(y), "l"(policy)
+               : "memory");
+}
+
 // ---- pairs of CTAs (cta_group::2): a 2-CTA cluster whose tensor-core work is issued by the even CTA.
 // TMEM allocation for the pair: issued by the same warp in both CTAs, the address written to the same shared
 // offset in each.

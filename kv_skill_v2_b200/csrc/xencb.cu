@@ -1215,7 +1215,7 @@ static int project_in_impl(const void* h, int h_dtype, int64_t n_rows, int d_m, 
   if (w8 && p8.rows && !sel_w) {
     float* rstd = rstd_out ? rstd_out : reinterpret_cast<float*>(ws + p8.out_bytes + p8.x8_bytes + p8.sx_bytes);
     uint8_t* x8 = reinterpret_cast<uint8_t*>(ws + p8.out_bytes);
-    const F8RowStats stats{0, (flags & XENCB_PIN_RMS) ? 1 : 0, rms_eps, gate_w, gate_b, gate_b_dev, rstd,
+    const F8RowStats stats{(flags & XENCB_PIN_RMS) ? 1 : 0, rms_eps, gate_w, gate_b, gate_b_dev, rstd,
                            gate_w ? gate_out : nullptr};
     rc = launch_quant_f8(h, h_dtype, n_rows, d_m, x8, x8 + p8.x8_bytes, p8.sx_stride, stats, st);
     if (rc) return rc;
@@ -2210,7 +2210,7 @@ int xencb_quant8(const void* x, int dtype, int64_t n, int k, void* x8, void* sca
   const int rc = device_info(&di);
   if (rc) return rc;
   if (n > INT32_MAX) return fail(XENCB_ENOTSUP, "quant8: too many rows");
-  return launch_quant_f8(x, dtype, n, k, x8, static_cast<uint8_t*>(scale), (k + F8_BK - 1) / F8_BK, F8RowStats{1},
+  return launch_quant_f8(x, dtype, n, k, x8, static_cast<uint8_t*>(scale), (k + F8_BK - 1) / F8_BK, F8RowStats{},
                          static_cast<cudaStream_t>(stream));
 }
 
