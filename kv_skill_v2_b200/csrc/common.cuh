@@ -26,8 +26,8 @@ __device__ __forceinline__ void flag_error(unsigned int bits) { atomicOr(&g_dev_
 // merge, the row split, the 3xF16 GEMM, the projection row kernels, the fused decode router, the adapters' shrink and
 // expand, the shared read's split, read and combine, and the page copies). pdl_wait()
 // returns once the grid before this one in the stream has completed and its writes are visible (a no-op for a
-// plain launch). Before it such a kernel only reads, and only data that no kernel still running can be writing:
-// the GEMM's weight tiles and the router's summary keys (Library data), the row kernels' hidden-state rows
+// plain launch). Before it such a kernel only asks L2 for data (the GEMMs' weight tiles, the router's summary keys), and
+// reads only what no kernel still running can be writing: the row kernels' hidden-state rows
 // (they start after the GEMM has passed its own wait, so the kernel that wrote h has completed; with an expand in
 // between, that starts after the GEMM's wait and they after it), and the shared read's q (its plan is a plain launch,
 // so whatever wrote q has completed). Nothing is written before the wait. pdl_trigger() lets the next grid be scheduled.

@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(SR_THREADS) split_rows_f16x2_kernel(const T* _
                                                                       __half* __restrict__ hi, __half* __restrict__ lo,
                                                                       float* __restrict__ inv_scale) {
   __shared__ float red[SR_THREADS / 32];
-  pdl_trigger();  // the GEMM that follows may start on its weight tiles now
+  pdl_trigger();  // the GEMM that follows may ask for its weight tiles now
   pdl_wait();
   const int64_t m = blockIdx.x;
   const T* xr = x + m * K;
@@ -224,39 +224,22 @@ __global__ void __launch_bounds__(H3_THREADS, MINB) gemm_f16x3_kernel(const __gr
   __syncthreads();
   tc_fence_after();
   const uint32_t taddr = *tmem_slot;
-  // Under programmatic dependent launch the producer requests the weight tiles of the first stage before the
-  // row split this GEMM reads has finished (no kernel of the step writes the weights); everything else waits.
+  const uint64_t keep = policy_evict_last();
+  // Under programmatic dependent launch the weight tiles of the first stage are asked into L2 before the row split this
+  // GEMM reads has finished, and read behind the wait: what wrote them (xencb_weights_prep) may be a launch just before.
   // One stage, not the whole ring: measured in the decode steps, requesting every stage early competes with the
   // kernels still running (config 2: 162.3 -> 161.2 us per step, config 4: 607 -> 597 us with one stage).
-  const int npre = min(nkb, 1);
-  if (threadIdx.x != 0) {
-    pdl_wait();
-    pdl_trigger();
-  }
+  if (threadIdx.x == 0 && nkb > 0) tma_prefetch_2d(&map_w, 0, wrow0, keep);
+  pdl_wait();
+  pdl_trigger();
   // zero the per-row completion counters the following reduce kernel counts on (stream order)
   if (row_done && blockIdx.x == 0 && blockIdx.z == 0)
-    for (int64_t i = m0 + threadIdx.x; i < min(M, m0 + H3_BN); i += blockDim.x)
-      if (threadIdx.x != 0) row_done[i] = 0;
+    for (int64_t i = m0 + threadIdx.x; i < min(M, m0 + H3_BN); i += blockDim.x) row_done[i] = 0;
 
   if (warp == 0) {
     // ------------------------------------------------------------------------------------------- producer
     if (lane == 0) {
-      const uint64_t keep = policy_evict_last();
-      for (int kb = 0; kb < npre; ++kb) {
-        unsigned char* st = smem + kb * H3_STAGE;
-        mbar_arrive_expect_tx(&full[kb], H3_STAGE);
-        tma_load_2d_hint(st, &map_w, 0, wrow0 + kb * 2 * H3_BM, &full[kb], keep);
-      }
-      pdl_wait();
-      pdl_trigger();
-      if (row_done && blockIdx.x == 0 && blockIdx.z == 0 && m0 < M) row_done[m0] = 0;
-      for (int kb = 0; kb < npre; ++kb) {
-        unsigned char* st = smem + kb * H3_STAGE;
-        const int k = kbeg + kb * H3_BK;
-        tma_load_2d(st + 2 * H3_WBOX, &map_x, k, (int)m0, &full[kb]);
-        tma_load_2d(st + 2 * H3_WBOX + H3_XBOX, &map_x, k, (int)(M + m0), &full[kb]);
-      }
-      for (int kb = npre; kb < nkb; ++kb) {
+      for (int kb = 0; kb < nkb; ++kb) {
         const int s = kb % STAGES, use = kb / STAGES;
         if (use > 0 && (!mbar_wait_spin(&sfree[s], (use - 1) & 1) || *abort_flag)) { *abort_flag = 1; break; }
         unsigned char* st = smem + s * H3_STAGE;

@@ -17,7 +17,7 @@ def kernels(path):
             yield re.search(r"\b\w+_kernel\b", text).group(), text
 
 
-@pytest.mark.parametrize("name", ["gemm_f8.cuh", "mass.cuh", "read_shared.cuh"])
+@pytest.mark.parametrize("name", ["gemm_f8.cuh", "gemm_f16x3.cuh", "mass.cuh", "read_shared.cuh"])
 def test_operands_are_loaded_behind_the_wait(name):
     """A launch may begin while the one before it runs; what that one wrote is there behind the wait only."""
     seen = 0
