@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define XENCB_ABI_VERSION 8
+#define XENCB_ABI_VERSION 9
 
 #if defined(__GNUC__)
 #define XENCB_API __attribute__((visibility("default")))
@@ -405,15 +405,19 @@ XENCB_API int xencb_project_out_adapted(const float* r, int64_t n_rows, int d_s,
  *   y[r, n] = sum over blocks b of 2^(e_x[r, b] + e_w[n, b]) * sum_{k in b} x8[r, k] w8[n, k]
  * in place of x @ W^T, accumulated in float32; the rows (h as it is given, r) are quantised in the call. Everything else,
  * 1/rms and the gate among it, comes from the rows in full. Any d_m (d_s) on the input side; outputs as there. A row
- * that holds a value that is not finite comes out as NaN. */
+ * that holds a value that is not finite comes out as NaN.
+ * Workspace: the matching *8_workspace bytes are enough for every call of these sizes; *8_workspace_for says what one with
+ * (selector != 0) or without sel_w needs. Many rows without a selector need far less, as no partial sums are written. */
 XENCB_API int xencb_quant8(const void* x, int dtype, int64_t n, int k, void* x8, void* scale, void* stream);
 XENCB_API size_t xencb_project_in8_workspace(int64_t n_rows, int d_m, int d_s);
+XENCB_API size_t xencb_project_in8_workspace_for(int64_t n_rows, int d_m, int d_s, int selector);
 XENCB_API int xencb_project_in8(const void* h, int h_dtype, int64_t n_rows, int d_m, const void* w8,
                                 const void* w_scale, const float* b_in, int d_s, int flags, const float* gate_w,
                                 float gate_b, const float* gate_b_dev, const float* sel_w, const float* sel_b,
                                 int n_cand, float rms_eps, float* q_out, float* gate_out, float* rstd_out,
                                 float* z_out, void* workspace, size_t workspace_bytes, void* stream);
 XENCB_API size_t xencb_project_out8_workspace(int64_t n_rows, int d_s, int d_m);
+XENCB_API size_t xencb_project_out8_workspace_for(int64_t n_rows, int d_s, int d_m, int selector);
 XENCB_API int xencb_project_out8(const float* r, int64_t n_rows, int d_s, const void* w8, const void* w_scale,
                                  const float* b_out, int d_m, float scale, const float* log_scale_dev,
                                  const float* gate, const float* sel_w, float log_alpha, const float* log_alpha_dev,

@@ -19,7 +19,7 @@ OK, EINVAL, ECUDA, ENOTSUP = 0, 1, 2, 3
 DEV_TIMEOUT, DEV_CLAMPED, DEV_BADPAGE, DEV_BADROWS, DEV_BADADAPTER = 1, 2, 4, 8, 16
 PIN_RMS, PIN_L2 = 1, 2
 NOALLOC_SCRATCH_BYTES = 16 << 20
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 _p, _i, _i64, _f, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
 
@@ -83,9 +83,11 @@ SIGNATURES: dict = {
                                        _p, _p, _i, _p, _i, _i, _p, _i64, _p, _sz, _p]),
     "xencb_quant8": (_i, [_p, _i, _i64, _i, _p, _p, _p]),
     "xencb_project_in8_workspace": (_sz, [_i64, _i, _i]),
+    "xencb_project_in8_workspace_for": (_sz, [_i64, _i, _i, _i]),
     "xencb_project_in8": (_i, [_p, _i, _i64, _i, _p, _p, _p, _i, _i, _p, _f, _p, _p, _p, _i, _f, _p, _p, _p, _p, _p, _sz,
                                _p]),
     "xencb_project_out8_workspace": (_sz, [_i64, _i, _i]),
+    "xencb_project_out8_workspace_for": (_sz, [_i64, _i, _i, _i]),
     "xencb_project_out8": (_i, [_p, _i64, _i, _p, _p, _p, _i, _f, _p, _p, _p, _f, _p, _p, _p, _i, _p, _p, _p, _p, _sz,
                                 _p]),
     "xencb_pages_fork_workspace": (_sz, [_i64, _i]),

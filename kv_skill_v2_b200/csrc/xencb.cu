@@ -349,7 +349,7 @@ struct Weight8 {
 
 struct F8Plan {
   int bn, nb, bps, sx_stride;
-  bool rows;  // gemm_f8_rows_kernel, where the call's arguments allow it
+  bool rows;  // gemm_f8_rows_kernel, which ends the projection: nothing of the workspace but this is used
   GemmPlan gp;
   size_t out_bytes, x8_bytes, sx_bytes, rstd_bytes, total;
 };
@@ -357,9 +357,10 @@ struct F8Plan {
 // Calls with tiles of 128 rows and 256 output features for a quarter of the device take gemm_f8_rows_kernel (captured
 // in / out, this form against split K: 2048 -> 4096, 384 rows 19.2 / 14.5 us against 20.1 / 20.7; 4096 -> 2048, 600 rows
 // 25.7 / 21.1 against 27.1 / 26.6, 1024 rows 26.4 / 22.5 against 36.4 / 35.2); it keeps two tiles' scale factors in tensor
-// memory, blocks of up to 40. The others split K: BN = 64 and 128 where all rows fit one tile (the CTAs stream the
-// weights), 256 where they do not, so that a weight tile is fetched a quarter as often.
-F8Plan plan_f8(int64_t M, int N, int K, int sms) {
+// memory, blocks of up to 40, and has no part in a LayerSelector's logits and matched norm (`selector`). The others split
+// K: BN = 64 and 128 where all rows fit one tile (the CTAs stream the weights), 256 where they do not, so that a weight tile
+// is fetched a quarter as often.
+F8Plan plan_f8(int64_t M, int N, int K, int sms, bool selector) {
   F8Plan p;
   p.bn = M <= 64 ? 64 : M <= 128 ? 128 : 256;
   p.nb = (K + F8_BK - 1) / F8_BK;
@@ -373,8 +374,8 @@ F8Plan plan_f8(int64_t M, int N, int K, int sms) {
   p.gp.part_bytes = align_up((size_t)p.gp.splits * (size_t)M * (size_t)N * sizeof(float), 256);
   p.sx_stride = (p.nb + 3) / 4 * 4;
   const int64_t tiles_n = (N + FR_BN - 1) / FR_BN;
-  p.rows = (p.nb + 3) / 4 <= FR_MAX_WORDS && 4 * tiles_n * ((M + FR_BM - 1) / FR_BM) >= sms;
-  p.out_bytes = std::max(p.gp.part_bytes, p.rows ? align_up((size_t)M * 2 * tiles_n * sizeof(float2), 256) : 0);
+  p.rows = !selector && (p.nb + 3) / 4 <= FR_MAX_WORDS && 4 * tiles_n * ((M + FR_BM - 1) / FR_BM) >= sms;
+  p.out_bytes = p.rows ? align_up((size_t)M * 2 * tiles_n * sizeof(float2), 256) : p.gp.part_bytes;
   p.x8_bytes = align_up((size_t)M * p.nb * F8_BK, 256);
   p.sx_bytes = align_up((size_t)M * p.sx_stride, 256);
   p.rstd_bytes = align_up((size_t)M * sizeof(float), 256);
@@ -1182,11 +1183,11 @@ static int project_in_impl(const void* h, int h_dtype, int64_t n_rows, int d_m, 
   if (rc) return rc;
   const int nch = (d_s + PIN_CHUNK - 1) / PIN_CHUNK;
   if (w8 && (rc = check_weight8("project_in8", *w8, n_rows, d_s))) return rc;
-  const F8Plan p8 = w8 ? plan_f8(n_rows, d_s, d_m, di.sms) : F8Plan{};
+  const F8Plan p8 = w8 ? plan_f8(n_rows, d_s, d_m, di.sms, sel_w != nullptr) : F8Plan{};
   const size_t slice = adapters ? adapt_part_extra(n_rows, d_s, d_m, di.sms) : 0;
   const size_t g_bytes = w8 ? p8.total : gemm_ws_bytes(n_rows, d_s, d_m, di.sms, true) + slice;
-  const size_t nq_bytes = align_up((size_t)n_rows * nch * sizeof(float), 256);
-  const size_t rd_bytes = align_up((size_t)n_rows * sizeof(int), 256);
+  const size_t nq_bytes = p8.rows ? 0 : align_up((size_t)n_rows * nch * sizeof(float), 256);
+  const size_t rd_bytes = p8.rows ? 0 : align_up((size_t)n_rows * sizeof(int), 256);
   const size_t need = g_bytes + nq_bytes + rd_bytes + (adapters ? adapt_t_bytes(n_rows, adapters->r) : 0);
   if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
     return fail(XENCB_EINVAL, "project_in: workspace needs %zu bytes, 256-byte aligned (got %zu)", need,
@@ -1212,7 +1213,7 @@ static int project_in_impl(const void* h, int h_dtype, int64_t n_rows, int d_m, 
     }
     if (rc) return rc;
   }
-  if (w8 && p8.rows && !sel_w) {
+  if (p8.rows) {
     float* rstd = rstd_out ? rstd_out : reinterpret_cast<float*>(ws + p8.out_bytes + p8.x8_bytes + p8.sx_bytes);
     uint8_t* x8 = reinterpret_cast<uint8_t*>(ws + p8.out_bytes);
     const F8RowStats stats{(flags & XENCB_PIN_RMS) ? 1 : 0, rms_eps, gate_w, gate_b, gate_b_dev, rstd,
@@ -2039,12 +2040,12 @@ static int project_out_impl(const float* r, int64_t n_rows, int d_s, const float
   if (rc) return rc;
   const int nch = (d_m + PIN_CHUNK - 1) / PIN_CHUNK;
   if (w8 && (rc = check_weight8("project_out8", *w8, n_rows, d_m))) return rc;
-  const F8Plan p8 = w8 ? plan_f8(n_rows, d_m, d_s, di.sms) : F8Plan{};
+  const F8Plan p8 = w8 ? plan_f8(n_rows, d_m, d_s, di.sms, sel_w != nullptr) : F8Plan{};
   const size_t slice = adapters ? adapt_part_extra(n_rows, d_m, d_s, di.sms) : 0;
   const size_t g_bytes = w8 ? p8.total : gemm_ws_bytes(n_rows, d_m, d_s, di.sms, false) + slice;
-  const size_t d_bytes = align_up((size_t)n_rows * d_m * sizeof(float), 256);
-  const size_t np_bytes = align_up((size_t)n_rows * nch * 3 * sizeof(float), 256);
-  const size_t rd_bytes = align_up((size_t)n_rows * sizeof(int), 256);
+  const size_t d_bytes = p8.rows ? 0 : align_up((size_t)n_rows * d_m * sizeof(float), 256);
+  const size_t np_bytes = p8.rows ? 0 : align_up((size_t)n_rows * nch * 3 * sizeof(float), 256);
+  const size_t rd_bytes = p8.rows ? 0 : align_up((size_t)n_rows * sizeof(int), 256);
   const size_t need = g_bytes + d_bytes + np_bytes + rd_bytes + (adapters ? adapt_t_bytes(n_rows, adapters->r) : 0);
   if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
     return fail(XENCB_EINVAL, "project_out: workspace needs %zu bytes, 256-byte aligned (got %zu)", need,
@@ -2066,7 +2067,7 @@ static int project_out_impl(const float* r, int64_t n_rows, int d_s, const float
     rc = launch_adapt_shrink<float>(r, ad, adapt_dtype, st);
     if (rc) return rc;
   }
-  if (w8 && p8.rows && !sel_w) {
+  if (p8.rows) {
     uint8_t* x8 = reinterpret_cast<uint8_t*>(ws + p8.out_bytes);
     rc = launch_quant_f8(r, XENCB_F32, n_rows, d_s, x8, x8 + p8.x8_bytes, p8.sx_stride, F8RowStats{}, st);
     if (rc) return rc;
@@ -2214,12 +2215,17 @@ int xencb_quant8(const void* x, int dtype, int64_t n, int k, void* x8, void* sca
                          static_cast<cudaStream_t>(stream));
 }
 
-size_t xencb_project_in8_workspace(int64_t n_rows, int d_m, int d_s) {
+size_t xencb_project_in8_workspace_for(int64_t n_rows, int d_m, int d_s, int selector) {
   DevInfo di;
   if (n_rows <= 0 || d_m <= 0 || d_s <= 0 || device_info(&di)) return 0;
+  const F8Plan p = plan_f8(n_rows, d_s, d_m, di.sms, selector != 0);
+  if (p.rows) return p.total;
   const int nch = (d_s + PIN_CHUNK - 1) / PIN_CHUNK;
-  return plan_f8(n_rows, d_s, d_m, di.sms).total + align_up((size_t)n_rows * nch * sizeof(float), 256) +
-         align_up((size_t)n_rows * sizeof(int), 256);
+  return p.total + align_up((size_t)n_rows * nch * sizeof(float), 256) + align_up((size_t)n_rows * sizeof(int), 256);
+}
+
+size_t xencb_project_in8_workspace(int64_t n_rows, int d_m, int d_s) {
+  return std::max(xencb_project_in8_workspace_for(n_rows, d_m, d_s, 0), xencb_project_in8_workspace_for(n_rows, d_m, d_s, 1));
 }
 
 int xencb_project_in8(const void* h, int h_dtype, int64_t n_rows, int d_m, const void* w8, const void* w_scale,
@@ -2232,12 +2238,18 @@ int xencb_project_in8(const void* h, int h_dtype, int64_t n_rows, int d_m, const
                          nullptr, nullptr, 0, &w);
 }
 
-size_t xencb_project_out8_workspace(int64_t n_rows, int d_s, int d_m) {
+size_t xencb_project_out8_workspace_for(int64_t n_rows, int d_s, int d_m, int selector) {
   DevInfo di;
   if (n_rows <= 0 || d_m <= 0 || d_s <= 0 || device_info(&di)) return 0;
+  const F8Plan p = plan_f8(n_rows, d_m, d_s, di.sms, selector != 0);
+  if (p.rows) return p.total;
   const int nch = (d_m + PIN_CHUNK - 1) / PIN_CHUNK;
-  return plan_f8(n_rows, d_m, d_s, di.sms).total + align_up((size_t)n_rows * d_m * sizeof(float), 256) +
+  return p.total + align_up((size_t)n_rows * d_m * sizeof(float), 256) +
          align_up((size_t)n_rows * nch * 3 * sizeof(float), 256) + align_up((size_t)n_rows * sizeof(int), 256);
+}
+
+size_t xencb_project_out8_workspace(int64_t n_rows, int d_s, int d_m) {
+  return std::max(xencb_project_out8_workspace_for(n_rows, d_s, d_m, 0), xencb_project_out8_workspace_for(n_rows, d_s, d_m, 1));
 }
 
 int xencb_project_out8(const float* r, int64_t n_rows, int d_s, const void* w8, const void* w_scale, const float* b_out,

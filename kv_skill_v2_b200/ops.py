@@ -268,7 +268,7 @@ def project_in(h2: torch.Tensor, w_in, b_in=None, *, rms: bool = True, l2: bool 
     gb, gb_dev = _dev_scalar(gate_b, "gate_b")
     with _on_device(dev):
         if w8 is not None:
-            ws = _workspace(_workspace_bytes(dev, "xencb_project_in8_workspace", R, d_m, d_s), dev)
+            ws = _workspace(_workspace_bytes(dev, "xencb_project_in8_workspace_for", R, d_m, d_s, sel_w is not None), dev)
             N.call("xencb_project_in8", _ptr(h2), _hdt(h2, "h"), R, d_m, w8_at, w8_scale, _ptr(b_in), d_s, flags,
                    _ptr(gate_w), gb, _ptr(gb_dev), _ptr(sel_w), _ptr(sel_b), n_cand, eps, _ptr(q), _ptr(gate),
                    _ptr(rstd), _ptr(z), _ptr(ws), ws.numel(), _stream(dev))
@@ -427,7 +427,7 @@ def project_out(r: torch.Tensor, w_out, h2: torch.Tensor, *, b_out=None, scale: 
     ls_dev = None if log_scale is None else _dev_scalar(log_scale, "log_scale")[1]
     with _on_device(dev):
         if w8 is not None:
-            ws = _workspace(_workspace_bytes(dev, "xencb_project_out8_workspace", R, d_s, d_m), dev)
+            ws = _workspace(_workspace_bytes(dev, "xencb_project_out8_workspace_for", R, d_s, d_m, sel_w is not None), dev)
             N.call("xencb_project_out8", _ptr(r), R, d_s, w8_at, w8_scale, _ptr(b_out), d_m, float(scale),
                    _ptr(ls_dev), _ptr(gate), _ptr(sel_w), la, _ptr(la_dev), _ptr(pos_mask), _ptr(h2), _hdt(h2, "h"),
                    _ptr(delta), _ptr(h_out), _ptr(rel), _ptr(ws), ws.numel(), _stream(dev))

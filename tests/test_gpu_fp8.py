@@ -12,6 +12,7 @@ import math
 import pytest
 import torch
 
+from kv_skill_v2_b200 import _native as N
 from kv_skill_v2_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -266,3 +267,43 @@ def test_refusals():
         ops.project_in(h, w8, adapters=a, adapter_of=torch.zeros(4, dtype=torch.int32, device="cuda"))
     with pytest.raises(ValueError):
         ops.project_out(h, w8, torch.zeros(4, 60, device="cuda"))
+
+
+@pytest.mark.parametrize("R,d_in,d_out", [(1, 300, 64), (9, 256, 512), (70, 512, 1024), (200, 640, 260), (1024, 1024, 2048),
+                                          (6000, 384, 1284)])
+@pytest.mark.parametrize("selector", [False, True])
+def test_the_workspace_of_a_call_is_enough_and_no_less_is(R, d_in, d_out, selector):
+    g, guard = gen(50), 4096
+    h, W = rows(R, d_in, 51, dtype=torch.bfloat16), rows(d_out, d_in, 52) * d_in ** -0.5
+    r, hm = rows(R, d_in, 53), torch.randn(R, d_out, generator=g, device="cuda").to(torch.bfloat16)
+    sel_in, sel_row = torch.randn(3, d_in, generator=g, device="cuda") * 0.02, torch.rand(R, generator=g, device="cuda")
+    w8 = ops.weights_fp8(W)
+    want_q, _, _, want_z = ops.project_in(h, w8, sel_w=sel_in if selector else None)
+    want = ops.project_out(r, w8, hm, sel_w=sel_row if selector else None, want_rel=True)
+    q, z = torch.empty_like(want_q), torch.empty(R, 3, device="cuda")
+    delta, rel = torch.empty_like(hm), torch.empty(R, device="cuda")
+    at, stream = (lambda t: None if t is None else t.data_ptr()), torch.cuda.current_stream().cuda_stream
+    calls = [("xencb_project_in8", N.lib().xencb_project_in8_workspace_for(R, d_in, d_out, selector),
+              N.lib().xencb_project_in8_workspace(R, d_in, d_out), lambda ws, n: N.lib().xencb_project_in8(
+                  at(h), N.BF16, R, d_in, at(w8.w), at(w8.scale), None, d_out, N.PIN_RMS | N.PIN_L2, None, 0.0, None,
+                  at(sel_in) if selector else None, None, 3 if selector else 0, 1e-6, at(q), None, None,
+                  at(z) if selector else None, ws, n, stream)),
+             ("xencb_project_out8", N.lib().xencb_project_out8_workspace_for(R, d_in, d_out, selector),
+              N.lib().xencb_project_out8_workspace(R, d_in, d_out), lambda ws, n: N.lib().xencb_project_out8(
+                  at(r), R, d_in, at(w8.w), at(w8.scale), None, d_out, 1.0, None, None, at(sel_row) if selector else None,
+                  0.0, None, None, at(hm), N.BF16, at(delta), None, at(rel), ws, n, stream))]
+    for name, need, most, call in calls:
+        assert 0 < need <= most, name
+        ws = torch.full((need + guard,), 0x5A, dtype=torch.uint8, device="cuda")
+        assert call(at(ws), need - 1) == N.EINVAL and call(at(ws), need) == N.OK, name
+        assert bool((ws[need:] == 0x5A).all()), name
+    assert torch.equal(q, want_q) and (not selector or torch.equal(z, want_z))
+    assert torch.equal(delta, want[0]) and torch.equal(rel, want[2])
+
+
+def test_many_rows_do_not_ask_for_partial_sums():
+    # 8-bit rows, their factors, 1/rms and two sums for every 128 outputs of a row
+    for query, d_in, d_out in (("in8", 5120, 2048), ("out8", 2048, 4096)):
+        size = getattr(N.lib(), f"xencb_project_{query}_workspace_for")
+        assert size(16384, d_in, d_out, 0) <= 16384 * (d_in + d_in // 128 + 4 + d_out // 128 * 8) + 1024
+        assert size(16384, d_in, d_out, 1) > 16384 * d_out * 4
