@@ -2418,6 +2418,15 @@ int xencb_pages_evict(const void* const* pools, void* const* pools_out, const in
   if (new_rows <= 0 || new_rows > page_rows)
     return fail(XENCB_EINVAL, "pages_evict: new_rows=%d must be 1 .. page_rows=%d", new_rows, page_rows);
   if (floor < 0) return fail(XENCB_EINVAL, "pages_evict: floor=%d must not be negative", floor);
+  // the pools of each launch move in units of 16 bytes where all of them can; a page's units fit 31 bits
+  const auto launch_unit = [&](int i0) {
+    for (int i = i0; i < std::min(n_pools, i0 + PG_POOLS); ++i)
+      if (!aligned(pools[i], 16) || !aligned(pools_out[i], 16) || row_bytes[i] % 16 != 0) return 2;
+    return 16;
+  };
+  for (int i = 0; i < n_pools; ++i)  // (known before anything moves)
+    if (row_bytes[i] / launch_unit(i / PG_POOLS * PG_POOLS) > INT32_MAX / page_rows)
+      return fail(XENCB_ENOTSUP, "pages_evict: the pages of pool %d are too large", i);
   int inplace = 0;
   for (int i = 0; i < n_pools; ++i) inplace += pools_out[i] == pools[i];
   if (inplace && (inplace != n_pools || new_rows != page_rows))
@@ -2482,22 +2491,19 @@ int xencb_pages_evict(const void* const* pools, void* const* pools_out, const in
   for (int i0 = 0; i0 < n_pools; i0 += PG_POOLS) {
     EvictPools pp{};
     const int n = std::min(PG_POOLS, n_pools - i0);
-    bool vec = true;
     for (int i = 0; i < n; ++i) {
       pp.src[i] = static_cast<const char*>(pools[i0 + i]);
       pp.dst[i] = static_cast<char*>(pools_out[i0 + i]);
       pp.row_bytes[i] = row_bytes[i0 + i];
-      vec = vec && aligned(pp.src[i], 16) && aligned(pp.dst[i], 16) && pp.row_bytes[i] % 16 == 0;
     }
-    const int64_t unit = vec ? 16 : 2;
+    const int64_t unit = launch_unit(i0);
+    const bool vec = unit == 16;
     int64_t slices = 0;
     for (int i = 0; i < n; ++i) {
       pp.first[i] = (int)slices;
       const int64_t row = pp.row_bytes[i] / unit;
-      if (row * page_rows > INT32_MAX) return fail(XENCB_ENOTSUP, "pages_evict: the pools' pages are too large");
       slices += inplace ? (row + EV_THREADS - 1) / EV_THREADS
                         : (row * new_rows + EV_THREADS * EV_UNROLL - 1) / (EV_THREADS * EV_UNROLL);
-      if (slices > INT32_MAX) return fail(XENCB_ENOTSUP, "pages_evict: the pools' pages are too large");
     }
     for (int i = n; i <= PG_POOLS; ++i) pp.first[i] = (int)slices;
     pp.slices = (int)slices;

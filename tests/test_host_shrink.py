@@ -101,3 +101,20 @@ def test_mass_and_8_bit_calls_refuse_bad_arguments():
     for bad in ((None, 0, 4, 64, p, p), (p, 0, 0, 64, p, p), (p, 0, 4, 0, p, p), (p, 9, 4, 64, p, p), (p, 0, 4, 64, None, p),
                 (p, 0, 4, 64, p, None), (p, 0, 4, 64, ctypes.c_void_p(264), p)):
         assert call("xencb_quant8", *bad, None) == N.EINVAL, bad
+
+
+def test_evict_refuses_pages_that_are_too_large_before_anything_moves():
+    """The last of 33 pools, which the second launch would move: refused with the arguments (no device is needed to say so)."""
+    p, big = ctypes.c_void_p(256), 1 << 40
+    at = (ctypes.c_void_p * 33)(*[4096 * (i + 1) for i in range(33)])
+
+    def evict(row, odd=0):
+        rows = (ctypes.c_int64 * 33)(*[16] * 32, row)
+        pools = (ctypes.c_void_p * 33)(*[at[i] for i in range(32)], big + odd)
+        return call("xencb_pages_evict", pools, pools, rows, 33, 4, 8, 8, p, p, 2, None, 1, ctypes.c_void_p(1 << 20), None, 3, 0,
+                    1, p, p, p, p, 8, None)
+
+    for row, odd in ((1 << 33, 0), (1 << 45, 0), (1 << 30, 2), ((1 << 29) + 2, 0)):  # (in 16-byte units, or in 2-byte ones)
+        assert evict(row, odd) == N.ENOTSUP and b"pool 32" in N.lib().xencb_last_error(), (row, odd)
+    for row, odd in ((16, 0), (1 << 30, 0), ((1 << 28) - 2, 2)):  # a workspace of 8 bytes ends the calls that get past it
+        assert evict(row, odd) == N.EINVAL and b"workspace" in N.lib().xencb_last_error(), (row, odd)
