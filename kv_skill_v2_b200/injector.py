@@ -456,8 +456,8 @@ class LibraryInjector(XEncInjector):
         self.last_attn: dict = {}
         # record_mass: every softmax read adds the attention that its rows give to the Library's slots to slot_mass[layer]
         # [pages, page_rows] (ops.read_mass), after mass_decay times what is there; PagedLibrary.evict goes by it. Rows
-        # whose position mask is 0 do not count, nor do rows whose query or routing is not finite: what they leave would stay,
-        # for every later reader of their pages
+        # whose position mask or LayerSelector weight is 0 do not count (others count in full), nor do rows whose query or
+        # routing is not finite: what they leave would stay, for every later reader of their pages
         self.record_mass = False
         self.mass_decay = 1.0
         self.slot_mass: dict = {}

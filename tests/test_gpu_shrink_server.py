@@ -3,12 +3,14 @@ spoil the attention that others recorded, recorded attention goes with the pages
 
 from __future__ import annotations
 
+from types import SimpleNamespace
+
 import pytest
 import torch
 
-from kv_skill_v2_b200 import LibraryInjector, ops
+from kv_skill_v2_b200 import LayerSelector, Library, LibraryInjector, ops
 from tests._fixtures import TinyReader
-from tests.test_gpu_shrink import D_M, D_S, DEV, LAYERS, chunks, interface, library, step
+from tests.test_gpu_shrink import D_M, D_S, DEV, LAYERS, chunks, close, interface, library, step
 
 pytestmark = pytest.mark.gpu
 
@@ -248,3 +250,51 @@ def test_masses_that_do_not_fit_are_refused():
         lib.evict(torch.zeros(P, N, device="cuda"), 4, per_layer=True)
     assert torch.equal(lib.pages(1).page_of, table) and torch.equal(lib.pages(1).slots, slots)
     inj.detach()
+
+
+@pytest.mark.parametrize("k", [1, 2])
+@pytest.mark.parametrize("T", [1, 40])
+@pytest.mark.parametrize("share", [False, True])
+def test_rows_that_a_selector_drops_give_no_attention(k, T, share):
+    """A LayerSelector's rows count in full at the layers that have a weight for them, not at the others."""
+    g = torch.Generator(device="cuda").manual_seed(80)
+    lib, itf = library(81), interface(82)
+    sel = LayerSelector(D_M, LAYERS, k=k, alpha_init=0.05).cuda().requires_grad_(False)
+    sel.u.weight.copy_(torch.randn(sel.u.weight.shape, generator=g, device="cuda"))
+    inj = LibraryInjector(TinyReader(D_M, 5).cuda(), itf, top_k=2, selector=sel, share_pages=share)
+    inj.load_library(lib)
+    inj.record_mass = True
+    h = torch.randn(3, T, D_M, generator=g, device="cuda")
+    with torch.no_grad():
+        for i, li in enumerate(LAYERS):
+            inj._inject(h, li)
+            w = sel.weights()[..., i]
+            assert bool(((w > 0) & (w < 1)).any()) == (k == 2)
+            close(inj.slot_mass[li], step(h, itf, lib, li, 2, live=w != 0)[1], 1e-4)
+    assert abs(float(sum(m.sum() for m in inj.slot_mass.values())) - 3 * T * k) < 1e-3 * T
+    inj.detach()
+
+
+def test_a_library_of_its_own_and_the_last_tokens_attention():
+    """record_mass on a Library that is not paged, alone and beside record_attn."""
+    g = torch.Generator(device="cuda").manual_seed(83)
+    unit = lambda n: torch.nn.functional.normalize(torch.randn(n, D_S, generator=g, device="cuda"), dim=-1).half().float()  # noqa: E731
+    lib = Library([{"K": {0.25: unit(n), 0.75: unit(n)}} for n in (17, 30, 5, 24)], LAYERS, [0.25, 0.75])
+    itf = interface(84)
+    h = torch.randn(2, 5, D_M, generator=g, device="cuda")
+    got, attn = [], []
+    for mass, last in ((True, False), (True, True), (False, True)):
+        inj = LibraryInjector(TinyReader(D_M, 5).cuda(), itf, top_k=2)
+        inj.load_library(lib)
+        inj.record_mass, inj.record_attn = mass, last
+        with torch.no_grad():
+            for li in LAYERS:
+                inj._inject(h, li)
+        got.append(inj.slot_mass)
+        attn.append(inj.last_attn)
+        inj.detach()
+    paged = SimpleNamespace(pages=lambda li: lib.pages(li, DEV), n_chunks=lib.n_chunks)
+    for li in LAYERS:
+        close(got[0][li], step(h.view(1, 10, D_M), itf, paged, li, 2)[1], 1e-4)
+        assert torch.equal(got[1][li], got[0][li]) and torch.equal(attn[1][li], attn[2][li])
+    assert got[2] == {}
