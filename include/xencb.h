@@ -294,7 +294,8 @@ XENCB_API int xencb_read_shared(const void* q, int q_dtype, int64_t n_rows, int 
  * Arguments as xencb_read_shared's; prior [n_pages, page_rows] or NULL (0; decay is then not used); mass [n_pages,
  * page_rows] float32, may be prior itself. Every page is written. Float32 q takes part with 22 bits (16 with bf16 slots), a
  * 16-bit q exactly. The sums are added in the order of the rows: the same call gives the same bits. Slots at or past
- * n_valid may hold anything. f16 / bf16 slots, d_s a multiple of 8, page_rows at most 2048. */
+ * n_valid may hold anything. Pairs with wk 0 or NaN (what the routing gives a query that is not finite) read nothing, so that
+ * such a row leaves nothing in a mass that is added to. f16 / bf16 slots, d_s a multiple of 8, page_rows at most 2048. */
 XENCB_API size_t xencb_read_mass_workspace(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows,
                                            int slots_dtype, int q_dtype);
 XENCB_API int xencb_read_mass(const void* q, int q_dtype, int64_t n_rows, int d_s, const void* slots, int slots_dtype,

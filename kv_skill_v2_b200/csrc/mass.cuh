@@ -102,10 +102,11 @@ struct MassArgs {
   float* mass;
 };
 
-// The page that pair i reads and its valid slots; -1: none. Bad tables are flagged where `flag` is set.
+// The page that pair i reads and its valid slots; -1: none. Bad tables are flagged where `flag` is set. A weight of NaN, the
+// routing of a query that is not finite, reads nothing, as 0 does: the sums are added to call after call.
 __device__ __forceinline__ int ms_page(const MassArgs& a, int i, bool flag, int* nv) {
   const int c = a.idx[i];
-  if (c < 0 || a.wk[i] == 0.f) return -1;
+  if (c < 0 || !(fabsf(a.wk[i]) > 0.f)) return -1;
   const int64_t at = (int64_t)((unsigned)i / (unsigned)a.k / (unsigned)a.rows_per_lib) * a.C + c;
   const int page = c < a.C ? a.page_of[at] : -1;
   if (page < 0 || page >= a.n_pages) {

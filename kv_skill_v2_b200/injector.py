@@ -457,7 +457,7 @@ class LibraryInjector(XEncInjector):
         # record_mass: every softmax read adds the attention that its rows give to the Library's slots to slot_mass[layer]
         # [pages, page_rows] (ops.read_mass), after mass_decay times what is there; PagedLibrary.evict goes by it. Rows
         # whose position mask or LayerSelector weight is 0 do not count (others count in full), nor do rows whose query or
-        # routing is not finite: what they leave would stay, for every later reader of their pages
+        # summary keys are not finite (their routing weights are NaN): what they left would stay, for every later reader
         self.record_mass = False
         self.mass_decay = 1.0
         self.slot_mass: dict = {}
@@ -629,12 +629,9 @@ class LibraryInjector(XEncInjector):
             raise ValueError("record_mass: the linear read has no attention weights")
         if self.force_attn is not None:
             raise ValueError("record_mass: force_attn replaces the read's attention")
-        size = torch.linalg.vector_norm(q, float("inf"), dim=-1, keepdim=True) * wk
-        counts = size - size == 0  # (neither infinite nor NaN)
         pm = self._pos_mask(h)
         if pm is not None:
-            counts = counts & (pm != 0).view(-1, 1)
-        wk = torch.where(counts, wk, 0.0)
+            wk = torch.where((pm != 0).view(-1, 1), wk, 0.0)
         mass = self.slot_mass.get(li)
         if mass is None and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("record_mass: run the step once before it is captured (slot_mass is what replays add to)")

@@ -137,6 +137,18 @@ def test_a_row_that_is_not_finite_reaches_only_what_it_reads():
     assert torch.equal(got[others], want[others])
 
 
+@pytest.mark.parametrize("T", [40, 300])
+def test_pairs_whose_weight_is_nan_read_nothing(T):
+    q, pages, idx, wk, T = case(12, 1, T, 6, 0, 64, 64, 3)  # (with and without a plan)
+    wk[5], wk[7, 1], q[5] = float("nan"), -float("nan"), float("nan")
+    mass = torch.rand(6, 64, device="cuda")
+    got = ops.read_mass(q, pages, idx, wk, rows_per_lib=T, mass=mass, decay=0.5)
+    assert bool(got.isfinite().all())
+    clean = torch.nan_to_num(wk, nan=0.0)
+    assert torch.equal(got, ops.read_mass(q, pages, idx, clean, rows_per_lib=T, mass=mass, decay=0.5))
+    close(got, reference(q, pages, idx, clean, T, prior=mass, decay=0.5), 2e-5)
+
+
 def test_rows_of_any_size():
     # a power of two of q is taken out row by row. Scores of up to 2^6 are off by 2^-22 of that, 12 times that is 2e-4 of a
     # weight on either side of the softmax; scores of next to nothing by nothing
