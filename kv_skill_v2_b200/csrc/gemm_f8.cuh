@@ -5,7 +5,7 @@
 //   part[z][m][n] = sum_{blocks b of split z} 2^(ex[m, b] + ew[n, b]) sum_{k in b} X8[m, k] W8[n, k]
 //
 // A power of two costs a floating-point format nothing but range, and the tensor core applies it itself (ue8m0 scale
-// factors), so the accumulator runs over the whole split in float32. The instruction takes a scale per row and 32 columns:
+// factors), so the accumulator runs over a split's blocks in float32. The instruction takes a scale per row and 32 columns:
 // the four products of a block use the same one. The factors of a CTA's rows lie in tensor memory for all of its blocks,
 // four blocks to a 32-bit word; the instruction descriptor names the byte.
 //
@@ -28,6 +28,10 @@ namespace xencb {
 constexpr int F8_BM = 128;   // output features per CTA
 constexpr int F8_BK = 128;   // columns of a block: one scale factor a row, one 128-byte swizzle row
 constexpr int F8_THREADS = 32 * 6;
+// Blocks that one accumulator runs over. The tensor core's drops bits below its running value at every product, towards zero:
+// 3.5e-8 to 4.4e-8 of the result for each block (32, 40, 64 and 94 blocks: 1.1e-6, 1.6e-6, 2.8e-6 and 4.1e-6 off in norm;
+// float32 sums are 2e-7 to 4e-7 off). Longer splits are cut; the rows kernel, below, takes its accumulator out more often.
+constexpr int F8_RUN = 20;
 __host__ __device__ constexpr int f8_stage(int bn) { return (F8_BM + bn) * F8_BK; }
 __host__ __device__ constexpr int f8_stages(int bn) { return bn == 64 ? 8 : bn == 128 ? 6 : 4; }
 __host__ __device__ constexpr size_t f8_smem(int bn) { return 1024 + (size_t)f8_stages(bn) * f8_stage(bn) + 1024; }
@@ -113,7 +117,8 @@ struct F8RowStats {
   float* gate;          // [M] or null
 };
 
-// HBM bounds it: 16384 float32 rows of 2048 (168 MB with their 8-bit form) take 28 us, 6.0 TB/s.
+// HBM bounds it: 16384 float32 rows of 2048 (168 MB with their 8-bit form) take 28 us, 6.0 TB/s. 128 threads a row of float32
+// (256: 38 us), 256 of 16 bits (2048 rows of 5120 7.6 us, with 128 7.9; 16384 rows of 4096 43, with 128 37).
 // One CTA per row, 16 threads a block of 128 columns (8 values each, four times as many of a thread on their way, held as
 // they came). x8 rows are kp = 128 ceil(K / 128) bytes, zeros behind column K; scale[row * stride + b] = e + 127.
 template <typename T> __host__ __device__ constexpr int f8q_threads() { return sizeof(T) == 4 ? 128 : 256; }
@@ -244,7 +249,6 @@ struct F8Args {
 
 // X's factors lie behind W's: a word of four blocks like W's, or (TX) a word of one block, in BN / 32 columns.
 constexpr int F8_FUSED_ROWS = 8;
-constexpr int F8_MAX_FUSED = 120;  // blocks of a split then
 
 template <int BN, typename TX>
 __global__ void __launch_bounds__(F8_THREADS, 1) gemm_f8_kernel(const __grid_constant__ CUtensorMap map_w,
@@ -467,16 +471,19 @@ __global__ void __launch_bounds__(F8_THREADS, 1) gemm_f8_kernel(const __grid_con
 // where the product is and no partials are written. Persistent: 8 epilogue warps take the accumulator into registers and
 // give it back before they store, so that the next tile's products run meanwhile; they also bring the next tile's scale
 // factors (two sets of them in tensor memory).
-// 16384 rows 2048 -> 4096 take 116 us, 2.4 PFLOP/s, with h + delta in place of delta 149; 103 without the stores, 94 without
+// 16384 rows 2048 -> 4096 take 116 to 122 us, 2.3 PFLOP/s, with h + delta in place of delta 149, with the sums of the mag term
+// too, as the hook calls it, 190 (h is loaded where it is used, beside v's 128 registers); 103 without the stores, 94 without
 // the epilogue, 83 as the products alone: the operands (1.6 GB from L2), what the epilogue writes and its arithmetic each add
 // about 11 to the products, which run at 3.3 PFLOP/s. (h on its way four groups before its use: 158.) 2048 rows 5120 -> 2048
-// are one tile a CTA: 25 us, 15 of it products.
+// are one tile a CTA: 28 to 30 us, 15 of it products. The accumulator is taken out every FR_RUN blocks: 40 blocks at once were
+// 1.6e-6 of the result off, in three runs 5e-7, for 1.3 us.
 //   project_in   q = y * rstd + b; the row's sum of squares by pieces of 128 columns, for f8_norm_kernel
 //   project_out  delta = scale * gate * (y + b) * mask in h's type, h + delta; sums of squares of delta and h for the mag term
 constexpr int FR_BM = 128, FR_BN = 256, FR_STAGES = 4;
 constexpr int FR_STAGE = (FR_BM + FR_BN) * F8_BK;
 constexpr int FR_WORD_COLS = FR_BM / 32 + FR_BN / 32;
 constexpr int FR_MAX_WORDS = (512 - FR_BN) / 2 / FR_WORD_COLS;  // two sets
+constexpr int FR_RUN = 16;  // blocks that the accumulator runs over before it is added up in registers
 constexpr int FR_EPI = 8;
 constexpr int FR_THREADS = 32 * (4 + FR_EPI);
 constexpr size_t FR_SMEM = 1024 + (size_t)FR_STAGES * FR_STAGE + 256;
@@ -530,6 +537,8 @@ __global__ void __launch_bounds__(FR_THREADS, 1) gemm_f8_rows_kernel(const __gri
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int words = (a.nb + 3) / 4;
+  // the accumulator's runs, of nearly one length
+  const int runs = (a.nb + FR_RUN - 1) / FR_RUN, run = (a.nb + runs - 1) / runs;
 
   if (threadIdx.x == 0) {
     prefetch_tensormap(&map_x);
@@ -589,26 +598,29 @@ __global__ void __launch_bounds__(FR_THREADS, 1) gemm_f8_rows_kernel(const __gri
       if (elect_one()) {
         RsRing ring{0, 0};
         bool ok = true;
-        uint32_t i = 0;
+        uint32_t i = 0, acc = 0;
         for (int64_t t = blockIdx.x; t < a.tiles && ok; t += gridDim.x, ++i) {
           if (!(ok = mbar_wait_spin(&sf_full[i & 1], (i >> 1) & 1))) break;
-          if (i > 0 && !(ok = mbar_wait_spin(acc_empty, (i - 1) & 1))) break;
-          tc_fence_after();
           const uint32_t sf = taddr + FR_BN + (i & 1) * (FR_MAX_WORDS * FR_WORD_COLS);
-          for (int kb = 0; kb < a.nb; ++kb) {
-            if (!(ok = mbar_wait_spin(&full[ring.st], ring.phase))) break;
+          for (int k0 = 0; k0 < a.nb && ok; k0 += run, ++acc) {
+            if (acc > 0 && !(ok = mbar_wait_spin(acc_empty, (acc - 1) & 1))) break;
             tc_fence_after();
-            const uint32_t sb = smem_u32(smem + ring.st * FR_STAGE);
-            const uint32_t sa = sf + (kb >> 2) * FR_WORD_COLS;
-            const uint32_t idesc = f8_idesc(FR_BN, 0) | ((uint32_t)(kb & 3) << 4) | ((uint32_t)(kb & 3) << 29);
+            const int k1 = min(a.nb, k0 + run);
+            for (int kb = k0; kb < k1; ++kb) {
+              if (!(ok = mbar_wait_spin(&full[ring.st], ring.phase))) break;
+              tc_fence_after();
+              const uint32_t sb = smem_u32(smem + ring.st * FR_STAGE);
+              const uint32_t sa = sf + (kb >> 2) * FR_WORD_COLS;
+              const uint32_t idesc = f8_idesc(FR_BN, 0) | ((uint32_t)(kb & 3) << 4) | ((uint32_t)(kb & 3) << 29);
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-              tc_mma_mx8(taddr, umma_desc_k_sw128(sb + ks * 32), umma_desc_k_sw128(sb + FR_BM * F8_BK + ks * 32), idesc,
-                         sa, sa + FR_BM / 32, kb > 0 || ks > 0);
-            tc_commit(&empty[ring.st]);
-            ring.next(FR_STAGES);
+              for (int ks = 0; ks < 4; ++ks)
+                tc_mma_mx8(taddr, umma_desc_k_sw128(sb + ks * 32), umma_desc_k_sw128(sb + FR_BM * F8_BK + ks * 32), idesc,
+                           sa, sa + FR_BM / 32, kb > k0 || ks > 0);
+              tc_commit(&empty[ring.st]);
+              ring.next(FR_STAGES);
+            }
+            if (ok) tc_commit(acc_full);
           }
-          if (ok) tc_commit(acc_full);
         }
         if (!ok) *abort_flag = 1;
       }
@@ -650,7 +662,7 @@ __global__ void __launch_bounds__(FR_THREADS, 1) gemm_f8_rows_kernel(const __gri
     };
     if (blockIdx.x < a.tiles) scales(blockIdx.x, 0);
     const float ls = a.log_scale_dev ? expf(__ldg(a.log_scale_dev)) : 1.f;
-    uint32_t i = 0;
+    uint32_t i = 0, acc = 0;
     for (int64_t t = blockIdx.x; t < a.tiles; t += gridDim.x, ++i) {
       // (the products of the tile before, which used this set, are done: its accumulator was waited for)
       if (t + gridDim.x < a.tiles) scales(t + gridDim.x, i + 1);
@@ -659,15 +671,33 @@ __global__ void __launch_bounds__(FR_THREADS, 1) gemm_f8_rows_kernel(const __gri
       const bool in = m < a.M;
       float mul = in && a.mul ? a.mul[m] : 1.f;
       if (OUT) mul *= a.scale * ls * (a.pos_mask && in ? a.pos_mask[m] : 1.f);
-      done(*abort_flag || mbar_wait_spin(acc_full, i & 1));
-      tc_fence_after();
+      auto arrived = [&] {
+        done(*abort_flag || mbar_wait_spin(acc_full, acc & 1));
+        tc_fence_after();
+      };
+      auto taken = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty);
+        __syncwarp();
+        ++acc;
+      };
       float v[128];
+      arrived();
 #pragma unroll
       for (int g = 0; g < 128; g += 32) tc_ld32(tl + half * 128 + g, v + g);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty);
-      __syncwarp();
+      taken();
+      for (int k0 = run; k0 < a.nb; k0 += run) {
+        arrived();
+#pragma unroll
+        for (int g = 0; g < 128; g += 16) {  // (there are no registers for more beside v)
+          float x[16];
+          tc_ld16(tl + half * 128 + g, x);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[g + e] += x[e];
+        }
+        taken();
+      }
       if (*abort_flag) {
 #pragma unroll
         for (int g = 0; g < 128; ++g) v[g] = 0.f;

@@ -367,7 +367,9 @@ F8Plan plan_f8(int64_t M, int N, int K, int sms, bool selector) {
   const int64_t tiles = ((int64_t)(N + F8_BM - 1) / F8_BM) * ((M + p.bn - 1) / p.bn);
   const int64_t s = std::min<int64_t>(std::max<int64_t>(1, sms / tiles), p.nb);
   // (blocks b0 .. b0 + bps - 1 lie in at most (bps + 6) / 4 words of scale factors)
-  p.bps = std::min((int)((p.nb + s - 1) / s), M <= F8_FUSED_ROWS ? F8_MAX_FUSED : 4 * f8_max_words(p.bn) - 6);
+  static_assert(F8_RUN + 6 <= 4 * f8_max_words(256), "a run's scale factors fit tensor memory");
+  const int64_t n_splits = std::max<int64_t>(s, (p.nb + F8_RUN - 1) / F8_RUN);
+  p.bps = (int)((p.nb + n_splits - 1) / n_splits);
   p.gp.tc = true;
   p.gp.kps = p.bps * F8_BK;
   p.gp.splits = (p.nb + p.bps - 1) / p.bps;
