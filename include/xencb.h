@@ -292,8 +292,8 @@ XENCB_API int xencb_read_shared(const void* q, int q_dtype, int64_t n_rows, int 
  *   mass[p, n] = decay * prior[p, n] + sum over rows t and routed chunks j with page_of[lib(t), idx[t, j]] = p and
  *                n < n_valid[lib(t), idx[t, j]] of wk[t, j] * softmax over n of (read_temp * q[t] . slots[p, n])
  * Arguments as xencb_read_shared's; prior [n_pages, page_rows] or NULL (0; decay is then not used); mass [n_pages,
- * page_rows] float32, may be prior itself. Every page is written. Float32 q takes part with 22 bits (16 with bf16 slots), a
- * 16-bit q exactly. The sums are added in the order of the rows: the same call gives the same bits. Slots at or past
+ * page_rows] float32, may be prior itself. Every page is written. Float32 q takes part with 22 bits (with bf16 slots 24,
+ * or 16 in calls of n_rows * k * d_s >= 4096 * n_pages, whose many pairs average it out), a 16-bit q exactly. The sums are added in the order of the rows: the same call gives the same bits. Slots at or past
  * n_valid may hold anything. Pairs with wk 0 or NaN (what the routing gives a query that is not finite) read nothing, so that
  * such a row leaves nothing in a mass that is added to. f16 / bf16 slots, d_s a multiple of 8, page_rows at most 2048. */
 XENCB_API size_t xencb_read_mass_workspace(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows,

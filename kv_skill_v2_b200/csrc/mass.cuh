@@ -21,7 +21,10 @@
 // 32 pairs is a butterfly over the warp's lanes (31 shuffles for 32 slots).
 //
 // Precision. Float32 q enters as hi + lo in 16 bits, two products into one accumulator: 22 bits with f16 slots, 16 with
-// bf16. A 16-bit q is one product, exact (bf16 q fits f16's 11 bits, but for values 2^-28 below the row's largest). The
+// bf16. There a pair's weights come out 12 * 2^-17 / sqrt(d_s) and so off, which a sum over many pairs averages out (measured,
+// in norm: 3.5e-6 sqrt(64 / d_s) / sqrt(pairs a page)) and few do not: calls with pairs * d_s < MS_THREE * pages, which wait
+// for latency anyway, take hi + mid + lo, 24 bits (64 columns, 6 pairs a page: 1.4e-6 -> 1.1e-7). A 16-bit q is exact: one
+// product, two for an f16 q with bf16 slots (bf16 q fits f16's 11 bits, but for values 2^-28 below the row's largest). The
 // tensor core's accumulator drops bits below its running value, so it runs over MS_CHUNK or MS_CHUNK_FEW blocks of 64 columns
 // and is added up in float32 registers.
 //
@@ -29,7 +32,9 @@
 // TB/s; 1024 pages with few pairs each run at 5.6 TB/s). Full tiles: 128 pairs x 512 slots x 2048 columns take 22.9 us of
 // products (165 cycles per M 128, N 256, K 16) on a cluster of two, hi and lo; the softmax adds 5 us a tile (softmax 3.2k
 // cycles, exchange 1.9k, column sums 3.9k), which the next tile's products do not cover: 4096 float32 rows with 4 of 64
-// pages each take 95 us, 0.44 of the rate of the products alone.
+// pages each take 97 us, 0.43 of the rate of the products alone (a 16-bit q 70). Listing the pairs is pages x pairs, as every
+// page's CTA reads every pair's page: 15 us of the rows' launch there, 136 with all 64 pages a row (scores 903), 957 with
+// 16384 rows, 128 of 1024 pages each (scores 7468).
 #pragma once
 
 #include <math_constants.h>
@@ -45,6 +50,7 @@ constexpr int MS_MAX_CS = 8;      // CTAs per cluster: pages of up to 2048 slots
 constexpr int MS_CHUNK = 4;       // blocks of 64 columns per accumulator
 constexpr int MS_CHUNK_FEW = 2;   // of calls of few pairs, whose errors no sum averages out (64 rows, top-4: 5.6e-7 -> 3.3e-7);
                                   // it costs them nothing, prompts 3 % for the same error
+constexpr int MS_THREE = 4096;    // (3.5e-6 / 8 = 4.4e-7 off from there on)
 constexpr int MS_ATILE = MS_M * 128;
 constexpr int MS_BTILE = MS_N * 128;
 constexpr int MS_PRODUCERS = 4;   // warps that bring Q
@@ -54,15 +60,18 @@ constexpr int MS_THREADS = 32 * (MS_LOW + MS_EPI);
 constexpr int MS_REGS_LOW = 56, MS_REGS_HIGH = 200;  // registers of a thread of these warps, and of the others
 constexpr int MS_REGS = 32 * (MS_LOW * MS_REGS_LOW + MS_EPI * MS_REGS_HIGH);
 constexpr int MS_FEW = 64;        // pairs of a tile whose hi and lo rows fit one 128-row operand
+__host__ __device__ constexpr int ms_few(int terms) { return terms == 3 ? 32 : MS_FEW; }  // (or hi, mid and lo rows)
 constexpr int MS_ONE_CTA = 2048;  // pairs that one CTA counts
 constexpr int MS_DIRECT = 512;    // pairs of a call without a plan
 constexpr int MS_XPITCH = 17;     // 16 columns of the lo rows' sums on their way to the hi rows' lanes
 __host__ __device__ constexpr int ms_stage(int terms) { return terms * MS_ATILE + MS_BTILE; }
 // stages of the ring: what the maxima and sums of cs CTAs (two generations, two halves of the slots each) leave
-__host__ __device__ constexpr int ms_stages(int terms, int cs) { return (cs <= 4 ? 1 : 0) + (terms == 2 ? 2 : 3); }
+__host__ __device__ constexpr int ms_stages(int terms, int cs) {
+  return terms == 3 ? 2 : (cs <= 4 ? 1 : 0) + (terms == 2 ? 2 : 3);
+}
 __host__ __device__ constexpr size_t ms_smem(int terms, int cs) {
   return 1024 + (size_t)ms_stages(terms, cs) * ms_stage(terms) + (size_t)cs * 4 * MS_M * 8 + 4 * MS_N * 4 +
-         (terms == 2 ? 2 * MS_FEW * MS_XPITCH * 4 : 0) + 256;
+         (terms >= 2 ? 2 * MS_FEW * MS_XPITCH * 4 : 0) + 256;
 }
 
 struct __align__(16) MassTile {
@@ -92,7 +101,7 @@ struct MassArgs {
   int slots;      // of the list of tiles (those without pairs are skipped)
   // rows
   float* rinv;    // [R]: 1 / (the row's power of two)
-  const void* q16;  // [terms, R, d_s]
+  const void* q16;  // [terms, R, d_s]: hi, (mid,) lo
   // scores
   int cs, per;    // CTAs per cluster, slots per CTA
   float qscale;   // read_temp * log2(e)
@@ -325,15 +334,19 @@ __global__ void __launch_bounds__(MS_ROWS_THREADS) mass_rows_kernel(const MassAr
   }
   if (threadIdx.x == 0) a.rinv[row] = 1.f / s;
   auto emit = [&](int i, const float* w) {
-    alignas(16) T hi[8], lo[8];
+    float left[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      hi[e] = from_f32<T>(w[e] * s);
-      if (TERMS == 2) lo[e] = from_f32<T>(w[e] * s - to_f32(hi[e]));
+    for (int e = 0; e < 8; ++e) left[e] = w[e] * s;
+#pragma unroll
+    for (int t = 0; t < TERMS; ++t) {
+      alignas(16) T x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = from_f32<T>(left[e]);
+        left[e] -= to_f32(x[e]);
+      }
+      *reinterpret_cast<uint4*>(out + (t * a.n_rows + row) * a.d_s + i) = *reinterpret_cast<const uint4*>(x);
     }
-    *reinterpret_cast<uint4*>(out + row * a.d_s + i) = *reinterpret_cast<const uint4*>(hi);
-    if (TERMS == 2)
-      *reinterpret_cast<uint4*>(out + (a.n_rows + row) * a.d_s + i) = *reinterpret_cast<const uint4*>(lo);
   };
 #pragma unroll
   for (int h = 0; h < HELD; ++h) {
@@ -360,7 +373,7 @@ struct MsSmem {
   unsigned char* stages;
   float* stat;   // [2][2 cs][128][2]: by the parity of the tile, maximum and sum of each pair's half of a CTA's slots
   float* cols;   // [4][256]: column sums of the lane quarters
-  float* xch;    // [2][64][MS_XPITCH]: sums of the lo rows of few pairs
+  float* xch;    // [2][64][MS_XPITCH]: sums of the lo rows of few pairs, or of the mid and the lo rows
   uint64_t *full, *empty, *s_full, *s_empty, *st;
   uint32_t* tmem;
   volatile int *abort_flag, *last;
@@ -378,7 +391,7 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
   s.stat = reinterpret_cast<float*>(s.stages + n_st * STAGE);
   s.cols = s.stat + cs * 4 * MS_M * 2;
   s.xch = s.cols + 4 * MS_N;
-  s.full = reinterpret_cast<uint64_t*>(s.xch + (TERMS == 2 ? 2 * MS_FEW * MS_XPITCH : 0));
+  s.full = reinterpret_cast<uint64_t*>(s.xch + (TERMS >= 2 ? 2 * MS_FEW * MS_XPITCH : 0));
   s.empty = s.full + 4;
   s.s_full = s.empty + 4;
   s.s_empty = s.s_full + 2;
@@ -420,7 +433,7 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
   const uint32_t taddr = *s.tmem;
   pdl_wait();
   const int n_tiles = a.direct ? a.slots : *a.n_tiles;
-  auto stacked = [](const MassTile& t) { return TERMS == 2 && t.count <= MS_FEW; };
+  auto stacked = [](const MassTile& t) { return TERMS >= 2 && t.count <= ms_few(TERMS); };
   auto done = [&](bool arrived) {
     if (!arrived) *s.abort_flag = 1;
     __syncwarp();
@@ -499,14 +512,14 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
       const int t0 = threadIdx.x - 128;
       const int sub = t0 >> 3, ch = t0 & 7;
       const char* q = static_cast<const char*>(a.q16);
-      const int64_t row_bytes = (int64_t)a.d_s * 2, lo = a.n_rows * row_bytes;
+      const int64_t row_bytes = (int64_t)a.d_s * 2, term_bytes = a.n_rows * row_bytes;
       RsRing ring{0, 0};
       uint32_t used = 0;
       bool ok = true;
       for (int t = cluster; t < n_tiles && ok; t += n_clusters) {
         const MassTile tile = a.tiles[t];
         if (tile.count == 0 || seg0 >= tile.nv) continue;
-        const uint32_t lo_at = stacked(tile) ? MS_FEW * 128 : MS_ATILE;
+        const uint32_t term_at = stacked(tile) ? ms_few(TERMS) * 128 : MS_ATILE;
         int rows[PASSES];
   #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
@@ -529,7 +542,8 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
               const char* src = q + rows[i] * row_bytes + (in ? col * 2 : 0);
               const uint32_t dst = st + r * 128 + ((ch ^ (r & 7)) << 4);
               ms_copy16(dst, src, in ? 16 : 0);
-              if (TERMS == 2) ms_copy16(dst + lo_at, src + lo, in ? 16 : 0);
+              if (TERMS >= 2) ms_copy16(dst + term_at, src + term_bytes, in ? 16 : 0);
+              if (TERMS == 3) ms_copy16(dst + 2 * term_at, src + 2 * term_bytes, in ? 16 : 0);
             }
           }
           ms_copies_arrive(&s.full[ring.st]);
@@ -554,7 +568,8 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
       const MassTile tile = a.tiles[t];
       if (tile.count == 0) continue;
       const bool few = stacked(tile), here = r < tile.count, any = quarter * 32 < tile.count;
-      const bool drain = (few ? quarter & 1 : quarter) * 32 < tile.count && width > 0;  // this warp's lanes hold sums
+      const bool drain = (few ? (TERMS == 3 ? 0 : quarter & 1) : quarter) * 32 < tile.count && width > 0 &&
+                         (TERMS < 3 || !few || quarter < 3);  // this warp's lanes hold sums
       int nv = 0;
       float w = 0.f, c = 0.f;
       if (here) {
@@ -600,6 +615,22 @@ __global__ void __launch_bounds__(MS_THREADS, 1)
             for (int i = 0; i < 16; ++i) v[g + i] += x[i];
           }
           named_bar_sync(2 + half * 2 + (quarter & 1), 64);
+        }
+      }
+      if (TERMS == 3 && few && drain) {  // the mid and lo rows' sums, 32 and 64 lanes further
+        float* x = s.xch + (half * MS_FEW + lane) * MS_XPITCH;
+#pragma unroll
+        for (int g = 0; g < 128; g += 16) {
+          if (quarter > 0) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[(quarter - 1) * 32 * MS_XPITCH + i] = v[g + i];
+          }
+          named_bar_sync(2 + half, 96);
+          if (quarter == 0) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[g + i] += x[i] + x[32 * MS_XPITCH + i];
+          }
+          named_bar_sync(2 + half, 96);
         }
       }
       // e^(score - max) of this half, its maximum and sum

@@ -1039,6 +1039,7 @@ int plan_mass(int64_t n_rows, int k, int d_s, int64_t n_pages, int page_rows, in
   p->n_pairs = n_rows * k;
   // a 16-bit q is one product where the slots' type holds it (bf16's 8 bits fit f16)
   p->terms = q_dtype == XENCB_F32 || (q_dtype == XENCB_F16 && slots_dtype == XENCB_BF16) ? 2 : 1;
+  if (q_dtype == XENCB_F32 && slots_dtype == XENCB_BF16 && p->n_pairs * d_s < MS_THREE * n_pages) p->terms = 3;
   p->cs = (page_rows + MS_N - 1) / MS_N;
   p->per = (int)align_up((size_t)(page_rows + p->cs - 1) / p->cs, 16);
   // few pairs over few pages: no plan, but room in every page for all of them
@@ -2009,7 +2010,8 @@ int xencb_read_mass(const void* q, int q_dtype, int64_t n_rows, int d_s, const v
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto go = [&](auto run) { return run(q, q_dtype, p, a, slots, q16, di.sms, st); };
   if (slots_dtype == XENCB_BF16)
-    return p.terms == 2 ? go(run_mass<__nv_bfloat16, 2>) : go(run_mass<__nv_bfloat16, 1>);
+    return p.terms == 3 ? go(run_mass<__nv_bfloat16, 3>)
+                        : p.terms == 2 ? go(run_mass<__nv_bfloat16, 2>) : go(run_mass<__nv_bfloat16, 1>);
   return p.terms == 2 ? go(run_mass<__half, 2>) : go(run_mass<__half, 1>);
 }
 

@@ -88,6 +88,20 @@ def test_mass(shape, slots, q):
     assert not ops.device_status(torch.device("cuda:0"))
 
 
+@pytest.mark.parametrize("shape", [(1, 1, 1, 0, 300, 512, 1), (1, 1, 4, 0, 700, 2560, 1), (1, 4, 20, 0, 96, 256, 2),
+                                   (3, 20, 20, 4, 100, 64, 3), (2, 30, 20, 4, 300, 512, 4), (1, 40, 1, 0, 520, 64, 1),
+                                   (1, 1, 2, 0, 2048, 72, 2), (1, 90, 2, 0, 257, 40, 2), (1, 150, 2, 0, 64, 24, 1),
+                                   (1, 700, 8, 0, 90, 64, 2), (4, 300, 6, 2, 260, 128, 4)])
+@pytest.mark.parametrize("slots", [F16, BF16])
+def test_a_float32_query_keeps_its_precision(shape, slots):
+    """In norm: 22 or 24 bits of q are next to nothing (2e-7 of a weight), 16 are 4.4e-7 where a call has as many pairs a page
+    as it must have for them, float32 scores and sums 2e-7 or so: 1e-6 bounds it, whatever the slots' type."""
+    a = case(13, *shape, slots=slots)
+    want = reference(*a)
+    off = float((ops.read_mass(*a[:4], rows_per_lib=a[4]).double() - want).norm() / want.norm())
+    assert off < 1e-6, off
+
+
 def test_prior_decay_and_in_place():
     a = case(2, 2, 9, 4, 3, 100, 128, 3)
     prior = torch.rand(a[1].slots.shape[:2], device="cuda")
