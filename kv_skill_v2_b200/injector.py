@@ -507,7 +507,8 @@ class LibraryInjector(XEncInjector):
         if slot_mass:
             kept = {}
             for li, m in slot_mass.items():
-                slots = (lib.pages(li, dev, self.slot_dtype) if isinstance(lib, Library) else lib.pages(li)).slots
+                slots = (lib.pages(li, dev, self.slot_dtype, require_nonempty=self.read_softmax) if isinstance(lib, Library)
+                         else lib.pages(li)).slots
                 P, N = slots.shape[:2]
                 if m.dtype != torch.float32 or m.dim() != 2 or m.shape[1] != N or m.shape[0] > P or not m.is_contiguous() \
                         or m.device != slots.device:
