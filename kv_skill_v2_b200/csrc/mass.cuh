@@ -32,9 +32,9 @@
 // TB/s; 1024 pages with few pairs each run at 5.6 TB/s). Full tiles: 128 pairs x 512 slots x 2048 columns take 22.9 us of
 // products (165 cycles per M 128, N 256, K 16) on a cluster of two, hi and lo; the softmax adds 5 us a tile (softmax 3.2k
 // cycles, exchange 1.9k, column sums 3.9k), which the next tile's products do not cover: 4096 float32 rows with 4 of 64
-// pages each take 97 us, 0.43 of the rate of the products alone (a 16-bit q 70). Listing the pairs is pages x pairs, as every
-// page's CTA reads every pair's page: 15 us of the rows' launch there, 136 with all 64 pages a row (scores 903), 957 with
-// 16384 rows, 128 of 1024 pages each (scores 7468).
+// pages each take 95 us, 0.44 of the rate of the products alone (a 16-bit q 70). Listing the pairs is pages x pairs, as every
+// page's CTA reads every pair's page: 15 us of the rows' launch there, 136 with all 64 pages a row (scores 900), 1000 with
+// 16384 rows, 128 of 1024 pages each (scores 7300).
 #pragma once
 
 #include <math_constants.h>
