@@ -325,3 +325,19 @@ def test_long_sums_keep_their_precision(R, k, n, selector, bound):
     want = values(h) @ values(W).t()
     off = float((got - want).norm() / want.norm())
     assert off < bound, off
+
+
+@pytest.mark.parametrize("R,k,n", [(5000, 5000, 1800), (9000, 2176, 1284), (20000, 2304, 516), (2600, 4224, 2052)])
+def test_several_tiles_of_several_runs(R, k, n):
+    """Calls of many rows whose CTAs take several tiles, the accumulator out two or three times in each (odd and even)."""
+    h, W = rows(R, k, 64, dtype=torch.bfloat16), rows(n, k, 65) * k ** -0.5
+    w8 = ops.weights_fp8(W)
+    y = values(h) @ values(W).t()
+    assert rel(ops.project_in(h, w8, rms=False, l2=False)[0], y) < TOL
+    assert rel(ops.project_in(h, w8)[0], y / y.norm(dim=-1, keepdim=True)) < TOL
+    r, x = h.float(), torch.randn(R, n, generator=gen(66), device="cuda").to(torch.bfloat16)
+    _, got, mag = ops.project_out(r, w8, x, scale=0.5, want_delta=False, h_out=torch.empty_like(x), want_rel=True)
+    want, half = x.double() + 0.5 * y, torch.finfo(torch.bfloat16).eps / 2
+    assert float((got.double() - want).abs().max() / want.abs().max()) < TOL + 2 * half
+    want = 0.5 * y.norm(dim=-1) / (x.double().norm(dim=-1) + 1e-6)
+    assert float((mag.double() - want).abs().max() / want.max()) < TOL + half

@@ -102,6 +102,20 @@ def test_a_float32_query_keeps_its_precision(shape, slots):
     assert off < 1e-6, off
 
 
+@pytest.mark.parametrize("shape", [(1, 165, 1, 0, 520, 24, 1), (1, 660, 4, 0, 260, 24, 1), (2, 500, 10, 5, 700, 16, 3),
+                                   (1, 33, 2, 0, 1300, 104, 1), (3, 400, 40, 30, 40, 48, 7)])
+def test_three_terms_over_several_tiles(shape):
+    # bf16 slots and few columns: pages of more pairs than a tile holds, with more and fewer than fit one operand in the last
+    a = case(14, *shape, slots=BF16)
+    prior = torch.rand(a[1].slots.shape[:2], device="cuda")
+    got = ops.read_mass(*a[:4], rows_per_lib=a[4], mass=prior, decay=0.5)
+    want = reference(*a, prior=prior, decay=0.5)
+    close(got, want, 2e-5)
+    assert float((got.double() - want).norm() / want.norm()) < 1e-6
+    assert torch.equal(got, ops.read_mass(*a[:4], rows_per_lib=a[4], mass=prior, decay=0.5))
+    assert not ops.device_status(torch.device("cuda:0"))
+
+
 def test_prior_decay_and_in_place():
     a = case(2, 2, 9, 4, 3, 100, 128, 3)
     prior = torch.rand(a[1].slots.shape[:2], device="cuda")
