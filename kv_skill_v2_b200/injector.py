@@ -108,8 +108,8 @@ class ExternalSkillInjector:
         # projection weights in the 3xF16 form (ops.weights_prep)
         self.gemm_f16x3 = True
         # the projections in 8-bit floating point (ops.weights_fp8; rows quantised in the call): a quarter of the prepared
-        # weights' bytes and, for prompts, a fifth of the projections' time, at e4m3's precision. It moves the routing too, so it
-        # is the caller's choice. Not beside adapters
+        # weights' bytes and, for prompts, a fifth to a third of the projections' time, at e4m3's precision. It moves the
+        # routing too, so it is the caller's choice. Not beside adapters
         self.gemm_fp8 = False
         # prepared weights by form, storage, version and shape (_prepared)
         self._wprep: dict = {}

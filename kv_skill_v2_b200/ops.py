@@ -779,8 +779,9 @@ def read_mass(q: torch.Tensor, pages: Pages, idx: torch.Tensor, wk: torch.Tensor
 
     q [R, d_s] float32 / float16 / bfloat16; idx, wk [R, k] as route gives them; a page that several Libraries name gets
     the attention of all of them. out: where to write it (may be `mass` itself). float32 q takes part with 22 bits (with
-    bfloat16 slots 24 in calls of few pairs, else 16, which many pairs average out), a 16-bit q exactly; the same call gives the same bits. Slots at or past n_valid may hold anything.
-    Pairs with wk 0 or NaN (what route gives a query that is not finite) read nothing.
+    bfloat16 slots 24 in calls of few pairs, else 16, which many pairs average out), a 16-bit q exactly; the same call gives
+    the same bits. Slots at or past n_valid may hold anything. Pairs with wk 0 or NaN (what route gives a query that is not
+    finite) read nothing.
     Raises NotImplementedError for float32 slots, d_s not a multiple of 8 and pages of more than 2048 rows."""
     po, nv = pages.page_of, pages.n_valid
     if po.dtype is not torch.int32 or nv.dtype is not torch.int32 or po.dim() != 2 or nv.shape != po.shape \
